@@ -508,6 +508,126 @@ typedef struct tp_onehot_args {
 int tp_onehot_linear_forward(const tp_linear_args* a, const tp_onehot_args* oh, void* stream);
 int tp_onehot_linear_backward(const tp_linear_grad_args* ga, const tp_onehot_args* oh, void* stream);
 
+/* AdamW with both moments in 8 bits (tp_adamw_step keeps them in 32): 16.1 bytes of traffic per
+ * element and step instead of 28, 2.1 bytes of state instead of 8.  A member's elements are cut into
+ * blocks of 128 with one fp32 scale per moment.
+ *   exp_avg:    e4m3 codes times max |m| / 448
+ *   exp_avg_sq: the root of the second moment, codes 16 e + f of value 2^(e - 15) (1 + f / 16)
+ *               (0 for code 0), times max sqrt(v) / 1.9375
+ * Both are rounded up or down at random in proportion to the distance, with 16 bits each (the low
+ * half for exp_avg) of word (element & 3) of Philox4x32-10, key = seed, counter = (element >> 2, id,
+ * member_base + member, step): a member's states depend neither on the launch nor on the sharding.
+ * The parameters take the update from the unrounded moments.  A block whose largest magnitude is
+ * below 2^-100 is stored as zeros; one that holds an infinity or a NaN gets a NaN scale, so that
+ * all its 128 moments read as NaN.  Zero codes and scales are zero moments (a fresh or reset state). */
+typedef struct tp_opt8_tensor {
+  float* p;
+  const float* grad;
+  uint8_t* exp_avg;         /* as p */
+  float* exp_avg_scale;     /* (members, ceil(inner / 128)) */
+  uint8_t* exp_avg_sq;      /* as p */
+  float* exp_avg_sq_scale;  /* (members, ceil(inner / 128)) */
+  const int64_t* step;      /* per-member step counts (already incremented), or NULL */
+  int64_t numel;            /* a multiple of inner */
+  int64_t inner;            /* elements of one member, at most 2^33 */
+  uint32_t id;              /* the tensor's number in the random counter */
+} tp_opt8_tensor;
+
+typedef struct tp_adamw8_args {
+  int32_t n_tensors;
+  tp_opt8_tensor t[TP_MAX_OPT_TENSORS];
+  tp_hparam lr, beta1, beta2, eps, weight_decay;
+  int64_t step;             /* scalar step (already incremented) when t[i].step == NULL */
+  uint64_t seed;
+  uint32_t member_base;     /* global id of member 0 */
+} tp_adamw8_args;
+int tp_adamw8_step(const tp_adamw8_args* a, void* stream);
+
+/* The moments that a state of tp_adamw8_step stands for, exp_avg and exp_avg_sq (the root
+ * squared), in fp32 or bf16. */
+typedef struct tp_opt8_values {
+  const uint8_t* exp_avg;
+  const float* exp_avg_scale;
+  const uint8_t* exp_avg_sq;
+  const float* exp_avg_sq_scale;
+  void* m;
+  void* v;
+  int64_t numel;
+  int64_t inner;
+} tp_opt8_values;
+
+typedef struct tp_adamw8_moments_args {
+  int32_t n_tensors;
+  tp_opt8_values t[TP_MAX_OPT_TENSORS];
+  int32_t dtype;            /* TP_DTYPE_F32 or TP_DTYPE_BF16: type of m and v */
+} tp_adamw8_moments_args;
+int tp_adamw8_moments(const tp_adamw8_moments_args* a, void* stream);
+
+/* Layer norm of a pack.  Row r of member m is normalised over its first n_features[m] columns,
+ *   y = (x - mean) rstd w + b,  rstd = 1 / sqrt(var + eps)  (biased variance, fp32 statistics),
+ * and the columns beyond are zero in y and dx and not read.  The backward writes
+ *   dx = rstd (g - mean(g) - xhat mean(g xhat)), g = dy w;  dw = sum_r dy xhat;  db = sum_r dy
+ * with sums in fp32 in a fixed order.  x and dy are addressed by member and row strides (elements;
+ * a member stride of 0 is an input that all members share); the outputs are contiguous. */
+typedef struct tp_layer_norm_args {
+  int32_t P, B, W;
+  int32_t dtype;                 /* TP_DTYPE_F32 or TP_DTYPE_BF16: x, y, dy */
+  int64_t x_member_stride, x_row_stride;
+  const int32_t* n_features;     /* device (P,), or NULL (= W) */
+  const void* x;
+  const float* weight;           /* (P, W), or NULL (ones) */
+  const float* bias;             /* (P, W), or NULL (zeros); forward only */
+  float eps;
+  void* y;                       /* forward: (P, B, W) */
+  float* mean;                   /* (P, B): written by the forward, read by the backward */
+  float* rstd;                   /* (P, B) */
+  const void* dy;                /* backward */
+  int64_t dy_member_stride, dy_row_stride;
+  void* dx;                      /* (P, B, W), or NULL */
+  int32_t dx_dtype;              /* type of dx: dtype, or TP_DTYPE_F32 (per-member terms that the
+                                    caller adds up over the members) */
+  float* dweight;                /* (P, W), or NULL */
+  float* dbias;                  /* (P, W), or NULL */
+  void* workspace;               /* backward with dweight or dbias: tp_layer_norm_workspace_size */
+  size_t workspace_bytes;
+} tp_layer_norm_args;
+size_t tp_layer_norm_workspace_size(int32_t P, int32_t B, int32_t W);
+int tp_layer_norm_forward(const tp_layer_norm_args* a, void* stream);
+int tp_layer_norm_backward(const tp_layer_norm_args* a, void* stream);
+
+/* Log probabilities of given labels from raw scores, with entropies and the best classes:
+ *   log p_c = z_c - log sum exp z,  H = -sum_c p_c log p_c
+ * and the scores' gradient from the gradients g_l of the label's log probability and g_h of H,
+ *   dz_c = g_l ([c = label] - p_c) - g_h p_c (log p_c + H).
+ * A label equal to ignore_index gives 0 and takes no gradient from g_l; one outside [0, C) gives NaN
+ * (and a NaN gradient where g_l is given).  Classes may be masked with -inf; a row of nothing but
+ * -inf has log p = -inf, H = 0 and a zero gradient; a NaN or +inf makes its row NaN.  The best
+ * classes come in descending order, NaN first, equal scores by ascending index. */
+typedef struct tp_label_log_probs_args {
+  int64_t rows;
+  int32_t C;
+  int32_t dtype;                 /* TP_DTYPE_F32 or TP_DTYPE_BF16: logits and dlogits */
+  const void* logits;            /* rows of C scores */
+  int64_t logits_stride;         /* elements from row to row */
+  const int64_t* labels;         /* (label_rows,): row r has label r % label_rows */
+  int64_t label_rows;
+  int64_t ignore_index;
+  int32_t top_k;                 /* 0 .. min(C, TP_MAX_TOP_K) */
+  float* log_prob;               /* forward: (rows,) */
+  float* entropy;                /* forward: (rows,) */
+  float* top_log_prob;           /* forward, top_k > 0: (rows, top_k) */
+  int64_t* top_label;            /* forward, top_k > 0: (rows, top_k) */
+  float* stats;                  /* (rows, 3): written by the forward, read by the backward */
+  const float* g_log_prob;       /* backward: (rows,) or NULL */
+  const float* g_entropy;        /* backward: (rows,) or NULL */
+  int32_t g_log_prob_stride;     /* 1, or 0: one value for every row */
+  int32_t g_entropy_stride;
+  void* dlogits;                 /* backward: (rows, C) */
+} tp_label_log_probs_args;
+#define TP_MAX_TOP_K 32
+int tp_label_log_probs_forward(const tp_label_log_probs_args* a, void* stream);
+int tp_label_log_probs_backward(const tp_label_log_probs_args* a, void* stream);
+
 /* Clears and returns the device-side error flag (TP_OK or TP_ETIMEOUT). */
 int tp_device_error(void);
 

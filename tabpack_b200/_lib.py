@@ -18,6 +18,7 @@ TP_DTYPE_BF16 = 1
 TP_DTYPE_F64 = 2
 TP_MAX_OPT_TENSORS = 32
 TP_NOALLOC_SCRATCH_BYTES = 16 << 20
+TP_MAX_TOP_K = 32
 
 _c_int32_p = ctypes.POINTER(ctypes.c_int32)
 _c_float_p = ctypes.POINTER(ctypes.c_float)
@@ -144,6 +145,57 @@ class GreedyArgs(ctypes.Structure):
     ]
 
 
+class Opt8Tensor(ctypes.Structure):
+    _fields_ = [
+        ('p', ctypes.c_void_p), ('grad', ctypes.c_void_p), ('exp_avg', ctypes.c_void_p),
+        ('exp_avg_scale', ctypes.c_void_p), ('exp_avg_sq', ctypes.c_void_p), ('exp_avg_sq_scale', ctypes.c_void_p),
+        ('step', ctypes.c_void_p), ('numel', ctypes.c_int64), ('inner', ctypes.c_int64), ('id', ctypes.c_uint32),
+    ]
+
+
+class AdamW8Args(ctypes.Structure):
+    _fields_ = [
+        ('n_tensors', ctypes.c_int32), ('t', Opt8Tensor * TP_MAX_OPT_TENSORS),
+        ('lr', HParam), ('beta1', HParam), ('beta2', HParam), ('eps', HParam), ('weight_decay', HParam),
+        ('step', ctypes.c_int64), ('seed', ctypes.c_uint64), ('member_base', ctypes.c_uint32),
+    ]
+
+
+class Opt8Values(ctypes.Structure):
+    _fields_ = [
+        ('exp_avg', ctypes.c_void_p), ('exp_avg_scale', ctypes.c_void_p), ('exp_avg_sq', ctypes.c_void_p),
+        ('exp_avg_sq_scale', ctypes.c_void_p), ('m', ctypes.c_void_p), ('v', ctypes.c_void_p),
+        ('numel', ctypes.c_int64), ('inner', ctypes.c_int64),
+    ]
+
+
+class AdamW8MomentsArgs(ctypes.Structure):
+    _fields_ = [('n_tensors', ctypes.c_int32), ('t', Opt8Values * TP_MAX_OPT_TENSORS), ('dtype', ctypes.c_int32)]
+
+
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = [
+        ('P', ctypes.c_int32), ('B', ctypes.c_int32), ('W', ctypes.c_int32), ('dtype', ctypes.c_int32),
+        ('x_member_stride', ctypes.c_int64), ('x_row_stride', ctypes.c_int64), ('n_features', ctypes.c_void_p),
+        ('x', ctypes.c_void_p), ('weight', ctypes.c_void_p), ('bias', ctypes.c_void_p), ('eps', ctypes.c_float),
+        ('y', ctypes.c_void_p), ('mean', ctypes.c_void_p), ('rstd', ctypes.c_void_p), ('dy', ctypes.c_void_p),
+        ('dy_member_stride', ctypes.c_int64), ('dy_row_stride', ctypes.c_int64), ('dx', ctypes.c_void_p),
+        ('dx_dtype', ctypes.c_int32), ('dweight', ctypes.c_void_p), ('dbias', ctypes.c_void_p),
+        ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_size_t),
+    ]
+
+
+class LabelLogProbsArgs(ctypes.Structure):
+    _fields_ = [
+        ('rows', ctypes.c_int64), ('C', ctypes.c_int32), ('dtype', ctypes.c_int32), ('logits', ctypes.c_void_p),
+        ('logits_stride', ctypes.c_int64), ('labels', ctypes.c_void_p), ('label_rows', ctypes.c_int64),
+        ('ignore_index', ctypes.c_int64), ('top_k', ctypes.c_int32), ('log_prob', ctypes.c_void_p),
+        ('entropy', ctypes.c_void_p), ('top_log_prob', ctypes.c_void_p), ('top_label', ctypes.c_void_p),
+        ('stats', ctypes.c_void_p), ('g_log_prob', ctypes.c_void_p), ('g_entropy', ctypes.c_void_p),
+        ('g_log_prob_stride', ctypes.c_int32), ('g_entropy_stride', ctypes.c_int32), ('dlogits', ctypes.c_void_p),
+    ]
+
+
 # kernel families of tp_profile_stop, in TP_PROF_* order
 TP_PROF_KINDS = ('fwd', 'dgrad', 'wgrad', 'newton_schulz_gram', 'newton_schulz_update', 'gemm_f32', 'act_backward',
                  'muon_elementwise', 'adamw', 'weight_cast', 'input', 'embedding', 'onehot', 'metric', 'greedy',
@@ -192,6 +244,13 @@ SIGNATURES = {
     'tp_binary_roc_auc': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64,
                                          ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
                                          ctypes.c_void_p]),
+    'tp_adamw8_step': (ctypes.c_int, [ctypes.POINTER(AdamW8Args), ctypes.c_void_p]),
+    'tp_adamw8_moments': (ctypes.c_int, [ctypes.POINTER(AdamW8MomentsArgs), ctypes.c_void_p]),
+    'tp_layer_norm_workspace_size': (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
+    'tp_layer_norm_forward': (ctypes.c_int, [ctypes.POINTER(LayerNormArgs), ctypes.c_void_p]),
+    'tp_layer_norm_backward': (ctypes.c_int, [ctypes.POINTER(LayerNormArgs), ctypes.c_void_p]),
+    'tp_label_log_probs_forward': (ctypes.c_int, [ctypes.POINTER(LabelLogProbsArgs), ctypes.c_void_p]),
+    'tp_label_log_probs_backward': (ctypes.c_int, [ctypes.POINTER(LabelLogProbsArgs), ctypes.c_void_p]),
     'tp_device_error': (ctypes.c_int, []),
     'tp_last_error_string': (ctypes.c_char_p, []),
     'tp_version': (ctypes.c_char_p, []),

@@ -23,6 +23,9 @@
 #include "roc_auc.cuh"
 #include "embeddings.cuh"
 #include "onehot.cuh"
+#include "adamw8.cuh"
+#include "layer_norm.cuh"
+#include "log_probs.cuh"
 
 namespace tp {
 namespace {
@@ -1566,6 +1569,274 @@ int tp_adamw_step(const tp_adamw_args* a, void* stream) {
     adamw_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(ts, s, (int)m0);
     TP_CUDA_TRY(cudaGetLastError());
   }
+  return TP_OK;
+}
+
+// Tiles of a launch over several packs: tensor i's members have member_tiles[i] tiles of
+// `tile_blocks` state blocks each.
+static int adamw8_tiles(int n, const int64_t* numel, const int64_t* inner, int tile_blocks, uint32_t* tile0,
+                        uint32_t* member_tiles) {
+  int64_t total = 0;
+  for (int i = 0; i < n; ++i) {
+    if (numel[i] <= 0 || inner[i] <= 0 || inner[i] > (1ll << 33) || numel[i] % inner[i] != 0)
+      return fail(TP_EINVAL, "tensor %d: %lld elements do not make members of %lld", i, (long long)numel[i],
+                  (long long)inner[i]);
+    const int64_t nb = (inner[i] + ADAMW8_BLOCK - 1) / ADAMW8_BLOCK;
+    const int64_t mt = (nb + tile_blocks - 1) / tile_blocks;
+    const int64_t members = numel[i] / inner[i];
+    tile0[i] = (uint32_t)total;
+    member_tiles[i] = (uint32_t)mt;
+    if (members > 0x7FFFFFFFLL / mt || (total += members * mt) > 0x7FFFFFFFLL)
+      return fail(TP_EINVAL, "too many elements for one 8-bit AdamW launch");
+  }
+  tile0[n] = (uint32_t)total;
+  return TP_OK;
+}
+
+static bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+int tp_adamw8_step(const tp_adamw8_args* a, void* stream) {
+  TP_PROF(TP_PROF_ADAMW, static_cast<cudaStream_t>(stream));
+  if (!a || a->n_tensors <= 0 || a->n_tensors > TP_MAX_OPT_TENSORS) return fail(TP_EINVAL, "bad tensor count");
+  AdamW8Tensors ts{};
+  int64_t numel[TP_MAX_OPT_TENSORS], inner[TP_MAX_OPT_TENSORS];
+  ts.n = a->n_tensors;
+  bool any_scalar_step = false;
+  for (int i = 0; i < a->n_tensors; ++i) {
+    const tp_opt8_tensor& t = a->t[i];
+    if (!t.p || !t.grad || !t.exp_avg || !t.exp_avg_scale || !t.exp_avg_sq || !t.exp_avg_sq_scale)
+      return fail(TP_EINVAL, "tensor %d: null pointer", i);
+    if (!aligned4(t.p) || !aligned4(t.grad) || !aligned4(t.exp_avg_scale) || !aligned4(t.exp_avg_sq_scale))
+      return fail(TP_EALIGN, "tensor %d: fp32 data must be 4-byte aligned", i);
+    any_scalar_step |= t.step == nullptr;
+    numel[i] = t.numel;
+    inner[i] = t.inner;
+    ts.t[i] = t;
+  }
+  if (any_scalar_step && a->step <= 0) return fail(TP_EINVAL, "the step count must be positive");
+  int rc = adamw8_tiles(ts.n, numel, inner, ADAMW8_TILE, ts.tile0, ts.member_tiles);
+  if (rc) return rc;
+  AdamW8Scalars s{};
+  s.lr = a->lr.per_member;
+  s.beta1 = a->beta1.per_member;
+  s.beta2 = a->beta2.per_member;
+  s.eps = a->eps.per_member;
+  s.wd = a->weight_decay.per_member;
+  const double lr = a->lr.scalar, b1 = a->beta1.scalar, b2 = a->beta2.scalar;
+  s.lr_s = (float)lr;
+  s.beta1_s = (float)b1;
+  s.beta2_s = (float)b2;
+  s.eps_s = (float)a->eps.scalar;
+  s.wd_s = (float)a->weight_decay.scalar;
+  s.wd_mult_s = (float)(1.0 - lr * a->weight_decay.scalar);
+  s.one_m_b1_s = (float)(1.0 - b1);
+  s.one_m_b2_s = (float)(1.0 - b2);
+  s.step = a->step;
+  if (any_scalar_step) {
+    if (!s.beta1) {
+      const double bc1 = 1.0 - std::pow(b1, (double)a->step);
+      s.bc1_s = (float)bc1;
+      s.step_size_s = (float)(lr / bc1);
+    }
+    if (!s.beta2) s.inv_sqrt_bc2_s = (float)(1.0 / std::sqrt(1.0 - std::pow(b2, (double)a->step)));
+  }
+  philox_key_schedule((uint32_t)a->seed, (uint32_t)(a->seed >> 32), s.ks);
+  s.member_base = a->member_base;
+  adamw8_kernel<<<ts.tile0[ts.n], 32 * ADAMW8_WARPS, 0, static_cast<cudaStream_t>(stream)>>>(ts, s);
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+int tp_adamw8_moments(const tp_adamw8_moments_args* a, void* stream) {
+  TP_PROF(TP_PROF_ADAMW, static_cast<cudaStream_t>(stream));
+  if (!a || a->n_tensors <= 0 || a->n_tensors > TP_MAX_OPT_TENSORS) return fail(TP_EINVAL, "bad tensor count");
+  if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad moment dtype");
+  AdamW8Moments ts{};
+  int64_t numel[TP_MAX_OPT_TENSORS], inner[TP_MAX_OPT_TENSORS];
+  ts.n = a->n_tensors;
+  for (int i = 0; i < a->n_tensors; ++i) {
+    const tp_opt8_values& t = a->t[i];
+    if (!t.exp_avg || !t.exp_avg_scale || !t.exp_avg_sq || !t.exp_avg_sq_scale || !t.m || !t.v)
+      return fail(TP_EINVAL, "tensor %d: null pointer", i);
+    numel[i] = t.numel;
+    inner[i] = t.inner;
+    ts.t[i] = t;
+  }
+  int rc = adamw8_tiles(ts.n, numel, inner, ADAMW8_TILE, ts.tile0, ts.member_tiles);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->dtype == TP_DTYPE_BF16)
+    adamw8_moments_kernel<__nv_bfloat16><<<ts.tile0[ts.n], 32 * ADAMW8_WARPS, 0, st>>>(ts);
+  else
+    adamw8_moments_kernel<float><<<ts.tile0[ts.n], 32 * ADAMW8_WARPS, 0, st>>>(ts);
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+static int check_layer_norm(const tp_layer_norm_args* a) {
+  if (!a) return fail(TP_EINVAL, "null layer norm arguments");
+  if (a->P <= 0 || a->B <= 0 || a->W <= 0)
+    return fail(TP_EINVAL, "layer norm needs P, B, W > 0 (got %d, %d, %d)", a->P, a->B, a->W);
+  if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad layer norm dtype");
+  if (!a->x || !a->mean || !a->rstd) return fail(TP_EINVAL, "null layer norm input");
+  if ((int64_t)a->P * a->B > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many rows for one layer norm call");
+  return TP_OK;
+}
+
+static LayerNormArgs layer_norm_args(const tp_layer_norm_args* a) {
+  LayerNormArgs k{};
+  k.P = a->P;
+  k.B = a->B;
+  k.W = a->W;
+  k.xm = a->x_member_stride;
+  k.xr = a->x_row_stride;
+  k.dym = a->dy_member_stride;
+  k.dyr = a->dy_row_stride;
+  k.n = a->n_features;
+  k.x = a->x;
+  k.w = a->weight;
+  k.b = a->bias;
+  k.eps = a->eps;
+  k.y = a->y;
+  k.mean = a->mean;
+  k.rstd = a->rstd;
+  k.dy = a->dy;
+  k.dx = a->dx;
+  k.dx_f32 = a->dx_dtype == TP_DTYPE_F32;
+  k.dw = a->dweight;
+  k.db = a->dbias;
+  return k;
+}
+
+// Row splits of the parameter gradients: about two blocks per SM, at least 16 rows each.
+static int layer_norm_splits(int P, int B, int W) {
+  const long long base = (long long)P * ((W + 255) / 256);
+  const long long s = std::min<long long>((2 * 148 + base - 1) / base, (B + 15) / 16);
+  return (int)std::max<long long>(1, s);
+}
+
+size_t tp_layer_norm_workspace_size(int32_t P, int32_t B, int32_t W) {
+  if (P <= 0 || B <= 0 || W <= 0) return 0;
+  const int s = layer_norm_splits(P, B, W);
+  return s > 1 ? (size_t)2 * P * s * W * sizeof(float) : 0;
+}
+
+int tp_layer_norm_forward(const tp_layer_norm_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  TP_PROF(TP_PROF_OTHER, st);
+  int rc = check_layer_norm(a);
+  if (rc) return rc;
+  if (!a->y) return fail(TP_EINVAL, "null layer norm output");
+  const LayerNormArgs k = layer_norm_args(a);
+  if (a->dtype == TP_DTYPE_BF16)
+    layer_norm_forward_kernel<__nv_bfloat16><<<(unsigned)(k.P * k.B), 256, 0, st>>>(k);
+  else
+    layer_norm_forward_kernel<float><<<(unsigned)(k.P * k.B), 256, 0, st>>>(k);
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+int tp_layer_norm_backward(const tp_layer_norm_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  TP_PROF(TP_PROF_OTHER, st);
+  int rc = check_layer_norm(a);
+  if (rc) return rc;
+  if (!a->dy) return fail(TP_EINVAL, "null layer norm gradient");
+  if (a->dx && a->dx_dtype != a->dtype && a->dx_dtype != TP_DTYPE_F32) return fail(TP_EINVAL, "bad dx dtype");
+  LayerNormArgs k = layer_norm_args(a);
+  const bool bf16 = a->dtype == TP_DTYPE_BF16;
+  if (a->dx) {
+    if (bf16)
+      layer_norm_dx_kernel<__nv_bfloat16><<<(unsigned)(k.P * k.B), 256, 0, st>>>(k);
+    else
+      layer_norm_dx_kernel<float><<<(unsigned)(k.P * k.B), 256, 0, st>>>(k);
+  }
+  if (a->dweight || a->dbias) {
+    k.S = layer_norm_splits(k.P, k.B, k.W);
+    k.rows_per_split = (k.B + k.S - 1) / k.S;
+    const size_t need = tp_layer_norm_workspace_size(k.P, k.B, k.W);
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned4(a->workspace)))
+      return fail(TP_EINVAL, "layer norm workspace of %zu bytes is smaller than the %zu needed, or not aligned",
+                  a->workspace_bytes, need);
+    if (k.P > 65535) return fail(TP_EINVAL, "too many members for one layer norm call");
+    k.partial = static_cast<float*>(a->workspace);
+    const unsigned cols = (k.W + 255) / 256;
+    if (bf16)
+      layer_norm_dw_kernel<__nv_bfloat16><<<dim3(cols, k.P, k.S), 256, 0, st>>>(k);
+    else
+      layer_norm_dw_kernel<float><<<dim3(cols, k.P, k.S), 256, 0, st>>>(k);
+    if (k.S > 1) layer_norm_finish_kernel<<<dim3(cols, k.P), 256, 0, st>>>(k);
+  }
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+static int check_label_log_probs(const tp_label_log_probs_args* a) {
+  if (!a) return fail(TP_EINVAL, "null label log probability arguments");
+  if (a->rows <= 0 || a->rows > 0x7FFFFFFFLL || a->C <= 0)
+    return fail(TP_EINVAL, "label log probabilities need rows and classes > 0 (got %lld, %d)", (long long)a->rows, a->C);
+  if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad logits dtype");
+  if (!a->logits || !a->labels || !a->stats) return fail(TP_EINVAL, "null logits, labels or statistics");
+  if (a->label_rows <= 0 || a->rows % a->label_rows != 0)
+    return fail(TP_EINVAL, "%lld labels do not divide %lld rows", (long long)a->label_rows, (long long)a->rows);
+  if (a->logits_stride < a->C && a->rows > 1) return fail(TP_EINVAL, "rows of logits overlap");
+  return TP_OK;
+}
+
+static LogProbsArgs label_log_probs_args(const tp_label_log_probs_args* a) {
+  LogProbsArgs k{};
+  k.rows = a->rows;
+  k.C = a->C;
+  k.ld = a->logits_stride;
+  k.logits = a->logits;
+  k.labels = a->labels;
+  k.label_rows = a->label_rows;
+  k.ignore_index = a->ignore_index;
+  k.k = a->top_k;
+  k.log_prob = a->log_prob;
+  k.entropy = a->entropy;
+  k.top = a->top_log_prob;
+  k.which = a->top_label;
+  k.stats = a->stats;
+  k.g_l = a->g_log_prob;
+  k.g_h = a->g_entropy;
+  k.g_l_stride = a->g_log_prob_stride;
+  k.g_h_stride = a->g_entropy_stride;
+  k.dlogits = a->dlogits;
+  return k;
+}
+
+int tp_label_log_probs_forward(const tp_label_log_probs_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  TP_PROF(TP_PROF_OTHER, st);
+  int rc = check_label_log_probs(a);
+  if (rc) return rc;
+  if (!a->log_prob || !a->entropy) return fail(TP_EINVAL, "null log probability or entropy output");
+  if (a->top_k < 0 || a->top_k > TP_MAX_TOP_K || a->top_k > a->C)
+    return fail(TP_EINVAL, "top_k must be in 0 .. min(C, %d), got %d", TP_MAX_TOP_K, a->top_k);
+  if (a->top_k > 0 && (!a->top_log_prob || !a->top_label)) return fail(TP_EINVAL, "null best-class output");
+  const LogProbsArgs k = label_log_probs_args(a);
+  if (a->dtype == TP_DTYPE_BF16)
+    log_probs_forward_kernel<__nv_bfloat16><<<(unsigned)k.rows, 256, 0, st>>>(k);
+  else
+    log_probs_forward_kernel<float><<<(unsigned)k.rows, 256, 0, st>>>(k);
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+int tp_label_log_probs_backward(const tp_label_log_probs_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  TP_PROF(TP_PROF_OTHER, st);
+  int rc = check_label_log_probs(a);
+  if (rc) return rc;
+  if (!a->dlogits) return fail(TP_EINVAL, "null logits gradient");
+  if ((a->g_log_prob_stride | a->g_entropy_stride) & ~1) return fail(TP_EINVAL, "gradient strides must be 0 or 1");
+  const LogProbsArgs k = label_log_probs_args(a);
+  if (a->dtype == TP_DTYPE_BF16)
+    log_probs_backward_kernel<__nv_bfloat16><<<(unsigned)k.rows, 256, 0, st>>>(k);
+  else
+    log_probs_backward_kernel<float><<<(unsigned)k.rows, 256, 0, st>>>(k);
+  TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;
 }
 

@@ -28,7 +28,7 @@ import enum
 import itertools
 import math
 import weakref
-from typing import Any, Final
+from typing import Any, Final, NamedTuple
 
 import torch
 import torch.nn as nn
@@ -842,6 +842,145 @@ class DropoutPack(ModulePack):
                                 rows=x.shape[1], cols=x.shape[2])
         scale = (1.0 / (1.0 - p)).to(x.dtype)
         return x * mask.to(x.dtype) * scale.view(-1, 1, 1)
+
+
+class _LayerNormFn(torch.autograd.Function):
+    """`ops.layer_norm_forward` / `ops.layer_norm_backward`; statistics and parameters in fp32."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, n_features, eps):
+        y, mean, rstd = ops.layer_norm_forward(x, weight, bias, n_features=n_features, eps=eps)
+        ctx.save_for_backward(x, weight, mean, rstd, n_features)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd, n_features = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = ops.layer_norm_backward(dy, x, weight, mean, rstd, n_features=n_features, need_dx=need[0],
+                                             need_dw=need[1], need_db=need[2])
+        return dx, dw, db, None, None
+
+
+class LayerNormPack(ModulePack):
+    """Layer norm of a pack (no counterpart in the reference): each member normalises its rows over
+    its own first `n_features` columns, with its own scale and shift (`tp_layer_norm_forward`).
+
+    Input (pack_size, batch, max_n_features) bf16 or fp32, or a member's rows shared by all
+    (an expanded input, as `PackView` returns it); the output has the input's type, zeros beyond each
+    member's width, and the padding of the input is not read.
+    """
+
+    def __init__(self, n_features: int | list[int], *, max_n_features: int | None = None, eps: float = 1e-5,
+                 elementwise_affine: bool = True, bias: bool = True, pack_size: int, device=None) -> None:
+        if pack_size <= 0:
+            raise ValueError('The pack size must be positive')
+        if not math.isfinite(eps) or eps <= 0.0:
+            raise ValueError('The epsilon value must be finite and positive')
+        buf, max_n = _positive_int_pack(n_features, max_n_features, pack_size=pack_size)
+        super().__init__()
+        self.register_buffer('n_features', None if buf is None else _mark_buffer(buf.to(device)))
+        self._max_n_features = max_n
+        self.eps = float(eps)
+        shape = (pack_size, max_n)
+        self.weight = ParameterPack(torch.empty(shape, device=device)) if elementwise_affine else None
+        self.bias = ParameterPack(torch.empty(shape, device=device)) if elementwise_affine and bias else None
+        self.reset_parameters()
+
+    @property
+    def pack_size(self) -> int:
+        for t in (self.weight, self.n_features):
+            if t is not None:
+                return t.shape[PACK_DIM]
+        raise RuntimeError('Cannot infer the pack size')
+
+    @property
+    def max_n_features(self) -> int:
+        return self._max_n_features
+
+    def reset_parameters(self, *, pack_idx: Tensor | None = None) -> None:
+        if pack_idx is not None:
+            check_pack_idx(pack_idx, self.pack_size)
+        with torch.no_grad():
+            for p, value in ((self.weight, 1.0), (self.bias, 0.0)):
+                if p is not None:
+                    p[slice(None) if pack_idx is None else pack_idx] = value
+
+    def replace(self, *, pack_idx: Tensor, n_features: list[int] | None = None) -> None:
+        check_pack_idx(pack_idx, self.pack_size)
+        if n_features is not None:
+            if len(n_features) != len(pack_idx):
+                raise ValueError('Each provided hyperparameter list must contain one value for each selected pack member')
+            if self.n_features is None:
+                raise RuntimeError('Cannot replace feature counts that are shared by all pack members')
+            if not all(0 < v <= self.max_n_features for v in n_features):
+                raise ValueError('Feature counts must be positive and must not exceed the allocated maximum')
+            self.n_features[pack_idx] = torch.tensor(n_features, dtype=self.n_features.dtype,
+                                                     device=self.n_features.device)
+        self.reset_parameters(pack_idx=pack_idx)
+
+    def forward(self, x: Tensor, pack_idx: Tensor | None = None) -> Tensor:
+        if x.ndim != 3:
+            raise ValueError('The input must have three dimensions')
+        if x.shape[-1] != self.max_n_features:
+            raise ValueError('The number of input features must be equal to the maximum supported number of features')
+        if not x.is_cuda:
+            raise RuntimeError('tabpack_b200 packs run on CUDA devices only')
+        w, b, n = self.weight, self.bias, self.n_features
+        P = self.try_get_pack_size()
+        if pack_idx is not None:
+            check_pack_idx(pack_idx, P)
+            w, b, n = (_select(t, pack_idx) for t in (w, b, n))
+            n, P = _widths(n), len(pack_idx)
+        else:
+            n = _widths_cached(self, 'n', n)
+        if x.shape[PACK_DIM] not in (1, x.shape[PACK_DIM] if P is None else P):
+            raise ValueError('The pack dimension of the input must match the selected pack size')
+        if (w is not None or n is not None) and P > 1 and (x.shape[PACK_DIM] == 1 or x.stride(PACK_DIM) == 0):
+            x = x[0]  # rows that the members share: their gradient is added up in fp32
+        return _LayerNormFn.apply(x, w, b, n, self.eps)
+
+
+class LabelLogProbs(NamedTuple):
+    """What `label_log_probs` returns; the last two are None without `top_k` and take no gradient."""
+
+    log_prob: Tensor
+    entropy: Tensor
+    top_log_prob: Tensor | None
+    top_label: Tensor | None
+
+
+class _LabelLogProbsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, top_k, ignore_index):
+        ctx.set_materialize_grads(False)
+        log_prob, entropy, top, which, stats = ops.label_log_probs_forward(logits, labels, top_k=top_k,
+                                                                           ignore_index=ignore_index)
+        ctx.save_for_backward(logits, labels, stats)
+        ctx.ignore_index = ignore_index
+        ctx.mark_non_differentiable(*(t for t in (top, which) if t is not None))
+        return log_prob, entropy, top, which
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_log_prob, g_entropy, *_):
+        if g_log_prob is None and g_entropy is None:
+            return None, None, None, None
+        logits, labels, stats = ctx.saved_tensors
+        return ops.label_log_probs_backward(g_log_prob, g_entropy, logits, labels, stats,
+                                            ignore_index=ctx.ignore_index), None, None, None
+
+
+def label_log_probs(logits: Tensor, labels: Tensor, *, top_k: int = 0, ignore_index: int = -100) -> LabelLogProbs:
+    """Log probabilities of `labels` under softmax(logits), the entropies, and the `top_k` best
+    classes of each row, in fp32 from one pass over the raw outputs (`tp_label_log_probs_forward`).
+
+    logits (pack_size, batch, classes), or any leading dimensions, bf16 or fp32; labels int64
+    (pack_size, batch), or (batch,) shared by the members.  `log_prob` and `entropy` are
+    differentiable; rows whose label is `ignore_index` have log probability 0 and no gradient from
+    it.  Classes masked with -inf take no part."""
+    return LabelLogProbs(*_LabelLogProbsFn.apply(logits, labels, top_k, ignore_index))
 
 
 class MLPBackbonePack(ModulePack):

@@ -721,6 +721,340 @@ def binary_roc_auc(scores: Tensor, labels: Tensor, workspace: Tensor | None = No
     return out
 
 
+def _call(name: str, args, device: torch.device) -> None:
+    """`name(args)` on the current stream of `device`, whichever device is current."""
+    fn = getattr(load(), name)
+    if device.index == torch.cuda.current_device():
+        check(fn(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream), name)
+    else:
+        with torch.cuda.device(device):
+            check(fn(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream), name)
+
+
+def _same_device(device: torch.device, **tensors: Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f'{name} must be on {device}, got {t.device}')
+
+
+ADAMW8_BLOCK = 128
+"""Elements of a member that share one scale per moment in `adamw8_step`'s states."""
+
+
+def adamw8_state(p: Tensor) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """Zero moments of `adamw8_step` for a parameter pack (P, ...): (exp_avg, exp_avg_scale,
+    exp_avg_sq, exp_avg_sq_scale), uint8 codes of p's shape and fp32 (P, blocks) scales."""
+    P = p.shape[0]
+    nb = (p.numel() // max(P, 1) + ADAMW8_BLOCK - 1) // ADAMW8_BLOCK
+    codes = lambda: torch.zeros(p.shape, dtype=torch.uint8, device=p.device)  # noqa: E731
+    scales = lambda: torch.zeros((P, nb), dtype=torch.float32, device=p.device)  # noqa: E731
+    return codes(), scales(), codes(), scales()
+
+
+def _adamw8_check(shape, device, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale) -> int:
+    """Checks one tensor's state; returns the elements of one member."""
+    inner = 1
+    for n in shape[1:]:
+        inner *= n
+    nb = (inner + ADAMW8_BLOCK - 1) // ADAMW8_BLOCK
+    for name, t in (('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq)):
+        if t.dtype != torch.uint8 or t.shape != shape or t.device != device or not t.is_contiguous():
+            raise TypeError(f'{name} must be a contiguous uint8 {tuple(shape)} tensor on {device}')
+    for name, t in (('exp_avg_scale', exp_avg_scale), ('exp_avg_sq_scale', exp_avg_sq_scale)):
+        if t.dtype != torch.float32 or t.shape != (shape[0], nb) or t.device != device or not t.is_contiguous():
+            raise TypeError(f'{name} must be a contiguous fp32 ({shape[0]}, {nb}) tensor on {device}')
+    return inner
+
+
+def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, *, steps=None,
+                step: int = 0, lr, beta1, beta2, eps, weight_decay, seed: int, member_base: int = 0,
+                tensor_base: int = 0) -> None:
+    """Grouped AdamW over parameter packs (each (P, ...) fp32, contiguous) with both moments in
+    8 bits, in place; see `tp_adamw8_step` and `adamw8_state`.
+
+    `steps` (per-tensor (P,) int64 tensors, already incremented) or the scalar `step` give the
+    bias-correction step.  Hyperparameters are floats or (P,) fp32 CUDA tensors.  `seed`, the
+    step, the member (`member_base` + position) and the tensor's number (`tensor_base` + position)
+    give the random bits of the moments' rounding.  Tensors are chunked into launches of at most 32.
+    """
+    n = len(params)
+    if not all(len(t) == n for t in (grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales)) or (
+            steps is not None and len(steps) != n):
+        raise ValueError('one gradient, state and step per parameter is required')
+    if steps is None and int(step) <= 0:
+        raise ValueError('the step count must be positive')
+    device = params[0].device if n else None
+    hp = []
+    for name, v in (('lr', lr), ('beta1', beta1), ('beta2', beta2), ('eps', eps), ('weight_decay', weight_decay)):
+        if isinstance(v, Tensor):
+            _same_device(device, **{name: v})
+            v = v.contiguous()
+        hp.append(v)
+    sizes = {v.numel() for v in hp if isinstance(v, Tensor)}
+    for s in range(0, n, _lib.TP_MAX_OPT_TENSORS):
+        a = _lib.AdamW8Args()
+        used = 0
+        for i in range(s, min(n, s + _lib.TP_MAX_OPT_TENSORS)):
+            p, g = params[i], grads[i]
+            if p.dtype != torch.float32 or not p.is_cuda or not p.is_contiguous() or p.ndim == 0:
+                raise TypeError('param must be a contiguous fp32 CUDA tensor with a pack dimension')
+            if g.dtype != torch.float32 or g.shape != p.shape or not g.is_contiguous():
+                raise TypeError('grad must be a contiguous fp32 tensor of the shape of its parameter')
+            _same_device(device, param=p, grad=g)
+            inner = _adamw8_check(p.shape, device, exp_avgs[i], exp_avg_scales[i], exp_avg_sqs[i],
+                                  exp_avg_sq_scales[i])
+            P = p.shape[0]
+            if sizes and sizes != {P}:
+                raise ValueError('per-member hyperparameters must have one value per member')
+            st = None
+            if steps is not None:
+                st = steps[i]
+                if st.dtype != torch.int64 or st.shape != (P,) or st.device != device or not st.is_contiguous():
+                    raise TypeError(f'steps must be contiguous int64 ({P},) tensors on {device}')
+                st = st.data_ptr()
+            if P == 0 or inner == 0:
+                continue
+            a.t[used] = (p.data_ptr(), g.data_ptr(), exp_avgs[i].data_ptr(), exp_avg_scales[i].data_ptr(),
+                         exp_avg_sqs[i].data_ptr(), exp_avg_sq_scales[i].data_ptr(), st, P * inner, inner,
+                         (tensor_base + i) & 0xFFFFFFFF)
+            used += 1
+        if used == 0:
+            continue
+        a.n_tensors = used
+        a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = (_hparam(v) for v in hp)
+        a.step, a.seed = int(step), int(seed) & 0xFFFFFFFFFFFFFFFF
+        a.member_base = int(member_base) & 0xFFFFFFFF
+        _call('tp_adamw8_step', a, device)
+    # updated in place: bump the version counters as torch's in-place ops do
+    increment_version([*params, *exp_avgs, *exp_avg_scales, *exp_avg_sqs, *exp_avg_sq_scales])
+
+
+def adamw8_moments(exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, *,
+                   dtype: torch.dtype = torch.float32) -> tuple[list[Tensor], list[Tensor]]:
+    """The moments that `adamw8_step`'s states stand for: lists of exp_avg and exp_avg_sq, of the
+    codes' shapes in fp32 or bf16 (a code has at most five significant bits, its square ten: bf16
+    rounds the latter); see `tp_adamw8_moments`."""
+    n = len(exp_avgs)
+    if not all(len(t) == n for t in (exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales)):
+        raise ValueError('every state needs its codes and scales')
+    code = _dtype_code(dtype)
+    m, v = [], []
+    for s in range(0, n, _lib.TP_MAX_OPT_TENSORS):
+        a = _lib.AdamW8MomentsArgs()
+        used = 0
+        for i in range(s, min(n, s + _lib.TP_MAX_OPT_TENSORS)):
+            q = exp_avgs[i]
+            if not q.is_cuda or q.ndim == 0:
+                raise TypeError('exp_avg must be a CUDA tensor with a pack dimension')
+            inner = _adamw8_check(q.shape, exp_avgs[0].device, q, exp_avg_scales[i], exp_avg_sqs[i],
+                                  exp_avg_sq_scales[i])
+            mi, vi = (torch.empty(q.shape, dtype=dtype, device=q.device) for _ in range(2))
+            m.append(mi)
+            v.append(vi)
+            if q.numel() == 0:
+                continue
+            a.t[used] = (q.data_ptr(), exp_avg_scales[i].data_ptr(), exp_avg_sqs[i].data_ptr(),
+                         exp_avg_sq_scales[i].data_ptr(), mi.data_ptr(), vi.data_ptr(), q.numel(), inner)
+            used += 1
+        if used:
+            a.n_tensors, a.dtype = used, code
+            _call('tp_adamw8_moments', a, exp_avgs[0].device)
+    return m, v
+
+
+def _rows_strided(name: str, t: Tensor, P: int, B: int, W: int) -> tuple[Tensor, int, int]:
+    """A (P, B, W) view of t ((B, W): shared by the members) whose rows are contiguous, with its
+    member and row strides; copied only where the columns are not contiguous."""
+    if t.ndim == 2:
+        t = t.unsqueeze(0).expand(P, -1, -1)
+    if t.shape != (P, B, W):
+        raise ValueError(f'{name} must be ({P}, {B}, {W}) or ({B}, {W}), got {tuple(t.shape)}')
+    if W > 1 and t.stride(2) != 1:
+        t = t.contiguous()
+    return t, t.stride(0) if P > 1 else 0, t.stride(1) if B > 1 else 0
+
+
+def _norm_args(x: Tensor, weight: Tensor | None, bias: Tensor | None, n_features: Tensor | None,
+               P: int | None) -> tuple[_lib.LayerNormArgs, tuple]:
+    if x.ndim not in (2, 3):
+        raise ValueError('x must be (pack_size, batch, features) or a shared (batch, features)')
+    if not x.is_cuda:
+        raise RuntimeError('x must be a CUDA tensor (tabpack_b200 has no CPU path)')
+    ref = weight if weight is not None else bias if bias is not None else n_features
+    if P is None:
+        P = x.shape[0] if x.ndim == 3 else 1 if ref is None else ref.shape[0]
+    B, W = x.shape[-2:]
+    a = _lib.LayerNormArgs(P=P, B=B, W=W, dtype=_dtype_code(x.dtype), dx_dtype=_dtype_code(x.dtype))
+    x, a.x_member_stride, a.x_row_stride = _rows_strided('x', x, P, B, W)
+    _same_device(x.device, weight=weight, bias=bias, n_features=n_features)
+    if n_features is not None and n_features.shape != (P,):
+        raise ValueError(f'n_features must be ({P},), got {tuple(n_features.shape)}')
+    for name, t in (('weight', weight), ('bias', bias)):
+        if t is not None and t.shape != (P, W):
+            raise ValueError(f'{name} must be ({P}, {W}), got {tuple(t.shape)}')
+    weight, bias = _cuda('weight', weight, torch.float32), _cuda('bias', bias, torch.float32)
+    n_features = _i32('n_features', n_features)
+    a.n_features, a.x, a.weight, a.bias = _ptr(n_features), x.data_ptr(), _ptr(weight), _ptr(bias)
+    return a, (x, weight, bias, n_features)
+
+
+def layer_norm_forward(x: Tensor, weight: Tensor | None, bias: Tensor | None, *, n_features: Tensor | None = None,
+                       eps: float = 1e-5) -> tuple[Tensor, Tensor, Tensor]:
+    """Layer norm of x (P, B, W), or (B, W) shared by the members, bf16 or fp32, with each member's
+    own weight and bias (P, W) fp32 or None; see `tp_layer_norm_forward`.  `n_features` (P,): member
+    m's rows are normalised over their first n_features[m] columns, the others are zero in y.
+    Returns (y (P, B, W), mean (P, B), rstd (P, B)); the backward takes the last two."""
+    if not eps >= 0.0 or eps == float('inf'):
+        raise ValueError('eps must be finite and not negative')
+    a, keep = _norm_args(x, weight, bias, n_features, None)
+    P, B, W, dev = a.P, a.B, a.W, x.device
+    y = torch.empty((P, B, W), dtype=x.dtype, device=dev)
+    stats = torch.empty((2, P, B), dtype=torch.float32, device=dev)
+    mean, rstd = stats[0], stats[1]
+    if y.numel():
+        a.eps, a.y, a.mean, a.rstd = eps, y.data_ptr(), mean.data_ptr(), rstd.data_ptr()
+        _call('tp_layer_norm_forward', a, dev)
+    del keep
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy: Tensor, x: Tensor, weight: Tensor | None, mean: Tensor, rstd: Tensor, *,
+                        n_features: Tensor | None = None, need_dx: bool = True, need_dw: bool = True,
+                        need_db: bool = True) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
+    """Backward of `layer_norm_forward`: (dx of x's shape and type, dw (P, W), db (P, W) fp32); a
+    shared x takes the sum over the members.  See `tp_layer_norm_backward`."""
+    a, keep = _norm_args(x, weight, None, n_features, dy.shape[0])
+    P, B, W, dev = a.P, a.B, a.W, x.device
+    if dy.ndim != 3 or dy.dtype != x.dtype:
+        raise TypeError(f'dy must be a ({P}, {B}, {W}) {x.dtype} tensor')
+    _same_device(dev, dy=dy, mean=mean, rstd=rstd)
+    for name, t in (('mean', mean), ('rstd', rstd)):
+        if t.shape != (P, B) or t.dtype != torch.float32 or not t.is_contiguous():
+            raise TypeError(f'{name} must be the contiguous fp32 ({P}, {B}) tensor of the forward')
+    dy, a.dy_member_stride, a.dy_row_stride = _rows_strided('dy', dy, P, B, W)
+    shared = x.ndim == 2
+    dx = dw = db = ws = None
+    if need_dx:
+        # the members' terms of a shared input are added up before they are rounded
+        dx = torch.empty((P, B, W), dtype=torch.float32 if shared else x.dtype, device=dev)
+        if shared:
+            a.dx_dtype = TP_DTYPE_F32
+    if need_dw:
+        dw = torch.empty((P, W), dtype=torch.float32, device=dev)
+    if need_db:
+        db = torch.empty((P, W), dtype=torch.float32, device=dev)
+    if P and B and W and (need_dx or need_dw or need_db):
+        a.dy, a.mean, a.rstd = dy.data_ptr(), mean.data_ptr(), rstd.data_ptr()
+        a.dx, a.dweight, a.dbias = _ptr(dx), _ptr(dw), _ptr(db)
+        if need_dw or need_db:
+            need = load().tp_layer_norm_workspace_size(P, B, W)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            a.workspace, a.workspace_bytes = _ptr(ws), need
+        _call('tp_layer_norm_backward', a, dev)
+    else:
+        for t in (dw, db):
+            if t is not None:
+                t.zero_()
+    del keep, ws
+    if dx is not None and shared:
+        dx = dx.sum(0).to(x.dtype)
+    return dx, dw, db
+
+
+def _logit_rows(logits: Tensor) -> tuple[Tensor, int, int]:
+    """logits (..., C) as rows at one stride: (tensor, rows, stride), copied only where the rows
+    are not at one stride."""
+    C = logits.shape[-1]
+    rows = logits.numel() // C
+    stride, expect = C, None
+    ok = C == 1 or logits.stride(-1) == 1
+    for n, s in zip(reversed(logits.shape[:-1]), reversed(logits.stride()[:-1])):
+        if n == 1:
+            continue
+        if expect is None:
+            stride = expect = s
+        ok &= s == expect
+        expect *= n
+    if not ok or stride < C:
+        logits, stride = logits.contiguous(), C
+    return logits, rows, stride
+
+
+def _log_probs_args(logits: Tensor, labels: Tensor, ignore_index: int) -> tuple[_lib.LabelLogProbsArgs, tuple]:
+    if not logits.is_cuda:
+        raise RuntimeError('logits must be a CUDA tensor (tabpack_b200 has no CPU path)')
+    if logits.ndim == 0 or logits.shape[-1] == 0:
+        raise ValueError('logits must have at least one class')
+    if labels.dtype != torch.int64:
+        raise TypeError('labels must have the int64 data type')
+    lead = logits.shape[:-1]
+    if labels.ndim > len(lead) or labels.shape != lead[len(lead) - labels.ndim:]:
+        raise ValueError('The label and logit shapes are incompatible; only missing leading label dimensions '
+                         'may be broadcast')
+    _same_device(logits.device, labels=labels)
+    a = _lib.LabelLogProbsArgs(C=logits.shape[-1], dtype=_dtype_code(logits.dtype), ignore_index=ignore_index)
+    logits, a.rows, a.logits_stride = _logit_rows(logits)
+    labels = labels.contiguous()
+    a.logits, a.labels, a.label_rows = logits.data_ptr(), labels.data_ptr(), labels.numel()
+    return a, (logits, labels)
+
+
+def label_log_probs_forward(logits: Tensor, labels: Tensor, *, top_k: int = 0, ignore_index: int = -100
+                            ) -> tuple[Tensor, Tensor, Tensor | None, Tensor | None, Tensor]:
+    """Log probabilities of `labels` under softmax(logits), with entropies and the `top_k` best
+    classes; see `tp_label_log_probs_forward`.  logits (..., C) bf16 or fp32; labels int64 of
+    the leading shape, or without its first dimensions (labels that the members share).  Returns
+    (log_prob, entropy, top_log_prob or None, top_label or None, stats): fp32 of the leading
+    shape, (..., top_k) fp32 and int64, and the statistics that the backward takes."""
+    a, keep = _log_probs_args(logits, labels, ignore_index)
+    lead, dev = logits.shape[:-1], logits.device
+    if not 0 <= top_k <= min(a.C, _lib.TP_MAX_TOP_K):
+        raise ValueError(f'top_k must be between 0 and {min(a.C, _lib.TP_MAX_TOP_K)}, got {top_k}')
+    log_prob, entropy = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
+    stats = torch.empty((a.rows, 3), dtype=torch.float32, device=dev)
+    top = which = None
+    if top_k:
+        top = torch.empty((*lead, top_k), dtype=torch.float32, device=dev)
+        which = torch.empty((*lead, top_k), dtype=torch.int64, device=dev)
+    if a.rows:
+        a.top_k, a.log_prob, a.entropy, a.stats = top_k, log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr()
+        a.top_log_prob, a.top_label = _ptr(top), _ptr(which)
+        _call('tp_label_log_probs_forward', a, dev)
+    del keep
+    return log_prob, entropy, top, which, stats
+
+
+def _row_gradient(name: str, g: Tensor | None, lead, device) -> tuple[Tensor | None, int]:
+    """A per-row fp32 gradient and its stride: 0 for one value that was expanded over the rows."""
+    if g is None:
+        return None, 0
+    if g.shape != lead or g.dtype != torch.float32 or g.device != device:
+        raise TypeError(f'{name} must be a {tuple(lead)} fp32 tensor on {device}')
+    if all(s == 0 or n == 1 for n, s in zip(g.shape, g.stride())):
+        return g, 0
+    return g.contiguous(), 1
+
+
+def label_log_probs_backward(g_log_prob: Tensor | None, g_entropy: Tensor | None, logits: Tensor, labels: Tensor,
+                             stats: Tensor, *, ignore_index: int = -100) -> Tensor:
+    """The gradient of the logits (contiguous, of their shape and type) from the gradients of
+    `label_log_probs_forward`'s log_prob and entropy (either may be None);
+    see `tp_label_log_probs_backward`."""
+    a, keep = _log_probs_args(logits, labels, ignore_index)
+    lead, dev = logits.shape[:-1], logits.device
+    if stats.shape != (a.rows, 3) or stats.dtype != torch.float32 or stats.device != dev or not stats.is_contiguous():
+        raise TypeError('stats must be the tensor that the forward returned')
+    g_log_prob, a.g_log_prob_stride = _row_gradient('g_log_prob', g_log_prob, lead, dev)
+    g_entropy, a.g_entropy_stride = _row_gradient('g_entropy', g_entropy, lead, dev)
+    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    if a.rows:
+        a.stats, a.dlogits = stats.data_ptr(), dlogits.data_ptr()
+        a.g_log_prob, a.g_entropy = _ptr(g_log_prob), _ptr(g_entropy)
+        _call('tp_label_log_probs_backward', a, dev)
+    del keep
+    return dlogits
+
+
 def device_error() -> int:
     """Read and clear the device-side error flag (0 or TP_ETIMEOUT)."""
     return load().tp_device_error()

@@ -138,11 +138,16 @@ class OptimizerPack(torch.optim.Optimizer):
 
 
 def _adamw_group(opt: torch.optim.Optimizer, params, *, lr, beta1, beta2, eps, weight_decay,
-                 support_replacement: bool) -> None:
-    """Grouped AdamW launches over the group's parameter packs (`optim.py:347-427`).
+                 support_replacement: bool, first: int = 0) -> None:
+    """Grouped AdamW launches over the group's parameter packs (`optim.py:347-427`); `first` is the
+    number of the group's first parameter among the optimizer's.
 
     Parameters whose scalar step counters differ (a parameter that first received a
     gradient later) go to separate launches; per-member step tensors go to one."""
+    hp = dict(lr=_hp(lr), beta1=_hp(beta1), beta2=_hp(beta2), eps=_hp(eps), weight_decay=_hp(weight_decay))
+    if getattr(opt, 'state_bits', 32) == 8:
+        _adamw8_group(opt, params, hp, support_replacement=support_replacement, first=first)
+        return
     batches: dict = {}
     for p in params:
         if p.grad is None:
@@ -161,7 +166,6 @@ def _adamw_group(opt: torch.optim.Optimizer, params, *, lr, beta1, beta2, eps, w
         # its version like an in-place update
         batches.setdefault(key, []).append((p, p.grad.data.contiguous(), st['exp_avg'], st['exp_avg_sq'],
                                             st['step']))
-    hp = dict(lr=_hp(lr), beta1=_hp(beta1), beta2=_hp(beta2), eps=_hp(eps), weight_decay=_hp(weight_decay))
     for key, items in batches.items():
         ps, gs, ms, vs, steps = (list(t) for t in zip(*items))
         if key == 'tensor':
@@ -170,18 +174,115 @@ def _adamw_group(opt: torch.optim.Optimizer, params, *, lr, beta1, beta2, eps, w
             ops.adamw_step(ps, gs, ms, vs, step=key, **hp)
 
 
-class AdamWPack(OptimizerPack):
-    """`AdamWPack` (`optim.py:269-427`) on the grouped AdamW kernel."""
+def _adamw8_group(opt: torch.optim.Optimizer, params, hp: dict, *, support_replacement: bool, first: int) -> None:
+    """`_adamw_group` with both moments in 8 bits.  A parameter's number in the random counter is
+    its place among the optimizer's parameters, and the members count from `opt.member_base`."""
+    batches: dict = {}
+    for i, p in enumerate(params):
+        if p.grad is None:
+            continue
+        if p.grad.is_sparse:
+            raise RuntimeError('Sparse gradients are not supported')
+        st = opt.state[p]
+        if len(st) == 0:
+            st['step'] = (torch.zeros(p.shape[PACK_DIM], dtype=torch.int64, device=p.device)
+                          if support_replacement else 0)
+            st['exp_avg'], st['exp_avg_scale'], st['exp_avg_sq'], st['exp_avg_sq_scale'] = ops.adamw8_state(p.data)
+        st['step'] += 1
+        key = 'tensor' if isinstance(st['step'], Tensor) else int(st['step'])
+        # runs of consecutive parameters share a launch
+        runs = batches.setdefault(key, [])
+        if not runs or runs[-1][-1][0] != i - 1:
+            runs.append([])
+        runs[-1].append((i, p, p.grad.data.contiguous(), st))
+    keys = ('exp_avg', 'exp_avg_scale', 'exp_avg_sq', 'exp_avg_sq_scale')
+    for key, runs in batches.items():
+        for run in runs:
+            when = dict(steps=[st['step'] for *_, st in run]) if key == 'tensor' else dict(step=key)
+            ops.adamw8_step([p for _, p, _, _ in run], [g for _, _, g, _ in run],
+                            *([st[k] for *_, st in run] for k in keys), **when, **hp, seed=opt.state_seed,
+                            member_base=opt.member_base, tensor_base=first + run[0][0])
+
+
+def _check_state_bits(state_bits: int) -> int:
+    if state_bits not in (8, 32):
+        raise ValueError('The moments of AdamW are held in 8 or 32 bits')
+    return state_bits
+
+
+class _EightBitStates:
+    """What an optimizer pack with 8-bit AdamW moments adds: `state_bits`, the seed of their
+    rounding (drawn from torch's global generator unless given) and the global id of member 0
+    (a sharded trainer sets it: a member's states then do not depend on the sharding)."""
+
+    state_bits = 32
+    state_seed = 0
+    member_base = 0
+
+    def _init_states(self, state_bits: int, state_seed: int | None) -> None:
+        self.state_bits = state_bits
+        self.state_seed = (int(torch.randint(0, 2**62, (1,)).item()) if state_seed is None and state_bits == 8
+                           else int(state_seed or 0))
+        self.member_base = 0
+
+    def state_dict(self):
+        out = super().state_dict()
+        if self.state_bits == 8:
+            out['state_seed'] = self.state_seed
+        return out
+
+    def load_state_dict(self, state_dict) -> None:
+        """The base class casts the states of fp32 parameters to fp32: the codes go back to uint8
+        (their values are whole numbers below 256) and tensor step counts to int64.  States of the
+        other width are refused."""
+        packed = [st for st in state_dict['state'].values() if 'exp_avg' in st]
+        if any(('exp_avg_scale' in st) != (self.state_bits == 8) for st in packed):
+            raise ValueError(f'The loaded moments are not held in {self.state_bits} bits')
+        if self.state_bits != 8:
+            super().load_state_dict(state_dict)
+            return
+        state_dict = dict(state_dict)
+        seed = state_dict.pop('state_seed', None)
+        super().load_state_dict(state_dict)
+        if seed is not None:
+            self.state_seed = int(seed)
+        for st in self.state.values():
+            if 'exp_avg_scale' not in st:
+                continue
+            for k, dtype in (('exp_avg', torch.uint8), ('exp_avg_sq', torch.uint8), ('step', torch.int64)):
+                if isinstance(st[k], Tensor):
+                    st[k] = st[k].to(dtype)
+
+    def moments(self, p: ParameterPack) -> tuple[Tensor, Tensor]:
+        """The first and second moment of a parameter in fp32, whatever width they are held in."""
+        st = self.state[p]
+        if 'exp_avg' not in st:
+            raise ValueError('The parameter has no AdamW moments')
+        if 'exp_avg_scale' not in st:
+            return st['exp_avg'], st['exp_avg_sq']
+        m, v = ops.adamw8_moments([st['exp_avg']], [st['exp_avg_scale']], [st['exp_avg_sq']],
+                                  [st['exp_avg_sq_scale']])
+        return m[0], v[0]
+
+
+class AdamWPack(_EightBitStates, OptimizerPack):
+    """`AdamWPack` (`optim.py:269-427`) on the grouped AdamW kernel.
+
+    `state_bits=8` (no counterpart in the reference) holds both moments in 8 bits with one scale
+    per 128 elements (`ops.adamw8_step`): state keys `exp_avg`, `exp_avg_sq` (uint8 codes) and
+    `exp_avg_scale`, `exp_avg_sq_scale`; `moments(p)` reads them back."""
 
     def __init__(self, params, *, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay, pack_size: int,
-                 support_replacement: bool = False):
+                 support_replacement: bool = False, state_bits: int = 32, state_seed: int | None = None):
         if pack_size <= 0:
             raise ValueError('The pack size must be positive')
+        _check_state_bits(state_bits)
         super().__init__(params, _defaults([
             ('lr', lr, _check_lr), ('beta1', beta1, _check_momentum), ('beta2', beta2, _check_momentum),
             ('eps', eps, _check_eps), ('weight_decay', weight_decay, _check_weight_decay)], pack_size=pack_size),
             pack_size=pack_size)
         self._support_replacement: Final = support_replacement
+        self._init_states(state_bits, state_seed)
 
     def replace(self, *, pack_idx: Tensor, lr=None, beta1=None, beta2=None, eps=None, weight_decay=None) -> None:
         if not self._support_replacement:
@@ -217,9 +318,11 @@ def _widths(module: LinearPack):
     return outf, inf
 
 
-class MuonAdamWPack(OptimizerPack):
+class MuonAdamWPack(_EightBitStates, OptimizerPack):
     """`MuonAdamWPack` (`optim.py:495-861`): Muon for backbone block weights (one
-    parameter per group, built with `make_muon_parameter_group`), AdamW for the rest."""
+    parameter per group, built with `make_muon_parameter_group`), AdamW for the rest.
+    `adamw_state_bits=8` holds the latter's moments in 8 bits as `AdamWPack(state_bits=8)` does;
+    Muon's momentum stays in 32."""
 
     @staticmethod
     def make_muon_parameter_group(module: LinearPack) -> dict[str, Any]:
@@ -231,9 +334,11 @@ class MuonAdamWPack(OptimizerPack):
     def __init__(self, params, *, adamw_lr, adamw_beta1=0.9, adamw_beta2=0.999, adamw_eps=1e-8, weight_decay,
                  muon_lr, muon_momentum=0.95, muon_newton_schulz_steps: int = 5, muon_nesterov: bool = True,
                  muon_skip_zero_updates: bool = False, pack_size: int, support_replacement: bool = False,
-                 allow_inplace_grad_mutation: bool, compile_muon_newton_schulz: bool = False):
+                 allow_inplace_grad_mutation: bool, compile_muon_newton_schulz: bool = False,
+                 adamw_state_bits: int = 32, state_seed: int | None = None):
         if pack_size <= 0:
             raise ValueError('The pack size must be positive')
+        _check_state_bits(adamw_state_bits)
         del compile_muon_newton_schulz  # the Newton-Schulz iterations always run on the tcgen05 kernels
         super().__init__(params, {
             'muon': False, 'muon_newton_schulz_steps': muon_newton_schulz_steps, 'muon_nesterov': muon_nesterov,
@@ -246,6 +351,7 @@ class MuonAdamWPack(OptimizerPack):
         self._support_replacement: Final = support_replacement
         self._allow_inplace_grad_mutation: Final = allow_inplace_grad_mutation
         self._workspaces: dict = {}
+        self._init_states(adamw_state_bits, state_seed)
 
     def add_param_group(self, param_group):
         out = super().add_param_group(param_group)
@@ -379,9 +485,11 @@ def _muon_groups(opt: torch.optim.Optimizer, groups: list, *, workspaces: dict,
 def adamw_step(opt: torch.optim.Optimizer, *, support_replacement: bool) -> None:
     """`AdamWPack.step` (`optim.py:347-427`) over every group of `opt` (keys `lr`, `beta1`,
     `beta2`, `eps`, `weight_decay`), one grouped AdamW launch per group."""
+    first = 0
     for g in opt.param_groups:
         _adamw_group(opt, g['params'], lr=g['lr'], beta1=g['beta1'], beta2=g['beta2'], eps=g['eps'],
-                     weight_decay=g['weight_decay'], support_replacement=support_replacement)
+                     weight_decay=g['weight_decay'], support_replacement=support_replacement, first=first)
+        first += len(g['params'])
 
 
 def muon_adamw_step(opt: torch.optim.Optimizer, *, workspaces: dict, allow_inplace_grad_mutation: bool,
@@ -401,10 +509,13 @@ def muon_adamw_step(opt: torch.optim.Optimizer, *, workspaces: dict, allow_inpla
         else:
             for g in groups:
                 _muon_group(opt, g, workspaces=workspaces, allow_inplace_grad_mutation=allow_inplace_grad_mutation)
+    first = 0
     for g in opt.param_groups:
         if not g['muon']:
             _adamw_group(opt, g['params'], lr=g['adamw_lr'], beta1=g['adamw_beta1'], beta2=g['adamw_beta2'],
-                         eps=g['adamw_eps'], weight_decay=g['weight_decay'], support_replacement=support_replacement)
+                         eps=g['adamw_eps'], weight_decay=g['weight_decay'], support_replacement=support_replacement,
+                         first=first)
+        first += len(g['params'])
 
 
 def optimizer_pack_remove(optimizer, *, pack_idx: Tensor, old_to_new_parameters) -> None:

@@ -37,7 +37,7 @@ from torch import Tensor
 from tabpack_b200 import ops
 from tabpack_b200.ensemble import compute_unsanitized_ensemble_predictions, greedy_ensemble
 from tabpack_b200.metrics import PackScore
-from tabpack_b200.nn import CosineEmbeddingsPack, LinearPack, TabPack
+from tabpack_b200.nn import CosineEmbeddingsPack, LinearPack, TabPack, label_log_probs
 from tabpack_b200.optim import AdamWPack, MuonAdamWPack, split_weight_decay
 from tabpack_b200.shard import allreduce_sum_, assign_replacements, gather_members, member_ranges
 
@@ -118,8 +118,15 @@ def _merge(base: dict, update: dict) -> dict:
     return out
 
 
-def member_loss(loss: str, y_pred: Tensor, y: Tensor) -> Tensor:
-    """Per-member training loss (P,) from raw outputs (P, B, d_out) and labels (P, B)."""
+def member_loss(loss: str, y_pred: Tensor, y: Tensor, *, entropy_weight: float = 0.0) -> Tensor:
+    """Per-member training loss (P,) from raw outputs (P, B, d_out) and labels (P, B).  With
+    `entropy_weight` w (loss 'ce' only) each row's loss is -log p(label) - w H, H the entropy of the
+    predicted classes: w > 0 penalises confident predictions (`label_log_probs`)."""
+    if entropy_weight:
+        if loss != 'ce':
+            raise ValueError("an entropy weight needs the loss 'ce'")
+        out = label_log_probs(y_pred, y)
+        return -(out.log_prob + entropy_weight * out.entropy).mean(1)
     if loss == 'mse':
         return ((y_pred[..., 0] - y) ** 2).mean(1)
     if loss == 'bce':
@@ -238,8 +245,8 @@ class PackTrainer:
                  per_member_optimizer: list[dict] | None = None, loss: str, seed: int, device,
                  autocast_bf16: bool = True, group=None, cost: list[float] | None = None,
                  member_range: tuple[int, int] | None = None, init_on_host: bool = False,
-                 n_models: int | None = None) -> None:
-        """`member_range` pins this trainer to global members [lo, hi) without a process
+                 n_models: int | None = None, entropy_weight: float = 0.0) -> None:
+        """`entropy_weight`: see `member_loss`.  `member_range` pins this trainer to global members [lo, hi) without a process
         group (several shards on one device); otherwise the group's rank picks its range.
         `init_on_host` draws the initial parameters with host generators (the same values on
         every machine and device; slower for large packs).
@@ -250,6 +257,9 @@ class PackTrainer:
         models to the next ids.  The pack's maximum shapes (`model`) must fit every model."""
         if loss not in _LOSSES:
             raise ValueError(f'loss must be one of {_LOSSES}')
+        if not math.isfinite(entropy_weight) or (entropy_weight and loss != 'ce'):
+            raise ValueError("entropy_weight must be finite and needs the loss 'ce'")
+        self.entropy_weight = float(entropy_weight)
         self.n_models = n_members if n_models is None else int(n_models)
         if self.n_models < n_members:
             raise ValueError('n_models must be at least the number of pack slots')
@@ -301,6 +311,8 @@ class PackTrainer:
                                 generator_device=self._init_device)
         okw = dict(optimizer)
         otype = okw.pop('type')
+        # the rounding of 8-bit AdamW moments is keyed by the run's seed and the global member
+        okw.setdefault('state_seed', _mix(self.seed, 0x8B))
         if per_member_optimizer is not None:
             okw.update(_transpose(per_member_optimizer[lo:hi]))
         if otype == 'muon':
@@ -325,6 +337,7 @@ class PackTrainer:
                                  support_replacement=replacement, **okw)
         else:
             raise ValueError("optimizer type must be 'muon' or 'adamw'")
+        self.opt.member_base = lo
 
     @staticmethod
     def _check_ranges(ranges: list[tuple[int, int]]) -> None:
@@ -355,7 +368,8 @@ class PackTrainer:
             with torch.autocast('cuda', dtype=torch.bfloat16, enabled=self.autocast):
                 # the batch gather runs inside the first-layer input build where it can
                 out = self.model.forward_rows(data.get('x_num'), data.get('x_cat'), idx)
-            losses = member_loss(self.loss, out.float(), y)
+            losses = (member_loss(self.loss, out, y, entropy_weight=self.entropy_weight) if self.entropy_weight
+                      else member_loss(self.loss, out.float(), y))
             losses.sum().backward()
             self.opt.step()
             self.opt.zero_grad()
