@@ -617,7 +617,8 @@ typedef struct tp_label_log_probs_args {
   float* entropy;                /* forward: (rows,) */
   float* top_log_prob;           /* forward, top_k > 0: (rows, top_k) */
   int64_t* top_label;            /* forward, top_k > 0: (rows, top_k) */
-  float* stats;                  /* (rows, 3): written by the forward, read by the backward */
+  float* stats;                  /* C > TP_LABEL_STATS_CLASSES: (rows, 3), written by the forward and
+                                    read by the backward (shorter rows are reduced anew); else NULL */
   const float* g_log_prob;       /* backward: (rows,) or NULL */
   const float* g_entropy;        /* backward: (rows,) or NULL */
   int32_t g_log_prob_stride;     /* 1, or 0: one value for every row */
@@ -625,6 +626,7 @@ typedef struct tp_label_log_probs_args {
   void* dlogits;                 /* backward: (rows, C) */
 } tp_label_log_probs_args;
 #define TP_MAX_TOP_K 32
+#define TP_LABEL_STATS_CLASSES 256
 int tp_label_log_probs_forward(const tp_label_log_probs_args* a, void* stream);
 int tp_label_log_probs_backward(const tp_label_log_probs_args* a, void* stream);
 

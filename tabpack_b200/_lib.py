@@ -19,6 +19,7 @@ TP_DTYPE_F64 = 2
 TP_MAX_OPT_TENSORS = 32
 TP_NOALLOC_SCRATCH_BYTES = 16 << 20
 TP_MAX_TOP_K = 32
+TP_LABEL_STATS_CLASSES = 256
 
 _c_int32_p = ctypes.POINTER(ctypes.c_int32)
 _c_float_p = ctypes.POINTER(ctypes.c_float)

@@ -1773,10 +1773,14 @@ int tp_layer_norm_backward(const tp_layer_norm_args* a, void* stream) {
 
 static int check_label_log_probs(const tp_label_log_probs_args* a) {
   if (!a) return fail(TP_EINVAL, "null label log probability arguments");
-  if (a->rows <= 0 || a->rows > 0x7FFFFFFFLL || a->C <= 0)
-    return fail(TP_EINVAL, "label log probabilities need rows and classes > 0 (got %lld, %d)", (long long)a->rows, a->C);
+  if (a->rows <= 0 || a->rows > 0x7FFFFFFFLL || a->C <= 0 || a->C > (1 << 30))
+    return fail(TP_EINVAL, "label log probabilities need rows and classes > 0, classes <= 2^30 (got %lld, %d)",
+                (long long)a->rows, a->C);
   if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad logits dtype");
-  if (!a->logits || !a->labels || !a->stats) return fail(TP_EINVAL, "null logits, labels or statistics");
+  if (!a->logits || !a->labels || (a->C > LP_REREAD && !a->stats))
+    return fail(TP_EINVAL, "null logits, labels or statistics");
+  if (reinterpret_cast<uintptr_t>(a->logits) % (a->dtype == TP_DTYPE_BF16 ? 2 : 4) != 0)
+    return fail(TP_EALIGN, "the logits are not aligned to their type");
   if (a->label_rows <= 0 || a->rows % a->label_rows != 0)
     return fail(TP_EINVAL, "%lld labels do not divide %lld rows", (long long)a->label_rows, (long long)a->rows);
   if (a->logits_stride < a->C && a->rows > 1) return fail(TP_EINVAL, "rows of logits overlap");
@@ -1806,6 +1810,59 @@ static LogProbsArgs label_log_probs_args(const tp_label_log_probs_args* a) {
   return k;
 }
 
+}  // extern "C"
+
+namespace tp {
+namespace {
+
+// A row's classes and, where its first element is not on a 16-byte boundary, the elements before it.
+int held_size(const tp_label_log_probs_args* a, int size) {
+  const int V = 16 / size;
+  const bool aligned = aligned16(a->logits) && (a->rows == 1 || a->logits_stride % V == 0);
+  return a->C > 1024 ? a->C : aligned ? a->C : a->C + V - 1;
+}
+
+template <typename T, bool TOP>
+void launch_log_probs(const LogProbsArgs& k, int held, cudaStream_t st) {
+  const auto blocks = [&](int lanes) { return (unsigned)((k.rows * lanes + 255) / 256); };
+  if (held <= 16) {
+    log_probs_held_forward_kernel<T, 1, 16, TOP><<<blocks(1), 256, 0, st>>>(k);
+  } else if (held <= 64) {
+    log_probs_held_forward_kernel<T, 8, 8, TOP><<<blocks(8), 256, 0, st>>>(k);
+  } else if (held <= 256) {
+    log_probs_held_forward_kernel<T, 32, 8, TOP><<<blocks(32), 256, 0, st>>>(k);
+  } else if (held <= 1024) {
+    log_probs_held_forward_kernel<T, 32, 32, TOP><<<blocks(32), 256, 0, st>>>(k);
+  } else {
+    // a thread per 64 scores, at least 4 warps; a few rows take all the threads a block has
+    const int want = k.rows < 296 ? 1024 : std::min(512, std::max(128, (k.C / 64 + 31) / 32 * 32));
+    log_probs_long_forward_kernel<T, TOP><<<(unsigned)k.rows, want, 0, st>>>(k);
+  }
+}
+
+template <typename T>
+void launch_log_probs_backward(const LogProbsArgs& k, int held, cudaStream_t st) {
+  const auto blocks = [&](int lanes) { return (unsigned)((k.rows * lanes + 255) / 256); };
+  if (k.C > LP_REREAD) {
+    constexpr int V = 16 / sizeof(T);
+    const int chunks = (k.C + V - 1 + LP_CHUNK - 1) / LP_CHUNK;
+    log_probs_stream_backward_kernel<T><<<(unsigned)((k.rows * chunks + 7) / 8), 256, 0, st>>>(k, chunks);
+  } else if (held <= 16) {
+    log_probs_held_backward_kernel<T, 1, 16><<<blocks(1), 256, 0, st>>>(k);
+  } else if (held <= 64) {
+    log_probs_held_backward_kernel<T, 8, 8><<<blocks(8), 256, 0, st>>>(k);
+  } else if (held <= 256) {
+    log_probs_held_backward_kernel<T, 32, 8><<<blocks(32), 256, 0, st>>>(k);
+  } else {
+    log_probs_held_backward_kernel<T, 32, 16><<<blocks(32), 256, 0, st>>>(k);
+  }
+}
+
+}  // namespace
+}  // namespace tp
+
+extern "C" {
+
 int tp_label_log_probs_forward(const tp_label_log_probs_args* a, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   TP_PROF(TP_PROF_OTHER, st);
@@ -1816,10 +1873,16 @@ int tp_label_log_probs_forward(const tp_label_log_probs_args* a, void* stream) {
     return fail(TP_EINVAL, "top_k must be in 0 .. min(C, %d), got %d", TP_MAX_TOP_K, a->top_k);
   if (a->top_k > 0 && (!a->top_log_prob || !a->top_label)) return fail(TP_EINVAL, "null best-class output");
   const LogProbsArgs k = label_log_probs_args(a);
-  if (a->dtype == TP_DTYPE_BF16)
-    log_probs_forward_kernel<__nv_bfloat16><<<(unsigned)k.rows, 256, 0, st>>>(k);
+  const bool bf16 = a->dtype == TP_DTYPE_BF16;
+  const int held = held_size(a, bf16 ? 2 : 4);
+  if (bf16 && a->top_k)
+    launch_log_probs<__nv_bfloat16, true>(k, held, st);
+  else if (bf16)
+    launch_log_probs<__nv_bfloat16, false>(k, held, st);
+  else if (a->top_k)
+    launch_log_probs<float, true>(k, held, st);
   else
-    log_probs_forward_kernel<float><<<(unsigned)k.rows, 256, 0, st>>>(k);
+    launch_log_probs<float, false>(k, held, st);
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;
 }
@@ -1832,10 +1895,14 @@ int tp_label_log_probs_backward(const tp_label_log_probs_args* a, void* stream) 
   if (!a->dlogits) return fail(TP_EINVAL, "null logits gradient");
   if ((a->g_log_prob_stride | a->g_entropy_stride) & ~1) return fail(TP_EINVAL, "gradient strides must be 0 or 1");
   const LogProbsArgs k = label_log_probs_args(a);
-  if (a->dtype == TP_DTYPE_BF16)
-    log_probs_backward_kernel<__nv_bfloat16><<<(unsigned)k.rows, 256, 0, st>>>(k);
+  const bool bf16 = a->dtype == TP_DTYPE_BF16;
+  if (reinterpret_cast<uintptr_t>(a->dlogits) % (bf16 ? 2 : 4) != 0)
+    return fail(TP_EALIGN, "the logits gradient is not aligned to its type");
+  const int held = held_size(a, bf16 ? 2 : 4);
+  if (bf16)
+    launch_log_probs_backward<__nv_bfloat16>(k, held, st);
   else
-    log_probs_backward_kernel<float><<<(unsigned)k.rows, 256, 0, st>>>(k);
+    launch_log_probs_backward<float>(k, held, st);
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;
 }

@@ -1005,19 +1005,19 @@ def label_log_probs_forward(logits: Tensor, labels: Tensor, *, top_k: int = 0, i
     classes; see `tp_label_log_probs_forward`.  logits (..., C) bf16 or fp32; labels int64 of
     the leading shape, or without its first dimensions (labels that the members share).  Returns
     (log_prob, entropy, top_log_prob or None, top_label or None, stats): fp32 of the leading
-    shape, (..., top_k) fp32 and int64, and the statistics that the backward takes."""
+    shape, (..., top_k) fp32 and int64, and what the backward takes."""
     a, keep = _log_probs_args(logits, labels, ignore_index)
     lead, dev = logits.shape[:-1], logits.device
     if not 0 <= top_k <= min(a.C, _lib.TP_MAX_TOP_K):
         raise ValueError(f'top_k must be between 0 and {min(a.C, _lib.TP_MAX_TOP_K)}, got {top_k}')
     log_prob, entropy = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
-    stats = torch.empty((a.rows, 3), dtype=torch.float32, device=dev)
+    stats = torch.empty((a.rows, 3) if a.C > _lib.TP_LABEL_STATS_CLASSES else 0, dtype=torch.float32, device=dev)
     top = which = None
     if top_k:
         top = torch.empty((*lead, top_k), dtype=torch.float32, device=dev)
         which = torch.empty((*lead, top_k), dtype=torch.int64, device=dev)
     if a.rows:
-        a.top_k, a.log_prob, a.entropy, a.stats = top_k, log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr()
+        a.top_k, a.log_prob, a.entropy, a.stats = top_k, log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr() or None
         a.top_log_prob, a.top_label = _ptr(top), _ptr(which)
         _call('tp_label_log_probs_forward', a, dev)
     del keep
@@ -1042,13 +1042,14 @@ def label_log_probs_backward(g_log_prob: Tensor | None, g_entropy: Tensor | None
     see `tp_label_log_probs_backward`."""
     a, keep = _log_probs_args(logits, labels, ignore_index)
     lead, dev = logits.shape[:-1], logits.device
-    if stats.shape != (a.rows, 3) or stats.dtype != torch.float32 or stats.device != dev or not stats.is_contiguous():
+    want = (a.rows, 3) if a.C > _lib.TP_LABEL_STATS_CLASSES else (0,)
+    if stats.shape != want or stats.dtype != torch.float32 or stats.device != dev or not stats.is_contiguous():
         raise TypeError('stats must be the tensor that the forward returned')
     g_log_prob, a.g_log_prob_stride = _row_gradient('g_log_prob', g_log_prob, lead, dev)
     g_entropy, a.g_entropy_stride = _row_gradient('g_entropy', g_entropy, lead, dev)
     dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
     if a.rows:
-        a.stats, a.dlogits = stats.data_ptr(), dlogits.data_ptr()
+        a.stats, a.dlogits = stats.data_ptr() or None, dlogits.data_ptr()
         a.g_log_prob, a.g_entropy = _ptr(g_log_prob), _ptr(g_entropy)
         _call('tp_label_log_probs_backward', a, dev)
     del keep
