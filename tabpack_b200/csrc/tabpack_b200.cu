@@ -1708,16 +1708,94 @@ static LayerNormArgs layer_norm_args(const tp_layer_norm_args* a) {
   return k;
 }
 
-// Row splits of the parameter gradients: about two blocks per SM, at least 16 rows each.
-static int layer_norm_splits(int P, int B, int W) {
-  const long long base = (long long)P * ((W + 255) / 256);
-  const long long s = std::min<long long>((2 * 148 + base - 1) / base, (B + 15) / 16);
-  return (int)std::max<long long>(1, s);
+}  // extern "C"
+
+namespace tp {
+namespace {
+
+// Lanes of a row's group: 16 elements each.
+int norm_lanes(int W) {
+  for (int g : {8, 32, 64, 128, 256})
+    if (W <= g * NORM_E) return g;
+  return 512;
 }
+
+// Splits of a member's rows over blocks.  `slots` blocks run at once; a block takes at least
+// two rows per group where there are so many.  Among one to four waves' worth of blocks the
+// count whose last wave is fullest.
+int norm_splits(int P, int B, int W, int slots) {
+  const int threads = norm_lanes(W) > 256 ? 512 : 256;
+  const int groups = W > NORM_HELD ? 1 : threads / norm_lanes(W);
+  const int most = std::max(1, (B + 2 * groups - 1) / (2 * groups));
+  int best = 1;
+  double fill = 0.0;
+  for (int k = 1; k <= 4; ++k) {
+    const int s = std::min<long long>(most, std::max<long long>(1, (long long)slots * k / P));
+    const long long blocks = (long long)P * s;
+    const double f = (double)blocks / (double)((blocks + slots - 1) / slots * slots);
+    if (f > fill * 1.02) {
+      fill = f;
+      best = s;
+    }
+  }
+  return best;
+}
+
+// Blocks of the backward that run at once: 128 registers a thread.
+int norm_backward_splits(int P, int B, int W) { return norm_splits(P, B, W, norm_lanes(W) > 256 ? 148 : 296); }
+
+template <typename T, int V, int G>
+void launch_norm(LayerNormArgs k, bool backward, cudaStream_t st) {
+  const unsigned blocks = (unsigned)k.P * k.S;
+  if (backward)
+    layer_norm_held_backward_kernel<T, V, G><<<blocks, NormGroup<G>::THREADS, 0, st>>>(k);
+  else
+    layer_norm_held_forward_kernel<T, V, G><<<blocks, NormGroup<G>::THREADS, 0, st>>>(k);
+}
+
+// The vector form needs every row of every operand on a 16-byte boundary.
+template <typename T>
+void launch_norm_held(const LayerNormArgs& k, bool backward, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  bool vec = k.W % V == 0 && k.W % 4 == 0 && aligned16(k.x) && k.xm % V == 0 && k.xr % V == 0 && aligned16(k.w) &&
+             aligned16(k.b);
+  if (backward)
+    vec = vec && aligned16(k.dy) && k.dym % V == 0 && k.dyr % V == 0 && aligned16(k.dx);
+  else
+    vec = vec && aligned16(k.y);
+  if (!vec) {
+    if (k.W <= 32 * NORM_E)
+      launch_norm<T, 1, 32>(k, backward, st);
+    else if (k.W <= 128 * NORM_E)
+      launch_norm<T, 1, 128>(k, backward, st);
+    else
+      launch_norm<T, 1, 512>(k, backward, st);
+    return;
+  }
+  switch (norm_lanes(k.W)) {
+    case 8: return launch_norm<T, V, 8>(k, backward, st);
+    case 32: return launch_norm<T, V, 32>(k, backward, st);
+    case 64: return launch_norm<T, V, 64>(k, backward, st);
+    case 128: return launch_norm<T, V, 128>(k, backward, st);
+    case 256: return launch_norm<T, V, 256>(k, backward, st);
+    default: return launch_norm<T, V, 512>(k, backward, st);
+  }
+}
+
+template <typename T>
+void launch_norm_wide_backward(const LayerNormArgs& k, cudaStream_t st) {
+  if (k.dx) layer_norm_dx_kernel<T><<<(unsigned)k.P * k.B, 256, 0, st>>>(k);
+  if (k.dw || k.db) layer_norm_dw_kernel<T><<<dim3((k.W + 255) / 256, k.P, k.S), 256, 0, st>>>(k);
+}
+
+}  // namespace
+}  // namespace tp
+
+extern "C" {
 
 size_t tp_layer_norm_workspace_size(int32_t P, int32_t B, int32_t W) {
   if (P <= 0 || B <= 0 || W <= 0) return 0;
-  const int s = layer_norm_splits(P, B, W);
+  const int s = norm_backward_splits(P, B, W);
   return s > 1 ? (size_t)2 * P * s * W * sizeof(float) : 0;
 }
 
@@ -1727,11 +1805,20 @@ int tp_layer_norm_forward(const tp_layer_norm_args* a, void* stream) {
   int rc = check_layer_norm(a);
   if (rc) return rc;
   if (!a->y) return fail(TP_EINVAL, "null layer norm output");
-  const LayerNormArgs k = layer_norm_args(a);
-  if (a->dtype == TP_DTYPE_BF16)
-    layer_norm_forward_kernel<__nv_bfloat16><<<(unsigned)(k.P * k.B), 256, 0, st>>>(k);
-  else
-    layer_norm_forward_kernel<float><<<(unsigned)(k.P * k.B), 256, 0, st>>>(k);
+  LayerNormArgs k = layer_norm_args(a);
+  const bool bf16 = a->dtype == TP_DTYPE_BF16;
+  if (k.W > NORM_HELD) {
+    if (bf16)
+      layer_norm_forward_kernel<__nv_bfloat16><<<(unsigned)k.P * k.B, 256, 0, st>>>(k);
+    else
+      layer_norm_forward_kernel<float><<<(unsigned)k.P * k.B, 256, 0, st>>>(k);
+  } else {
+    k.S = norm_splits(k.P, k.B, k.W, norm_lanes(k.W) > 256 ? 296 : 592);
+    if (bf16)
+      launch_norm_held<__nv_bfloat16>(k, false, st);
+    else
+      launch_norm_held<float>(k, false, st);
+  }
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;
 }
@@ -1744,28 +1831,32 @@ int tp_layer_norm_backward(const tp_layer_norm_args* a, void* stream) {
   if (!a->dy) return fail(TP_EINVAL, "null layer norm gradient");
   if (a->dx && a->dx_dtype != a->dtype && a->dx_dtype != TP_DTYPE_F32) return fail(TP_EINVAL, "bad dx dtype");
   LayerNormArgs k = layer_norm_args(a);
-  const bool bf16 = a->dtype == TP_DTYPE_BF16;
-  if (a->dx) {
-    if (bf16)
-      layer_norm_dx_kernel<__nv_bfloat16><<<(unsigned)(k.P * k.B), 256, 0, st>>>(k);
-    else
-      layer_norm_dx_kernel<float><<<(unsigned)(k.P * k.B), 256, 0, st>>>(k);
-  }
-  if (a->dweight || a->dbias) {
-    k.S = layer_norm_splits(k.P, k.B, k.W);
-    k.rows_per_split = (k.B + k.S - 1) / k.S;
+  k.S = norm_backward_splits(k.P, k.B, k.W);
+  const bool params = a->dweight || a->dbias;
+  if (params) {
     const size_t need = tp_layer_norm_workspace_size(k.P, k.B, k.W);
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned4(a->workspace)))
       return fail(TP_EINVAL, "layer norm workspace of %zu bytes is smaller than the %zu needed, or not aligned",
                   a->workspace_bytes, need);
-    if (k.P > 65535) return fail(TP_EINVAL, "too many members for one layer norm call");
     k.partial = static_cast<float*>(a->workspace);
-    const unsigned cols = (k.W + 255) / 256;
+  } else if (!a->dx) {
+    return TP_OK;
+  }
+  const bool bf16 = a->dtype == TP_DTYPE_BF16;
+  if (k.W > NORM_HELD) {
+    if (k.P > 65535) return fail(TP_EINVAL, "too many members of this width for one layer norm call");
     if (bf16)
-      layer_norm_dw_kernel<__nv_bfloat16><<<dim3(cols, k.P, k.S), 256, 0, st>>>(k);
+      launch_norm_wide_backward<__nv_bfloat16>(k, st);
     else
-      layer_norm_dw_kernel<float><<<dim3(cols, k.P, k.S), 256, 0, st>>>(k);
-    if (k.S > 1) layer_norm_finish_kernel<<<dim3(cols, k.P), 256, 0, st>>>(k);
+      launch_norm_wide_backward<float>(k, st);
+  } else if (bf16) {
+    launch_norm_held<__nv_bfloat16>(k, true, st);
+  } else {
+    launch_norm_held<float>(k, true, st);
+  }
+  if (params && k.S > 1) {
+    const int col_blocks = (k.W + 31) / 32;
+    layer_norm_finish_kernel<<<(unsigned)k.P * col_blocks, 256, 0, st>>>(k, col_blocks);
   }
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;

@@ -134,7 +134,7 @@ def test_shared_input(W, dtype):
 
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize('W,ld', [(10, 16), (100, 104), (300, 301), (64, 65)])
+@pytest.mark.parametrize('W,ld', [(10, 16), (100, 104), (104, 112), (300, 301), (64, 65), (2000, 2008)])
 def test_rows_of_padded_buffers(W, ld, dtype):
     """Column slices of wider buffers: rows that are not packed, aligned and not; the buffer's other
     columns hold NaN, as does the padding beyond each member's width."""
@@ -149,6 +149,8 @@ def test_rows_of_padded_buffers(W, ld, dtype):
             x = view
         else:
             dy = view
+    for m in range(3):
+        w[m, int(n[m]):] = b[m, int(n[m]):] = float('nan')
     run_and_check(x, dy, w, b, n)
 
 
