@@ -15,8 +15,12 @@
 //
 // Everything a code depends on is computed in fp32 with one rounding per operation (no fused
 // multiply-add), so a stored state does not depend on how the compiler contracts.  The parameter
-// update uses the unrounded moments and the approximate reciprocal and division (2 ulp), below the
-// rounding of p itself.
+// update uses the unrounded moments and an approximate reciprocal (1 ulp), below the rounding of p.
+//
+// Bound: 16.1 bytes an element against some 70 instructions (a quarter of them the random bits), near
+// the point where the SM's issue slots and the memory take equally long.  So the fp32 arithmetic is
+// done in pairs (f32x2), the codes of a block are formed without the rules for subnormals, zeros and
+// empty blocks where a vote says that none is there, and the next block is on its way meanwhile.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -27,7 +31,6 @@ namespace tp {
 
 constexpr int ADAMW8_BLOCK = 128;        // elements per scale: one warp, four consecutive elements a lane
 constexpr int ADAMW8_WARPS = 8;
-constexpr int ADAMW8_TILE = 32;          // blocks of one CTA
 constexpr float ADAMW8_TINY = 7.8886090522101181e-31f;  // 2^-100: a block below it is stored as zeros
 
 struct AdamW8Scalars {
@@ -51,6 +54,7 @@ struct AdamW8Tensors {
   uint32_t tile0[TP_MAX_OPT_TENSORS + 1];        // first tile of each tensor; one tile = one CTA's blocks
   uint32_t member_tiles[TP_MAX_OPT_TENSORS];     // tiles of one member
   int n;
+  int tile_blocks;                               // blocks of one tile
 };
 
 struct AdamW8Member {
@@ -77,147 +81,290 @@ __device__ __forceinline__ AdamW8Member adamw8_member(const AdamW8Scalars& s, in
   return c;
 }
 
-__device__ __forceinline__ float4 adamw8_load_first(uint32_t c, float scale) {
+// Two fp32 values in one 64-bit register pair: one instruction, each half rounded on its own.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 halves(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Four e4m3 codes -> their values times `scale`, as pairs.
+__device__ __forceinline__ void adamw8_load_first(uint32_t c, f32x2 scale, f32x2 (&m)[2]) {
   const __half2 a(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c & 0xFFFFu), __NV_E4M3));
   const __half2 b(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c >> 16), __NV_E4M3));
   const float2 x = __half22float2(a), y = __half22float2(b);
-  return make_float4(__fmul_rn(x.x, scale), __fmul_rn(x.y, scale), __fmul_rn(y.x, scale), __fmul_rn(y.y, scale));
+  m[0] = mul2(pair(x.x, x.y), scale);
+  m[1] = mul2(pair(y.x, y.y), scale);
 }
 
-__device__ __forceinline__ float adamw8_load_root(uint32_t code, float scale) {
-  const float v = code ? __uint_as_float((code + (112u << 4)) << 19) : 0.0f;
-  return __fmul_rn(v, scale);
+// Four e4m4 codes: code c > 0 is the fp32 number with the bits (c + 112 * 16) << 19.
+__device__ __forceinline__ void adamw8_load_root(uint32_t c, f32x2 scale, f32x2 (&u)[2]) {
+  constexpr uint32_t bias = (112u << 4) << 19;
+  float v[4] = {__uint_as_float((c & 0xFFu) * (1u << 19) + bias), __uint_as_float((c & 0xFF00u) * (1u << 11) + bias),
+                __uint_as_float((c & 0xFF0000u) * (1u << 3) + bias), __uint_as_float((c >> 24) * (1u << 19) + bias)};
+  if (((c - 0x01010101u) & ~c & 0x80808080u) != 0) {  // a zero byte
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (((c >> (8 * j)) & 0xFFu) == 0) v[j] = 0.0f;
+  }
+  u[0] = mul2(pair(v[0], v[1]), scale);
+  u[1] = mul2(pair(v[2], v[3]), scale);
 }
 
-// e4m3 code of x / scale (inv = 1 / scale), rounded with the 16 random bits r.
-__device__ __forceinline__ uint32_t adamw8_store_first(float x, float inv, uint32_t r) {
-  const float y = fminf(__fmul_rn(fabsf(x), inv), 448.0f);
+// e4m3 code of |x| / scale = y for any y, rounded with the 16 random bits r.
+__device__ __forceinline__ uint32_t adamw8_code_first(float y, uint32_t r) {
   const uint32_t normal = ((__float_as_uint(y) + (r << 4)) >> 20) - (120u << 3);
   const uint32_t small = (uint32_t)__fadd_rn(__fmul_rn(y, 512.0f), __fmul_rn((float)r, 1.0f / 65536.0f));
-  return (y >= 0.015625f ? normal : small) | (x < 0.0f ? 128u : 0u);
+  return y >= 0.015625f ? normal : small;
 }
 
-// e4m4 code of u / scale.
-__device__ __forceinline__ uint32_t adamw8_store_root(float u, float inv, uint32_t r) {
-  const float y = fminf(__fmul_rn(u, inv), 1.9375f);
+// e4m4 code of u / scale = y.
+__device__ __forceinline__ uint32_t adamw8_code_root(float u, float y, uint32_t r) {
   const int code = (int)((__float_as_uint(y) + (r << 3)) >> 19) - (112 << 4);
   return u > 0.0f ? (uint32_t)min(max(code, 1), 255) : 0u;
 }
 
-// Scale and reciprocal of a block whose largest magnitude has the bits `big`.  A block that is
-// next to nothing is stored as zeros (its reciprocal would overflow); one with an infinity or a NaN
-// gets a NaN scale and zero codes, so that every moment of the block reads as NaN.
-__device__ __forceinline__ void adamw8_scale(uint32_t big, float top, float& scale, float& inv) {
-  const float b = __uint_as_float(big);
-  scale = 0.0f;
-  inv = 0.0f;
-  if (big >= 0x7F800000u) {
-    scale = __uint_as_float(0x7FC00000u);
-  } else if (b >= ADAMW8_TINY) {
-    scale = __fmul_rn(b, 1.0f / top);
-    inv = __fdiv_rn(1.0f, scale);
+__device__ __forceinline__ uint32_t bytes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// One lane's share of a block.
+struct AdamW8Lane {
+  float p[4], g[4];
+  uint32_t m, v;  // codes
+  float ms, vs;   // the block's scales
+};
+
+// Element j of lane `lane`: consecutive elements with vector access, else 32 apart, so that both
+// ways neighbouring lanes touch neighbouring memory.
+template <bool VEC>
+__device__ __forceinline__ int adamw8_at(int lane, int j) {
+  return VEC ? 4 * lane + j : lane + 32 * j;
+}
+
+struct AdamW8Ptr {
+  float* p;
+  const float* g;
+  uint8_t* m;
+  uint8_t* v;
+  float* ms;
+  float* vs;
+};
+
+// `left`: elements of the member from the block's first on.
+template <bool VEC>
+__device__ __forceinline__ void adamw8_fetch(AdamW8Lane& x, const AdamW8Ptr& a, int64_t b, int64_t left, int lane) {
+  x.ms = a.ms[b];
+  x.vs = a.vs[b];
+  const int64_t e = b * ADAMW8_BLOCK;
+  if (VEC) {
+    if (4 * lane < left) {
+      const float4 p4 = *reinterpret_cast<const float4*>(a.p + e + 4 * lane);
+      const float4 g4 = __ldcs(reinterpret_cast<const float4*>(a.g + e + 4 * lane));
+      x.p[0] = p4.x, x.p[1] = p4.y, x.p[2] = p4.z, x.p[3] = p4.w;
+      x.g[0] = g4.x, x.g[1] = g4.y, x.g[2] = g4.z, x.g[3] = g4.w;
+      x.m = *reinterpret_cast<const uint32_t*>(a.m + e + 4 * lane);
+      x.v = *reinterpret_cast<const uint32_t*>(a.v + e + 4 * lane);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x.p[j] = x.g[j] = 0.0f;
+    x.m = x.v = 0;
+  } else {
+    uint32_t mb[4], vb[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = lane + 32 * j;
+      const bool in = at < left;
+      x.p[j] = in ? a.p[e + at] : 0.0f;
+      x.g[j] = in ? __ldcs(a.g + e + at) : 0.0f;
+      mb[j] = in ? a.m[e + at] : 0u;
+      vb[j] = in ? a.v[e + at] : 0u;
+    }
+    x.m = bytes4(mb[0], mb[1], mb[2], mb[3]);
+    x.v = bytes4(vb[0], vb[1], vb[2], vb[3]);
   }
 }
 
-// The tensor, member and first block of tile `tile`.
-__device__ __forceinline__ int adamw8_tensor_of(const AdamW8Tensors& ts, uint32_t tile) {
-  int i = 0;
-  while (i + 1 < ts.n && tile >= ts.tile0[i + 1]) ++i;
-  return i;
+template <bool VEC>
+__device__ __forceinline__ void adamw8_block(const AdamW8Lane& x, const AdamW8Member& c, const AdamW8Ptr& a, int64_t b,
+                                             int64_t left, int lane, uint4 counter, const uint32_t* ks,
+                                             uint32_t* words) {
+  f32x2 m[2], u[2];
+  adamw8_load_first(x.m, pair(x.ms, x.ms), m);
+  adamw8_load_root(x.v, pair(x.vs, x.vs), u);
+  float mm[4], uu[4], p[4];
+  const f32x2 b1 = pair(c.b1, c.b1), o1 = pair(c.one_m_b1, c.one_m_b1), b2 = pair(c.b2, c.b2),
+              o2 = pair(c.one_m_b2, c.one_m_b2);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const f32x2 g = pair(x.g[2 * h], x.g[2 * h + 1]);
+    // the sums one by one: the assembler would contract a paired product and sum
+    const float2 ma = halves(mul2(m[h], b1)), mb = halves(mul2(g, o1));
+    const float2 va = halves(mul2(mul2(u[h], u[h]), b2)), vb = halves(mul2(mul2(g, g), o2));
+    mm[2 * h] = __fadd_rn(ma.x, mb.x), mm[2 * h + 1] = __fadd_rn(ma.y, mb.y);
+    uu[2 * h] = __fsqrt_rn(__fadd_rn(va.x, vb.x)), uu[2 * h + 1] = __fsqrt_rn(__fadd_rn(va.y, vb.y));
+    m[h] = pair(mm[2 * h], mm[2 * h + 1]);
+    // p (1 - lr wd) - step m / (u / sqrt(bc2) + eps)
+    u[h] = pair(uu[2 * h], uu[2 * h + 1]);
+    const float2 den = halves(fma2(u[h], pair(c.inv_sqrt_bc2, c.inv_sqrt_bc2), pair(c.eps, c.eps)));
+    const f32x2 r = pair(__fdividef(1.0f, den.x), __fdividef(1.0f, den.y));
+    const f32x2 up = mul2(mul2(m[h], pair(-c.step_size, -c.step_size)), r);
+    const float2 pf = halves(fma2(pair(x.p[2 * h], x.p[2 * h + 1]), pair(c.mult, c.mult), up));
+    p[2 * h] = pf.x, p[2 * h + 1] = pf.y;
+  }
+  const bool whole = left >= ADAMW8_BLOCK;
+  if (!whole) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (adamw8_at<VEC>(lane, j) >= left) mm[j] = uu[j] = 0.0f;
+  }
+  // the block's largest magnitudes (as integers: a NaN is above everything)
+  uint32_t mbig = 0, ubig = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    mbig = max(mbig, __float_as_uint(mm[j]) & 0x7FFFFFFFu);
+    ubig = max(ubig, __float_as_uint(uu[j]) & 0x7FFFFFFFu);
+  }
+  mbig = __reduce_max_sync(0xFFFFFFFFu, mbig);
+  ubig = __reduce_max_sync(0xFFFFFFFFu, ubig);
+  // even lanes form the first moment's scale, odd ones the root's
+  float scale = 0.0f, inv = 0.0f;
+  {
+    const uint32_t big = lane & 1 ? ubig : mbig;
+    if (big >= 0x7F800000u) {
+      scale = __uint_as_float(0x7FC00000u);  // every moment of the block reads as NaN
+    } else if (__uint_as_float(big) >= ADAMW8_TINY) {
+      scale = __fmul_rn(__uint_as_float(big), lane & 1 ? 1.0f / 1.9375f : 1.0f / 448.0f);
+      inv = __frcp_rn(scale);
+    }
+  }
+  const float minv = __shfl_sync(0xFFFFFFFFu, inv, 0), vinv = __shfl_sync(0xFFFFFFFFu, inv, 1);
+  const uint4 rnd = philox4x32_10_ks(counter, ks);
+  uint32_t rw[4] = {rnd.x, rnd.y, rnd.z, rnd.w};
+  if (!VEC) {  // the words of elements 4 l .. 4 l + 3 to the lanes that hold those elements
+    reinterpret_cast<uint4*>(words)[lane] = rnd;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) rw[j] = words[lane + 32 * j];
+    __syncwarp();
+  }
+  float ym[4], yu[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    ym[j] = __fmul_rn(fabsf(mm[j]), minv);
+    yu[j] = __fmul_rn(uu[j], vinv);
+  }
+  // a value scaled by the rounded reciprocal exceeds the code's largest by 3 ulp at most, which the
+  // random bits (16 of the 20 or 19 dropped ones, 8 or 16 ulp short of a carry) do not carry over
+  const bool usual = fminf(fminf(ym[0], ym[1]), fminf(ym[2], ym[3])) >= 0.015625f &&
+                     fminf(fminf(yu[0], yu[1]), fminf(yu[2], yu[3])) >= 3.2424927e-05f;  // 2^-15 (1 + 1 / 16)
+  uint32_t mc[4], vc[4];
+  if (__all_sync(0xFFFFFFFFu, usual)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      mc[j] = (__float_as_uint(ym[j]) + ((rw[j] << 4) & 0xFFFF0u) - ((120u << 3) << 20)) >> 20;
+      vc[j] = (__float_as_uint(yu[j]) + ((rw[j] >> 13) & 0x7FFF8u) - ((112u << 4) << 19)) >> 19;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      mc[j] = minv > 0.0f ? adamw8_code_first(ym[j], rw[j] & 0xFFFFu) : 0u;
+      vc[j] = vinv > 0.0f ? adamw8_code_root(uu[j], yu[j], rw[j] >> 16) : 0u;
+    }
+  }
+  // the signs are the top bits of the values' top bytes
+  const uint32_t signs = __byte_perm(__byte_perm(__float_as_uint(mm[0]), __float_as_uint(mm[1]), 0x0073),
+                                     __byte_perm(__float_as_uint(mm[2]), __float_as_uint(mm[3]), 0x0073), 0x5410);
+  uint32_t mo = bytes4(mc[0], mc[1], mc[2], mc[3]);
+  if (minv > 0.0f) mo |= signs & 0x80808080u;
+  const uint32_t vo = bytes4(vc[0], vc[1], vc[2], vc[3]);
+  const int64_t e = b * ADAMW8_BLOCK;
+  if (VEC) {
+    if (4 * lane < left) {
+      *reinterpret_cast<float4*>(a.p + e + 4 * lane) = make_float4(p[0], p[1], p[2], p[3]);
+      *reinterpret_cast<uint32_t*>(a.m + e + 4 * lane) = mo;
+      *reinterpret_cast<uint32_t*>(a.v + e + 4 * lane) = vo;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = lane + 32 * j;
+      if (at < left) {
+        a.p[e + at] = p[j];
+        a.m[e + at] = (uint8_t)(mo >> (8 * j));
+        a.v[e + at] = (uint8_t)(vo >> (8 * j));
+      }
+    }
+  }
+  if (lane < 2) (lane ? a.vs : a.ms)[b] = scale;
 }
 
-// One warp takes one block of 128 elements at a time: lane l holds elements 4 l .. 4 l + 3, the two
-// block maxima are warp reductions.
+template <bool VEC>
+__device__ __forceinline__ void adamw8_tile(const AdamW8Member& c, const AdamW8Ptr& a, int64_t first, int64_t last,
+                                            int64_t inner, uint4 counter, const uint32_t* ks, uint32_t* words) {
+  const int lane = lane_id();
+  int64_t b = first + warp_id();
+  if (b >= last) return;
+  AdamW8Lane next;
+  adamw8_fetch<VEC>(next, a, b, inner - b * ADAMW8_BLOCK, lane);
+  for (; b < last; b += ADAMW8_WARPS) {
+    const AdamW8Lane x = next;
+    const int64_t n = b + ADAMW8_WARPS;
+    if (n < last) adamw8_fetch<VEC>(next, a, n, inner - n * ADAMW8_BLOCK, lane);
+    counter.x = (uint32_t)(b * (ADAMW8_BLOCK / 4) + lane);
+    adamw8_block<VEC>(x, c, a, b, inner - b * ADAMW8_BLOCK, lane, counter, ks, words);
+  }
+}
+
+// One warp takes one block of 128 elements at a time, four a lane; the block's maxima are warp
+// reductions.  The grid is one CTA per tile of a member's blocks, over all members and tensors.
 __global__ void __launch_bounds__(32 * ADAMW8_WARPS) adamw8_kernel(const __grid_constant__ AdamW8Tensors ts,
                                                                    const __grid_constant__ AdamW8Scalars s) {
-  const int ti = adamw8_tensor_of(ts, blockIdx.x);
+  __shared__ AdamW8Member shared;
+  __shared__ __align__(16) uint32_t words[ADAMW8_WARPS][ADAMW8_BLOCK];
+  int ti = 0;
+  while (ti + 1 < ts.n && blockIdx.x >= ts.tile0[ti + 1]) ++ti;
   const tp_opt8_tensor& T = ts.t[ti];
   const uint32_t local = blockIdx.x - ts.tile0[ti];
-  const int m = (int)(local / ts.member_tiles[ti]);
+  const uint32_t m = local / ts.member_tiles[ti];
+  // the coefficients take a logarithm and an exponential each: one warp forms them
+  if (warp_id() == 0) {
+    const AdamW8Member c = adamw8_member(s, (int)m, T.step);
+    if (lane_id() == 0) shared = c;
+  }
+  __syncthreads();
+  const AdamW8Member c = shared;
   const int64_t inner = T.inner;
   const int64_t nb = (inner + ADAMW8_BLOCK - 1) / ADAMW8_BLOCK;
-  const int64_t first = (int64_t)(local % ts.member_tiles[ti]) * ADAMW8_TILE;
-  const int lane = lane_id();
-  const AdamW8Member c = adamw8_member(s, m, T.step);
-  const uint32_t step = (uint32_t)(T.step ? T.step[m] : s.step);
-  float* P = T.p + m * inner;
-  const float* G = T.grad + m * inner;
-  uint8_t* M = T.exp_avg + m * inner;
-  uint8_t* V = T.exp_avg_sq + m * inner;
-  float* MS = T.exp_avg_scale + m * nb;
-  float* VS = T.exp_avg_sq_scale + m * nb;
+  const int64_t first = (int64_t)(local - m * ts.member_tiles[ti]) * ts.tile_blocks;
+  const int64_t last = min(nb, first + ts.tile_blocks);
+  const AdamW8Ptr a = {T.p + m * inner,       T.grad + m * inner,       T.exp_avg + m * inner,
+                       T.exp_avg_sq + m * inner, T.exp_avg_scale + m * nb, T.exp_avg_sq_scale + m * nb};
+  const uint4 counter = make_uint4(0, T.id, s.member_base + m, (uint32_t)(T.step ? T.step[m] : s.step));
   const bool vec = (inner & 3) == 0 &&
                    ((reinterpret_cast<uintptr_t>(T.p) | reinterpret_cast<uintptr_t>(T.grad)) & 15u) == 0 &&
                    ((reinterpret_cast<uintptr_t>(T.exp_avg) | reinterpret_cast<uintptr_t>(T.exp_avg_sq)) & 3u) == 0;
-  const int64_t last = min(nb, first + ADAMW8_TILE);
-  for (int64_t b = first + warp_id(); b < last; b += ADAMW8_WARPS) {
-    const int64_t e = b * ADAMW8_BLOCK + 4 * lane;
-    const int have = (int)max((int64_t)0, min((int64_t)4, inner - e));
-    float p[4] = {0, 0, 0, 0}, g[4] = {0, 0, 0, 0};
-    uint32_t mc = 0, vc = 0;
-    if (vec && have == 4) {
-      const float4 p4 = *reinterpret_cast<const float4*>(P + e);
-      const float4 g4 = __ldcs(reinterpret_cast<const float4*>(G + e));
-      p[0] = p4.x, p[1] = p4.y, p[2] = p4.z, p[3] = p4.w;
-      g[0] = g4.x, g[1] = g4.y, g[2] = g4.z, g[3] = g4.w;
-      mc = *reinterpret_cast<const uint32_t*>(M + e);
-      vc = *reinterpret_cast<const uint32_t*>(V + e);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < have) {
-          p[j] = P[e + j];
-          g[j] = G[e + j];
-          mc |= (uint32_t)M[e + j] << (8 * j);
-          vc |= (uint32_t)V[e + j] << (8 * j);
-        }
-    }
-    const float4 m4 = adamw8_load_first(mc, MS[b]);
-    const float us = VS[b];
-    float mm[4] = {m4.x, m4.y, m4.z, m4.w}, u[4];
-    uint32_t mbig = 0, ubig = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float u0 = adamw8_load_root((vc >> (8 * j)) & 0xFFu, us);
-      mm[j] = __fadd_rn(__fmul_rn(mm[j], c.b1), __fmul_rn(g[j], c.one_m_b1));
-      u[j] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(u0, u0), c.b2), __fmul_rn(__fmul_rn(g[j], g[j]), c.one_m_b2)));
-      if (j >= have) mm[j] = u[j] = 0.0f;
-      mbig = max(mbig, __float_as_uint(fabsf(mm[j])));
-      ubig = max(ubig, __float_as_uint(u[j]) & 0x7FFFFFFFu);
-      p[j] = p[j] * c.mult - c.step_size * __fdividef(mm[j], u[j] * c.inv_sqrt_bc2 + c.eps);
-    }
-    mbig = __reduce_max_sync(0xFFFFFFFFu, mbig);
-    ubig = __reduce_max_sync(0xFFFFFFFFu, ubig);
-    float ms, minv, vs, vinv;
-    adamw8_scale(mbig, 448.0f, ms, minv);
-    adamw8_scale(ubig, 1.9375f, vs, vinv);
-    const uint4 r = philox4x32_10_ks(make_uint4((uint32_t)(e >> 2), T.id, s.member_base + (uint32_t)m, step), s.ks);
-    const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
-    uint32_t mo = 0, vo = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (minv > 0.0f) mo |= adamw8_store_first(mm[j], minv, rw[j] & 0xFFFFu) << (8 * j);
-      if (vinv > 0.0f) vo |= adamw8_store_root(u[j], vinv, rw[j] >> 16) << (8 * j);
-    }
-    if (vec && have == 4) {
-      *reinterpret_cast<float4*>(P + e) = make_float4(p[0], p[1], p[2], p[3]);
-      *reinterpret_cast<uint32_t*>(M + e) = mo;
-      *reinterpret_cast<uint32_t*>(V + e) = vo;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < have) {
-          P[e + j] = p[j];
-          M[e + j] = (uint8_t)(mo >> (8 * j));
-          V[e + j] = (uint8_t)(vo >> (8 * j));
-        }
-    }
-    __syncwarp();  // every lane has read the block's scales
-    if (lane == 0) {
-      MS[b] = ms;
-      VS[b] = vs;
-    }
-  }
+  if (vec)
+    adamw8_tile<true>(c, a, first, last, inner, counter, s.ks, words[warp_id()]);
+  else
+    adamw8_tile<false>(c, a, first, last, inner, counter, s.ks, words[warp_id()]);
 }
 
 struct AdamW8Moments {
@@ -225,6 +372,7 @@ struct AdamW8Moments {
   uint32_t tile0[TP_MAX_OPT_TENSORS + 1];
   uint32_t member_tiles[TP_MAX_OPT_TENSORS];
   int n;
+  int tile_blocks;
 };
 
 // The moments that the codes stand for: m and v = u^2, in fp32 or bf16.
@@ -234,22 +382,60 @@ __global__ void __launch_bounds__(32 * ADAMW8_WARPS) adamw8_moments_kernel(const
   while (ti + 1 < ts.n && blockIdx.x >= ts.tile0[ti + 1]) ++ti;
   const tp_opt8_values& A = ts.t[ti];
   const uint32_t local = blockIdx.x - ts.tile0[ti];
-  const int64_t m = local / ts.member_tiles[ti];
+  const uint32_t m = local / ts.member_tiles[ti];
   const int64_t inner = A.inner;
   const int64_t nb = (inner + ADAMW8_BLOCK - 1) / ADAMW8_BLOCK;
-  const int64_t first = (int64_t)(local % ts.member_tiles[ti]) * ADAMW8_TILE;
-  const int64_t last = min(nb, first + ADAMW8_TILE);
+  const int64_t first = (int64_t)(local - m * ts.member_tiles[ti]) * ts.tile_blocks;
+  const int64_t last = min(nb, first + ts.tile_blocks);
+  const uint8_t* mc = A.exp_avg + m * inner;
+  const uint8_t* vc = A.exp_avg_sq + m * inner;
+  const float* ms = A.exp_avg_scale + m * nb;
+  const float* vs = A.exp_avg_sq_scale + m * nb;
+  T* mo = reinterpret_cast<T*>(A.m) + m * inner;
+  T* vo = reinterpret_cast<T*>(A.v) + m * inner;
+  const bool vec = (inner & 3) == 0 &&
+                   ((reinterpret_cast<uintptr_t>(A.exp_avg) | reinterpret_cast<uintptr_t>(A.exp_avg_sq)) & 3u) == 0 &&
+                   ((reinterpret_cast<uintptr_t>(A.m) | reinterpret_cast<uintptr_t>(A.v)) & (4 * sizeof(T) - 1)) == 0;
+#pragma unroll 2
   for (int64_t b = first + warp_id(); b < last; b += ADAMW8_WARPS) {
-    const float ms = A.exp_avg_scale[m * nb + b], us = A.exp_avg_sq_scale[m * nb + b];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t e = b * ADAMW8_BLOCK + 32 * j + lane_id();
-      if (e < inner) {
-        const float x = adamw8_load_first(A.exp_avg[m * inner + e], ms).x;
-        const float u = adamw8_load_root(A.exp_avg_sq[m * inner + e], us);
-        reinterpret_cast<T*>(A.m)[m * inner + e] = from_f32<T>(x);
-        reinterpret_cast<T*>(A.v)[m * inner + e] = from_f32<T>(__fmul_rn(u, u));
+    const int64_t e = b * ADAMW8_BLOCK;
+    const int left = (int)min((int64_t)ADAMW8_BLOCK, inner - e), lane = lane_id();
+    uint32_t cm = 0, cv = 0;
+    if (vec) {
+      if (4 * lane < left) {
+        cm = __ldg(reinterpret_cast<const uint32_t*>(mc + e) + lane);
+        cv = __ldg(reinterpret_cast<const uint32_t*>(vc + e) + lane);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (lane + 32 * j < left) {
+          cm |= (uint32_t)mc[e + lane + 32 * j] << (8 * j);
+          cv |= (uint32_t)vc[e + lane + 32 * j] << (8 * j);
+        }
+    }
+    const float sm = ms[b], sv = vs[b];
+    f32x2 x[2], u[2];
+    adamw8_load_first(cm, pair(sm, sm), x);
+    adamw8_load_root(cv, pair(sv, sv), u);
+    const float2 x0 = halves(x[0]), x1 = halves(x[1]), u0 = halves(mul2(u[0], u[0])), u1 = halves(mul2(u[1], u[1]));
+    if (vec) {
+      if (4 * lane >= left) continue;
+      if constexpr (sizeof(T) == 2) {
+        reinterpret_cast<uint2*>(mo + e)[lane] = make_uint2(pack_bf16x2(x0.x, x0.y), pack_bf16x2(x1.x, x1.y));
+        reinterpret_cast<uint2*>(vo + e)[lane] = make_uint2(pack_bf16x2(u0.x, u0.y), pack_bf16x2(u1.x, u1.y));
+      } else {
+        reinterpret_cast<float4*>(mo + e)[lane] = make_float4(x0.x, x0.y, x1.x, x1.y);
+        reinterpret_cast<float4*>(vo + e)[lane] = make_float4(u0.x, u0.y, u1.x, u1.y);
+      }
+    } else {
+      const float xs[4] = {x0.x, x0.y, x1.x, x1.y}, us[4] = {u0.x, u0.y, u1.x, u1.y};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (lane + 32 * j < left) {
+          mo[e + lane + 32 * j] = from_f32<T>(xs[j]);
+          vo[e + lane + 32 * j] = from_f32<T>(us[j]);
+        }
     }
   }
 }

@@ -1572,25 +1572,29 @@ int tp_adamw_step(const tp_adamw_args* a, void* stream) {
   return TP_OK;
 }
 
-// Tiles of a launch over several packs: tensor i's members have member_tiles[i] tiles of
-// `tile_blocks` state blocks each.
-static int adamw8_tiles(int n, const int64_t* numel, const int64_t* inner, int tile_blocks, uint32_t* tile0,
-                        uint32_t* member_tiles) {
-  int64_t total = 0;
-  for (int i = 0; i < n; ++i) {
-    if (numel[i] <= 0 || inner[i] <= 0 || inner[i] > (1ll << 33) || numel[i] % inner[i] != 0)
-      return fail(TP_EINVAL, "tensor %d: %lld elements do not make members of %lld", i, (long long)numel[i],
-                  (long long)inner[i]);
-    const int64_t nb = (inner[i] + ADAMW8_BLOCK - 1) / ADAMW8_BLOCK;
-    const int64_t mt = (nb + tile_blocks - 1) / tile_blocks;
-    const int64_t members = numel[i] / inner[i];
-    tile0[i] = (uint32_t)total;
-    member_tiles[i] = (uint32_t)mt;
-    if (members > 0x7FFFFFFFLL / mt || (total += members * mt) > 0x7FFFFFFFLL)
-      return fail(TP_EINVAL, "too many elements for one 8-bit AdamW launch");
+// Tiles of a launch over several packs: tensor i's members have member_tiles[i] tiles of tile_blocks
+// state blocks each.  64 blocks a tile (8 a warp, which carry the tile's fixed cost), fewer
+// where that would leave SMs idle: at least two waves of 4 CTAs per SM, down to one block a warp.
+static int adamw8_tiles(int n, const int64_t* numel, const int64_t* inner, uint32_t* tile0, uint32_t* member_tiles,
+                        int* tile_blocks) {
+  for (int tb = 64;; tb /= 2) {
+    int64_t total = 0;
+    for (int i = 0; i < n; ++i) {
+      if (numel[i] <= 0 || inner[i] <= 0 || inner[i] > (1ll << 33) || numel[i] % inner[i] != 0)
+        return fail(TP_EINVAL, "tensor %d: %lld elements do not make members of %lld", i, (long long)numel[i],
+                    (long long)inner[i]);
+      const int64_t nb = (inner[i] + ADAMW8_BLOCK - 1) / ADAMW8_BLOCK;
+      const int64_t mt = (nb + tb - 1) / tb;
+      const int64_t members = numel[i] / inner[i];
+      tile0[i] = (uint32_t)total;
+      member_tiles[i] = (uint32_t)mt;
+      if (members > 0x7FFFFFFFLL / mt || (total += members * mt) > 0x7FFFFFFFLL)
+        return fail(TP_EINVAL, "too many elements for one 8-bit AdamW launch");
+    }
+    tile0[n] = (uint32_t)total;
+    *tile_blocks = tb;
+    if (tb == ADAMW8_WARPS || total >= 2 * 4 * 148) return TP_OK;
   }
-  tile0[n] = (uint32_t)total;
-  return TP_OK;
 }
 
 static bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
@@ -1614,7 +1618,7 @@ int tp_adamw8_step(const tp_adamw8_args* a, void* stream) {
     ts.t[i] = t;
   }
   if (any_scalar_step && a->step <= 0) return fail(TP_EINVAL, "the step count must be positive");
-  int rc = adamw8_tiles(ts.n, numel, inner, ADAMW8_TILE, ts.tile0, ts.member_tiles);
+  int rc = adamw8_tiles(ts.n, numel, inner, ts.tile0, ts.member_tiles, &ts.tile_blocks);
   if (rc) return rc;
   AdamW8Scalars s{};
   s.lr = a->lr.per_member;
@@ -1662,7 +1666,7 @@ int tp_adamw8_moments(const tp_adamw8_moments_args* a, void* stream) {
     inner[i] = t.inner;
     ts.t[i] = t;
   }
-  int rc = adamw8_tiles(ts.n, numel, inner, ADAMW8_TILE, ts.tile0, ts.member_tiles);
+  int rc = adamw8_tiles(ts.n, numel, inner, ts.tile0, ts.member_tiles, &ts.tile_blocks);
   if (rc) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (a->dtype == TP_DTYPE_BF16)
