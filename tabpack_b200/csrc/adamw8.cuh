@@ -31,6 +31,8 @@ namespace tp {
 
 constexpr int ADAMW8_BLOCK = 128;        // elements per scale: one warp, four consecutive elements a lane
 constexpr int ADAMW8_WARPS = 8;
+constexpr int ADAMW8_STAGES = 3;         // blocks of a warp on the way or in use
+constexpr int ADAMW8_STAGE = 32 * 40;    // bytes: p, g (16 a lane), both codes (4 a lane)
 constexpr float ADAMW8_TINY = 7.8886090522101181e-31f;  // 2^-100: a block below it is stored as zeros
 
 struct AdamW8Scalars {
@@ -54,7 +56,7 @@ struct AdamW8Tensors {
   uint32_t tile0[TP_MAX_OPT_TENSORS + 1];        // first tile of each tensor; one tile = one CTA's blocks
   uint32_t member_tiles[TP_MAX_OPT_TENSORS];     // tiles of one member
   int n;
-  int tile_blocks;                               // blocks of one tile
+  int tile_blocks;                               // blocks of one tile, 8 to 256
 };
 
 struct AdamW8Member {
@@ -79,29 +81,6 @@ __device__ __forceinline__ AdamW8Member adamw8_member(const AdamW8Scalars& s, in
   c.step_size = (s.lr || s.beta1 || steps) ? lr / bc1 : s.step_size_s;
   c.inv_sqrt_bc2 = (s.beta2 || steps) ? rsqrtf(bias_correction(c.one_m_b2, t)) : s.inv_sqrt_bc2_s;
   return c;
-}
-
-// Two fp32 values in one 64-bit register pair: one instruction, each half rounded on its own.
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pair(float a, float b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 halves(f32x2 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
 }
 
 // Four e4m3 codes -> their values times `scale`, as pairs.
@@ -144,6 +123,11 @@ __device__ __forceinline__ uint32_t bytes4(uint32_t a, uint32_t b, uint32_t c, u
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
+// The top bytes of four words.
+__device__ __forceinline__ uint32_t top4(const uint32_t (&w)[4]) {
+  return __byte_perm(__byte_perm(w[0], w[1], 0x0073), __byte_perm(w[2], w[3], 0x0073), 0x5410);
+}
+
 // One lane's share of a block.
 struct AdamW8Lane {
   float p[4], g[4];
@@ -158,54 +142,64 @@ __device__ __forceinline__ int adamw8_at(int lane, int j) {
   return VEC ? 4 * lane + j : lane + 32 * j;
 }
 
+// A lane's place in the warp's current block.
 struct AdamW8Ptr {
   float* p;
   const float* g;
   uint8_t* m;
   uint8_t* v;
-  float* ms;
-  float* vs;
+  __device__ void next() {
+    p += ADAMW8_BLOCK;
+    g += ADAMW8_BLOCK;
+    m += ADAMW8_BLOCK;
+    v += ADAMW8_BLOCK;
+  }
 };
 
-// `left`: elements of the member from the block's first on.
-template <bool VEC>
-__device__ __forceinline__ void adamw8_fetch(AdamW8Lane& x, const AdamW8Ptr& a, int64_t b, int64_t left, int lane) {
-  x.ms = a.ms[b];
-  x.vs = a.vs[b];
-  const int64_t e = b * ADAMW8_BLOCK;
-  if (VEC) {
-    if (4 * lane < left) {
-      const float4 p4 = *reinterpret_cast<const float4*>(a.p + e + 4 * lane);
-      const float4 g4 = __ldcs(reinterpret_cast<const float4*>(a.g + e + 4 * lane));
-      x.p[0] = p4.x, x.p[1] = p4.y, x.p[2] = p4.z, x.p[3] = p4.w;
-      x.g[0] = g4.x, x.g[1] = g4.y, x.g[2] = g4.z, x.g[3] = g4.w;
-      x.m = *reinterpret_cast<const uint32_t*>(a.m + e + 4 * lane);
-      x.v = *reinterpret_cast<const uint32_t*>(a.v + e + 4 * lane);
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x.p[j] = x.g[j] = 0.0f;
-    x.m = x.v = 0;
-  } else {
-    uint32_t mb[4], vb[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = lane + 32 * j;
-      const bool in = at < left;
-      x.p[j] = in ? a.p[e + at] : 0.0f;
-      x.g[j] = in ? __ldcs(a.g + e + at) : 0.0f;
-      mb[j] = in ? a.m[e + at] : 0u;
-      vb[j] = in ? a.v[e + at] : 0u;
-    }
-    x.m = bytes4(mb[0], mb[1], mb[2], mb[3]);
-    x.v = bytes4(vb[0], vb[1], vb[2], vb[3]);
+// Vector access: block `ahead` blocks on, copied to `stage` (each lane reads back what it
+// copied); `left`: elements of the member from that block's first on.
+__device__ __forceinline__ void adamw8_issue(uint32_t stage, const AdamW8Ptr& a, int ahead, int left, int lane) {
+  const int o = ahead * ADAMW8_BLOCK;
+  const bool in = 4 * lane < left;
+  if (left > 0) {
+    cp_async16(stage + 16 * lane, in ? a.p + o : a.p, in);
+    cp_async16(stage + 512 + 16 * lane, in ? a.g + o : a.g, in);
+    cp_async4(stage + 1024 + 4 * lane, in ? a.m + o : a.m, in);
+    cp_async4(stage + 1152 + 4 * lane, in ? a.v + o : a.v, in);
   }
+  cp_async_commit();
 }
 
+__device__ __forceinline__ void adamw8_take(AdamW8Lane& x, const char* stage, int lane) {
+  const float4 p4 = *reinterpret_cast<const float4*>(stage + 16 * lane);
+  const float4 g4 = *reinterpret_cast<const float4*>(stage + 512 + 16 * lane);
+  x.p[0] = p4.x, x.p[1] = p4.y, x.p[2] = p4.z, x.p[3] = p4.w;
+  x.g[0] = g4.x, x.g[1] = g4.y, x.g[2] = g4.z, x.g[3] = g4.w;
+  x.m = *reinterpret_cast<const uint32_t*>(stage + 1024 + 4 * lane);
+  x.v = *reinterpret_cast<const uint32_t*>(stage + 1152 + 4 * lane);
+}
+
+// Any alignment, the block `AHEAD` blocks on into registers.
+template <int AHEAD>
+__device__ __forceinline__ void adamw8_fetch(AdamW8Lane& x, const AdamW8Ptr& a, int left, int lane) {
+  constexpr int o = AHEAD * ADAMW8_BLOCK;
+  uint32_t mb[4], vb[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bool in = lane + 32 * j < left;
+    x.p[j] = in ? a.p[o + 32 * j] : 0.0f;
+    x.g[j] = in ? __ldcs(a.g + o + 32 * j) : 0.0f;
+    mb[j] = in ? a.m[o + 32 * j] : 0u;
+    vb[j] = in ? a.v[o + 32 * j] : 0u;
+  }
+  x.m = bytes4(mb[0], mb[1], mb[2], mb[3]);
+  x.v = bytes4(vb[0], vb[1], vb[2], vb[3]);
+}
+
+// One block; returns its new scales.
 template <bool VEC>
-__device__ __forceinline__ void adamw8_block(const AdamW8Lane& x, const AdamW8Member& c, const AdamW8Ptr& a, int64_t b,
-                                             int64_t left, int lane, uint4 counter, const uint32_t* ks,
-                                             uint32_t* words) {
+__device__ __forceinline__ float2 adamw8_block(const AdamW8Lane& x, const AdamW8Member& c, const AdamW8Ptr& a, int left,
+                                             int lane, uint4 counter, const uint32_t* ks, uint32_t* words) {
   f32x2 m[2], u[2];
   adamw8_load_first(x.m, pair(x.ms, x.ms), m);
   adamw8_load_root(x.v, pair(x.vs, x.vs), u);
@@ -236,12 +230,8 @@ __device__ __forceinline__ void adamw8_block(const AdamW8Lane& x, const AdamW8Me
       if (adamw8_at<VEC>(lane, j) >= left) mm[j] = uu[j] = 0.0f;
   }
   // the block's largest magnitudes (as integers: a NaN is above everything)
-  uint32_t mbig = 0, ubig = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    mbig = max(mbig, __float_as_uint(mm[j]) & 0x7FFFFFFFu);
-    ubig = max(ubig, __float_as_uint(uu[j]) & 0x7FFFFFFFu);
-  }
+  uint32_t mbig = __float_as_uint(max_nan(max_nan(fabsf(mm[0]), fabsf(mm[1])), max_nan(fabsf(mm[2]), fabsf(mm[3]))));
+  uint32_t ubig = __float_as_uint(max_nan(max_nan(uu[0], uu[1]), max_nan(uu[2], uu[3])));
   mbig = __reduce_max_sync(0xFFFFFFFFu, mbig);
   ubig = __reduce_max_sync(0xFFFFFFFFu, ubig);
   // even lanes form the first moment's scale, odd ones the root's
@@ -271,74 +261,111 @@ __device__ __forceinline__ void adamw8_block(const AdamW8Lane& x, const AdamW8Me
     ym[j] = __fmul_rn(fabsf(mm[j]), minv);
     yu[j] = __fmul_rn(uu[j], vinv);
   }
-  // a value scaled by the rounded reciprocal exceeds the code's largest by 3 ulp at most, which the
-  // random bits (16 of the 20 or 19 dropped ones, 8 or 16 ulp short of a carry) do not carry over
-  const bool usual = fminf(fminf(ym[0], ym[1]), fminf(ym[2], ym[3])) >= 0.015625f &&
-                     fminf(fminf(yu[0], yu[1]), fminf(yu[2], yu[3])) >= 3.2424927e-05f;  // 2^-15 (1 + 1 / 16)
+  // Codes of normal values: the number's bits plus the random ones below the code's last place, then
+  // the code's 8 bits, shifted into the top byte (e4m3: exponent offset 120, whose 0xC0 in that byte
+  // the packed word takes off; e4m4: offset 112, 0).  A value scaled by the rounded reciprocal
+  // exceeds the code's largest by 3 ulp at most, which the 16 random bits (16 and 8 ulp short of a
+  // carry) do not carry over.
   uint32_t mc[4], vc[4];
-  if (__all_sync(0xFFFFFFFFu, usual)) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      mc[j] = (__float_as_uint(ym[j]) + ((rw[j] << 4) & 0xFFFF0u) - ((120u << 3) << 20)) >> 20;
-      vc[j] = (__float_as_uint(yu[j]) + ((rw[j] >> 13) & 0x7FFF8u) - ((112u << 4) << 19)) >> 19;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      mc[j] = minv > 0.0f ? adamw8_code_first(ym[j], rw[j] & 0xFFFFu) : 0u;
-      vc[j] = vinv > 0.0f ? adamw8_code_root(uu[j], yu[j], rw[j] >> 16) : 0u;
-    }
+  for (int j = 0; j < 4; ++j) {
+    mc[j] = __float_as_uint(ym[j]) * 16u + __byte_perm(rw[j], 0, 0x4104);
+    vc[j] = __float_as_uint(yu[j]) * 32u + __byte_perm(rw[j], 0, 0x4324);
   }
-  // the signs are the top bits of the values' top bytes
-  const uint32_t signs = __byte_perm(__byte_perm(__float_as_uint(mm[0]), __float_as_uint(mm[1]), 0x0073),
-                                     __byte_perm(__float_as_uint(mm[2]), __float_as_uint(mm[3]), 0x0073), 0x5410);
-  uint32_t mo = bytes4(mc[0], mc[1], mc[2], mc[3]);
-  if (minv > 0.0f) mo |= signs & 0x80808080u;
-  const uint32_t vo = bytes4(vc[0], vc[1], vc[2], vc[3]);
-  const int64_t e = b * ADAMW8_BLOCK;
+  uint32_t mo = (top4(mc) & 0x7F7F7F7Fu) ^ 0x40404040u, vo = top4(vc);
+  const bool msmall = !(fminf(fminf(ym[0], ym[1]), fminf(ym[2], ym[3])) >= 0.015625f);  // 2^-6
+  const bool usmall = !(fminf(fminf(yu[0], yu[1]), fminf(yu[2], yu[3])) >= 3.2424927e-05f);  // 2^-15 (1 + 1 / 16)
+  if (__any_sync(0xFFFFFFFFu, msmall)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mc[j] = minv > 0.0f ? adamw8_code_first(ym[j], rw[j] & 0xFFFFu) : 0u;
+    mo = bytes4(mc[0], mc[1], mc[2], mc[3]);
+  }
+  if (__any_sync(0xFFFFFFFFu, usmall)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vc[j] = vinv > 0.0f ? adamw8_code_root(uu[j], yu[j], rw[j] >> 16) : 0u;
+    vo = bytes4(vc[0], vc[1], vc[2], vc[3]);
+  }
+  // the signs are the top bits of the values
+  const uint32_t mb[4] = {__float_as_uint(mm[0]), __float_as_uint(mm[1]), __float_as_uint(mm[2]), __float_as_uint(mm[3])};
+  if (minv > 0.0f) mo |= top4(mb) & 0x80808080u;
   if (VEC) {
     if (4 * lane < left) {
-      *reinterpret_cast<float4*>(a.p + e + 4 * lane) = make_float4(p[0], p[1], p[2], p[3]);
-      *reinterpret_cast<uint32_t*>(a.m + e + 4 * lane) = mo;
-      *reinterpret_cast<uint32_t*>(a.v + e + 4 * lane) = vo;
+      *reinterpret_cast<float4*>(a.p) = make_float4(p[0], p[1], p[2], p[3]);
+      *reinterpret_cast<uint32_t*>(a.m) = mo;
+      *reinterpret_cast<uint32_t*>(a.v) = vo;
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int at = lane + 32 * j;
-      if (at < left) {
-        a.p[e + at] = p[j];
-        a.m[e + at] = (uint8_t)(mo >> (8 * j));
-        a.v[e + at] = (uint8_t)(vo >> (8 * j));
+      if (lane + 32 * j < left) {
+        a.p[32 * j] = p[j];
+        a.m[32 * j] = (uint8_t)(mo >> (8 * j));
+        a.v[32 * j] = (uint8_t)(vo >> (8 * j));
       }
     }
   }
-  if (lane < 2) (lane ? a.vs : a.ms)[b] = scale;
+  return make_float2(__shfl_sync(0xFFFFFFFFu, scale, 0), __shfl_sync(0xFFFFFFFFu, scale, 1));
 }
 
+// The warp's share of a tile, `run` blocks from `run` times its number on (`blocks` in all).  `a`
+// points to the tile's first element, `left` are the elements of the member from there on.  Lane i
+// holds the scales of the warp's i-th block from first to last: one load and one store for the run.
+// (Scales stored block by block, 4 bytes into sectors that other warps read, cost half the time:
+// 850 us against 511 us for the same traffic without them, 209 M elements.)
 template <bool VEC>
-__device__ __forceinline__ void adamw8_tile(const AdamW8Member& c, const AdamW8Ptr& a, int64_t first, int64_t last,
-                                            int64_t inner, uint4 counter, const uint32_t* ks, uint32_t* words) {
-  const int lane = lane_id();
-  int64_t b = first + warp_id();
-  if (b >= last) return;
+__device__ __forceinline__ void adamw8_tile(const AdamW8Member& c, AdamW8Ptr a, float* ms, float* vs, int run, int blocks,
+                                            int left, uint4 counter, const uint32_t* ks, char* stages) {
+  const int lane = lane_id(), first = warp_id() * run, at = first * ADAMW8_BLOCK + (VEC ? 4 * lane : lane);
+  const int n = min(run, blocks - first);
+  if (n <= 0) return;
+  a.p += at;
+  a.g += at;
+  a.m += at;
+  a.v += at;
+  left -= first * ADAMW8_BLOCK;
+  counter.x += first * (ADAMW8_BLOCK / 4) + lane;
+  float sm = 0.0f, sv = 0.0f;
+  if (lane < n) sm = ms[first + lane], sv = vs[first + lane];
+  const uint32_t base = smem_u32(stages);
   AdamW8Lane next;
-  adamw8_fetch<VEC>(next, a, b, inner - b * ADAMW8_BLOCK, lane);
-  for (; b < last; b += ADAMW8_WARPS) {
-    const AdamW8Lane x = next;
-    const int64_t n = b + ADAMW8_WARPS;
-    if (n < last) adamw8_fetch<VEC>(next, a, n, inner - n * ADAMW8_BLOCK, lane);
-    counter.x = (uint32_t)(b * (ADAMW8_BLOCK / 4) + lane);
-    adamw8_block<VEC>(x, c, a, b, inner - b * ADAMW8_BLOCK, lane, counter, ks, words);
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < ADAMW8_STAGES - 1; ++i)
+      adamw8_issue(base + i * ADAMW8_STAGE, a, i, i < n ? left - i * ADAMW8_BLOCK : 0, lane);
+  } else {
+    adamw8_fetch<0>(next, a, left, lane);
   }
+  int slot = 0;
+  for (int i = 0; i < n; ++i) {
+    AdamW8Lane x;
+    if constexpr (VEC) {
+      cp_async_wait<ADAMW8_STAGES - 2>();
+      adamw8_take(x, stages + slot * ADAMW8_STAGE, lane);
+      const int into = slot == 0 ? ADAMW8_STAGES - 1 : slot - 1;  // the block before: read, and free
+      constexpr int ahead = ADAMW8_STAGES - 1;
+      adamw8_issue(base + into * ADAMW8_STAGE, a, ahead, i + ahead < n ? left - ahead * ADAMW8_BLOCK : 0, lane);
+      slot = slot + 1 == ADAMW8_STAGES ? 0 : slot + 1;
+    } else {
+      x = next;
+      if (i + 1 < n) adamw8_fetch<1>(next, a, left - ADAMW8_BLOCK, lane);
+    }
+    x.ms = __shfl_sync(0xFFFFFFFFu, sm, i);
+    x.vs = __shfl_sync(0xFFFFFFFFu, sv, i);
+    const float2 scale = adamw8_block<VEC>(x, c, a, left, lane, counter, ks, reinterpret_cast<uint32_t*>(stages));
+    if (lane == i) sm = scale.x, sv = scale.y;
+    a.next();
+    left -= ADAMW8_BLOCK;
+    counter.x += ADAMW8_BLOCK / 4;
+  }
+  if (lane < n) ms[first + lane] = sm, vs[first + lane] = sv;
 }
 
 // One warp takes one block of 128 elements at a time, four a lane; the block's maxima are warp
 // reductions.  The grid is one CTA per tile of a member's blocks, over all members and tensors.
-__global__ void __launch_bounds__(32 * ADAMW8_WARPS) adamw8_kernel(const __grid_constant__ AdamW8Tensors ts,
+__global__ void __launch_bounds__(32 * ADAMW8_WARPS, 4) adamw8_kernel(const __grid_constant__ AdamW8Tensors ts,
                                                                    const __grid_constant__ AdamW8Scalars s) {
   __shared__ AdamW8Member shared;
-  __shared__ __align__(16) uint32_t words[ADAMW8_WARPS][ADAMW8_BLOCK];
+  __shared__ __align__(16) char stages[ADAMW8_WARPS][ADAMW8_STAGES * ADAMW8_STAGE];
   int ti = 0;
   while (ti + 1 < ts.n && blockIdx.x >= ts.tile0[ti + 1]) ++ti;
   const tp_opt8_tensor& T = ts.t[ti];
@@ -354,17 +381,22 @@ __global__ void __launch_bounds__(32 * ADAMW8_WARPS) adamw8_kernel(const __grid_
   const int64_t inner = T.inner;
   const int64_t nb = (inner + ADAMW8_BLOCK - 1) / ADAMW8_BLOCK;
   const int64_t first = (int64_t)(local - m * ts.member_tiles[ti]) * ts.tile_blocks;
-  const int64_t last = min(nb, first + ts.tile_blocks);
-  const AdamW8Ptr a = {T.p + m * inner,       T.grad + m * inner,       T.exp_avg + m * inner,
-                       T.exp_avg_sq + m * inner, T.exp_avg_scale + m * nb, T.exp_avg_sq_scale + m * nb};
-  const uint4 counter = make_uint4(0, T.id, s.member_base + m, (uint32_t)(T.step ? T.step[m] : s.step));
+  const int blocks = (int)min((int64_t)ts.tile_blocks, nb - first);
+  const int64_t e = m * inner + first * ADAMW8_BLOCK;
+  const int left = (int)min((int64_t)ts.tile_blocks * ADAMW8_BLOCK, inner - first * ADAMW8_BLOCK);
+  const AdamW8Ptr a = {T.p + e, T.grad + e, T.exp_avg + e, T.exp_avg_sq + e};
+  float* ms = T.exp_avg_scale + m * nb + first;
+  float* vs = T.exp_avg_sq_scale + m * nb + first;
+  const int run = ts.tile_blocks / ADAMW8_WARPS;
+  const uint4 counter = make_uint4((uint32_t)(first * (ADAMW8_BLOCK / 4)), T.id, s.member_base + m,
+                                   (uint32_t)(T.step ? T.step[m] : s.step));
   const bool vec = (inner & 3) == 0 &&
                    ((reinterpret_cast<uintptr_t>(T.p) | reinterpret_cast<uintptr_t>(T.grad)) & 15u) == 0 &&
                    ((reinterpret_cast<uintptr_t>(T.exp_avg) | reinterpret_cast<uintptr_t>(T.exp_avg_sq)) & 3u) == 0;
   if (vec)
-    adamw8_tile<true>(c, a, first, last, inner, counter, s.ks, words[warp_id()]);
+    adamw8_tile<true>(c, a, ms, vs, run, blocks, left, counter, s.ks, stages[warp_id()]);
   else
-    adamw8_tile<false>(c, a, first, last, inner, counter, s.ks, words[warp_id()]);
+    adamw8_tile<false>(c, a, ms, vs, run, blocks, left, counter, s.ks, stages[warp_id()]);
 }
 
 struct AdamW8Moments {

@@ -47,13 +47,6 @@ constexpr int LP_CHUNK = 2048;       // classes of one warp in the streaming bac
 
 __device__ __forceinline__ float lp_nan() { return __uint_as_float(0x7FC00000u); }
 
-// max(a, b), NaN if either is.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // exp(x) for x <= 0 from the base-2 exponential (2^-22 relative, and x's rounding times |x|).
 __device__ __forceinline__ float exp_neg(float x) {
   float r;

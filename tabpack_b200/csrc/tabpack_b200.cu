@@ -1573,11 +1573,11 @@ int tp_adamw_step(const tp_adamw_args* a, void* stream) {
 }
 
 // Tiles of a launch over several packs: tensor i's members have member_tiles[i] tiles of tile_blocks
-// state blocks each.  64 blocks a tile (8 a warp, which carry the tile's fixed cost), fewer
-// where that would leave SMs idle: at least two waves of 4 CTAs per SM, down to one block a warp.
+// state blocks each.  128 blocks a tile (16 a warp, which carry the tile's fixed cost), fewer
+// where that would leave SMs idle: at least four waves of 4 CTAs per SM, down to one block a warp.
 static int adamw8_tiles(int n, const int64_t* numel, const int64_t* inner, uint32_t* tile0, uint32_t* member_tiles,
                         int* tile_blocks) {
-  for (int tb = 64;; tb /= 2) {
+  for (int tb = 128;; tb /= 2) {
     int64_t total = 0;
     for (int i = 0; i < n; ++i) {
       if (numel[i] <= 0 || inner[i] <= 0 || inner[i] > (1ll << 33) || numel[i] % inner[i] != 0)
@@ -1593,7 +1593,7 @@ static int adamw8_tiles(int n, const int64_t* numel, const int64_t* inner, uint3
     }
     tile0[n] = (uint32_t)total;
     *tile_blocks = tb;
-    if (tb == ADAMW8_WARPS || total >= 2 * 4 * 148) return TP_OK;
+    if (tb == ADAMW8_WARPS || total >= 4 * 4 * 148) return TP_OK;
   }
 }
 
