@@ -543,6 +543,11 @@ typedef struct tp_adamw8_args {
 } tp_adamw8_args;
 int tp_adamw8_step(const tp_adamw8_args* a, void* stream);
 
+/* Test hook: the square root of the 8-bit AdamW step against CUDA's correctly rounded one over the
+ * fp32 numbers with the bit patterns first .. first + count - 1; adds to *differ (device) twice the
+ * count of those that differ. */
+int tp_root_check(uint32_t first, uint32_t count, unsigned long long* differ, void* stream);
+
 /* The moments that a state of tp_adamw8_step stands for, exp_avg and exp_avg_sq (the root
  * squared), in fp32 or bf16. */
 typedef struct tp_opt8_values {

@@ -246,6 +246,7 @@ SIGNATURES = {
                                          ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
                                          ctypes.c_void_p]),
     'tp_adamw8_step': (ctypes.c_int, [ctypes.POINTER(AdamW8Args), ctypes.c_void_p]),
+    'tp_root_check': (ctypes.c_int, [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p]),
     'tp_adamw8_moments': (ctypes.c_int, [ctypes.POINTER(AdamW8MomentsArgs), ctypes.c_void_p]),
     'tp_layer_norm_workspace_size': (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
     'tp_layer_norm_forward': (ctypes.c_int, [ctypes.POINTER(LayerNormArgs), ctypes.c_void_p]),

@@ -31,7 +31,7 @@ namespace tp {
 
 constexpr int ADAMW8_BLOCK = 128;        // elements per scale: one warp, four consecutive elements a lane
 constexpr int ADAMW8_WARPS = 8;
-constexpr int ADAMW8_STAGES = 3;         // blocks of a warp on the way or in use
+constexpr int ADAMW8_STAGES = 4;         // blocks of a warp on the way or in use, a power of two
 constexpr int ADAMW8_STAGE = 32 * 40;    // bytes: p, g (16 a lane), both codes (4 a lane)
 constexpr float ADAMW8_TINY = 7.8886090522101181e-31f;  // 2^-100: a block below it is stored as zeros
 
@@ -74,13 +74,48 @@ __device__ __forceinline__ AdamW8Member adamw8_member(const AdamW8Scalars& s, in
   c.b2 = s.beta2 ? s.beta2[m] : s.beta2_s;
   c.one_m_b1 = s.beta1 ? __fsub_rn(1.0f, c.b1) : s.one_m_b1_s;
   c.one_m_b2 = s.beta2 ? __fsub_rn(1.0f, c.b2) : s.one_m_b2_s;
-  c.eps = s.eps ? s.eps[m] : s.eps_s;
+  c.eps = fmaxf(s.eps ? s.eps[m] : s.eps_s, 1.17549435e-38f);  // the denominator's reciprocal stays finite
   c.mult = (s.lr || s.wd) ? 1.0f - lr * (s.wd ? s.wd[m] : s.wd_s) : s.wd_mult_s;
   const float t = (float)(steps ? steps[m] : s.step);
   const float bc1 = (s.beta1 || steps) ? bias_correction(c.one_m_b1, t) : s.bc1_s;
   c.step_size = (s.lr || s.beta1 || steps) ? lr / bc1 : s.step_size_s;
   c.inv_sqrt_bc2 = (s.beta2 || steps) ? rsqrtf(bias_correction(c.one_m_b2, t)) : s.inv_sqrt_bc2_s;
   return c;
+}
+
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Correctly rounded square roots of two numbers from 2^-94 up (others: something within an ulp, or
+// NaN for 0, infinities and NaN).  Goldschmidt's iteration on s ~ sqrt(v) and h ~ 1 / (2 sqrt(v)) from
+// the approximate reciprocal root, then Markstein's correction s + h (v - s^2) with the residual exact in
+// a fused multiply-add (P. Markstein, IA-64 and Elementary Functions, 2000).  In pairs it takes half
+// the instructions of two calls; tp_root_check compares it with CUDA's over every mantissa.
+__device__ __forceinline__ f32x2 sqrt2(f32x2 v) {
+  const float2 f = halves(v);
+  float r0, r1;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(f.x));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(f.y));
+  const f32x2 r = pair(r0, r1), half = pair(0.5f, 0.5f), minus = pair(-1.0f, -1.0f);
+  f32x2 s = mul2(v, r), h = mul2(r, half);
+  const f32x2 e = fma2(mul2(s, minus), h, half);
+  s = fma2(s, e, s);
+  h = fma2(h, e, h);
+  return fma2(fma2(mul2(s, minus), s, v), h, s);
+}
+
+__global__ void root_check_kernel(uint32_t first, uint32_t count, unsigned long long* differ) {
+  unsigned long long n = 0;
+  for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < count; i += gridDim.x * blockDim.x) {
+    const float v = __uint_as_float(first + i);
+    const float2 s = halves(sqrt2(pair(v, v)));
+    n += __float_as_uint(s.x) != __float_as_uint(__fsqrt_rn(v));
+    n += __float_as_uint(s.y) != __float_as_uint(__fsqrt_rn(v));
+  }
+  if (n) atomicAdd(differ, n);
 }
 
 // Four e4m3 codes -> their values times `scale`, as pairs.
@@ -106,11 +141,12 @@ __device__ __forceinline__ void adamw8_load_root(uint32_t c, f32x2 scale, f32x2 
   u[1] = mul2(pair(v[2], v[3]), scale);
 }
 
-// e4m3 code of |x| / scale = y for any y, rounded with the 16 random bits r.
-__device__ __forceinline__ uint32_t adamw8_code_first(float y, uint32_t r) {
-  const uint32_t normal = ((__float_as_uint(y) + (r << 4)) >> 20) - (120u << 3);
-  const uint32_t small = (uint32_t)__fadd_rn(__fmul_rn(y, 512.0f), __fmul_rn((float)r, 1.0f / 65536.0f));
-  return y >= 0.015625f ? normal : small;
+// Subnormal e4m3 codes, y < 2^-6: floor(512 y + r / 2^16), left in the number's low byte by adding
+// 2^23 towards minus infinity.  `r8`: the 16 random bits r times 2^8; half of it is the fraction of
+// 1 + r / 2^16.
+__device__ __forceinline__ uint32_t adamw8_small_first(float y, uint32_t r8) {
+  const float r = __fsub_rn(__uint_as_float(0x3F800000u | r8 >> 1), 1.0f);
+  return __float_as_uint(__fadd_rd(__fmaf_rn(y, 512.0f, r), 8388608.0f));
 }
 
 // e4m4 code of u / scale = y.
@@ -127,6 +163,33 @@ __device__ __forceinline__ uint32_t bytes4(uint32_t a, uint32_t b, uint32_t c, u
 __device__ __forceinline__ uint32_t top4(const uint32_t (&w)[4]) {
   return __byte_perm(__byte_perm(w[0], w[1], 0x0073), __byte_perm(w[2], w[3], 0x0073), 0x5410);
 }
+
+// Philox4x32-10 over the first counter word with the other three fixed: the products of the first
+// round's third word and the second round's first do not depend on it.
+struct PhiloxGroup {
+  uint32_t a, b, y, w;  // w ^ key of the first round; second round: lo ^ key, hi ^ key, lo
+  const uint32_t* ks;
+  __device__ PhiloxGroup(uint32_t c1, uint32_t c2, uint32_t c3, const uint32_t* keys) : ks(keys) {
+    const uint64_t p1 = (uint64_t)0xCD9E8D57u * c2;
+    a = c3 ^ ks[1];
+    y = (uint32_t)p1 ^ ks[2];
+    const uint64_t p0 = (uint64_t)0xD2511F53u * ((uint32_t)(p1 >> 32) ^ c1 ^ ks[0]);
+    b = (uint32_t)(p0 >> 32) ^ ks[3];
+    w = (uint32_t)p0;
+  }
+  __device__ uint4 at(uint32_t c0) const {
+    const uint64_t p0 = (uint64_t)0xD2511F53u * c0;
+    const uint64_t p1 = (uint64_t)0xCD9E8D57u * ((uint32_t)(p0 >> 32) ^ a);
+    uint4 c = make_uint4((uint32_t)(p1 >> 32) ^ y, (uint32_t)p1, (uint32_t)p0 ^ b, w);
+#pragma unroll
+    for (int i = 2; i < 10; ++i) {
+      const uint64_t q0 = (uint64_t)0xD2511F53u * c.x, q1 = (uint64_t)0xCD9E8D57u * c.z;
+      c = make_uint4((uint32_t)(q1 >> 32) ^ c.y ^ ks[2 * i], (uint32_t)q1, (uint32_t)(q0 >> 32) ^ c.w ^ ks[2 * i + 1],
+                     (uint32_t)q0);
+    }
+    return c;
+  }
+};
 
 // One lane's share of a block.
 struct AdamW8Lane {
@@ -160,12 +223,18 @@ struct AdamW8Ptr {
 // copied); `left`: elements of the member from that block's first on.
 __device__ __forceinline__ void adamw8_issue(uint32_t stage, const AdamW8Ptr& a, int ahead, int left, int lane) {
   const int o = ahead * ADAMW8_BLOCK;
-  const bool in = 4 * lane < left;
-  if (left > 0) {
-    cp_async16(stage + 16 * lane, in ? a.p + o : a.p, in);
-    cp_async16(stage + 512 + 16 * lane, in ? a.g + o : a.g, in);
-    cp_async4(stage + 1024 + 4 * lane, in ? a.m + o : a.m, in);
-    cp_async4(stage + 1152 + 4 * lane, in ? a.v + o : a.v, in);
+  const uint32_t s16 = stage + 16 * lane, s4 = stage + 1024 + 4 * lane;
+  if (left >= ADAMW8_BLOCK) {
+    cp_async16(s16, a.p + o, true);
+    cp_async16(s16 + 512, a.g + o, true);
+    cp_async4(s4, a.m + o, true);
+    cp_async4(s4 + 128, a.v + o, true);
+  } else if (left > 0) {
+    const bool in = 4 * lane < left;
+    cp_async16(s16, in ? a.p + o : a.p, in);
+    cp_async16(s16 + 512, in ? a.g + o : a.g, in);
+    cp_async4(s4, in ? a.m + o : a.m, in);
+    cp_async4(s4 + 128, in ? a.v + o : a.v, in);
   }
   cp_async_commit();
 }
@@ -199,11 +268,12 @@ __device__ __forceinline__ void adamw8_fetch(AdamW8Lane& x, const AdamW8Ptr& a, 
 // One block; returns its new scales.
 template <bool VEC>
 __device__ __forceinline__ float2 adamw8_block(const AdamW8Lane& x, const AdamW8Member& c, const AdamW8Ptr& a, int left,
-                                             int lane, uint4 counter, const uint32_t* ks, uint32_t* words) {
+                                             int lane, const PhiloxGroup& philox, uint32_t group, uint32_t* words) {
   f32x2 m[2], u[2];
   adamw8_load_first(x.m, pair(x.ms, x.ms), m);
   adamw8_load_root(x.v, pair(x.vs, x.vs), u);
   float mm[4], uu[4], p[4];
+  f32x2 v[2];
   const f32x2 b1 = pair(c.b1, c.b1), o1 = pair(c.one_m_b1, c.one_m_b1), b2 = pair(c.b2, c.b2),
               o2 = pair(c.one_m_b2, c.one_m_b2);
 #pragma unroll
@@ -213,27 +283,42 @@ __device__ __forceinline__ float2 adamw8_block(const AdamW8Lane& x, const AdamW8
     const float2 ma = halves(mul2(m[h], b1)), mb = halves(mul2(g, o1));
     const float2 va = halves(mul2(mul2(u[h], u[h]), b2)), vb = halves(mul2(mul2(g, g), o2));
     mm[2 * h] = __fadd_rn(ma.x, mb.x), mm[2 * h + 1] = __fadd_rn(ma.y, mb.y);
-    uu[2 * h] = __fsqrt_rn(__fadd_rn(va.x, vb.x)), uu[2 * h + 1] = __fsqrt_rn(__fadd_rn(va.y, vb.y));
     m[h] = pair(mm[2 * h], mm[2 * h + 1]);
-    // p (1 - lr wd) - step m / (u / sqrt(bc2) + eps)
-    u[h] = pair(uu[2 * h], uu[2 * h + 1]);
+    v[h] = pair(__fadd_rn(va.x, vb.x), __fadd_rn(va.y, vb.y));
+    u[h] = sqrt2(v[h]);
+    const float2 uf = halves(u[h]);
+    uu[2 * h] = uf.x, uu[2 * h + 1] = uf.y;
+  }
+  // the block's largest magnitudes (as integers: a NaN is above everything) and the smallest root
+  float umin = fminf(fminf(uu[0], uu[1]), fminf(uu[2], uu[3]));
+  float umax = max_nan(max_nan(uu[0], uu[1]), max_nan(uu[2], uu[3]));
+  if (__any_sync(0xFFFFFFFFu, !(umin >= 7.1e-15f && umax < INFINITY))) {
+    // outside sqrt2's range (2^-94 up): zeros, next to zeros, infinities, NaN
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float2 vf = halves(v[h]);
+      uu[2 * h] = __fsqrt_rn(vf.x), uu[2 * h + 1] = __fsqrt_rn(vf.y);
+      u[h] = pair(uu[2 * h], uu[2 * h + 1]);
+    }
+    if (left < ADAMW8_BLOCK) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (adamw8_at<VEC>(lane, j) >= left) mm[j] = uu[j] = 0.0f;
+    }
+    umin = fminf(fminf(uu[0], uu[1]), fminf(uu[2], uu[3]));
+    umax = max_nan(max_nan(uu[0], uu[1]), max_nan(uu[2], uu[3]));
+  }
+  uint32_t mbig = __float_as_uint(max_nan(max_nan(fabsf(mm[0]), fabsf(mm[1])), max_nan(fabsf(mm[2]), fabsf(mm[3]))));
+  mbig = __reduce_max_sync(0xFFFFFFFFu, mbig);
+  const uint32_t ubig = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(umax));
+  // p (1 - lr wd) - step m / (u / sqrt(bc2) + eps)
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
     const float2 den = halves(fma2(u[h], pair(c.inv_sqrt_bc2, c.inv_sqrt_bc2), pair(c.eps, c.eps)));
-    const f32x2 r = pair(__fdividef(1.0f, den.x), __fdividef(1.0f, den.y));
-    const f32x2 up = mul2(mul2(m[h], pair(-c.step_size, -c.step_size)), r);
+    const f32x2 up = mul2(mul2(m[h], pair(-c.step_size, -c.step_size)), pair(reciprocal(den.x), reciprocal(den.y)));
     const float2 pf = halves(fma2(pair(x.p[2 * h], x.p[2 * h + 1]), pair(c.mult, c.mult), up));
     p[2 * h] = pf.x, p[2 * h + 1] = pf.y;
   }
-  const bool whole = left >= ADAMW8_BLOCK;
-  if (!whole) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (adamw8_at<VEC>(lane, j) >= left) mm[j] = uu[j] = 0.0f;
-  }
-  // the block's largest magnitudes (as integers: a NaN is above everything)
-  uint32_t mbig = __float_as_uint(max_nan(max_nan(fabsf(mm[0]), fabsf(mm[1])), max_nan(fabsf(mm[2]), fabsf(mm[3]))));
-  uint32_t ubig = __float_as_uint(max_nan(max_nan(uu[0], uu[1]), max_nan(uu[2], uu[3])));
-  mbig = __reduce_max_sync(0xFFFFFFFFu, mbig);
-  ubig = __reduce_max_sync(0xFFFFFFFFu, ubig);
   // even lanes form the first moment's scale, odd ones the root's
   float scale = 0.0f, inv = 0.0f;
   {
@@ -246,7 +331,7 @@ __device__ __forceinline__ float2 adamw8_block(const AdamW8Lane& x, const AdamW8
     }
   }
   const float minv = __shfl_sync(0xFFFFFFFFu, inv, 0), vinv = __shfl_sync(0xFFFFFFFFu, inv, 1);
-  const uint4 rnd = philox4x32_10_ks(counter, ks);
+  const uint4 rnd = philox.at(group);
   uint32_t rw[4] = {rnd.x, rnd.y, rnd.z, rnd.w};
   if (!VEC) {  // the words of elements 4 l .. 4 l + 3 to the lanes that hold those elements
     reinterpret_cast<uint4*>(words)[lane] = rnd;
@@ -274,11 +359,16 @@ __device__ __forceinline__ float2 adamw8_block(const AdamW8Lane& x, const AdamW8
   }
   uint32_t mo = (top4(mc) & 0x7F7F7F7Fu) ^ 0x40404040u, vo = top4(vc);
   const bool msmall = !(fminf(fminf(ym[0], ym[1]), fminf(ym[2], ym[3])) >= 0.015625f);  // 2^-6
-  const bool usmall = !(fminf(fminf(yu[0], yu[1]), fminf(yu[2], yu[3])) >= 3.2424927e-05f);  // 2^-15 (1 + 1 / 16)
+  const bool usmall = !(__fmul_rn(umin, vinv) >= 3.2424927e-05f);                       // 2^-15 (1 + 1 / 16)
   if (__any_sync(0xFFFFFFFFu, msmall)) {
+    uint32_t pick = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) mc[j] = minv > 0.0f ? adamw8_code_first(ym[j], rw[j] & 0xFFFFu) : 0u;
-    mo = bytes4(mc[0], mc[1], mc[2], mc[3]);
+    for (int j = 0; j < 4; ++j) {
+      mc[j] = adamw8_small_first(ym[j], __byte_perm(rw[j], 0, 0x4104));
+      if (!(ym[j] >= 0.015625f)) pick |= 0xFFu << (8 * j);
+    }
+    mo = (mo & ~pick) | (bytes4(mc[0], mc[1], mc[2], mc[3]) & pick);
+    if (!(minv > 0.0f)) mo = 0;
   }
   if (__any_sync(0xFFFFFFFFu, usmall)) {
 #pragma unroll
@@ -314,7 +404,7 @@ __device__ __forceinline__ float2 adamw8_block(const AdamW8Lane& x, const AdamW8
 // 850 us against 511 us for the same traffic without them, 209 M elements.)
 template <bool VEC>
 __device__ __forceinline__ void adamw8_tile(const AdamW8Member& c, AdamW8Ptr a, float* ms, float* vs, int run, int blocks,
-                                            int left, uint4 counter, const uint32_t* ks, char* stages) {
+                                            int left, const PhiloxGroup& philox, uint32_t group, char* stages) {
   const int lane = lane_id(), first = warp_id() * run, at = first * ADAMW8_BLOCK + (VEC ? 4 * lane : lane);
   const int n = min(run, blocks - first);
   if (n <= 0) return;
@@ -323,7 +413,7 @@ __device__ __forceinline__ void adamw8_tile(const AdamW8Member& c, AdamW8Ptr a, 
   a.m += at;
   a.v += at;
   left -= first * ADAMW8_BLOCK;
-  counter.x += first * (ADAMW8_BLOCK / 4) + lane;
+  group += first * (ADAMW8_BLOCK / 4) + lane;
   float sm = 0.0f, sv = 0.0f;
   if (lane < n) sm = ms[first + lane], sv = vs[first + lane];
   const uint32_t base = smem_u32(stages);
@@ -335,27 +425,25 @@ __device__ __forceinline__ void adamw8_tile(const AdamW8Member& c, AdamW8Ptr a, 
   } else {
     adamw8_fetch<0>(next, a, left, lane);
   }
-  int slot = 0;
   for (int i = 0; i < n; ++i) {
     AdamW8Lane x;
     if constexpr (VEC) {
       cp_async_wait<ADAMW8_STAGES - 2>();
-      adamw8_take(x, stages + slot * ADAMW8_STAGE, lane);
-      const int into = slot == 0 ? ADAMW8_STAGES - 1 : slot - 1;  // the block before: read, and free
-      constexpr int ahead = ADAMW8_STAGES - 1;
-      adamw8_issue(base + into * ADAMW8_STAGE, a, ahead, i + ahead < n ? left - ahead * ADAMW8_BLOCK : 0, lane);
-      slot = slot + 1 == ADAMW8_STAGES ? 0 : slot + 1;
+      adamw8_take(x, stages + i % ADAMW8_STAGES * ADAMW8_STAGE, lane);
+      constexpr int ahead = ADAMW8_STAGES - 1;  // into the stage of the block before: read, and free
+      adamw8_issue(base + (i + ahead) % ADAMW8_STAGES * ADAMW8_STAGE, a, ahead,
+                   i + ahead < n ? left - ahead * ADAMW8_BLOCK : 0, lane);
     } else {
       x = next;
       if (i + 1 < n) adamw8_fetch<1>(next, a, left - ADAMW8_BLOCK, lane);
     }
     x.ms = __shfl_sync(0xFFFFFFFFu, sm, i);
     x.vs = __shfl_sync(0xFFFFFFFFu, sv, i);
-    const float2 scale = adamw8_block<VEC>(x, c, a, left, lane, counter, ks, reinterpret_cast<uint32_t*>(stages));
+    const float2 scale = adamw8_block<VEC>(x, c, a, left, lane, philox, group, reinterpret_cast<uint32_t*>(stages));
     if (lane == i) sm = scale.x, sv = scale.y;
     a.next();
     left -= ADAMW8_BLOCK;
-    counter.x += ADAMW8_BLOCK / 4;
+    group += ADAMW8_BLOCK / 4;
   }
   if (lane < n) ms[first + lane] = sm, vs[first + lane] = sv;
 }
@@ -388,15 +476,15 @@ __global__ void __launch_bounds__(32 * ADAMW8_WARPS, 4) adamw8_kernel(const __gr
   float* ms = T.exp_avg_scale + m * nb + first;
   float* vs = T.exp_avg_sq_scale + m * nb + first;
   const int run = ts.tile_blocks / ADAMW8_WARPS;
-  const uint4 counter = make_uint4((uint32_t)(first * (ADAMW8_BLOCK / 4)), T.id, s.member_base + m,
-                                   (uint32_t)(T.step ? T.step[m] : s.step));
+  const PhiloxGroup philox(T.id, s.member_base + m, (uint32_t)(T.step ? T.step[m] : s.step), s.ks);
+  const uint32_t group = (uint32_t)(first * (ADAMW8_BLOCK / 4));
   const bool vec = (inner & 3) == 0 &&
                    ((reinterpret_cast<uintptr_t>(T.p) | reinterpret_cast<uintptr_t>(T.grad)) & 15u) == 0 &&
                    ((reinterpret_cast<uintptr_t>(T.exp_avg) | reinterpret_cast<uintptr_t>(T.exp_avg_sq)) & 3u) == 0;
   if (vec)
-    adamw8_tile<true>(c, a, ms, vs, run, blocks, left, counter, s.ks, stages[warp_id()]);
+    adamw8_tile<true>(c, a, ms, vs, run, blocks, left, philox, group, stages[warp_id()]);
   else
-    adamw8_tile<false>(c, a, ms, vs, run, blocks, left, counter, s.ks, stages[warp_id()]);
+    adamw8_tile<false>(c, a, ms, vs, run, blocks, left, philox, group, stages[warp_id()]);
 }
 
 struct AdamW8Moments {
@@ -428,46 +516,62 @@ __global__ void __launch_bounds__(32 * ADAMW8_WARPS) adamw8_moments_kernel(const
   const bool vec = (inner & 3) == 0 &&
                    ((reinterpret_cast<uintptr_t>(A.exp_avg) | reinterpret_cast<uintptr_t>(A.exp_avg_sq)) & 3u) == 0 &&
                    ((reinterpret_cast<uintptr_t>(A.m) | reinterpret_cast<uintptr_t>(A.v)) & (4 * sizeof(T) - 1)) == 0;
-#pragma unroll 2
-  for (int64_t b = first + warp_id(); b < last; b += ADAMW8_WARPS) {
-    const int64_t e = b * ADAMW8_BLOCK;
-    const int left = (int)min((int64_t)ADAMW8_BLOCK, inner - e), lane = lane_id();
-    uint32_t cm = 0, cv = 0;
-    if (vec) {
-      if (4 * lane < left) {
-        cm = __ldg(reinterpret_cast<const uint32_t*>(mc + e) + lane);
-        cv = __ldg(reinterpret_cast<const uint32_t*>(vc + e) + lane);
-      }
-    } else {
+  // a run of blocks per warp, lane i with the scales of its i-th; four blocks' codes loaded ahead of use
+  const int run = ts.tile_blocks / ADAMW8_WARPS, lane = lane_id();
+  const int64_t b0 = first + warp_id() * run;
+  const int n = (int)min((int64_t)run, last - b0);
+  float sm = 0.0f, sv = 0.0f;
+  if (lane < n) sm = ms[b0 + lane], sv = vs[b0 + lane];
+  for (int i0 = 0; i0 < n; i0 += 4) {
+    uint32_t cm[4], cv[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (lane + 32 * j < left) {
-          cm |= (uint32_t)mc[e + lane + 32 * j] << (8 * j);
-          cv |= (uint32_t)vc[e + lane + 32 * j] << (8 * j);
+    for (int k = 0; k < 4; ++k) {
+      cm[k] = cv[k] = 0;
+      if (i0 + k >= n) continue;
+      const int64_t e = (b0 + i0 + k) * ADAMW8_BLOCK;
+      const int left = (int)min((int64_t)ADAMW8_BLOCK, inner - e);
+      if (vec) {
+        if (4 * lane < left) {
+          cm[k] = __ldcs(reinterpret_cast<const uint32_t*>(mc + e) + lane);
+          cv[k] = __ldcs(reinterpret_cast<const uint32_t*>(vc + e) + lane);
         }
-    }
-    const float sm = ms[b], sv = vs[b];
-    f32x2 x[2], u[2];
-    adamw8_load_first(cm, pair(sm, sm), x);
-    adamw8_load_root(cv, pair(sv, sv), u);
-    const float2 x0 = halves(x[0]), x1 = halves(x[1]), u0 = halves(mul2(u[0], u[0])), u1 = halves(mul2(u[1], u[1]));
-    if (vec) {
-      if (4 * lane >= left) continue;
-      if constexpr (sizeof(T) == 2) {
-        reinterpret_cast<uint2*>(mo + e)[lane] = make_uint2(pack_bf16x2(x0.x, x0.y), pack_bf16x2(x1.x, x1.y));
-        reinterpret_cast<uint2*>(vo + e)[lane] = make_uint2(pack_bf16x2(u0.x, u0.y), pack_bf16x2(u1.x, u1.y));
       } else {
-        reinterpret_cast<float4*>(mo + e)[lane] = make_float4(x0.x, x0.y, x1.x, x1.y);
-        reinterpret_cast<float4*>(vo + e)[lane] = make_float4(u0.x, u0.y, u1.x, u1.y);
-      }
-    } else {
-      const float xs[4] = {x0.x, x0.y, x1.x, x1.y}, us[4] = {u0.x, u0.y, u1.x, u1.y};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (lane + 32 * j < left) {
-          mo[e + lane + 32 * j] = from_f32<T>(xs[j]);
-          vo[e + lane + 32 * j] = from_f32<T>(us[j]);
+        for (int j = 0; j < 4; ++j)
+          if (lane + 32 * j < left) {
+            cm[k] |= (uint32_t)mc[e + lane + 32 * j] << (8 * j);
+            cv[k] |= (uint32_t)vc[e + lane + 32 * j] << (8 * j);
+          }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (i0 + k >= n) break;
+      const int64_t e = (b0 + i0 + k) * ADAMW8_BLOCK;
+      const int left = (int)min((int64_t)ADAMW8_BLOCK, inner - e);
+      const float bm = __shfl_sync(0xFFFFFFFFu, sm, i0 + k), bv = __shfl_sync(0xFFFFFFFFu, sv, i0 + k);
+      f32x2 x[2], u[2];
+      adamw8_load_first(cm[k], pair(bm, bm), x);
+      adamw8_load_root(cv[k], pair(bv, bv), u);
+      const float2 x0 = halves(x[0]), x1 = halves(x[1]), u0 = halves(mul2(u[0], u[0])), u1 = halves(mul2(u[1], u[1]));
+      if (vec) {
+        if (4 * lane >= left) continue;
+        if constexpr (sizeof(T) == 2) {
+          reinterpret_cast<uint2*>(mo + e)[lane] = make_uint2(pack_bf16x2(x0.x, x0.y), pack_bf16x2(x1.x, x1.y));
+          reinterpret_cast<uint2*>(vo + e)[lane] = make_uint2(pack_bf16x2(u0.x, u0.y), pack_bf16x2(u1.x, u1.y));
+        } else {
+          reinterpret_cast<float4*>(mo + e)[lane] = make_float4(x0.x, x0.y, x1.x, x1.y);
+          reinterpret_cast<float4*>(vo + e)[lane] = make_float4(u0.x, u0.y, u1.x, u1.y);
         }
+      } else {
+        const float xs[4] = {x0.x, x0.y, x1.x, x1.y}, us[4] = {u0.x, u0.y, u1.x, u1.y};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (lane + 32 * j < left) {
+            mo[e + lane + 32 * j] = from_f32<T>(xs[j]);
+            vo[e + lane + 32 * j] = from_f32<T>(us[j]);
+          }
+      }
     }
   }
 }

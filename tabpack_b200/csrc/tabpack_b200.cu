@@ -1574,7 +1574,7 @@ int tp_adamw_step(const tp_adamw_args* a, void* stream) {
 
 // Tiles of a launch over several packs: tensor i's members have member_tiles[i] tiles of tile_blocks
 // state blocks each.  128 blocks a tile (16 a warp, which carry the tile's fixed cost), fewer
-// where that would leave SMs idle: at least four waves of 4 CTAs per SM, down to one block a warp.
+// where that would leave SMs idle: at least a wave of 4 CTAs per SM, down to one block a warp.
 static int adamw8_tiles(int n, const int64_t* numel, const int64_t* inner, uint32_t* tile0, uint32_t* member_tiles,
                         int* tile_blocks) {
   for (int tb = 128;; tb /= 2) {
@@ -1593,7 +1593,7 @@ static int adamw8_tiles(int n, const int64_t* numel, const int64_t* inner, uint3
     }
     tile0[n] = (uint32_t)total;
     *tile_blocks = tb;
-    if (tb == ADAMW8_WARPS || total >= 4 * 4 * 148) return TP_OK;
+    if (tb == ADAMW8_WARPS || total >= 4 * 148) return TP_OK;
   }
 }
 
@@ -1647,6 +1647,13 @@ int tp_adamw8_step(const tp_adamw8_args* a, void* stream) {
   philox_key_schedule((uint32_t)a->seed, (uint32_t)(a->seed >> 32), s.ks);
   s.member_base = a->member_base;
   adamw8_kernel<<<ts.tile0[ts.n], 32 * ADAMW8_WARPS, 0, static_cast<cudaStream_t>(stream)>>>(ts, s);
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+int tp_root_check(uint32_t first, uint32_t count, unsigned long long* differ, void* stream) {
+  if (!differ || count == 0) return fail(TP_EINVAL, "bad root check arguments");
+  root_check_kernel<<<1184, 256, 0, static_cast<cudaStream_t>(stream)>>>(first, count, differ);
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;
 }

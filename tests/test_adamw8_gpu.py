@@ -327,6 +327,19 @@ def test_refusals():
     assert torch.equal(p[0], before)
 
 
+def test_square_root_is_correctly_rounded():
+    """Every mantissa at an even and an odd exponent (the iteration is the same in every binade), and all
+    numbers at both ends of the range, against CUDA's square root bit for bit."""
+    from tabpack_b200 import _lib
+
+    differ = torch.zeros(1, dtype=torch.int64, device='cuda')
+    stream = torch.cuda.current_stream().cuda_stream
+    binade = 1 << 23
+    for exponent in (33, 34, 126, 127, 200, 252, 253):  # 2^-94, 2^-93, 1/2, 1, 2^73, 2^125, 2^126
+        _lib.check(_lib.load().tp_root_check(exponent * binade, binade, differ.data_ptr(), stream), 'tp_root_check')
+    assert differ.item() == 0
+
+
 # ------------------------------------------------------------------ the optimizer packs
 
 
