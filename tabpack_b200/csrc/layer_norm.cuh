@@ -8,8 +8,9 @@
 // instructions.  Rows of up to NORM_HELD columns stay in the registers of a group of G lanes (8 to
 // 512, 16 elements each), so x and dy are read once and the variance is summed around the mean.
 // A group walks over rows of one member: the member's w and b, and in the backward the columns' sums,
-// stay in registers, and the next row is on its way while the current one is reduced.  Wider rows
-// take the plain kernels at the end.
+// stay in registers, while the next rows are on their way to shared memory (asynchronous copies, 3
+// rows ahead in bf16: one row ahead in registers left the memory waiting, 383 us instead of 190 for
+// the forward of 16384 rows of 8192).  Wider rows take the plain kernels at the end.
 #pragma once
 
 #include "gemm_simt.cuh"
@@ -43,43 +44,32 @@ __device__ __forceinline__ int norm_width(const LayerNormArgs& a, int m) {
   return a.n ? min(max(a.n[m], 0), a.W) : a.W;
 }
 
-// V neighbouring elements in their own type: 16 bytes, or one element where nothing is aligned.
+// V neighbouring elements: 16 bytes, or one element where nothing is aligned.
 template <typename T, int V>
-struct NormVec {
-  uint4 u;
-  __device__ void load(const T* p) { u = *reinterpret_cast<const uint4*>(p); }
-  __device__ void zero() { u = make_uint4(0, 0, 0, 0); }
-  __device__ void get(float (&f)[V]) const {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ void norm_unpack(const uint4& u, float* f) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (sizeof(T) == 2) {
-        f[2 * e] = __uint_as_float(w[e] << 16);
-        f[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
-      } else {
-        f[e] = __uint_as_float(w[e]);
-      }
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (sizeof(T) == 2) {
+      f[2 * e] = __uint_as_float(w[e] << 16);
+      f[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
+    } else {
+      f[e] = __uint_as_float(w[e]);
     }
   }
-  __device__ static void store(T* p, const float (&f)[V]) {
-    uint4 w;
-    if constexpr (sizeof(T) == 2)
-      w = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                     pack_bf16x2(f[6], f[7]));
-    else
-      w = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-    *reinterpret_cast<uint4*>(p) = w;
-  }
-};
+}
 
-template <typename T>
-struct NormVec<T, 1> {
-  T u;
-  __device__ void load(const T* p) { u = *p; }
-  __device__ void zero() { u = from_f32<T>(0.f); }
-  __device__ void get(float (&f)[1]) const { f[0] = to_f32<T>(u); }
-  __device__ static void store(T* p, const float (&f)[1]) { *p = from_f32<T>(f[0]); }
-};
+template <typename T, int V>
+__device__ __forceinline__ void norm_store(T* p, const float* f) {
+  if constexpr (V == 1) {
+    *p = from_f32<T>(f[0]);
+  } else if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                                              pack_bf16x2(f[6], f[7]));
+  } else {
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+  }
+}
 
 // A group of G lanes of a block and its sums.
 template <int G>
@@ -91,54 +81,80 @@ struct NormGroup {
   __device__ NormGroup(float2* shared) : lane(threadIdx.x % G), group(threadIdx.x / G) {
     red = shared + group * 2 * WARPS;
   }
-  // Sums of u and v over the group, in every lane.
+  template <int PAIRS>  // 1: only u
   __device__ float2 sum(float u, float v) {
 #pragma unroll
     for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) {
       u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
-      v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+      if (PAIRS == 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
     }
     if constexpr (G > 32) {
       float2* r = red + half * WARPS;
       half ^= 1;
       if (lane % 32 == 0) r[lane / 32] = make_float2(u, v);
       asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(G) : "memory");
-      u = v = 0.f;
+      const float2 t = r[lane % WARPS];
+      u = t.x, v = t.y;
 #pragma unroll
-      for (int i = 0; i < WARPS; ++i) {
-        u += r[i].x;
-        v += r[i].y;
+      for (int o = WARPS / 2; o > 0; o >>= 1) {
+        u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
+        if (PAIRS == 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
       }
     }
     return make_float2(u, v);
   }
 };
 
-// A row's elements c0(k) .. c0(k) + V - 1 of one lane, k < E / V, as far as they are below n.
+// Rows of one operand on their way to a lane: its share of a row, K vectors c0(k) .. c0(k) + V - 1,
+// is copied to the lane's own part of a ring in shared memory (no barrier: a lane reads only what it
+// copied), with zeros from column n on; unaligned rows go through registers, one row ahead.
 template <typename T, int V, int G>
-struct NormRow {
-  static constexpr int K = NORM_E / V;
-  NormVec<T, V> raw[K];
+struct NormRows {
+  static constexpr int K = NORM_E / V, THREADS = NormGroup<G>::THREADS;
+  static constexpr int STAGE = V > 1 ? K * THREADS * 16 : 0;  // bytes of one row of every group
+  const T* row0;
+  int64_t stride;
+  int lane, n, last;
+  uint32_t ring;
+  const char* ring_ptr;
+  T next[V > 1 ? 1 : NORM_E];
   __device__ static int c0(int k, int lane) { return (k * G + lane) * V; }
-  __device__ void load(const T* row, int lane, int n) {
+  __device__ NormRows(const T* r0, int64_t stride_, int lane_, int n_, int last_, char* shared)
+      : row0(r0), stride(stride_), lane(lane_), n(n_), last(last_), ring(smem_u32(shared) + threadIdx.x * 16),
+        ring_ptr(shared + threadIdx.x * 16) {}
+  // Row r (the last one, where there is none) into stage `slot`.
+  __device__ void issue(int r, int slot) {
+    const T* row = row0 + min(r, last) * stride;
+    if constexpr (V > 1) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (c0(k, lane) < n)
-        raw[k].load(row + c0(k, lane));
-      else
-        raw[k].zero();
+      for (int k = 0; k < K; ++k) {
+        const int c = c0(k, lane), bytes = min(max((n - c) * (int)sizeof(T), 0), 16);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ring + slot * STAGE + k * THREADS * 16),
+                     "l"(bytes > 0 ? row + c : row), "r"(bytes)
+                     : "memory");
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) next[k] = c0(k, lane) < n ? row[c0(k, lane)] : from_f32<T>(0.f);
     }
   }
-  __device__ void get(float (&f)[NORM_E]) const {
+  __device__ void take(int slot, float (&f)[NORM_E]) const {
+    if constexpr (V > 1) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      float v[V];
-      raw[k].get(v);
+      for (int k = 0; k < K; ++k)
+        norm_unpack<T, V>(*reinterpret_cast<const uint4*>(ring_ptr + slot * STAGE + k * THREADS * 16), f + k * V);
+    } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) f[k * V + e] = v[e];
+      for (int k = 0; k < K; ++k) f[k] = to_f32<T>(next[k]);
     }
   }
 };
+
+// Vector k of a lane is whole for every lane of the group (no element at or beyond n).
+template <int V, int G>
+__device__ __forceinline__ bool norm_whole(int k, int n) {
+  return (k + 1) * G * V <= n;
+}
 
 // Lane's columns of a (W,) fp32 parameter, `other` where there is none.
 template <int V, int G>
@@ -165,52 +181,80 @@ __device__ __forceinline__ void norm_param(const float* p, int lane, int n, floa
   }
 }
 
+// Rows in flight per operand, the current one included.
+template <typename T, int V>
+struct NormDepth {
+  static constexpr int FORWARD = V == 1 ? 1 : sizeof(T) == 2 ? 4 : 3;
+  static constexpr int BACKWARD = V == 1 ? 1 : sizeof(T) == 2 ? 4 : 2;
+};
+
 template <typename T, int V, int G>
-__global__ void __launch_bounds__(NormGroup<G>::THREADS) layer_norm_held_forward_kernel(const LayerNormArgs a) {
+__global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS > 256 ? 1 : 3)
+    layer_norm_held_forward_kernel(const LayerNormArgs a) {
   using Grp = NormGroup<G>;
+  using Rows = NormRows<T, V, G>;
+  constexpr int D = NormDepth<T, V>::FORWARD, AHEAD = V == 1 ? 1 : D - 1;
   __shared__ float2 red[Grp::GROUPS * 2 * Grp::WARPS];
+  extern __shared__ __align__(16) char ring[];
   Grp grp(red);
   const int m = blockIdx.x / a.S, split = blockIdx.x % a.S;
   const int n = norm_width(a, m), lane = grp.lane, step = a.S * Grp::GROUPS;
   const float inv_n = 1.0f / (float)max(n, 1);
-  const T* x = static_cast<const T*>(a.x) + m * a.xm;
-  float w[NORM_E], b[NORM_E];
-  norm_param<V, G>(a.w ? a.w + (size_t)m * a.W : nullptr, lane, n, 1.f, w);
-  norm_param<V, G>(a.b ? a.b + (size_t)m * a.W : nullptr, lane, n, 0.f, b);
   // groups of one warp step together (their sums are warp-wide shuffles): rows beyond the last
   // are computed again from the last and not written
   const int first = split * Grp::GROUPS + grp.group;
   const int rounds = (a.B - split * Grp::GROUPS + step - 1) / step;
-  NormRow<T, V, G> next;
-  next.load(x + min(first, a.B - 1) * a.xr, lane, n);
+  Rows x(static_cast<const T*>(a.x) + m * a.xm, a.xr, lane, n, a.B - 1, ring);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) {
+    x.issue(first + i * step, i);
+    if (V > 1) cp_async_commit();
+  }
+  float w[NORM_E], b[NORM_E];
+  norm_param<V, G>(a.w ? a.w + (size_t)m * a.W : nullptr, lane, n, 1.f, w);
+  norm_param<V, G>(a.b ? a.b + (size_t)m * a.W : nullptr, lane, n, 0.f, b);
   for (int i = 0; i < rounds; ++i) {
     const int r = first + i * step;
     float f[NORM_E];
-    next.get(f);
-    if (i + 1 < rounds) next.load(x + min(r + step, a.B - 1) * a.xr, lane, n);
+    if (V > 1) cp_async_wait<(D > 1 ? D - 2 : 0)>();
+    x.take(i % D, f);
+    if (V > 1 || i + 1 < rounds) {
+      if (i + AHEAD < rounds) x.issue(r + AHEAD * step, (i + AHEAD) % D);
+      if (V > 1) cp_async_commit();
+    }
     float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < NORM_E; ++j) {
-      if (NormRow<T, V, G>::c0(j / V, lane) + j % V >= n) f[j] = 0.f;
-      s += f[j];
-    }
-    const float mean = grp.sum(s, 0.f).x * inv_n;
+    for (int j = 0; j < NORM_E; ++j) s += f[j];
+    const float mean = grp.template sum<1>(s, 0.f).x * inv_n;
     s = 0.f;
 #pragma unroll
-    for (int j = 0; j < NORM_E; ++j) {
-      f[j] = NormRow<T, V, G>::c0(j / V, lane) + j % V < n ? f[j] - mean : 0.f;
-      s += f[j] * f[j];
+    for (int k = 0; k < NORM_E / V; ++k) {
+      const int c = Rows::c0(k, lane);
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[k * V + e] -= mean;
+      if (!norm_whole<V, G>(k, n)) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (c + e >= n) f[k * V + e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += f[k * V + e] * f[k * V + e];
     }
-    const float rstd = 1.0f / sqrtf(grp.sum(s, 0.f).x * inv_n + a.eps);
+    const float rstd = rsqrtf(grp.template sum<1>(s, 0.f).x * inv_n + a.eps);
     if (r >= a.B) continue;
     T* y = static_cast<T*>(a.y) + ((int64_t)m * a.B + r) * a.W;
 #pragma unroll
     for (int k = 0; k < NORM_E / V; ++k) {
-      const int c = NormRow<T, V, G>::c0(k, lane);
+      const int c = Rows::c0(k, lane);
       float v[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = c + e < n ? f[k * V + e] * rstd * w[k * V + e] + b[k * V + e] : 0.f;
-      if (c < a.W) NormVec<T, V>::store(y + c, v);
+      for (int e = 0; e < V; ++e) v[e] = f[k * V + e] * rstd * w[k * V + e] + b[k * V + e];
+      if (!norm_whole<V, G>(k, n)) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (c + e >= n) v[e] = 0.f;
+      }
+      if (c < a.W) norm_store<T, V>(y + c, v);
     }
     if (lane == 0) {
       a.mean[(int64_t)m * a.B + r] = mean;
@@ -224,46 +268,57 @@ template <typename T, int V, int G>
 __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS > 256 ? 1 : 2)
     layer_norm_held_backward_kernel(const LayerNormArgs a) {
   using Grp = NormGroup<G>;
+  using Rows = NormRows<T, V, G>;
+  constexpr int D = NormDepth<T, V>::BACKWARD, AHEAD = V == 1 ? 1 : D - 1;
   __shared__ float2 red[Grp::GROUPS * 2 * Grp::WARPS];
-  __shared__ __align__(16) float cols[Grp::GROUPS > 1 ? Grp::THREADS * NORM_E : 1];
+  extern __shared__ __align__(16) char ring[];  // x, then dy; at the end the groups' column sums
   Grp grp(red);
   const int m = blockIdx.x / a.S, split = blockIdx.x % a.S;
   const int n = norm_width(a, m), lane = grp.lane, step = a.S * Grp::GROUPS;
   const float inv_n = 1.0f / (float)max(n, 1);
-  const T* x = static_cast<const T*>(a.x) + m * a.xm;
-  const T* dy = static_cast<const T*>(a.dy) + m * a.dym;
+  const int first = split * Grp::GROUPS + grp.group;
+  const int rounds = (a.B - split * Grp::GROUPS + step - 1) / step;
+  Rows x(static_cast<const T*>(a.x) + m * a.xm, a.xr, lane, n, a.B - 1, ring);
+  Rows dy(static_cast<const T*>(a.dy) + m * a.dym, a.dyr, lane, n, a.B - 1, ring + D * Rows::STAGE);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) {
+    x.issue(first + i * step, i);
+    dy.issue(first + i * step, i);
+    if (V > 1) cp_async_commit();
+  }
   const float* mean = a.mean + (int64_t)m * a.B;
   const float* rstd = a.rstd + (int64_t)m * a.B;
+  float nmean = mean[min(first, a.B - 1)], nrstd = rstd[min(first, a.B - 1)];
   float w[NORM_E], sw[NORM_E], sb[NORM_E];
   norm_param<V, G>(a.w ? a.w + (size_t)m * a.W : nullptr, lane, n, 1.f, w);
 #pragma unroll
   for (int j = 0; j < NORM_E; ++j) sw[j] = sb[j] = 0.f;
-  const int first = split * Grp::GROUPS + grp.group;
-  const int rounds = (a.B - split * Grp::GROUPS + step - 1) / step;
-  NormRow<T, V, G> nx, ndy;
-  float nmean = 0.f, nrstd = 0.f;
-  const auto fetch = [&](int r) {
-    r = min(r, a.B - 1);
-    nx.load(x + r * a.xr, lane, n);
-    ndy.load(dy + r * a.dyr, lane, n);
-    nmean = mean[r];
-    nrstd = rstd[r];
-  };
-  fetch(first);
   for (int i = 0; i < rounds; ++i) {
     const int r = first + i * step;
     float h[NORM_E], g[NORM_E];
-    nx.get(h);
-    ndy.get(g);
+    if (V > 1) cp_async_wait<(D > 1 ? D - 2 : 0)>();
+    x.take(i % D, h);
+    dy.take(i % D, g);
     const float mu = nmean, rs = nrstd;
-    if (i + 1 < rounds) fetch(r + step);
+    if (i + 1 < rounds) {
+      const int to = min(r + step, a.B - 1);
+      nmean = mean[to];
+      nrstd = rstd[to];
+    }
+    if (i + AHEAD < rounds) {
+      x.issue(r + AHEAD * step, (i + AHEAD) % D);
+      dy.issue(r + AHEAD * step, (i + AHEAD) % D);
+    }
+    if (V > 1) cp_async_commit();
     const bool live = r < a.B;
+    if (!live) {
+#pragma unroll
+      for (int j = 0; j < NORM_E; ++j) g[j] = 0.f;
+    }
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int j = 0; j < NORM_E; ++j) {
-      const bool in = live && NormRow<T, V, G>::c0(j / V, lane) + j % V < n;
-      h[j] = in ? (h[j] - mu) * rs : 0.f;
-      g[j] = in ? g[j] : 0.f;
+    for (int j = 0; j < NORM_E; ++j) {  // dy is 0 from column n on
+      h[j] = (h[j] - mu) * rs;
       sw[j] += g[j] * h[j];
       sb[j] += g[j];
       g[j] *= w[j];
@@ -271,29 +326,32 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
       s2 += g[j] * h[j];
     }
     if (a.dx == nullptr) continue;
-    const float2 t = grp.sum(s1, s2);
+    const float2 t = grp.template sum<2>(s1, s2);
     if (!live) continue;
     const float c1 = t.x * inv_n, c2 = t.y * inv_n;
     const int64_t at = ((int64_t)m * a.B + r) * a.W;
 #pragma unroll
     for (int k = 0; k < NORM_E / V; ++k) {
-      const int c = NormRow<T, V, G>::c0(k, lane);
+      const int c = Rows::c0(k, lane);
       float v[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        v[e] = c + e < n ? rs * (g[k * V + e] - c1 - h[k * V + e] * c2) : 0.f;
+      for (int e = 0; e < V; ++e) v[e] = rs * (g[k * V + e] - c1 - h[k * V + e] * c2);
+      if (!norm_whole<V, G>(k, n)) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (c + e >= n) v[e] = 0.f;
+      }
       if (c >= a.W) continue;
       if (sizeof(T) == 2 && a.dx_f32) {
         float* d = static_cast<float*>(a.dx) + at + c;
         if constexpr (V >= 4) {
 #pragma unroll
-          for (int e = 0; e < V; e += 4)
-            *reinterpret_cast<float4*>(d + e) = make_float4(v[e], v[(e + 1) % V], v[(e + 2) % V], v[(e + 3) % V]);
+          for (int e = 0; e < V; e += 4) norm_store<float, 4>(d + e, v + e);
         } else {
           d[0] = v[0];
         }
       } else {
-        NormVec<T, V>::store(static_cast<T*>(a.dx) + at + c, v);
+        norm_store<T, V>(static_cast<T*>(a.dx) + at + c, v);
       }
     }
   }
@@ -307,10 +365,12 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
     const float(&s)[NORM_E] = which ? sb : sw;
     float* o = which ? ob : ow;
     if constexpr (Grp::GROUPS > 1) {
+      float* cols = reinterpret_cast<float*>(ring);  // a group's columns in a row
+      if (V > 1) cp_async_wait<0>();
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < NORM_E; ++j)
-        cols[grp.group * G * NORM_E + NormRow<T, V, G>::c0(j / V, lane) + j % V] = s[j];
+        cols[grp.group * G * NORM_E + Rows::c0(j / V, lane) + j % V] = Rows::c0(j / V, lane) + j % V < n ? s[j] : 0.f;
       __syncthreads();
       for (int c = threadIdx.x; c < min(G * NORM_E, a.W); c += Grp::THREADS) {
         float t = 0.f;
@@ -321,8 +381,8 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
     } else {
 #pragma unroll
       for (int j = 0; j < NORM_E; ++j) {
-        const int c = NormRow<T, V, G>::c0(j / V, lane) + j % V;
-        if (o && c < a.W) o[c] = s[j];
+        const int c = Rows::c0(j / V, lane) + j % V;
+        if (o && c < a.W) o[c] = c < n ? s[j] : 0.f;
       }
     }
   }

@@ -1755,18 +1755,40 @@ int norm_splits(int P, int B, int W, int slots) {
 // Blocks of the backward that run at once: 128 registers a thread.
 int norm_backward_splits(int P, int B, int W) { return norm_splits(P, B, W, norm_lanes(W) > 256 ? 148 : 296); }
 
+// Shared memory above 48 KB (static and dynamic) has to be asked for, once per kernel and device.
+template <auto* KERNEL>
+int allow_shared(size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  TP_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (bytes <= 40 * 1024 || (dev < 64 && (done.load(std::memory_order_relaxed) & bit))) return TP_OK;
+  TP_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return TP_OK;
+}
+
 template <typename T, int V, int G>
-void launch_norm(LayerNormArgs k, bool backward, cudaStream_t st) {
+int launch_norm(LayerNormArgs k, bool backward, cudaStream_t st) {
+  using Grp = NormGroup<G>;
   const unsigned blocks = (unsigned)k.P * k.S;
-  if (backward)
-    layer_norm_held_backward_kernel<T, V, G><<<blocks, NormGroup<G>::THREADS, 0, st>>>(k);
-  else
-    layer_norm_held_forward_kernel<T, V, G><<<blocks, NormGroup<G>::THREADS, 0, st>>>(k);
+  constexpr size_t stage = NormRows<T, V, G>::STAGE;
+  if (backward) {
+    constexpr size_t cols = Grp::GROUPS > 1 ? Grp::THREADS * NORM_E * sizeof(float) : 0;
+    constexpr size_t bytes = std::max<size_t>(2 * NormDepth<T, V>::BACKWARD * stage, cols);
+    if (int rc = allow_shared<layer_norm_held_backward_kernel<T, V, G>>(bytes)) return rc;
+    layer_norm_held_backward_kernel<T, V, G><<<blocks, Grp::THREADS, bytes, st>>>(k);
+  } else {
+    constexpr size_t bytes = NormDepth<T, V>::FORWARD * stage;
+    if (int rc = allow_shared<layer_norm_held_forward_kernel<T, V, G>>(bytes)) return rc;
+    layer_norm_held_forward_kernel<T, V, G><<<blocks, Grp::THREADS, bytes, st>>>(k);
+  }
+  return TP_OK;
 }
 
 // The vector form needs every row of every operand on a 16-byte boundary.
 template <typename T>
-void launch_norm_held(const LayerNormArgs& k, bool backward, cudaStream_t st) {
+int launch_norm_held(const LayerNormArgs& k, bool backward, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   bool vec = k.W % V == 0 && k.W % 4 == 0 && aligned16(k.x) && k.xm % V == 0 && k.xr % V == 0 && aligned16(k.w) &&
              aligned16(k.b);
@@ -1775,13 +1797,9 @@ void launch_norm_held(const LayerNormArgs& k, bool backward, cudaStream_t st) {
   else
     vec = vec && aligned16(k.y);
   if (!vec) {
-    if (k.W <= 32 * NORM_E)
-      launch_norm<T, 1, 32>(k, backward, st);
-    else if (k.W <= 128 * NORM_E)
-      launch_norm<T, 1, 128>(k, backward, st);
-    else
-      launch_norm<T, 1, 512>(k, backward, st);
-    return;
+    if (k.W <= 32 * NORM_E) return launch_norm<T, 1, 32>(k, backward, st);
+    if (k.W <= 128 * NORM_E) return launch_norm<T, 1, 128>(k, backward, st);
+    return launch_norm<T, 1, 512>(k, backward, st);
   }
   switch (norm_lanes(k.W)) {
     case 8: return launch_norm<T, V, 8>(k, backward, st);
@@ -1824,11 +1842,9 @@ int tp_layer_norm_forward(const tp_layer_norm_args* a, void* stream) {
     else
       layer_norm_forward_kernel<float><<<(unsigned)k.P * k.B, 256, 0, st>>>(k);
   } else {
-    k.S = norm_splits(k.P, k.B, k.W, norm_lanes(k.W) > 256 ? 296 : 592);
-    if (bf16)
-      launch_norm_held<__nv_bfloat16>(k, false, st);
-    else
-      launch_norm_held<float>(k, false, st);
+    k.S = norm_splits(k.P, k.B, k.W, norm_lanes(k.W) > 256 ? 148 : 444);
+    rc = bf16 ? launch_norm_held<__nv_bfloat16>(k, false, st) : launch_norm_held<float>(k, false, st);
+    if (rc) return rc;
   }
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;
@@ -1860,10 +1876,9 @@ int tp_layer_norm_backward(const tp_layer_norm_args* a, void* stream) {
       launch_norm_wide_backward<__nv_bfloat16>(k, st);
     else
       launch_norm_wide_backward<float>(k, st);
-  } else if (bf16) {
-    launch_norm_held<__nv_bfloat16>(k, true, st);
   } else {
-    launch_norm_held<float>(k, true, st);
+    rc = bf16 ? launch_norm_held<__nv_bfloat16>(k, true, st) : launch_norm_held<float>(k, true, st);
+    if (rc) return rc;
   }
   if (params && k.S > 1) {
     const int col_blocks = (k.W + 31) / 32;
