@@ -8,9 +8,12 @@
 // instructions.  Rows of up to NORM_HELD columns stay in the registers of a group of G lanes (8 to
 // 512, 16 elements each), so x and dy are read once and the variance is summed around the mean.
 // A group walks over rows of one member: the member's w and b, and in the backward the columns' sums,
-// stay in registers, while the next rows are on their way to shared memory (asynchronous copies, 3
-// rows ahead in bf16: one row ahead in registers left the memory waiting, 383 us instead of 190 for
-// the forward of 16384 rows of 8192).  Wider rows take the plain kernels at the end.
+// stay in registers, while the next rows are on their way to shared memory (asynchronous copies: one
+// row ahead in registers left the memory waiting, 192 us instead of 114 for the forward of 16384 rows
+// of 8192 in bf16).  The forward takes two rows at a time, which share each reduction's latency.
+// Arithmetic is in pairs (f32x2).  Ragged rows need no tests per element: the copies fill x and dy with
+// zeros from column n on, and a factor of 0 there takes the mean (and the mean gradient) off
+// nothing.  Wider rows take the plain kernels at the end.
 #pragma once
 
 #include "gemm_simt.cuh"
@@ -45,17 +48,18 @@ __device__ __forceinline__ int norm_width(const LayerNormArgs& a, int m) {
 }
 
 // V neighbouring elements: 16 bytes, or one element where nothing is aligned.
+constexpr int NORM_H = NORM_E / 2;  // pairs
+
+// Vector k's pairs.
 template <typename T, int V>
-__device__ __forceinline__ void norm_unpack(const uint4& u, float* f) {
+__device__ __forceinline__ void norm_unpack(const uint4& u, f32x2* f) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if constexpr (sizeof(T) == 2) {
-      f[2 * e] = __uint_as_float(w[e] << 16);
-      f[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
-    } else {
-      f[e] = __uint_as_float(w[e]);
-    }
+    for (int e = 0; e < 4; ++e) f[e] = pair(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xFFFF0000u));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) f[e] = pair(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
   }
 }
 
@@ -138,58 +142,107 @@ struct NormRows {
       for (int k = 0; k < K; ++k) next[k] = c0(k, lane) < n ? row[c0(k, lane)] : from_f32<T>(0.f);
     }
   }
-  __device__ void take(int slot, float (&f)[NORM_E]) const {
+  __device__ void take(int slot, f32x2 (&f)[NORM_H]) const {
     if constexpr (V > 1) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        norm_unpack<T, V>(*reinterpret_cast<const uint4*>(ring_ptr + slot * STAGE + k * THREADS * 16), f + k * V);
+        norm_unpack<T, V>(*reinterpret_cast<const uint4*>(ring_ptr + slot * STAGE + k * THREADS * 16), f + k * V / 2);
     } else {
 #pragma unroll
-      for (int k = 0; k < K; ++k) f[k] = to_f32<T>(next[k]);
+      for (int k = 0; k < NORM_H; ++k) f[k] = pair(to_f32<T>(next[2 * k]), to_f32<T>(next[2 * k + 1]));
     }
   }
 };
 
-// Vector k of a lane is whole for every lane of the group (no element at or beyond n).
+// 1 for the lane's columns below n, 0 for the others.
 template <int V, int G>
-__device__ __forceinline__ bool norm_whole(int k, int n) {
-  return (k + 1) * G * V <= n;
+__device__ __forceinline__ void norm_mask(int lane, int n, f32x2 (&f)[NORM_H]) {
+#pragma unroll
+  for (int h = 0; h < NORM_H; ++h) {
+    const int c = (2 * h / V * G + lane) * V + 2 * h % V, d = V == 1 ? c + G : c + 1;
+    f[h] = pair(c < n ? 1.f : 0.f, d < n ? 1.f : 0.f);
+  }
 }
 
-// Lane's columns of a (W,) fp32 parameter, `other` where there is none.
-template <int V, int G>
-__device__ __forceinline__ void norm_param(const float* p, int lane, int n, float other, float (&f)[NORM_E]) {
+__device__ __forceinline__ float norm_add(const f32x2 (&f)[NORM_H]) {
+  f32x2 s = f[0];
+#pragma unroll
+  for (int h = 1; h < NORM_H; ++h) s = add2(s, f[h]);
+  const float2 t = halves(s);
+  return t.x + t.y;
+}
+
+// Writes a lane's share of a row; `odd`: a row with a NaN, whose padding is not zero by itself.
+template <typename T, int V, int G>
+__device__ __forceinline__ void norm_write(T* row, const f32x2 (&f)[NORM_H], int lane, int n, int W, bool odd) {
 #pragma unroll
   for (int k = 0; k < NORM_E / V; ++k) {
     const int c = (k * G + lane) * V;
-    if (V >= 4 && p && c < n) {
-#pragma unroll
-      for (int e = 0; e < V; e += 4) {
-        const float4 q = __ldg(reinterpret_cast<const float4*>(p + c + e));
-        f[k * V + e] = q.x;
-        f[k * V + (e + 1) % V] = q.y;
-        f[k * V + (e + 2) % V] = q.z;
-        f[k * V + (e + 3) % V] = q.w;
-      }
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (c + e >= n) f[k * V + e] = other;  // the padding may hold anything
+    float v[V];
+    if constexpr (V == 1) {
+      const float2 t = halves(f[k / 2]);
+      v[0] = k % 2 ? t.y : t.x;
     } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) f[k * V + e] = p && c + e < n ? __ldg(p + c + e) : other;
+      for (int e = 0; e < V; e += 2) {
+        const float2 t = halves(f[(k * V + e) / 2]);
+        v[e] = t.x, v[e + 1] = t.y;
+      }
+    }
+    if (odd) {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (c + e >= n) v[e] = 0.f;
+    }
+    if (c < W) {
+      if constexpr (V == 8 && sizeof(T) == 4) {
+        norm_store<float, 4>(row + c, v);
+        norm_store<float, 4>(row + c + 4, v + 4);
+      } else {
+        norm_store<T, V>(row + c, v);
+      }
     }
   }
 }
 
-// Rows in flight per operand, the current one included.
+// Lane's columns of a (W,) fp32 parameter, `other` where there is none and from column n on (the
+// padding may hold anything).
+template <int V, int G>
+__device__ __forceinline__ void norm_param(const float* p, int lane, int n, float other, f32x2 (&f)[NORM_H]) {
+  float v[NORM_E];
+#pragma unroll
+  for (int k = 0; k < NORM_E / V; ++k) {
+    const int c = (k * G + lane) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[k * V + e] = other;
+    if (V >= 4 && p && c + V <= n) {
+#pragma unroll
+      for (int e = 0; e < V; e += 4) {
+        const float4 q = __ldg(reinterpret_cast<const float4*>(p + c + e));
+        v[k * V + e] = q.x;
+        v[k * V + (e + 1) % V] = q.y;
+        v[k * V + (e + 2) % V] = q.z;
+        v[k * V + (e + 3) % V] = q.w;
+      }
+    } else if (p) {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (c + e < n) v[k * V + e] = __ldg(p + c + e);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < NORM_H; ++h) f[h] = pair(v[2 * h], v[2 * h + 1]);
+}
+
+// Stages of the ring, the current one included: two rows each forward, one backward.
 template <typename T, int V>
 struct NormDepth {
-  static constexpr int FORWARD = V == 1 ? 1 : sizeof(T) == 2 ? 4 : 3;
+  static constexpr int FORWARD = V == 1 ? 1 : sizeof(T) == 2 ? 3 : 2;
   static constexpr int BACKWARD = V == 1 ? 1 : sizeof(T) == 2 ? 4 : 2;
 };
 
 template <typename T, int V, int G>
-__global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS > 256 ? 1 : 3)
+__global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS > 256 ? 1 : 2)
     layer_norm_held_forward_kernel(const LayerNormArgs a) {
   using Grp = NormGroup<G>;
   using Rows = NormRows<T, V, G>;
@@ -203,62 +256,60 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
   // groups of one warp step together (their sums are warp-wide shuffles): rows beyond the last
   // are computed again from the last and not written
   const int first = split * Grp::GROUPS + grp.group;
-  const int rounds = (a.B - split * Grp::GROUPS + step - 1) / step;
-  Rows x(static_cast<const T*>(a.x) + m * a.xm, a.xr, lane, n, a.B - 1, ring);
+  const int rounds = (a.B - split * Grp::GROUPS + 2 * step - 1) / (2 * step);
+  const T* x0 = static_cast<const T*>(a.x) + m * a.xm;
+  Rows xa(x0, a.xr, lane, n, a.B - 1, ring), xb(x0, a.xr, lane, n, a.B - 1, ring + D * Rows::STAGE);
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) {
-    x.issue(first + i * step, i);
+    xa.issue(first + 2 * i * step, i);
+    xb.issue(first + (2 * i + 1) * step, i);
     if (V > 1) cp_async_commit();
   }
-  float w[NORM_E], b[NORM_E];
+  f32x2 w[NORM_H], b[NORM_H], mask[NORM_H];
   norm_param<V, G>(a.w ? a.w + (size_t)m * a.W : nullptr, lane, n, 1.f, w);
   norm_param<V, G>(a.b ? a.b + (size_t)m * a.W : nullptr, lane, n, 0.f, b);
+  norm_mask<V, G>(lane, n, mask);
   for (int i = 0; i < rounds; ++i) {
-    const int r = first + i * step;
-    float f[NORM_E];
+    const int r = first + 2 * i * step;
+    f32x2 f[2][NORM_H];
     if (V > 1) cp_async_wait<(D > 1 ? D - 2 : 0)>();
-    x.take(i % D, f);
-    if (V > 1 || i + 1 < rounds) {
-      if (i + AHEAD < rounds) x.issue(r + AHEAD * step, (i + AHEAD) % D);
-      if (V > 1) cp_async_commit();
+    xa.take(i % D, f[0]);
+    xb.take(i % D, f[1]);
+    if (i + AHEAD < rounds) {
+      xa.issue(r + 2 * AHEAD * step, (i + AHEAD) % D);
+      xb.issue(r + (2 * AHEAD + 1) * step, (i + AHEAD) % D);
     }
-    float s = 0.f;
+    if (V > 1) cp_async_commit();
+    const float2 sum = grp.template sum<2>(norm_add(f[0]), norm_add(f[1]));
+    const float mean[2] = {sum.x * inv_n, sum.y * inv_n};
+    float sq[2];
 #pragma unroll
-    for (int j = 0; j < NORM_E; ++j) s += f[j];
-    const float mean = grp.template sum<1>(s, 0.f).x * inv_n;
-    s = 0.f;
+    for (int q = 0; q < 2; ++q) {
+      const f32x2 minus = pair(-mean[q], -mean[q]);
+      f32x2 s = pair(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < NORM_E / V; ++k) {
-      const int c = Rows::c0(k, lane);
-#pragma unroll
-      for (int e = 0; e < V; ++e) f[k * V + e] -= mean;
-      if (!norm_whole<V, G>(k, n)) {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (c + e >= n) f[k * V + e] = 0.f;
+      for (int h = 0; h < NORM_H; ++h) {
+        f[q][h] = fma2(mask[h], minus, f[q][h]);
+        s = fma2(f[q][h], f[q][h], s);
       }
-#pragma unroll
-      for (int e = 0; e < V; ++e) s += f[k * V + e] * f[k * V + e];
+      const float2 t = halves(s);
+      sq[q] = t.x + t.y;
     }
-    const float rstd = rsqrtf(grp.template sum<1>(s, 0.f).x * inv_n + a.eps);
-    if (r >= a.B) continue;
-    T* y = static_cast<T*>(a.y) + ((int64_t)m * a.B + r) * a.W;
+    const float2 var = grp.template sum<2>(sq[0], sq[1]);
 #pragma unroll
-    for (int k = 0; k < NORM_E / V; ++k) {
-      const int c = Rows::c0(k, lane);
-      float v[V];
+    for (int q = 0; q < 2; ++q) {
+      const int row = r + q * step;
+      if (row >= a.B) continue;
+      const float rstd = rsqrtf((q ? var.y : var.x) * inv_n + a.eps);
+      const f32x2 rs = pair(rstd, rstd);
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = f[k * V + e] * rstd * w[k * V + e] + b[k * V + e];
-      if (!norm_whole<V, G>(k, n)) {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (c + e >= n) v[e] = 0.f;
+      for (int h = 0; h < NORM_H; ++h) f[q][h] = fma2(mul2(f[q][h], rs), w[h], b[h]);
+      const int64_t at = (int64_t)m * a.B + row;
+      norm_write<T, V, G>(static_cast<T*>(a.y) + at * a.W, f[q], lane, n, a.W, !(rstd < INFINITY));
+      if (lane == 0) {
+        a.mean[at] = mean[q];
+        a.rstd[at] = rstd;
       }
-      if (c < a.W) norm_store<T, V>(y + c, v);
-    }
-    if (lane == 0) {
-      a.mean[(int64_t)m * a.B + r] = mean;
-      a.rstd[(int64_t)m * a.B + r] = rstd;
     }
   }
 }
@@ -289,15 +340,16 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
   const float* mean = a.mean + (int64_t)m * a.B;
   const float* rstd = a.rstd + (int64_t)m * a.B;
   float nmean = mean[min(first, a.B - 1)], nrstd = rstd[min(first, a.B - 1)];
-  float w[NORM_E], sw[NORM_E], sb[NORM_E];
+  f32x2 w[NORM_H], sw[NORM_H], sb[NORM_H], mask[NORM_H];
   norm_param<V, G>(a.w ? a.w + (size_t)m * a.W : nullptr, lane, n, 1.f, w);
+  norm_mask<V, G>(lane, n, mask);
 #pragma unroll
-  for (int j = 0; j < NORM_E; ++j) sw[j] = sb[j] = 0.f;
+  for (int h = 0; h < NORM_H; ++h) sw[h] = sb[h] = pair(0.f, 0.f);
   for (int i = 0; i < rounds; ++i) {
     const int r = first + i * step;
-    float h[NORM_E], g[NORM_E];
+    f32x2 xh[NORM_H], g[NORM_H];
     if (V > 1) cp_async_wait<(D > 1 ? D - 2 : 0)>();
-    x.take(i % D, h);
+    x.take(i % D, xh);
     dy.take(i % D, g);
     const float mu = nmean, rs = nrstd;
     if (i + 1 < rounds) {
@@ -313,47 +365,32 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
     const bool live = r < a.B;
     if (!live) {
 #pragma unroll
-      for (int j = 0; j < NORM_E; ++j) g[j] = 0.f;
+      for (int h = 0; h < NORM_H; ++h) g[h] = pair(0.f, 0.f);
     }
-    float s1 = 0.f, s2 = 0.f;
+    const f32x2 minus = pair(-mu, -mu), scale = pair(rs, rs);
+    f32x2 s1 = pair(0.f, 0.f), s2 = s1;
 #pragma unroll
-    for (int j = 0; j < NORM_E; ++j) {  // dy is 0 from column n on
-      h[j] = (h[j] - mu) * rs;
-      sw[j] += g[j] * h[j];
-      sb[j] += g[j];
-      g[j] *= w[j];
-      s1 += g[j];
-      s2 += g[j] * h[j];
+    for (int h = 0; h < NORM_H; ++h) {  // xhat and dy are 0 from column n on
+      xh[h] = mul2(fma2(mask[h], minus, xh[h]), scale);
+      sw[h] = fma2(g[h], xh[h], sw[h]);
+      sb[h] = add2(sb[h], g[h]);
+      g[h] = mul2(g[h], w[h]);
+      s1 = add2(s1, g[h]);
+      s2 = fma2(g[h], xh[h], s2);
     }
     if (a.dx == nullptr) continue;
-    const float2 t = grp.template sum<2>(s1, s2);
+    const float2 u = halves(s1), v = halves(s2);
+    const float2 t = grp.template sum<2>(u.x + u.y, v.x + v.y);
     if (!live) continue;
-    const float c1 = t.x * inv_n, c2 = t.y * inv_n;
+    const f32x2 c1 = pair(-t.x * inv_n, -t.x * inv_n), c2 = pair(-t.y * inv_n, -t.y * inv_n);
+#pragma unroll
+    for (int h = 0; h < NORM_H; ++h) g[h] = mul2(fma2(xh[h], c2, fma2(mask[h], c1, g[h])), scale);
     const int64_t at = ((int64_t)m * a.B + r) * a.W;
-#pragma unroll
-    for (int k = 0; k < NORM_E / V; ++k) {
-      const int c = Rows::c0(k, lane);
-      float v[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = rs * (g[k * V + e] - c1 - h[k * V + e] * c2);
-      if (!norm_whole<V, G>(k, n)) {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (c + e >= n) v[e] = 0.f;
-      }
-      if (c >= a.W) continue;
-      if (sizeof(T) == 2 && a.dx_f32) {
-        float* d = static_cast<float*>(a.dx) + at + c;
-        if constexpr (V >= 4) {
-#pragma unroll
-          for (int e = 0; e < V; e += 4) norm_store<float, 4>(d + e, v + e);
-        } else {
-          d[0] = v[0];
-        }
-      } else {
-        norm_store<T, V>(static_cast<T*>(a.dx) + at + c, v);
-      }
-    }
+    const bool odd = !(fabsf(t.x) + fabsf(t.y) < INFINITY && rs < INFINITY);
+    if (sizeof(T) == 2 && a.dx_f32)
+      norm_write<float, V, G>(static_cast<float*>(a.dx) + at, g, lane, n, a.W, odd);
+    else
+      norm_write<T, V, G>(static_cast<T*>(a.dx) + at, g, lane, n, a.W, odd);
   }
   if (!a.dw && !a.db) return;
   // the block's groups in ascending order, then (with several splits) the finishing kernel
@@ -362,7 +399,12 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
   float* ob = a.S > 1 ? a.partial + (size_t)a.P * a.S * a.W + row : a.db ? a.db + row : nullptr;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    const float(&s)[NORM_E] = which ? sb : sw;
+    float s[NORM_E];
+#pragma unroll
+    for (int h = 0; h < NORM_H; ++h) {
+      const float2 t = halves(which ? sb[h] : sw[h]);
+      s[2 * h] = t.x, s[2 * h + 1] = t.y;
+    }
     float* o = which ? ob : ow;
     if constexpr (Grp::GROUPS > 1) {
       float* cols = reinterpret_cast<float*>(ring);  // a group's columns in a row
@@ -501,9 +543,10 @@ __global__ void __launch_bounds__(256) layer_norm_dw_kernel(const LayerNormArgs 
   }
 }
 
-// The splits' partial sums: 32 columns a block, eight threads over the splits of each in turn.
-__global__ void __launch_bounds__(256) layer_norm_finish_kernel(const LayerNormArgs a, int col_blocks) {
-  __shared__ float2 part[8][32];
+// The splits' partial sums: 32 columns a block, SLICES threads over the splits of each in turn.
+template <int SLICES>
+__global__ void __launch_bounds__(32 * SLICES) layer_norm_finish_kernel(const LayerNormArgs a, int col_blocks) {
+  __shared__ float2 part[SLICES][32];
   const int m = blockIdx.x / col_blocks, lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int c = (blockIdx.x % col_blocks) * 32 + lane;
   float2 s = make_float2(0.f, 0.f);
@@ -511,7 +554,7 @@ __global__ void __launch_bounds__(256) layer_norm_finish_kernel(const LayerNormA
     const float* p = a.partial + (size_t)m * a.S * a.W + c;
     const size_t second = (size_t)a.P * a.S * a.W;
 #pragma unroll 4
-    for (int i = slice; i < a.S; i += 8) {
+    for (int i = slice; i < a.S; i += SLICES) {
       s.x += p[(size_t)i * a.W];
       s.y += p[second + (size_t)i * a.W];
     }
@@ -520,7 +563,7 @@ __global__ void __launch_bounds__(256) layer_norm_finish_kernel(const LayerNormA
   __syncthreads();
   if (slice != 0 || c >= a.W) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
+  for (int i = 1; i < SLICES; ++i) {
     s.x += part[i][lane].x;
     s.y += part[i][lane].y;
   }

@@ -1779,7 +1779,7 @@ int launch_norm(LayerNormArgs k, bool backward, cudaStream_t st) {
     if (int rc = allow_shared<layer_norm_held_backward_kernel<T, V, G>>(bytes)) return rc;
     layer_norm_held_backward_kernel<T, V, G><<<blocks, Grp::THREADS, bytes, st>>>(k);
   } else {
-    constexpr size_t bytes = NormDepth<T, V>::FORWARD * stage;
+    constexpr size_t bytes = 2 * NormDepth<T, V>::FORWARD * stage;
     if (int rc = allow_shared<layer_norm_held_forward_kernel<T, V, G>>(bytes)) return rc;
     layer_norm_held_forward_kernel<T, V, G><<<blocks, Grp::THREADS, bytes, st>>>(k);
   }
@@ -1842,7 +1842,7 @@ int tp_layer_norm_forward(const tp_layer_norm_args* a, void* stream) {
     else
       layer_norm_forward_kernel<float><<<(unsigned)k.P * k.B, 256, 0, st>>>(k);
   } else {
-    k.S = norm_splits(k.P, k.B, k.W, norm_lanes(k.W) > 256 ? 148 : 444);
+    k.S = norm_splits(k.P, k.B, k.W, norm_lanes(k.W) > 256 ? 148 : 296);
     rc = bf16 ? launch_norm_held<__nv_bfloat16>(k, false, st) : launch_norm_held<float>(k, false, st);
     if (rc) return rc;
   }
@@ -1882,7 +1882,10 @@ int tp_layer_norm_backward(const tp_layer_norm_args* a, void* stream) {
   }
   if (params && k.S > 1) {
     const int col_blocks = (k.W + 31) / 32;
-    layer_norm_finish_kernel<<<(unsigned)k.P * col_blocks, 256, 0, st>>>(k, col_blocks);
+    if (k.S > 32)
+      layer_norm_finish_kernel<32><<<(unsigned)k.P * col_blocks, 1024, 0, st>>>(k, col_blocks);
+    else
+      layer_norm_finish_kernel<8><<<(unsigned)k.P * col_blocks, 256, 0, st>>>(k, col_blocks);
   }
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;

@@ -219,6 +219,24 @@ def test_nonfinite_rows_stay_by_themselves():
     assert torch.equal(y[~bad], clean[~bad])
 
 
+def test_padding_of_nonfinite_rows_is_zero():
+    from tabpack_b200 import ops
+
+    for W, dtype in ((200, torch.bfloat16), (200, torch.float32), (77, torch.float32), (3000, torch.bfloat16),
+                     (9000, torch.bfloat16)):
+        x, dy, w, b, n = make(2, 6, W, dtype, seed=W)
+        n[0], n[1] = W - 5, W // 2
+        x[0, 1, 3], x[1, 2, 0], dy[0, 4, 2] = float('nan'), float('inf'), float('nan')
+        y, mean, rstd = ops.layer_norm_forward(x, w, b, n_features=n)
+        dx, dw, db = ops.layer_norm_backward(dy, x, w, mean, rstd, n_features=n)
+        for m in range(2):
+            k = int(n[m])
+            for t in (y[m], dx[m], dw[m:m + 1], db[m:m + 1]):
+                assert (t[..., k:] == 0).all()
+        assert torch.isnan(y[0, 1, :k]).all() and torch.isnan(dx[0, 4, :k]).all() and torch.isnan(dw[1, :k]).all()
+        assert torch.isfinite(db[1]).all() and torch.isfinite(y[0, 4]).all()
+
+
 def test_widths_outside_the_row_are_clamped():
     """A width of zero leaves zeros; one beyond the row is the row."""
     from tabpack_b200 import ops
