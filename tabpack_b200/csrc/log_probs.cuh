@@ -13,8 +13,13 @@
 // Memory bounds these kernels: 2 or 4 bytes a class against 8 to 12 instructions.  Rows of up
 // to 1024 classes are held in registers by a thread (16), 8 lanes (64) or a warp (256, 1024), so the
 // row is read once and the softmax takes its maximum first; longer rows take one block and one pass
-// with a running maximum.  Rows start anywhere: whole 16-byte vectors are loaded between the
-// first and last boundary inside the row, single elements before and after.
+// with a running maximum, the next 64 bytes of each thread on their way meanwhile.  Rows start anywhere:
+// whole 16-byte vectors are loaded between the first and last boundary inside the row, single elements
+// before and after.
+//
+// The best classes cost little more than a comparison for 32 scores: the k-th largest of the 32 lanes'
+// maxima is a bound that at least k scores reach and few others do; what reaches it goes through
+// shared memory into one sort of 32 keys, and a sorted list of 32 takes the result in.
 #pragma once
 
 #include "gemm_simt.cuh"
@@ -54,6 +59,20 @@ __device__ __forceinline__ float exp_neg(float x) {
   return r;
 }
 
+__device__ __forceinline__ f32x2 exp_neg2(f32x2 x) {
+  const float2 y = halves(mul2(x, pair(1.4426950408889634f, 1.4426950408889634f)));
+  float2 r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(y.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(y.y));
+  return pair(r.x, r.y);
+}
+
+// z - max, bounded below, of two scores.
+__device__ __forceinline__ f32x2 bounded2(f32x2 d) {
+  const float2 t = halves(d);
+  return pair(max_nan(t.x, LP_FAR), max_nan(t.y, LP_FAR));
+}
+
 // Ascending integer order of floats, at least 1: NaN above everything, -0 equal to +0.
 __device__ __forceinline__ uint32_t class_order(float v) {
   uint32_t u = __float_as_uint(v + 0.0f);
@@ -77,19 +96,29 @@ struct Row {
   }
   __device__ int vectors() const { return (phase + C + V - 1) / V; }
   __device__ int first(int i) const { return i * V - phase; }  // class of vector i's first element
-  // Vector i; elements outside the row read as -inf.
-  __device__ void load(int i, float (&v)[V]) const {
+  // Vector i as it is stored; elements outside the row read as -inf.
+  __device__ uint4 raw(int i) const {
     const int c0 = first(i);
-    if (c0 >= 0 && c0 + V <= C) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(base) + i);
-      unpack(u, v);
-    } else {
+    if (c0 >= 0 && c0 + V <= C) return __ldg(reinterpret_cast<const uint4*>(base) + i);
+    uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        v[e] = (c0 + e >= 0 && c0 + e < C) ? to_f32<T>(base[(int64_t)i * V + e]) : -INFINITY;
+    for (int e = 0; e < V; ++e) {
+      const bool in = c0 + e >= 0 && c0 + e < C;
+      const T* p = base + (int64_t)i * V + e;
+      if constexpr (sizeof(T) == 2) {
+        const uint32_t h = in ? *reinterpret_cast<const uint16_t*>(p) : 0xFF80u;
+        w[e / 2] = e % 2 ? w[e / 2] | h << 16 : h;
+      } else {
+        w[e] = in ? *reinterpret_cast<const uint32_t*>(p) : 0xFF800000u;
+      }
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  __device__ static void unpack(const uint4& u, float (&v)[V]) {
+  __device__ static uint4 nothing() {
+    const uint32_t w = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;
+    return make_uint4(w, w, w, w);
+  }
+  __device__ static void unpack(const uint4& u, float* v) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -100,6 +129,23 @@ struct Row {
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(w[e]);
+    }
+  }
+  // Writes vector i of a row that begins at `out` (C elements), by 16 bytes where it can.
+  __device__ void store(T* out, int i, const float (&d)[V]) const {
+    const int c0 = first(i);
+    if (c0 >= 0 && c0 + V <= C && (reinterpret_cast<uintptr_t>(out + c0) & 15u) == 0) {
+      uint4 u;
+      if constexpr (sizeof(T) == 2)
+        u = make_uint4(pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3]), pack_bf16x2(d[4], d[5]),
+                       pack_bf16x2(d[6], d[7]));
+      else
+        u = make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2]), __float_as_uint(d[3]));
+      *reinterpret_cast<uint4*>(out + c0) = u;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (c0 + e >= 0 && c0 + e < C) out[c0 + e] = from_f32<T>(d[e]);
     }
   }
 };
@@ -139,12 +185,11 @@ __device__ __forceinline__ void write_best(const LogProbsArgs& a, int64_t row, i
   a.which[row * a.k + j] = c;
 }
 
-// Gradient of one score, before the label's own term.
+// dz = p (a + b log p) with a = -(g_l + g_H H), b = -g_H, and g_l at the label.
 struct RowGrad {
-  float a, b;  // dz = p (a + b log p): a = -(g_l + g_H H), b = -g_H
-  float gl;    // at the label
-  int y;       // -1: no label's term
-  bool empty;
+  f32x2 m, L, a, b;  // the first two negated
+  float gl;
+  int y;             // -1: no label's term
 };
 
 __device__ __forceinline__ RowGrad row_grad(const LogProbsArgs& a, int64_t row, const RowStats& st) {
@@ -157,20 +202,31 @@ __device__ __forceinline__ RowGrad row_grad(const LogProbsArgs& a, int64_t row, 
     g.gl = 0.f;
   else if (y < 0 || y >= a.C)
     g.gl = lp_nan();
-  else
+  else if (!st.empty())
     g.y = (int)y;
-  g.a = -(g.gl + gh * st.H);
-  g.b = -gh;
-  g.empty = st.empty();
+  const float u = st.empty() ? 0.f : -(g.gl + gh * st.H), m = st.empty() ? 0.f : -st.m;
+  g.a = pair(u, u);
+  g.b = pair(-gh, -gh);
+  g.m = pair(m, m);  // a row without classes: every p is 0
+  g.L = pair(-st.L, -st.L);
   return g;
 }
 
-__device__ __forceinline__ float score_grad(const RowGrad& g, const RowStats& st, float z, int c) {
-  // a masked class: p = 0 and a finite log p, so that its product is 0
-  const float lp = max_nan(z - st.m - st.L, LP_FAR);
-  float d = exp_neg(lp) * (g.a + g.b * lp);
-  if (c == g.y) d += g.gl;
-  return g.empty ? 0.f : d;
+// In place, V scores from class c0 on.
+template <int V>
+__device__ __forceinline__ void score_grad(const RowGrad& g, float (&z)[V], int c0) {
+#pragma unroll
+  for (int e = 0; e < V; e += 2) {
+    // a masked class: p = 0 and a finite log p, so that its product is 0
+    const f32x2 lp = bounded2(add2(add2(pair(z[e], z[e + 1]), g.m), g.L));
+    const float2 d = halves(mul2(exp_neg2(lp), fma2(g.b, lp, g.a)));
+    z[e] = d.x, z[e + 1] = d.y;
+  }
+  if ((unsigned)(g.y - c0) < (unsigned)V && g.y >= 0) {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (c0 + e == g.y) z[e] += g.gl;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -195,31 +251,128 @@ struct HeldRow {
   static constexpr int V = Row<T>::V;
   float z[E];
   __device__ void load(const Row<T>& r, int lane) {
+    uint4 u[E / V];
 #pragma unroll
-    for (int j = 0; j < E / V; ++j) {
-      float v[V];
-      r.load(j * G + lane, v);
+    for (int j = 0; j < E / V; ++j) u[j] = r.raw(j * G + lane);
 #pragma unroll
-      for (int e = 0; e < V; ++e) z[j * V + e] = v[e];
-    }
+    for (int j = 0; j < E / V; ++j) Row<T>::unpack(u[j], z + j * V);
   }
   __device__ RowStats stats() const {
     float m = z[0];
 #pragma unroll
     for (int j = 1; j < E; ++j) m = fmaxf(m, z[j]);
     m = group_max<G>(fmaxf(m, -INFINITY));
-    const float m0 = m == -INFINITY ? 0.f : m;
-    float s = 0.f, t = 0.f;
+    const float m0 = m == -INFINITY ? 0.f : -m;
+    f32x2 s = pair(0.f, 0.f), t = s;
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const float d = max_nan(z[j] - m0, LP_FAR), e = exp_neg(d);
-      s += e;
-      t += e * d;
+    for (int j = 0; j < E; j += 2) {
+      const f32x2 d = bounded2(add2(pair(z[j], z[j + 1]), pair(m0, m0))), e = exp_neg2(d);
+      s = add2(s, e);
+      t = fma2(e, d, t);
     }
-    return row_stats(m, group_sum<G>(s), group_sum<G>(t));
+    const float2 a = halves(s), b = halves(t);
+    return row_stats(m, group_sum<G>(a.x + a.y), group_sum<G>(b.x + b.y));
   }
   __device__ static int at(const Row<T>& r, int lane, int j) { return r.first((j / V) * G + lane) + j % V; }
 };
+
+// ---------------------------------------------------------------------------
+// Best classes of a warp.  A key is a score's order and the class's complement (ties to the lowest
+// class), 0 where there is none.
+// ---------------------------------------------------------------------------
+typedef unsigned long long class_key;
+constexpr int LP_CANDIDATES = 128;  // keys of one piece in shared memory
+
+__device__ __forceinline__ class_key make_key(uint32_t order, uint32_t c) {
+  return ((class_key)order << 32) | (uint32_t)~c;
+}
+
+// Bitonic networks over the lanes, descending (Batcher, 1968): all stages, or the last only, which
+// sorts a bitonic sequence.
+template <typename K>
+__device__ __forceinline__ K lanes_exchange(K v, int stride, bool keep_max) {
+  const K o = __shfl_xor_sync(0xFFFFFFFFu, v, stride);
+  return (v < o) == keep_max ? o : v;
+}
+template <typename K>
+__device__ __forceinline__ K lanes_merge(K v) {
+#pragma unroll
+  for (int stride = 16; stride > 0; stride >>= 1) v = lanes_exchange(v, stride, (lane_id() & stride) == 0);
+  return v;
+}
+template <typename K>
+__device__ __forceinline__ K lanes_sort(K v) {
+#pragma unroll
+  for (int size = 2; size < 32; size <<= 1)
+#pragma unroll
+    for (int stride = size >> 1; stride > 0; stride >>= 1)
+      v = lanes_exchange(v, stride, ((lane_id() & stride) == 0) == ((lane_id() & size) == 0));
+  return lanes_merge(v);
+}
+
+// The warp's 32 best classes so far, lane i the i-th.
+struct BestList {
+  class_key key = 0;
+  __device__ class_key limit(int k) const { return __shfl_sync(0xFFFFFFFFu, key, k - 1); }
+  // Takes in the lanes' keys, descending.
+  __device__ void join(class_key sorted) {
+    const class_key o = __shfl_sync(0xFFFFFFFFu, sorted, 31 - lane_id());
+    key = lanes_merge(max(key, o));
+  }
+  // Every lane of the warp with the same `k`.
+  __device__ void insert(class_key k) {
+    const unsigned above = __ballot_sync(0xFFFFFFFFu, key > k);
+    const class_key up = __shfl_up_sync(0xFFFFFFFFu, key, 1);
+    const int pos = __popc(above);
+    if (lane_id() == pos) key = k;
+    if (lane_id() > pos) key = up;
+  }
+};
+
+// Takes the lanes' N scores into the list.  `cls(j)`: the class of a lane's j-th score, -1 for none;
+// `bound`: an order that the k best scores of list and lanes reach.  What reaches it, usually little
+// more than k keys, is gathered in `buf` (LP_CANDIDATES keys and a counter of this warp, 0 on entry
+// and on exit); where it does not fit (many equal scores) the keys are inserted one by one.
+template <int N, typename F>
+__device__ __forceinline__ void best_take(BestList& best, int k, const float (&z)[N], F cls, uint32_t bound,
+                                          class_key* buf, int* count) {
+  class_key limit = best.limit(k);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const uint32_t o = class_order(z[j]);
+    const int c = cls(j);
+    if (o >= bound && c >= 0) {
+      const class_key key = make_key(o, (uint32_t)c);
+      if (key > limit) {
+        const int at = atomicAdd(count, 1);
+        if (at < LP_CANDIDATES) buf[at] = key;
+      }
+    }
+  }
+  __syncwarp();
+  const int n = *count;
+  __syncwarp();
+  if (lane_id() == 0) *count = 0;
+  if (n <= LP_CANDIDATES) {
+    for (int i = 0; i < n; i += 32) best.join(lanes_sort(i + lane_id() < n ? buf[i + lane_id()] : (class_key)0));
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = cls(j);
+      const class_key key = c >= 0 ? make_key(class_order(z[j]), (uint32_t)c) : (class_key)0;
+      unsigned todo = __ballot_sync(0xFFFFFFFFu, key > limit);
+      while (todo) {
+        const class_key one = __shfl_sync(0xFFFFFFFFu, key, __ffs(todo) - 1);
+        todo &= todo - 1;
+        if (one > limit) {
+          best.insert(one);
+          limit = best.limit(k);
+        }
+      }
+    }
+  }
+  __syncwarp();
+}
 
 // blockDim 256; a row beyond the last is computed again from the last and not written.
 template <typename T, int G, int E, bool TOP>
@@ -234,7 +387,24 @@ __global__ void __launch_bounds__(256) log_probs_held_forward_kernel(const LogPr
   const RowStats st = h.stats();
   const bool mine = lane == 0 && at < a.rows;
   if (mine) write_row<T>(a, row, z, st);
-  if constexpr (TOP) {
+  if constexpr (TOP && G == 32) {
+    __shared__ class_key buf[8][LP_CANDIDATES];
+    __shared__ int count[8];
+    if (lane == 0) count[warp_id()] = 0;
+    uint32_t mine_max = 0;
+    const auto cls = [&](int j) {
+      const int c = h.at(r, lane, j);
+      return c < a.C ? c : -1;
+    };
+#pragma unroll
+    for (int j = 0; j < E; ++j) mine_max = max(mine_max, cls(j) >= 0 ? class_order(h.z[j]) : 0u);
+    __syncwarp();
+    // fewer than k lanes with a score: the bound is 0 and every score passes
+    const uint32_t bound = __shfl_sync(0xFFFFFFFFu, lanes_sort(mine_max), a.k - 1);
+    BestList best;
+    best_take<E>(best, a.k, h.z, cls, bound, buf[warp_id()], &count[warp_id()]);
+    if (lane < a.k && at < a.rows) write_best(a, row, lane, (uint32_t)(best.key >> 32), (uint32_t)~(uint32_t)best.key, st);
+  } else if constexpr (TOP) {
     // k rounds: the lanes' best unused classes, then the group's; its lane looks for its next best
     uint32_t order[E];
     uint32_t best = 0, where = 0xFFFFFFFFu;
@@ -246,15 +416,10 @@ __global__ void __launch_bounds__(256) log_probs_held_forward_kernel(const LogPr
     }
     for (int i = 0; i < a.k; ++i) {
       uint32_t b = best, w = where;
-      if constexpr (G == 32) {
-        b = __reduce_max_sync(0xFFFFFFFFu, best);
-        w = __reduce_min_sync(0xFFFFFFFFu, best == b ? where : 0xFFFFFFFFu);
-      } else {
 #pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) {
-          const uint32_t bo = __shfl_xor_sync(0xFFFFFFFFu, b, o), wo = __shfl_xor_sync(0xFFFFFFFFu, w, o);
-          if (bo > b || (bo == b && wo < w)) b = bo, w = wo;
-        }
+      for (int o = G / 2; o > 0; o >>= 1) {
+        const uint32_t bo = __shfl_xor_sync(0xFFFFFFFFu, b, o), wo = __shfl_xor_sync(0xFFFFFFFFu, w, o);
+        if (bo > b || (bo == b && wo < w)) b = bo, w = wo;
       }
       if (mine) write_best(a, row, i, b, w, st);
       if (w == where) {
@@ -281,14 +446,21 @@ __global__ void __launch_bounds__(256) log_probs_held_backward_kernel(const LogP
   h.load(r, lane);
   const RowStats st = h.stats();
   const RowGrad g = row_grad(a, row, st);
+  constexpr int V = Row<T>::V;
   if constexpr (G == 1) {
     // the warp's 32 rows are one piece of dlogits: gather them in shared memory and write it in words
     __shared__ __align__(16) T stage[8][32 * E];
     T* mine = stage[warp_id()];
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const int c = h.at(r, lane, j);
-      if (c >= 0 && c < a.C) mine[lane_id() * a.C + c] = from_f32<T>(score_grad(g, st, h.z[j], c));
+    for (int j = 0; j < E / V; ++j) {
+      float d[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[e] = h.z[j * V + e];
+      const int c0 = h.at(r, lane, j * V);
+      score_grad<V>(g, d, c0);
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (c0 + e >= 0 && c0 + e < a.C) mine[lane_id() * a.C + c0 + e] = from_f32<T>(d[e]);
     }
     __syncwarp();
     const int64_t row0 = at - lane_id();
@@ -306,26 +478,13 @@ __global__ void __launch_bounds__(256) log_probs_held_backward_kernel(const LogP
   } else {
     if (at >= a.rows) return;
     T* out = static_cast<T*>(a.dlogits) + row * a.C;
-    constexpr int V = Row<T>::V;
 #pragma unroll
     for (int j = 0; j < E / V; ++j) {
-      const int c0 = r.first(j * G + lane);
       float d[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) d[e] = score_grad(g, st, h.z[j * V + e], c0 + e);
-      if (c0 >= 0 && c0 + V <= a.C && (reinterpret_cast<uintptr_t>(out + c0) & 15u) == 0) {
-        uint4 u;
-        if constexpr (sizeof(T) == 2)
-          u = make_uint4(pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3]), pack_bf16x2(d[4], d[5]),
-                         pack_bf16x2(d[6], d[7]));
-        else
-          u = make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2]), __float_as_uint(d[3]));
-        *reinterpret_cast<uint4*>(out + c0) = u;
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (c0 + e >= 0 && c0 + e < a.C) out[c0 + e] = from_f32<T>(d[e]);
-      }
+      for (int e = 0; e < V; ++e) d[e] = h.z[j * V + e];
+      score_grad<V>(g, d, r.first(j * G + lane));
+      r.store(out, j * G + lane, d);
     }
   }
 }
@@ -334,133 +493,112 @@ __global__ void __launch_bounds__(256) log_probs_held_backward_kernel(const LogP
 // Long rows: one block per row, one pass.
 // ---------------------------------------------------------------------------
 
-// The warp's 32 best classes so far, lane i the i-th: order and the class's complement (ties to
-// the lowest class), 0 where there is none yet.
-struct BestList {
-  unsigned long long key = 0;
-  __device__ static unsigned long long make(uint32_t order, uint32_t c) {
-    return ((unsigned long long)order << 32) | (uint32_t)~c;
-  }
-  __device__ unsigned long long threshold(int k) const { return __shfl_sync(0xFFFFFFFFu, key, k - 1); }
-  // Every lane of the warp with the same `k`.
-  __device__ void insert(unsigned long long k) {
-    const unsigned above = __ballot_sync(0xFFFFFFFFu, key > k);
-    const unsigned long long up = __shfl_up_sync(0xFFFFFFFFu, key, 1);
-    const int pos = __popc(above);
-    if (lane_id() == pos) key = k;
-    if (lane_id() > pos) key = up;
-  }
-};
-
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(1024) log_probs_long_forward_kernel(const LogProbsArgs a) {
-  constexpr int V = Row<T>::V, U = 32 / V;  // vectors in flight: 32 scores a thread
+  constexpr int V = Row<T>::V, U = 4;  // vectors of a thread in one piece
   __shared__ float red[3][32];
-  __shared__ unsigned long long keys[TOP ? 32 * TP_MAX_TOP_K : 1];
+  __shared__ class_key buf[TOP ? 32 : 1][TOP ? LP_CANDIDATES : 1];
+  __shared__ int count[32];
   const int64_t row = blockIdx.x;
   const T* z = static_cast<const T*>(a.logits) + row * a.ld;
   const Row<T> r(z, a.C);
-  const int nv = r.vectors(), threads = blockDim.x, warps = threads >> 5;
-  float m = -INFINITY, s = 0.f, t = 0.f;
+  const int nv = r.vectors(), threads = blockDim.x, warps = threads >> 5, wid = warp_id();
+  if (TOP && lane_id() == 0) count[wid] = 0;
+  __syncwarp();
+  float m = -INFINITY;
+  f32x2 s = pair(0.f, 0.f), t = s;
   BestList best;
-  unsigned long long limit = 0;
+  uint32_t limit = 0;  // order of the k-th best so far
+  uint4 next[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = u * threads + threadIdx.x;
+    next[u] = i < nv ? r.raw(i) : Row<T>::nothing();
+  }
   for (int i0 = 0; i0 < nv; i0 += U * threads) {
-    float v[U][V];
+    float v[U * V];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * threads + threadIdx.x;
-      if (i < nv) {
-        r.load(i, v[u]);
-      } else {
+    for (int u = 0; u < U; ++u) Row<T>::unpack(next[u], v + u * V);
+    if (i0 + U * threads < nv) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[u][e] = -INFINITY;
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + (U + u) * threads + threadIdx.x;
+        next[u] = i < nv ? r.raw(i) : Row<T>::nothing();
       }
     }
     float cm = -INFINITY;
-    bool nan = false;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        cm = fmaxf(cm, v[u][e]);
-        if (TOP) nan |= v[u][e] != v[u][e];
-      }
+    for (int e = 0; e < U * V; ++e) cm = fmaxf(cm, v[e]);
     if (cm > m) {
       if (m != -INFINITY) {
         const float d = fmaxf(m - cm, LP_FAR), c = exp_neg(d);
-        t = c * (t + s * d);
-        s *= c;
+        t = mul2(pair(c, c), fma2(s, pair(d, d), t));
+        s = mul2(s, pair(c, c));
       }
       m = cm;
     }
-    const float m0 = m == -INFINITY ? 0.f : m;
+    const float m0 = m == -INFINITY ? 0.f : -m;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float d = max_nan(v[u][e] - m0, LP_FAR), x = exp_neg(d);
-        s += x;
-        t += x * d;
-      }
+    for (int e = 0; e < U * V; e += 2) {
+      const f32x2 d = bounded2(add2(pair(v[e], v[e + 1]), pair(m0, m0))), x = exp_neg2(d);
+      s = add2(s, x);
+      t = fma2(x, d, t);
+    }
     if constexpr (TOP) {
-      // most pieces hold nothing above the k-th best: one comparison for 32 scores
-      const bool any = nan || class_order(cm) >= (uint32_t)(limit >> 32);
-      if (__any_sync(0xFFFFFFFFu, any)) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int c0 = r.first(i0 + u * threads + threadIdx.x);
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const int c = c0 + e;
-            const bool in = c >= 0 && c < a.C;
-            const unsigned long long k = in ? BestList::make(class_order(v[u][e]), (uint32_t)c) : 0ull;
-            unsigned todo = __ballot_sync(0xFFFFFFFFu, k > limit);
-            while (todo) {
-              const unsigned long long kk = __shfl_sync(0xFFFFFFFFu, k, __ffs(todo) - 1);
-              todo &= todo - 1;
-              if (kk > limit) {
-                best.insert(kk);
-                limit = best.threshold(a.k);
-              }
-            }
-          }
-        }
+      // a NaN is above every limit, and in the sum from then on
+      const float2 ss = halves(s);
+      const uint32_t mine = ss.x + ss.y != ss.x + ss.y ? 0xFFFFFFFFu : class_order(cm);
+      if (__any_sync(0xFFFFFFFFu, mine >= limit)) {
+        const auto cls = [&](int j) {
+          const int c = r.first(i0 + j / V * threads + threadIdx.x) + j % V;
+          return c < a.C ? c : -1;
+        };
+        // until the list is full, the k-th largest of the lanes' maxima (-inf in a lane without scores:
+        // every score reaches it); a NaN's place in the order is above its lane's maximum
+        const uint32_t bound = max(limit, __shfl_sync(0xFFFFFFFFu, lanes_sort(class_order(cm)), a.k - 1));
+        best_take<U * V>(best, a.k, v, cls, bound, buf[wid], &count[wid]);
+        limit = (uint32_t)(best.limit(a.k) >> 32);
       }
     }
   }
   // join the threads' sums at the block's maximum
   const float wm = group_max<32>(m);
-  if (lane_id() == 0) red[0][warp_id()] = wm;
-  if (TOP && lane_id() < a.k) keys[warp_id() * a.k + lane_id()] = best.key;
+  if (lane_id() == 0) red[0][wid] = wm;
+  if (TOP) buf[wid][lane_id()] = best.key;
   __syncthreads();
   const float bm = group_max<32>(lane_id() < warps ? red[0][lane_id()] : -INFINITY);
-  if (m != -INFINITY) {
-    const float d = fmaxf(m - bm, LP_FAR), c = m == bm ? 1.f : exp_neg(d);
-    t = m == bm ? t : c * (t + s * d);
-    s *= c;
+  const float2 sh = halves(s), th = halves(t);
+  float s1 = sh.x + sh.y, t1 = th.x + th.y;
+  if (m != -INFINITY && m != bm) {
+    const float d = fmaxf(m - bm, LP_FAR), c = exp_neg(d);
+    t1 = c * (t1 + s1 * d);
+    s1 *= c;
   }
-  s = group_sum<32>(s);
-  t = group_sum<32>(t);
+  s1 = group_sum<32>(s1);
+  t1 = group_sum<32>(t1);
   if (lane_id() == 0) {
-    red[1][warp_id()] = s;
-    red[2][warp_id()] = t;
+    red[1][wid] = s1;
+    red[2][wid] = t1;
   }
-  __syncthreads();
-  if (warp_id() != 0) return;
-  s = group_sum<32>(lane_id() < warps ? red[1][lane_id()] : 0.f);
-  t = group_sum<32>(lane_id() < warps ? red[2][lane_id()] : 0.f);
-  const RowStats st = row_stats(bm, s, t);
-  if (lane_id() == 0) write_row<T>(a, row, z, st);
   if constexpr (TOP) {
-    for (int i = a.k; i < warps * a.k; ++i) {
-      const unsigned long long k = keys[i];
-      if (k > limit) {
-        best.insert(k);
-        limit = best.threshold(a.k);
+    // the warps' lists, two by two
+    for (int half = 16; half > 0; half >>= 1) {
+      if (wid < half && wid + half < warps) {
+        best.join(buf[wid + half][lane_id()]);
+        buf[wid][lane_id()] = best.key;
       }
+      __syncthreads();
     }
-    if (lane_id() < a.k) write_best(a, row, lane_id(), (uint32_t)(best.key >> 32), (uint32_t)~(uint32_t)best.key, st);
+  } else {
+    __syncthreads();
   }
+  if (wid != 0) return;
+  s1 = group_sum<32>(lane_id() < warps ? red[1][lane_id()] : 0.f);
+  t1 = group_sum<32>(lane_id() < warps ? red[2][lane_id()] : 0.f);
+  const RowStats st = row_stats(bm, s1, t1);
+  if (lane_id() == 0) write_row<T>(a, row, z, st);
+  if (TOP && lane_id() < a.k)
+    write_best(a, row, lane_id(), (uint32_t)(best.key >> 32), (uint32_t)~(uint32_t)best.key, st);
 }
 
 // One warp per LP_CHUNK scores of a row.
@@ -479,28 +617,21 @@ __global__ void __launch_bounds__(256) log_probs_stream_backward_kernel(const Lo
   st.L = a.stats[3 * row + 1];
   st.H = a.stats[3 * row + 2];
   const RowGrad g = row_grad(a, row, st);
-  const bool same = ((reinterpret_cast<uintptr_t>(out) / sizeof(T)) & (V - 1)) == (uintptr_t)r.phase;
+  for (int u0 = 0; u0 < U; u0 += 4) {
+    uint4 raw[4];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = i0 + 32 * u;
-    if (i >= nv) break;
-    float v[V];
-    r.load(i, v);
-    const int c0 = r.first(i);
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + 32 * (u0 + u);
+      raw[u] = i < nv ? r.raw(i) : Row<T>::nothing();
+    }
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = score_grad(g, st, v[e], c0 + e);
-    if (same && c0 >= 0 && c0 + V <= a.C) {
-      uint4 w;
-      if constexpr (sizeof(T) == 2)
-        w = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                       pack_bf16x2(v[6], v[7]));
-      else
-        w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-      *reinterpret_cast<uint4*>(out + c0) = w;
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (c0 + e >= 0 && c0 + e < a.C) out[c0 + e] = from_f32<T>(v[e]);
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + 32 * (u0 + u);
+      if (i >= nv) return;
+      float d[V];
+      Row<T>::unpack(raw[u], d);
+      score_grad<V>(g, d, r.first(i));
+      r.store(out, i, d);
     }
   }
 }
