@@ -17,9 +17,10 @@
 // whole 16-byte vectors are loaded between the first and last boundary inside the row, single elements
 // before and after.
 //
-// The best classes cost little more than a comparison for 32 scores: the k-th largest of the 32 lanes'
-// maxima is a bound that at least k scores reach and few others do; what reaches it goes through
-// shared memory into one sort of 32 keys, and a sorted list of 32 takes the result in.
+// The best classes take nothing from the pass: the k-th largest of the threads' maxima is a bound that
+// at least k scores reach and few others do.  Only the threads whose maximum reaches it have
+// their scores looked at again (a long row's from the cache, spread over the block); what reaches the
+// bound goes through shared memory into a sort of 32 keys and a sorted list of 32.
 #pragma once
 
 #include "gemm_simt.cuh"
@@ -257,11 +258,14 @@ struct HeldRow {
 #pragma unroll
     for (int j = 0; j < E / V; ++j) Row<T>::unpack(u[j], z + j * V);
   }
-  __device__ RowStats stats() const {
-    float m = z[0];
+  __device__ float own_max() const {  // of the lane's scores, -inf without any (a NaN is passed over)
+    float m = -INFINITY;
 #pragma unroll
-    for (int j = 1; j < E; ++j) m = fmaxf(m, z[j]);
-    m = group_max<G>(fmaxf(m, -INFINITY));
+    for (int j = 0; j < E; ++j) m = fmaxf(m, z[j]);
+    return m;
+  }
+  __device__ RowStats stats(float own) const {
+    const float m = group_max<G>(own);
     const float m0 = m == -INFINITY ? 0.f : -m;
     f32x2 s = pair(0.f, 0.f), t = s;
 #pragma unroll
@@ -330,23 +334,21 @@ struct BestList {
 };
 
 // Takes the lanes' N scores into the list.  `cls(j)`: the class of a lane's j-th score, -1 for none;
-// `bound`: an order that the k best scores of list and lanes reach.  What reaches it, usually little
+// `bound`: a value that the k best scores reach (a NaN does too).  What reaches it, usually little
 // more than k keys, is gathered in `buf` (LP_CANDIDATES keys and a counter of this warp, 0 on entry
 // and on exit); where it does not fit (many equal scores) the keys are inserted one by one.
 template <int N, typename F>
-__device__ __forceinline__ void best_take(BestList& best, int k, const float (&z)[N], F cls, uint32_t bound,
-                                          class_key* buf, int* count) {
+__device__ __forceinline__ void best_take(BestList& best, int k, const float (&z)[N], F cls, float bound, class_key* buf,
+                                          int* count) {
   class_key limit = best.limit(k);
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const uint32_t o = class_order(z[j]);
+    if (z[j] < bound) continue;
     const int c = cls(j);
-    if (o >= bound && c >= 0) {
-      const class_key key = make_key(o, (uint32_t)c);
-      if (key > limit) {
-        const int at = atomicAdd(count, 1);
-        if (at < LP_CANDIDATES) buf[at] = key;
-      }
+    const class_key key = make_key(class_order(z[j]), (uint32_t)c);
+    if (c >= 0 && key > limit) {
+      const int at = atomicAdd(count, 1);
+      if (at < LP_CANDIDATES) buf[at] = key;
     }
   }
   __syncwarp();
@@ -356,10 +358,14 @@ __device__ __forceinline__ void best_take(BestList& best, int k, const float (&z
   if (n <= LP_CANDIDATES) {
     for (int i = 0; i < n; i += 32) best.join(lanes_sort(i + lane_id() < n ? buf[i + lane_id()] : (class_key)0));
   } else {
-#pragma unroll
+#pragma unroll 1
     for (int j = 0; j < N; ++j) {
       const int c = cls(j);
-      const class_key key = c >= 0 ? make_key(class_order(z[j]), (uint32_t)c) : (class_key)0;
+      float v = z[0];  // z[j] without an index into registers
+#pragma unroll
+      for (int i = 1; i < N; ++i)
+        if (i == j) v = z[i];
+      const class_key key = c >= 0 ? make_key(class_order(v), (uint32_t)c) : (class_key)0;
       unsigned todo = __ballot_sync(0xFFFFFFFFu, key > limit);
       while (todo) {
         const class_key one = __shfl_sync(0xFFFFFFFFu, key, __ffs(todo) - 1);
@@ -384,54 +390,60 @@ __global__ void __launch_bounds__(256) log_probs_held_forward_kernel(const LogPr
   const Row<T> r(z, a.C);
   HeldRow<T, G, E> h;
   h.load(r, lane);
-  const RowStats st = h.stats();
+  const float own = h.own_max();
+  const RowStats st = h.stats(own);
   const bool mine = lane == 0 && at < a.rows;
   if (mine) write_row<T>(a, row, z, st);
-  if constexpr (TOP && G == 32) {
-    __shared__ class_key buf[8][LP_CANDIDATES];
-    __shared__ int count[8];
-    if (lane == 0) count[warp_id()] = 0;
-    uint32_t mine_max = 0;
-    const auto cls = [&](int j) {
-      const int c = h.at(r, lane, j);
-      return c < a.C ? c : -1;
-    };
+  if constexpr (TOP) {
+    // a round per class costs 25 + 3 E instructions, the sorts some 300 in all
+    if (G < 32 || (E == 8 && a.k <= 8)) {
+      // k rounds: the lanes' best unused classes, then the group's; its lane looks for its next best
+      uint32_t order[E];
+      uint32_t best = 0, where = 0xFFFFFFFFu;
 #pragma unroll
-    for (int j = 0; j < E; ++j) mine_max = max(mine_max, cls(j) >= 0 ? class_order(h.z[j]) : 0u);
-    __syncwarp();
-    // fewer than k lanes with a score: the bound is 0 and every score passes
-    const uint32_t bound = __shfl_sync(0xFFFFFFFFu, lanes_sort(mine_max), a.k - 1);
-    BestList best;
-    best_take<E>(best, a.k, h.z, cls, bound, buf[warp_id()], &count[warp_id()]);
-    if (lane < a.k && at < a.rows) write_best(a, row, lane, (uint32_t)(best.key >> 32), (uint32_t)~(uint32_t)best.key, st);
-  } else if constexpr (TOP) {
-    // k rounds: the lanes' best unused classes, then the group's; its lane looks for its next best
-    uint32_t order[E];
-    uint32_t best = 0, where = 0xFFFFFFFFu;
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const int c = h.at(r, lane, j);
-      order[j] = (c >= 0 && c < a.C) ? class_order(h.z[j]) : 0u;
-      if (order[j] > best) best = order[j], where = (uint32_t)c;
-    }
-    for (int i = 0; i < a.k; ++i) {
-      uint32_t b = best, w = where;
-#pragma unroll
-      for (int o = G / 2; o > 0; o >>= 1) {
-        const uint32_t bo = __shfl_xor_sync(0xFFFFFFFFu, b, o), wo = __shfl_xor_sync(0xFFFFFFFFu, w, o);
-        if (bo > b || (bo == b && wo < w)) b = bo, w = wo;
+      for (int j = 0; j < E; ++j) {
+        const int c = h.at(r, lane, j);
+        order[j] = (c >= 0 && c < a.C) ? class_order(h.z[j]) : 0u;
+        if (order[j] > best) best = order[j], where = (uint32_t)c;
       }
-      if (mine) write_best(a, row, i, b, w, st);
-      if (w == where) {
-        best = 0;
-        where = 0xFFFFFFFFu;
+      for (int i = 0; i < a.k; ++i) {
+        uint32_t b = best, w = where;
+        if constexpr (G == 32) {
+          b = __reduce_max_sync(0xFFFFFFFFu, best);
+          w = __reduce_min_sync(0xFFFFFFFFu, best == b ? where : 0xFFFFFFFFu);
+        } else {
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const uint32_t c = (uint32_t)h.at(r, lane, j);
-          if (c == w) order[j] = 0;
-          if (order[j] > best) best = order[j], where = c;
+          for (int o = G / 2; o > 0; o >>= 1) {
+            const uint32_t bo = __shfl_xor_sync(0xFFFFFFFFu, b, o), wo = __shfl_xor_sync(0xFFFFFFFFu, w, o);
+            if (bo > b || (bo == b && wo < w)) b = bo, w = wo;
+          }
+        }
+        if (mine) write_best(a, row, i, b, w, st);
+        if (w == where) {
+          best = 0;
+          where = 0xFFFFFFFFu;
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            const uint32_t c = (uint32_t)h.at(r, lane, j);
+            if (c == w) order[j] = 0;
+            if (order[j] > best) best = order[j], where = c;
+          }
         }
       }
+    } else if constexpr (G == 32) {
+      __shared__ class_key buf[8][LP_CANDIDATES];
+      __shared__ int count[8];
+      if (lane == 0) count[warp_id()] = 0;
+      __syncwarp();
+      const auto cls = [&](int j) {
+        const int c = h.at(r, lane, j);
+        return c < a.C ? c : -1;
+      };
+      const float bound = class_value(__shfl_sync(0xFFFFFFFFu, lanes_sort(class_order(own)), a.k - 1));
+      BestList best;
+      best_take<E>(best, a.k, h.z, cls, bound, buf[warp_id()], &count[warp_id()]);
+      if (lane < a.k && at < a.rows)
+        write_best(a, row, lane, (uint32_t)(best.key >> 32), (uint32_t)~(uint32_t)best.key, st);
     }
   }
 }
@@ -444,7 +456,7 @@ __global__ void __launch_bounds__(256) log_probs_held_backward_kernel(const LogP
   const Row<T> r(static_cast<const T*>(a.logits) + row * a.ld, a.C);
   HeldRow<T, G, E> h;
   h.load(r, lane);
-  const RowStats st = h.stats();
+  const RowStats st = h.stats(h.own_max());
   const RowGrad g = row_grad(a, row, st);
   constexpr int V = Row<T>::V;
   if constexpr (G == 1) {
@@ -498,17 +510,16 @@ __global__ void __launch_bounds__(1024) log_probs_long_forward_kernel(const LogP
   constexpr int V = Row<T>::V, U = 4;  // vectors of a thread in one piece
   __shared__ float red[3][32];
   __shared__ class_key buf[TOP ? 32 : 1][TOP ? LP_CANDIDATES : 1];
-  __shared__ int count[32];
+  __shared__ uint32_t maxima[TOP ? 32 : 1][32];
+  __shared__ uint16_t again[TOP ? 1024 : 1];  // threads whose scores are looked at again
+  __shared__ int count[33];                   // of each warp's buf; last: of `again`
   const int64_t row = blockIdx.x;
   const T* z = static_cast<const T*>(a.logits) + row * a.ld;
   const Row<T> r(z, a.C);
   const int nv = r.vectors(), threads = blockDim.x, warps = threads >> 5, wid = warp_id();
-  if (TOP && lane_id() == 0) count[wid] = 0;
-  __syncwarp();
+  if (TOP && lane_id() == 0) count[wid] = count[32] = 0;
   float m = -INFINITY;
   f32x2 s = pair(0.f, 0.f), t = s;
-  BestList best;
-  uint32_t limit = 0;  // order of the k-th best so far
   uint4 next[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -544,31 +555,20 @@ __global__ void __launch_bounds__(1024) log_probs_long_forward_kernel(const LogP
       s = add2(s, x);
       t = fma2(x, d, t);
     }
-    if constexpr (TOP) {
-      // a NaN is above every limit, and in the sum from then on
-      const float2 ss = halves(s);
-      const uint32_t mine = ss.x + ss.y != ss.x + ss.y ? 0xFFFFFFFFu : class_order(cm);
-      if (__any_sync(0xFFFFFFFFu, mine >= limit)) {
-        const auto cls = [&](int j) {
-          const int c = r.first(i0 + j / V * threads + threadIdx.x) + j % V;
-          return c < a.C ? c : -1;
-        };
-        // until the list is full, the k-th largest of the lanes' maxima (-inf in a lane without scores:
-        // every score reaches it); a NaN's place in the order is above its lane's maximum
-        const uint32_t bound = max(limit, __shfl_sync(0xFFFFFFFFu, lanes_sort(class_order(cm)), a.k - 1));
-        best_take<U * V>(best, a.k, v, cls, bound, buf[wid], &count[wid]);
-        limit = (uint32_t)(best.limit(a.k) >> 32);
-      }
-    }
   }
   // join the threads' sums at the block's maximum
   const float wm = group_max<32>(m);
   if (lane_id() == 0) red[0][wid] = wm;
-  if (TOP) buf[wid][lane_id()] = best.key;
-  __syncthreads();
-  const float bm = group_max<32>(lane_id() < warps ? red[0][lane_id()] : -INFINITY);
   const float2 sh = halves(s), th = halves(t);
   float s1 = sh.x + sh.y, t1 = th.x + th.y;
+  uint32_t order = 0;
+  if constexpr (TOP) {
+    // a thread with a NaN, which its sum then holds, is above all; one without scores counts as -inf
+    order = s1 != s1 ? 0xFFFFFFFFu : class_order(m);
+    maxima[wid][lane_id()] = lanes_sort(order);
+  }
+  __syncthreads();
+  const float bm = group_max<32>(lane_id() < warps ? red[0][lane_id()] : -INFINITY);
   if (m != -INFINITY && m != bm) {
     const float d = fmaxf(m - bm, LP_FAR), c = exp_neg(d);
     t1 = c * (t1 + s1 * d);
@@ -580,14 +580,43 @@ __global__ void __launch_bounds__(1024) log_probs_long_forward_kernel(const LogP
     red[1][wid] = s1;
     red[2][wid] = t1;
   }
+  BestList best;
   if constexpr (TOP) {
-    // the warps' lists, two by two
+    // the k-th largest of all threads' maxima: the warps' sorted lists, two by two
+    uint32_t list = maxima[wid][lane_id()];
     for (int half = 16; half > 0; half >>= 1) {
       if (wid < half && wid + half < warps) {
+        list = lanes_merge(max(list, maxima[wid + half][31 - lane_id()]));
+        maxima[wid][lane_id()] = list;
+      }
+      __syncthreads();
+    }
+    const uint32_t bound = maxima[0][a.k - 1];
+    if (order >= bound) again[atomicAdd(&count[32], 1)] = (uint16_t)threadIdx.x;
+    __syncthreads();
+    // those threads' vectors, spread over the block
+    const int per = (nv + threads - 1) / threads;
+    const int64_t tasks = (int64_t)count[32] * per;
+    for (int64_t p0 = wid * 32; p0 < tasks; p0 += threads) {
+      const int64_t p = p0 + lane_id();
+      const int i = p < tasks ? again[p / per] + (int)(p % per) * threads : nv;
+      float v[V];
+      Row<T>::unpack(i < nv ? r.raw(i) : Row<T>::nothing(), v);
+      const auto cls = [&](int j) {
+        const int c = r.first(i) + j;
+        return i < nv && c < a.C ? c : -1;
+      };
+      best_take<V>(best, a.k, v, cls, class_value(bound), buf[wid], &count[wid]);
+    }
+    const int lists = (int)min((int64_t)warps, (tasks + 31) / 32);
+    buf[wid][lane_id()] = best.key;
+    __syncthreads();
+    for (int half = 16; half > 0; half >>= 1) {
+      if (wid < half && wid + half < lists) {
         best.join(buf[wid + half][lane_id()]);
         buf[wid][lane_id()] = best.key;
       }
-      __syncthreads();
+      if (half < lists) __syncthreads();
     }
   } else {
     __syncthreads();
