@@ -721,20 +721,35 @@ def binary_roc_auc(scores: Tensor, labels: Tensor, workspace: Tensor | None = No
     return out
 
 
-def _call(name: str, args, device: torch.device) -> None:
-    """`name(args)` on the current stream of `device`, whichever device is current."""
+def _call(name: str, args, device: int) -> None:
+    """`name(args)` on the current stream of device number `device`, whichever device is current.
+    (The raw stream handle: building a `torch.cuda.Stream` takes as long as the launch.)"""
     fn = getattr(load(), name)
-    if device.index == torch.cuda.current_device():
-        check(fn(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream), name)
+    if device == torch._C._cuda_getDevice():
+        check(fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device)), name)
     else:
         with torch.cuda.device(device):
-            check(fn(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream), name)
+            check(fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device)), name)
 
 
-def _same_device(device: torch.device, **tensors: Tensor | None) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f'{name} must be on {device}, got {t.device}')
+def _device_of(name: str, t: Tensor) -> int:
+    i = t.get_device()
+    if i < 0:
+        raise RuntimeError(f'{name} must be a CUDA tensor (tabpack_b200 has no CPU path)')
+    return i
+
+
+def _operand(name: str, t: Tensor | None, shape: tuple, dtype: torch.dtype, device: int) -> Tensor | None:
+    """`t` contiguous, checked against the shape, type and device that it has to have."""
+    if t is None:
+        return None
+    if t.dtype is not dtype:
+        raise TypeError(f'{name} must have dtype {dtype}, got {t.dtype}')
+    if t.shape != shape:
+        raise ValueError(f'{name} must be {shape}, got {tuple(t.shape)}')
+    if t.get_device() != device:
+        raise ValueError(f'{name} must be on cuda:{device}, got {t.device}')
+    return t if t.is_contiguous() else t.contiguous()
 
 
 ADAMW8_BLOCK = 128
@@ -751,19 +766,17 @@ def adamw8_state(p: Tensor) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     return codes(), scales(), codes(), scales()
 
 
-def _adamw8_check(shape, device, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale) -> int:
-    """Checks one tensor's state; returns the elements of one member."""
-    inner = 1
-    for n in shape[1:]:
-        inner *= n
-    nb = (inner + ADAMW8_BLOCK - 1) // ADAMW8_BLOCK
-    for name, t in (('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq)):
-        if t.dtype != torch.uint8 or t.shape != shape or t.device != device or not t.is_contiguous():
-            raise TypeError(f'{name} must be a contiguous uint8 {tuple(shape)} tensor on {device}')
-    for name, t in (('exp_avg_scale', exp_avg_scale), ('exp_avg_sq_scale', exp_avg_sq_scale)):
-        if t.dtype != torch.float32 or t.shape != (shape[0], nb) or t.device != device or not t.is_contiguous():
-            raise TypeError(f'{name} must be a contiguous fp32 ({shape[0]}, {nb}) tensor on {device}')
-    return inner
+def _adamw8_state_fits(shape, P: int, nb: int, device: int, m: Tensor, ms: Tensor, v: Tensor, vs: Tensor) -> bool:
+    return (m.dtype is torch.uint8 and v.dtype is torch.uint8 and m.shape == shape and v.shape == shape
+            and ms.dtype is torch.float32 and vs.dtype is torch.float32 and ms.shape == (P, nb) and vs.shape == (P, nb)
+            and m.get_device() == device and v.get_device() == device and ms.get_device() == device
+            and vs.get_device() == device and m.is_contiguous() and v.is_contiguous() and ms.is_contiguous()
+            and vs.is_contiguous())
+
+
+def _adamw8_state_error(shape, P: int, nb: int, device: int) -> TypeError:
+    return TypeError(f'exp_avg and exp_avg_sq must be contiguous uint8 {tuple(shape)} tensors, exp_avg_scale and '
+                     f'exp_avg_sq_scale contiguous fp32 ({P}, {nb}) tensors, on cuda:{device}')
 
 
 def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, *, steps=None,
@@ -778,50 +791,59 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq
     give the random bits of the moments' rounding.  Tensors are chunked into launches of at most 32.
     """
     n = len(params)
-    if not all(len(t) == n for t in (grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales)) or (
+    if not n == len(grads) == len(exp_avgs) == len(exp_avg_scales) == len(exp_avg_sqs) == len(exp_avg_sq_scales) or (
             steps is not None and len(steps) != n):
         raise ValueError('one gradient, state and step per parameter is required')
     if steps is None and int(step) <= 0:
         raise ValueError('the step count must be positive')
-    device = params[0].device if n else None
-    hp = []
+    if n == 0:
+        return
+    device = _device_of('param', params[0])
+    hp, members = [], None
     for name, v in (('lr', lr), ('beta1', beta1), ('beta2', beta2), ('eps', eps), ('weight_decay', weight_decay)):
         if isinstance(v, Tensor):
-            _same_device(device, **{name: v})
-            v = v.contiguous()
-        hp.append(v)
-    sizes = {v.numel() for v in hp if isinstance(v, Tensor)}
-    for s in range(0, n, _lib.TP_MAX_OPT_TENSORS):
-        a = _lib.AdamW8Args()
-        used = 0
-        for i in range(s, min(n, s + _lib.TP_MAX_OPT_TENSORS)):
-            p, g = params[i], grads[i]
-            if p.dtype != torch.float32 or not p.is_cuda or not p.is_contiguous() or p.ndim == 0:
-                raise TypeError('param must be a contiguous fp32 CUDA tensor with a pack dimension')
-            if g.dtype != torch.float32 or g.shape != p.shape or not g.is_contiguous():
-                raise TypeError('grad must be a contiguous fp32 tensor of the shape of its parameter')
-            _same_device(device, param=p, grad=g)
-            inner = _adamw8_check(p.shape, device, exp_avgs[i], exp_avg_scales[i], exp_avg_sqs[i],
-                                  exp_avg_sq_scales[i])
-            P = p.shape[0]
-            if sizes and sizes != {P}:
+            if v.get_device() != device:
+                raise ValueError(f'{name} must be on cuda:{device}, got {v.device}')
+            if members not in (None, v.numel()):
                 raise ValueError('per-member hyperparameters must have one value per member')
-            st = None
-            if steps is not None:
-                st = steps[i]
-                if st.dtype != torch.int64 or st.shape != (P,) or st.device != device or not st.is_contiguous():
-                    raise TypeError(f'steps must be contiguous int64 ({P},) tensors on {device}')
-                st = st.data_ptr()
-            if P == 0 or inner == 0:
-                continue
-            a.t[used] = (p.data_ptr(), g.data_ptr(), exp_avgs[i].data_ptr(), exp_avg_scales[i].data_ptr(),
-                         exp_avg_sqs[i].data_ptr(), exp_avg_sq_scales[i].data_ptr(), st, P * inner, inner,
-                         (tensor_base + i) & 0xFFFFFFFF)
-            used += 1
-        if used == 0:
+            v, members = v.contiguous(), v.numel()
+        hp.append(v)
+    f32 = torch.float32
+    calls, a, used = [], None, 0
+    for i, p in enumerate(params):
+        g, m, ms, v, vs = grads[i], exp_avgs[i], exp_avg_scales[i], exp_avg_sqs[i], exp_avg_sq_scales[i]
+        shape = p.shape
+        if p.dtype is not f32 or p.get_device() != device or not p.is_contiguous() or not shape:
+            raise TypeError(f'param must be a contiguous fp32 tensor with a pack dimension on cuda:{device}')
+        if g.dtype is not f32 or g.get_device() != device or g.shape != shape or not g.is_contiguous():
+            raise TypeError(f'grad must be a contiguous fp32 tensor of the shape of its parameter on cuda:{device}')
+        P, numel = shape[0], p.numel()
+        inner = numel // P if P else 0
+        nb = (inner + ADAMW8_BLOCK - 1) // ADAMW8_BLOCK
+        if not _adamw8_state_fits(shape, P, nb, device, m, ms, v, vs):
+            raise _adamw8_state_error(shape, P, nb, device)
+        if members is not None and members != P:
+            raise ValueError('per-member hyperparameters must have one value per member')
+        st = None
+        if steps is not None:
+            st = steps[i]
+            if st.dtype is not torch.int64 or st.shape != (P,) or st.get_device() != device or not st.is_contiguous():
+                raise TypeError(f'steps must be contiguous int64 ({P},) tensors on cuda:{device}')
+            st = st.data_ptr()
+        if numel == 0:
             continue
+        if used % _lib.TP_MAX_OPT_TENSORS == 0:
+            a = _lib.AdamW8Args()
+            calls.append(a)
+            used = 0
+        a.t[used] = (p.data_ptr(), g.data_ptr(), m.data_ptr(), ms.data_ptr(), v.data_ptr(), vs.data_ptr(), st, numel,
+                     inner, (tensor_base + i) & 0xFFFFFFFF)
+        used += 1
         a.n_tensors = used
-        a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = (_hparam(v) for v in hp)
+    hp = [_hparam(v) for v in hp]
+    # every argument is checked before the first launch
+    for a in calls:
+        a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = hp
         a.step, a.seed = int(step), int(seed) & 0xFFFFFFFFFFFFFFFF
         a.member_base = int(member_base) & 0xFFFFFFFF
         _call('tp_adamw8_step', a, device)
@@ -835,67 +857,55 @@ def adamw8_moments(exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, *,
     codes' shapes in fp32 or bf16 (a code has at most five significant bits, its square ten: bf16
     rounds the latter); see `tp_adamw8_moments`."""
     n = len(exp_avgs)
-    if not all(len(t) == n for t in (exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales)):
+    if not n == len(exp_avg_scales) == len(exp_avg_sqs) == len(exp_avg_sq_scales):
         raise ValueError('every state needs its codes and scales')
     code = _dtype_code(dtype)
-    m, v = [], []
-    for s in range(0, n, _lib.TP_MAX_OPT_TENSORS):
-        a = _lib.AdamW8MomentsArgs()
-        used = 0
-        for i in range(s, min(n, s + _lib.TP_MAX_OPT_TENSORS)):
-            q = exp_avgs[i]
-            if not q.is_cuda or q.ndim == 0:
-                raise TypeError('exp_avg must be a CUDA tensor with a pack dimension')
-            inner = _adamw8_check(q.shape, exp_avgs[0].device, q, exp_avg_scales[i], exp_avg_sqs[i],
-                                  exp_avg_sq_scales[i])
-            mi, vi = (torch.empty(q.shape, dtype=dtype, device=q.device) for _ in range(2))
-            m.append(mi)
-            v.append(vi)
-            if q.numel() == 0:
-                continue
-            a.t[used] = (q.data_ptr(), exp_avg_scales[i].data_ptr(), exp_avg_sqs[i].data_ptr(),
-                         exp_avg_sq_scales[i].data_ptr(), mi.data_ptr(), vi.data_ptr(), q.numel(), inner)
-            used += 1
-        if used:
-            a.n_tensors, a.dtype = used, code
-            _call('tp_adamw8_moments', a, exp_avgs[0].device)
-    return m, v
+    if n == 0:
+        return [], []
+    device = _device_of('exp_avg', exp_avgs[0])
+    out_m, out_v = [], []
+    calls, a, used = [], None, 0
+    for i, m in enumerate(exp_avgs):
+        ms, v, vs = exp_avg_scales[i], exp_avg_sqs[i], exp_avg_sq_scales[i]
+        shape = m.shape
+        if not shape:
+            raise TypeError('a state must have a pack dimension')
+        P, numel = shape[0], m.numel()
+        inner = numel // P if P else 0
+        nb = (inner + ADAMW8_BLOCK - 1) // ADAMW8_BLOCK
+        if not _adamw8_state_fits(shape, P, nb, device, m, ms, v, vs):
+            raise _adamw8_state_error(shape, P, nb, device)
+        om, ov = m.new_empty(shape, dtype=dtype), m.new_empty(shape, dtype=dtype)
+        out_m.append(om)
+        out_v.append(ov)
+        if numel == 0:
+            continue
+        if used % _lib.TP_MAX_OPT_TENSORS == 0:
+            a = _lib.AdamW8MomentsArgs(dtype=code)
+            calls.append(a)
+            used = 0
+        a.t[used] = (m.data_ptr(), ms.data_ptr(), v.data_ptr(), vs.data_ptr(), om.data_ptr(), ov.data_ptr(), numel, inner)
+        used += 1
+        a.n_tensors = used
+    for a in calls:
+        _call('tp_adamw8_moments', a, device)
+    return out_m, out_v
 
 
-def _rows_strided(name: str, t: Tensor, P: int, B: int, W: int) -> tuple[Tensor, int, int]:
-    """A (P, B, W) view of t ((B, W): shared by the members) whose rows are contiguous, with its
-    member and row strides; copied only where the columns are not contiguous."""
-    if t.ndim == 2:
-        t = t.unsqueeze(0).expand(P, -1, -1)
-    if t.shape != (P, B, W):
-        raise ValueError(f'{name} must be ({P}, {B}, {W}) or ({B}, {W}), got {tuple(t.shape)}')
-    if W > 1 and t.stride(2) != 1:
+def _norm_rows(name: str, t: Tensor, dtype: torch.dtype, device: int, shape: tuple) -> tuple[Tensor, int, int]:
+    """`t` with contiguous columns (copied where they are not), and its member and row strides; a
+    (batch, features) tensor is shared by the members (member stride 0)."""
+    if t.dtype is not dtype:
+        raise TypeError(f'{name} must have dtype {dtype}, got {t.dtype}')
+    if t.get_device() != device:
+        raise ValueError(f'{name} must be on cuda:{device}, got {t.device}')
+    if t.shape != (shape if t.ndim == 3 else shape[1:]):
+        raise ValueError(f'{name} must be {shape} or {shape[1:]}, got {tuple(t.shape)}')
+    stride = t.stride()
+    if stride[-1] != 1 and shape[2] != 1:
         t = t.contiguous()
-    return t, t.stride(0) if P > 1 else 0, t.stride(1) if B > 1 else 0
-
-
-def _norm_args(x: Tensor, weight: Tensor | None, bias: Tensor | None, n_features: Tensor | None,
-               P: int | None) -> tuple[_lib.LayerNormArgs, tuple]:
-    if x.ndim not in (2, 3):
-        raise ValueError('x must be (pack_size, batch, features) or a shared (batch, features)')
-    if not x.is_cuda:
-        raise RuntimeError('x must be a CUDA tensor (tabpack_b200 has no CPU path)')
-    ref = weight if weight is not None else bias if bias is not None else n_features
-    if P is None:
-        P = x.shape[0] if x.ndim == 3 else 1 if ref is None else ref.shape[0]
-    B, W = x.shape[-2:]
-    a = _lib.LayerNormArgs(P=P, B=B, W=W, dtype=_dtype_code(x.dtype), dx_dtype=_dtype_code(x.dtype))
-    x, a.x_member_stride, a.x_row_stride = _rows_strided('x', x, P, B, W)
-    _same_device(x.device, weight=weight, bias=bias, n_features=n_features)
-    if n_features is not None and n_features.shape != (P,):
-        raise ValueError(f'n_features must be ({P},), got {tuple(n_features.shape)}')
-    for name, t in (('weight', weight), ('bias', bias)):
-        if t is not None and t.shape != (P, W):
-            raise ValueError(f'{name} must be ({P}, {W}), got {tuple(t.shape)}')
-    weight, bias = _cuda('weight', weight, torch.float32), _cuda('bias', bias, torch.float32)
-    n_features = _i32('n_features', n_features)
-    a.n_features, a.x, a.weight, a.bias = _ptr(n_features), x.data_ptr(), _ptr(weight), _ptr(bias)
-    return a, (x, weight, bias, n_features)
+        stride = t.stride()
+    return t, stride[0] if len(stride) == 3 and shape[0] > 1 else 0, stride[-2] if shape[1] > 1 else 0
 
 
 def layer_norm_forward(x: Tensor, weight: Tensor | None, bias: Tensor | None, *, n_features: Tensor | None = None,
@@ -904,17 +914,28 @@ def layer_norm_forward(x: Tensor, weight: Tensor | None, bias: Tensor | None, *,
     own weight and bias (P, W) fp32 or None; see `tp_layer_norm_forward`.  `n_features` (P,): member
     m's rows are normalised over their first n_features[m] columns, the others are zero in y.
     Returns (y (P, B, W), mean (P, B), rstd (P, B)); the backward takes the last two."""
-    if not eps >= 0.0 or eps == float('inf'):
+    if not 0.0 <= eps < float('inf'):
         raise ValueError('eps must be finite and not negative')
-    a, keep = _norm_args(x, weight, bias, n_features, None)
-    P, B, W, dev = a.P, a.B, a.W, x.device
-    y = torch.empty((P, B, W), dtype=x.dtype, device=dev)
-    stats = torch.empty((2, P, B), dtype=torch.float32, device=dev)
-    mean, rstd = stats[0], stats[1]
-    if y.numel():
-        a.eps, a.y, a.mean, a.rstd = eps, y.data_ptr(), mean.data_ptr(), rstd.data_ptr()
-        _call('tp_layer_norm_forward', a, dev)
-    del keep
+    if x.ndim not in (2, 3):
+        raise ValueError('x must be (pack_size, batch, features) or a shared (batch, features)')
+    device, dtype = _device_of('x', x), x.dtype
+    code = _dtype_code(dtype)
+    if x.ndim == 3:
+        P, B, W = x.shape
+    else:
+        B, W = x.shape
+        P = next((t.shape[0] for t in (weight, bias, n_features) if t is not None), 1)
+    x, sm, sr = _norm_rows('x', x, dtype, device, (P, B, W))
+    weight = _operand('weight', weight, (P, W), torch.float32, device)
+    bias = _operand('bias', bias, (P, W), torch.float32, device)
+    if n_features is not None:
+        n_features = _operand('n_features', n_features.to(torch.int32), (P,), torch.int32, device)
+    y = x.new_empty((P, B, W))
+    mean, rstd = x.new_empty((P, B), dtype=torch.float32), x.new_empty((P, B), dtype=torch.float32)
+    if P and B and W:
+        a = _lib.LayerNormArgs(P, B, W, code, sm, sr, _ptr(n_features), x.data_ptr(), _ptr(weight), _ptr(bias), eps,
+                               y.data_ptr(), mean.data_ptr(), rstd.data_ptr())
+        _call('tp_layer_norm_forward', a, device)
     return y, mean, rstd
 
 
@@ -923,136 +944,137 @@ def layer_norm_backward(dy: Tensor, x: Tensor, weight: Tensor | None, mean: Tens
                         need_db: bool = True) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
     """Backward of `layer_norm_forward`: (dx of x's shape and type, dw (P, W), db (P, W) fp32); a
     shared x takes the sum over the members.  See `tp_layer_norm_backward`."""
-    a, keep = _norm_args(x, weight, None, n_features, dy.shape[0])
-    P, B, W, dev = a.P, a.B, a.W, x.device
-    if dy.ndim != 3 or dy.dtype != x.dtype:
-        raise TypeError(f'dy must be a ({P}, {B}, {W}) {x.dtype} tensor')
-    _same_device(dev, dy=dy, mean=mean, rstd=rstd)
+    if dy.ndim != 3 or x.ndim not in (2, 3):
+        raise ValueError('dy must be (pack_size, batch, features), and x too or shared (batch, features)')
+    device, dtype = _device_of('x', x), x.dtype
+    code = _dtype_code(dtype)
+    shape = P, B, W = tuple(dy.shape)
+    x, sm, sr = _norm_rows('x', x, dtype, device, shape)
+    dy, dm, dr = _norm_rows('dy', dy, dtype, device, shape)
+    weight = _operand('weight', weight, (P, W), torch.float32, device)
+    if n_features is not None:
+        n_features = _operand('n_features', n_features.to(torch.int32), (P,), torch.int32, device)
     for name, t in (('mean', mean), ('rstd', rstd)):
-        if t.shape != (P, B) or t.dtype != torch.float32 or not t.is_contiguous():
+        if t.shape != (P, B) or t.dtype is not torch.float32 or t.get_device() != device or not t.is_contiguous():
             raise TypeError(f'{name} must be the contiguous fp32 ({P}, {B}) tensor of the forward')
-    dy, a.dy_member_stride, a.dy_row_stride = _rows_strided('dy', dy, P, B, W)
     shared = x.ndim == 2
     dx = dw = db = ws = None
     if need_dx:
         # the members' terms of a shared input are added up before they are rounded
-        dx = torch.empty((P, B, W), dtype=torch.float32 if shared else x.dtype, device=dev)
-        if shared:
-            a.dx_dtype = TP_DTYPE_F32
+        dx = x.new_empty(shape, dtype=torch.float32 if shared else dtype)
     if need_dw:
-        dw = torch.empty((P, W), dtype=torch.float32, device=dev)
+        dw = x.new_empty((P, W), dtype=torch.float32)
     if need_db:
-        db = torch.empty((P, W), dtype=torch.float32, device=dev)
+        db = x.new_empty((P, W), dtype=torch.float32)
     if P and B and W and (need_dx or need_dw or need_db):
-        a.dy, a.mean, a.rstd = dy.data_ptr(), mean.data_ptr(), rstd.data_ptr()
-        a.dx, a.dweight, a.dbias = _ptr(dx), _ptr(dw), _ptr(db)
-        if need_dw or need_db:
-            need = load().tp_layer_norm_workspace_size(P, B, W)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            a.workspace, a.workspace_bytes = _ptr(ws), need
-        _call('tp_layer_norm_backward', a, dev)
+        need = load().tp_layer_norm_workspace_size(P, B, W) if need_dw or need_db else 0
+        if need:
+            ws = x.new_empty(need, dtype=torch.uint8)
+        a = _lib.LayerNormArgs(P, B, W, code, sm, sr, _ptr(n_features), x.data_ptr(), _ptr(weight), None, 0.0, None,
+                               mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dm, dr, _ptr(dx),
+                               TP_DTYPE_F32 if shared else code, _ptr(dw), _ptr(db), _ptr(ws), need)
+        _call('tp_layer_norm_backward', a, device)
     else:
         for t in (dw, db):
             if t is not None:
                 t.zero_()
-    del keep, ws
-    if dx is not None and shared:
-        dx = dx.sum(0).to(x.dtype)
+    if shared and dx is not None:
+        dx = dx.sum(0).to(dtype)
     return dx, dw, db
 
 
 def _logit_rows(logits: Tensor) -> tuple[Tensor, int, int]:
     """logits (..., C) as rows at one stride: (tensor, rows, stride), copied only where the rows
     are not at one stride."""
-    C = logits.shape[-1]
-    rows = logits.numel() // C
-    stride, expect = C, None
-    ok = C == 1 or logits.stride(-1) == 1
-    for n, s in zip(reversed(logits.shape[:-1]), reversed(logits.stride()[:-1])):
-        if n == 1:
-            continue
-        if expect is None:
-            stride = expect = s
-        ok &= s == expect
-        expect *= n
+    shape, strides = logits.shape, logits.stride()
+    C = shape[-1]
+    rows, stride, ok = 1, C, C == 1 or strides[-1] == 1
+    for d in range(len(shape) - 2, -1, -1):
+        if shape[d] != 1:
+            if rows == 1:
+                stride = strides[d]
+            elif strides[d] != stride * rows:
+                ok = False
+            rows *= shape[d]
     if not ok or stride < C:
         logits, stride = logits.contiguous(), C
     return logits, rows, stride
 
 
-def _log_probs_args(logits: Tensor, labels: Tensor, ignore_index: int) -> tuple[_lib.LabelLogProbsArgs, tuple]:
-    if not logits.is_cuda:
-        raise RuntimeError('logits must be a CUDA tensor (tabpack_b200 has no CPU path)')
+def _log_probs_operands(logits: Tensor, labels: Tensor):
+    device = _device_of('logits', logits)
+    lead = logits.shape[:-1]
     if logits.ndim == 0 or logits.shape[-1] == 0:
         raise ValueError('logits must have at least one class')
-    if labels.dtype != torch.int64:
+    if labels.dtype is not torch.int64:
         raise TypeError('labels must have the int64 data type')
-    lead = logits.shape[:-1]
-    if labels.ndim > len(lead) or labels.shape != lead[len(lead) - labels.ndim:]:
+    if labels.shape != lead[len(lead) - labels.ndim:] or labels.ndim > len(lead):
         raise ValueError('The label and logit shapes are incompatible; only missing leading label dimensions '
                          'may be broadcast')
-    _same_device(logits.device, labels=labels)
-    a = _lib.LabelLogProbsArgs(C=logits.shape[-1], dtype=_dtype_code(logits.dtype), ignore_index=ignore_index)
-    logits, a.rows, a.logits_stride = _logit_rows(logits)
-    labels = labels.contiguous()
-    a.logits, a.labels, a.label_rows = logits.data_ptr(), labels.data_ptr(), labels.numel()
-    return a, (logits, labels)
+    if labels.get_device() != device:
+        raise ValueError(f'labels must be on cuda:{device}, got {labels.device}')
+    code = _dtype_code(logits.dtype)
+    logits, rows, stride = _logit_rows(logits)
+    return device, code, lead, logits, rows, stride, labels if labels.is_contiguous() else labels.contiguous()
 
 
 def label_log_probs_forward(logits: Tensor, labels: Tensor, *, top_k: int = 0, ignore_index: int = -100
-                            ) -> tuple[Tensor, Tensor, Tensor | None, Tensor | None, Tensor]:
+                            ) -> tuple[Tensor, Tensor, Tensor | None, Tensor | None, Tensor | None]:
     """Log probabilities of `labels` under softmax(logits), with entropies and the `top_k` best
     classes; see `tp_label_log_probs_forward`.  logits (..., C) bf16 or fp32; labels int64 of
     the leading shape, or without its first dimensions (labels that the members share).  Returns
-    (log_prob, entropy, top_log_prob or None, top_label or None, stats): fp32 of the leading
+    (log_prob, entropy, top_log_prob or None, top_label or None, stats or None): fp32 of the leading
     shape, (..., top_k) fp32 and int64, and what the backward takes."""
-    a, keep = _log_probs_args(logits, labels, ignore_index)
-    lead, dev = logits.shape[:-1], logits.device
-    if not 0 <= top_k <= min(a.C, _lib.TP_MAX_TOP_K):
-        raise ValueError(f'top_k must be between 0 and {min(a.C, _lib.TP_MAX_TOP_K)}, got {top_k}')
-    log_prob, entropy = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
-    stats = torch.empty((a.rows, 3) if a.C > _lib.TP_LABEL_STATS_CLASSES else 0, dtype=torch.float32, device=dev)
+    device, code, lead, logits, rows, stride, labels = _log_probs_operands(logits, labels)
+    C = logits.shape[-1]
+    if not 0 <= top_k <= min(C, _lib.TP_MAX_TOP_K):
+        raise ValueError(f'top_k must be between 0 and {min(C, _lib.TP_MAX_TOP_K)}, got {top_k}')
+    f32 = torch.float32
+    log_prob, entropy = logits.new_empty(lead, dtype=f32), logits.new_empty(lead, dtype=f32)
+    stats = logits.new_empty((rows, 3), dtype=f32) if C > _lib.TP_LABEL_STATS_CLASSES else None
     top = which = None
     if top_k:
-        top = torch.empty((*lead, top_k), dtype=torch.float32, device=dev)
-        which = torch.empty((*lead, top_k), dtype=torch.int64, device=dev)
-    if a.rows:
-        a.top_k, a.log_prob, a.entropy, a.stats = top_k, log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr() or None
-        a.top_log_prob, a.top_label = _ptr(top), _ptr(which)
-        _call('tp_label_log_probs_forward', a, dev)
-    del keep
+        top = logits.new_empty((*lead, top_k), dtype=f32)
+        which = logits.new_empty((*lead, top_k), dtype=torch.int64)
+    if rows:
+        a = _lib.LabelLogProbsArgs(rows, C, code, logits.data_ptr(), stride, labels.data_ptr(), labels.numel(),
+                                   ignore_index, top_k, log_prob.data_ptr(), entropy.data_ptr(), _ptr(top),
+                                   _ptr(which), _ptr(stats))
+        _call('tp_label_log_probs_forward', a, device)
     return log_prob, entropy, top, which, stats
 
 
-def _row_gradient(name: str, g: Tensor | None, lead, device) -> tuple[Tensor | None, int]:
+def _row_gradient(name: str, g: Tensor | None, lead, device: int) -> tuple[Tensor | None, int]:
     """A per-row fp32 gradient and its stride: 0 for one value that was expanded over the rows."""
     if g is None:
         return None, 0
-    if g.shape != lead or g.dtype != torch.float32 or g.device != device:
-        raise TypeError(f'{name} must be a {tuple(lead)} fp32 tensor on {device}')
-    if all(s == 0 or n == 1 for n, s in zip(g.shape, g.stride())):
+    if g.shape != lead or g.dtype is not torch.float32 or g.get_device() != device:
+        raise TypeError(f'{name} must be a {tuple(lead)} fp32 tensor on cuda:{device}')
+    if g.is_contiguous():
+        return g, 1
+    if not any(g.stride()):
         return g, 0
     return g.contiguous(), 1
 
 
 def label_log_probs_backward(g_log_prob: Tensor | None, g_entropy: Tensor | None, logits: Tensor, labels: Tensor,
-                             stats: Tensor, *, ignore_index: int = -100) -> Tensor:
+                             stats: Tensor | None, *, ignore_index: int = -100) -> Tensor:
     """The gradient of the logits (contiguous, of their shape and type) from the gradients of
     `label_log_probs_forward`'s log_prob and entropy (either may be None);
     see `tp_label_log_probs_backward`."""
-    a, keep = _log_probs_args(logits, labels, ignore_index)
-    lead, dev = logits.shape[:-1], logits.device
-    want = (a.rows, 3) if a.C > _lib.TP_LABEL_STATS_CLASSES else (0,)
-    if stats.shape != want or stats.dtype != torch.float32 or stats.device != dev or not stats.is_contiguous():
+    device, code, lead, logits, rows, stride, labels = _log_probs_operands(logits, labels)
+    C = logits.shape[-1]
+    if C > _lib.TP_LABEL_STATS_CLASSES and (stats is None or stats.shape != (rows, 3) or stats.get_device() != device
+                                            or stats.dtype is not torch.float32 or not stats.is_contiguous()):
         raise TypeError('stats must be the tensor that the forward returned')
-    g_log_prob, a.g_log_prob_stride = _row_gradient('g_log_prob', g_log_prob, lead, dev)
-    g_entropy, a.g_entropy_stride = _row_gradient('g_entropy', g_entropy, lead, dev)
-    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-    if a.rows:
-        a.stats, a.dlogits = stats.data_ptr() or None, dlogits.data_ptr()
-        a.g_log_prob, a.g_entropy = _ptr(g_log_prob), _ptr(g_entropy)
-        _call('tp_label_log_probs_backward', a, dev)
-    del keep
+    g_log_prob, sl = _row_gradient('g_log_prob', g_log_prob, lead, device)
+    g_entropy, sh = _row_gradient('g_entropy', g_entropy, lead, device)
+    dlogits = logits.new_empty((*lead, C))
+    if rows:
+        a = _lib.LabelLogProbsArgs(rows, C, code, logits.data_ptr(), stride, labels.data_ptr(), labels.numel(),
+                                   ignore_index, 0, None, None, None, None, _ptr(stats), _ptr(g_log_prob),
+                                   _ptr(g_entropy), sl, sh, dlogits.data_ptr())
+        _call('tp_label_log_probs_backward', a, device)
     return dlogits
 
 

@@ -368,6 +368,7 @@ def test_refusals():
         ops.label_log_probs_forward(z[..., :0], y)
     with pytest.raises(ValueError):
         ops.label_log_probs_forward(z, y.cpu())
+    z, y, g_l, g_h = make((3, 4), 300, torch.float32)
     stats = ops.label_log_probs_forward(z, y)[-1]
     with pytest.raises(TypeError):
         ops.label_log_probs_backward(g_l.bfloat16(), None, z, y, stats)
