@@ -11,9 +11,9 @@
 // stay in registers, while the next rows are on their way to shared memory (asynchronous copies: one
 // row ahead in registers left the memory waiting, 192 us instead of 114 for the forward of 16384 rows
 // of 8192 in bf16).  The forward takes two rows at a time, which share each reduction's latency.
-// Arithmetic is in pairs (f32x2).  Ragged rows need no tests per element: the copies fill x and dy with
-// zeros from column n on, and a factor of 0 there takes the mean (and the mean gradient) off
-// nothing.  Wider rows take the plain kernels at the end.
+// Arithmetic is in pairs (f32x2).  Ragged rows need few tests per element: the copies fill x and dy with
+// zeros from column n on, forward a factor of 0 there takes the mean off nothing, and backward only
+// the written padding is cleared.  Wider rows take the plain kernels at the end.
 #pragma once
 
 #include "gemm_simt.cuh"
@@ -85,27 +85,32 @@ struct NormGroup {
   __device__ NormGroup(float2* shared) : lane(threadIdx.x % G), group(threadIdx.x / G) {
     red = shared + group * 2 * WARPS;
   }
-  template <int PAIRS>  // 1: only u
+  // Sums of u and v over the group, in every lane.
   __device__ float2 sum(float u, float v) {
+    if constexpr (G < 32) {
 #pragma unroll
-    for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) {
-      u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
-      if (PAIRS == 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    }
-    if constexpr (G > 32) {
-      float2* r = red + half * WARPS;
-      half ^= 1;
-      if (lane % 32 == 0) r[lane / 32] = make_float2(u, v);
-      asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(G) : "memory");
-      const float2 t = r[lane % WARPS];
-      u = t.x, v = t.y;
-#pragma unroll
-      for (int o = WARPS / 2; o > 0; o >>= 1) {
+      for (int o = G / 2; o > 0; o >>= 1) {
         u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
-        if (PAIRS == 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+        v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
       }
+      return make_float2(u, v);
     }
-    return make_float2(u, v);
+    // the lower half of the warp adds up u, the upper one v: 7 exchanges instead of 10
+    const bool upper = lane & 16;
+    float t = upper ? v : u;
+    t += __shfl_xor_sync(0xFFFFFFFFu, upper ? u : v, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+    if constexpr (G > 32) {
+      float* r = reinterpret_cast<float*>(red + half * WARPS);
+      half ^= 1;
+      if (lane % 16 == 0) r[lane / 32 + (upper ? WARPS : 0)] = t;
+      asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(G) : "memory");
+      t = r[lane % WARPS + (upper ? WARPS : 0)];
+#pragma unroll
+      for (int o = WARPS / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+    }
+    return make_float2(__shfl_sync(0xFFFFFFFFu, t, 0), __shfl_sync(0xFFFFFFFFu, t, 16));
   }
 };
 
@@ -116,37 +121,47 @@ template <typename T, int V, int G>
 struct NormRows {
   static constexpr int K = NORM_E / V, THREADS = NormGroup<G>::THREADS;
   static constexpr int STAGE = V > 1 ? K * THREADS * 16 : 0;  // bytes of one row of every group
-  const T* row0;
-  int64_t stride;
-  int lane, n, last;
-  uint32_t ring;
-  const char* ring_ptr;
+  const T* p;     // the lane's first element of the next row to come
+  int64_t step;   // elements to the row after
+  int left;       // columns below n from the lane's first on
+  char* ring;
   T next[V > 1 ? 1 : NORM_E];
   __device__ static int c0(int k, int lane) { return (k * G + lane) * V; }
-  __device__ NormRows(const T* r0, int64_t stride_, int lane_, int n_, int last_, char* shared)
-      : row0(r0), stride(stride_), lane(lane_), n(n_), last(last_), ring(smem_u32(shared) + threadIdx.x * 16),
-        ring_ptr(shared + threadIdx.x * 16) {}
-  // Row r (the last one, where there is none) into stage `slot`.
-  __device__ void issue(int r, int slot) {
-    const T* row = row0 + min(r, last) * stride;
-    if constexpr (V > 1) {
+  // Rows first, first + by, ... of a member's `rows`.
+  __device__ NormRows(const T* rows, int64_t stride, int first, int by, int lane, int n, char* shared, int stages)
+      : p(rows + first * stride + lane * V), step(by * stride), left(n - lane * V), ring(shared + threadIdx.x * 16) {
+    if constexpr (V > 1) {  // vectors without a column are never copied
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (left - k * G * V <= 0)
+          for (int i = 0; i < stages; ++i)
+            *reinterpret_cast<uint4*>(ring + i * STAGE + k * THREADS * 16) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  // The next row, if there is one, into stage `slot`.
+  __device__ void issue(int slot, bool valid) {
+    if (valid) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = c0(k, lane), bytes = min(max((n - c) * (int)sizeof(T), 0), 16);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ring + slot * STAGE + k * THREADS * 16),
-                     "l"(bytes > 0 ? row + c : row), "r"(bytes)
-                     : "memory");
+        const int have = left - k * G * V;
+        if constexpr (V > 1) {
+          if (have > 0)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(ring) + slot * STAGE + k * THREADS * 16),
+                         "l"(p + k * G * V), "r"(min(have, V) * (int)sizeof(T))
+                         : "memory");
+        } else {
+          next[k] = have > 0 ? p[k * G] : from_f32<T>(0.f);
+        }
       }
-    } else {
-#pragma unroll
-      for (int k = 0; k < K; ++k) next[k] = c0(k, lane) < n ? row[c0(k, lane)] : from_f32<T>(0.f);
     }
+    p += step;
+    if (V > 1) cp_async_commit();
   }
   __device__ void take(int slot, f32x2 (&f)[NORM_H]) const {
     if constexpr (V > 1) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        norm_unpack<T, V>(*reinterpret_cast<const uint4*>(ring_ptr + slot * STAGE + k * THREADS * 16), f + k * V / 2);
+        norm_unpack<T, V>(*reinterpret_cast<const uint4*>(ring + slot * STAGE + k * THREADS * 16), f + k * V / 2);
     } else {
 #pragma unroll
       for (int k = 0; k < NORM_H; ++k) f[k] = pair(to_f32<T>(next[2 * k]), to_f32<T>(next[2 * k + 1]));
@@ -172,9 +187,9 @@ __device__ __forceinline__ float norm_add(const f32x2 (&f)[NORM_H]) {
   return t.x + t.y;
 }
 
-// Writes a lane's share of a row; `odd`: a row with a NaN, whose padding is not zero by itself.
+// Writes a lane's share of a row; `clear`: the padding is not zero by itself (a NaN in the row, say).
 template <typename T, int V, int G>
-__device__ __forceinline__ void norm_write(T* row, const f32x2 (&f)[NORM_H], int lane, int n, int W, bool odd) {
+__device__ __forceinline__ void norm_write(T* row, const f32x2 (&f)[NORM_H], int lane, int n, int W, bool clear) {
 #pragma unroll
   for (int k = 0; k < NORM_E / V; ++k) {
     const int c = (k * G + lane) * V;
@@ -189,7 +204,7 @@ __device__ __forceinline__ void norm_write(T* row, const f32x2 (&f)[NORM_H], int
         v[e] = t.x, v[e + 1] = t.y;
       }
     }
-    if (odd) {
+    if (clear && (k + 1) * G * V > n) {
 #pragma unroll
       for (int e = 0; e < V; ++e)
         if (c + e >= n) v[e] = 0.f;
@@ -234,7 +249,7 @@ __device__ __forceinline__ void norm_param(const float* p, int lane, int n, floa
   for (int h = 0; h < NORM_H; ++h) f[h] = pair(v[2 * h], v[2 * h + 1]);
 }
 
-// Stages of the ring, the current one included: two rows each forward, one backward.
+// Stages of the ring, the current one included: two rows each forward, one of x and dy backward.
 template <typename T, int V>
 struct NormDepth {
   static constexpr int FORWARD = V == 1 ? 1 : sizeof(T) == 2 ? 3 : 2;
@@ -253,34 +268,31 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
   const int m = blockIdx.x / a.S, split = blockIdx.x % a.S;
   const int n = norm_width(a, m), lane = grp.lane, step = a.S * Grp::GROUPS;
   const float inv_n = 1.0f / (float)max(n, 1);
-  // groups of one warp step together (their sums are warp-wide shuffles): rows beyond the last
-  // are computed again from the last and not written
+  // groups of one warp step together (their sums are warp-wide shuffles): rows beyond the last are
+  // computed from what the ring holds and not written
   const int first = split * Grp::GROUPS + grp.group;
   const int rounds = (a.B - split * Grp::GROUPS + 2 * step - 1) / (2 * step);
   const T* x0 = static_cast<const T*>(a.x) + m * a.xm;
-  Rows xa(x0, a.xr, lane, n, a.B - 1, ring), xb(x0, a.xr, lane, n, a.B - 1, ring + D * Rows::STAGE);
+  Rows xa(x0, a.xr, first, 2 * step, lane, n, ring, D);
+  Rows xb(x0, a.xr, first + step, 2 * step, lane, n, ring + D * Rows::STAGE, D);
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) {
-    xa.issue(first + 2 * i * step, i);
-    xb.issue(first + (2 * i + 1) * step, i);
-    if (V > 1) cp_async_commit();
+    xa.issue(i, first + 2 * i * step < a.B);
+    xb.issue(i, first + (2 * i + 1) * step < a.B);
   }
   f32x2 w[NORM_H], b[NORM_H], mask[NORM_H];
   norm_param<V, G>(a.w ? a.w + (size_t)m * a.W : nullptr, lane, n, 1.f, w);
   norm_param<V, G>(a.b ? a.b + (size_t)m * a.W : nullptr, lane, n, 0.f, b);
   norm_mask<V, G>(lane, n, mask);
-  for (int i = 0; i < rounds; ++i) {
-    const int r = first + 2 * i * step;
+  T* y = static_cast<T*>(a.y) + ((int64_t)m * a.B + first) * a.W;
+  for (int i = 0, r = first; i < rounds; ++i, r += 2 * step) {
     f32x2 f[2][NORM_H];
-    if (V > 1) cp_async_wait<(D > 1 ? D - 2 : 0)>();
+    if (V > 1) cp_async_wait<(D > 1 ? 2 * (D - 2) : 0)>();
     xa.take(i % D, f[0]);
     xb.take(i % D, f[1]);
-    if (i + AHEAD < rounds) {
-      xa.issue(r + 2 * AHEAD * step, (i + AHEAD) % D);
-      xb.issue(r + (2 * AHEAD + 1) * step, (i + AHEAD) % D);
-    }
-    if (V > 1) cp_async_commit();
-    const float2 sum = grp.template sum<2>(norm_add(f[0]), norm_add(f[1]));
+    xa.issue((i + AHEAD) % D, r + 2 * AHEAD * step < a.B);
+    xb.issue((i + AHEAD) % D, r + (2 * AHEAD + 1) * step < a.B);
+    const float2 sum = grp.sum(norm_add(f[0]), norm_add(f[1]));
     const float mean[2] = {sum.x * inv_n, sum.y * inv_n};
     float sq[2];
 #pragma unroll
@@ -295,21 +307,22 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
       const float2 t = halves(s);
       sq[q] = t.x + t.y;
     }
-    const float2 var = grp.template sum<2>(sq[0], sq[1]);
+    const float2 var = grp.sum(sq[0], sq[1]);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int row = r + q * step;
-      if (row >= a.B) continue;
-      const float rstd = rsqrtf((q ? var.y : var.x) * inv_n + a.eps);
-      const f32x2 rs = pair(rstd, rstd);
+      if (row < a.B) {
+        const float rstd = rsqrtf((q ? var.y : var.x) * inv_n + a.eps);
+        const f32x2 rs = pair(rstd, rstd);
 #pragma unroll
-      for (int h = 0; h < NORM_H; ++h) f[q][h] = fma2(mul2(f[q][h], rs), w[h], b[h]);
-      const int64_t at = (int64_t)m * a.B + row;
-      norm_write<T, V, G>(static_cast<T*>(a.y) + at * a.W, f[q], lane, n, a.W, !(rstd < INFINITY));
-      if (lane == 0) {
-        a.mean[at] = mean[q];
-        a.rstd[at] = rstd;
+        for (int h = 0; h < NORM_H; ++h) f[q][h] = fma2(mul2(f[q][h], rs), w[h], b[h]);
+        norm_write<T, V, G>(y, f[q], lane, n, a.W, !(rstd < INFINITY));
+        if (lane == 0) {
+          a.mean[(int64_t)m * a.B + row] = mean[q];
+          a.rstd[(int64_t)m * a.B + row] = rstd;
+        }
       }
+      y += (int64_t)step * a.W;
     }
   }
 }
@@ -329,49 +342,45 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
   const float inv_n = 1.0f / (float)max(n, 1);
   const int first = split * Grp::GROUPS + grp.group;
   const int rounds = (a.B - split * Grp::GROUPS + step - 1) / step;
-  Rows x(static_cast<const T*>(a.x) + m * a.xm, a.xr, lane, n, a.B - 1, ring);
-  Rows dy(static_cast<const T*>(a.dy) + m * a.dym, a.dyr, lane, n, a.B - 1, ring + D * Rows::STAGE);
+  Rows x(static_cast<const T*>(a.x) + m * a.xm, a.xr, first, step, lane, n, ring, D);
+  Rows dy(static_cast<const T*>(a.dy) + m * a.dym, a.dyr, first, step, lane, n, ring + D * Rows::STAGE, D);
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) {
-    x.issue(first + i * step, i);
-    dy.issue(first + i * step, i);
-    if (V > 1) cp_async_commit();
+    x.issue(i, first + i * step < a.B);
+    dy.issue(i, first + i * step < a.B);
   }
-  const float* mean = a.mean + (int64_t)m * a.B;
-  const float* rstd = a.rstd + (int64_t)m * a.B;
-  float nmean = mean[min(first, a.B - 1)], nrstd = rstd[min(first, a.B - 1)];
-  f32x2 w[NORM_H], sw[NORM_H], sb[NORM_H], mask[NORM_H];
+  const float* mean = a.mean + (int64_t)m * a.B + first;
+  const float* rstd = a.rstd + (int64_t)m * a.B + first;
+  float nmean = 0.f, nrstd = 0.f;
+  if (first < a.B) nmean = *mean, nrstd = *rstd;
+  f32x2 w[NORM_H], sw[NORM_H], sb[NORM_H];
   norm_param<V, G>(a.w ? a.w + (size_t)m * a.W : nullptr, lane, n, 1.f, w);
-  norm_mask<V, G>(lane, n, mask);
 #pragma unroll
   for (int h = 0; h < NORM_H; ++h) sw[h] = sb[h] = pair(0.f, 0.f);
-  for (int i = 0; i < rounds; ++i) {
-    const int r = first + i * step;
+  const bool dx_f32 = sizeof(T) == 2 && a.dx_f32;
+  char* dx = static_cast<char*>(a.dx) + ((int64_t)m * a.B + first) * a.W * (dx_f32 ? 4 : sizeof(T));
+  const int64_t dx_step = (int64_t)step * a.W * (dx_f32 ? 4 : sizeof(T));
+  for (int i = 0, r = first; i < rounds; ++i, r += step, dx += dx_step) {
     f32x2 xh[NORM_H], g[NORM_H];
-    if (V > 1) cp_async_wait<(D > 1 ? D - 2 : 0)>();
+    if (V > 1) cp_async_wait<(D > 1 ? 2 * (D - 2) : 0)>();
     x.take(i % D, xh);
     dy.take(i % D, g);
     const float mu = nmean, rs = nrstd;
-    if (i + 1 < rounds) {
-      const int to = min(r + step, a.B - 1);
-      nmean = mean[to];
-      nrstd = rstd[to];
-    }
-    if (i + AHEAD < rounds) {
-      x.issue(r + AHEAD * step, (i + AHEAD) % D);
-      dy.issue(r + AHEAD * step, (i + AHEAD) % D);
-    }
-    if (V > 1) cp_async_commit();
+    mean += step;
+    rstd += step;
+    if (r + step < a.B) nmean = *mean, nrstd = *rstd;
+    x.issue((i + AHEAD) % D, r + AHEAD * step < a.B);
+    dy.issue((i + AHEAD) % D, r + AHEAD * step < a.B);
     const bool live = r < a.B;
     if (!live) {
 #pragma unroll
-      for (int h = 0; h < NORM_H; ++h) g[h] = pair(0.f, 0.f);
+      for (int h = 0; h < NORM_H; ++h) g[h] = xh[h] = pair(0.f, 0.f);
     }
     const f32x2 minus = pair(-mu, -mu), scale = pair(rs, rs);
     f32x2 s1 = pair(0.f, 0.f), s2 = s1;
 #pragma unroll
-    for (int h = 0; h < NORM_H; ++h) {  // xhat and dy are 0 from column n on
-      xh[h] = mul2(fma2(mask[h], minus, xh[h]), scale);
+    for (int h = 0; h < NORM_H; ++h) {  // dy is 0 from column n on
+      xh[h] = mul2(add2(xh[h], minus), scale);
       sw[h] = fma2(g[h], xh[h], sw[h]);
       sb[h] = add2(sb[h], g[h]);
       g[h] = mul2(g[h], w[h]);
@@ -380,17 +389,16 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
     }
     if (a.dx == nullptr) continue;
     const float2 u = halves(s1), v = halves(s2);
-    const float2 t = grp.template sum<2>(u.x + u.y, v.x + v.y);
+    const float2 t = grp.sum(u.x + u.y, v.x + v.y);
     if (!live) continue;
     const f32x2 c1 = pair(-t.x * inv_n, -t.x * inv_n), c2 = pair(-t.y * inv_n, -t.y * inv_n);
 #pragma unroll
-    for (int h = 0; h < NORM_H; ++h) g[h] = mul2(fma2(xh[h], c2, fma2(mask[h], c1, g[h])), scale);
-    const int64_t at = ((int64_t)m * a.B + r) * a.W;
-    const bool odd = !(fabsf(t.x) + fabsf(t.y) < INFINITY && rs < INFINITY);
-    if (sizeof(T) == 2 && a.dx_f32)
-      norm_write<float, V, G>(static_cast<float*>(a.dx) + at, g, lane, n, a.W, odd);
+    for (int h = 0; h < NORM_H; ++h) g[h] = mul2(fma2(xh[h], c2, add2(g[h], c1)), scale);
+    const bool ragged = n < a.W;
+    if (dx_f32)
+      norm_write<float, V, G>(reinterpret_cast<float*>(dx), g, lane, n, a.W, ragged);
     else
-      norm_write<T, V, G>(static_cast<T*>(a.dx) + at, g, lane, n, a.W, odd);
+      norm_write<T, V, G>(reinterpret_cast<T*>(dx), g, lane, n, a.W, ragged);
   }
   if (!a.dw && !a.db) return;
   // the block's groups in ascending order, then (with several splits) the finishing kernel
