@@ -405,35 +405,48 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
   const size_t row = ((size_t)m * a.S + split) * a.W;
   float* ow = a.S > 1 ? a.partial + row : a.dw ? a.dw + row : nullptr;
   float* ob = a.S > 1 ? a.partial + (size_t)a.P * a.S * a.W + row : a.db ? a.db + row : nullptr;
+  if constexpr (Grp::GROUPS > 1) {
+    float* cols = reinterpret_cast<float*>(ring);  // dw of every group's columns, then db
+    constexpr int HALF = Grp::THREADS * NORM_E;
+    if (V > 1) cp_async_wait<0>();
+    __syncthreads();
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    float s[NORM_E];
+    for (int k = 0; k < NORM_E / V; ++k) {
+      float* to = cols + grp.group * G * NORM_E + Rows::c0(k, lane);
+      if constexpr (V == 1) {
+        const float2 u = halves(sw[k / 2]), v = halves(sb[k / 2]);
+        to[0] = k % 2 ? u.y : u.x;
+        to[HALF] = k % 2 ? v.y : v.x;
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+          const int h = (k * V + e) / 2;
+          const float2 u = halves(sw[h]), u2 = halves(sw[h + 1]), v = halves(sb[h]), v2 = halves(sb[h + 1]);
+          *reinterpret_cast<float4*>(to + e) = make_float4(u.x, u.y, u2.x, u2.y);
+          *reinterpret_cast<float4*>(to + HALF + e) = make_float4(v.x, v.y, v2.x, v2.y);
+        }
+      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < min(G * NORM_E, a.W); c += Grp::THREADS) {
+      float u = 0.f, v = 0.f;
+#pragma unroll 8
+      for (int i = 0; i < Grp::GROUPS; ++i) {
+        u += cols[i * G * NORM_E + c];
+        v += cols[HALF + i * G * NORM_E + c];
+      }
+      if (ow) ow[c] = c < n ? u : 0.f;
+      if (ob) ob[c] = c < n ? v : 0.f;
+    }
+  } else {
 #pragma unroll
     for (int h = 0; h < NORM_H; ++h) {
-      const float2 t = halves(which ? sb[h] : sw[h]);
-      s[2 * h] = t.x, s[2 * h + 1] = t.y;
-    }
-    float* o = which ? ob : ow;
-    if constexpr (Grp::GROUPS > 1) {
-      float* cols = reinterpret_cast<float*>(ring);  // a group's columns in a row
-      if (V > 1) cp_async_wait<0>();
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < NORM_E; ++j)
-        cols[grp.group * G * NORM_E + Rows::c0(j / V, lane) + j % V] = Rows::c0(j / V, lane) + j % V < n ? s[j] : 0.f;
-      __syncthreads();
-      for (int c = threadIdx.x; c < min(G * NORM_E, a.W); c += Grp::THREADS) {
-        float t = 0.f;
-#pragma unroll 8
-        for (int i = 0; i < Grp::GROUPS; ++i) t += cols[i * G * NORM_E + c];
-        if (o) o[c] = t;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NORM_E; ++j) {
-        const int c = Rows::c0(j / V, lane) + j % V;
-        if (o && c < a.W) o[c] = c < n ? s[j] : 0.f;
-      }
+      const int c = Rows::c0(2 * h / V, lane) + 2 * h % V, d = V == 1 ? c + G : c + 1;
+      const float2 u = halves(sw[h]), v = halves(sb[h]);
+      if (ow && c < a.W) ow[c] = c < n ? u.x : 0.f;
+      if (ow && d < a.W) ow[d] = d < n ? u.y : 0.f;
+      if (ob && c < a.W) ob[c] = c < n ? v.x : 0.f;
+      if (ob && d < a.W) ob[d] = d < n ? v.y : 0.f;
     }
   }
 }

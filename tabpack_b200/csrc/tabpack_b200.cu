@@ -1774,7 +1774,7 @@ int launch_norm(LayerNormArgs k, bool backward, cudaStream_t st) {
   const unsigned blocks = (unsigned)k.P * k.S;
   constexpr size_t stage = NormRows<T, V, G>::STAGE;
   if (backward) {
-    constexpr size_t cols = Grp::GROUPS > 1 ? Grp::THREADS * NORM_E * sizeof(float) : 0;
+    constexpr size_t cols = Grp::GROUPS > 1 ? 2 * Grp::THREADS * NORM_E * sizeof(float) : 0;
     constexpr size_t bytes = std::max<size_t>(2 * NormDepth<T, V>::BACKWARD * stage, cols);
     if (int rc = allow_shared<layer_norm_held_backward_kernel<T, V, G>>(bytes)) return rc;
     layer_norm_held_backward_kernel<T, V, G><<<blocks, Grp::THREADS, bytes, st>>>(k);
