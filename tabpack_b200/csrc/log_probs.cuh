@@ -33,7 +33,7 @@ struct LogProbsArgs {
   int64_t ld;              // row stride of the logits
   const void* logits;
   const int64_t* labels;
-  int64_t label_rows;      // row r has label r % label_rows
+  uint32_t label_rows;     // row r has label r % label_rows; 0: its own
   int64_t ignore_index;
   int k;
   float* log_prob;
@@ -151,6 +151,11 @@ struct Row {
   }
 };
 
+// A row's label, loaded before the row is reduced.
+__device__ __forceinline__ int64_t row_label(const LogProbsArgs& a, int64_t row) {
+  return a.labels[a.label_rows ? (uint32_t)row % a.label_rows : (uint32_t)row];
+}
+
 struct RowStats {
   float m, L, H;  // m = -inf and L = 0: no classes
   __device__ bool empty() const { return m == -INFINITY && L == 0.f; }
@@ -165,13 +170,20 @@ __device__ __forceinline__ RowStats row_stats(float m, float s, float t) {
 }
 
 // What the row's leader writes.
-template <typename T>
-__device__ __forceinline__ void write_row(const LogProbsArgs& a, int64_t row, const T* z, const RowStats& st) {
-  const int64_t y = a.labels[row % a.label_rows];
-  float lp = 0.f;
-  if (y != a.ignore_index)
-    lp = (y < 0 || y >= a.C) ? lp_nan() : st.empty() ? -INFINITY : to_f32<T>(z[y]) - st.m - st.L;
-  a.log_prob[row] = lp;
+struct RowLabel {
+  float z;        // the label's score
+  bool in, skip;  // a class of the row; equal to ignore_index
+  template <typename T>
+  __device__ RowLabel(const LogProbsArgs& a, int64_t row, const T* scores) {
+    const int64_t y = row_label(a, row);
+    skip = y == a.ignore_index;
+    in = y >= 0 && y < a.C;
+    z = in ? to_f32<T>(scores[y]) : 0.f;
+  }
+};
+
+__device__ __forceinline__ void write_row(const LogProbsArgs& a, int64_t row, const RowLabel& y, const RowStats& st) {
+  a.log_prob[row] = y.skip ? 0.f : !y.in ? lp_nan() : st.empty() ? -INFINITY : y.z - st.m - st.L;
   a.entropy[row] = st.H;
   if (a.C > LP_REREAD) {
     a.stats[3 * row] = st.m;
@@ -193,11 +205,22 @@ struct RowGrad {
   int y;             // -1: no label's term
 };
 
-__device__ __forceinline__ RowGrad row_grad(const LogProbsArgs& a, int64_t row, const RowStats& st) {
+// What a row's gradient takes besides its scores, loaded before the row is reduced.
+struct RowUpstream {
+  int64_t y;
+  float gl, gh;
+  __device__ RowUpstream(const LogProbsArgs& a, int64_t row) {
+    y = row_label(a, row);
+    gl = a.g_l ? a.g_l[row * a.g_l_stride] : 0.f;
+    gh = a.g_h ? a.g_h[row * a.g_h_stride] : 0.f;
+  }
+};
+
+__device__ __forceinline__ RowGrad row_grad(const LogProbsArgs& a, const RowUpstream& up, const RowStats& st) {
   RowGrad g;
-  const int64_t y = a.labels[row % a.label_rows];
-  g.gl = a.g_l ? a.g_l[row * a.g_l_stride] : 0.f;
-  const float gh = a.g_h ? a.g_h[row * a.g_h_stride] : 0.f;
+  const int64_t y = up.y;
+  const float gh = up.gh;
+  g.gl = up.gl;
   g.y = -1;
   if (!a.g_l || y == a.ignore_index)
     g.gl = 0.f;
@@ -388,12 +411,13 @@ __global__ void __launch_bounds__(256) log_probs_held_forward_kernel(const LogPr
   const int lane = threadIdx.x & (G - 1);
   const T* z = static_cast<const T*>(a.logits) + row * a.ld;
   const Row<T> r(z, a.C);
+  const RowLabel label(a, row, z);
   HeldRow<T, G, E> h;
   h.load(r, lane);
   const float own = h.own_max();
   const RowStats st = h.stats(own);
   const bool mine = lane == 0 && at < a.rows;
-  if (mine) write_row<T>(a, row, z, st);
+  if (mine) write_row(a, row, label, st);
   if constexpr (TOP) {
     // a round per class costs 25 + 3 E instructions, the sorts some 300 in all
     if (G < 32 || (E == 8 && a.k <= 8)) {
@@ -454,10 +478,11 @@ __global__ void __launch_bounds__(256) log_probs_held_backward_kernel(const LogP
   const int64_t row = min(at, a.rows - 1);
   const int lane = threadIdx.x & (G - 1);
   const Row<T> r(static_cast<const T*>(a.logits) + row * a.ld, a.C);
+  const RowUpstream up(a, row);
   HeldRow<T, G, E> h;
   h.load(r, lane);
   const RowStats st = h.stats(h.own_max());
-  const RowGrad g = row_grad(a, row, st);
+  const RowGrad g = row_grad(a, up, st);
   constexpr int V = Row<T>::V;
   if constexpr (G == 1) {
     // the warp's 32 rows are one piece of dlogits: gather them in shared memory and write it in words
@@ -625,7 +650,7 @@ __global__ void __launch_bounds__(1024) log_probs_long_forward_kernel(const LogP
   s1 = group_sum<32>(lane_id() < warps ? red[1][lane_id()] : 0.f);
   t1 = group_sum<32>(lane_id() < warps ? red[2][lane_id()] : 0.f);
   const RowStats st = row_stats(bm, s1, t1);
-  if (lane_id() == 0) write_row<T>(a, row, z, st);
+  if (lane_id() == 0) write_row(a, row, RowLabel(a, row, z), st);
   if (TOP && lane_id() < a.k)
     write_best(a, row, lane_id(), (uint32_t)(best.key >> 32), (uint32_t)~(uint32_t)best.key, st);
 }
@@ -634,18 +659,18 @@ __global__ void __launch_bounds__(1024) log_probs_long_forward_kernel(const LogP
 template <typename T>
 __global__ void __launch_bounds__(256) log_probs_stream_backward_kernel(const LogProbsArgs a, int chunks) {
   constexpr int V = Row<T>::V, U = LP_CHUNK / (32 * V);
-  const int64_t task = (int64_t)blockIdx.x * 8 + warp_id();
-  const int64_t row = task / chunks;
+  const uint32_t task = blockIdx.x * 8 + warp_id();
+  const uint32_t row = task / (uint32_t)chunks;
   if (row >= a.rows) return;
-  const int i0 = (int)(task % chunks) * (LP_CHUNK / V) + lane_id();
-  const Row<T> r(static_cast<const T*>(a.logits) + row * a.ld, a.C);
-  T* out = static_cast<T*>(a.dlogits) + row * a.C;
+  const int i0 = (int)(task % (uint32_t)chunks) * (LP_CHUNK / V) + lane_id();
+  const Row<T> r(static_cast<const T*>(a.logits) + (int64_t)row * a.ld, a.C);
+  T* out = static_cast<T*>(a.dlogits) + (int64_t)row * a.C;
   const int nv = r.vectors();
   RowStats st;
-  st.m = a.stats[3 * row];
-  st.L = a.stats[3 * row + 1];
-  st.H = a.stats[3 * row + 2];
-  const RowGrad g = row_grad(a, row, st);
+  st.m = a.stats[3 * (int64_t)row];
+  st.L = a.stats[3 * (int64_t)row + 1];
+  st.H = a.stats[3 * (int64_t)row + 2];
+  const RowGrad g = row_grad(a, RowUpstream(a, row), st);
   for (int u0 = 0; u0 < U; u0 += 4) {
     uint4 raw[4];
 #pragma unroll

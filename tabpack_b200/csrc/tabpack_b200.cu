@@ -1914,7 +1914,7 @@ static LogProbsArgs label_log_probs_args(const tp_label_log_probs_args* a) {
   k.ld = a->logits_stride;
   k.logits = a->logits;
   k.labels = a->labels;
-  k.label_rows = a->label_rows;
+  k.label_rows = a->label_rows == a->rows ? 0u : (uint32_t)a->label_rows;
   k.ignore_index = a->ignore_index;
   k.k = a->top_k;
   k.log_prob = a->log_prob;
@@ -1961,11 +1961,12 @@ void launch_log_probs(const LogProbsArgs& k, int held, cudaStream_t st) {
 }
 
 template <typename T>
-void launch_log_probs_backward(const LogProbsArgs& k, int held, cudaStream_t st) {
+int launch_log_probs_backward(const LogProbsArgs& k, int held, cudaStream_t st) {
   const auto blocks = [&](int lanes) { return (unsigned)((k.rows * lanes + 255) / 256); };
   if (k.C > LP_REREAD) {
     constexpr int V = 16 / sizeof(T);
     const int chunks = (k.C + V - 1 + LP_CHUNK - 1) / LP_CHUNK;
+    if (k.rows * chunks > 0xFFFFFFF0ll) return fail(TP_EINVAL, "too many scores for one call");
     log_probs_stream_backward_kernel<T><<<(unsigned)((k.rows * chunks + 7) / 8), 256, 0, st>>>(k, chunks);
   } else if (held <= 16) {
     log_probs_held_backward_kernel<T, 1, 16><<<blocks(1), 256, 0, st>>>(k);
@@ -1976,6 +1977,7 @@ void launch_log_probs_backward(const LogProbsArgs& k, int held, cudaStream_t st)
   } else {
     log_probs_held_backward_kernel<T, 32, 16><<<blocks(32), 256, 0, st>>>(k);
   }
+  return TP_OK;
 }
 
 }  // namespace
@@ -2019,10 +2021,8 @@ int tp_label_log_probs_backward(const tp_label_log_probs_args* a, void* stream) 
   if (reinterpret_cast<uintptr_t>(a->dlogits) % (bf16 ? 2 : 4) != 0)
     return fail(TP_EALIGN, "the logits gradient is not aligned to its type");
   const int held = held_size(a, bf16 ? 2 : 4);
-  if (bf16)
-    launch_log_probs_backward<__nv_bfloat16>(k, held, st);
-  else
-    launch_log_probs_backward<float>(k, held, st);
+  rc = bf16 ? launch_log_probs_backward<__nv_bfloat16>(k, held, st) : launch_log_probs_backward<float>(k, held, st);
+  if (rc) return rc;
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;
 }
