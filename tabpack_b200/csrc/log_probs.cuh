@@ -11,8 +11,10 @@
 // row with nothing but -inf has S = 0 and is told by that: log p = -inf, H = 0, no gradient.
 //
 // Memory bounds these kernels: 2 or 4 bytes a class against 8 to 12 instructions.  Rows of up
-// to 1024 classes are held in registers by a thread (16), 8 lanes (64) or a warp (256, 1024), so the
-// row is read once and the softmax takes its maximum first; longer rows take one block and one pass
+// to 1024 classes are held in registers, 16 scores a lane (32 from 512 classes on) of a thread, 4, 8,
+// 16 or 32 lanes, so the row is read once and the softmax takes its maximum first (a row's fixed cost,
+// reductions and label, is paid once per group: 8 scores a lane took half again as long on 50 and 200
+// classes); longer rows take one block and one pass
 // with a running maximum, the next 64 bytes of each thread on their way meanwhile.  Rows start anywhere:
 // whole 16-byte vectors are loaded between the first and last boundary inside the row, single elements
 // before and after.
@@ -236,14 +238,14 @@ __device__ __forceinline__ RowGrad row_grad(const LogProbsArgs& a, const RowUpst
   return g;
 }
 
-// In place, V scores from class c0 on.
-template <int V>
-__device__ __forceinline__ void score_grad(const RowGrad& g, float (&z)[V], int c0) {
+// In place, V scores from class c0 on; `known`: their probabilities, where they are at hand.
+template <int V, bool KNOWN>
+__device__ __forceinline__ void score_grad(const RowGrad& g, float (&z)[V], int c0, const float* known) {
 #pragma unroll
   for (int e = 0; e < V; e += 2) {
     // a masked class: p = 0 and a finite log p, so that its product is 0
     const f32x2 lp = bounded2(add2(add2(pair(z[e], z[e + 1]), g.m), g.L));
-    const float2 d = halves(mul2(exp_neg2(lp), fma2(g.b, lp, g.a)));
+    const float2 d = halves(mul2(KNOWN ? pair(known[e], known[e + 1]) : exp_neg2(lp), fma2(g.b, lp, g.a)));
     z[e] = d.x, z[e + 1] = d.y;
   }
   if ((unsigned)(g.y - c0) < (unsigned)V && g.y >= 0) {
@@ -254,7 +256,7 @@ __device__ __forceinline__ void score_grad(const RowGrad& g, float (&z)[V], int 
 }
 
 // ---------------------------------------------------------------------------
-// Rows in registers: G lanes (1, 8 or 32) hold E scores each, vectors of the row in turn.
+// Rows in registers: G lanes (1 to 32) hold E scores each, vectors of the row in turn.
 // ---------------------------------------------------------------------------
 template <int G>
 __device__ __forceinline__ float group_max(float v) {
@@ -287,7 +289,9 @@ struct HeldRow {
     for (int j = 0; j < E; ++j) m = fmaxf(m, z[j]);
     return m;
   }
-  __device__ RowStats stats(float own) const {
+  // KEEP: leaves exp(z - max) / S in `p`.
+  template <bool KEEP = false>
+  __device__ RowStats stats(float own, float* p = nullptr) const {
     const float m = group_max<G>(own);
     const float m0 = m == -INFINITY ? 0.f : -m;
     f32x2 s = pair(0.f, 0.f), t = s;
@@ -296,9 +300,19 @@ struct HeldRow {
       const f32x2 d = bounded2(add2(pair(z[j], z[j + 1]), pair(m0, m0))), e = exp_neg2(d);
       s = add2(s, e);
       t = fma2(e, d, t);
+      if constexpr (KEEP) {
+        const float2 f = halves(e);
+        p[j] = f.x, p[j + 1] = f.y;
+      }
     }
     const float2 a = halves(s), b = halves(t);
-    return row_stats(m, group_sum<G>(a.x + a.y), group_sum<G>(b.x + b.y));
+    const float sum = group_sum<G>(a.x + a.y);
+    if constexpr (KEEP) {
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+      for (int j = 0; j < E; ++j) p[j] *= inv;
+    }
+    return row_stats(m, sum, group_sum<G>(b.x + b.y));
   }
   __device__ static int at(const Row<T>& r, int lane, int j) { return r.first((j / V) * G + lane) + j % V; }
 };
@@ -419,8 +433,7 @@ __global__ void __launch_bounds__(256) log_probs_held_forward_kernel(const LogPr
   const bool mine = lane == 0 && at < a.rows;
   if (mine) write_row(a, row, label, st);
   if constexpr (TOP) {
-    // a round per class costs 25 + 3 E instructions, the sorts some 300 in all
-    if (G < 32 || (E == 8 && a.k <= 8)) {
+    if constexpr (G < 32) {
       // k rounds: the lanes' best unused classes, then the group's; its lane looks for its next best
       uint32_t order[E];
       uint32_t best = 0, where = 0xFFFFFFFFu;
@@ -432,15 +445,10 @@ __global__ void __launch_bounds__(256) log_probs_held_forward_kernel(const LogPr
       }
       for (int i = 0; i < a.k; ++i) {
         uint32_t b = best, w = where;
-        if constexpr (G == 32) {
-          b = __reduce_max_sync(0xFFFFFFFFu, best);
-          w = __reduce_min_sync(0xFFFFFFFFu, best == b ? where : 0xFFFFFFFFu);
-        } else {
 #pragma unroll
-          for (int o = G / 2; o > 0; o >>= 1) {
-            const uint32_t bo = __shfl_xor_sync(0xFFFFFFFFu, b, o), wo = __shfl_xor_sync(0xFFFFFFFFu, w, o);
-            if (bo > b || (bo == b && wo < w)) b = bo, w = wo;
-          }
+        for (int o = G / 2; o > 0; o >>= 1) {
+          const uint32_t bo = __shfl_xor_sync(0xFFFFFFFFu, b, o), wo = __shfl_xor_sync(0xFFFFFFFFu, w, o);
+          if (bo > b || (bo == b && wo < w)) b = bo, w = wo;
         }
         if (mine) write_best(a, row, i, b, w, st);
         if (w == where) {
@@ -454,7 +462,7 @@ __global__ void __launch_bounds__(256) log_probs_held_forward_kernel(const LogPr
           }
         }
       }
-    } else if constexpr (G == 32) {
+    } else {
       __shared__ class_key buf[8][LP_CANDIDATES];
       __shared__ int count[8];
       if (lane == 0) count[warp_id()] = 0;
@@ -481,48 +489,53 @@ __global__ void __launch_bounds__(256) log_probs_held_backward_kernel(const LogP
   const RowUpstream up(a, row);
   HeldRow<T, G, E> h;
   h.load(r, lane);
-  const RowStats st = h.stats(h.own_max());
+  float p[E];
+  const RowStats st = h.template stats<true>(h.own_max(), p);
   const RowGrad g = row_grad(a, up, st);
   constexpr int V = Row<T>::V;
-  if constexpr (G == 1) {
-    // the warp's 32 rows are one piece of dlogits: gather them in shared memory and write it in words
-    __shared__ __align__(16) T stage[8][32 * E];
-    T* mine = stage[warp_id()];
-#pragma unroll
-    for (int j = 0; j < E / V; ++j) {
-      float d[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) d[e] = h.z[j * V + e];
-      const int c0 = h.at(r, lane, j * V);
-      score_grad<V>(g, d, c0);
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (c0 + e >= 0 && c0 + e < a.C) mine[lane_id() * a.C + c0 + e] = from_f32<T>(d[e]);
-    }
-    __syncwarp();
-    const int64_t row0 = at - lane_id();
-    const int n = (int)min((int64_t)32, a.rows - row0) * a.C;
-    if (n <= 0) return;
-    T* out = static_cast<T*>(a.dlogits) + row0 * a.C;  // 32 rows: whole 4-byte words from an aligned dlogits
-    constexpr int PER = 4 / sizeof(T);
-    if ((reinterpret_cast<uintptr_t>(out) & 3u) == 0) {
-      for (int i = lane_id(); i < n / PER; i += 32)
-        reinterpret_cast<uint32_t*>(out)[i] = reinterpret_cast<const uint32_t*>(mine)[i];
-      for (int i = n / PER * PER + lane_id(); i < n; i += 32) out[i] = mine[i];
-    } else {
-      for (int i = lane_id(); i < n; i += 32) out[i] = mine[i];
-    }
-  } else {
+  T* out = static_cast<T*>(a.dlogits) + row * a.C;
+  // the same for every row: a warp's groups stay together
+  const bool aligned = a.C % V == 0 && a.ld % V == 0 &&
+                       ((reinterpret_cast<uintptr_t>(a.dlogits) | reinterpret_cast<uintptr_t>(a.logits)) & 15u) == 0;
+  if (G == 32 || (G > 1 && aligned)) {
     if (at >= a.rows) return;
-    T* out = static_cast<T*>(a.dlogits) + row * a.C;
 #pragma unroll
     for (int j = 0; j < E / V; ++j) {
       float d[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) d[e] = h.z[j * V + e];
-      score_grad<V>(g, d, r.first(j * G + lane));
+      score_grad<V, true>(g, d, r.first(j * G + lane), p + j * V);
       r.store(out, j * G + lane, d);
     }
+  } else if constexpr (G < 32) {
+    // short rows that begin anywhere: the warp's rows are one piece of dlogits, gathered in shared
+    // memory and written 16 bytes at a time
+    __shared__ __align__(16) T stage[8][32 * E];
+    T* mine = stage[warp_id()];
+    const int slot = lane_id() / G;
+#pragma unroll
+    for (int j = 0; j < E / V; ++j) {
+      float d[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[e] = h.z[j * V + e];
+      const int c0 = r.first(j * G + lane);
+      score_grad<V, true>(g, d, c0, p + j * V);
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (c0 + e >= 0 && c0 + e < a.C) mine[slot * a.C + c0 + e] = from_f32<T>(d[e]);
+    }
+    __syncwarp();
+    const int64_t row0 = at - slot;
+    const int n = (int)max((int64_t)0, min((int64_t)(32 / G), a.rows - row0)) * a.C;
+    out = static_cast<T*>(a.dlogits) + row0 * a.C;
+    int i = 0;
+    if ((reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
+      for (; i + V <= n; i += V * 32)
+        if (i + V * (lane_id() + 1) <= n)
+          reinterpret_cast<uint4*>(out + i)[lane_id()] = reinterpret_cast<const uint4*>(mine + i)[lane_id()];
+      i = n / V * V;
+    }
+    for (i += lane_id(); i < n; i += 32) out[i] = mine[i];
   }
 }
 
@@ -684,7 +697,7 @@ __global__ void __launch_bounds__(256) log_probs_stream_backward_kernel(const Lo
       if (i >= nv) return;
       float d[V];
       Row<T>::unpack(raw[u], d);
-      score_grad<V>(g, d, r.first(i));
+      score_grad<V, false>(g, d, r.first(i), nullptr);
       r.store(out, i, d);
     }
   }

@@ -1948,9 +1948,13 @@ void launch_log_probs(const LogProbsArgs& k, int held, cudaStream_t st) {
   if (held <= 16) {
     log_probs_held_forward_kernel<T, 1, 16, TOP><<<blocks(1), 256, 0, st>>>(k);
   } else if (held <= 64) {
-    log_probs_held_forward_kernel<T, 8, 8, TOP><<<blocks(8), 256, 0, st>>>(k);
+    log_probs_held_forward_kernel<T, 4, 16, TOP><<<blocks(4), 256, 0, st>>>(k);
+  } else if (held <= 128) {
+    log_probs_held_forward_kernel<T, 8, 16, TOP><<<blocks(8), 256, 0, st>>>(k);
   } else if (held <= 256) {
-    log_probs_held_forward_kernel<T, 32, 8, TOP><<<blocks(32), 256, 0, st>>>(k);
+    log_probs_held_forward_kernel<T, 16, 16, TOP><<<blocks(16), 256, 0, st>>>(k);
+  } else if (held <= 512) {
+    log_probs_held_forward_kernel<T, 32, 16, TOP><<<blocks(32), 256, 0, st>>>(k);
   } else if (held <= 1024) {
     log_probs_held_forward_kernel<T, 32, 32, TOP><<<blocks(32), 256, 0, st>>>(k);
   } else {
@@ -1971,9 +1975,11 @@ int launch_log_probs_backward(const LogProbsArgs& k, int held, cudaStream_t st) 
   } else if (held <= 16) {
     log_probs_held_backward_kernel<T, 1, 16><<<blocks(1), 256, 0, st>>>(k);
   } else if (held <= 64) {
-    log_probs_held_backward_kernel<T, 8, 8><<<blocks(8), 256, 0, st>>>(k);
+    log_probs_held_backward_kernel<T, 4, 16><<<blocks(4), 256, 0, st>>>(k);
+  } else if (held <= 128) {
+    log_probs_held_backward_kernel<T, 8, 16><<<blocks(8), 256, 0, st>>>(k);
   } else if (held <= 256) {
-    log_probs_held_backward_kernel<T, 32, 8><<<blocks(32), 256, 0, st>>>(k);
+    log_probs_held_backward_kernel<T, 16, 16><<<blocks(16), 256, 0, st>>>(k);
   } else {
     log_probs_held_backward_kernel<T, 32, 16><<<blocks(32), 256, 0, st>>>(k);
   }

@@ -94,7 +94,7 @@ def run_and_check(z, y, g_l, g_h, k=0):
         assert top is None and which is None
 
 
-CLASSES = [1, 2, 3, 8, 10, 31, 32, 33, 64, 100, 255, 256, 257, 500, 1000, 1023, 1024, 1025, 2048, 2051, 5000, 16384,
+CLASSES = [1, 2, 3, 8, 10, 16, 17, 31, 32, 33, 64, 65, 100, 128, 129, 255, 256, 257, 500, 512, 513, 1000, 1023, 1024, 1025, 2048, 2051, 5000, 16384,
            32769, 51200, 131072, 200003]
 
 
@@ -218,6 +218,14 @@ def test_ignored_and_invalid_labels(C):
 @pytest.mark.parametrize('C,ld', [(10, 16), (9, 16), (33, 40), (1000, 1001), (3001, 3008)])
 def test_rows_of_padded_buffers(C, ld, dtype):
     run_and_check(*make((3, 7), C, dtype, seed=C, ld=ld), k=min(5, C))
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('C', [16, 24, 40, 64, 96, 128, 200, 256])
+def test_rows_on_different_boundaries(C, dtype):
+    """Whole vectors per row, but a stride that starts the rows of one warp on different boundaries."""
+    run_and_check(*make((2, 37), C, dtype, seed=C, ld=C + 1), k=min(5, C))
+    run_and_check(*make((2, 37), C, dtype, seed=C, ld=C + 4))
 
 
 def test_unaligned_storage_and_strided_rows():
