@@ -841,6 +841,8 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq
         used += 1
         a.n_tensors = used
     hp = [_hparam(v) for v in hp]
+    if len({p.data_ptr() for p in params if p.numel()}) < sum(1 for p in params if p.numel()):
+        raise ValueError('a parameter appears twice')
     # every argument is checked before the first launch
     for a in calls:
         a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = hp

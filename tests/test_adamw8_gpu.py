@@ -296,6 +296,8 @@ def test_refusals():
         call(p, g, *st, step=0)
     with pytest.raises(ValueError):
         call(p, [], *st)
+    with pytest.raises(ValueError):
+        call(p * 2, g * 2, *(t * 2 for t in st))
     with pytest.raises(TypeError):
         call([p[0].double()], g, *st)
     with pytest.raises(TypeError):

@@ -26,7 +26,8 @@ def norm_args(**kw):
 
 
 @pytest.mark.parametrize('bad', [dict(P=0), dict(B=0), dict(W=-1), dict(dtype=2), dict(x=None), dict(mean=None),
-                                 dict(rstd=None), dict(P=1 << 20, B=1 << 20)])
+                                 dict(rstd=None), dict(P=1 << 20, B=1 << 20), dict(B=(1 << 30) + 1, P=1),
+                                 dict(W=(1 << 30) + 8)])
 def test_layer_norm_refusals(bad):
     refused('tp_layer_norm_forward', norm_args(**bad))
     refused('tp_layer_norm_backward', norm_args(**bad))
