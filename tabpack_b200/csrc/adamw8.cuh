@@ -100,12 +100,13 @@ __device__ __forceinline__ f32x2 sqrt2(f32x2 v) {
   float r0, r1;
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(f.x));
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(f.y));
-  const f32x2 r = pair(r0, r1), half = pair(0.5f, 0.5f), minus = pair(-1.0f, -1.0f);
-  f32x2 s = mul2(v, r), h = mul2(r, half);
-  const f32x2 e = fma2(mul2(s, minus), h, half);
+  // h with its sign changed, so that no product needs one: s + (-h) (s^2 - v)
+  const f32x2 r = pair(r0, r1);
+  f32x2 s = mul2(v, r), h = mul2(r, pair(-0.5f, -0.5f));
+  const f32x2 e = fma2(s, h, pair(0.5f, 0.5f));
   s = fma2(s, e, s);
   h = fma2(h, e, h);
-  return fma2(fma2(mul2(s, minus), s, v), h, s);
+  return fma2(fma2(s, s, pair(-f.x, -f.y)), h, s);
 }
 
 __global__ void root_check_kernel(uint32_t first, uint32_t count, unsigned long long* differ) {
@@ -339,11 +340,13 @@ __device__ __forceinline__ float2 adamw8_block(const AdamW8Lane& x, const AdamW8
     for (int j = 0; j < 4; ++j) rw[j] = words[lane + 32 * j];
     __syncwarp();
   }
-  float ym[4], yu[4];
+  float ym[4], yu[4];  // signed and not: the first codes drop the sign bit
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    ym[j] = __fmul_rn(fabsf(mm[j]), minv);
-    yu[j] = __fmul_rn(uu[j], vinv);
+  for (int h = 0; h < 2; ++h) {
+    const float2 y = halves(mul2(pair(mm[2 * h], mm[2 * h + 1]), pair(minv, minv)));
+    const float2 z = halves(mul2(pair(uu[2 * h], uu[2 * h + 1]), pair(vinv, vinv)));
+    ym[2 * h] = y.x, ym[2 * h + 1] = y.y;
+    yu[2 * h] = z.x, yu[2 * h + 1] = z.y;
   }
   // Codes of normal values: the number's bits plus the random ones below the code's last place, then
   // the code's 8 bits, shifted into the top byte (e4m3: exponent offset 120, whose 0xC0 in that byte
@@ -357,14 +360,15 @@ __device__ __forceinline__ float2 adamw8_block(const AdamW8Lane& x, const AdamW8
     vc[j] = __float_as_uint(yu[j]) * 32u + __byte_perm(rw[j], 0, 0x4324);
   }
   uint32_t mo = (top4(mc) & 0x7F7F7F7Fu) ^ 0x40404040u, vo = top4(vc);
-  const bool msmall = !(fminf(fminf(ym[0], ym[1]), fminf(ym[2], ym[3])) >= 0.015625f);  // 2^-6
+  const bool msmall =
+      !(fminf(fminf(fabsf(ym[0]), fabsf(ym[1])), fminf(fabsf(ym[2]), fabsf(ym[3]))) >= 0.015625f);  // 2^-6
   const bool usmall = !(__fmul_rn(umin, vinv) >= 3.2424927e-05f);                       // 2^-15 (1 + 1 / 16)
   if (__any_sync(0xFFFFFFFFu, msmall)) {
     uint32_t pick = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      mc[j] = adamw8_small_first(ym[j], __byte_perm(rw[j], 0, 0x4104));
-      if (!(ym[j] >= 0.015625f)) pick |= 0xFFu << (8 * j);
+      mc[j] = adamw8_small_first(fabsf(ym[j]), __byte_perm(rw[j], 0, 0x4104));
+      if (!(fabsf(ym[j]) >= 0.015625f)) pick |= 0xFFu << (8 * j);
     }
     mo = (mo & ~pick) | (bytes4(mc[0], mc[1], mc[2], mc[3]) & pick);
     if (!(minv > 0.0f)) mo = 0;

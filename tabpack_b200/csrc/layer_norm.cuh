@@ -47,10 +47,9 @@ __device__ __forceinline__ int norm_width(const LayerNormArgs& a, int m) {
   return a.n ? min(max(a.n[m], 0), a.W) : a.W;
 }
 
-// V neighbouring elements: 16 bytes, or one element where nothing is aligned.
 constexpr int NORM_H = NORM_E / 2;  // pairs
 
-// Vector k's pairs.
+// V neighbouring elements are one vector: 16 bytes, or one element where nothing is aligned.
 template <typename T, int V>
 __device__ __forceinline__ void norm_unpack(const uint4& u, f32x2* f) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
