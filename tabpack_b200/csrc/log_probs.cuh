@@ -668,9 +668,10 @@ __global__ void __launch_bounds__(1024) log_probs_long_forward_kernel(const LogP
     write_best(a, row, lane_id(), (uint32_t)(best.key >> 32), (uint32_t)~(uint32_t)best.key, st);
 }
 
-// One warp per LP_CHUNK scores of a row.
+// One warp per LP_CHUNK scores of a row.  Five blocks an SM, 48 registers (50 registers, four
+// blocks: 348 us instead of 324 for 8192 rows of 65536 in bf16).
 template <typename T>
-__global__ void __launch_bounds__(256) log_probs_stream_backward_kernel(const LogProbsArgs a, int chunks) {
+__global__ void __launch_bounds__(256, 5) log_probs_stream_backward_kernel(const LogProbsArgs a, int chunks) {
   constexpr int V = Row<T>::V, U = LP_CHUNK / (32 * V);
   const uint32_t task = blockIdx.x * 8 + warp_id();
   const uint32_t row = task / (uint32_t)chunks;

@@ -1961,8 +1961,10 @@ void launch_log_probs(const LogProbsArgs& k, int held, cudaStream_t st) {
   } else if (held <= 1024) {
     log_probs_held_forward_kernel<T, 32, 32, TOP><<<blocks(32), 256, 0, st>>>(k);
   } else {
-    // a thread per 64 scores, at least 4 warps; a few rows take all the threads a block has
-    const int want = k.rows < 296 ? 1024 : std::min(512, std::max(128, (k.C / 64 + 31) / 32 * 32));
+    // a thread per 64 scores, 4 to 8 warps (8192 rows of 65536 in bf16: 184 us, with 16 warps 198, with
+    // 4 warps 180 but half again as long on 300 rows); rows that do not fill the SMs twice take all
+    // the threads a block has (4 rows of 51200: 5.9 us)
+    const int want = k.rows < 296 ? 1024 : std::min(256, std::max(128, (k.C / 64 + 31) / 32 * 32));
     log_probs_long_forward_kernel<T, TOP><<<(unsigned)k.rows, want, 0, st>>>(k);
   }
 }
