@@ -752,6 +752,16 @@ def _operand(name: str, t: Tensor | None, shape: tuple, dtype: torch.dtype, devi
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _empty2(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> Tensor:
+    """A contiguous (rows, cols) tensor (the strided form is the cheapest of torch's factories)."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
+def _empty_as(t: Tensor, dtype: torch.dtype) -> Tensor:
+    """A contiguous tensor of t's shape."""
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(tuple(t.shape), dtype=dtype)
+
+
 ADAMW8_BLOCK = 128
 """Elements of a member that share one scale per moment in `adamw8_step`'s states."""
 
@@ -877,7 +887,7 @@ def adamw8_moments(exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, *,
         nb = (inner + ADAMW8_BLOCK - 1) // ADAMW8_BLOCK
         if not _adamw8_state_fits(shape, P, nb, device, m, ms, v, vs):
             raise _adamw8_state_error(shape, P, nb, device)
-        om, ov = m.new_empty(shape, dtype=dtype), m.new_empty(shape, dtype=dtype)
+        om, ov = torch.empty_like(m, dtype=dtype), torch.empty_like(m, dtype=dtype)
         out_m.append(om)
         out_v.append(ov)
         if numel == 0:
@@ -931,9 +941,10 @@ def layer_norm_forward(x: Tensor, weight: Tensor | None, bias: Tensor | None, *,
     weight = _operand('weight', weight, (P, W), torch.float32, device)
     bias = _operand('bias', bias, (P, W), torch.float32, device)
     if n_features is not None:
-        n_features = _operand('n_features', n_features.to(torch.int32), (P,), torch.int32, device)
-    y = x.new_empty((P, B, W))
-    mean, rstd = x.new_empty((P, B), dtype=torch.float32), x.new_empty((P, B), dtype=torch.float32)
+        n_features = _operand('n_features', n_features if n_features.dtype is torch.int32
+                              else n_features.to(torch.int32), (P,), torch.int32, device)
+    y = _empty_as(x, dtype) if x.ndim == 3 else x.new_empty((P, B, W))
+    mean, rstd = _empty2(P, B, torch.float32, x.device), _empty2(P, B, torch.float32, x.device)
     if P and B and W:
         a = _lib.LayerNormArgs(P, B, W, code, sm, sr, _ptr(n_features), x.data_ptr(), _ptr(weight), _ptr(bias), eps,
                                y.data_ptr(), mean.data_ptr(), rstd.data_ptr())
@@ -955,7 +966,8 @@ def layer_norm_backward(dy: Tensor, x: Tensor, weight: Tensor | None, mean: Tens
     dy, dm, dr = _norm_rows('dy', dy, dtype, device, shape)
     weight = _operand('weight', weight, (P, W), torch.float32, device)
     if n_features is not None:
-        n_features = _operand('n_features', n_features.to(torch.int32), (P,), torch.int32, device)
+        n_features = _operand('n_features', n_features if n_features.dtype is torch.int32
+                              else n_features.to(torch.int32), (P,), torch.int32, device)
     for name, t in (('mean', mean), ('rstd', rstd)):
         if t.shape != (P, B) or t.dtype is not torch.float32 or t.get_device() != device or not t.is_contiguous():
             raise TypeError(f'{name} must be the contiguous fp32 ({P}, {B}) tensor of the forward')
@@ -963,15 +975,15 @@ def layer_norm_backward(dy: Tensor, x: Tensor, weight: Tensor | None, mean: Tens
     dx = dw = db = ws = None
     if need_dx:
         # the members' terms of a shared input are added up before they are rounded
-        dx = x.new_empty(shape, dtype=torch.float32 if shared else dtype)
+        dx = _empty_as(dy, torch.float32 if shared else dtype)
     if need_dw:
-        dw = x.new_empty((P, W), dtype=torch.float32)
+        dw = _empty2(P, W, torch.float32, x.device)
     if need_db:
-        db = x.new_empty((P, W), dtype=torch.float32)
+        db = _empty2(P, W, torch.float32, x.device)
     if P and B and W and (need_dx or need_dw or need_db):
         need = load().tp_layer_norm_workspace_size(P, B, W) if need_dw or need_db else 0
         if need:
-            ws = x.new_empty(need, dtype=torch.uint8)
+            ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=x.device)
         a = _lib.LayerNormArgs(P, B, W, code, sm, sr, _ptr(n_features), x.data_ptr(), _ptr(weight), None, 0.0, None,
                                mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dm, dr, _ptr(dx),
                                TP_DTYPE_F32 if shared else code, _ptr(dw), _ptr(db), _ptr(ws), need)
@@ -990,6 +1002,8 @@ def _logit_rows(logits: Tensor) -> tuple[Tensor, int, int]:
     are not at one stride."""
     shape, strides = logits.shape, logits.stride()
     C = shape[-1]
+    if logits.is_contiguous():
+        return logits, logits.numel() // C, C
     rows, stride, ok = 1, C, C == 1 or strides[-1] == 1
     for d in range(len(shape) - 2, -1, -1):
         if shape[d] != 1:
@@ -1032,8 +1046,11 @@ def label_log_probs_forward(logits: Tensor, labels: Tensor, *, top_k: int = 0, i
     if not 0 <= top_k <= min(C, _lib.TP_MAX_TOP_K):
         raise ValueError(f'top_k must be between 0 and {min(C, _lib.TP_MAX_TOP_K)}, got {top_k}')
     f32 = torch.float32
-    log_prob, entropy = logits.new_empty(lead, dtype=f32), logits.new_empty(lead, dtype=f32)
-    stats = logits.new_empty((rows, 3), dtype=f32) if C > _lib.TP_LABEL_STATS_CLASSES else None
+    if labels.shape == lead:
+        log_prob, entropy = torch.empty_like(labels, dtype=f32), torch.empty_like(labels, dtype=f32)
+    else:
+        log_prob, entropy = (logits.new_empty(tuple(lead), dtype=f32) for _ in range(2))
+    stats = _empty2(rows, 3, f32, logits.device) if C > _lib.TP_LABEL_STATS_CLASSES else None
     top = which = None
     if top_k:
         top = logits.new_empty((*lead, top_k), dtype=f32)
@@ -1071,7 +1088,7 @@ def label_log_probs_backward(g_log_prob: Tensor | None, g_entropy: Tensor | None
         raise TypeError('stats must be the tensor that the forward returned')
     g_log_prob, sl = _row_gradient('g_log_prob', g_log_prob, lead, device)
     g_entropy, sh = _row_gradient('g_entropy', g_entropy, lead, device)
-    dlogits = logits.new_empty((*lead, C))
+    dlogits = _empty_as(logits, logits.dtype)
     if rows:
         a = _lib.LabelLogProbsArgs(rows, C, code, logits.data_ptr(), stride, labels.data_ptr(), labels.numel(),
                                    ignore_index, 0, None, None, None, None, _ptr(stats), _ptr(g_log_prob),
