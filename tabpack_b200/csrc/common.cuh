@@ -224,7 +224,7 @@ inline FastDiv make_fastdiv(uint32_t d) {
 __device__ __forceinline__ uint32_t fastdiv(uint32_t n, const FastDiv& f) { return (__umulhi(n, f.m) + n) >> f.l; }
 
 // ---------------------------------------------------------------------------
-// Thread-block clusters (CTA pairs)
+// Thread-block clusters
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;
@@ -239,7 +239,7 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
   return r;
 }
 
-// Every thread of both CTAs; orders shared-memory writes (barrier init) before the peer's use.
+// Every thread of every CTA; orders shared-memory writes (barrier init) before the others' use.
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -262,6 +262,19 @@ __device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t bar_cluster
 // 32-bit store into shared memory given by its shared::cluster address (own or peer CTA).
 __device__ __forceinline__ void st_shared_cluster_u32(uint32_t addr_cluster, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr_cluster), "r"(v) : "memory");
+}
+
+// 32 and 64 bits from shared memory given by its shared::cluster address (own or another CTA of the
+// cluster), after a cluster_sync that follows their writing.
+__device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t addr_cluster) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr_cluster) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned long long ld_shared_cluster_u64(uint32_t addr_cluster) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr_cluster) : "memory");
+  return v;
 }
 
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* map) {

@@ -14,10 +14,9 @@
 // to 1024 classes are held in registers, 16 scores a lane (32 from 512 classes on) of a thread, 4, 8,
 // 16 or 32 lanes, so the row is read once and the softmax takes its maximum first (a row's fixed cost,
 // reductions and label, is paid once per group: 8 scores a lane took half again as long on 50 and 200
-// classes); longer rows take one block and one pass
-// with a running maximum, the next 64 bytes of each thread on their way meanwhile.  Rows start anywhere:
-// whole 16-byte vectors are loaded between the first and last boundary inside the row, single elements
-// before and after.
+// classes); longer rows take one block (few of them a cluster of up to eight) and one pass with a running
+// maximum, the next vectors of each thread on their way meanwhile.  Rows start anywhere: whole 16-byte
+// vectors are loaded between the first and last boundary inside the row, single elements before and after.
 //
 // The best classes take nothing from the pass: the k-th largest of the threads' maxima is a bound that
 // at least k scores reach and few others do.  Only the threads whose maximum reaches it have
@@ -51,6 +50,7 @@ struct LogProbsArgs {
 
 constexpr float LP_FAR = -200.0f;
 constexpr int LP_REREAD = TP_LABEL_STATS_CLASSES;  // rows up to here: the backward takes the statistics anew
+constexpr int LP_WARPS = 8;          // of a block on long rows, at most
 constexpr int LP_CHUNK = 2048;       // classes of one warp in the streaming backward
 
 __device__ __forceinline__ float lp_nan() { return __uint_as_float(0x7FC00000u); }
@@ -540,38 +540,81 @@ __global__ void __launch_bounds__(256) log_probs_held_backward_kernel(const LogP
 }
 
 // ---------------------------------------------------------------------------
-// Long rows: one block per row, one pass.
+// Long rows: one block per row (or a cluster, where the rows are few), one pass.
 // ---------------------------------------------------------------------------
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(1024) log_probs_long_forward_kernel(const LogProbsArgs a) {
-  constexpr int V = Row<T>::V, U = 4;  // vectors of a thread in one piece
-  __shared__ float red[3][32];
-  __shared__ class_key buf[TOP ? 32 : 1][TOP ? LP_CANDIDATES : 1];
-  __shared__ uint32_t maxima[TOP ? 32 : 1][32];
-  __shared__ uint16_t again[TOP ? 1024 : 1];  // threads whose scores are looked at again
-  __shared__ int count[33];                   // of each warp's buf; last: of `again`
-  const int64_t row = blockIdx.x;
+// Sums of exp(z - m) and exp(z - m) (z - m) taken over to a maximum `to` >= m.
+__device__ __forceinline__ void rescale(float m, float to, float& s, float& t) {
+  if (m == -INFINITY || m == to) return;
+  const float d = fmaxf(m - to, LP_FAR), c = exp_neg(d);
+  t = c * (t + s * d);
+  s *= c;
+}
+
+// n sorted lists of a block's warps, this warp's `list` also in lists[its number], two by two into
+// lists[0].  Every thread, after a __syncthreads; ends with one.
+__device__ __forceinline__ void merge_lists(uint32_t list, uint32_t (*lists)[32], int n) {
+  const int wid = warp_id();
+  for (int half = LP_WARPS / 2; half > 0; half >>= 1) {
+    if (wid < half && wid + half < n) {
+      list = lanes_merge(max(list, lists[wid + half][31 - lane_id()]));
+      lists[wid][lane_id()] = list;
+    }
+    __syncthreads();
+  }
+}
+
+// The same for best classes; warp 0 ends with the result in `best` and in lists[0].
+__device__ __forceinline__ void join_lists(BestList& best, class_key (*lists)[LP_CANDIDATES], int n) {
+  const int wid = warp_id();
+  for (int half = LP_WARPS / 2; half > 0; half >>= 1) {
+    if (wid < half && wid + half < n) {
+      best.join(lists[wid + half][lane_id()]);
+      lists[wid][lane_id()] = best.key;
+    }
+    if (half < n) __syncthreads();
+  }
+}
+
+// SPLIT: the row is spread over the `cluster` CTAs of a thread-block cluster, which read each other's
+// sums and lists through distributed shared memory; the first one writes.
+// A thread keeps 3 (bf16) or 4 (fp32) vectors on their way, which leaves room for four blocks an SM without
+// spills (8192 rows of 65536 in bf16: 190 us; 4 vectors with spills 221, with three blocks an SM 198; in
+// fp32, 4096 rows of 40000: 104 us with 4, 110 with 3).
+template <typename T, bool TOP, bool SPLIT>
+__global__ void __launch_bounds__(32 * LP_WARPS, SPLIT ? 1 : 4)
+    log_probs_long_forward_kernel(const LogProbsArgs a, int cluster) {
+  constexpr int V = Row<T>::V, U = V == 8 ? 3 : 4;  // vectors of a thread in one piece
+  __shared__ float red[3][LP_WARPS];
+  __shared__ class_key buf[TOP ? LP_WARPS : 1][TOP ? LP_CANDIDATES : 1];
+  __shared__ uint32_t maxima[TOP ? LP_WARPS : 1][32];
+  __shared__ uint16_t again[TOP ? 32 * LP_WARPS : 1];  // threads whose scores are looked at again
+  __shared__ int count[LP_WARPS + 1];                  // of each warp's buf; last: of `again`
+  __shared__ float sums[3];                            // SPLIT: this CTA's maximum and sums
+  __shared__ uint32_t all[TOP && SPLIT ? LP_WARPS : 1][32];
+  const int rank = SPLIT ? (int)cluster_ctarank() : 0, parts = SPLIT ? cluster : 1;
+  const int64_t row = blockIdx.x / (unsigned)parts;
   const T* z = static_cast<const T*>(a.logits) + row * a.ld;
   const Row<T> r(z, a.C);
   const int nv = r.vectors(), threads = blockDim.x, warps = threads >> 5, wid = warp_id();
-  if (TOP && lane_id() == 0) count[wid] = count[32] = 0;
+  const int stride = threads * parts, mine = rank * threads + threadIdx.x;  // vectors mine, mine + stride, ...
+  if (TOP && lane_id() == 0) count[wid] = count[LP_WARPS] = 0;
   float m = -INFINITY;
   f32x2 s = pair(0.f, 0.f), t = s;
   uint4 next[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int i = u * threads + threadIdx.x;
+    const int i = u * stride + mine;
     next[u] = i < nv ? r.raw(i) : Row<T>::nothing();
   }
-  for (int i0 = 0; i0 < nv; i0 += U * threads) {
+  for (int i0 = 0; i0 < nv; i0 += U * stride) {
     float v[U * V];
 #pragma unroll
     for (int u = 0; u < U; ++u) Row<T>::unpack(next[u], v + u * V);
-    if (i0 + U * threads < nv) {
+    if (i0 + U * stride < nv) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int i = i0 + (U + u) * threads + threadIdx.x;
+        const int i = i0 + (U + u) * stride + mine;
         next[u] = i < nv ? r.raw(i) : Row<T>::nothing();
       }
     }
@@ -599,45 +642,65 @@ __global__ void __launch_bounds__(1024) log_probs_long_forward_kernel(const LogP
   if (lane_id() == 0) red[0][wid] = wm;
   const float2 sh = halves(s), th = halves(t);
   float s1 = sh.x + sh.y, t1 = th.x + th.y;
-  uint32_t order = 0;
+  uint32_t order = 0, list = 0;  // the thread's maximum; the warp's, sorted
   if constexpr (TOP) {
     // a thread with a NaN, which its sum then holds, is above all; one without scores counts as -inf
     order = s1 != s1 ? 0xFFFFFFFFu : class_order(m);
-    maxima[wid][lane_id()] = lanes_sort(order);
+    list = lanes_sort(order);
+    maxima[wid][lane_id()] = list;
   }
   __syncthreads();
-  const float bm = group_max<32>(lane_id() < warps ? red[0][lane_id()] : -INFINITY);
-  if (m != -INFINITY && m != bm) {
-    const float d = fmaxf(m - bm, LP_FAR), c = exp_neg(d);
-    t1 = c * (t1 + s1 * d);
-    s1 *= c;
-  }
+  float bm = group_max<32>(lane_id() < warps ? red[0][lane_id()] : -INFINITY);
+  rescale(m, bm, s1, t1);
   s1 = group_sum<32>(s1);
   t1 = group_sum<32>(t1);
   if (lane_id() == 0) {
     red[1][wid] = s1;
     red[2][wid] = t1;
   }
-  BestList best;
   if constexpr (TOP) {
     // the k-th largest of all threads' maxima: the warps' sorted lists, two by two
-    uint32_t list = maxima[wid][lane_id()];
-    for (int half = 16; half > 0; half >>= 1) {
-      if (wid < half && wid + half < warps) {
-        list = lanes_merge(max(list, maxima[wid + half][31 - lane_id()]));
-        maxima[wid][lane_id()] = list;
-      }
+    merge_lists(list, maxima, warps);
+  } else {
+    __syncthreads();
+  }
+  if constexpr (SPLIT) {
+    s1 = group_sum<32>(lane_id() < warps ? red[1][lane_id()] : 0.f);
+    t1 = group_sum<32>(lane_id() < warps ? red[2][lane_id()] : 0.f);
+    if (threadIdx.x == 0) sums[0] = bm, sums[1] = s1, sums[2] = t1;
+    __syncwarp();
+    cluster_sync();
+    // lane i holds CTA i's maximum and sums
+    const bool other = lane_id() < parts;
+    const uint32_t at = mapa_shared(smem_u32(sums), other ? lane_id() : 0);
+    const float om = other ? __uint_as_float(ld_shared_cluster_u32(at)) : -INFINITY;
+    s1 = other ? __uint_as_float(ld_shared_cluster_u32(at + 4)) : 0.f;
+    t1 = other ? __uint_as_float(ld_shared_cluster_u32(at + 8)) : 0.f;
+    bm = group_max<32>(om);
+    rescale(om, bm, s1, t1);
+    s1 = group_sum<32>(s1);
+    t1 = group_sum<32>(t1);
+  }
+  BestList best;
+  if constexpr (TOP) {
+    uint32_t bound = maxima[0][a.k - 1];
+    if constexpr (SPLIT) {
+      // the CTAs' lists, one a warp, and again two by two
+      list = wid < parts ? ld_shared_cluster_u32(mapa_shared(smem_u32(&maxima[0][lane_id()]), wid)) : 0u;
+      all[wid][lane_id()] = list;
       __syncthreads();
+      merge_lists(list, all, parts);
+      bound = all[0][a.k - 1];
     }
-    const uint32_t bound = maxima[0][a.k - 1];
-    if (order >= bound) again[atomicAdd(&count[32], 1)] = (uint16_t)threadIdx.x;
+    if (order >= bound) again[atomicAdd(&count[LP_WARPS], 1)] = (uint16_t)threadIdx.x;
     __syncthreads();
     // those threads' vectors, spread over the block
-    const int per = (nv + threads - 1) / threads;
-    const int64_t tasks = (int64_t)count[32] * per;
+    const int per = (nv + stride - 1) / stride;
+    const int64_t tasks = (int64_t)count[LP_WARPS] * per;
     for (int64_t p0 = wid * 32; p0 < tasks; p0 += threads) {
       const int64_t p = p0 + lane_id();
-      const int i = p < tasks ? again[p / per] + (int)(p % per) * threads : nv;
+      const int64_t i64 = p < tasks ? rank * threads + again[p / per] + (p % per) * stride : nv;
+      const int i = (int)min(i64, (int64_t)nv);
       float v[V];
       Row<T>::unpack(i < nv ? r.raw(i) : Row<T>::nothing(), v);
       const auto cls = [&](int j) {
@@ -649,19 +712,28 @@ __global__ void __launch_bounds__(1024) log_probs_long_forward_kernel(const LogP
     const int lists = (int)min((int64_t)warps, (tasks + 31) / 32);
     buf[wid][lane_id()] = best.key;
     __syncthreads();
-    for (int half = 16; half > 0; half >>= 1) {
-      if (wid < half && wid + half < lists) {
-        best.join(buf[wid + half][lane_id()]);
-        buf[wid][lane_id()] = best.key;
+    join_lists(best, buf, lists);
+    if constexpr (SPLIT) {
+      __syncwarp();
+      cluster_sync();
+      if (rank == 0) {
+        if (wid > 0) best.key = wid < parts ? ld_shared_cluster_u64(mapa_shared(smem_u32(&buf[0][lane_id()]), wid)) : 0ull;
+        if (wid > 0) buf[wid][lane_id()] = best.key;
+        __syncthreads();
+        join_lists(best, buf, parts);
       }
-      if (half < lists) __syncthreads();
+      __syncwarp();
     }
-  } else {
-    __syncthreads();
+  }
+  if constexpr (SPLIT) {
+    cluster_sync();  // no CTA leaves while the first one reads its lists
+    if (rank != 0) return;
   }
   if (wid != 0) return;
-  s1 = group_sum<32>(lane_id() < warps ? red[1][lane_id()] : 0.f);
-  t1 = group_sum<32>(lane_id() < warps ? red[2][lane_id()] : 0.f);
+  if constexpr (!SPLIT) {
+    s1 = group_sum<32>(lane_id() < warps ? red[1][lane_id()] : 0.f);
+    t1 = group_sum<32>(lane_id() < warps ? red[2][lane_id()] : 0.f);
+  }
   const RowStats st = row_stats(bm, s1, t1);
   if (lane_id() == 0) write_row(a, row, RowLabel(a, row, z), st);
   if (TOP && lane_id() < a.k)

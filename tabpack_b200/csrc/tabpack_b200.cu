@@ -1946,7 +1946,7 @@ int held_size(const tp_label_log_probs_args* a, int size) {
 }
 
 template <typename T, bool TOP>
-void launch_log_probs(const LogProbsArgs& k, int held, cudaStream_t st) {
+int launch_log_probs(const LogProbsArgs& k, int held, cudaStream_t st) {
   const auto blocks = [&](int lanes) { return (unsigned)((k.rows * lanes + 255) / 256); };
   if (held <= 16) {
     log_probs_held_forward_kernel<T, 1, 16, TOP><<<blocks(1), 256, 0, st>>>(k);
@@ -1961,12 +1961,33 @@ void launch_log_probs(const LogProbsArgs& k, int held, cudaStream_t st) {
   } else if (held <= 1024) {
     log_probs_held_forward_kernel<T, 32, 32, TOP><<<blocks(32), 256, 0, st>>>(k);
   } else {
+    // Few long rows are split over clusters of 2 to 8 CTAs while the SMs hold one CTA each.  With 128000
+    // classes in bf16 one row takes 4.8 us instead of 12.5, 74 rows 8.7 instead of 12.7; with 51200 one row
+    // 4.7 instead of 6.7.  Shorter rows lose more to the cluster's barriers (16384 classes: 4.2 instead of
+    // 3.8, with the top classes 7.9 instead of 6.0), and two CTAs an SM gain nothing (74 rows: 12.1).
+    int parts = 1;
+    if (k.C >= 32768)
+      while (parts < 8 && k.rows * parts * 2 <= 148) parts *= 2;
+    if (parts > 1) {
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3((unsigned)k.rows * parts);
+      cfg.blockDim = dim3(32 * LP_WARPS);
+      cfg.stream = st;
+      cudaLaunchAttribute attr{};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = parts;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, log_probs_long_forward_kernel<T, TOP, true>, k, parts));
+      return TP_OK;
+    }
     // a thread per 64 scores, 4 to 8 warps (8192 rows of 65536 in bf16: 184 us, with 16 warps 198, with
-    // 4 warps 180 but half again as long on 300 rows); rows that do not fill the SMs twice take all
-    // the threads a block has (4 rows of 51200: 5.9 us)
-    const int want = k.rows < 296 ? 1024 : std::min(256, std::max(128, (k.C / 64 + 31) / 32 * 32));
-    log_probs_long_forward_kernel<T, TOP><<<(unsigned)k.rows, want, 0, st>>>(k);
+    // 4 warps 180 but half again as long on 300 rows)
+    const int want = std::min(32 * LP_WARPS, std::max(128, (k.C / 64 + 31) / 32 * 32));
+    log_probs_long_forward_kernel<T, TOP, false><<<(unsigned)k.rows, want, 0, st>>>(k, 1);
   }
+  return TP_OK;
 }
 
 template <typename T>
@@ -2008,14 +2029,11 @@ int tp_label_log_probs_forward(const tp_label_log_probs_args* a, void* stream) {
   const LogProbsArgs k = label_log_probs_args(a);
   const bool bf16 = a->dtype == TP_DTYPE_BF16;
   const int held = held_size(a, bf16 ? 2 : 4);
-  if (bf16 && a->top_k)
-    launch_log_probs<__nv_bfloat16, true>(k, held, st);
-  else if (bf16)
-    launch_log_probs<__nv_bfloat16, false>(k, held, st);
-  else if (a->top_k)
-    launch_log_probs<float, true>(k, held, st);
+  if (bf16)
+    rc = a->top_k ? launch_log_probs<__nv_bfloat16, true>(k, held, st) : launch_log_probs<__nv_bfloat16, false>(k, held, st);
   else
-    launch_log_probs<float, false>(k, held, st);
+    rc = a->top_k ? launch_log_probs<float, true>(k, held, st) : launch_log_probs<float, false>(k, held, st);
+  if (rc) return rc;
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;
 }

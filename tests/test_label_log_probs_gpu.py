@@ -122,6 +122,29 @@ def test_best_classes(C, k):
     run_and_check(*make((3, 4), C, torch.float32, seed=k, masked=0.5), k=k)
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('R', [1, 2, 18, 19, 37, 38, 74, 75, 149])
+def test_long_rows_of_every_split(R, dtype):
+    """Row counts on both sides of each rule that spreads a row over a cluster, the best classes
+    gathered in one part and spread over all, a NaN and a masked row among them."""
+    from tabpack_b200 import ops
+
+    C = 32779
+    z, y, g_l, g_h = make((R,), C, dtype, seed=R)
+    z[0, 8000:8032] += 20.0
+    z[-1, ::500] += 20.0
+    run_and_check(z, y, g_l, g_h, k=32)
+    if R > 2:
+        z[1], z[2, 9] = -INF, float('nan')
+        lp, H, top, which, stats = ops.label_log_probs_forward(z, y, top_k=2)
+        assert lp[1] == -INF and H[1] == 0 and which[1].tolist() == [0, 1]
+        assert torch.isnan(lp[2]) and which[2, 0] == 9
+        keep = [i for i in range(R) if i not in (1, 2)]
+        want, tol = plain(z[keep], y[keep], 2, g_l[keep].double(), g_h[keep].double())
+        near(lp[keep], want[0], tol[0], 'log_prob')
+        assert torch.equal(which[keep], want[3])
+
+
 @pytest.mark.parametrize('C', [40, 1024, 3000, 70000])
 def test_best_classes_in_hard_orders(C):
     """Ascending, descending and constant rows, few distinct values, the best at the end."""
