@@ -1982,10 +1982,14 @@ int launch_log_probs(const LogProbsArgs& k, int held, cudaStream_t st) {
       TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, log_probs_long_forward_kernel<T, TOP, true>, k, parts));
       return TP_OK;
     }
-    // a thread per 64 scores, 4 to 8 warps (8192 rows of 65536 in bf16: 184 us, with 16 warps 198, with
-    // 4 warps 180 but half again as long on 300 rows)
-    const int want = std::min(32 * LP_WARPS, std::max(128, (k.C / 64 + 31) / 32 * 32));
-    log_probs_long_forward_kernel<T, TOP, false><<<(unsigned)k.rows, want, 0, st>>>(k, 1);
+    // 2, 4 or 8 warps (3 and 5 leave an SM's four schedulers uneven): a thread per 128 scores or more, or
+    // per 64 where the SMs hold all rows at once.  4096 rows of 16000 in bf16 29.4 us with 4 warps against
+    // 35.0 with 8, 16384 rows of 12000 75 with 2 against 99 with 6; 300 rows of 16000 5.3 with 8 against
+    // 7.3 with 2.  (8192 rows of 65536: 16 warps take 14 us more than 8.)
+    const int64_t per = k.rows < 8 * 148 ? 64 : 128;
+    int threads = 64;
+    while (threads < 32 * LP_WARPS && threads * 2 * per <= k.C) threads *= 2;
+    log_probs_long_forward_kernel<T, TOP, false><<<(unsigned)k.rows, threads, 0, st>>>(k, 1);
   }
   return TP_OK;
 }

@@ -145,6 +145,12 @@ def test_long_rows_of_every_split(R, dtype):
         assert torch.equal(which[keep], want[3])
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('R,C', [(1183, 4099), (1183, 8200), (1184, 1500), (1184, 16390), (1184, 32800)])
+def test_long_rows_of_every_block_size(R, C, dtype):
+    run_and_check(*make((R,), C, dtype, seed=C, masked=0.3), k=32)
+
+
 @pytest.mark.parametrize('C', [40, 1024, 3000, 70000])
 def test_best_classes_in_hard_orders(C):
     """Ascending, descending and constant rows, few distinct values, the best at the end."""
