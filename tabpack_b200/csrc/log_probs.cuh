@@ -417,6 +417,23 @@ __device__ __forceinline__ void best_take(BestList& best, int k, const float (&z
   __syncwarp();
 }
 
+// A key of a held row's class: 32 bits are enough for bf16, whose scores have 16.
+template <typename T>
+struct HeldKey {
+  typedef class_key type;
+  __device__ static type make(float z, int c) { return make_key(class_order(z), (uint32_t)c); }
+  __device__ static uint32_t order(type k) { return (uint32_t)(k >> 32); }
+  __device__ static uint32_t class_of(type k) { return ~(uint32_t)k; }
+};
+template <>
+struct HeldKey<__nv_bfloat16> {
+  typedef uint32_t type;
+  // of an order's low half, all zeros or (below zero, and a NaN) all ones, nothing is lost
+  __device__ static type make(float z, int c) { return (class_order(z) & 0xFFFF0000u) | (uint32_t)(0xFFFF - c); }
+  __device__ static uint32_t order(type k) { return (k & 0x80000000u) ? (k & 0xFFFF0000u) : (k | 0xFFFFu); }
+  __device__ static uint32_t class_of(type k) { return 0xFFFFu - (k & 0xFFFFu); }
+};
+
 // blockDim 256; a row beyond the last is computed again from the last and not written.
 template <typename T, int G, int E, bool TOP>
 __global__ void __launch_bounds__(256) log_probs_held_forward_kernel(const LogProbsArgs a) {
@@ -434,32 +451,25 @@ __global__ void __launch_bounds__(256) log_probs_held_forward_kernel(const LogPr
   if (mine) write_row(a, row, label, st);
   if constexpr (TOP) {
     if constexpr (G < 32) {
-      // k rounds: the lanes' best unused classes, then the group's; its lane looks for its next best
-      uint32_t order[E];
-      uint32_t best = 0, where = 0xFFFFFFFFu;
+      // k rounds: the lanes' best classes below the last one taken, then the group's; its lane looks for
+      // its next best
+      typedef HeldKey<T> Key;
+      typename Key::type key[E], best = 0;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const int c = h.at(r, lane, j);
-        order[j] = (c >= 0 && c < a.C) ? class_order(h.z[j]) : 0u;
-        if (order[j] > best) best = order[j], where = (uint32_t)c;
+        key[j] = (c >= 0 && c < a.C) ? Key::make(h.z[j], c) : 0;
+        best = max(best, key[j]);
       }
       for (int i = 0; i < a.k; ++i) {
-        uint32_t b = best, w = where;
+        typename Key::type b = best;
 #pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) {
-          const uint32_t bo = __shfl_xor_sync(0xFFFFFFFFu, b, o), wo = __shfl_xor_sync(0xFFFFFFFFu, w, o);
-          if (bo > b || (bo == b && wo < w)) b = bo, w = wo;
-        }
-        if (mine) write_best(a, row, i, b, w, st);
-        if (w == where) {
+        for (int o = G / 2; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xFFFFFFFFu, b, o));
+        if (mine) write_best(a, row, i, Key::order(b), Key::class_of(b), st);
+        if (b == best) {
           best = 0;
-          where = 0xFFFFFFFFu;
 #pragma unroll
-          for (int j = 0; j < E; ++j) {
-            const uint32_t c = (uint32_t)h.at(r, lane, j);
-            if (c == w) order[j] = 0;
-            if (order[j] > best) best = order[j], where = c;
-          }
+          for (int j = 0; j < E; ++j) best = max(best, key[j] < b ? key[j] : 0);
         }
       }
     } else {
