@@ -589,8 +589,9 @@ typedef struct tp_layer_norm_args {
   const void* dy;                /* backward */
   int64_t dy_member_stride, dy_row_stride;
   void* dx;                      /* (P, B, W), or NULL */
-  int32_t dx_dtype;              /* type of dx: dtype, or TP_DTYPE_F32 (per-member terms that the
-                                    caller adds up over the members) */
+  int32_t dx_dtype;              /* type of dx: dtype, or TP_DTYPE_F32 */
+  void* dx_sum;                  /* (B, W) of type dtype, or NULL: the members' terms in dx, which is
+                                    then fp32, added up (the gradient of a shared x) */
   float* dweight;                /* (P, W), or NULL */
   float* dbias;                  /* (P, W), or NULL */
   void* workspace;               /* backward with dweight or dbias: tp_layer_norm_workspace_size */

@@ -181,8 +181,8 @@ class LayerNormArgs(ctypes.Structure):
         ('x', ctypes.c_void_p), ('weight', ctypes.c_void_p), ('bias', ctypes.c_void_p), ('eps', ctypes.c_float),
         ('y', ctypes.c_void_p), ('mean', ctypes.c_void_p), ('rstd', ctypes.c_void_p), ('dy', ctypes.c_void_p),
         ('dy_member_stride', ctypes.c_int64), ('dy_row_stride', ctypes.c_int64), ('dx', ctypes.c_void_p),
-        ('dx_dtype', ctypes.c_int32), ('dweight', ctypes.c_void_p), ('dbias', ctypes.c_void_p),
-        ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_size_t),
+        ('dx_dtype', ctypes.c_int32), ('dx_sum', ctypes.c_void_p), ('dweight', ctypes.c_void_p),
+        ('dbias', ctypes.c_void_p), ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_size_t),
     ]
 
 

@@ -1820,6 +1820,17 @@ void launch_norm_wide_backward(const LayerNormArgs& k, cudaStream_t st) {
   if (k.dw || k.db) layer_norm_dw_kernel<T><<<dim3((k.W + 255) / 256, k.P, k.S), 256, 0, st>>>(k);
 }
 
+template <typename T>
+void launch_norm_member_sum(const LayerNormArgs& k, void* out, cudaStream_t st) {
+  const int64_t n = (int64_t)k.B * k.W;
+  const float* terms = static_cast<const float*>(k.dx);
+  const auto blocks = [&](int v) { return (unsigned)std::min<int64_t>((n + 256 * v - 1) / (256 * v), 148 * 8); };
+  if (n % 4 == 0 && aligned16(terms) && aligned16(out))
+    layer_norm_member_sum_kernel<T, 4><<<blocks(4), 256, 0, st>>>(terms, static_cast<T*>(out), k.P, n);
+  else
+    layer_norm_member_sum_kernel<T, 1><<<blocks(1), 256, 0, st>>>(terms, static_cast<T*>(out), k.P, n);
+}
+
 }  // namespace
 }  // namespace tp
 
@@ -1860,6 +1871,8 @@ int tp_layer_norm_backward(const tp_layer_norm_args* a, void* stream) {
   if (rc) return rc;
   if (!a->dy) return fail(TP_EINVAL, "null layer norm gradient");
   if (a->dx && a->dx_dtype != a->dtype && a->dx_dtype != TP_DTYPE_F32) return fail(TP_EINVAL, "bad dx dtype");
+  if (a->dx_sum && (!a->dx || a->dx_dtype != TP_DTYPE_F32))
+    return fail(TP_EINVAL, "a sum over the members needs their terms in fp32");
   LayerNormArgs k = layer_norm_args(a);
   k.S = norm_backward_splits(k.P, k.B, k.W);
   const bool params = a->dweight || a->dbias;
@@ -1889,6 +1902,12 @@ int tp_layer_norm_backward(const tp_layer_norm_args* a, void* stream) {
       layer_norm_finish_kernel<32><<<(unsigned)k.P * col_blocks, 1024, 0, st>>>(k, col_blocks);
     else
       layer_norm_finish_kernel<8><<<(unsigned)k.P * col_blocks, 256, 0, st>>>(k, col_blocks);
+  }
+  if (a->dx_sum) {
+    if (bf16)
+      launch_norm_member_sum<__nv_bfloat16>(k, a->dx_sum, st);
+    else
+      launch_norm_member_sum<float>(k, a->dx_sum, st);
   }
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;

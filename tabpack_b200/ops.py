@@ -971,11 +971,14 @@ def layer_norm_backward(dy: Tensor, x: Tensor, weight: Tensor | None, mean: Tens
     for name, t in (('mean', mean), ('rstd', rstd)):
         if t.shape != (P, B) or t.dtype is not torch.float32 or t.get_device() != device or not t.is_contiguous():
             raise TypeError(f'{name} must be the contiguous fp32 ({P}, {B}) tensor of the forward')
-    shared = x.ndim == 2
-    dx = dw = db = ws = None
+    dx = dw = db = ws = terms = None
     if need_dx:
-        # the members' terms of a shared input are added up before they are rounded
-        dx = _empty_as(dy, torch.float32 if shared else dtype)
+        if x.ndim == 2:
+            dx = _empty2(B, W, dtype, x.device)
+            # the members' terms of a shared input are added up before they are rounded
+            terms = dx if P == 1 else torch.empty_strided((P, B, W), (B * W, W, 1), dtype=torch.float32, device=x.device)
+        else:
+            dx = terms = _empty_as(dy, dtype)
     if need_dw:
         dw = _empty2(P, W, torch.float32, x.device)
     if need_db:
@@ -985,15 +988,14 @@ def layer_norm_backward(dy: Tensor, x: Tensor, weight: Tensor | None, mean: Tens
         if need:
             ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=x.device)
         a = _lib.LayerNormArgs(P, B, W, code, sm, sr, _ptr(n_features), x.data_ptr(), _ptr(weight), None, 0.0, None,
-                               mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dm, dr, _ptr(dx),
-                               TP_DTYPE_F32 if shared else code, _ptr(dw), _ptr(db), _ptr(ws), need)
+                               mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dm, dr, _ptr(terms),
+                               code if terms is dx else TP_DTYPE_F32, None if terms is dx else dx.data_ptr(), _ptr(dw),
+                               _ptr(db), _ptr(ws), need)
         _call('tp_layer_norm_backward', a, device)
     else:
-        for t in (dw, db):
+        for t in (dx, dw, db):
             if t is not None:
                 t.zero_()
-    if shared and dx is not None:
-        dx = dx.sum(0).to(dtype)
     return dx, dw, db
 
 

@@ -134,6 +134,23 @@ def test_shared_input(W, dtype):
 
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('P,B,W', [(1, 5, 70), (2, 1, 1), (7, 333, 771), (300, 3, 65), (3, 600, 1024), (2, 3, 8200)])
+def test_members_of_a_shared_input(P, B, W, dtype):
+    """One member (no sum), few and many, an odd and a whole number of vectors."""
+    run_and_check(*make(P, B, W, dtype, shared=True, seed=P + W))
+
+
+@pytest.mark.parametrize('P,B', [(0, 3), (3, 0)])
+def test_shared_input_without_rows_or_members(P, B):
+    from tabpack_b200 import ops
+
+    x, stat = torch.ones(B, 8, device='cuda'), torch.ones(P, B, device='cuda')
+    dx, dw, db = ops.layer_norm_backward(torch.ones(P, B, 8, device='cuda'), x, None, stat, stat)
+    assert torch.equal(dx, torch.zeros(B, 8, device='cuda'))
+    assert torch.equal(dw, torch.zeros(P, 8, device='cuda')) and torch.equal(db, dw)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize('W,ld', [(10, 16), (100, 104), (104, 112), (300, 301), (64, 65), (2000, 2008)])
 def test_rows_of_padded_buffers(W, ld, dtype):
     """Column slices of wider buffers: rows that are not packed, aligned and not; the buffer's other

@@ -45,6 +45,11 @@ def test_layer_norm_direction_refusals():
         refused('tp_layer_norm_backward', norm_args(P=P, B=B, W=W, dweight=FAKE, **ws), 'workspace')
 
 
+@pytest.mark.parametrize('bad', [dict(dx=None), dict(dx_dtype=1)])
+def test_layer_norm_member_sums_need_terms_in_fp32(bad):
+    refused('tp_layer_norm_backward', norm_args(dx_sum=FAKE, **{'dx_dtype': 0, **bad}), 'sum over the members')
+
+
 def test_layer_norm_workspace_sizes():
     size = _lib.load().tp_layer_norm_workspace_size
     assert size(0, 4, 4) == size(4, 0, 4) == size(4, 4, -1) == 0
