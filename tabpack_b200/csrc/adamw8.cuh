@@ -21,7 +21,7 @@
 // the point where the SM's issue slots and the memory take equally long.  So the fp32 arithmetic is
 // done in pairs (f32x2), the codes of a block are formed without the rules for subnormals, zeros and
 // empty blocks where a vote says that none is there, and the next blocks are on their way to shared
-// memory meanwhile.  209 M elements: 617 us, 5.5 TB/s, 86 % of a copy's rate.
+// memory meanwhile.  209 M elements: 607 us, 5.6 TB/s, 87 % of a copy's rate.
 #pragma once
 
 #include <cuda_fp8.h>
