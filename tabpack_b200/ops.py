@@ -819,7 +819,7 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq
             v, members = v.contiguous(), v.numel()
         hp.append(v)
     f32 = torch.float32
-    calls, a, used = [], None, 0
+    calls, a, used, count, written = [], None, 0, 0, set()
     for i, p in enumerate(params):
         g, m, ms, v, vs = grads[i], exp_avgs[i], exp_avg_scales[i], exp_avg_sqs[i], exp_avg_sq_scales[i]
         shape = p.shape
@@ -846,13 +846,15 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq
             a = _lib.AdamW8Args()
             calls.append(a)
             used = 0
-        a.t[used] = (p.data_ptr(), g.data_ptr(), m.data_ptr(), ms.data_ptr(), v.data_ptr(), vs.data_ptr(), st, numel,
-                     inner, (tensor_base + i) & 0xFFFFFFFF)
+        out = p.data_ptr(), m.data_ptr(), ms.data_ptr(), v.data_ptr(), vs.data_ptr()
+        written.update(out)
+        a.t[used] = (out[0], g.data_ptr(), *out[1:], st, numel, inner, (tensor_base + i) & 0xFFFFFFFF)
         used += 1
+        count += 1
         a.n_tensors = used
     hp = [_hparam(v) for v in hp]
-    if len({p.data_ptr() for p in params if p.numel()}) < sum(1 for p in params if p.numel()):
-        raise ValueError('a parameter appears twice')
+    if len(written) < 5 * count:
+        raise ValueError('a parameter or a state appears twice')
     # every argument is checked before the first launch
     for a in calls:
         a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = hp

@@ -285,6 +285,22 @@ def test_other_stream_and_graph():
             assert torch.equal(a, b)
 
 
+def test_a_state_given_twice_is_refused():
+    """Two parameters on one state, or both moments in one tensor, would be updated by two threads."""
+    from tabpack_b200 import ops
+
+    p, g, st = on_gpu(make([(2, 300), (2, 300)], seed=12))
+    before = [t.clone() for t in p]
+    for j in range(4):
+        bad = [list(t) for t in st]
+        bad[j][1] = bad[j][0]
+        with pytest.raises(ValueError, match='twice'):
+            ops.adamw8_step(p, g, *bad, **SCALAR, seed=1, step=1)
+    with pytest.raises(ValueError, match='twice'):
+        ops.adamw8_step(p, g, st[0], st[1], st[0], st[3], **SCALAR, seed=1, step=1)
+    assert all(torch.equal(a, b) for a, b in zip(p, before))
+
+
 def test_refusals():
     from tabpack_b200 import ops
 
