@@ -1,6 +1,7 @@
 // C ABI of the B200 packed-ensemble hot path (declared in include/tabpack_b200.h).
 // One translation unit: host-side validation, TMA descriptor encoding and kernel
 // dispatch for every entry point.
+#include <initializer_list>
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -160,6 +161,13 @@ int make_gather_map(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t 
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// All of them (or null) on boundaries of `size` bytes, a power of two.
+bool aligned_to(size_t size, std::initializer_list<const void*> pointers) {
+  uintptr_t all = 0;
+  for (const void* p : pointers) all |= reinterpret_cast<uintptr_t>(p);
+  return (all & (size - 1)) == 0;
+}
+size_t dtype_size(int dtype) { return dtype == TP_DTYPE_BF16 ? 2 : 4; }
 
 // Workspace of tp_linear_backward_noalloc (device memory reserved at module load).
 // Host code must not pass this symbol to a kernel: on the host it is only a
@@ -1598,8 +1606,6 @@ static int adamw8_tiles(int n, const int64_t* numel, const int64_t* inner, uint3
   }
 }
 
-static bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
-
 int tp_adamw8_step(const tp_adamw8_args* a, void* stream) {
   TP_PROF(TP_PROF_ADAMW, static_cast<cudaStream_t>(stream));
   if (!a || a->n_tensors <= 0 || a->n_tensors > TP_MAX_OPT_TENSORS) return fail(TP_EINVAL, "bad tensor count");
@@ -1611,8 +1617,8 @@ int tp_adamw8_step(const tp_adamw8_args* a, void* stream) {
     const tp_opt8_tensor& t = a->t[i];
     if (!t.p || !t.grad || !t.exp_avg || !t.exp_avg_scale || !t.exp_avg_sq || !t.exp_avg_sq_scale)
       return fail(TP_EINVAL, "tensor %d: null pointer", i);
-    if (!aligned4(t.p) || !aligned4(t.grad) || !aligned4(t.exp_avg_scale) || !aligned4(t.exp_avg_sq_scale))
-      return fail(TP_EALIGN, "tensor %d: fp32 data must be 4-byte aligned", i);
+    if (!aligned_to(4, {t.p, t.grad, t.exp_avg_scale, t.exp_avg_sq_scale}) || !aligned_to(8, {t.step}))
+      return fail(TP_EALIGN, "tensor %d: data not aligned to its type", i);
     any_scalar_step |= t.step == nullptr;
     numel[i] = t.numel;
     inner[i] = t.inner;
@@ -1670,6 +1676,8 @@ int tp_adamw8_moments(const tp_adamw8_moments_args* a, void* stream) {
     const tp_opt8_values& t = a->t[i];
     if (!t.exp_avg || !t.exp_avg_scale || !t.exp_avg_sq || !t.exp_avg_sq_scale || !t.m || !t.v)
       return fail(TP_EINVAL, "tensor %d: null pointer", i);
+    if (!aligned_to(4, {t.exp_avg_scale, t.exp_avg_sq_scale}) || !aligned_to(dtype_size(a->dtype), {t.m, t.v}))
+      return fail(TP_EALIGN, "tensor %d: data not aligned to its type", i);
     numel[i] = t.numel;
     inner[i] = t.inner;
     ts.t[i] = t;
@@ -1694,6 +1702,9 @@ static int check_layer_norm(const tp_layer_norm_args* a) {
   // (row numbers a few splits ahead stay in 32 bits)
   if ((int64_t)a->P * a->B > (1ll << 30) || a->W > (1 << 30))
     return fail(TP_EINVAL, "too many rows or columns for one layer norm call");
+  if (!aligned_to(dtype_size(a->dtype), {a->x, a->y, a->dy, a->dx_sum}) || !aligned_to(dtype_size(a->dx_dtype), {a->dx}) ||
+      !aligned_to(4, {a->n_features, a->weight, a->bias, a->mean, a->rstd, a->dweight, a->dbias}))
+    return fail(TP_EALIGN, "layer norm data not aligned to its type");
   return TP_OK;
 }
 
@@ -1878,7 +1889,7 @@ int tp_layer_norm_backward(const tp_layer_norm_args* a, void* stream) {
   const bool params = a->dweight || a->dbias;
   if (params) {
     const size_t need = tp_layer_norm_workspace_size(k.P, k.B, k.W);
-    if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned4(a->workspace)))
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned_to(4, {a->workspace})))
       return fail(TP_EINVAL, "layer norm workspace of %zu bytes is smaller than the %zu needed, or not aligned",
                   a->workspace_bytes, need);
     k.partial = static_cast<float*>(a->workspace);
@@ -1921,8 +1932,9 @@ static int check_label_log_probs(const tp_label_log_probs_args* a) {
   if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad logits dtype");
   if (!a->logits || !a->labels || (a->C > LP_REREAD && !a->stats))
     return fail(TP_EINVAL, "null logits, labels or statistics");
-  if (reinterpret_cast<uintptr_t>(a->logits) % (a->dtype == TP_DTYPE_BF16 ? 2 : 4) != 0)
-    return fail(TP_EALIGN, "the logits are not aligned to their type");
+  if (!aligned_to(dtype_size(a->dtype), {a->logits, a->dlogits}) || !aligned_to(8, {a->labels, a->top_label}) ||
+      !aligned_to(4, {a->log_prob, a->entropy, a->top_log_prob, a->stats, a->g_log_prob, a->g_entropy}))
+    return fail(TP_EALIGN, "label log probabilities: data not aligned to its type");
   if (a->label_rows <= 0 || a->rows % a->label_rows != 0)
     return fail(TP_EINVAL, "%lld labels do not divide %lld rows", (long long)a->label_rows, (long long)a->rows);
   if (a->logits_stride < a->C && a->rows > 1) return fail(TP_EINVAL, "rows of logits overlap");
@@ -2070,8 +2082,6 @@ int tp_label_log_probs_backward(const tp_label_log_probs_args* a, void* stream) 
   if ((a->g_log_prob_stride | a->g_entropy_stride) & ~1) return fail(TP_EINVAL, "gradient strides must be 0 or 1");
   const LogProbsArgs k = label_log_probs_args(a);
   const bool bf16 = a->dtype == TP_DTYPE_BF16;
-  if (reinterpret_cast<uintptr_t>(a->dlogits) % (bf16 ? 2 : 4) != 0)
-    return fail(TP_EALIGN, "the logits gradient is not aligned to its type");
   const int held = held_size(a, bf16 ? 2 : 4);
   rc = bf16 ? launch_log_probs_backward<__nv_bfloat16>(k, held, st) : launch_log_probs_backward<float>(k, held, st);
   if (rc) return rc;

@@ -93,6 +93,14 @@ def adamw_args(n=1, tensor=None, **kw):
     return a
 
 
+def moments_args(**kw):
+    a = _lib.AdamW8MomentsArgs(n_tensors=1, dtype=1)
+    t = dict(exp_avg=FAKE, exp_avg_scale=FAKE, exp_avg_sq=FAKE, exp_avg_sq_scale=FAKE, m=FAKE, v=FAKE, numel=256,
+             inner=128)
+    a.t[0] = _lib.Opt8Values(**{**t, **kw})
+    return a
+
+
 @pytest.mark.parametrize('bad', [dict(p=None), dict(grad=None), dict(exp_avg=None), dict(exp_avg_scale=None),
                                  dict(exp_avg_sq=None), dict(exp_avg_sq_scale=None), dict(numel=0), dict(inner=0),
                                  dict(numel=200), dict(inner=(1 << 33) + 1, numel=(1 << 33) + 1), dict(p=FAKE + 2),
@@ -111,6 +119,23 @@ def test_adamw8_argument_refusals():
     m = _lib.AdamW8MomentsArgs(n_tensors=1, dtype=2)
     refused('tp_adamw8_moments', m, 'dtype')
     refused('tp_adamw8_moments', _lib.AdamW8MomentsArgs(n_tensors=1, dtype=0), 'null')
+
+
+@pytest.mark.parametrize('call,args', [
+    ('tp_layer_norm_forward', lambda: norm_args(x=FAKE + 1)), ('tp_layer_norm_forward', lambda: norm_args(y=FAKE + 1)),
+    ('tp_layer_norm_forward', lambda: norm_args(weight=FAKE + 2)),
+    ('tp_layer_norm_backward', lambda: norm_args(dx_dtype=0, dx=FAKE + 2)),
+    ('tp_layer_norm_backward', lambda: norm_args(dtype=0, dx_dtype=0, dx_sum=FAKE + 2)),
+    ('tp_layer_norm_backward', lambda: norm_args(rstd=FAKE + 2)),
+    ('tp_label_log_probs_forward', lambda: labels_args(labels=FAKE + 4)),
+    ('tp_label_log_probs_forward', lambda: labels_args(top_k=1, top_log_prob=FAKE, top_label=FAKE + 4)),
+    ('tp_label_log_probs_forward', lambda: labels_args(log_prob=FAKE + 2)),
+    ('tp_label_log_probs_backward', lambda: labels_args(g_entropy=FAKE + 2)),
+    ('tp_adamw8_step', lambda: adamw_args(tensor=dict(step=FAKE + 4))),
+    ('tp_adamw8_moments', lambda: moments_args(m=FAKE + 1)),
+    ('tp_adamw8_moments', lambda: moments_args(exp_avg_sq_scale=FAKE + 2))])
+def test_misaligned_data_is_refused(call, args):
+    refused(call, args(), 'aligned')
 
 
 def test_cpu_tensors_are_refused():
