@@ -973,26 +973,26 @@ def layer_norm_backward(dy: Tensor, x: Tensor, weight: Tensor | None, mean: Tens
     for name, t in (('mean', mean), ('rstd', rstd)):
         if t.shape != (P, B) or t.dtype is not torch.float32 or t.get_device() != device or not t.is_contiguous():
             raise TypeError(f'{name} must be the contiguous fp32 ({P}, {B}) tensor of the forward')
-    dx = dw = db = ws = terms = None
+    dx = dw = db = None
+    # the members' terms of a shared input are added up before they are rounded
+    terms = 0
     if need_dx:
-        if x.ndim == 2:
-            dx = _empty2(B, W, dtype, x.device)
-            # the members' terms of a shared input are added up before they are rounded
-            terms = dx if P == 1 else torch.empty_strided((P, B, W), (B * W, W, 1), dtype=torch.float32, device=x.device)
-        else:
-            dx = terms = _empty_as(dy, dtype)
+        dx = _empty2(B, W, dtype, x.device) if x.ndim == 2 else _empty_as(dy, dtype)
+        terms = P * B * W if x.ndim == 2 and P > 1 else 0
     if need_dw:
         dw = _empty2(P, W, torch.float32, x.device)
     if need_db:
         db = _empty2(P, W, torch.float32, x.device)
     if P and B and W and (need_dx or need_dw or need_db):
         need = load().tp_layer_norm_workspace_size(P, B, W) if need_dw or need_db else 0
-        if need:
-            ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=x.device)
+        ws = None
+        if need or terms:
+            scratch = torch.empty_strided((terms + need // 4,), (1,), dtype=torch.float32, device=x.device)
+            ws = scratch.data_ptr()
         a = _lib.LayerNormArgs(P, B, W, code, sm, sr, _ptr(n_features), x.data_ptr(), _ptr(weight), None, 0.0, None,
-                               mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dm, dr, _ptr(terms),
-                               code if terms is dx else TP_DTYPE_F32, None if terms is dx else dx.data_ptr(), _ptr(dw),
-                               _ptr(db), _ptr(ws), need)
+                               mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dm, dr, ws if terms else _ptr(dx),
+                               TP_DTYPE_F32 if terms else code, dx.data_ptr() if terms else None, _ptr(dw), _ptr(db),
+                               ws + 4 * terms if need else None, need)
         _call('tp_layer_norm_backward', a, device)
     else:
         for t in (dx, dw, db):
