@@ -363,6 +363,34 @@ def test_other_stream_and_graph():
                 assert torch.equal(a, t)
 
 
+def test_split_rows_in_a_graph_and_on_two_streams():
+    """Rows spread over clusters, captured and replayed with new scores, and two such calls at once."""
+    from tabpack_b200 import ops
+
+    sets = [make((3,), 40000, torch.bfloat16, seed=s)[:2] for s in (31, 32)]
+    want = [ops.label_log_probs_forward(z, y, top_k=8) for z, y in sets]
+    z, y = (t.clone() for t in sets[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.label_log_probs_forward(z, y, top_k=8)
+    for (zs, ys), expected in zip(sets, want):
+        z.copy_(zs)
+        y.copy_(ys)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, expected))
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, (zs, ys), g in zip(streams, sets, got):
+            with torch.cuda.stream(s):
+                g.append(ops.label_log_probs_forward(zs, ys, top_k=8))
+    torch.cuda.synchronize()
+    for g, expected in zip(got, want):
+        assert all(torch.equal(a, b) for out in g for a, b in zip(out, expected))
+
+
 # ------------------------------------------------------------------ the function with autograd
 
 
