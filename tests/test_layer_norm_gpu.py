@@ -128,6 +128,14 @@ def test_rows_and_members(P, B, W, dtype):
 
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('P,B', [(2, 1), (3, 63), (2, 64), (2, 65), (1, 1000), (70, 33)])
+@pytest.mark.parametrize('W', [3, 16, 63, 64, 72, 128, 131, 136, 255, 256])
+def test_narrow_rows(W, P, B, dtype):
+    """Groups of 4, 8 and 16 lanes, whole and odd vectors, around a block's number of groups."""
+    run_and_check(*make(P, B, W, dtype, seed=W + B))
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize('W', [24, 130, 1024])
 def test_shared_input(W, dtype):
     run_and_check(*make(6, 37, W, dtype, shared=True, seed=W))
