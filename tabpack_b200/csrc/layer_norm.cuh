@@ -49,28 +49,47 @@ __device__ __forceinline__ int norm_width(const LayerNormArgs& a, int m) {
 
 constexpr int NORM_H = NORM_E / 2;  // pairs
 
-// V neighbouring elements are one vector: 16 bytes, or one element where nothing is aligned.
+// V neighbouring elements are one vector: 16 bytes, 8 or 4 where all rows start on such boundaries only,
+// or one element where nothing is aligned.
+template <int BYTES>
+struct NormWord {
+  typedef uint4 type;
+};
+template <>
+struct NormWord<8> {
+  typedef uint2 type;
+};
+template <>
+struct NormWord<4> {
+  typedef uint32_t type;
+};
+
 template <typename T, int V>
-__device__ __forceinline__ void norm_unpack(const uint4& u, f32x2* f) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-  if constexpr (sizeof(T) == 2) {
+__device__ __forceinline__ void norm_unpack(const char* from, f32x2* f) {
+  typedef typename NormWord<V * sizeof(T)>::type Word;
+  const Word u = *reinterpret_cast<const Word*>(from);
+  uint32_t w[sizeof(Word) / 4];
+  memcpy(w, &u, sizeof(Word));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = pair(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xFFFF0000u));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) f[e] = pair(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
-  }
+  for (int e = 0; e < V / 2; ++e)
+    f[e] = sizeof(T) == 2 ? pair(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xFFFF0000u))
+                          : pair(__uint_as_float(w[(2 * e) % (sizeof(Word) / 4)]),
+                                 __uint_as_float(w[(2 * e + 1) % (sizeof(Word) / 4)]));
 }
 
 template <typename T, int V>
 __device__ __forceinline__ void norm_store(T* p, const float* f) {
   if constexpr (V == 1) {
     *p = from_f32<T>(f[0]);
-  } else if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                                              pack_bf16x2(f[6], f[7]));
   } else {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+    typedef typename NormWord<V * sizeof(T)>::type Word;
+    uint32_t w[sizeof(Word) / 4];
+#pragma unroll
+    for (int e = 0; e < (int)sizeof(Word) / 4; ++e)
+      w[e] = sizeof(T) == 2 ? pack_bf16x2(f[(2 * e) % V], f[(2 * e + 1) % V]) : __float_as_uint(f[e % V]);
+    Word u;
+    memcpy(&u, w, sizeof(Word));
+    *reinterpret_cast<Word*>(p) = u;
   }
 }
 
@@ -119,7 +138,8 @@ struct NormGroup {
 template <typename T, int V, int G>
 struct NormRows {
   static constexpr int K = NORM_E / V, THREADS = NormGroup<G>::THREADS;
-  static constexpr int STAGE = V > 1 ? K * THREADS * 16 : 0;  // bytes of one row of every group
+  static constexpr int VB = V * sizeof(T);                    // bytes of a vector
+  static constexpr int STAGE = V > 1 ? K * THREADS * VB : 0;  // of one row of every group
   const T* p;     // the lane's first element of the next row to come
   int64_t step;   // elements to the row after
   int left;       // columns below n from the lane's first on
@@ -128,13 +148,13 @@ struct NormRows {
   __device__ static int c0(int k, int lane) { return (k * G + lane) * V; }
   // Rows first, first + by, ... of a member's `rows`.
   __device__ NormRows(const T* rows, int64_t stride, int first, int by, int lane, int n, char* shared, int stages)
-      : p(rows + first * stride + lane * V), step(by * stride), left(n - lane * V), ring(shared + threadIdx.x * 16) {
+      : p(rows + first * stride + lane * V), step(by * stride), left(n - lane * V), ring(shared + threadIdx.x * VB) {
     if constexpr (V > 1) {  // vectors without a column are never copied
 #pragma unroll
       for (int k = 0; k < K; ++k)
         if (left - k * G * V <= 0)
           for (int i = 0; i < stages; ++i)
-            *reinterpret_cast<uint4*>(ring + i * STAGE + k * THREADS * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<typename NormWord<VB>::type*>(ring + i * STAGE + k * THREADS * VB) = {};
     }
   }
   // The next row, if there is one, into stage `slot`.
@@ -144,10 +164,16 @@ struct NormRows {
       for (int k = 0; k < K; ++k) {
         const int have = left - k * G * V;
         if constexpr (V > 1) {
-          if (have > 0)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(ring) + slot * STAGE + k * THREADS * 16),
-                         "l"(p + k * G * V), "r"(min(have, V) * (int)sizeof(T))
-                         : "memory");
+          const uint32_t to = smem_u32(ring) + slot * STAGE + k * THREADS * VB, bytes = min(have, V) * sizeof(T);
+          if constexpr (VB == 16) {
+            if (have > 0)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(p + k * G * V), "r"(bytes)
+                           : "memory");
+          } else {
+            if (have > 0)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(p + k * G * V), "n"(VB), "r"(bytes)
+                           : "memory");
+          }
         } else {
           next[k] = have > 0 ? p[k * G] : from_f32<T>(0.f);
         }
@@ -160,7 +186,7 @@ struct NormRows {
     if constexpr (V > 1) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        norm_unpack<T, V>(*reinterpret_cast<const uint4*>(ring + slot * STAGE + k * THREADS * 16), f + k * V / 2);
+        norm_unpack<T, V>(ring + slot * STAGE + k * THREADS * VB, f + k * V / 2);
     } else {
 #pragma unroll
       for (int k = 0; k < NORM_H; ++k) f[k] = pair(to_f32<T>(next[2 * k]), to_f32<T>(next[2 * k + 1]));
@@ -416,6 +442,10 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
         const float2 u = halves(sw[k / 2]), v = halves(sb[k / 2]);
         to[0] = k % 2 ? u.y : u.x;
         to[HALF] = k % 2 ? v.y : v.x;
+      } else if constexpr (V == 2) {
+        const float2 u = halves(sw[k]), v = halves(sb[k]);
+        *reinterpret_cast<float2*>(to) = u;
+        *reinterpret_cast<float2*>(to + HALF) = v;
       } else {
 #pragma unroll
         for (int e = 0; e < V; e += 4) {

@@ -136,6 +136,18 @@ def test_narrow_rows(W, P, B, dtype):
 
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('shared', [False, True])
+@pytest.mark.parametrize('W,ld,at', [(12, 20, 0), (12, 20, 1), (12, 20, 2), (12, 20, 4), (20, 22, 0), (20, 22, 2), (10, 16, 6),
+                                     (100, 104, 4), (300, 304, 2), (1204, 1206, 2), (4002, 4004, 2)])
+def test_rows_on_every_boundary(W, ld, at, shared, dtype):
+    """Column slices at an offset: rows on boundaries of 2, 4, 8 and 16 bytes."""
+    x, dy, w, b, n = make(4, 21, ld, dtype, shared=shared, seed=W + at)
+    n = (n * W // ld).clamp(min=1).to(torch.int32)
+    cut = lambda t: t[..., at:at + W]  # noqa: E731
+    run_and_check(cut(x), cut(dy), cut(w).contiguous(), cut(b).contiguous(), n)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize('W', [24, 130, 1024])
 def test_shared_input(W, dtype):
     run_and_check(*make(6, 37, W, dtype, shared=True, seed=W))
