@@ -5,7 +5,7 @@
 //   dx = rstd (g - mean(g) - xhat mean(g xhat)) with g = dy w;  dw = sum_r dy xhat;  db = sum_r dy
 //
 // Memory bounds all of it: 4 bytes per element forward and 6 backward in bf16, 10 to 20
-// instructions.  Rows of up to NORM_HELD columns stay in the registers of a group of G lanes (8 to
+// instructions.  Rows of up to NORM_HELD columns stay in the registers of a group of G lanes (4 to
 // 512, 16 elements each), so x and dy are read once and the variance is summed around the mean.
 // A group walks over rows of one member: the member's w and b, and in the backward the columns' sums,
 // stay in registers, while the next rows are on their way to shared memory (asynchronous copies: one
