@@ -622,16 +622,19 @@ def _widths(buf: Tensor | None) -> Tensor | None:
 
 def _widths_cached(module: nn.Module, name: str, buf: Tensor | None) -> Tensor | None:
     """int32 copy of a width buffer, kept while the buffer is unchanged: one tensor per buffer
-    state, so caches may key on its identity."""
+    state, so caches may key on its identity.  The entry holds the buffer itself: a member
+    selection installs a buffer of its own, and the next one may get the address of the last."""
     if buf is None:
         return None
+    if buf.is_inference():  # without a version: a change would not be seen
+        return _widths(buf)
     cache = module.__dict__.setdefault('_widths_i32', {})
     key = (buf.data_ptr(), buf._version, buf.dtype, tuple(buf.shape))
     hit = cache.get(name)
-    if hit is None or hit[0] != key:
-        hit = (key, buf.to(torch.int32))
+    if hit is None or hit[0] is not buf or hit[1] != key:
+        hit = (buf, key, buf.to(torch.int32))
         cache[name] = hit
-    return hit[1]
+    return hit[2]
 
 
 # >>> module packs

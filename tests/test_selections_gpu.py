@@ -1,0 +1,38 @@
+"""Member selections in a row, captures and streams: a module's int32 widths and bf16 weights are those
+of the tensors that it holds at the call."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope='module', autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip('needs a GPU')
+
+
+def norm_pack(P=12, W=40):
+    from tabpack_b200.nn import LayerNormPack
+
+    pack = LayerNormPack([1 + (11 * i + 6) % W for i in range(P)], max_n_features=W, pack_size=P).cuda().eval()
+    gen = torch.Generator(device='cuda').manual_seed(0)
+    with torch.no_grad():
+        pack.weight.copy_(torch.rand(P, W, generator=gen, device='cuda'))
+        pack.bias.copy_(torch.rand(P, W, generator=gen, device='cuda'))
+    return pack, torch.randn(P, 7, W, generator=gen, device='cuda')
+
+
+SELECTIONS = [[0, 4, 7], [1, 2, 3], [11, 10, 9], [5, 0, 6], [2, 2, 8]]
+
+
+def test_layer_norm_selections_in_a_row():
+    """Equally many members each time, no call on the whole pack between."""
+    pack, x = norm_pack()
+    with torch.no_grad():
+        picks = [torch.tensor(s, device='cuda') for s in SELECTIONS]
+        want = [pack(x[i], i) for i in picks]
+        for i, t in zip(picks, want):
+            with pack.temporarily_select(pack_idx=i):
+                assert torch.equal(pack(x[i]), t)
