@@ -293,6 +293,26 @@ def _reusable(buf: Tensor | None, shape, dtype: torch.dtype, device) -> bool:
     return use_count is not None and use_count() == 1
 
 
+class _Same:
+    """Equal for one living tensor object only.  An address and a version do not tell a tensor: one that
+    a member selection installs may lie where the last selection's lay, at the same version."""
+
+    __slots__ = ('ref',)
+    __hash__ = None
+
+    def __init__(self, t: Tensor) -> None:
+        self.ref = weakref.ref(t)
+
+    def __eq__(self, other) -> bool:
+        t = self.ref()
+        return t is not None and isinstance(other, _Same) and other.ref() is t
+
+
+def _state(t: Tensor | None):
+    """What a cache compares to tell whether `t` is the tensor that it saw, unchanged."""
+    return None if t is None else (_Same(t), t.data_ptr(), t._version, tuple(t.shape))
+
+
 class _WeightCache:
     """bf16 copy of an fp32 weight pack, refreshed when the weight changes (optimizer steps
     and in-place updates bump the parameter's version counter).
@@ -306,17 +326,13 @@ class _WeightCache:
         self.key = None
         self.value = None
 
-    @staticmethod
-    def _tag(t):
-        return None if t is None else (t.data_ptr(), t._version, tuple(t.shape))
-
     def get(self, w: Tensor, dtype: torch.dtype, cols: int, rows: int | None = None, widths=None) -> Tensor:
         rows = w.shape[-2] if rows is None else rows
         if w.dtype == dtype and w.shape[-1] == cols and w.shape[-2] == rows:
             return w.detach()
         out_f, in_f, nb, bi = widths if widths is not None else (None, None, None, 0)
         key = (w.data_ptr(), w._version, dtype, cols, rows, tuple(w.shape),
-               self._tag(out_f), self._tag(in_f), self._tag(nb), bi)
+               _state(out_f), _state(in_f), _state(nb), bi, _Same(w))
         if self.key != key:
             self.key = None
             if dtype == torch.bfloat16 and w.dtype == torch.float32 and w.is_cuda and w.is_contiguous():
@@ -340,7 +356,8 @@ class _WeightCache:
         when it holds `w`'s current values (its key is at `w`'s present version) and nothing but
         this cache holds it; else None, and the next forward casts again."""
         key, buf = self.key, self.value
-        if key is None or buf is None or key[0] != w.data_ptr() or key[1] != w._version or key[2] != torch.bfloat16:
+        if (key is None or buf is None or key[0] != w.data_ptr() or key[1] != w._version or key[2] != torch.bfloat16
+                or key[-1] != _Same(w)):
             return None
         if buf is w or not _reusable(buf, tuple(buf.shape), torch.bfloat16, w.device):
             return None
@@ -390,7 +407,7 @@ class _OneHotWeightCache:
         self.onehot_t = None
 
     def get(self, w: Tensor, out_f: Tensor | None, n_dense: int, rows: int, dense_cols: int) -> tuple[Tensor, Tensor]:
-        key = (w.data_ptr(), w._version, tuple(w.shape), _WeightCache._tag(out_f), n_dense, rows, dense_cols)
+        key = (_state(w), _state(out_f), n_dense, rows, dense_cols)
         if self.key != key:
             self.key = None
             P, _, C = w.shape
@@ -538,12 +555,10 @@ def packed_linear(x: Tensor, weight: Tensor, bias: Tensor | None, *, in_features
         kw['row_index'] = row_index
     cfg = {'kw': kw, 'w_shape': tuple(weight.shape), 'in_cols': in_cols, 'dx_cols': int(dx_cols)}
     if dw_slot is not None:
-        tag = lambda t: None if t is None else (t.data_ptr(), t._version, tuple(t.shape))  # noqa: E731
         cfg['dw_slot'] = dw_slot
-        cfg['dw_key'] = (tag(out_features), tag(in_features), tag(n_blocks), int(block_index))
+        cfg['dw_key'] = (_state(out_features), _state(in_features), _state(n_blocks), int(block_index))
     if y_slot is not None and dtype == torch.bfloat16 and torch.is_grad_enabled():
-        tag = lambda t: None if t is None else (t.data_ptr(), t._version, tuple(t.shape))  # noqa: E731
-        key = (tag(out_features), tag(in_features), tag(n_blocks), int(block_index))
+        key = (_state(out_features), _state(in_features), _state(n_blocks), int(block_index))
         if rows == max_out:
             cfg['y_slot'], cfg['y_key'] = y_slot.setdefault('y', {}), key
         if x.ndim == 3 and cols == in_cols and row_index is None and not dx_cols:

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from tabpack_b200.nn import LayerNormPack, LinearPack, _widths_cached
+from tabpack_b200.nn import LayerNormPack, LinearPack, _state, _WeightCache, _widths_cached
 
 
 def test_widths_of_another_buffer_at_the_same_address():
@@ -47,3 +47,48 @@ def test_widths_are_kept_until_the_buffer_changes():
         assert _widths_cached(module, 'n', made).tolist() == [6, 1]
         made[0] = 2
         assert _widths_cached(module, 'n', made).tolist() == [2, 1]
+
+
+def test_bf16_copy_of_another_weight_at_the_same_address():
+    memory = np.ones((2, 8, 8), np.float32)
+    cache, first = _WeightCache(), torch.from_numpy(memory)
+    copy = cache.get(first, torch.bfloat16, 8)
+    assert (copy == 1).all() and cache.get(first, torch.bfloat16, 8) is copy
+    memory[:] = 2
+    second = torch.from_numpy(memory)
+    assert second.data_ptr() == first.data_ptr() and second._version == first._version
+    assert (cache.get(second, torch.bfloat16, 8) == 2).all()
+    assert cache.begin_update(first) is None
+    second.fill_(3)
+    assert (cache.get(second, torch.bfloat16, 8) == 3).all()
+
+
+def test_bf16_copy_follows_the_widths():
+    """A copy made for one set of widths is not taken for another set at the same address."""
+    memory, w = np.array([8, 8], np.int32), torch.ones(2, 8, 8)
+    cache, a = _WeightCache(), torch.from_numpy(memory)
+    copy = cache.get(w, torch.bfloat16, 8, widths=(a, None, None, 0))
+    assert cache.get(w, torch.bfloat16, 8, widths=(a, None, None, 0)) is copy
+    assert cache.get(w, torch.bfloat16, 8, widths=(torch.from_numpy(memory), None, None, 0)) is not copy
+
+
+def test_states_of_tensors():
+    t = torch.zeros(3)
+    assert _state(t) == _state(t) and _state(None) is None and _state(t) != _state(t.view(3))
+    before = _state(t)
+    t += 1
+    assert _state(t) != before
+    gone = _state(torch.zeros(3))
+    assert gone != gone[:0] + _state(torch.zeros(3)) and not gone[0] == gone[0]
+
+
+@pytest.mark.parametrize('k', [3, 300])
+def test_bf16_copies_of_selections_in_a_row(k):
+    linear = LinearPack(8, 8, pack_size=3000).eval()
+    with torch.no_grad():
+        linear.weight.copy_(torch.arange(3000.0)[:, None, None].bfloat16().expand(3000, 8, 8))
+        for i in range(20):
+            idx = torch.arange(k) * 7 + 31 * i
+            with linear.temporarily_select(pack_idx=idx):
+                copy = linear._cache.get(linear.weight, torch.bfloat16, 8)
+                assert torch.equal(copy.float(), linear.weight)

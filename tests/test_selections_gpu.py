@@ -36,3 +36,37 @@ def test_layer_norm_selections_in_a_row():
         for i, t in zip(picks, want):
             with pack.temporarily_select(pack_idx=i):
                 assert torch.equal(pack(x[i]), t)
+
+
+@pytest.mark.parametrize('ragged', [False, True])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_linear_selections_in_a_row(ragged, dtype):
+    from tabpack_b200.nn import LinearPack
+
+    P = 12
+    torch.manual_seed(1)
+    linear = LinearPack(24, [8 + (5 * i) % 33 for i in range(P)] if ragged else 40, max_out_features=40,
+                        pack_size=P).cuda().eval()
+    x = torch.randn(P, 9, 24, device='cuda').to(dtype)
+    with torch.no_grad():
+        picks = [torch.tensor(s, device='cuda') for s in SELECTIONS]
+        want = [linear(x[i], i) for i in picks]
+        for i, t in zip(picks, want):
+            with linear.temporarily_select(pack_idx=i):
+                assert torch.equal(linear(x[i]), t)
+
+
+def test_one_hot_weights_of_another_tensor_at_the_same_address():
+    from tabpack_b200.nn import _OneHotWeightCache
+
+    memory = torch.empty(2, 16, 12, device='cuda')
+    view = lambda: torch.empty(0, device='cuda').set_(memory.untyped_storage(), 0, memory.shape)  # noqa: E731
+    cache, got = _OneHotWeightCache(), []
+    for value in (1.0, 2.0):
+        memory.fill_(value)
+        w = view()
+        got.append([t.clone() for t in cache.get(w, None, 4, 16, 8)])
+        assert cache.get(w, None, 4, 16, 8)[0] is cache.dense
+        del w
+    for a, b in zip(*got):
+        assert torch.equal(2 * a, b)
