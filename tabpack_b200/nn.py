@@ -898,7 +898,9 @@ class LayerNormPack(ModulePack):
             raise ValueError('The epsilon value must be finite and positive')
         buf, max_n = _positive_int_pack(n_features, max_n_features, pack_size=pack_size)
         super().__init__()
-        self.register_buffer('n_features', None if buf is None else _mark_buffer(buf.to(device)))
+        # int32, as the kernels read it: a call converts and keeps nothing, so that one on another stream or in
+        # a graph, and a graph's replays, see the buffer itself
+        self.register_buffer('n_features', None if buf is None else _mark_buffer(buf.to(device, torch.int32)))
         self._max_n_features = max_n
         self.eps = float(eps)
         shape = (pack_size, max_n)
@@ -950,9 +952,8 @@ class LayerNormPack(ModulePack):
         if pack_idx is not None:
             check_pack_idx(pack_idx, P)
             w, b, n = (_select(t, pack_idx) for t in (w, b, n))
-            n, P = _widths(n), len(pack_idx)
-        else:
-            n = _widths_cached(self, 'n', n)
+            P = len(pack_idx)
+        n = _widths(n)
         if x.shape[PACK_DIM] not in (1, x.shape[PACK_DIM] if P is None else P):
             raise ValueError('The pack dimension of the input must match the selected pack size')
         if (w is not None or n is not None) and P > 1 and (x.shape[PACK_DIM] == 1 or x.stride(PACK_DIM) == 0):

@@ -92,3 +92,14 @@ def test_bf16_copies_of_selections_in_a_row(k):
             with linear.temporarily_select(pack_idx=idx):
                 copy = linear._cache.get(linear.weight, torch.bfloat16, 8)
                 assert torch.equal(copy.float(), linear.weight)
+
+
+def test_layer_norm_widths_are_kept_as_the_kernels_read_them():
+    """int32, through construction, replacement and a checkpoint written with other integers."""
+    pack = LayerNormPack([3, 5], pack_size=2)
+    state = {**pack.state_dict(), 'n_features': torch.tensor([4, 2])}
+    pack.load_state_dict(state)
+    assert pack.n_features.dtype == torch.int32 and pack.n_features.tolist() == [4, 2]
+    pack.replace(pack_idx=torch.tensor([1]), n_features=[5])
+    pack.load_state_dict_at(state, pack_idx=torch.tensor([0]), state_dict_idx=torch.tensor([1]))
+    assert pack.n_features.dtype == torch.int32 and pack.n_features.tolist() == [2, 5]

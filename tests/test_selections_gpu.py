@@ -70,3 +70,20 @@ def test_one_hot_weights_of_another_tensor_at_the_same_address():
         del w
     for a, b in zip(*got):
         assert torch.equal(2 * a, b)
+
+
+def test_layer_norm_captured_first():
+    """A graph may hold a pack's first call, and its replays follow the members' widths."""
+    pack, x = norm_pack()
+    every = torch.arange(12, device='cuda')
+    with torch.no_grad():
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = pack(x)
+        assert torch.equal(pack(x), pack(x, every))
+        graph.replay()
+        assert torch.equal(y, pack(x))
+        pack.replace(pack_idx=torch.tensor([3, 5], device='cuda'), n_features=[40, 2])
+        graph.replay()
+        assert torch.equal(y, pack(x, every)) and torch.equal(y, pack(x))
