@@ -313,6 +313,12 @@ def _state(t: Tensor | None):
     return None if t is None else (_Same(t), t.data_ptr(), t._version, tuple(t.shape))
 
 
+def _capturing(t: Tensor) -> bool:
+    """True while calls on `t` are recorded into a CUDA graph: what they write is there after a replay
+    only, so no later call may take it from a cache."""
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class _WeightCache:
     """bf16 copy of an fp32 weight pack, refreshed when the weight changes (optimizer steps
     and in-place updates bump the parameter's version counter).
@@ -334,6 +340,8 @@ class _WeightCache:
         key = (w.data_ptr(), w._version, dtype, cols, rows, tuple(w.shape),
                _state(out_f), _state(in_f), _state(nb), bi, _Same(w))
         if self.key != key:
+            if _capturing(w):
+                self = _WeightCache()
             self.key = None
             if dtype == torch.bfloat16 and w.dtype == torch.float32 and w.is_cuda and w.is_contiguous():
                 shape = (w.shape[0], rows, cols)
@@ -409,6 +417,8 @@ class _OneHotWeightCache:
     def get(self, w: Tensor, out_f: Tensor | None, n_dense: int, rows: int, dense_cols: int) -> tuple[Tensor, Tensor]:
         key = (_state(w), _state(out_f), n_dense, rows, dense_cols)
         if self.key != key:
+            if _capturing(w):
+                self = _OneHotWeightCache()
             self.key = None
             P, _, C = w.shape
             n_onehot = C - n_dense
@@ -647,6 +657,8 @@ def _widths_cached(module: nn.Module, name: str, buf: Tensor | None) -> Tensor |
     key = (buf.data_ptr(), buf._version, buf.dtype, tuple(buf.shape))
     hit = cache.get(name)
     if hit is None or hit[0] is not buf or hit[1] != key:
+        if _capturing(buf):
+            return _widths(buf)
         hit = (buf, key, buf.to(torch.int32))
         cache[name] = hit
     return hit[2]
@@ -1132,6 +1144,8 @@ class MLPBackbonePack(ModulePack):
             return nb.to(torch.int32)
         key = (self.n_blocks.data_ptr(), self.n_blocks._version if not self.n_blocks.is_inference() else -1)
         if self._nb_cache is None or self._nb_cache[0] != key:
+            if _capturing(nb):
+                return nb.to(torch.int32)
             self._nb_cache = (key, nb.to(torch.int32))
         return self._nb_cache[1]
 

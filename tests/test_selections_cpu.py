@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+from tabpack_b200 import nn
 from tabpack_b200.nn import LayerNormPack, LinearPack, _state, _WeightCache, _widths_cached
 
 
@@ -103,3 +104,21 @@ def test_layer_norm_widths_are_kept_as_the_kernels_read_them():
     pack.replace(pack_idx=torch.tensor([1]), n_features=[5])
     pack.load_state_dict_at(state, pack_idx=torch.tensor([0]), state_dict_idx=torch.tensor([1]))
     assert pack.n_features.dtype == torch.int32 and pack.n_features.tolist() == [2, 5]
+
+
+def test_copies_recorded_into_a_graph_are_not_kept(monkeypatch):
+    """While a graph is captured nothing is computed: what it will write on a replay is no one else's copy, and a
+    copy that was there before is taken as it is."""
+    monkeypatch.setattr(nn, '_capturing', lambda t: True)
+    module, buf = torch.nn.Module(), torch.tensor([3, 5])
+    cache, w = _WeightCache(), torch.ones(2, 8, 8)
+    backbone = nn.MLPBackbonePack(d_in=4, n_blocks=[1, 2], d_block=[8, 8], dropout=0.0, pack_size=2)
+    widths, copy, depths = _widths_cached(module, 'n', buf), cache.get(w, torch.bfloat16, 8), backbone._n_blocks_i32(None)
+    assert widths.tolist() == [3, 5] and (copy == 1).all() and depths.tolist() == [1, 2]
+    assert cache.key is None and cache.value is None and backbone._nb_cache is None
+    monkeypatch.undo()
+    kept = _widths_cached(module, 'n', buf), cache.get(w, torch.bfloat16, 8), backbone._n_blocks_i32(None)
+    assert kept[0] is not widths and kept[1] is not copy and kept[2] is not depths
+    monkeypatch.setattr(nn, '_capturing', lambda t: True)
+    assert _widths_cached(module, 'n', buf) is kept[0] and cache.get(w, torch.bfloat16, 8) is kept[1]
+    assert backbone._n_blocks_i32(None) is kept[2]

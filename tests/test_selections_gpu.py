@@ -87,3 +87,24 @@ def test_layer_norm_captured_first():
         pack.replace(pack_idx=torch.tensor([3, 5], device='cuda'), n_features=[40, 2])
         graph.replay()
         assert torch.equal(y, pack(x, every)) and torch.equal(y, pack(x))
+
+
+def test_linear_captured_first():
+    """A layer's first call recorded into a graph: a call outside makes its own copies of widths and weights."""
+    from tabpack_b200.nn import LinearPack
+
+    torch.manual_seed(2)
+    linear = LinearPack(24, [8 + (5 * i) % 33 for i in range(12)], max_out_features=40, pack_size=12).cuda().eval()
+    x = torch.randn(12, 9, 24, device='cuda').bfloat16()
+    every = torch.arange(12, device='cuda')
+    with torch.no_grad():
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = linear(x)
+        assert torch.equal(linear(x), linear(x, every))
+        graph.replay()
+        assert torch.equal(y, linear(x))
+        linear.weight.mul_(2)
+        graph.replay()
+        assert torch.equal(y, linear(x))
