@@ -852,12 +852,12 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq
         used += 1
         count += 1
         a.n_tensors = used
-    hp = [_hparam(v) for v in hp]
+    values = [_hparam(v) for v in hp]  # bare pointers: `hp` holds the contiguous copies until the last launch
     if len(written) < 5 * count:
         raise ValueError('a parameter or a state appears twice')
     # every argument is checked before the first launch
     for a in calls:
-        a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = hp
+        a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = values
         a.step, a.seed = int(step), int(seed) & 0xFFFFFFFFFFFFFFFF
         a.member_base = int(member_base) & 0xFFFFFFFF
         _call('tp_adamw8_step', a, device)

@@ -482,3 +482,24 @@ def test_muon_pack_with_8_bit_rest():
     # the first step takes the same unrounded moments
     assert torch.equal(out[0][0], out[1][0])
     assert torch.allclose(out[0][1], out[1][1], rtol=0, atol=1e-3 * 64 * U + 3 * U)
+
+
+def test_strided_member_hyperparameters(monkeypatch):
+    """A column of a table of hyperparameters: its copy lives until the launch, whatever is allocated before."""
+    from tabpack_b200 import ops
+
+    P = 5
+    ts = make([(P, 33, 20), (P, 256)], seed=13)
+    hp = per_member(P, seed=4)
+    call, taken = ops._call, []
+
+    def busy(*args):
+        taken.extend(torch.full((P,), float('nan'), device='cuda') for _ in range(64))
+        call(*args)
+
+    monkeypatch.setattr(ops, '_call', busy)
+    p, g, st = on_gpu(ts)
+    table = torch.stack([torch.from_numpy(v) for v in hp.values()], 1).cuda()
+    ops.adamw8_step(p, g, *st, step=3, seed=17, **{k: table[:, i] for i, k in enumerate(hp)})
+    check(ts, p, st, hp, 3, 17)
+    assert len(taken) == 64
