@@ -393,6 +393,7 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
     const float mu = nmean, rs = nrstd;
     mean += step;
     rstd += step;
+    nmean = nrstd = 0.f;  // beyond the last row: xhat = 0, times dy = 0
     if (r + step < a.B) nmean = *mean, nrstd = *rstd;
     x.issue((i + AHEAD) % D, r + AHEAD * step < a.B);
     dy.issue((i + AHEAD) % D, r + AHEAD * step < a.B);
@@ -400,6 +401,16 @@ __global__ void __launch_bounds__(NormGroup<G>::THREADS, NormGroup<G>::THREADS >
     if (!live) {
 #pragma unroll
       for (int h = 0; h < NORM_H; ++h) g[h] = xh[h] = pair(0.f, 0.f);
+    }
+    // columns from n on hold x = 0: where -mean rstd is no number of fp32 they take x = mean, since an infinite
+    // xhat times dy = 0 would make the row's sum a NaN
+    if (!(fabsf(mu * rs) < INFINITY)) {
+#pragma unroll
+      for (int h = 0; h < NORM_H; ++h) {
+        const int c = Rows::c0(2 * h / V, lane) + 2 * h % V, d = V == 1 ? c + G : c + 1;
+        const float2 t = halves(xh[h]);
+        xh[h] = pair(c < n ? t.x : mu, d < n ? t.y : mu);
+      }
     }
     const f32x2 minus = pair(-mu, -mu), scale = pair(rs, rs);
     f32x2 s1 = pair(0.f, 0.f), s2 = s1;

@@ -509,3 +509,48 @@ def test_refusals():
     grad, = torch.autograd.grad(out.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         grad.sum().backward()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('W,n,B,value,eps', [
+    (W, n, B, 2.0**80, 1e-30) for W, n, B in [(72, 64, 40), (77, 64, 70), (300, 256, 9), (301, 256, 19), (2000, 1024, 5),
+                                              (2001, 1024, 3), (4096, 4096, 7), (6000, 4096, 2), (9000, 8192, 3)]
+] + [(72, 64, 40, 2.0**120, 1e-5), (77, 64, 70, 2.0**120, 1e-5)])
+def test_large_constant_rows(W, n, B, value, eps, dtype):
+    """Rows of one large power of two, as many columns as a power of two: mean and variance are exact, xhat is 0
+    (64 x 2^120 and 8192 x 2^80 are numbers of fp32).  |mean| rstd leaves the fp32 range, so a column that is not
+    part of the row, taken as x = 0, would bring in an infinity.  dx = rstd (dy w - mean(dy w)): D + 16 roundings
+    of the magnitudes."""
+    from tabpack_b200 import ops
+
+    x, dy, w, b, _ = make(2, B, W, dtype, ragged=False, seed=W)
+    x.fill_(value)
+    k = torch.full((2,), n, dtype=torch.int32, device='cuda')
+    y, mean, rstd = ops.layer_norm_forward(x, w, b, n_features=k, eps=eps)
+    assert (mean == value).all()
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, mean, rstd, n_features=k)
+    assert torch.equal(y[..., :n], b[:, None, :n].to(dtype).expand(2, B, n)) and (y[..., n:] == 0).all()
+    assert torch.equal(dw, torch.zeros_like(dw)) and (db[:, n:] == 0).all()
+    dy64 = dy[..., :n].double()
+    g, r = dy64 * w[:, None, :n].double(), 1 / float(eps) ** 0.5
+    want = r * (g - g.mean(2, keepdim=True))
+    tol = U * (D + 16) * r * (g.abs() + g.abs().mean(2, keepdim=True))
+    check(dx[..., :n], want, tol, dtype, 'dx')
+    check(db[:, :n], dy64.sum(1), U * (B + 4) * dy64.abs().sum(1), torch.float32, 'db')
+    assert (dx[..., n:] == 0).all()
+
+
+def test_large_constant_rows_of_a_shared_input():
+    from tabpack_b200 import ops
+
+    x, dy, w, b, _ = make(3, 21, 72, torch.float32, shared=True, seed=1)
+    x.fill_(2.0**120)
+    k = torch.full((3,), 64, dtype=torch.int32, device='cuda')
+    y, mean, rstd = ops.layer_norm_forward(x, w, b, n_features=k)
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, mean, rstd, n_features=k)
+    g = dy[..., :64].double() * w[:, None, :64].double()
+    r = 1e-5**-0.5
+    want = (r * (g - g.mean(2, keepdim=True))).sum(0)
+    size = (r * (g.abs() + g.abs().mean(2, keepdim=True))).sum(0)
+    check(dx[:, :64], want, U * (D + 20) * size, torch.float32, 'dx')
+    assert (dx[:, 64:] == 0).all() and (dw == 0).all() and torch.isfinite(db).all()
