@@ -563,12 +563,13 @@ def optimizer_pack_reset_state(optimizer, *, pack_idx: Tensor) -> None:
 
 
 def should_skip_weight_decay(module_name: str, module, parameter_name: str, parameter) -> bool:
-    """`should_skip_weight_decay` (`optim.py:929-943`) for the packs of this package: biases
-    and the frequencies of cosine embeddings take no weight decay."""
+    """`should_skip_weight_decay` (`optim.py:929-943`) for the packs of this package: biases,
+    the frequencies of cosine embeddings and the scales of layer norms take no weight decay."""
     del module_name
-    from tabpack_b200.nn import CosineEmbeddingsPack
+    from tabpack_b200.nn import CosineEmbeddingsPack, LayerNormPack
 
-    return parameter_name.endswith('bias') or (isinstance(module, CosineEmbeddingsPack) and parameter is module.weight)
+    return parameter_name.endswith('bias') or (isinstance(module, (CosineEmbeddingsPack, LayerNormPack))
+                                               and parameter is module.weight)
 
 
 def split_weight_decay(model) -> tuple[list, list]:

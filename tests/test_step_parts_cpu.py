@@ -242,3 +242,14 @@ def test_oracle_codes_round_to_neighbours():
         again, s2 = store(load(codes, s), rng.integers(0, 65536, y.shape))
         kept = np.abs(load(again, s2) - load(codes, s)) <= 4 * 2.0**-24 * np.abs(load(codes, s))
         assert kept.mean() >= 0.99  # a value an ulp below its code is rounded down by 1 in 2^16
+
+
+def test_layer_norm_takes_no_weight_decay():
+    from tabpack_b200.nn import LinearPack
+    from tabpack_b200.optim import split_weight_decay
+
+    model = torch.nn.Sequential(LinearPack(4, 8, pack_size=2), LayerNormPack(8, pack_size=2),
+                                LayerNormPack(8, bias=False, pack_size=2), LinearPack(8, 3, pack_size=2))
+    decay, no_decay = split_weight_decay(model)
+    assert [id(p) for p in decay] == [id(model[0].weight), id(model[3].weight)]
+    assert len(no_decay) == len(list(model.parameters())) - 2
