@@ -878,8 +878,8 @@ class _LayerNormFn(torch.autograd.Function):
     """`ops.layer_norm_forward` / `ops.layer_norm_backward`; statistics and parameters in fp32."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, n_features, eps):
-        y, mean, rstd = ops.layer_norm_forward(x, weight, bias, n_features=n_features, eps=eps)
+    def forward(ctx, x, weight, bias, n_features, eps, pack_size):
+        y, mean, rstd = ops.layer_norm_forward(x, weight, bias, n_features=n_features, eps=eps, pack_size=pack_size)
         ctx.save_for_backward(x, weight, mean, rstd, n_features)
         return y
 
@@ -890,7 +890,7 @@ class _LayerNormFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx, dw, db = ops.layer_norm_backward(dy, x, weight, mean, rstd, n_features=n_features, need_dx=need[0],
                                              need_dw=need[1], need_db=need[2])
-        return dx, dw, db, None, None
+        return dx, dw, db, None, None, None
 
 
 class LayerNormPack(ModulePack):
@@ -966,11 +966,16 @@ class LayerNormPack(ModulePack):
             w, b, n = (_select(t, pack_idx) for t in (w, b, n))
             P = len(pack_idx)
         n = _widths(n)
-        if x.shape[PACK_DIM] not in (1, x.shape[PACK_DIM] if P is None else P):
+        size = x.shape[PACK_DIM]
+        if size not in (1, size if P is None else P):
             raise ValueError('The pack dimension of the input must match the selected pack size')
-        if (w is not None or n is not None) and P > 1 and (x.shape[PACK_DIM] == 1 or x.stride(PACK_DIM) == 0):
+        if size > 1:
+            P, shared = size, x.stride(PACK_DIM) == 0
+        else:  # without parameters or widths the members' rows are the same, and stay one
+            shared = (w is not None or n is not None) and P > 1
+        if shared:
             x = x[0]  # rows that the members share: their gradient is added up in fp32
-        return _LayerNormFn.apply(x, w, b, n, self.eps)
+        return _LayerNormFn.apply(x, w, b, n, self.eps, P if shared else None)
 
 
 class LabelLogProbs(NamedTuple):

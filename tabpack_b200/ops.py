@@ -923,10 +923,11 @@ def _norm_rows(name: str, t: Tensor, dtype: torch.dtype, device: int, shape: tup
 
 
 def layer_norm_forward(x: Tensor, weight: Tensor | None, bias: Tensor | None, *, n_features: Tensor | None = None,
-                       eps: float = 1e-5) -> tuple[Tensor, Tensor, Tensor]:
+                       eps: float = 1e-5, pack_size: int | None = None) -> tuple[Tensor, Tensor, Tensor]:
     """Layer norm of x (P, B, W), or (B, W) shared by the members, bf16 or fp32, with each member's
     own weight and bias (P, W) fp32 or None; see `tp_layer_norm_forward`.  `n_features` (P,): member
     m's rows are normalised over their first n_features[m] columns, the others are zero in y.
+    `pack_size`: P, where a shared x has nothing else that tells it (1 if not given).
     Returns (y (P, B, W), mean (P, B), rstd (P, B)); the backward takes the last two."""
     if not 0.0 <= eps < float('inf'):
         raise ValueError('eps must be finite and not negative')
@@ -936,9 +937,15 @@ def layer_norm_forward(x: Tensor, weight: Tensor | None, bias: Tensor | None, *,
     code = _dtype_code(dtype)
     if x.ndim == 3:
         P, B, W = x.shape
+        if pack_size not in (None, P):
+            raise ValueError(f'x has {P} members, not {pack_size}')
     else:
         B, W = x.shape
-        P = next((t.shape[0] for t in (weight, bias, n_features) if t is not None), 1)
+        if pack_size is not None and pack_size < 0:
+            raise ValueError('the pack size must not be negative')
+        P = pack_size
+        if P is None:
+            P = next((t.shape[0] for t in (weight, bias, n_features) if t is not None), 1)
     x, sm, sr = _norm_rows('x', x, dtype, device, (P, B, W))
     weight = _operand('weight', weight, (P, W), torch.float32, device)
     bias = _operand('bias', bias, (P, W), torch.float32, device)

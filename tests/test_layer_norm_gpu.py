@@ -554,3 +554,42 @@ def test_large_constant_rows_of_a_shared_input():
     size = (r * (g.abs() + g.abs().mean(2, keepdim=True))).sum(0)
     check(dx[:, :64], want, U * (D + 20) * size, torch.float32, 'dx')
     assert (dx[:, 64:] == 0).all() and (dw == 0).all() and torch.isfinite(db).all()
+
+
+@pytest.mark.parametrize('P', [2, 64])
+def test_module_without_parameters_adds_a_shared_gradient_in_fp32(P):
+    """bf16 rows that the members share: their gradient is rounded once, whatever the number of members."""
+    from tabpack_b200 import nn as tnn
+
+    pack = tnn.LayerNormPack(24, elementwise_affine=False, pack_size=P).cuda()
+    x = torch.randn(5, 24, device='cuda').bfloat16().requires_grad_()
+    dy = torch.randn(P, 5, 24, device='cuda').bfloat16()
+    y = pack(x.expand(P, -1, -1))
+    assert y.shape == (P, 5, 24)
+    y.backward(dy)
+    want = tol = 0
+    for m in range(P):
+        one, room = plain(x.detach(), None, None, 24, pack.eps, dy[m])
+        want, tol = want + one[1], tol + room[1] + U * (P + 1) * one[1].abs()
+        check(y[m].detach(), one[0], room[0], torch.bfloat16, f'y of member {m}')
+    check(x.grad, want, tol, torch.bfloat16, 'dx')
+    # selected members, and rows with a pack dimension of their own
+    idx = torch.arange(P - 1, device='cuda')
+    assert torch.equal(pack(x.detach().expand(P - 1, -1, -1), idx), y.detach()[:-1])
+    assert torch.equal(pack(x.detach()[None]), y.detach()[:1])
+    assert torch.equal(pack(x.detach().repeat(P, 1, 1)), y.detach())
+
+
+def test_pack_size_of_a_shared_input():
+    from tabpack_b200 import ops
+
+    x, _, w, _, _ = make(3, 6, 16, torch.float32, shared=True, ragged=False, seed=2)
+    one, mean, rstd = ops.layer_norm_forward(x, None, None)
+    y, means, rstds = ops.layer_norm_forward(x, None, None, pack_size=3)
+    assert one.shape == (1, 6, 16) and y.shape == (3, 6, 16) and means.shape == rstds.shape == (3, 6)
+    for m in range(3):
+        assert torch.equal(y[m], one[0]) and torch.equal(means[m], mean[0]) and torch.equal(rstds[m], rstd[0])
+    assert torch.equal(ops.layer_norm_forward(x, w, None, pack_size=3)[0], ops.layer_norm_forward(x, w, None)[0])
+    for args in ((x, w, None), (x.expand(3, -1, -1), None, None), (x, None, None)):
+        with pytest.raises(ValueError):
+            ops.layer_norm_forward(*args, pack_size=-1 if args[0].ndim == 2 and args[1] is None else 2)
