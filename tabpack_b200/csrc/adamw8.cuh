@@ -111,8 +111,9 @@ __device__ __forceinline__ f32x2 sqrt2(f32x2 v) {
 
 __global__ void root_check_kernel(uint32_t first, uint32_t count, unsigned long long* differ) {
   unsigned long long n = 0;
-  for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < count; i += gridDim.x * blockDim.x) {
-    const float v = __uint_as_float(first + i);
+  // 64 bits: next to the largest count a 32-bit number would start again from 0
+  for (uint64_t i = blockIdx.x * blockDim.x + threadIdx.x; i < count; i += gridDim.x * blockDim.x) {
+    const float v = __uint_as_float(first + (uint32_t)i);
     const float2 s = halves(sqrt2(pair(v, v)));
     n += __float_as_uint(s.x) != __float_as_uint(__fsqrt_rn(v));
     n += __float_as_uint(s.y) != __float_as_uint(__fsqrt_rn(v));

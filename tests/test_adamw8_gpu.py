@@ -503,3 +503,13 @@ def test_strided_member_hyperparameters(monkeypatch):
     ops.adamw8_step(p, g, *st, step=3, seed=17, **{k: table[:, i] for i, k in enumerate(hp)})
     check(ts, p, st, hp, 3, 17)
     assert len(taken) == 64
+
+
+def test_square_root_check_of_all_numbers_ends():
+    """The largest count: 2^32 - 1 patterns from 2^-94 on, past the end of the finite numbers and round again."""
+    from tabpack_b200 import _lib
+
+    differ = torch.zeros(1, dtype=torch.int64, device='cuda')
+    stream = torch.cuda.current_stream().cuda_stream
+    _lib.check(_lib.load().tp_root_check(33 << 23, 0xFFFFFFFF, differ.data_ptr(), stream), 'tp_root_check')
+    assert differ.item() > 0  # zeros, subnormals and negative numbers are outside its range
