@@ -233,25 +233,22 @@ class _EightBitStates:
 
     def load_state_dict(self, state_dict) -> None:
         """The base class casts the states of fp32 parameters to fp32: the codes go back to uint8
-        (their values are whole numbers below 256) and tensor step counts to int64.  States of the
-        other width are refused."""
+        (their values are whole numbers below 256).  It leaves the step counts where they were saved:
+        tensors of them go to their parameter's device.  States of the other width are refused."""
         packed = [st for st in state_dict['state'].values() if 'exp_avg' in st]
         if any(('exp_avg_scale' in st) != (self.state_bits == 8) for st in packed):
             raise ValueError(f'The loaded moments are not held in {self.state_bits} bits')
-        if self.state_bits != 8:
-            super().load_state_dict(state_dict)
-            return
         state_dict = dict(state_dict)
         seed = state_dict.pop('state_seed', None)
         super().load_state_dict(state_dict)
-        if seed is not None:
+        if seed is not None and self.state_bits == 8:
             self.state_seed = int(seed)
-        for st in self.state.values():
-            if 'exp_avg_scale' not in st:
-                continue
-            for k, dtype in (('exp_avg', torch.uint8), ('exp_avg_sq', torch.uint8), ('step', torch.int64)):
-                if isinstance(st[k], Tensor):
-                    st[k] = st[k].to(dtype)
+        for p, st in self.state.items():
+            if isinstance(st.get('step'), Tensor):
+                st['step'] = st['step'].to(p.device, torch.int64)
+            if 'exp_avg_scale' in st:
+                for k in ('exp_avg', 'exp_avg_sq'):
+                    st[k] = st[k].to(torch.uint8)
 
     def moments(self, p: ParameterPack) -> tuple[Tensor, Tensor]:
         """The first and second moment of a parameter in fp32, whatever width they are held in."""

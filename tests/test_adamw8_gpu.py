@@ -513,3 +513,31 @@ def test_square_root_check_of_all_numbers_ends():
     stream = torch.cuda.current_stream().cuda_stream
     _lib.check(_lib.load().tp_root_check(33 << 23, 0xFFFFFFFF, differ.data_ptr(), stream), 'tp_root_check')
     assert differ.item() > 0  # zeros, subnormals and negative numbers are outside its range
+
+
+@pytest.mark.parametrize('bits', [8, 32])
+def test_checkpoint_through_a_file_read_to_the_host(bits, tmp_path):
+    """Saved, read with map_location='cpu' and loaded: training continues bit for bit."""
+    from tabpack_b200.optim import AdamWPack
+
+    kw = dict(lr=1e-3, weight_decay=0.01, pack_size=3, support_replacement=True, state_bits=bits)
+    a, b = _packs(), _packs()
+    oa, ob = AdamWPack(a, **kw), AdamWPack(b, **kw)
+    for step in range(3):
+        _grads(a, step)
+        oa.step()
+    torch.save({'opt': oa.state_dict(), 'params': [p.data for p in a]}, tmp_path / 'checkpoint.pt')
+    saved = torch.load(tmp_path / 'checkpoint.pt', map_location='cpu', weights_only=True)
+    for p, t in zip(b, saved['params']):
+        p.data.copy_(t)
+    ob.load_state_dict(saved['opt'])
+    for p in b:
+        assert all(t.device == p.device for t in ob.state[p].values())
+    for step in range(3, 6):
+        for params, opt in ((a, oa), (b, ob)):
+            _grads(params, step)
+            opt.step()
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
+        for k, t in oa.state[p].items():
+            assert torch.equal(t, ob.state[q][k])

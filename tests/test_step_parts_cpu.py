@@ -253,3 +253,23 @@ def test_layer_norm_takes_no_weight_decay():
     decay, no_decay = split_weight_decay(model)
     assert [id(p) for p in decay] == [id(model[0].weight), id(model[3].weight)]
     assert len(no_decay) == len(list(model.parameters())) - 2
+
+
+@pytest.mark.parametrize('cls,kw', [(AdamWPack, {}), (AdamWPack, dict(state_bits=8)), (MuonAdamWPack, {}),
+                                    (MuonAdamWPack, dict(adamw_state_bits=8))])
+def test_loaded_step_counts_go_to_their_parameter(cls, kw):
+    """A checkpoint read to the host: torch moves the moments, and leaves what is called 'step'."""
+    p, opt = _opt(cls, support_replacement=True, **kw)
+    state = {'step': torch.tensor([3, 5]), 'exp_avg': torch.ones(2, 200), 'exp_avg_sq': torch.ones(2, 200)}
+    if kw:
+        state = dict(zip(('exp_avg', 'exp_avg_scale', 'exp_avg_sq', 'exp_avg_sq_scale'), ops.adamw8_state(p.data)),
+                     step=state['step'])
+    opt.state[p] = state
+    q = ParameterPack(torch.zeros(2, 200, device='meta'))
+    base = dict(lr=1e-3, weight_decay=0.0) if cls is AdamWPack else dict(
+        adamw_lr=1e-3, muon_lr=1e-2, weight_decay=0.0, allow_inplace_grad_mutation=False)
+    other = cls([q], pack_size=2, support_replacement=True, **base, **kw)
+    other.load_state_dict(opt.state_dict())
+    assert set(other.state[q]) == set(state)
+    for k, t in other.state[q].items():
+        assert t.device.type == 'meta' and t.dtype == state[k].dtype, k
