@@ -249,6 +249,10 @@ class _EightBitStates:
             if 'exp_avg_scale' in st:
                 for k in ('exp_avg', 'exp_avg_sq'):
                     st[k] = st[k].to(torch.uint8)
+                # the codes are copies by now; scales that stay the loaded ones would follow another optimizer's
+                for k in ('exp_avg_scale', 'exp_avg_sq_scale', 'step'):
+                    if isinstance(st[k], Tensor):
+                        st[k] = st[k].clone()
 
     def moments(self, p: ParameterPack) -> tuple[Tensor, Tensor]:
         """The first and second moment of a parameter in fp32, whatever width they are held in."""

@@ -273,3 +273,17 @@ def test_loaded_step_counts_go_to_their_parameter(cls, kw):
     assert set(other.state[q]) == set(state)
     for k, t in other.state[q].items():
         assert t.device.type == 'meta' and t.dtype == state[k].dtype, k
+
+
+def test_loaded_8_bit_states_are_copies_as_a_whole():
+    """Codes without their scales are worth nothing: what another optimizer goes on to do to the loaded tensors
+    changes neither."""
+    p, opt = _opt(state_bits=8, support_replacement=True)
+    names = ('exp_avg', 'exp_avg_scale', 'exp_avg_sq', 'exp_avg_sq_scale')
+    opt.state[p] = {**dict(zip(names, ops.adamw8_state(p.data))), 'step': torch.tensor([3, 5])}
+    q, other = _opt(state_bits=8, support_replacement=True)
+    other.load_state_dict(opt.state_dict())
+    before = {k: t.clone() for k, t in other.state[q].items()}
+    for t in opt.state[p].values():
+        t.add_(1)
+    assert all(torch.equal(t, before[k]) for k, t in other.state[q].items())
