@@ -256,7 +256,7 @@ class _EightBitStates:
 
     def moments(self, p: ParameterPack) -> tuple[Tensor, Tensor]:
         """The first and second moment of a parameter in fp32, whatever width they are held in."""
-        st = self.state[p]
+        st = self.state.get(p, {})  # (indexing would add an entry for p)
         if 'exp_avg' not in st:
             raise ValueError('The parameter has no AdamW moments')
         if 'exp_avg_scale' not in st:

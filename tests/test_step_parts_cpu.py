@@ -287,3 +287,11 @@ def test_loaded_8_bit_states_are_copies_as_a_whole():
     for t in opt.state[p].values():
         t.add_(1)
     assert all(torch.equal(t, before[k]) for k, t in other.state[q].items())
+
+
+def test_moments_of_an_unknown_parameter_leave_the_optimizer_alone():
+    p, opt = _opt(state_bits=8)
+    for stranger in (p, ParameterPack(torch.zeros(2, 3))):
+        with pytest.raises(ValueError):
+            opt.moments(stranger)
+    assert len(opt.state) == 0 and opt.state_dict()['state'] == {}
