@@ -1624,6 +1624,9 @@ int tp_adamw8_step(const tp_adamw8_args* a, void* stream) {
     inner[i] = t.inner;
     ts.t[i] = t;
   }
+  if (!aligned_to(4, {a->lr.per_member, a->beta1.per_member, a->beta2.per_member, a->eps.per_member,
+                      a->weight_decay.per_member}))
+    return fail(TP_EALIGN, "hyperparameters not aligned to their type");
   if (any_scalar_step && a->step <= 0) return fail(TP_EINVAL, "the step count must be positive");
   int rc = adamw8_tiles(ts.n, numel, inner, ts.tile0, ts.member_tiles, &ts.tile_blocks);
   if (rc) return rc;

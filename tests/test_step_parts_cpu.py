@@ -295,3 +295,10 @@ def test_moments_of_an_unknown_parameter_leave_the_optimizer_alone():
         with pytest.raises(ValueError):
             opt.moments(stranger)
     assert len(opt.state) == 0 and opt.state_dict()['state'] == {}
+
+
+@pytest.mark.parametrize('name', ['lr', 'beta1', 'beta2', 'eps', 'weight_decay'])
+def test_misaligned_hyperparameters_are_refused(name):
+    a = adamw_args()
+    getattr(a, name).per_member = FAKE + 2
+    refused('tp_adamw8_step', a, 'aligned')
