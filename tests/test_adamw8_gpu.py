@@ -541,3 +541,45 @@ def test_checkpoint_through_a_file_read_to_the_host(bits, tmp_path):
         assert torch.equal(p, q)
         for k, t in oa.state[p].items():
             assert torch.equal(t, ob.state[q][k])
+
+
+# A launch of 1184 tiles or more gives a warp a run of 16 blocks of a member (64 a tile), a smaller one 8,
+# 4, 2 or 1; a member's last tile and last block are partial in all of these.
+RUNS = [[(1184, 2100)], [(1184, 2101)], [(600, 8200)], [(600, 8197)], [(600, 4100)], [(600, 4103)], [(300, 8188)],
+        [(300, 8191)], [(150, 8064)], [(150, 8063)], [(700, 2052), (500, 1023)], [(1, 1300000)]]
+
+
+@pytest.mark.parametrize('shapes', RUNS, ids=str)
+def test_runs_of_blocks(shapes):
+    """Codes and scales bit for bit where a warp takes many blocks, with vectors and without, and the moments
+    of the same states in both types.
+
+    The parameters' bound at the head of this file counts roundings of the update itself.  Among millions of
+    elements some have b1 m and (1 - b1) g that all but cancel: two products and the constant 1 - b1 are each
+    off by u of these terms, not of their sum (rounded to fp32 with the rest in 64 bits, the first moment alone
+    leaves that bound by 4e-13 at |p| = 7e-7).  So 3 u of what the two terms, added up, would move p by."""
+    from tabpack_b200 import ops
+
+    ts = make(shapes, seed=sum(map(sum, shapes)))
+    ts[0]['g'][:, 130:400:7] = 0.0
+    ts[0]['exp_avg'][0, :256] = ts[0]['exp_avg_sq'][0, :256] = 0
+    p, g, st = on_gpu(ts)
+    for dtype in (torch.float32, torch.bfloat16):
+        m, v = ops.adamw8_moments(*st, dtype=dtype)
+        for i, t in enumerate(ts):
+            first = o8.load_first(t['exp_avg'], t['exp_avg_scale'])
+            root = o8.load_root(t['exp_avg_sq'], t['exp_avg_sq_scale'])
+            for got, want in ((m[i], first), (v[i], root * root)):
+                assert torch.equal(got.cpu(), torch.from_numpy(want.reshape(t['shape'])).to(dtype))
+    step_gpu(p, g, st, SCALAR, 5, 21, tensor_base=2)
+    lr, b1, b2 = SCALAR['lr'], SCALAR['beta1'], SCALAR['beta2']
+    for i, t in enumerate(ts):
+        p64, size, want = expect(t, i + 2, SCALAR, 5, 21)
+        for k, got in zip(KEYS, st):
+            np.testing.assert_array_equal(got[i].cpu().numpy().reshape(want[k].shape), want[k], err_msg=f'{k} {i}')
+        m0, u0 = o8.load_first(t['exp_avg'], t['exp_avg_scale']), o8.load_root(t['exp_avg_sq'], t['exp_avg_sq_scale'])
+        m0, u0, g64 = (x.astype(np.float64) for x in (m0, u0, t['g']))
+        root = np.sqrt((b2 * u0**2 + (1 - b2) * g64**2) / (1 - b2**5)) + SCALAR['eps']
+        terms = lr / (1 - b1**5) * (np.abs(b1 * m0) + np.abs((1 - b1) * g64)) / root
+        bound = U * (3 * np.abs(t['p']) + 64 * size + 3 * terms) + 2.0**-126
+        assert (np.abs(p[i].cpu().numpy().reshape(p64.shape) - p64) <= bound).all()
