@@ -593,3 +593,33 @@ def test_pack_size_of_a_shared_input():
     for args in ((x, w, None), (x.expand(3, -1, -1), None, None), (x, None, None)):
         with pytest.raises(ValueError):
             ops.layer_norm_forward(*args, pack_size=-1 if args[0].ndim == 2 and args[1] is None else 2)
+
+
+# Many members, so that a member's rows are split little: a group of every number of lanes (4 to 512)
+# takes 4 to 20 pairs of rows forward and 8 to 40 rows backward, several times round the rows on their way
+# (3 pairs and 4 rows in bf16, 2 and 2 in fp32); on boundaries of 16 bytes and off them.
+MANY_ROUNDS = [(300, 2300, 48), (300, 2301, 63), (300, 2299, 50), (300, 1100, 128), (300, 1201, 100), (300, 700, 256),
+               (300, 701, 203), (300, 350, 512), (64, 1024, 512), (300, 351, 331), (300, 170, 1024), (300, 171, 771),
+               (300, 90, 2048), (300, 91, 1500), (300, 50, 4096), (300, 51, 2501), (150, 40, 8192), (150, 41, 5001),
+               (296, 40, 4100)]
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('P,B,W', MANY_ROUNDS)
+def test_many_rounds(P, B, W, dtype):
+    x, dy, w, b, n = make(P, B, W, dtype, seed=W + B)
+    x, dy = x.clone(), dy.clone()
+    for m in range(0, P, 7):
+        x[m, :, int(n[m]):] = dy[m, :, int(n[m]):] = float('nan')
+    run_and_check(x, dy, w, b, n)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('P,B,W', [(300, 700, 256), (300, 90, 2048)])
+def test_many_rounds_of_rows_apart(P, B, W, dtype):
+    """Rows of a wider buffer, on every boundary that they can start on."""
+    for ld, at in ((W + 8, 8), (W + 4, 4), (W + 2, 2), (W + 1, 1)):
+        x, dy, w, b, n = make(P, B, ld, dtype, seed=ld)
+        n = (n * W // ld).clamp(min=1).to(torch.int32)
+        cut = lambda t: t[..., at:at + W]  # noqa: E731
+        run_and_check(cut(x), cut(dy), cut(w).contiguous(), cut(b).contiguous(), n)
