@@ -441,3 +441,41 @@ def test_refusals():
         ops.label_log_probs_backward(g_l[:1], None, z, y, stats)
     with pytest.raises(TypeError):
         ops.label_log_probs_backward(g_l, None, z, y, torch.zeros(2, 7, device='cuda'))
+
+
+def lengths(piece, counts, vector):
+    """Rows just below, at and above whole numbers of a block's or cluster's pieces."""
+    return [c * piece + d for c in counts for d in (-vector - 1, -1, 0, 1, vector)]
+
+
+SIZE = {torch.bfloat16: (8, 3), torch.float32: (4, 4)}  # scores of a vector, vectors of a thread in one piece
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('R,parts', [(3, 8), (30, 4), (60, 2), (100, 1)])
+def test_long_rows_without_best_classes(R, parts, dtype):
+    """The forward that loads whole pieces without a check per vector, over clusters of 8, 4 and 2 CTAs and on
+    one; rows on 16-byte boundaries and off them."""
+    V, U4 = SIZE[dtype]
+    piece = 256 * parts * V * U4
+    for i, C in enumerate(lengths(piece, [c for c in (2, 3, 5, 7, 9) if 32768 < c * piece - 9][:2], V)):
+        run_and_check(*make((R,), C, dtype, seed=C, ld=C + i % 3, masked=0.2 * (i % 2)))
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('R,threads,classes', [(5, 64, 4200), (5, 128, 9000), (5, 256, 17000), (1184, 64, 6000),
+                                               (1184, 128, 20000), (1184, 256, 33000)])
+def test_block_sizes_without_best_classes(R, threads, classes, dtype):
+    """Blocks of 2, 4 and 8 warps, by the length and the number of the rows."""
+    V, U4 = SIZE[dtype]
+    piece = threads * V * U4
+    for i, C in enumerate(lengths(piece, [classes // piece + 1], V)):
+        run_and_check(*make((R,), C, dtype, seed=C, ld=C + i % 3))
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('P,B,C', [(4, 6, 5000), (2, 9, 40000), (3, 20, 33001), (40, 30, 1500), (2, 1, 70000)])
+def test_shared_labels_of_long_rows_with_best_classes(P, B, C, dtype):
+    z, y, g_l, g_h = make((P, B), C, dtype, seed=C)
+    run_and_check(z, y[0], g_l, g_h, k=9)
+    run_and_check(z, y[0], g_l, g_h)
