@@ -583,3 +583,37 @@ def test_runs_of_blocks(shapes):
         terms = lr / (1 - b1**5) * (np.abs(b1 * m0) + np.abs((1 - b1) * g64)) / root
         bound = U * (3 * np.abs(t['p']) + 64 * size + 3 * terms) + 2.0**-126
         assert (np.abs(p[i].cpu().numpy().reshape(p64.shape) - p64) <= bound).all()
+
+
+@pytest.mark.parametrize('inner', [1_100_000_004, 1_100_000_003])
+def test_elements_beyond_32_bits(inner):
+    """The last blocks of two members of 1.1 billion elements, in a fresh state (22 GB)."""
+    from oracle.philox import philox4x32_10
+    from tabpack_b200 import ops
+
+    p, g = (torch.zeros(2, inner, device='cuda') for _ in range(2))
+    st = [[t] for t in ops.adamw8_state(p)]
+    lo = (inner - 300) // 128 * 128
+    gen = torch.Generator(device='cuda').manual_seed(inner % 7)
+    g[:, lo:] = torch.randn(2, inner - lo, generator=gen, device='cuda') * 1e-2
+    hp = {**SCALAR, 'weight_decay': 0.0}
+    ops.adamw8_step([p], [g], *st, step=1, seed=41, member_base=5, tensor_base=3, **hp)
+    n, tail = inner - lo, g[:, lo:].cpu().numpy()
+    f32, zero = np.float32, np.zeros((2, inner - lo), np.float32)
+    m, u = o8.moments32(zero, zero, tail, f32(0.9), f32(0.999), f32(1 - 0.9), f32(1 - 0.999))
+    group = np.arange(lo // 4, (inner + 3) // 4, dtype=np.uint32)[None]
+    member = np.array([[5], [6]], np.uint32)
+    words = philox4x32_10(*np.broadcast_arrays(group, np.uint32(3), member, np.uint32(1)), np.uint32(41), np.uint32(0))
+    words = np.stack(words, -1).reshape(2, -1)[:, :n]
+    want = (*o8.store_first(m, words & 0xFFFF), *o8.store_root(u, words >> 16))
+    for (t,), w in zip(st, want):
+        np.testing.assert_array_equal(t[:, t.shape[1] - w.shape[1]:].cpu().numpy(), w)
+    p64, size = o8.step64(zero, tail, zero, zero, lr=hp['lr'], b1=0.9, b2=0.999, eps=1e-8, wd=0.0, t=1.0)
+    assert (np.abs(p[:, lo:].cpu().numpy() - p64) <= U * 64 * size).all()
+    assert not p[:, 128:lo].any() and not st[0][0][:, :lo].any()
+    first, root = ops.adamw8_moments(*st, dtype=torch.bfloat16)
+    for got, (codes, scales), load, power in ((first[0], want[:2], o8.load_first, 1), (root[0], want[2:], o8.load_root, 2)):
+        value = torch.from_numpy(load(codes, scales) ** power).bfloat16()
+        assert torch.equal(got[:, lo:].cpu(), value)
+    del p, g, st, first, root, got
+    torch.cuda.empty_cache()

@@ -479,3 +479,29 @@ def test_shared_labels_of_long_rows_with_best_classes(P, B, C, dtype):
     z, y, g_l, g_h = make((P, B), C, dtype, seed=C)
     run_and_check(z, y[0], g_l, g_h, k=9)
     run_and_check(z, y[0], g_l, g_h)
+
+
+@pytest.mark.parametrize('R,C,dtype', [(36000, 60001, torch.bfloat16), (4400000, 500, torch.bfloat16),
+                                       (9000000, 243, torch.float32), (220000000, 10, torch.bfloat16)])
+def test_scores_beyond_32_bits(R, C, dtype):
+    """The first and last rows of more than 2^31 scores: long rows, held ones with and without statistics."""
+    from tabpack_b200 import ops
+
+    few = 4
+    zs, ys, g_l, g_h = make((2 * few,), C, dtype, seed=C)
+    z, y = torch.zeros(R, C, dtype=dtype, device='cuda'), torch.zeros(R, dtype=torch.int64, device='cuda')
+    gl, gh = torch.zeros(R, device='cuda'), torch.zeros(R, device='cuda')
+    at = torch.cat([torch.arange(few, device='cuda'), torch.arange(R - few, R, device='cuda')])
+    z[at], y[at], gl[at], gh[at] = zs, ys, g_l, g_h
+    k = 3
+    lp, H, top, which, stats = ops.label_log_probs_forward(z, y, top_k=k)
+    dz = ops.label_log_probs_backward(gl, gh, z, y, stats)
+    want, tol = plain(zs, ys, k, g_l.double(), g_h.double())
+    near(lp[at], want[0], tol[0], 'log_prob')
+    near(H[at], want[1], tol[1], 'entropy')
+    near(top[at], want[2], tol[2], 'top_log_prob')
+    assert torch.equal(which[at], want[3])
+    near(dz[at], want[4], tol[3], 'dlogits', dtype)
+    assert not dz[few: R - few].any() and (which[R // 2] == torch.arange(k, device='cuda')).all()
+    del z, dz, lp, H, top, which, stats
+    torch.cuda.empty_cache()

@@ -623,3 +623,28 @@ def test_many_rounds_of_rows_apart(P, B, W, dtype):
         n = (n * W // ld).clamp(min=1).to(torch.int32)
         cut = lambda t: t[..., at:at + W]  # noqa: E731
         run_and_check(cut(x), cut(dy), cut(w).contiguous(), cut(b).contiguous(), n)
+
+
+@pytest.mark.parametrize('P,B,W,dtype', [(2, 140000, 8000, torch.bfloat16), (3, 1000000, 771, torch.float32),
+                                         (3, 80000, 9001, torch.bfloat16)])
+def test_elements_beyond_32_bits(P, B, W, dtype):
+    """The last rows of more than 2^31 elements, forward and backward, and the parameters' gradients where only
+    those rows have one."""
+    from tabpack_b200 import ops
+
+    few = 5
+    xs, dys, w, b, n = make(P, few, W, dtype, seed=W)
+    x, dy = (torch.zeros(P, B, W, dtype=dtype, device='cuda') for _ in range(2))
+    x[:, B - few:], dy[:, B - few:] = xs, dys
+    y, mean, rstd = ops.layer_norm_forward(x, w, b, n_features=n)
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, mean, rstd, n_features=n)
+    for m in range(P):
+        k = int(n[m])
+        want, tol = plain(xs[m], w[m], b[m], k, 1e-5, dys[m])
+        check(y[m, B - few:], want[0], tol[0], dtype, 'y')
+        check(dx[m, B - few:], want[1], tol[1], dtype, 'dx')
+        check(dw[m], want[2], tol[2], torch.float32, 'dw')
+        check(db[m], want[3], tol[3], torch.float32, 'db')
+        assert torch.equal(y[m, B // 2, :k], b[m, :k].to(dtype)) and not dx[m, : B - few].any()
+    del x, dy, y, dx, mean, rstd
+    torch.cuda.empty_cache()
