@@ -295,17 +295,21 @@ def _reusable(buf: Tensor | None, shape, dtype: torch.dtype, device) -> bool:
 
 class _Same:
     """Equal for one living tensor object only.  An address and a version do not tell a tensor: one that
-    a member selection installs may lie where the last selection's lay, at the same version."""
+    a member selection installs may lie where the last selection's lay, at the same version.  Copies (of
+    a module that is copied or saved as a whole) equal nothing."""
 
     __slots__ = ('ref',)
     __hash__ = None
 
-    def __init__(self, t: Tensor) -> None:
-        self.ref = weakref.ref(t)
+    def __init__(self, t: Tensor | None = None) -> None:
+        self.ref = None if t is None else weakref.ref(t)
 
     def __eq__(self, other) -> bool:
-        t = self.ref()
-        return t is not None and isinstance(other, _Same) and other.ref() is t
+        t = None if self.ref is None else self.ref()
+        return t is not None and isinstance(other, _Same) and other.ref is not None and other.ref() is t
+
+    def __reduce__(self):
+        return _Same, ()
 
 
 def _state(t: Tensor | None):

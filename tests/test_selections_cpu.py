@@ -1,6 +1,8 @@
 """What a module keeps from call to call (int32 widths, bf16 weights) belongs to one tensor: a member
 selection installs tensors of its own, which may lie where the last selection's lay (no GPU)."""
 
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -122,3 +124,17 @@ def test_copies_recorded_into_a_graph_are_not_kept(monkeypatch):
     monkeypatch.setattr(nn, '_capturing', lambda t: True)
     assert _widths_cached(module, 'n', buf) is kept[0] and cache.get(w, torch.bfloat16, 8) is kept[1]
     assert backbone._n_blocks_i32(None) is kept[2]
+
+
+def test_modules_in_use_are_copied_and_saved(tmp_path):
+    """A whole module after a call: its copies are made anew where it arrives."""
+    linear = LinearPack(8, [4, 8], pack_size=2)
+    use = lambda m: m._cache.get(m.weight, torch.bfloat16, 8, widths=(  # noqa: E731
+        _widths_cached(m, 'out', m.out_features), None, None, 0))
+    first = use(linear)
+    torch.save(linear, tmp_path / 'linear.pt')
+    for other in (copy.deepcopy(linear), torch.load(tmp_path / 'linear.pt', weights_only=False)):
+        with torch.no_grad():
+            other.weight.fill_(2)
+        assert (use(other) == 2).all() and use(other) is use(other)
+    assert use(linear) is first
