@@ -21,7 +21,7 @@
 // the point where the SM's issue slots and the memory take equally long.  So the fp32 arithmetic is
 // done in pairs (f32x2), the codes of a block are formed without the rules for subnormals, zeros and
 // empty blocks where a vote says that none is there, and the next blocks are on their way to shared
-// memory meanwhile.  209 M elements: 607 us, 5.6 TB/s, 87 % of a copy's rate.
+// memory meanwhile.  209 M elements: 610 to 617 us, 5.5 TB/s, 86 % of a copy's rate.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -453,8 +453,9 @@ __device__ __forceinline__ void adamw8_tile(const AdamW8Member& c, AdamW8Ptr a, 
 
 // One warp takes one block of 128 elements at a time, four a lane; the block's maxima are warp
 // reductions.  The grid is one CTA per tile of a member's blocks, over all members and tensors.
-// Six CTAs of four warps an SM: 72 registers a thread without spills (64 with: 655 us instead of 632
-// for 209 M elements in CTAs of eight warps; 617 in CTAs of four).
+// Six CTAs of four warps an SM, 78 registers a thread and no spills: 610 to 617 us for 209 M elements.  Seven
+// CTAs (72 registers, no spills) take 627 to 632, eight (64, with spills) 624 to 635, three of eight warps 644
+// to 651.
 __global__ void __launch_bounds__(32 * ADAMW8_WARPS, 6) adamw8_kernel(const __grid_constant__ AdamW8Tensors ts,
                                                                       const __grid_constant__ AdamW8Scalars s) {
   __shared__ AdamW8Member shared;

@@ -1582,8 +1582,8 @@ int tp_adamw_step(const tp_adamw_args* a, void* stream) {
 
 // Tiles of a launch over several packs: tensor i's members have member_tiles[i] tiles of tile_blocks
 // state blocks each.  64 blocks a tile (16 a warp, which carry the tile's fixed cost: 209 M elements
-// take 617 us, with 32 blocks 644), halved down to one block a warp until there are 1184 tiles, 8 per SM
-// (2.9 M elements in odd members: 16.3 us, with 64 blocks in 370 tiles 18.8).
+// take 610 to 617 us, with 32 blocks 638 to 643), halved down to one block a warp until there are 1184 tiles, 8
+// per SM (2.9 M elements in odd members: 16.6 us, with 64 blocks in 370 tiles 22.1).
 static int adamw8_tiles(int n, const int64_t* numel, const int64_t* inner, uint32_t* tile0, uint32_t* member_tiles,
                         int* tile_blocks) {
   for (int tb = 64;; tb /= 2) {
@@ -1743,7 +1743,10 @@ namespace {
 
 // Lanes of a row's group: 16 elements each, as few as hold the row (131072 rows of 256 in bf16 with 16 lanes
 // 26 + 44 us, with 32 lanes 37 + 60; rows off 16-byte boundaries gain more, since they take an instruction per
-// element: 665144 rows of 50 in fp32 with 4 lanes 73 + 110 us, with 32 lanes 317 + 453).
+// element: 665144 rows of 50 in fp32 with 4 lanes 73 + 110 us, with 32 lanes 317 + 453).  So do the wider groups:
+// 65536 rows of 1024 in bf16 take 46 + 76 us with 64 lanes and 78 + 127 with 128, 32768 of 2048 46 + 75 with 128
+// and 79 + 131 with 256, 16384 of 4096 44 + 88 with 256 and 87 + 151 with 512; element by element 65536 of 771 in
+// fp32 86 + 147 with 64 and 150 + 245 with 128.
 int norm_lanes(int W) {
   for (int g : {4, 8, 16, 32, 64, 128, 256})
     if (W <= g * NORM_E) return g;
