@@ -314,7 +314,7 @@ def _encode(x, format):
     q = torch.where(scale[..., None] > 0, x.abs() / scale[..., None], 0.0)
     # the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6; in the middle the even code
     code = ((q > 0.25).to(torch.uint8) + (q >= 0.75) + (q > 1.25) + (q >= 1.75) + (q > 2.5) + (q >= 3.5) + (q > 5))
-    return code + 8 * (x < 0), byte, row
+    return code + 8 * (x < 0).to(torch.uint8), byte, row
 
 
 def _decode(code, byte, row, format, K):
