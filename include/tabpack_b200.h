@@ -645,6 +645,156 @@ const char* tp_last_error_string(void);
 /* Library version string. */
 const char* tp_version(void);
 
+/* Routing of rows to members.  Per row of scores z over E members (E <= 1024): p = softmax(z) in fp32, the
+ * top_k (<= 32, <= E) best finite z in descending order (ties: lowest member; NaN first) as `expert` (-1 where a row
+ * has fewer), their `weight` p / (sum of the chosen p) with renormalize, else p (0 for -1).  The (row, slot) pairs are
+ * sorted by member, stably: `position` is a pair's place, `offsets` (E + 1) where the members' rows begin; pairs
+ * without a member come behind offsets[E].  importance[e] = sum over rows of p_e.  Scores of -inf take no part; a row
+ * of nothing else has no members; a NaN or +inf makes its row's weights (and the importance) NaN.
+ * The backward forms dlogits (rows, E), contiguous, from the gradients of weight and importance (either may be NULL):
+ *   dz_e = [e chosen] w_e (g_e - s) + p_e (h_e - sum_c p_c h_c)          s = sum_chosen w g, with renormalize,
+ *   dz_e = [e chosen] w_e g_e + p_e (h_e - sum_c p_c h_c - s)            without. */
+#define TP_ROUTE_MAX_EXPERTS 1024
+#define TP_ROUTE_MAX_K 32
+typedef struct tp_route_args {
+  int64_t rows;             /* rows * top_k < 2^31 */
+  int32_t E, top_k;
+  int32_t dtype;            /* TP_DTYPE_F32 or TP_DTYPE_BF16: logits, dlogits */
+  int32_t renormalize;
+  const void* logits;
+  int64_t logits_stride;    /* elements between rows */
+  float* weight;            /* (rows, top_k): written by the forward, read by the backward */
+  int32_t* expert;          /* (rows, top_k) */
+  int32_t* position;        /* (rows, top_k), forward */
+  int32_t* offsets;         /* (E + 1), forward */
+  float* importance;        /* (E), forward */
+  void* workspace;          /* forward: tp_route_workspace_size */
+  size_t workspace_bytes;
+  const float* g_weight;    /* backward: (rows, top_k), or NULL */
+  const float* g_importance; /* (E), or NULL */
+  void* dlogits;
+} tp_route_args;
+size_t tp_route_workspace_size(int64_t rows, int32_t E, int32_t top_k);
+int tp_route_forward(const tp_route_args* a, void* stream);
+int tp_route_backward(const tp_route_args* a, void* stream);
+
+/* Moves of rows by such a plan (position (rows, k) a permutation of 0 .. rows k - 1, offsets (E + 1)):
+ *   tp_dispatch_rows: out[position[t, j]] = x[t], (rows k, W); zero rows for places at or behind offsets[E]
+ *   tp_combine_rows:  out[t] = sum_j weight[t, j] x[position[t, j]], (rows, W), sums in fp32; weight NULL: ones; places
+ *                     at or behind offsets[E] take no part (their rows of x are not read)
+ *   tp_combine_rows_backward: dy[position[t, j]] = weight[t, j] dout[t] (zero rows as in dispatch), dweight[t, j] =
+ *                     <dout[t], x[position[t, j]]>; either may be NULL.
+ * Places outside 0 .. rows k - 1 are passed over. */
+typedef struct tp_rows_args {
+  int64_t rows;             /* rows * k < 2^31 */
+  int32_t k, W, E;
+  int32_t dtype;            /* TP_DTYPE_F32 or TP_DTYPE_BF16: x, out, dout, dy */
+  const int32_t* position;
+  const int32_t* offsets;
+  const float* weight;
+  const void* x;
+  int64_t x_stride;         /* elements between rows of x */
+  void* out;                /* contiguous */
+  const void* dout;
+  int64_t dout_stride;
+  void* dy;                 /* contiguous */
+  float* dweight;
+} tp_rows_args;
+int tp_dispatch_rows(const tp_rows_args* a, void* stream);
+int tp_combine_rows(const tp_rows_args* a, void* stream);
+int tp_combine_rows_backward(const tp_rows_args* a, void* stream);
+
+/* Linear layer of a pack over ragged groups of rows: member m's rows are offsets[m] .. offsets[m + 1] - 1 of x,
+ *   y = relu(x w_m^T + b_m),  g = dy [y > 0],  dx = g w_m,  dw_m = g^T x,  db_m = sum g.
+ * offsets (device, P + 1) do not decrease and stay within 0 .. rows (what does not is cut).  Rows of no member are zero
+ * in y and dx and take no part in dw and db.  A member takes its first in_features columns and out_features outputs;
+ * what lies beyond takes no part, whatever it holds, and is zero in every result.  BF16: x_stride, w_stride and
+ * dy_stride (without relu) are multiples of 8 and their pointers on 16-byte boundaries. */
+typedef struct tp_ragged_linear_args {
+  int32_t P;
+  int32_t max_in, max_out;
+  int32_t dtype;            /* TP_DTYPE_F32 or TP_DTYPE_BF16: x, w, y, dy, dx */
+  int64_t rows;             /* < 2^31 */
+  const int32_t* offsets;
+  const int32_t* in_features;  /* (P), or NULL (= max_in) */
+  const int32_t* out_features; /* (P), or NULL (= max_out) */
+  int32_t relu;
+  const void* x;            /* (rows, max_in) */
+  int64_t x_stride;
+  const void* w;            /* (P, max_out, max_in), rows at w_stride */
+  int64_t w_stride;
+  const float* bias;        /* (P, max_out), or NULL; forward */
+  void* y;                  /* (rows, max_out) contiguous: written by the forward, read by the backward with relu */
+  const void* dy;           /* backward: (rows, max_out) */
+  int64_t dy_stride;
+  void* dx;                 /* (rows, max_in) contiguous, or NULL */
+  float* dw;                /* (P, max_out, max_in) contiguous, or NULL */
+  float* dbias;             /* (P, max_out), or NULL */
+  void* workspace;          /* backward: tp_ragged_linear_workspace_size */
+  size_t workspace_bytes;
+} tp_ragged_linear_args;
+size_t tp_ragged_linear_workspace_size(const tp_ragged_linear_args* a);
+int tp_ragged_linear_forward(const tp_ragged_linear_args* a, void* stream);
+int tp_ragged_linear_backward(const tp_ragged_linear_args* a, void* stream);
+
+/* Rows in 4-bit floating point: e2m1 codes times a scale per block of columns.  TP_FP4_NV: blocks of 16, scale s 2^r,
+ * 2^r the row's power of two with max|row| <= 2688 2^r < 2 max|row|, s = e4m3(max|block| / (6 2^r)).  TP_FP4_MX: blocks
+ * of 32, scale 2^(floor(log2 max|block|) - 2).  Both powers are at least 2^-100; codes are rounded to nearest, ties to
+ * even, and at most 6 in magnitude.  A row with a NaN or an infinity is NaN as a whole.
+ * codes: two a byte, the even column's in the low half, rows of tp_fp4_pitch(K) = 16 ceil(K / 32) bytes, zeros behind
+ * column K.  scales: tiles of 128 rows by 4 blocks, byte 16 (row % 32) + 4 (row / 32) + block % 4 of a tile's 512;
+ * tp_fp4_scale_tiles(K, format) tiles a row of tiles (K rounded up to 256 columns), zero bytes where there is no block.
+ * P groups of rows begin in a tile of their own: equal groups of `rows / P` rows (offsets NULL) group g in row of tiles
+ * g ceil(rows / P / 128); ragged ones (offsets as in tp_ragged_linear_args) in floor(offsets[g] / 128) + g, which takes
+ * rows / 128 + P rows of tiles in all.  row_scale: 2^r, or 1 (TP_FP4_MX), or NaN. */
+#define TP_FP4_NV 0
+#define TP_FP4_MX 1
+typedef struct tp_fp4_args {
+  int32_t P;
+  int32_t K;
+  int32_t format;           /* TP_FP4_* */
+  int32_t dtype;            /* TP_DTYPE_F32 or TP_DTYPE_BF16: x */
+  int64_t rows;             /* < 2^31 */
+  const int32_t* offsets;   /* (P + 1), or NULL */
+  const int32_t* n_features; /* (P): columns of a group's rows that count, or NULL (= K) */
+  const void* x;            /* (rows, K), quantise */
+  int64_t x_stride;
+  uint8_t* codes;
+  uint8_t* scales;
+  float* row_scale;
+  void* values;             /* (rows, K) bf16, tp_fp4_values (it holds them exactly) */
+} tp_fp4_args;
+int32_t tp_fp4_pitch(int32_t K);
+int32_t tp_fp4_scale_tiles(int32_t K, int32_t format);
+int tp_fp4_quantize(const tp_fp4_args* a, void* stream);
+int tp_fp4_values(const tp_fp4_args* a, void* stream);
+
+/* y = relu(q(x) q(w_m)^T + b_m) over rows of x in 4 bits (x.codes, x.scales, x.row_scale as written by tp_fp4_quantize
+ * for the same groups) and weights in 4 bits (P groups of N rows, without offsets), sums in fp32.  Groups as in
+ * tp_fp4_args; x_shared: every member reads the same `rows` rows (P results of them; offsets NULL).  Rows of no member
+ * are zero. */
+typedef struct tp_fp4_linear_args {
+  int32_t P;
+  int32_t K, N;
+  int32_t format;
+  int32_t dtype;            /* TP_DTYPE_F32 or TP_DTYPE_BF16: y */
+  int32_t x_shared;
+  int64_t rows;             /* rows of x */
+  const int32_t* offsets;
+  const int32_t* in_features;  /* (P): columns that count (the codes beyond are zero), or NULL */
+  const int32_t* out_features; /* (P), or NULL (= N) */
+  const uint8_t* x_codes;
+  const uint8_t* x_scales;
+  const float* x_row_scale;
+  const uint8_t* w_codes;
+  const uint8_t* w_scales;
+  const float* w_row_scale;
+  const float* bias;        /* (P, N), or NULL */
+  int32_t relu;
+  void* y;                  /* (rows, N); (P, rows, N) with x_shared */
+} tp_fp4_linear_args;
+int tp_fp4_linear_forward(const tp_fp4_linear_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,9 @@ TP_MAX_OPT_TENSORS = 32
 TP_NOALLOC_SCRATCH_BYTES = 16 << 20
 TP_MAX_TOP_K = 32
 TP_LABEL_STATS_CLASSES = 256
+TP_ROUTE_MAX_EXPERTS = 1024
+TP_ROUTE_MAX_K = 32
+TP_FP4 = {'nvfp4': 0, 'mxfp4': 1}
 
 _c_int32_p = ctypes.POINTER(ctypes.c_int32)
 _c_float_p = ctypes.POINTER(ctypes.c_float)
@@ -197,6 +200,59 @@ class LabelLogProbsArgs(ctypes.Structure):
     ]
 
 
+class RouteArgs(ctypes.Structure):
+    _fields_ = [
+        ('rows', ctypes.c_int64), ('E', ctypes.c_int32), ('top_k', ctypes.c_int32), ('dtype', ctypes.c_int32),
+        ('renormalize', ctypes.c_int32), ('logits', ctypes.c_void_p), ('logits_stride', ctypes.c_int64),
+        ('weight', ctypes.c_void_p), ('expert', ctypes.c_void_p), ('position', ctypes.c_void_p),
+        ('offsets', ctypes.c_void_p), ('importance', ctypes.c_void_p), ('workspace', ctypes.c_void_p),
+        ('workspace_bytes', ctypes.c_size_t), ('g_weight', ctypes.c_void_p), ('g_importance', ctypes.c_void_p),
+        ('dlogits', ctypes.c_void_p),
+    ]
+
+
+class RowsArgs(ctypes.Structure):
+    _fields_ = [
+        ('rows', ctypes.c_int64), ('k', ctypes.c_int32), ('W', ctypes.c_int32), ('E', ctypes.c_int32),
+        ('dtype', ctypes.c_int32), ('position', ctypes.c_void_p), ('offsets', ctypes.c_void_p),
+        ('weight', ctypes.c_void_p), ('x', ctypes.c_void_p), ('x_stride', ctypes.c_int64), ('out', ctypes.c_void_p),
+        ('dout', ctypes.c_void_p), ('dout_stride', ctypes.c_int64), ('dy', ctypes.c_void_p),
+        ('dweight', ctypes.c_void_p),
+    ]
+
+
+class RaggedLinearArgs(ctypes.Structure):
+    _fields_ = [
+        ('P', ctypes.c_int32), ('max_in', ctypes.c_int32), ('max_out', ctypes.c_int32), ('dtype', ctypes.c_int32),
+        ('rows', ctypes.c_int64), ('offsets', ctypes.c_void_p), ('in_features', ctypes.c_void_p),
+        ('out_features', ctypes.c_void_p), ('relu', ctypes.c_int32), ('x', ctypes.c_void_p),
+        ('x_stride', ctypes.c_int64), ('w', ctypes.c_void_p), ('w_stride', ctypes.c_int64), ('bias', ctypes.c_void_p),
+        ('y', ctypes.c_void_p), ('dy', ctypes.c_void_p), ('dy_stride', ctypes.c_int64), ('dx', ctypes.c_void_p),
+        ('dw', ctypes.c_void_p), ('dbias', ctypes.c_void_p), ('workspace', ctypes.c_void_p),
+        ('workspace_bytes', ctypes.c_size_t),
+    ]
+
+
+class Fp4Args(ctypes.Structure):
+    _fields_ = [
+        ('P', ctypes.c_int32), ('K', ctypes.c_int32), ('format', ctypes.c_int32), ('dtype', ctypes.c_int32),
+        ('rows', ctypes.c_int64), ('offsets', ctypes.c_void_p), ('n_features', ctypes.c_void_p),
+        ('x', ctypes.c_void_p), ('x_stride', ctypes.c_int64), ('codes', ctypes.c_void_p), ('scales', ctypes.c_void_p),
+        ('row_scale', ctypes.c_void_p), ('values', ctypes.c_void_p),
+    ]
+
+
+class Fp4LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ('P', ctypes.c_int32), ('K', ctypes.c_int32), ('N', ctypes.c_int32), ('format', ctypes.c_int32),
+        ('dtype', ctypes.c_int32), ('x_shared', ctypes.c_int32), ('rows', ctypes.c_int64),
+        ('offsets', ctypes.c_void_p), ('in_features', ctypes.c_void_p), ('out_features', ctypes.c_void_p),
+        ('x_codes', ctypes.c_void_p), ('x_scales', ctypes.c_void_p), ('x_row_scale', ctypes.c_void_p),
+        ('w_codes', ctypes.c_void_p), ('w_scales', ctypes.c_void_p), ('w_row_scale', ctypes.c_void_p),
+        ('bias', ctypes.c_void_p), ('relu', ctypes.c_int32), ('y', ctypes.c_void_p),
+    ]
+
+
 # kernel families of tp_profile_stop, in TP_PROF_* order
 TP_PROF_KINDS = ('fwd', 'dgrad', 'wgrad', 'newton_schulz_gram', 'newton_schulz_update', 'gemm_f32', 'act_backward',
                  'muon_elementwise', 'adamw', 'weight_cast', 'input', 'embedding', 'onehot', 'metric', 'greedy',
@@ -253,6 +309,20 @@ SIGNATURES = {
     'tp_layer_norm_backward': (ctypes.c_int, [ctypes.POINTER(LayerNormArgs), ctypes.c_void_p]),
     'tp_label_log_probs_forward': (ctypes.c_int, [ctypes.POINTER(LabelLogProbsArgs), ctypes.c_void_p]),
     'tp_label_log_probs_backward': (ctypes.c_int, [ctypes.POINTER(LabelLogProbsArgs), ctypes.c_void_p]),
+    'tp_route_workspace_size': (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]),
+    'tp_route_forward': (ctypes.c_int, [ctypes.POINTER(RouteArgs), ctypes.c_void_p]),
+    'tp_route_backward': (ctypes.c_int, [ctypes.POINTER(RouteArgs), ctypes.c_void_p]),
+    'tp_dispatch_rows': (ctypes.c_int, [ctypes.POINTER(RowsArgs), ctypes.c_void_p]),
+    'tp_combine_rows': (ctypes.c_int, [ctypes.POINTER(RowsArgs), ctypes.c_void_p]),
+    'tp_combine_rows_backward': (ctypes.c_int, [ctypes.POINTER(RowsArgs), ctypes.c_void_p]),
+    'tp_ragged_linear_workspace_size': (ctypes.c_size_t, [ctypes.POINTER(RaggedLinearArgs)]),
+    'tp_ragged_linear_forward': (ctypes.c_int, [ctypes.POINTER(RaggedLinearArgs), ctypes.c_void_p]),
+    'tp_ragged_linear_backward': (ctypes.c_int, [ctypes.POINTER(RaggedLinearArgs), ctypes.c_void_p]),
+    'tp_fp4_pitch': (ctypes.c_int32, [ctypes.c_int32]),
+    'tp_fp4_scale_tiles': (ctypes.c_int32, [ctypes.c_int32, ctypes.c_int32]),
+    'tp_fp4_quantize': (ctypes.c_int, [ctypes.POINTER(Fp4Args), ctypes.c_void_p]),
+    'tp_fp4_values': (ctypes.c_int, [ctypes.POINTER(Fp4Args), ctypes.c_void_p]),
+    'tp_fp4_linear_forward': (ctypes.c_int, [ctypes.POINTER(Fp4LinearArgs), ctypes.c_void_p]),
     'tp_device_error': (ctypes.c_int, []),
     'tp_last_error_string': (ctypes.c_char_p, []),
     'tp_version': (ctypes.c_char_p, []),

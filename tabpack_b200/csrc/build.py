@@ -2,7 +2,7 @@
 
     python -m tabpack_b200.csrc.build [--verbose]
 
-The library is a single translation unit (`tabpack_b200.cu`) linked against the
+The library's two translation units (`tabpack_b200.cu`, `routed.cu`) are linked against the
 static CUDA runtime, so it only needs the NVIDIA driver at run time.
 """
 
@@ -17,8 +17,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, 'libtabpack_b200.so')
-SOURCES = ['tabpack_b200.cu']
-# every header beside the translation unit, so that an edit to any of them triggers a rebuild
+SOURCES = ['tabpack_b200.cu', 'routed.cu']
+# every header beside the translation units, so that an edit to any of them triggers a rebuild
 HEADERS = sorted(f for f in os.listdir(HERE) if f.endswith('.cuh'))
 
 
@@ -51,6 +51,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         '-Xcompiler', '-fPIC', '-shared', '-cudart', 'static',
         '--expt-relaxed-constexpr',
         '-I', os.path.join(ROOT, 'include'), '-I', HERE,
+        '--threads', str(len(SOURCES)),
         '-o', LIB + '.tmp',
     ] + [os.path.join(HERE, s) for s in SOURCES]
     if verbose:

@@ -1,0 +1,687 @@
+// Rows in 4-bit floating point with a scale per block of columns, and products of such rows.
+//
+// A value is an e2m1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) times its block's scale:
+//   nvfp4: blocks of 16 columns, scale s 2^r.  2^r is the row's: the power of two with max|row| <= 2688 2^r <
+//          2 max|row| (at least 2^-100), 2688 = 6 * 448; s = e4m3(max|block| / (6 2^r)), at most 448.
+//   mxfp4: blocks of 32 columns, scale 2^(floor(log2 max|block|) - 2), at least 2^-100; larger values than 6 scales
+//          become 6 scales.
+// Codes are rounded to nearest, ties to the even code.  Every scale of the nvfp4 form has four significant bits, so
+// x / scale is a tie only where it is one exactly, and a correctly rounded quotient decides as the exact one would.
+// A row with a NaN or an infinity is NaN as a whole (its row scale).
+//
+// Layout.  Codes: two a byte, the even column's in the low half, rows of 16 ceil(K / 32) bytes, zeros at the end.
+// Scales: as the tensor core takes them, tiles of 128 rows by 4 blocks, byte 16 (row % 32) + 4 (row / 32) + block % 4
+// of the tile's 512; a row of tiles covers K rounded up to 256 columns.  Groups of rows begin in a tile of their own:
+// group g of equal groups of B rows in tile g ceil(B / 128), ragged group g in tile floor(first row / 128) + g (which
+// leaves every group the tiles that it needs, since floor(b / 128) - floor(a / 128) + 1 >= ceil((b - a) / 128)).
+#pragma once
+
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace tp {
+
+enum : int { FP4_NV = 0, FP4_MX = 1 };
+
+struct Fp4Rows {
+  uint8_t* codes;    // (rows, pitch)
+  uint8_t* scales;   // (tiles, atoms, 512)
+  float* row_scale;  // (rows): 2^r (nvfp4) or 1 (mxfp4); NaN for a row that is not finite
+  int pitch, atoms;
+};
+
+// Groups of rows: P equal ones of B rows, or ragged ones by their offsets.
+struct Fp4Groups {
+  int P;
+  long long rows;          // of the matrix
+  int B;                   // equal groups
+  const int32_t* offsets;  // (P + 1) device, or null
+};
+
+__device__ __forceinline__ long long fp4_first_row(const Fp4Groups& g, int m) {
+  if (g.offsets == nullptr) return (long long)m * g.B;
+  return min(max((long long)__ldg(g.offsets + m), 0ll), g.rows);
+}
+__device__ __forceinline__ long long fp4_end_row(const Fp4Groups& g, int m) {
+  if (g.offsets == nullptr) return (long long)(m + 1) * g.B;
+  const long long first = fp4_first_row(g, m);
+  return max(first, min((long long)__ldg(g.offsets + m + 1), g.rows));
+}
+__device__ __forceinline__ long long fp4_first_tile(const Fp4Groups& g, int m) {
+  if (g.offsets == nullptr) return (long long)m * ((g.B + 127) / 128);
+  return fp4_first_row(g, m) / 128 + m;
+}
+// Group and first row of a tile; false where no row lies in it.
+__device__ __forceinline__ bool fp4_tile(const Fp4Groups& g, long long tile, int& m, long long& row0, int& rows) {
+  if (g.offsets == nullptr) {
+    const int per = (g.B + 127) / 128;
+    m = (int)(tile / per);
+  } else {
+    int lo = 0, hi = g.P - 1;  // the last group whose first tile is not behind this one
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (fp4_first_tile(g, mid) <= tile)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    m = lo;
+  }
+  if (m >= g.P) return false;
+  row0 = fp4_first_row(g, m) + (tile - fp4_first_tile(g, m)) * 128;
+  const long long end = fp4_end_row(g, m);
+  if (row0 >= end || tile < fp4_first_tile(g, m)) return false;
+  rows = (int)min(128ll, end - row0);
+  return true;
+}
+
+__device__ __forceinline__ float pow2f(int n) { return __uint_as_float((uint32_t)(n + 127) << 23); }
+
+// 2^r of a row with largest magnitude `big`: its significand against that of 2688 = 1.3125 * 2^11.
+__device__ __forceinline__ float nvfp4_row_scale(float big) {
+  const uint32_t u = __float_as_uint(big);
+  const int e = (int)(u >> 23) - 127;
+  const int r = e - ((u & 0x7FFFFFu) > 0x280000u ? 10 : 11);
+  return pow2f(max(r, -100));
+}
+
+struct Fp4QuantArgs {
+  Fp4Groups groups;
+  int K;
+  const void* x;
+  long long ld;
+  const int32_t* n_features;  // (P) or null: columns of a group's rows that count
+  Fp4Rows out;
+  int tiles;
+};
+
+// Eight values as four bytes of codes, the first in the lowest half byte.
+__device__ __forceinline__ uint32_t fp4_pack8(const float (&q)[8]) {
+  uint32_t r;
+  asm("{\n .reg .b8 a, b, c, d;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+      " mov.b32 %0, {a, b, c, d};\n}\n"
+      : "=r"(r)
+      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
+  return r;
+}
+
+// One block's codes and scale byte from its values; `row` is the row's 2^r (nvfp4).
+template <int FORMAT, int N>
+__device__ __forceinline__ uint8_t fp4_block(const float (&x)[N], float row, uint32_t (&codes)[N / 8]) {
+  float big = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) big = fmaxf(big, fabsf(x[i]));
+  float s;
+  uint8_t byte;
+  if constexpr (FORMAT == FP4_NV) {
+    byte = (uint8_t)__nv_cvt_float_to_fp8(__fdiv_rn(big, 6.f * row), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t e = byte >> 3, f = byte & 7u;
+    s = (e ? __uint_as_float(((e + 120u) << 23) | (f << 20)) : (float)f * 0.001953125f) * row;
+  } else {
+    const int e = max((int)(__float_as_uint(big) >> 23) - 129, -100);
+    byte = (uint8_t)(e + 127);
+    s = pow2f(e);
+  }
+  const float inv = s > 0.f ? 1.f / s : 0.f;
+#pragma unroll
+  for (int j = 0; j < N / 8; ++j) {
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float v = x[8 * j + i];
+      q[i] = v * inv;
+      // the correctly rounded quotient (Markstein: one correction by the exact remainder)
+      if constexpr (FORMAT == FP4_NV) q[i] = fmaf(fmaf(-q[i], s, v), inv, q[i]);
+    }
+    codes[j] = fp4_pack8(q);
+  }
+  return byte;
+}
+
+// A block of the grid takes 8 rows of a tile, a warp each: rows i, i + 32, i + 64, i + 96 for two consecutive i, whose
+// scale bytes make up whole 32-byte sectors of the tile.
+template <typename T, int FORMAT>
+__global__ void __launch_bounds__(256) fp4_quantize_kernel(const Fp4QuantArgs a) {
+  constexpr int N = FORMAT == FP4_NV ? 16 : 32;
+  const int tile = blockIdx.x >> 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = 2 * (blockIdx.x & 15) + (warp & 1) + 32 * (warp >> 1);  // row of the tile
+  int m, rows;
+  long long row0;
+  if (!fp4_tile(a.groups, tile, m, row0, rows)) return;
+  const bool live = r < rows;
+  const long long row = row0 + r;
+  const int n = a.n_features ? min(__ldg(a.n_features + m), a.K) : a.K;
+  const T* x = static_cast<const T*>(a.x) + row * a.ld;
+  float big = 0.f;
+  if (live) {
+    for (int c = lane; c < n; c += 32) big = max_nan(big, fabsf((float)x[c]));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) big = max_nan(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+  }
+  const bool finite = big < INFINITY;
+  const float scale = FORMAT == FP4_NV ? nvfp4_row_scale(big) : 1.f;
+  if (live && lane == 0) a.out.row_scale[row] = finite ? scale : __uint_as_float(0x7FC00000u);
+  const int blocks = a.out.atoms * 4;  // with those of the padding, which are zero
+  uint8_t* to = a.out.scales + (long long)tile * a.out.atoms * 512;
+  for (int b = lane; b < blocks; b += 32) {
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = b * N + i;
+      v[i] = (live && finite && c < n) ? (float)x[c] : 0.f;
+    }
+    uint32_t codes[N / 8];
+    const uint8_t byte = fp4_block<FORMAT, N>(v, scale, codes);
+    to[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = live ? byte : (uint8_t)0;
+    if (live && b * (N / 2) < a.out.pitch) {
+      uint32_t* cp = reinterpret_cast<uint32_t*>(a.out.codes + row * a.out.pitch + b * (N / 2));
+#pragma unroll
+      for (int j = 0; j < N / 8; ++j) cp[j] = codes[j];
+    }
+  }
+}
+
+struct Fp4ValuesArgs {
+  Fp4Groups groups;
+  int K;
+  Fp4Rows in;
+  __nv_bfloat16* out;  // (rows, K)
+};
+
+__device__ __forceinline__ float fp4_value(uint32_t code) {
+  // e2m1 as fp32: 0 and 0.5 below the normal numbers
+  const uint32_t m = code & 7u;
+  const float v = m < 2u ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
+  return (code & 8u) ? -v : v;
+}
+
+template <int FORMAT>
+__global__ void __launch_bounds__(256) fp4_values_kernel(const Fp4ValuesArgs a) {
+  constexpr int N = FORMAT == FP4_NV ? 16 : 32;
+  const int tile = blockIdx.x >> 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = 2 * (blockIdx.x & 15) + (warp & 1) + 32 * (warp >> 1);
+  int m, rows;
+  long long row0;
+  if (!fp4_tile(a.groups, tile, m, row0, rows) || r >= rows) return;
+  const long long row = row0 + r;
+  const float rs = a.in.row_scale[row];
+  const uint8_t* from = a.in.scales + (long long)tile * a.in.atoms * 512;
+  for (int b = lane; b * N < a.K; b += 32) {
+    const uint32_t byte = from[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)];
+    float s;
+    if (FORMAT == FP4_NV) {
+      const uint32_t e = byte >> 3, f = byte & 7u;
+      s = (e ? __uint_as_float(((e + 120u) << 23) | (f << 20)) : (float)f * 0.001953125f) * rs;
+    } else {
+      s = pow2f((int)byte - 127) * rs;
+    }
+    const uint8_t* cp = a.in.codes + row * a.in.pitch + b * (N / 2);
+    for (int i = 0; i < N && b * N + i < a.K; ++i)
+      a.out[row * a.K + b * N + i] = __float2bfloat16_rn(fp4_value((cp[i >> 1] >> (4 * (i & 1))) & 15u) * s);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// y = relu(q(x) q(w_m)^T + b_m): both operands in 4 bits, block scales applied by the tensor core, sums in fp32, row
+// scales in the epilogue.  A = rows of x (128 a tile), B = rows of w; both K-major, 256 columns (128 bytes) a stage.
+// The scales of a stage are copied from shared to tensor memory by tcgen05.cp, which the tensor core runs in order
+// with the products of the same thread.
+// ---------------------------------------------------------------------------
+struct Fp4Problem {
+  Fp4Groups groups;  // rows of x; groups.P members
+  int x_shared;      // equal groups that all read the same rows of x
+  int K, N;
+  const int32_t* in_f;   // (P) or null
+  const int32_t* out_f;  // (P) or null
+  const uint8_t* x_scales;
+  const float* x_row;
+  const uint8_t* w_scales;  // (P, ceil(N / 128), atoms, 512)
+  const float* w_row;       // (P, N)
+  int atoms;                // of 512 bytes per 128 rows of x or w
+  const float* bias;        // (P, N) or null
+  int relu;
+  void* y;  // (rows of y, N)
+  int y_f32, y_vec;
+  int n_tiles;
+};
+
+enum : int { FT_MMA = 0, FT_ZERO = 1, FT_END = 2 };
+struct Fp4Tile {
+  int kind, member, x_row, y_row, rows, nt, x_tile, n_valid;
+};
+
+template <int BN_, int FORMAT>
+struct Fp4Cfg {
+  static constexpr int BM = 128, BN = BN_, BK = 256;
+  static constexpr int ATOMS = FORMAT == FP4_NV ? 4 : 2;  // scale tiles of 128 rows a stage
+  static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128;
+  static constexpr int SB_TILES = BN > 128 ? BN / 128 : 1;
+  static constexpr int SA_BYTES = ATOMS * 512, SB_BYTES = SB_TILES * ATOMS * 512;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;
+  static constexpr int STAGES = BN == 256 ? 3 : BN == 128 ? 5 : 6;
+  static constexpr int ACCS = BN == 256 ? 1 : 2;
+  static constexpr int SA_COL = ACCS * BN, SB_COL = SA_COL + 16;  // tensor memory columns of the scales
+  static constexpr int TMEM_COLS = BN == 64 ? 256 : 512;
+  static_assert(SB_COL + SB_TILES * ATOMS * 4 <= TMEM_COLS, "tensor memory");
+  static constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
+  static constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
+  static constexpr int TRING = 4;
+  static constexpr int CTRL_BYTES = 512;
+  static constexpr int ROW_BYTES = 144;  // a warp's staged row of 32 values, padded
+  static constexpr int WCOLS = BN / 2;
+  static constexpr int SMEM_BYTES =
+      1024 + STAGES * STAGE_BYTES + CTRL_BYTES + EPI_WARPS * (32 * ROW_BYTES + WCOLS * 8);
+  static_assert(SMEM_BYTES <= 227 * 1024, "fits an SM");
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// 128 rows' scales (32 x 16 bytes) into four columns of tensor memory, the same in each quarter of the lanes.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)(128 >> 4) << 32;  // 8-row groups 128 bytes apart, no swizzle
+  d |= (uint64_t)1 << 46;
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+
+template <int FORMAT>
+__device__ __forceinline__ void umma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa,
+                                         uint32_t sb, uint32_t accumulate) {
+  if constexpr (FORMAT == FP4_NV)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+}
+
+// Instruction descriptor: A and B e2m1, M = 128; scales e4m3 (nvfp4) or powers of two (mxfp4), `id` the half of a
+// scale word that this product takes (mxfp4: 0 or 2).
+template <int FORMAT>
+__device__ __forceinline__ uint32_t idesc_fp4(int n, uint32_t id) {
+  return (id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((FORMAT == FP4_MX ? 1u : 0u) << 23) |
+         (1u << 27) | (id << 29);
+}
+
+template <int BN, int FORMAT>
+__global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
+    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Fp4Problem pr) {
+  using Cfg = Fp4Cfg<BN, FORMAT>;
+  extern __shared__ uint8_t dyn_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
+  uint8_t* smA = smem;
+  uint8_t* smB = smA + Cfg::STAGES * Cfg::A_BYTES;
+  uint8_t* smSA = smB + Cfg::STAGES * Cfg::B_BYTES;
+  uint8_t* smSB = smSA + Cfg::STAGES * Cfg::SA_BYTES;
+  uint8_t* ctrl = smem + Cfg::STAGES * Cfg::STAGE_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ctrl);
+  uint64_t* empty = full + Cfg::STAGES;
+  uint64_t* tfull = empty + Cfg::STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* done_bar = tempty + 2;
+  constexpr int TRING = Cfg::TRING;
+  uint64_t* tr_full = done_bar + 1;
+  uint64_t* tr_empty = tr_full + TRING;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tr_empty + TRING);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* ring = reinterpret_cast<volatile int*>(ctrl + 256);
+  static_assert(8 * (2 * Cfg::STAGES + 5 + 2 * TRING) + 8 <= 256 && 256 + 32 * TRING <= Cfg::CTRL_BYTES, "control block");
+  const int warp = warp_id(), lane = lane_id();
+  const int n_sb_tiles = (pr.N + 127) / 128;  // scale tiles of a member's rows of w
+
+  // (`whole`: all lanes of the warp read, and lane 0 frees the slot once they have)
+  auto ring_read = [&](int k, bool whole) -> Fp4Tile {
+    Fp4Tile t;
+    const int s = k & (TRING - 1);
+    if (!mbar_wait(&tr_full[s], (uint32_t)(k / TRING) & 1u, abort_flag)) {
+      t.kind = FT_END;
+      return t;
+    }
+    const volatile int* e = ring + 8 * s;
+    t.kind = e[0];
+    t.member = e[1];
+    t.x_row = e[2];
+    t.y_row = e[3];
+    t.rows = e[4];
+    t.nt = e[5];
+    t.x_tile = e[6];
+    t.n_valid = e[7];
+    if (whole) __syncwarp();
+    if (!whole || lane == 0) mbar_arrive(&tr_empty[s]);
+    return t;
+  };
+  auto k_blocks = [&](int member) {
+    const int k = pr.in_f ? min(__ldg(pr.in_f + member), pr.K) : pr.K;
+    return (k + Cfg::BK - 1) / Cfg::BK;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], Cfg::EPI_WARPS);
+    }
+    mbar_init(done_bar, 1);
+    for (int i = 0; i < TRING; ++i) {
+      mbar_init(&tr_full[i], 1);
+      mbar_init(&tr_empty[i], 2 + Cfg::EPI_WARPS);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        const Fp4Tile t = ring_read(k, false);
+        if (t.kind == FT_END) break;
+        if (t.kind != FT_MMA) continue;
+        const int kblocks = k_blocks(t.member);
+        const uint8_t* sa = pr.x_scales + (long long)t.x_tile * pr.atoms * 512;
+        const int sb_tile = t.nt * BN / 128;
+        const uint8_t* sb = pr.w_scales + ((long long)t.member * n_sb_tiles + sb_tile) * pr.atoms * 512;
+        const int sb_n = min(Cfg::SB_TILES, n_sb_tiles - sb_tile);
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[stage], Cfg::A_BYTES + Cfg::B_BYTES + Cfg::SA_BYTES + sb_n * Cfg::ATOMS * 512);
+          tma_load_3d(smA + stage * Cfg::A_BYTES, &tmA, &full[stage], kb * 128, t.x_row, 0);
+          tma_load_3d(smB + stage * Cfg::B_BYTES, &tmB, &full[stage], kb * 128, t.nt * BN, t.member);
+          bulk_load(smSA + stage * Cfg::SA_BYTES, sa + kb * Cfg::ATOMS * 512, Cfg::ATOMS * 512, &full[stage]);
+          for (int c = 0; c < sb_n; ++c)
+            bulk_load(smSB + stage * Cfg::SB_BYTES + c * Cfg::ATOMS * 512,
+                      sb + ((long long)c * pr.atoms + kb * Cfg::ATOMS) * 512, Cfg::ATOMS * 512, &full[stage]);
+          if (++stage == Cfg::STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA
+    if (lane == 0) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        const Fp4Tile t = ring_read(k, false);
+        if (t.kind == FT_END) break;
+        if (t.kind != FT_MMA) continue;
+        const int n_mma = min(BN, (t.n_valid - t.nt * BN + 15) & ~15);
+        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+        // tiles of 64 columns take one half of a scale tile of 128
+        const uint32_t sb_shift = BN == 64 ? (uint32_t)(t.nt & 1) * 2u : 0u;
+        if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, abort_flag)) break;
+        tc_fence_after();
+        const int kblocks = k_blocks(t.member);
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait(&full[stage], phase, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smSA + stage * Cfg::SA_BYTES), sb = smem_u32(smSB + stage * Cfg::SB_BYTES);
+#pragma unroll
+          for (int i = 0; i < Cfg::ATOMS; ++i) tmem_copy_scales(tmem_base + Cfg::SA_COL + 4 * i, sa + 512 * i);
+          // a product's columns of w take consecutive columns of scales: tile c of step i at (i * tiles + c) * 4
+#pragma unroll
+          for (int i = 0; i < Cfg::ATOMS; ++i)
+#pragma unroll
+            for (int c = 0; c < Cfg::SB_TILES; ++c)
+              tmem_copy_scales(tmem_base + Cfg::SB_COL + 4 * (i * Cfg::SB_TILES + c), sb + 512 * (c * Cfg::ATOMS + i));
+          const uint32_t a_base = smem_u32(smA + stage * Cfg::A_BYTES), b_base = smem_u32(smB + stage * Cfg::B_BYTES);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const int i = FORMAT == FP4_NV ? s : s >> 1;
+            const uint32_t id = FORMAT == FP4_NV ? 0u : (uint32_t)(s & 1) * 2u;
+            umma_fp4<FORMAT>(d_tmem, smem_desc_sw128(a_base + s * 32, 16, 1024), smem_desc_sw128(b_base + s * 32, 16, 1024),
+                             idesc_fp4<FORMAT>(n_mma, id), tmem_base + Cfg::SA_COL + 4 * i,
+                             tmem_base + Cfg::SB_COL + 4 * i * Cfg::SB_TILES + sb_shift, (kb | s) != 0 ? 1u : 0u);
+          }
+          umma_commit(&empty[stage]);
+          if (++stage == Cfg::STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        umma_commit(&tfull[acc]);
+        if (++acc == Cfg::ACCS) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      umma_commit(done_bar);
+      volatile int no_abort = 0;
+      mbar_wait(done_bar, 0, &no_abort);
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ scheduler
+    int pub = 0;
+    auto publish = [&](const Fp4Tile& t) -> bool {
+      const int s = pub & (TRING - 1);
+      if (!mbar_wait(&tr_empty[s], ((uint32_t)(pub / TRING) & 1u) ^ 1u, abort_flag)) return false;
+      __syncwarp();
+      if (lane == 0) {
+        volatile int* e = ring + 8 * s;
+        e[0] = t.kind;
+        e[1] = t.member;
+        e[2] = t.x_row;
+        e[3] = t.y_row;
+        e[4] = t.rows;
+        e[5] = t.nt;
+        e[6] = t.x_tile;
+        e[7] = t.n_valid;
+        mbar_arrive(&tr_full[s]);
+      }
+      ++pub;
+      return true;
+    };
+    const Fp4Groups& g = pr.groups;
+    // rows of group i: members, then (ragged) the rows before the first and behind the last member's
+    const int n_groups = g.offsets ? g.P + 2 : g.P;
+    auto group = [&](int i, int& first, int& end) {
+      if (i < g.P) {
+        first = (int)fp4_first_row(g, i);
+        end = (int)fp4_end_row(g, i);
+      } else if (i == g.P) {
+        first = 0;
+        end = (int)fp4_first_row(g, 0);
+      } else {
+        first = (int)fp4_first_row(g, g.P);
+        end = (int)g.rows;
+      }
+    };
+    Fp4Tile t;
+    bool ok = true;
+    int g0 = 0, first = 0, end = 0, tiles = 0, inc = 0;
+    long long before = 0;
+    auto load_groups = [&]() {
+      first = end = 0;
+      if (g0 + lane < n_groups) group(g0 + lane, first, end);
+      tiles = (end - first + Cfg::BM - 1) / Cfg::BM * pr.n_tiles;
+      inc = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+        if (lane >= o) inc += v;
+      }
+    };
+    load_groups();
+    for (long long i = blockIdx.x; ok; i += gridDim.x) {
+      int sum = __shfl_sync(0xFFFFFFFFu, inc, 31);
+      while (i >= before + sum && g0 + 32 < n_groups) {
+        before += sum;
+        g0 += 32;
+        load_groups();
+        sum = __shfl_sync(0xFFFFFFFFu, inc, 31);
+      }
+      if (i >= before + sum) break;
+      const int local = (int)(i - before);
+      const int who = __ffs(__ballot_sync(0xFFFFFFFFu, local < inc)) - 1;
+      const int r = local - __shfl_sync(0xFFFFFFFFu, inc - tiles, who);
+      const int f = __shfl_sync(0xFFFFFFFFu, first, who), e = __shfl_sync(0xFFFFFFFFu, end, who);
+      const int mts = (e - f + Cfg::BM - 1) / Cfg::BM;
+      t.member = g0 + who;
+      t.nt = r / mts;
+      const int mt = r - t.nt * mts;
+      t.y_row = f + mt * Cfg::BM;
+      t.x_row = pr.x_shared ? mt * Cfg::BM : t.y_row;
+      t.rows = min(Cfg::BM, e - t.y_row);
+      t.kind = FT_ZERO;
+      t.n_valid = t.x_tile = 0;
+      if (t.member < g.P) {
+        t.x_tile = (int)(pr.x_shared ? 0 : fp4_first_tile(g, t.member)) + mt;
+        t.n_valid = pr.out_f ? min(__ldg(pr.out_f + t.member), pr.N) : pr.N;
+        if (t.nt * BN < t.n_valid && k_blocks(t.member) > 0) t.kind = FT_MMA;
+      }
+      ok = publish(t);
+    }
+    if (ok) {
+      t.kind = FT_END;
+      publish(t);
+    }
+  } else if (warp >= Cfg::EPI_WARP0) {
+    // ------------------------------------------------------------------ epilogue
+    const int ew = warp - Cfg::EPI_WARP0;
+    const int q = warp & 3, half = ew >> 2;
+    constexpr int WCOLS = Cfg::WCOLS;
+    constexpr int NCH = WCOLS / 32;
+    uint8_t* stage_warp = ctrl + Cfg::CTRL_BYTES + ew * (32 * Cfg::ROW_BYTES + WCOLS * 8);
+    float* sbias = reinterpret_cast<float*>(stage_warp + 32 * Cfg::ROW_BYTES);
+    float* sscale = sbias + WCOLS;
+    uint8_t* stage_row = stage_warp + lane * Cfg::ROW_BYTES;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int k = 0;; ++k) {
+      const Fp4Tile t = ring_read(k, true);
+      if (t.kind == FT_END) break;
+      const int cbase = t.nt * BN + half * WCOLS;
+      const int nch = min(NCH, max(0, (pr.N - cbase + 31) / 32));
+      const int rows = t.rows - q * 32;
+      const long long row0 = (long long)t.y_row + q * 32;
+      const bool mma = t.kind == FT_MMA;
+      float rs = 0.f;
+      if (mma) {
+        __syncwarp();
+        for (int j = lane; j < WCOLS; j += 32) {
+          const bool in = cbase + j < t.n_valid;
+          sbias[j] = (in && pr.bias) ? __ldg(pr.bias + (long long)t.member * pr.N + cbase + j) : 0.f;
+          sscale[j] = in ? __ldg(pr.w_row + (long long)t.member * pr.N + cbase + j) : 0.f;
+        }
+        if (lane < rows) rs = __ldg(pr.x_row + (long long)t.x_row + q * 32 + lane);
+        __syncwarp();
+        if (!mbar_wait(&tfull[acc], acc_phase, abort_flag)) break;
+        tc_fence_after();
+      }
+      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * WCOLS);
+      if (rows > 0) {
+#pragma unroll 1
+        for (int c = 0; c < nch; ++c) {
+          uint32_t v[32];
+          if (mma) {
+            tmem_ld_32x32b_x32(t_row + (uint32_t)(32 * c), v);
+            tmem_wait_ld();
+          }
+          const int nv = t.n_valid - (cbase + 32 * c);
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int o = 32 * c + j + e;
+              x[e] = 0.f;
+              if (mma) {
+                x[e] = fmaf(__uint_as_float(v[j + e]) * rs, sscale[o], sbias[o]);
+                if (pr.relu) x[e] = max_nan(x[e], 0.f);
+                if (j + e >= nv) x[e] = 0.f;
+              }
+            }
+            if (pr.y_f32) {
+              *reinterpret_cast<float4*>(stage_row + j * 4) = make_float4(x[0], x[1], x[2], x[3]);
+              *reinterpret_cast<float4*>(stage_row + j * 4 + 16) = make_float4(x[4], x[5], x[6], x[7]);
+            } else {
+              *reinterpret_cast<uint4*>(stage_row + j * 2) =
+                  make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+            }
+          }
+          __syncwarp();
+          const int col0 = cbase + 32 * c;
+          if (pr.y_vec) {
+            // 16-byte pieces: 8 (fp32) or 4 (bf16) of a row
+            const int per = pr.y_f32 ? 8 : 4, size = pr.y_f32 ? 4 : 2;
+            for (int i = lane; i < 32 * per; i += 32) {
+              const int r = i / per, p = i - r * per;
+              if (r < rows && (col0 * size + 16 * p) < pr.N * size)
+                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(pr.y) + ((row0 + r) * pr.N + col0) * size + 16 * p) =
+                    *reinterpret_cast<const uint4*>(stage_warp + r * Cfg::ROW_BYTES + 16 * p);
+            }
+          } else if (col0 + lane < pr.N) {
+            for (int r = 0; r < min(rows, 32); ++r) {
+              const long long at = (row0 + r) * pr.N + col0 + lane;
+              if (pr.y_f32)
+                static_cast<float*>(pr.y)[at] = *reinterpret_cast<const float*>(stage_warp + r * Cfg::ROW_BYTES + 4 * lane);
+              else
+                static_cast<__nv_bfloat16*>(pr.y)[at] =
+                    *reinterpret_cast<const __nv_bfloat16*>(stage_warp + r * Cfg::ROW_BYTES + 2 * lane);
+            }
+          }
+        }
+      }
+      if (mma) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[acc]);
+        if (++acc == Cfg::ACCS) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+}
+
+}  // namespace tp

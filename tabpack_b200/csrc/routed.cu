@@ -1,0 +1,642 @@
+// C ABI of routing, row moves, ragged linear layers, and 4-bit rows and products (declared in
+// include/tabpack_b200.h): host-side validation, tensor maps and kernel dispatch.
+#include <algorithm>
+
+#include "fp4.cuh"
+#include "host.cuh"
+#include "ragged_gemm.cuh"
+#include "routing.cuh"
+
+namespace tp {
+
+// This translation unit's share of the device-side error flag (read and cleared).
+int take_routed_error(int* v) {
+  TP_CUDA_TRY(cudaMemcpyFromSymbol(v, g_device_error, sizeof(int)));
+  const int zero = 0;
+  TP_CUDA_TRY(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)));
+  return TP_OK;
+}
+
+namespace {
+
+// More than 48 KB of shared memory for a kernel: once per device and kernel.
+template <auto* KERNEL>
+int allow_smem(size_t bytes) {
+  static std::atomic<size_t> have[64] = {};
+  int dev = 0;
+  TP_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return fail(TP_EUNSUPPORTED, "device index %d out of range", dev);
+  if (have[dev].load(std::memory_order_relaxed) >= bytes) return TP_OK;
+  TP_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  have[dev].store(bytes, std::memory_order_relaxed);
+  return TP_OK;
+}
+
+// ------------------------------------------------------------------ routing
+
+// Rows of a block: few rows go to one block, many to at most two blocks an SM.
+int route_rows_per_block(int64_t rows, int32_t k) {
+  if (rows * k <= 1024) return (int)std::max<int64_t>(rows, 1);
+  return (int)std::max<int64_t>(64, (rows + 147) / 148);
+}
+int route_blocks(int64_t rows, int32_t k) {
+  const int per = route_rows_per_block(rows, k);
+  return (int)((rows + per - 1) / per);
+}
+
+int check_route(const tp_route_args* a) {
+  if (!a) return fail(TP_EINVAL, "null routing arguments");
+  if (a->rows <= 0 || a->E <= 0 || a->E > ROUTE_MAX_EXPERTS || a->top_k <= 0 ||
+      a->top_k > std::min(ROUTE_MAX_K, a->E) || a->rows * a->top_k >= (1ll << 31))
+    return fail(TP_EINVAL, "routing needs rows > 0, 1 to %d members, top_k up to %d and the members, rows top_k < 2^31 "
+                "(got %lld, %d, %d)", ROUTE_MAX_EXPERTS, ROUTE_MAX_K, (long long)a->rows, a->E, a->top_k);
+  if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad logits dtype");
+  if (!a->logits || !a->weight || !a->expert) return fail(TP_EINVAL, "null logits, weights or members");
+  if (a->logits_stride < a->E && a->rows > 1) return fail(TP_EINVAL, "rows of logits overlap");
+  if (!aligned_to(dtype_size(a->dtype), {a->logits, a->dlogits}) ||
+      !aligned_to(4, {a->weight, a->expert, a->position, a->offsets, a->importance, a->workspace, a->g_weight, a->g_importance}))
+    return fail(TP_EALIGN, "routing data not aligned to its type");
+  return TP_OK;
+}
+
+RouteArgs route_args(const tp_route_args* a) {
+  RouteArgs k{};
+  k.rows = (int)a->rows;
+  k.E = a->E;
+  k.k = a->top_k;
+  k.renorm = a->renormalize;
+  k.ld = a->logits_stride;
+  k.logits = a->logits;
+  k.weight = a->weight;
+  k.expert = a->expert;
+  k.position = a->position;
+  k.offsets = a->offsets;
+  k.importance = a->importance;
+  k.rows_per_block = route_rows_per_block(a->rows, a->top_k);
+  k.g_weight = a->g_weight;
+  k.g_importance = a->g_importance;
+  k.dlogits = a->dlogits;
+  return k;
+}
+
+template <typename T, int V>
+int launch_route(const RouteArgs& k, cudaStream_t st) {
+  const int blocks = (k.rows + k.rows_per_block - 1) / k.rows_per_block;
+  const size_t smem = route_shared_bytes(k.E);
+  if (blocks == 1) {
+    int rc = allow_smem<route_small_kernel<T, V>>(smem);
+    if (rc) return rc;
+    route_small_kernel<T, V><<<1, 32 * ROUTE_WARPS, smem, st>>>(k);
+  } else {
+    int rc = allow_smem<route_gate_kernel<T, V>>(smem);
+    if (!rc) rc = allow_smem<route_place_kernel>(smem);
+    if (rc) return rc;
+    route_gate_kernel<T, V><<<blocks, 32 * ROUTE_WARPS, smem, st>>>(k);
+    route_place_kernel<<<blocks, 32 * ROUTE_WARPS, smem, st>>>(k);
+  }
+  return TP_OK;
+}
+
+template <typename T, int V>
+int launch_route_backward(const RouteArgs& k, cudaStream_t st) {
+  route_backward_kernel<T, V><<<(k.rows + 7) / 8, 256, 0, st>>>(k);
+  return TP_OK;
+}
+
+// Registers a lane needs for a row of E scores.
+template <typename T>
+int dispatch_route(const RouteArgs& k, bool backward, cudaStream_t st) {
+#define TP_ROUTE_V(v) \
+  if (k.E <= 32 * v) return backward ? launch_route_backward<T, v>(k, st) : launch_route<T, v>(k, st);
+  TP_ROUTE_V(1)
+  TP_ROUTE_V(2)
+  TP_ROUTE_V(4)
+  TP_ROUTE_V(9)
+  TP_ROUTE_V(16)
+  TP_ROUTE_V(32)
+#undef TP_ROUTE_V
+  return fail(TP_EINVAL, "too many members");
+}
+
+// ------------------------------------------------------------------ row moves
+
+int check_rows(const tp_rows_args* a) {
+  if (!a) return fail(TP_EINVAL, "null row move arguments");
+  if (a->rows <= 0 || a->k <= 0 || a->k > ROUTE_MAX_K || a->W <= 0 || a->E <= 0 || a->rows * a->k >= (1ll << 31))
+    return fail(TP_EINVAL, "row moves need rows, W, E > 0, 1 <= k <= %d, rows k < 2^31 (got %lld, %d, %d, %d)", ROUTE_MAX_K,
+                (long long)a->rows, a->W, a->E, a->k);
+  if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad row dtype");
+  if (!a->position || !a->offsets) return fail(TP_EINVAL, "null plan");
+  if (!aligned_to(dtype_size(a->dtype), {a->x, a->out, a->dout, a->dy}) ||
+      !aligned_to(4, {a->position, a->offsets, a->weight, a->dweight}))
+    return fail(TP_EALIGN, "rows not aligned to their type");
+  return TP_OK;
+}
+
+RowsArgs rows_args(const tp_rows_args* a) {
+  RowsArgs k{};
+  k.T = (int)a->rows;
+  k.k = a->k;
+  k.W = a->W;
+  k.E = a->E;
+  k.position = a->position;
+  k.offsets = a->offsets;
+  k.weight = a->weight;
+  k.x = a->x;
+  k.x_ld = a->x_stride;
+  k.out = a->out;
+  k.dout = a->dout;
+  k.dout_ld = a->dout_stride;
+  k.dy = a->dy;
+  k.dw = a->dweight;
+  return k;
+}
+
+// The widest vectors (bytes) on which every row of the given tables begins.
+int rows_vector(const tp_rows_args* a) {
+  const int size = (int)dtype_size(a->dtype);
+  long long all = (long long)a->W * size | 16;
+  if (a->x) all |= reinterpret_cast<intptr_t>(a->x) | a->x_stride * size;
+  if (a->out) all |= reinterpret_cast<intptr_t>(a->out);
+  if (a->dout) all |= reinterpret_cast<intptr_t>(a->dout) | a->dout_stride * size;
+  if (a->dy) all |= reinterpret_cast<intptr_t>(a->dy);
+  return (int)(all & -all);
+}
+
+enum { ROWS_DISPATCH, ROWS_COMBINE, ROWS_BACKWARD };
+
+template <typename T, int BYTES>
+int launch_rows(RowsArgs k, int what, cudaStream_t st) {
+  k.vecs = k.W / (BYTES / (int)sizeof(T));
+  k.div_vecs = make_fastdiv((uint32_t)k.vecs);
+  if (what != ROWS_BACKWARD) {
+    const long long blocks = ((long long)k.T * k.vecs + 255) / 256;
+    if (blocks > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many elements for one row move");
+    if (what == ROWS_DISPATCH)
+      rows_dispatch_kernel<T, BYTES><<<(unsigned)blocks, 256, 0, st>>>(k);
+    else
+      rows_combine_kernel<T, BYTES><<<(unsigned)blocks, 256, 0, st>>>(k);
+  } else if (k.vecs <= 16) {
+    rows_combine_backward_kernel<T, BYTES, 8><<<(k.T + 31) / 32, 256, 0, st>>>(k);
+  } else if (k.vecs <= 128) {
+    rows_combine_backward_kernel<T, BYTES, 32><<<(k.T + 7) / 8, 256, 0, st>>>(k);
+  } else {
+    rows_combine_backward_kernel<T, BYTES, 256><<<k.T, 256, 0, st>>>(k);
+  }
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+int dispatch_rows(const tp_rows_args* a, int what, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  TP_PROF(TP_PROF_OTHER, st);
+  const RowsArgs k = rows_args(a);
+  const int v = rows_vector(a);
+  if (a->dtype == TP_DTYPE_BF16) {
+    switch (v) {
+      case 2: return launch_rows<__nv_bfloat16, 2>(k, what, st);
+      case 4: return launch_rows<__nv_bfloat16, 4>(k, what, st);
+      case 8: return launch_rows<__nv_bfloat16, 8>(k, what, st);
+      default: return launch_rows<__nv_bfloat16, 16>(k, what, st);
+    }
+  }
+  switch (v) {
+    case 4: return launch_rows<float, 4>(k, what, st);
+    case 8: return launch_rows<float, 8>(k, what, st);
+    default: return launch_rows<float, 16>(k, what, st);
+  }
+}
+
+// ------------------------------------------------------------------ ragged linear layers
+
+// A (planes, rows, inner) tensor with rows at `ld` elements, in 128-byte swizzled boxes of box_inner x box_rows.
+int make_map_ld(CUtensorMap* map, CUtensorMapDataType type, int size, const void* ptr, uint64_t inner, uint64_t rows,
+                uint64_t planes, uint64_t ld, uint32_t box_inner, uint32_t box_rows) {
+  auto enc = encode_fn();
+  if (!enc) return fail(TP_EUNSUPPORTED, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {inner, rows, planes};
+  cuuint64_t strides[2] = {ld * size, ld * size * rows};
+  cuuint32_t box[3] = {box_inner, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, type, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(TP_EINVAL, "cuTensorMapEncodeTiled failed (%d) for dims %llu x %llu x %llu", (int)r,
+                (unsigned long long)planes, (unsigned long long)rows, (unsigned long long)inner);
+  return TP_OK;
+}
+
+constexpr int32_t MAX_WIDTH = 1 << 24;
+
+int check_ragged(const tp_ragged_linear_args* a) {
+  if (!a) return fail(TP_EINVAL, "null ragged linear arguments");
+  if (a->P <= 0 || a->P > 65535 || a->max_in <= 0 || a->max_out <= 0 || a->max_in > MAX_WIDTH || a->max_out > MAX_WIDTH ||
+      a->rows <= 0 || a->rows >= (1ll << 31) - 256)
+    return fail(TP_EINVAL, "a ragged linear layer needs 1 <= P <= 65535, widths > 0, 0 < rows < 2^31 - 256 (got %d, %d, %d, %lld)",
+                a->P, a->max_in, a->max_out, (long long)a->rows);
+  if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad ragged linear dtype");
+  if (!a->offsets || !a->x || !a->w) return fail(TP_EINVAL, "null offsets, x or w");
+  if (a->x_stride < a->max_in || a->w_stride < a->max_in) return fail(TP_EINVAL, "rows of x or w overlap");
+  if (!aligned_to(4, {a->offsets, a->in_features, a->out_features, a->bias, a->dw, a->dbias}) ||
+      !aligned_to(dtype_size(a->dtype), {a->x, a->w, a->y, a->dy, a->dx}))
+    return fail(TP_EALIGN, "ragged linear data not aligned to its type");
+  if (a->dtype == TP_DTYPE_BF16 && (!aligned16(a->x) || !aligned16(a->w) || a->x_stride % 8 || a->w_stride % 8))
+    return fail(TP_EALIGN, "bf16 x and w need 16-byte aligned rows");
+  return TP_OK;
+}
+
+RaggedProblem ragged_problem(const tp_ragged_linear_args* a) {
+  RaggedProblem p{};
+  p.P = a->P;
+  p.R = (int)a->rows;
+  p.in = a->max_in;
+  p.out = a->max_out;
+  p.offsets = a->offsets;
+  p.in_f = a->in_features;
+  p.out_f = a->out_features;
+  return p;
+}
+
+template <int BN, int MODE>
+int launch_ragged(RaggedProblem p, const CUtensorMap& ma, const CUtensorMap& mb, long long tiles, cudaStream_t st) {
+  using Cfg = RaggedCfg<BN, MODE>;
+  int rc = allow_smem<ragged_gemm_kernel<BN, MODE>>(Cfg::SMEM_BYTES);
+  if (rc) return rc;
+  const int grid = (int)std::min<long long>(std::max<long long>(tiles, 1), device_info().sms);
+  TP_PROF(MODE == RAGGED_FWD ? TP_PROF_FWD : MODE == RAGGED_DGRAD ? TP_PROF_DGRAD : TP_PROF_WGRAD, st);
+  ragged_gemm_kernel<BN, MODE><<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(ma, mb, p);
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+// bf16 operands: A and B with their row strides.
+template <int MODE>
+int ragged_bf16(RaggedProblem p, const void* a_ptr, long long a_ld, const void* b_ptr, long long b_ld, cudaStream_t st) {
+  const int cols = MODE == RAGGED_DGRAD ? p.in : p.out;  // columns of the result
+  // tiles along the rows: every member that has rows ends in a partial one
+  const long long m_tiles = MODE == RAGGED_WGRAD ? (long long)p.P * ((p.in + 127) / 128)
+                                                 : std::max<long long>(std::min(p.P, p.R), p.R / 128 + std::min(p.P, p.R) / 2);
+  // the widest tile that still gives every SM one
+  int bn = 256;
+  while (bn > 64 && m_tiles * ((cols + bn - 1) / bn) < device_info().sms) bn /= 2;
+  p.n_tiles = (cols + bn - 1) / bn;
+  p.m_tiles = (p.in + 127) / 128;
+  p.c_vec = aligned16(p.c) && cols % 8 == 0;
+  const long long most = MODE == RAGGED_WGRAD ? m_tiles * p.n_tiles : ((long long)p.R / 128 + p.P + 2) * p.n_tiles;
+  if (most > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many tiles");
+  const auto T = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  CUtensorMap ma, mb;
+  int rc;
+  if (MODE == RAGGED_FWD) {
+    rc = make_map_ld(&ma, T, 2, a_ptr, p.in, p.R, 1, a_ld, 64, 128);
+    if (!rc) rc = make_map_ld(&mb, T, 2, b_ptr, p.in, p.out, p.P, b_ld, 64, bn);
+  } else if (MODE == RAGGED_DGRAD) {
+    rc = make_map_ld(&ma, T, 2, a_ptr, p.out, p.R, 1, a_ld, 64, 128);
+    if (!rc) rc = make_map_ld(&mb, T, 2, b_ptr, p.in, p.out, p.P, b_ld, 64, 64);
+  } else {
+    rc = make_map_ld(&ma, T, 2, a_ptr, p.in, p.R, 1, a_ld, 64, 64);
+    if (!rc) rc = make_map_ld(&mb, T, 2, b_ptr, p.out, p.R, 1, b_ld, 64, 64);
+  }
+  if (rc) return rc;
+  switch (bn) {
+    case 256: return launch_ragged<256, MODE>(p, ma, mb, most, st);
+    case 128: return launch_ragged<128, MODE>(p, ma, mb, most, st);
+    default: return launch_ragged<64, MODE>(p, ma, mb, most, st);
+  }
+}
+
+template <int MODE>
+int ragged_f32(RaggedProblem p, const void* a_ptr, long long a_ld, const void* b_ptr, long long b_ld, cudaStream_t st) {
+  RaggedSimt s{p, static_cast<const float*>(a_ptr), a_ld, static_cast<const float*>(b_ptr), b_ld};
+  s.p.n_tiles = ((MODE == RAGGED_DGRAD ? p.in : p.out) + 63) / 64;
+  s.p.m_tiles = (p.in + 63) / 64;
+  const long long grid = (MODE == RAGGED_WGRAD ? (long long)p.P * s.p.m_tiles : (long long)p.R / 64 + p.P + 2) * s.p.n_tiles;
+  if (grid > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many tiles");
+  TP_PROF(TP_PROF_GEMM_F32, st);
+  ragged_simt_kernel<MODE><<<(unsigned)grid, 256, 0, st>>>(s);
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+// Shares of a member's rows in the bias gradient: about eight blocks an SM, 64 rows each at least.
+int ragged_shares(const tp_ragged_linear_args* a) {
+  const long long strips = (a->max_out + 63) / 64;
+  const long long want = 8ll * 148 / std::max(1ll, strips * a->P), most = a->rows / ((long long)a->P * 64);
+  return (int)std::max(1ll, std::min({want, most, 64ll}));
+}
+// Columns between rows of the copy of g; 0: dy is taken as it is.
+long long ragged_g_stride(const tp_ragged_linear_args* a) {
+  if (a->dx == nullptr && a->dw == nullptr) return 0;
+  if (a->relu) return a->dtype == TP_DTYPE_BF16 ? (a->max_out + 7ll) / 8 * 8 : a->max_out;
+  if (a->dtype == TP_DTYPE_BF16 && (a->dy_stride % 8 || !aligned16(a->dy))) return (a->max_out + 7ll) / 8 * 8;
+  return 0;
+}
+size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// ------------------------------------------------------------------ 4-bit rows
+
+int check_fp4_groups(int32_t P, int32_t K, int32_t format, int64_t rows, const int32_t* offsets, bool shared) {
+  if (P <= 0 || P > (1 << 20) || K <= 0 || K > MAX_WIDTH || rows <= 0 || rows >= (1ll << 31) - 256)
+    return fail(TP_EINVAL, "4-bit rows need P, K > 0, 0 < rows < 2^31 - 256 (got %d, %d, %lld)", P, K, (long long)rows);
+  if (format != TP_FP4_NV && format != TP_FP4_MX) return fail(TP_EINVAL, "bad 4-bit format %d", format);
+  if (!offsets && !shared && rows % P) return fail(TP_EINVAL, "%lld rows are not %d equal groups", (long long)rows, P);
+  if (!aligned_to(4, {offsets})) return fail(TP_EALIGN, "offsets not aligned to their type");
+  return TP_OK;
+}
+
+long long fp4_row_tiles(const Fp4Groups& g) {
+  return g.offsets ? g.rows / 128 + g.P : (long long)g.P * ((g.B + 127) / 128);
+}
+
+int check_fp4(const tp_fp4_args* a) {
+  if (!a) return fail(TP_EINVAL, "null 4-bit row arguments");
+  int rc = check_fp4_groups(a->P, a->K, a->format, a->rows, a->offsets, false);
+  if (rc) return rc;
+  if (!a->codes || !a->scales || !a->row_scale) return fail(TP_EINVAL, "null codes or scales");
+  if (!aligned_to(16, {a->codes, a->scales}) || !aligned_to(4, {a->row_scale, a->n_features}) || !aligned_to(2, {a->values}))
+    return fail(TP_EALIGN, "codes and scales need 16-byte boundaries");
+  return TP_OK;
+}
+
+Fp4Groups fp4_groups(int32_t P, int64_t rows, const int32_t* offsets) {
+  Fp4Groups g{};
+  g.P = P;
+  g.rows = rows;
+  g.B = offsets ? 0 : (int)(rows / P);
+  g.offsets = offsets;
+  return g;
+}
+
+Fp4Rows fp4_rows(const tp_fp4_args* a) {
+  Fp4Rows r{};
+  r.codes = a->codes;
+  r.scales = a->scales;
+  r.row_scale = a->row_scale;
+  r.pitch = tp_fp4_pitch(a->K);
+  r.atoms = tp_fp4_scale_tiles(a->K, a->format);
+  return r;
+}
+
+template <int BN, int FORMAT>
+int launch_fp4(Fp4Problem p, const CUtensorMap& ma, const CUtensorMap& mb, long long tiles, cudaStream_t st) {
+  using Cfg = Fp4Cfg<BN, FORMAT>;
+  int rc = allow_smem<fp4_gemm_kernel<BN, FORMAT>>(Cfg::SMEM_BYTES);
+  if (rc) return rc;
+  const int grid = (int)std::min<long long>(std::max<long long>(tiles, 1), device_info().sms);
+  TP_PROF(TP_PROF_FWD, st);
+  fp4_gemm_kernel<BN, FORMAT><<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(ma, mb, p);
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+}  // namespace
+}  // namespace tp
+
+using namespace tp;
+
+extern "C" {
+
+size_t tp_route_workspace_size(int64_t rows, int32_t E, int32_t top_k) {
+  if (rows <= 0 || E <= 0 || top_k <= 0) return 0;
+  return (size_t)route_blocks(rows, top_k) * (2 * (size_t)E + 1) * 4;
+}
+
+int tp_route_forward(const tp_route_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  TP_PROF(TP_PROF_OTHER, st);
+  int rc = check_route(a);
+  if (rc) return rc;
+  if (!a->position || !a->offsets || !a->importance) return fail(TP_EINVAL, "null routing output");
+  const size_t need = tp_route_workspace_size(a->rows, a->E, a->top_k);
+  if (!a->workspace || a->workspace_bytes < need)
+    return fail(TP_EINVAL, "routing workspace of %zu bytes is smaller than the %zu needed", a->workspace_bytes, need);
+  RouteArgs k = route_args(a);
+  k.counts = static_cast<int32_t*>(a->workspace);
+  k.partial = reinterpret_cast<float*>(k.counts + (size_t)route_blocks(a->rows, a->top_k) * (a->E + 1));
+  rc = a->dtype == TP_DTYPE_BF16 ? dispatch_route<__nv_bfloat16>(k, false, st) : dispatch_route<float>(k, false, st);
+  if (rc) return rc;
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+int tp_route_backward(const tp_route_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  TP_PROF(TP_PROF_OTHER, st);
+  int rc = check_route(a);
+  if (rc) return rc;
+  if (!a->dlogits) return fail(TP_EINVAL, "null routing gradient");
+  const RouteArgs k = route_args(a);
+  rc = a->dtype == TP_DTYPE_BF16 ? dispatch_route<__nv_bfloat16>(k, true, st) : dispatch_route<float>(k, true, st);
+  if (rc) return rc;
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+int tp_dispatch_rows(const tp_rows_args* a, void* stream) {
+  int rc = check_rows(a);
+  if (rc) return rc;
+  if (!a->x || !a->out) return fail(TP_EINVAL, "null rows");
+  tp_rows_args b = *a;
+  b.dout = nullptr;
+  b.dy = nullptr;
+  return dispatch_rows(&b, ROWS_DISPATCH, stream);
+}
+
+int tp_combine_rows(const tp_rows_args* a, void* stream) {
+  int rc = check_rows(a);
+  if (rc) return rc;
+  if (!a->x || !a->out) return fail(TP_EINVAL, "null rows");
+  tp_rows_args b = *a;
+  b.dout = nullptr;
+  b.dy = nullptr;
+  return dispatch_rows(&b, ROWS_COMBINE, stream);
+}
+
+int tp_combine_rows_backward(const tp_rows_args* a, void* stream) {
+  int rc = check_rows(a);
+  if (rc) return rc;
+  if (!a->dout || (a->dweight && !a->x)) return fail(TP_EINVAL, "null rows");
+  if (!a->dy && !a->dweight) return TP_OK;
+  tp_rows_args b = *a;
+  b.out = nullptr;
+  if (!b.dweight) b.x = nullptr;
+  return dispatch_rows(&b, ROWS_BACKWARD, stream);
+}
+
+size_t tp_ragged_linear_workspace_size(const tp_ragged_linear_args* a) {
+  if (!a || a->P <= 0 || a->max_out <= 0 || a->rows <= 0) return 0;
+  size_t n = round256((size_t)a->rows * (size_t)ragged_g_stride(a) * dtype_size(a->dtype));
+  if (a->dbias && ragged_shares(a) > 1) n += (size_t)ragged_shares(a) * a->P * a->max_out * sizeof(float);
+  return n;
+}
+
+int tp_ragged_linear_forward(const tp_ragged_linear_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int rc = check_ragged(a);
+  if (rc) return rc;
+  if (!a->y) return fail(TP_EINVAL, "null ragged linear output");
+  RaggedProblem p = ragged_problem(a);
+  p.bias = a->bias;
+  p.relu = a->relu;
+  p.c = a->y;
+  if (a->dtype == TP_DTYPE_BF16) return ragged_bf16<RAGGED_FWD>(p, a->x, a->x_stride, a->w, a->w_stride, st);
+  return ragged_f32<RAGGED_FWD>(p, a->x, a->x_stride, a->w, a->w_stride, st);
+}
+
+int tp_ragged_linear_backward(const tp_ragged_linear_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int rc = check_ragged(a);
+  if (rc) return rc;
+  if (!a->dy || (a->relu && !a->y)) return fail(TP_EINVAL, "null ragged linear gradient or output");
+  if (a->dy_stride < a->max_out) return fail(TP_EINVAL, "rows of dy overlap");
+  const size_t need = tp_ragged_linear_workspace_size(a);
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace)))
+    return fail(TP_EINVAL, "ragged linear workspace of %zu bytes is smaller than the %zu needed, or not aligned",
+                a->workspace_bytes, need);
+  const bool bf16 = a->dtype == TP_DTYPE_BF16;
+  const long long g_ld = ragged_g_stride(a);
+  const void* g = g_ld ? a->workspace : a->dy;
+  const long long ld = g_ld ? g_ld : a->dy_stride;
+  if (g_ld || a->dbias) {
+    RaggedAct k{};
+    k.P = a->P;
+    k.R = (int)a->rows;
+    k.N = a->max_out;
+    k.S = ragged_shares(a);
+    k.offsets = a->offsets;
+    k.out_f = a->out_features;
+    k.dy = a->dy;
+    k.dy_ld = a->dy_stride;
+    k.y = a->relu ? a->y : nullptr;
+    k.g = g_ld ? a->workspace : nullptr;
+    k.g_ld = g_ld;
+    k.db = a->dbias;
+    k.partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) +
+                                         round256((size_t)a->rows * (size_t)g_ld * dtype_size(a->dtype)));
+    TP_PROF(TP_PROF_ACT_BACKWARD, st);
+    const dim3 grid((a->max_out + 63) / 64, a->P, k.S);
+    if (bf16)
+      ragged_act_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(k);
+    else
+      ragged_act_kernel<float><<<grid, 256, 0, st>>>(k);
+    if (a->dbias && k.S > 1)
+      ragged_bias_kernel<<<(unsigned)(((long long)a->P * a->max_out + 255) / 256), 256, 0, st>>>(k);
+    TP_CUDA_TRY(cudaGetLastError());
+  }
+  RaggedProblem p = ragged_problem(a);
+  if (a->dx) {
+    p.c = a->dx;
+    rc = bf16 ? ragged_bf16<RAGGED_DGRAD>(p, g, ld, a->w, a->w_stride, st)
+              : ragged_f32<RAGGED_DGRAD>(p, g, ld, a->w, a->w_stride, st);
+    if (rc) return rc;
+  }
+  if (a->dw) {
+    p.c = a->dw;
+    rc = bf16 ? ragged_bf16<RAGGED_WGRAD>(p, a->x, a->x_stride, g, ld, st)
+              : ragged_f32<RAGGED_WGRAD>(p, a->x, a->x_stride, g, ld, st);
+    if (rc) return rc;
+  }
+  return TP_OK;
+}
+
+int32_t tp_fp4_pitch(int32_t K) { return (K + 31) / 32 * 16; }
+int32_t tp_fp4_scale_tiles(int32_t K, int32_t format) { return (K + 255) / 256 * (format == TP_FP4_MX ? 2 : 4); }
+
+int tp_fp4_quantize(const tp_fp4_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  TP_PROF(TP_PROF_OTHER, st);
+  int rc = check_fp4(a);
+  if (rc) return rc;
+  if (!a->x || (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16)) return fail(TP_EINVAL, "null x or bad dtype");
+  if (a->x_stride < a->K && a->rows > 1) return fail(TP_EINVAL, "rows of x overlap");
+  if (!aligned_to(dtype_size(a->dtype), {a->x})) return fail(TP_EALIGN, "x not aligned to its type");
+  Fp4QuantArgs k{};
+  k.groups = fp4_groups(a->P, a->rows, a->offsets);
+  k.K = a->K;
+  k.x = a->x;
+  k.ld = a->x_stride;
+  k.n_features = a->n_features;
+  k.out = fp4_rows(a);
+  const long long blocks = fp4_row_tiles(k.groups) * 16;
+  if (blocks > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many rows");
+  const bool bf16 = a->dtype == TP_DTYPE_BF16, nv = a->format == TP_FP4_NV;
+  auto kern = bf16 ? (nv ? fp4_quantize_kernel<__nv_bfloat16, FP4_NV> : fp4_quantize_kernel<__nv_bfloat16, FP4_MX>)
+                   : (nv ? fp4_quantize_kernel<float, FP4_NV> : fp4_quantize_kernel<float, FP4_MX>);
+  kern<<<(unsigned)blocks, 256, 0, st>>>(k);
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+int tp_fp4_values(const tp_fp4_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  TP_PROF(TP_PROF_OTHER, st);
+  int rc = check_fp4(a);
+  if (rc) return rc;
+  if (!a->values) return fail(TP_EINVAL, "null values");
+  Fp4ValuesArgs k{};
+  k.groups = fp4_groups(a->P, a->rows, a->offsets);
+  k.K = a->K;
+  k.in = fp4_rows(a);
+  k.out = static_cast<__nv_bfloat16*>(a->values);
+  const long long blocks = fp4_row_tiles(k.groups) * 16;
+  if (blocks > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many rows");
+  (a->format == TP_FP4_NV ? fp4_values_kernel<FP4_NV> : fp4_values_kernel<FP4_MX>)<<<(unsigned)blocks, 256, 0, st>>>(k);
+  TP_CUDA_TRY(cudaGetLastError());
+  return TP_OK;
+}
+
+int tp_fp4_linear_forward(const tp_fp4_linear_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (!a) return fail(TP_EINVAL, "null 4-bit linear arguments");
+  int rc = check_fp4_groups(a->P, a->K, a->format, a->rows, a->offsets, a->x_shared != 0);
+  if (rc) return rc;
+  if (a->N <= 0 || a->N > MAX_WIDTH) return fail(TP_EINVAL, "a 4-bit linear layer needs N > 0 (got %d)", a->N);
+  if (a->x_shared && a->offsets) return fail(TP_EINVAL, "shared rows have no offsets");
+  if (a->x_shared && a->rows * a->P >= (1ll << 31) - 256) return fail(TP_EINVAL, "too many rows of y");
+  if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad 4-bit linear dtype");
+  if (!a->x_codes || !a->x_scales || !a->x_row_scale || !a->w_codes || !a->w_scales || !a->w_row_scale || !a->y)
+    return fail(TP_EINVAL, "null 4-bit linear operand or output");
+  if (!aligned_to(16, {a->x_codes, a->x_scales, a->w_codes, a->w_scales}) ||
+      !aligned_to(4, {a->x_row_scale, a->w_row_scale, a->bias, a->in_features, a->out_features}) ||
+      !aligned_to(dtype_size(a->dtype), {a->y}))
+    return fail(TP_EALIGN, "codes and scales need 16-byte boundaries");
+  Fp4Problem p{};
+  p.groups = fp4_groups(a->P, a->x_shared ? a->rows * a->P : a->rows, a->offsets);
+  p.x_shared = a->x_shared;
+  p.K = a->K;
+  p.N = a->N;
+  p.in_f = a->in_features;
+  p.out_f = a->out_features;
+  p.x_scales = a->x_scales;
+  p.x_row = a->x_row_scale;
+  p.w_scales = a->w_scales;
+  p.w_row = a->w_row_scale;
+  p.atoms = tp_fp4_scale_tiles(a->K, a->format);
+  p.bias = a->bias;
+  p.relu = a->relu;
+  p.y = a->y;
+  p.y_f32 = a->dtype == TP_DTYPE_F32;
+  p.y_vec = aligned16(a->y) && (long long)a->N * dtype_size(a->dtype) % 16 == 0;
+  const long long rows = p.groups.rows;
+  const long long m_tiles = p.groups.offsets ? std::max<long long>(std::min<long long>(a->P, rows), rows / 128 + std::min<long long>(a->P, rows) / 2)
+                                             : (long long)a->P * ((p.groups.B + 127) / 128);
+  int bn = 256;
+  while (bn > 64 && m_tiles * ((a->N + bn - 1) / bn) < device_info().sms) bn /= 2;
+  p.n_tiles = (a->N + bn - 1) / bn;
+  const long long most = (p.groups.offsets ? rows / 128 + a->P + 2 : m_tiles) * p.n_tiles;
+  if (most > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many tiles");
+  const int pitch = tp_fp4_pitch(a->K);
+  const auto T = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  CUtensorMap ma, mb;
+  rc = make_map_ld(&ma, T, 1, a->x_codes, pitch, a->rows, 1, pitch, 128, 128);
+  if (!rc) rc = make_map_ld(&mb, T, 1, a->w_codes, pitch, a->N, a->P, pitch, 128, bn);
+  if (rc) return rc;
+  const bool nv = a->format == TP_FP4_NV;
+  switch (bn) {
+    case 256: return nv ? launch_fp4<256, FP4_NV>(p, ma, mb, most, st) : launch_fp4<256, FP4_MX>(p, ma, mb, most, st);
+    case 128: return nv ? launch_fp4<128, FP4_NV>(p, ma, mb, most, st) : launch_fp4<128, FP4_MX>(p, ma, mb, most, st);
+    default: return nv ? launch_fp4<64, FP4_NV>(p, ma, mb, most, st) : launch_fp4<64, FP4_MX>(p, ma, mb, most, st);
+  }
+}
+
+}  // extern "C"

@@ -8,6 +8,7 @@ All arithmetic happens in the CUDA kernels; CPU tensors are rejected.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 from torch import Tensor
@@ -1106,6 +1107,396 @@ def label_log_probs_backward(g_log_prob: Tensor | None, g_entropy: Tensor | None
                                    _ptr(g_entropy), sl, sh, dlogits.data_ptr())
         _call('tp_label_log_probs_backward', a, device)
     return dlogits
+
+
+def _rows2(name: str, t: Tensor, shape: tuple, dtype: torch.dtype, device: int) -> tuple[Tensor, int]:
+    """A matrix with contiguous columns and rows that do not overlap (copied where it has none), and its row stride."""
+    if t.dtype is not dtype:
+        raise TypeError(f'{name} must have dtype {dtype}, got {t.dtype}')
+    if t.shape != shape:
+        raise ValueError(f'{name} must be {shape}, got {tuple(t.shape)}')
+    if t.get_device() != device:
+        raise ValueError(f'{name} must be on cuda:{device}, got {t.device}')
+    if t.is_contiguous():
+        return t, shape[1]
+    sr, sc = t.stride()
+    if (sc != 1 and shape[1] != 1) or (shape[0] > 1 and sr < shape[1]):
+        return t.contiguous(), shape[1]
+    return t, sr if shape[0] > 1 else shape[1]
+
+
+def _members(name: str, t: Tensor | None, n: int, device: int) -> Tensor | None:
+    """Whole numbers of the members as int32, or None."""
+    if t is None:
+        return None
+    if t.is_floating_point() or t.is_complex() or t.dtype is torch.bool:
+        raise TypeError(f'{name} must hold whole numbers, got {t.dtype}')
+    return _operand(name, t if t.dtype is torch.int32 else t.to(torch.int32), (n,), torch.int32, device)
+
+
+def route_forward(logits: Tensor, top_k: int, *, renormalize: bool = True
+                  ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """Routing of rows to members by scores (T, E), bf16 or fp32; see `tp_route_forward`.  Returns
+    (weight (T, top_k) fp32, expert (T, top_k) int32, position (T, top_k) int32, offsets (E + 1,)
+    int32, importance (E,) fp32)."""
+    if logits.ndim != 2:
+        raise ValueError('logits must be (rows, members)')
+    device = _device_of('logits', logits)
+    code = _dtype_code(logits.dtype)
+    T, E = logits.shape
+    if not 1 <= E <= _lib.TP_ROUTE_MAX_EXPERTS:
+        raise ValueError(f'logits must have 1 to {_lib.TP_ROUTE_MAX_EXPERTS} members, got {E}')
+    if not 1 <= top_k <= min(E, _lib.TP_ROUTE_MAX_K):
+        raise ValueError(f'top_k must be between 1 and {min(E, _lib.TP_ROUTE_MAX_K)}, got {top_k}')
+    logits, stride = _rows2('logits', logits, (T, E), logits.dtype, device)
+    dev, i32, f32 = logits.device, torch.int32, torch.float32
+    weight, expert, position = (_empty2(T, top_k, d, dev) for d in (f32, i32, i32))
+    if not T:
+        return weight, expert, position, torch.zeros(E + 1, dtype=i32, device=dev), torch.zeros(E, device=dev)
+    offsets = torch.empty_strided((E + 1,), (1,), dtype=i32, device=dev)
+    importance = torch.empty_strided((E,), (1,), dtype=f32, device=dev)
+    need = load().tp_route_workspace_size(T, E, top_k)
+    ws = torch.empty_strided((need // 4,), (1,), dtype=i32, device=dev)
+    a = _lib.RouteArgs(T, E, top_k, code, int(renormalize), logits.data_ptr(), stride, weight.data_ptr(),
+                       expert.data_ptr(), position.data_ptr(), offsets.data_ptr(), importance.data_ptr(), ws.data_ptr(),
+                       need)
+    _call('tp_route_forward', a, device)
+    return weight, expert, position, offsets, importance
+
+
+def route_backward(g_weight: Tensor | None, g_importance: Tensor | None, logits: Tensor, weight: Tensor, expert: Tensor,
+                   *, renormalize: bool = True) -> Tensor:
+    """The scores' gradient (contiguous, of their shape and type) from those of `route_forward`'s
+    weight and importance (either may be None); see `tp_route_backward`."""
+    if logits.ndim != 2 or weight.ndim != 2:
+        raise ValueError('logits must be (rows, members), weight (rows, top_k)')
+    device = _device_of('logits', logits)
+    code = _dtype_code(logits.dtype)
+    T, E = logits.shape
+    k = weight.shape[1]
+    if not 1 <= E <= _lib.TP_ROUTE_MAX_EXPERTS or not 1 <= k <= min(E, _lib.TP_ROUTE_MAX_K):
+        raise ValueError(f'{k} of {E} members cannot be routed to')
+    logits, stride = _rows2('logits', logits, (T, E), logits.dtype, device)
+    weight = _operand('weight', weight, (T, k), torch.float32, device)
+    expert = _operand('expert', expert, (T, k), torch.int32, device)
+    g_weight = _operand('g_weight', g_weight, (T, k), torch.float32, device)
+    g_importance = _operand('g_importance', g_importance, (E,), torch.float32, device)
+    dlogits = _empty2(T, E, logits.dtype, logits.device)
+    if T:
+        a = _lib.RouteArgs(T, E, k, code, int(renormalize), logits.data_ptr(), stride, weight.data_ptr(),
+                           expert.data_ptr(), None, None, None, None, 0, _ptr(g_weight), _ptr(g_importance),
+                           dlogits.data_ptr())
+        _call('tp_route_backward', a, device)
+    return dlogits
+
+
+def _plan(position: Tensor, offsets: Tensor, device: int) -> tuple[Tensor, Tensor, int, int, int]:
+    if position.ndim != 2 or offsets.ndim != 1 or offsets.shape[0] < 2:
+        raise ValueError('position must be (rows, k), offsets (members + 1,)')
+    T, k = position.shape
+    if not 1 <= k <= _lib.TP_ROUTE_MAX_K:
+        raise ValueError(f'a row goes to 1 to {_lib.TP_ROUTE_MAX_K} members, got {k}')
+    E = offsets.shape[0] - 1
+    return (_operand('position', position, (T, k), torch.int32, device),
+            _operand('offsets', offsets, (E + 1,), torch.int32, device), T, k, E)
+
+
+def dispatch_rows(x: Tensor, position: Tensor, offsets: Tensor) -> Tensor:
+    """(T k, W): row t of x (T, W) at each of its places, zero rows behind the last member's; see
+    `tp_dispatch_rows`.  `position` and `offsets` are `route_forward`'s."""
+    if x.ndim != 2:
+        raise ValueError('x must be (rows, features)')
+    device = _device_of('x', x)
+    code = _dtype_code(x.dtype)
+    position, offsets, T, k, E = _plan(position, offsets, device)
+    W = x.shape[1]
+    x, stride = _rows2('x', x, (T, W), x.dtype, device)
+    out = _empty2(T * k, W, x.dtype, x.device)
+    if T and W:
+        a = _lib.RowsArgs(T, k, W, E, code, position.data_ptr(), offsets.data_ptr(), None, x.data_ptr(), stride,
+                          out.data_ptr())
+        _call('tp_dispatch_rows', a, device)
+    return out
+
+
+def combine_rows(y: Tensor, weight: Tensor | None, position: Tensor, offsets: Tensor) -> Tensor:
+    """(T, W): the sum of a row's k rows of y (T k, W), times weight (T, k) fp32 if given; see
+    `tp_combine_rows`.  Without a weight it is also the backward of `dispatch_rows`."""
+    if y.ndim != 2:
+        raise ValueError('y must be (rows k, features)')
+    device = _device_of('y', y)
+    code = _dtype_code(y.dtype)
+    position, offsets, T, k, E = _plan(position, offsets, device)
+    W = y.shape[1]
+    y, stride = _rows2('y', y, (T * k, W), y.dtype, device)
+    weight = _operand('weight', weight, (T, k), torch.float32, device)
+    out = _empty2(T, W, y.dtype, y.device)
+    if T and W:
+        a = _lib.RowsArgs(T, k, W, E, code, position.data_ptr(), offsets.data_ptr(), _ptr(weight), y.data_ptr(), stride,
+                          out.data_ptr())
+        _call('tp_combine_rows', a, device)
+    return out
+
+
+def combine_rows_backward(dout: Tensor, y: Tensor, weight: Tensor | None, position: Tensor, offsets: Tensor, *,
+                          need_dy: bool = True, need_dweight: bool = True) -> tuple[Tensor | None, Tensor | None]:
+    """Backward of `combine_rows`: (dy (T k, W), zero rows behind the last member's; dweight (T, k));
+    see `tp_combine_rows_backward`."""
+    if dout.ndim != 2 or y.ndim != 2:
+        raise ValueError('dout must be (rows, features), y (rows k, features)')
+    device = _device_of('y', y)
+    code = _dtype_code(y.dtype)
+    position, offsets, T, k, E = _plan(position, offsets, device)
+    W = y.shape[1]
+    y, stride = _rows2('y', y, (T * k, W), y.dtype, device)
+    dout, dstride = _rows2('dout', dout, (T, W), y.dtype, device)
+    weight = _operand('weight', weight, (T, k), torch.float32, device)
+    dy = _empty2(T * k, W, y.dtype, y.device) if need_dy else None
+    dw = _empty2(T, k, torch.float32, y.device) if need_dweight else None
+    if T and W and (need_dy or need_dweight):
+        a = _lib.RowsArgs(T, k, W, E, code, position.data_ptr(), offsets.data_ptr(), _ptr(weight), y.data_ptr(), stride,
+                          None, dout.data_ptr(), dstride, _ptr(dy), _ptr(dw))
+        _call('tp_combine_rows_backward', a, device)
+    elif dw is not None:
+        dw.zero_()
+    return dy, dw
+
+
+def _vector_rows(name: str, t: Tensor, shape: tuple, device: int) -> tuple[Tensor, int]:
+    """A matrix as an operand of the ragged products: bf16 rows on 16-byte boundaries (copied to such where not)."""
+    t, stride = _rows2(name, t, shape, t.dtype, device)
+    if t.dtype is torch.bfloat16 and (stride % 8 or t.data_ptr() % 16):
+        cols = _round(shape[1], 8)
+        wide = _empty2(shape[0], cols, t.dtype, t.device)
+        wide[:, : shape[1]] = t
+        return wide, cols
+    return t, stride
+
+
+def _ragged_weight(weight: Tensor, device: int) -> tuple[Tensor, int]:
+    P, N, K = weight.shape
+    if weight.is_contiguous() and (weight.dtype is torch.float32 or (K % 8 == 0 and weight.data_ptr() % 16 == 0)):
+        return weight, K
+    s = weight.stride()
+    if s[2] == 1 and s[1] >= K and s[0] == N * s[1] and (weight.dtype is torch.float32 or (
+            s[1] % 8 == 0 and weight.data_ptr() % 16 == 0)):
+        return weight, s[1]
+    cols = K if weight.dtype is torch.float32 else _round(K, 8)
+    wide = weight.new_empty((P, N, cols))
+    wide[..., :K] = weight
+    return wide, cols
+
+
+def _ragged_operands(x, weight, offsets, in_features, out_features):
+    if x.ndim != 2 or weight.ndim != 3:
+        raise ValueError('x must be (rows, features), weight (pack_size, out, in)')
+    device, dtype = _device_of('x', x), x.dtype
+    code = _dtype_code(dtype)
+    P, N, K = weight.shape
+    if not P or not N or not K:
+        raise ValueError('weight must not be empty')
+    if weight.dtype is not dtype:
+        raise TypeError(f'weight must have dtype {dtype}, got {weight.dtype}')
+    if weight.get_device() != device:
+        raise ValueError(f'weight must be on cuda:{device}, got {weight.device}')
+    if x.shape[1] != K:
+        raise ValueError(f'x must have {K} features, got {x.shape[1]}')
+    offsets = _members('offsets', offsets, P + 1, device)
+    return (device, code, offsets, _members('in_features', in_features, P, device),
+            _members('out_features', out_features, P, device))
+
+
+def ragged_linear_forward(x: Tensor, weight: Tensor, bias: Tensor | None, offsets: Tensor, *,
+                          in_features: Tensor | None = None, out_features: Tensor | None = None,
+                          relu: bool = False) -> Tensor:
+    """Linear layer (+ReLU) of a pack over ragged groups of rows: member m's rows are
+    x[offsets[m] : offsets[m + 1]] of x (R, in), bf16 or fp32 like weight (P, out, in); bias (P, out)
+    fp32 or None; offsets (P + 1,) on the device, not decreasing, within 0 .. R.  Returns y (R, out), zero
+    in the rows of no member and beyond a member's out_features; see `tp_ragged_linear_forward`."""
+    device, code, offsets, inf, outf = _ragged_operands(x, weight, offsets, in_features, out_features)
+    P, N, K = weight.shape
+    R = x.shape[0]
+    bias = _operand('bias', bias, (P, N), torch.float32, device)
+    y = _empty2(R, N, x.dtype, x.device)
+    if R:
+        x, xs = _vector_rows('x', x, (R, K), device)
+        w, ws = _ragged_weight(weight, device)
+        a = _lib.RaggedLinearArgs(P, K, N, code, R, offsets.data_ptr(), _ptr(inf), _ptr(outf), int(relu), x.data_ptr(),
+                                  xs, w.data_ptr(), ws, _ptr(bias), y.data_ptr())
+        _call('tp_ragged_linear_forward', a, device)
+    return y
+
+
+def ragged_linear_backward(dy: Tensor, x: Tensor, weight: Tensor, y: Tensor | None, offsets: Tensor, *,
+                           in_features: Tensor | None = None, out_features: Tensor | None = None, relu: bool = False,
+                           need_dx: bool = True, need_dw: bool = True, need_db: bool = True
+                           ) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
+    """Backward of `ragged_linear_forward`: (dx (R, in) of x's type, dw (P, out, in), db (P, out) fp32);
+    `y` is the forward's output, needed with relu.  See `tp_ragged_linear_backward`."""
+    device, code, offsets, inf, outf = _ragged_operands(x, weight, offsets, in_features, out_features)
+    P, N, K = weight.shape
+    R = x.shape[0]
+    dev, f32 = x.device, torch.float32
+    dy, ds = _rows2('dy', dy, (R, N), x.dtype, device)
+    if relu:
+        if y is None:
+            raise ValueError("the forward's output is needed with relu")
+        y = _operand('y', y, (R, N), x.dtype, device)
+    dx = _empty2(R, K, x.dtype, dev) if need_dx else None
+    dw = torch.empty_strided((P, N, K), (N * K, K, 1), dtype=f32, device=dev) if need_dw else None
+    db = _empty2(P, N, f32, dev) if need_db else None
+    if not (need_dx or need_dw or need_db):
+        return None, None, None
+    if not R:
+        return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
+    x, xs = _vector_rows('x', x, (R, K), device)
+    w, ws = _ragged_weight(weight, device)
+    a = _lib.RaggedLinearArgs(P, K, N, code, R, offsets.data_ptr(), _ptr(inf), _ptr(outf), int(relu), x.data_ptr(), xs,
+                              w.data_ptr(), ws, None, _ptr(y) if relu else None, dy.data_ptr(), ds, _ptr(dx), _ptr(dw),
+                              _ptr(db))
+    need = load().tp_ragged_linear_workspace_size(ctypes.byref(a))
+    if need:
+        scratch = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = scratch.data_ptr(), need
+    _call('tp_ragged_linear_backward', a, device)
+    return dx, dw, db
+
+
+class Fp4Rows(NamedTuple):
+    """Rows in 4-bit floating point, as `fp4_quantize` returns them and `fp4_linear_forward` takes a
+    layer's weights; the layout is described at `tp_fp4_args`."""
+
+    codes: Tensor  # (..., rows, 16 ceil(columns / 32)) uint8: two a byte
+    scales: Tensor  # (..., row tiles, column tiles, 512) uint8: a byte per block of columns
+    row_scale: Tensor  # (..., rows) fp32
+    columns: int
+    format: str  # 'nvfp4' or 'mxfp4'
+
+
+def _fp4_format(format: str) -> int:
+    code = _lib.TP_FP4.get(format)
+    if code is None:
+        raise ValueError(f"format must be 'nvfp4' or 'mxfp4', got {format!r}")
+    return code
+
+
+def _fp4_pitch(K: int) -> int:
+    return (K + 31) // 32 * 16
+
+
+def _fp4_scale_tiles(K: int, code: int) -> int:
+    return (K + 255) // 256 * (4 if code == 0 else 2)
+
+
+def fp4_quantize(x: Tensor, format: str = 'nvfp4', *, offsets: Tensor | None = None,
+                 n_features: Tensor | None = None) -> Fp4Rows:
+    """x (R, K) or (P, R, K), bf16 or fp32, in 4-bit floating point with a scale per block of columns;
+    see `tp_fp4_quantize`.  `n_features` (P,): only the first columns of a member's rows count (the others
+    are zero).  `offsets` (P + 1,): x is (R, K), member m's rows are x[offsets[m] : offsets[m + 1]] (those
+    of no member stay unwritten), and the scales are laid out for `fp4_linear_forward` over these groups."""
+    code = _fp4_format(format)
+    if x.ndim not in (2, 3) or (offsets is not None and x.ndim != 2):
+        raise ValueError('x must be (rows, columns) or (pack_size, rows, columns)')
+    device = _device_of('x', x)
+    dtype = _dtype_code(x.dtype)
+    K = x.shape[-1]
+    if not K:
+        raise ValueError('x must have columns')
+    lead = tuple(x.shape[:-1])
+    rows = x.numel() // K
+    if offsets is not None:
+        if offsets.ndim != 1 or offsets.shape[0] < 2:
+            raise ValueError('offsets must be (pack_size + 1,)')
+        P = offsets.shape[0] - 1
+        offsets = _members('offsets', offsets, P + 1, device)
+        tiles = (rows // 128 + P,)
+    else:
+        P = x.shape[0] if x.ndim == 3 else 1
+        tiles = (*lead[:-1], (lead[-1] + 127) // 128)
+    n_features = _members('n_features', n_features, P, device)
+    x, stride = _rows2('x', x if x.ndim == 2 else x.reshape(rows, K), (rows, K), x.dtype, device)
+    u8, dev = torch.uint8, x.device
+    codes = torch.empty((*lead, _fp4_pitch(K)), dtype=u8, device=dev)
+    scales = torch.empty((*tiles, _fp4_scale_tiles(K, code), 512), dtype=u8, device=dev)
+    row_scale = torch.empty(lead, dtype=torch.float32, device=dev)
+    if rows:
+        a = _lib.Fp4Args(P, K, code, dtype, rows, _ptr(offsets), _ptr(n_features), x.data_ptr(), stride,
+                         codes.data_ptr(), scales.data_ptr(), row_scale.data_ptr())
+        _call('tp_fp4_quantize', a, device)
+    return Fp4Rows(codes, scales, row_scale, K, format)
+
+
+def _fp4_checked(name: str, q: Fp4Rows, device: int, tiles: tuple) -> Fp4Rows:
+    """Codes and scales of the shapes that their columns and format ask for, contiguous."""
+    lead, code = tuple(q.row_scale.shape), _fp4_format(q.format)
+    codes = _operand(f'{name}.codes', q.codes, (*lead, _fp4_pitch(q.columns)), torch.uint8, device)
+    scales = _operand(f'{name}.scales', q.scales, (*tiles, _fp4_scale_tiles(q.columns, code), 512), torch.uint8, device)
+    row_scale = _operand(f'{name}.row_scale', q.row_scale, lead, torch.float32, device)
+    if codes.data_ptr() % 16 or scales.data_ptr() % 16:
+        codes, scales = codes.clone(), scales.clone()
+    return Fp4Rows(codes, scales, row_scale, q.columns, q.format)
+
+
+def fp4_values(q: Fp4Rows) -> Tensor:
+    """The values that `fp4_quantize`'s rows (without offsets) stand for, bf16 (which holds them exactly)."""
+    device = _device_of('codes', q.codes)
+    lead = tuple(q.row_scale.shape)
+    if len(lead) not in (1, 2) or q.columns < 1:
+        raise ValueError('the rows must be (rows, columns) or (pack_size, rows, columns)')
+    q = _fp4_checked('q', q, device, (*lead[:-1], (lead[-1] + 127) // 128))
+    out = torch.empty((*lead, q.columns), dtype=torch.bfloat16, device=q.codes.device)
+    if out.numel():
+        a = _lib.Fp4Args(lead[0] if len(lead) == 2 else 1, q.columns, _fp4_format(q.format), 0, q.row_scale.numel(), None,
+                         None, None, 0, q.codes.data_ptr(), q.scales.data_ptr(), q.row_scale.data_ptr(), out.data_ptr())
+        _call('tp_fp4_values', a, device)
+    return out
+
+
+def fp4_linear_forward(x: Tensor, weight: Fp4Rows, bias: Tensor | None = None, offsets: Tensor | None = None, *,
+                       in_features: Tensor | None = None, out_features: Tensor | None = None,
+                       relu: bool = False) -> Tensor:
+    """Linear layer (+ReLU) of a pack with both operands in 4 bits; see `tp_fp4_linear_forward`.  `weight`:
+    `fp4_quantize` of (P, out, in) (its columns beyond a member's in_features zero); x, bf16 or fp32, is
+    quantised in the weight's format: (P, B, in) or (B, in) shared by the members, giving (P, B, out), or with
+    `offsets` (P + 1,) ragged groups of rows (R, in), giving (R, out).  Bias (P, out) fp32 or None.  The
+    result has x's type."""
+    device = _device_of('x', x)
+    dtype = _dtype_code(x.dtype)
+    if weight.row_scale.ndim != 2:
+        raise ValueError('weight must be (pack_size, out, in) in 4 bits')
+    P, N = weight.row_scale.shape
+    K = weight.columns
+    if not P or not N or K < 1:
+        raise ValueError('weight must not be empty')
+    if weight.codes.get_device() != device:
+        raise ValueError(f'weight must be on cuda:{device}, got {weight.codes.device}')
+    weight = _fp4_checked('weight', weight, device, (P, (N + 127) // 128))
+    if x.shape[-1] != K:
+        raise ValueError(f'x must have {K} features, got {x.shape[-1]}')
+    bias = _operand('bias', bias, (P, N), torch.float32, device)
+    inf, outf = _members('in_features', in_features, P, device), _members('out_features', out_features, P, device)
+    shared = offsets is None and x.ndim == 2
+    if offsets is not None:
+        offsets = _members('offsets', offsets, P + 1, device)
+        if x.ndim != 2:
+            raise ValueError('x must be (rows, features) with offsets')
+    elif x.ndim == 3 and x.shape[0] != P:
+        raise ValueError(f'x must have {P} members, got {x.shape[0]}')
+    elif x.ndim not in (2, 3):
+        raise ValueError('x must be (pack_size, batch, features) or a shared (batch, features)')
+    if shared and inf is not None and P > 1:
+        # members of different widths see different rows, and have scales of their own
+        x, shared = x.expand(P, *x.shape), False
+    y = torch.empty((P, x.shape[0], N) if shared else (*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    if not x.numel():
+        return y
+    q = fp4_quantize(x, weight.format, offsets=offsets, n_features=inf)
+    a = _lib.Fp4LinearArgs(P, K, N, _fp4_format(weight.format), dtype, int(shared), q.row_scale.numel(), _ptr(offsets),
+                           _ptr(inf), _ptr(outf), q.codes.data_ptr(), q.scales.data_ptr(), q.row_scale.data_ptr(),
+                           weight.codes.data_ptr(), weight.scales.data_ptr(), weight.row_scale.data_ptr(), _ptr(bias),
+                           int(relu), y.data_ptr())
+    _call('tp_fp4_linear_forward', a, device)
+    return y
 
 
 def device_error() -> int:
