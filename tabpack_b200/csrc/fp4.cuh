@@ -16,7 +16,7 @@
 // leaves every group the tiles that it needs, since floor(b / 128) - floor(a / 128) + 1 >= ceil((b - a) / 128)).
 #pragma once
 
-#include <cuda_fp4.h>
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -127,29 +127,98 @@ __device__ __forceinline__ uint8_t fp4_block(const float (&x)[N], float row, uin
     s = pow2f(e);
   }
   const float inv = s > 0.f ? 1.f / s : 0.f;
+  const f32x2 inv2 = pair(inv, inv), neg2 = pair(-s, -s);
 #pragma unroll
   for (int j = 0; j < N / 8; ++j) {
     float q[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float v = x[8 * j + i];
-      q[i] = v * inv;
+    for (int i = 0; i < 8; i += 2) {
+      const f32x2 v = pair(x[8 * j + i], x[8 * j + i + 1]);
+      f32x2 t = mul2(v, inv2);
       // the correctly rounded quotient (Markstein: one correction by the exact remainder)
-      if constexpr (FORMAT == FP4_NV) q[i] = fmaf(fmaf(-q[i], s, v), inv, q[i]);
+      if constexpr (FORMAT == FP4_NV) t = fma2(fma2(neg2, t, v), inv2, t);
+      const float2 h = halves(t);
+      q[i] = h.x;
+      q[i + 1] = h.y;
     }
     codes[j] = fp4_pack8(q);
   }
   return byte;
 }
 
-// A block of the grid takes 8 rows of a tile, a warp each: rows i, i + 32, i + 64, i + 96 for two consecutive i, whose
-// scale bytes make up whole 32-byte sectors of the tile.
-template <typename T, int FORMAT>
+// N values from column c on, zeros from column n on.  VEC: the row is on a 16-byte boundary, and so is c.
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void fp4_load(const T* x, int c, int n, float (&v)[N]) {
+  if (VEC && c + N <= n) {
+    constexpr int L = N * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T);
+    uint4 u[L];
+#pragma unroll
+    for (int i = 0; i < L; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(x + c) + i);
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 2) {
+          v[E * i + 2 * j] = __uint_as_float(w[j] << 16);
+          v[E * i + 2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        } else {
+          v[E * i + j] = __uint_as_float(w[j]);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = c + i < n ? (float)x[c + i] : 0.f;
+  }
+}
+
+// The largest magnitude of a row among the columns of this thread's part (of G), NaN if one is.
+template <typename T, int G, bool VEC>
+__device__ __forceinline__ float fp4_row_max(const T* x, int n, int at) {
+  float big = 0.f;
+  int c0 = 0;
+  if constexpr (VEC) {
+    constexpr int E = 16 / (int)sizeof(T), U = 4;
+    const int vecs = n / E;
+    auto take = [&](const uint4& u) {
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      if constexpr (sizeof(T) == 2) {
+        // magnitudes of bf16 are in the order of their bits, NaN above infinity
+        uint32_t m = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+        for (int j = 1; j < 4; ++j) m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
+        big = max_nan(big, max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u)));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) big = max_nan(big, fabsf(__uint_as_float(w[j])));
+      }
+    };
+    int i = at;
+    for (; i + (U - 1) * G < vecs; i += U * G) {
+      uint4 u[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) u[j] = __ldg(reinterpret_cast<const uint4*>(x) + i + j * G);
+#pragma unroll
+      for (int j = 0; j < U; ++j) take(u[j]);
+    }
+    for (; i < vecs; i += G) take(__ldg(reinterpret_cast<const uint4*>(x) + i));
+    c0 = vecs * E;
+  }
+  for (int c = c0 + at; c < n; c += G) big = max_nan(big, fabsf((float)x[c]));
+  return big;
+}
+
+// G threads a row.  G = 32: a block takes 8 rows of a tile, i, i + 32, i + 64, i + 96 for two consecutive i, whose
+// scale bytes make up whole 32-byte sectors of the tile.  G = 256: one row (few rows: latency counts).
+template <typename T, int FORMAT, int G, bool VEC>
 __global__ void __launch_bounds__(256) fp4_quantize_kernel(const Fp4QuantArgs a) {
   constexpr int N = FORMAT == FP4_NV ? 16 : 32;
-  const int tile = blockIdx.x >> 4;
+  constexpr int PER = 128 * G / 256;  // blocks of the grid a tile
+  const int tile = blockIdx.x / PER, part = blockIdx.x % PER;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = 2 * (blockIdx.x & 15) + (warp & 1) + 32 * (warp >> 1);  // row of the tile
+  const int at = G == 32 ? lane : (int)threadIdx.x;
+  const int r = G == 32 ? 2 * part + (warp & 1) + 32 * (warp >> 1) : part;  // row of the tile
   int m, rows;
   long long row0;
   if (!fp4_tile(a.groups, tile, m, row0, rows)) return;
@@ -157,33 +226,46 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const Fp4QuantArgs a)
   const long long row = row0 + r;
   const int n = a.n_features ? min(__ldg(a.n_features + m), a.K) : a.K;
   const T* x = static_cast<const T*>(a.x) + row * a.ld;
-  float big = 0.f;
-  if (live) {
-    for (int c = lane; c < n; c += 32) big = max_nan(big, fabsf((float)x[c]));
+  __shared__ float warp_max[8];
+  float scale = 1.f, big = 0.f;
+  auto row_max = [&]() {
 #pragma unroll
     for (int o = 16; o; o >>= 1) big = max_nan(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+    if constexpr (G > 32) {
+      if (lane == 0) warp_max[warp] = big;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < 8; ++w) big = max_nan(big, warp_max[w]);
+    }
+  };
+  if constexpr (FORMAT == FP4_NV) {
+    if (live) big = fp4_row_max<T, G, VEC>(x, n, at);
+    row_max();
+    scale = nvfp4_row_scale(big);
   }
-  const bool finite = big < INFINITY;
-  const float scale = FORMAT == FP4_NV ? nvfp4_row_scale(big) : 1.f;
-  if (live && lane == 0) a.out.row_scale[row] = finite ? scale : __uint_as_float(0x7FC00000u);
   const int blocks = a.out.atoms * 4;  // with those of the padding, which are zero
   uint8_t* to = a.out.scales + (long long)tile * a.out.atoms * 512;
-  for (int b = lane; b < blocks; b += 32) {
+  const bool zero = !live || (FORMAT == FP4_NV && !(big < INFINITY));
+  for (int b = at; b < blocks; b += G) {
     float v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = b * N + i;
-      v[i] = (live && finite && c < n) ? (float)x[c] : 0.f;
-    }
+    fp4_load<T, N, VEC>(x, b * N, zero ? 0 : n, v);
     uint32_t codes[N / 8];
     const uint8_t byte = fp4_block<FORMAT, N>(v, scale, codes);
-    to[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = live ? byte : (uint8_t)0;
-    if (live && b * (N / 2) < a.out.pitch) {
-      uint32_t* cp = reinterpret_cast<uint32_t*>(a.out.codes + row * a.out.pitch + b * (N / 2));
+    if constexpr (FORMAT == FP4_MX) {
 #pragma unroll
-      for (int j = 0; j < N / 8; ++j) cp[j] = codes[j];
+      for (int i = 0; i < N; ++i) big = max_nan(big, fabsf(v[i]));
+    }
+    to[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = live && b * N < a.K ? byte : (uint8_t)0;
+    if (live && b * (N / 2) < a.out.pitch) {
+      uint8_t* cp = a.out.codes + row * a.out.pitch + b * (N / 2);
+      if constexpr (FORMAT == FP4_NV)
+        *reinterpret_cast<uint2*>(cp) = make_uint2(codes[0], codes[1]);
+      else
+        *reinterpret_cast<uint4*>(cp) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
     }
   }
+  if constexpr (FORMAT == FP4_MX) row_max();
+  if (live && at == 0) a.out.row_scale[row] = big < INFINITY ? scale : __uint_as_float(0x7FC00000u);
 }
 
 struct Fp4ValuesArgs {
@@ -193,27 +275,38 @@ struct Fp4ValuesArgs {
   __nv_bfloat16* out;  // (rows, K)
 };
 
-__device__ __forceinline__ float fp4_value(uint32_t code) {
-  // e2m1 as fp32: 0 and 0.5 below the normal numbers
-  const uint32_t m = code & 7u;
-  const float v = m < 2u ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-  return (code & 8u) ? -v : v;
+// Four codes' values times s, which bf16 holds exactly, as two words of two.
+__device__ __forceinline__ uint2 fp4_decode4(uint32_t codes, float s) {
+  uint32_t lo, hi;
+  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %2;\n"
+      " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
+  const float2 x = __half22float2(*reinterpret_cast<__half2*>(&lo)), y = __half22float2(*reinterpret_cast<__half2*>(&hi));
+  return make_uint2(pack_bf16x2(x.x * s, x.y * s), pack_bf16x2(y.x * s, y.y * s));
 }
 
-template <int FORMAT>
+// A thread takes eight columns (four bytes of codes), consecutive threads consecutive ones.
+template <int FORMAT, int G, bool VEC>
 __global__ void __launch_bounds__(256) fp4_values_kernel(const Fp4ValuesArgs a) {
   constexpr int N = FORMAT == FP4_NV ? 16 : 32;
-  const int tile = blockIdx.x >> 4;
+  constexpr int PER = 128 * G / 256;
+  const int tile = blockIdx.x / PER, part = blockIdx.x % PER;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = 2 * (blockIdx.x & 15) + (warp & 1) + 32 * (warp >> 1);
+  const int at = G == 32 ? lane : (int)threadIdx.x;
+  const int r = G == 32 ? 2 * part + (warp & 1) + 32 * (warp >> 1) : part;
   int m, rows;
   long long row0;
   if (!fp4_tile(a.groups, tile, m, row0, rows) || r >= rows) return;
   const long long row = row0 + r;
-  const float rs = a.in.row_scale[row];
-  const uint8_t* from = a.in.scales + (long long)tile * a.in.atoms * 512;
-  for (int b = lane; b * N < a.K; b += 32) {
-    const uint32_t byte = from[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)];
+  const float rs = __ldg(a.in.row_scale + row);
+  const uint8_t* from = a.in.scales + (long long)tile * a.in.atoms * 512 + (r & 31) * 16 + (r >> 5) * 4;
+  const uint32_t* codes = reinterpret_cast<const uint32_t*>(a.in.codes + row * a.in.pitch);
+  __nv_bfloat16* out = a.out + row * a.K;
+#pragma unroll 4
+  for (int i = at; 8 * i < a.K; i += G) {
+    const int b = 8 * i / N;
+    const uint32_t byte = __ldg(from + (b >> 2) * 512 + (b & 3)), c = __ldg(codes + i);
     float s;
     if (FORMAT == FP4_NV) {
       const uint32_t e = byte >> 3, f = byte & 7u;
@@ -221,9 +314,15 @@ __global__ void __launch_bounds__(256) fp4_values_kernel(const Fp4ValuesArgs a) 
     } else {
       s = pow2f((int)byte - 127) * rs;
     }
-    const uint8_t* cp = a.in.codes + row * a.in.pitch + b * (N / 2);
-    for (int i = 0; i < N && b * N + i < a.K; ++i)
-      a.out[row * a.K + b * N + i] = __float2bfloat16_rn(fp4_value((cp[i >> 1] >> (4 * (i & 1))) & 15u) * s);
+    const uint2 lo = fp4_decode4(c, s), hi = fp4_decode4(c >> 16, s);
+    if (VEC && 8 * i + 8 <= a.K) {
+      *reinterpret_cast<uint4*>(out + 8 * i) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    } else {
+      const uint32_t w[4] = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (8 * i + j < a.K) reinterpret_cast<uint16_t*>(out)[8 * i + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+    }
   }
 }
 

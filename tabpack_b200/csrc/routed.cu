@@ -377,6 +377,34 @@ Fp4Rows fp4_rows(const tp_fp4_args* a) {
   return r;
 }
 
+// Rows of up to this many tiles go to a block each: a warp a row leaves most of the GPU idle there, and takes a
+// row's pieces one after the other.
+constexpr long long FP4_FEW_TILES = 8;
+
+template <typename T, int FORMAT>
+int launch_quantize(const Fp4QuantArgs& k, bool vec, cudaStream_t st) {
+  const long long tiles = fp4_row_tiles(k.groups);
+  const bool few = tiles <= FP4_FEW_TILES;
+  const long long blocks = tiles * (few ? 128 : 16);
+  if (blocks > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many rows");
+  auto kern = few ? (vec ? fp4_quantize_kernel<T, FORMAT, 256, true> : fp4_quantize_kernel<T, FORMAT, 256, false>)
+                  : (vec ? fp4_quantize_kernel<T, FORMAT, 32, true> : fp4_quantize_kernel<T, FORMAT, 32, false>);
+  kern<<<(unsigned)blocks, 256, 0, st>>>(k);
+  return TP_OK;
+}
+
+template <int FORMAT>
+int launch_values(const Fp4ValuesArgs& k, bool vec, cudaStream_t st) {
+  const long long tiles = fp4_row_tiles(k.groups);
+  const bool few = tiles <= FP4_FEW_TILES;
+  const long long blocks = tiles * (few ? 128 : 16);
+  if (blocks > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many rows");
+  auto kern = few ? (vec ? fp4_values_kernel<FORMAT, 256, true> : fp4_values_kernel<FORMAT, 256, false>)
+                  : (vec ? fp4_values_kernel<FORMAT, 32, true> : fp4_values_kernel<FORMAT, 32, false>);
+  kern<<<(unsigned)blocks, 256, 0, st>>>(k);
+  return TP_OK;
+}
+
 template <int BN, int FORMAT>
 int launch_fp4(Fp4Problem p, const CUtensorMap& ma, const CUtensorMap& mb, long long tiles, cudaStream_t st) {
   using Cfg = Fp4Cfg<BN, FORMAT>;
@@ -557,12 +585,11 @@ int tp_fp4_quantize(const tp_fp4_args* a, void* stream) {
   k.ld = a->x_stride;
   k.n_features = a->n_features;
   k.out = fp4_rows(a);
-  const long long blocks = fp4_row_tiles(k.groups) * 16;
-  if (blocks > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many rows");
-  const bool bf16 = a->dtype == TP_DTYPE_BF16, nv = a->format == TP_FP4_NV;
-  auto kern = bf16 ? (nv ? fp4_quantize_kernel<__nv_bfloat16, FP4_NV> : fp4_quantize_kernel<__nv_bfloat16, FP4_MX>)
-                   : (nv ? fp4_quantize_kernel<float, FP4_NV> : fp4_quantize_kernel<float, FP4_MX>);
-  kern<<<(unsigned)blocks, 256, 0, st>>>(k);
+  const size_t size = dtype_size(a->dtype);
+  const bool vec = aligned16(a->x) && a->x_stride * size % 16 == 0, nv = a->format == TP_FP4_NV;
+  rc = a->dtype == TP_DTYPE_BF16 ? (nv ? launch_quantize<__nv_bfloat16, FP4_NV>(k, vec, st) : launch_quantize<__nv_bfloat16, FP4_MX>(k, vec, st))
+                                 : (nv ? launch_quantize<float, FP4_NV>(k, vec, st) : launch_quantize<float, FP4_MX>(k, vec, st));
+  if (rc) return rc;
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;
 }
@@ -578,9 +605,9 @@ int tp_fp4_values(const tp_fp4_args* a, void* stream) {
   k.K = a->K;
   k.in = fp4_rows(a);
   k.out = static_cast<__nv_bfloat16*>(a->values);
-  const long long blocks = fp4_row_tiles(k.groups) * 16;
-  if (blocks > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many rows");
-  (a->format == TP_FP4_NV ? fp4_values_kernel<FP4_NV> : fp4_values_kernel<FP4_MX>)<<<(unsigned)blocks, 256, 0, st>>>(k);
+  const bool vec = aligned16(a->values) && a->K % 8 == 0;
+  rc = a->format == TP_FP4_NV ? launch_values<FP4_NV>(k, vec, st) : launch_values<FP4_MX>(k, vec, st);
+  if (rc) return rc;
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;
 }
