@@ -12,7 +12,17 @@
 // its tiles by sums over the warp.  A group's last tile reads rows of the next group (they are not stored), and the
 // last block of a cut K loop holds elements beyond the cut: the MMA warp writes zeros over those in shared memory
 // before it multiplies, since a zero factor on one side alone would let a NaN of another member through.
+//
+// Large groups run on CTA pairs (cta_group::2): 256 x 256 tiles of which each CTA stages 128 rows of A and half of B,
+// two thirds of the operand bytes per product.  A stage that needs zeros then completes on a barrier of its own CTA;
+// the peer reports its zeros to the leader, which issues the products.
+//
+// WGRAD sums at most RAGGED_SEGMENT rows in one accumulator and adds the pieces up in dw with the rounding of fp32:
+// the tensor core's own sums do not round to nearest, and over 23054 rows came out 2.6e-5 off (5e-6 with the cut).
+// Few tiles over many rows are split over CTAs, into parts that a second launch adds up in order.
 #pragma once
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -20,6 +30,7 @@ namespace tp {
 
 enum : int { RAGGED_FWD = 0, RAGGED_DGRAD = 1, RAGGED_WGRAD = 2 };
 enum : int { RT_MMA = 0, RT_ZERO = 1, RT_END = 2 };
+constexpr int RAGGED_SEGMENT = 4096;
 
 struct RaggedProblem {
   int P, R;                // members, rows of the matrix
@@ -33,6 +44,7 @@ struct RaggedProblem {
   int c_vec;               // rows of y / dx lie on 16-byte boundaries
   int m_tiles;             // wgrad: tiles of a member along `in`
   int n_tiles;             // tiles along the columns of the result (forward: out, dgrad: in, wgrad: out)
+  int splits;              // wgrad: parts of a member's rows; c holds a (P, out, in) result for each
 };
 
 // Rows of group g: members 0 .. P - 1, then the rows before the first and behind the last member's.
@@ -48,22 +60,29 @@ __device__ __forceinline__ void ragged_group(const RaggedProblem& p, int g, int&
   }
 }
 
+// forward, dgrad: `rows` rows from row0 on; wgrad: input features from row0 on, `rows` is the first row of the sum,
+// `part` its part, `add` whether it goes on top of what dw holds.
 struct RaggedTile {
-  int kind, member, row0, rows, nt, k_len, n_valid, m_valid;
+  int kind, member, row0, rows, nt, k_len, n_valid, m_valid, part, add;
 };
 
-template <int BN_, int MODE>
+template <int BN_, int MODE, bool PAIR_>
 struct RaggedCfg {
+  static constexpr bool PAIR = PAIR_;
+  static_assert(!PAIR || BN_ == 256, "pairs take tiles of 256 columns");
   static constexpr int BM = 128, BN = BN_, BK = 64;
+  static constexpr int TILE_M = PAIR ? 256 : 128;
+  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;  // columns of B that a CTA stages
   static constexpr bool A_MN = MODE == RAGGED_WGRAD;
   static constexpr bool B_MN = MODE != RAGGED_FWD;
-  static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 7;
+  static constexpr int A_BYTES = BM * BK * 2, B_BYTES = B_ROWS * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = PAIR ? 6 : BN == 256 ? 4 : BN == 128 ? 6 : 7;
   static constexpr int TMEM_COLS = 2 * BN;
   static constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
   static constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
   static constexpr int TRING = 4;
-  static constexpr int CTRL_BYTES = 512;
+  static constexpr int RING_INTS = 10;
+  static constexpr int CTRL_BYTES = 640;
   static constexpr int ROW_BYTES = 80;  // a warp's staged row of 32 bf16, padded against bank conflicts
   static constexpr int WCOLS = BN / 2;  // columns of an epilogue warp
   static constexpr int SMEM_BYTES =
@@ -115,30 +134,49 @@ __device__ __forceinline__ void ragged_flush(__nv_bfloat16* c, int ld, int vec, 
   }
 }
 
-template <int BN, int MODE>
-__global__ void __launch_bounds__(RaggedCfg<BN, MODE>::THREADS, 1)
+// Arrive on the mbarrier at this offset in both CTAs of the pair once this thread's MMAs so far have completed.
+__device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+// Columns that a pair multiplies in a tile: the rest of the member's, rounded up to 32 (16 a CTA).
+__device__ __forceinline__ int ragged_n(bool pair, int bn, const RaggedTile& t) {
+  const int left = t.n_valid - t.nt * bn;
+  return min(bn, pair ? (left + 31) & ~31 : (left + 15) & ~15);
+}
+
+template <int BN, int MODE, bool PAIR>
+__global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR>::THREADS, 1)
     ragged_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const RaggedProblem pr) {
-  using Cfg = RaggedCfg<BN, MODE>;
+  using Cfg = RaggedCfg<BN, MODE, PAIR>;
+  constexpr int STAGES = Cfg::STAGES, TRING = Cfg::TRING;
   extern __shared__ uint8_t dyn_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
   uint8_t* smA = smem;
-  uint8_t* smB = smem + Cfg::STAGES * Cfg::A_BYTES;
-  uint8_t* ctrl = smem + Cfg::STAGES * Cfg::STAGE_BYTES;
+  uint8_t* smB = smem + STAGES * Cfg::A_BYTES;
+  uint8_t* ctrl = smem + STAGES * Cfg::STAGE_BYTES;
   uint64_t* full = reinterpret_cast<uint64_t*>(ctrl);
-  uint64_t* empty = full + Cfg::STAGES;
-  uint64_t* tfull = empty + Cfg::STAGES;
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
   uint64_t* tempty = tfull + 2;
   uint64_t* done_bar = tempty + 2;
-  constexpr int TRING = Cfg::TRING;
   uint64_t* tr_full = done_bar + 1;
   uint64_t* tr_empty = tr_full + TRING;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tr_empty + TRING);
+  uint64_t* cut_full = tr_empty + TRING;    // pairs: a stage that needs zeros has landed in this CTA
+  uint64_t* cut_peer = cut_full + STAGES;   // pairs: the peer has put in its zeros
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(cut_peer + STAGES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* ring = reinterpret_cast<volatile int*>(ctrl + 256);  // 8 ints a slot
-  static_assert(8 * (2 * Cfg::STAGES + 5 + 2 * TRING) + 8 <= 256 && 256 + 32 * TRING <= Cfg::CTRL_BYTES, "control block");
+  volatile int* ring = reinterpret_cast<volatile int*>(ctrl + 384);
+  static_assert(8 * (4 * STAGES + 5 + 2 * TRING) + 8 <= 384 && 384 + 4 * Cfg::RING_INTS * TRING <= Cfg::CTRL_BYTES,
+                "control block");
 
   const int warp = warp_id(), lane = lane_id();
+  const int rank = PAIR ? (int)cluster_ctarank() : 0;
+  const int worker = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, workers = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
 
   // (`whole`: all lanes of the warp read, and lane 0 frees the slot once they have)
   auto ring_read = [&](int k, bool whole) -> RaggedTile {
@@ -148,7 +186,7 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE>::THREADS, 1)
       t.kind = RT_END;
       return t;
     }
-    const volatile int* e = ring + 8 * s;
+    const volatile int* e = ring + Cfg::RING_INTS * s;
     t.kind = e[0];
     t.member = e[1];
     t.row0 = e[2];
@@ -157,151 +195,262 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE>::THREADS, 1)
     t.k_len = e[5];
     t.n_valid = e[6];
     t.m_valid = e[7];
+    t.part = e[8];
+    t.add = e[9];
     if (whole) __syncwarp();
     if (!whole || lane == 0) mbar_arrive(&tr_empty[s]);
     return t;
   };
+  // a K loop over the whole width ends where the copies fill with zeros by themselves
+  const int k_full = MODE == RAGGED_FWD ? pr.in : MODE == RAGGED_DGRAD ? pr.out : -1;
+  auto is_cut = [&](const RaggedTile& t) { return (t.k_len & 15) != 0 && t.k_len != k_full; };
+  // zeros from element `left` of a stage's K on, up to the next step of 16; by a whole warp
+  auto zero_tail = [&](int stage, int left) {
+    uint8_t* a = smA + stage * Cfg::A_BYTES;
+    uint8_t* b = smB + stage * Cfg::B_BYTES;
+    const int end = (left + 15) & ~15;
+    if constexpr (Cfg::A_MN)
+      zero_mn_major(a, Cfg::BM / 64, left, end, lane);
+    else
+      zero_k_major(a, Cfg::BM, left, end, lane);
+    if constexpr (Cfg::B_MN)
+      zero_mn_major(b, Cfg::B_ROWS / 64, left, end, lane);
+    else
+      zero_k_major(b, Cfg::B_ROWS, left, end, lane);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+  };
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < Cfg::STAGES; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      mbar_init(&cut_full[s], 1);
+      mbar_init(&cut_peer[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], Cfg::EPI_WARPS);
+      mbar_init(&tempty[i], PAIR ? 2 * Cfg::EPI_WARPS : Cfg::EPI_WARPS);  // the leader's counts both CTAs
     }
     mbar_init(done_bar, 1);
     for (int i = 0; i < TRING; ++i) {
       mbar_init(&tr_full[i], 1);
-      mbar_init(&tr_empty[i], 2 + Cfg::EPI_WARPS);  // producer, MMA warp, epilogue warps
+      mbar_init(&tr_empty[i], 3 + Cfg::EPI_WARPS);  // producers, MMA warp, epilogue warps
     }
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
   }
-  if (warp == 1) tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+  if (warp == 1) {
+    if constexpr (PAIR)
+      tmem_alloc_pair(tmem_slot, Cfg::TMEM_COLS);
+    else
+      tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+  }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the peer's barriers are initialised before any remote arrive
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------ producer
+  if (warp == 0 || warp == 3) {
+    // ------------------------------------------------------------------ producers: A by warp 0, B by warp 3
+    // (one thread takes about 190 cycles a copy, a stage's products 512: with both operands on one thread the issue of
+    // copies bound the gradients, whose operands take two each)
     if (lane == 0) {
+      const bool is_a = warp == 0;
+      const CUtensorMap* map = is_a ? &tmA : &tmB;
+      constexpr bool WG = MODE == RAGGED_WGRAD;
+      const int boxes = is_a ? (Cfg::A_MN ? Cfg::BM / 64 : 1) : (Cfg::B_MN ? Cfg::B_ROWS / 64 : 1);
+      const bool mn = is_a ? Cfg::A_MN : Cfg::B_MN;
+      uint8_t* const ring0 = is_a ? smA : smB;
+      const int bytes = is_a ? Cfg::A_BYTES : Cfg::B_BYTES;
+      const uint32_t leader0 = PAIR ? mapa_shared(smem_u32(full), 0) : 0;
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
+      // One stage: a pair's bytes complete on the leader's barrier, those of a stage that needs zeros (OWN) on this
+      // CTA's own.  The A producer announces the bytes of both (B's may arrive first: the phase waits for its arrival).
+      auto produce = [&](auto own, int x, int y, int z) -> bool {
+        constexpr bool OWN = decltype(own)::value;
+        if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag)) return false;
+        uint64_t* bar = PAIR && OWN ? &cut_full[stage] : &full[stage];
+        if (is_a) {
+          if (OWN)
+            mbar_arrive_expect_tx(bar, Cfg::STAGE_BYTES);
+          else if (rank == 0)
+            mbar_arrive_expect_tx(bar, 2 * Cfg::STAGE_BYTES);
+        }
+        uint8_t* dst = ring0 + stage * bytes;
+        for (int c = 0; c < boxes; ++c) {
+          if constexpr (OWN)
+            tma_load_3d(dst + c * 8192, map, bar, x + (mn ? c * 64 : 0), y, z);
+          else
+            tma_load_3d_pair(dst + c * 8192, map, leader0 + 8u * stage, x + (mn ? c * 64 : 0), y, z);
+        }
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+        return true;
+      };
       for (int k = 0; ok; ++k) {
         const RaggedTile t = ring_read(k, false);
         if (t.kind == RT_END) break;
         if (t.kind != RT_MMA) continue;
         const int kblocks = (t.k_len + Cfg::BK - 1) / Cfg::BK;
-        for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag)) {
-            ok = false;
-            break;
-          }
-          uint8_t* a = smA + stage * Cfg::A_BYTES;
-          uint8_t* b = smB + stage * Cfg::B_BYTES;
-          const int k0 = kb * Cfg::BK;
-          mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
-          if constexpr (MODE == RAGGED_WGRAD) {
-            // row0: the tile's first input feature; `rows`: the member's first row
-#pragma unroll
-            for (int c = 0; c < Cfg::BM / 64; ++c) tma_load_3d(a + c * 8192, &tmA, &full[stage], t.row0 + c * 64, t.rows + k0, 0);
-#pragma unroll
-            for (int c = 0; c < BN / 64; ++c) tma_load_3d(b + c * 8192, &tmB, &full[stage], t.nt * BN + c * 64, t.rows + k0, 0);
-          } else {
-            tma_load_3d(a, &tmA, &full[stage], k0, t.row0, 0);
-            if constexpr (MODE == RAGGED_FWD) {
-              tma_load_3d(b, &tmB, &full[stage], k0, t.nt * BN, t.member);
-            } else {
-#pragma unroll
-              for (int c = 0; c < BN / 64; ++c) tma_load_3d(b + c * 8192, &tmB, &full[stage], t.nt * BN + c * 64, k0, t.member);
-            }
-          }
-          if (++stage == Cfg::STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+        // the copies' coordinates: along K and along the other side
+        const int b_col = t.nt * BN + (PAIR ? rank * (ragged_n(true, BN, t) / 2) : 0);
+        const int other = is_a ? t.row0 + rank * Cfg::BM : b_col;
+        const int k_first = WG ? t.rows : 0, z = (is_a || WG) ? 0 : t.member;
+        const int common = !PAIR ? 0 : is_cut(t) ? kblocks - 1 : kblocks;  // stages on the common barrier
+        int kb = 0;
+        for (; ok && kb < common; ++kb) {
+          const int at = k_first + kb * Cfg::BK;
+          ok = produce(std::bool_constant<!PAIR>(), mn ? other : at, mn ? at : other, z);
+        }
+        for (; ok && kb < kblocks; ++kb) {
+          const int at = k_first + kb * Cfg::BK;
+          ok = produce(std::bool_constant<true>(), mn ? other : at, mn ? at : other, z);
         }
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA
+  } else if (warp == 1 && rank == 0) {
+    // ------------------------------------------------------------------ MMA (a pair's leader fills both CTAs' TMEM)
     int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
-    const int k_full = MODE == RAGGED_FWD ? pr.in : MODE == RAGGED_DGRAD ? pr.out : -1;
+    uint32_t phase = 0, acc_phase = 0, cut_phase = 0;  // cut_phase: a bit per stage
     bool ok = true;
+    // descriptors of the first stage; the address field counts 16 bytes
+    const uint64_t adesc0 = Cfg::A_MN ? smem_desc_sw128(smem_u32(smA), 8192, 1024) : smem_desc_sw128(smem_u32(smA), 16, 1024);
+    const uint64_t bdesc0 = Cfg::B_MN ? smem_desc_sw128(smem_u32(smB), 8192, 1024) : smem_desc_sw128(smem_u32(smB), 16, 1024);
     for (int k = 0; ok; ++k) {
       const RaggedTile t = ring_read(k, true);
       if (t.kind == RT_END) break;
       if (t.kind != RT_MMA) continue;
-      const int n_mma = min(BN, (t.n_valid - t.nt * BN + 15) & ~15);
-      const uint32_t idesc = idesc_bf16_f32(n_mma, Cfg::A_MN, Cfg::B_MN);
+      const uint32_t idesc = idesc_bf16_f32(ragged_n(PAIR, BN, t), Cfg::A_MN, Cfg::B_MN, Cfg::TILE_M);
       const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
       if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, abort_flag)) break;
       tc_fence_after();
       const int kblocks = (t.k_len + Cfg::BK - 1) / Cfg::BK;
-      for (int kb = 0; kb < kblocks; ++kb) {
-        if (!mbar_wait(&full[stage], phase, abort_flag)) {
-          ok = false;
-          break;
-        }
-        uint8_t* a = smA + stage * Cfg::A_BYTES;
-        uint8_t* b = smB + stage * Cfg::B_BYTES;
-        const int left = min(Cfg::BK, t.k_len - kb * Cfg::BK);
-        const int steps = (left + 15) >> 4;
-        // (a K loop over the whole width ends where the copies fill with zeros by themselves)
-        if ((left & 15) && t.k_len != k_full) {
-          if constexpr (Cfg::A_MN)
-            zero_mn_major(a, Cfg::BM / 64, left, 16 * steps, lane);
-          else
-            zero_k_major(a, Cfg::BM, left, 16 * steps, lane);
-          if constexpr (Cfg::B_MN)
-            zero_mn_major(b, BN / 64, left, 16 * steps, lane);
-          else
-            zero_k_major(b, BN, left, 16 * steps, lane);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t a_base = smem_u32(a), b_base = smem_u32(b);
-          for (int s = 0; s < steps; ++s) {
-            const uint64_t adesc = Cfg::A_MN ? smem_desc_sw128(a_base + s * 2048, 8192, 1024)
-                                             : smem_desc_sw128(a_base + s * 32, 16, 1024);
-            const uint64_t bdesc = Cfg::B_MN ? smem_desc_sw128(b_base + s * 2048, 8192, 1024)
-                                             : smem_desc_sw128(b_base + s * 32, 16, 1024);
-            umma_f16(d_tmem, adesc, bdesc, idesc, (kb | s) != 0 ? 1u : 0u);
+      const int last = t.k_len - (kblocks - 1) * Cfg::BK;  // elements of the last block
+      const bool cut = is_cut(t);
+      // a stage's products and its release, by one thread
+      auto multiply = [&](int stage, int steps, bool first) {
+        const uint64_t adesc = adesc0 + (uint64_t)(stage * (Cfg::A_BYTES / 16));
+        const uint64_t bdesc = bdesc0 + (uint64_t)(stage * (Cfg::B_BYTES / 16));
+#pragma unroll
+        for (int s = 0; s < Cfg::BK / 16; ++s) {
+          // 16 elements further along K: 32 bytes of a K-major row, 16 rows of an MN-major block (in units of 16 bytes)
+          const uint64_t ad = adesc + (uint64_t)(s * (Cfg::A_MN ? 128 : 2)), bd = bdesc + (uint64_t)(s * (Cfg::B_MN ? 128 : 2));
+          const uint32_t on = (first && s == 0) ? 0u : 1u;
+          if (s < steps) {
+            if constexpr (PAIR)
+              umma_f16_pair(d_tmem, ad, bd, idesc, on);
+            else
+              umma_f16(d_tmem, ad, bd, idesc, on);
           }
+        }
+        if constexpr (PAIR) {  // frees the stage in both CTAs
+          umma_commit_both(&empty[stage]);
+        } else {
           umma_commit(&empty[stage]);
         }
-        __syncwarp();
-        if (++stage == Cfg::STAGES) {
+      };
+      // one thread goes through the blocks; the whole warp comes together for one that needs zeros
+      const int plain = cut ? kblocks - 1 : kblocks;
+      if (lane == 0) {
+        int st = stage;
+        uint32_t ph = phase;
+        for (int kb = 0; kb < plain; ++kb) {
+          if (!mbar_wait(&full[st], ph, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (kb < kblocks - 1)
+            multiply(st, Cfg::BK / 16, kb == 0);
+          else
+            multiply(st, (last + 15) >> 4, kb == 0);
+          if (++st == STAGES) {
+            st = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      phase ^= (uint32_t)((stage + plain) / STAGES) & 1u;
+      stage = (stage + plain) % STAGES;
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (ok && cut) {
+        if constexpr (PAIR) {
+          const uint32_t ph = (cut_phase >> stage) & 1u;
+          ok = mbar_wait(&cut_full[stage], ph, abort_flag);
+          if (__all_sync(0xFFFFFFFFu, ok)) {
+            zero_tail(stage, last);
+            ok = mbar_wait<true>(&cut_peer[stage], ph, abort_flag);
+          }
+          if (lane == 0) mbar_arrive(&full[stage]);  // the stage's phase goes on without the common barrier
+          cut_phase ^= 1u << stage;
+        } else {
+          ok = mbar_wait(&full[stage], phase, abort_flag);
+          if (__all_sync(0xFFFFFFFFu, ok)) zero_tail(stage, last);
+        }
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (ok) {
+          tc_fence_after();
+          if (lane == 0) multiply(stage, (last + 15) >> 4, kblocks == 1);
+          __syncwarp();
+        }
+        if (++stage == STAGES) {
           stage = 0;
           phase ^= 1u;
         }
       }
       if (!ok) break;
-      if (lane == 0) umma_commit(&tfull[acc]);
+      if (lane == 0) {
+        if constexpr (PAIR) {
+          umma_commit_both(&tfull[acc]);
+        } else {
+          umma_commit(&tfull[acc]);
+        }
+      }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
     }
-    if (lane == 0) umma_commit(done_bar);  // every MMA of this CTA has completed once it flips
+    if (lane == 0) {  // every MMA of this CTA has completed once it flips
+      if constexpr (PAIR)
+        umma_commit_pair(smem_u32(done_bar));
+      else
+        umma_commit(done_bar);
+    }
     volatile int no_abort = 0;
     mbar_wait(done_bar, 0, &no_abort);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ zeros of a pair's second CTA
+    int stage = 0;
+    uint32_t cut_phase = 0;
+    for (int k = 0;; ++k) {
+      const RaggedTile t = ring_read(k, true);
+      if (t.kind == RT_END) break;
+      if (t.kind != RT_MMA) continue;
+      const int kblocks = (t.k_len + Cfg::BK - 1) / Cfg::BK;
+      const int last = (stage + kblocks - 1) % STAGES;
+      stage = (stage + kblocks) % STAGES;
+      if (!is_cut(t)) continue;
+      const bool ok = mbar_wait(&cut_full[last], (cut_phase >> last) & 1u, abort_flag);
+      cut_phase ^= 1u << last;
+      if (!__all_sync(0xFFFFFFFFu, ok)) break;
+      zero_tail(last, t.k_len - (kblocks - 1) * Cfg::BK);
+      if (lane == 0) mbar_arrive_release_cluster(mapa_shared(smem_u32(&cut_peer[last]), 0));
+    }
   } else if (warp == 2) {
-    // ------------------------------------------------------------------ scheduler
+    // ------------------------------------------------------------------ scheduler (a pair's CTAs find the same tiles)
     int pub = 0;
     auto publish = [&](const RaggedTile& t) -> bool {
       const int s = pub & (TRING - 1);
-      if (!mbar_wait(&tr_empty[s], ((uint32_t)(pub / TRING) & 1u) ^ 1u, abort_flag)) return false;
-      __syncwarp();
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait(&tr_empty[s], ((uint32_t)(pub / TRING) & 1u) ^ 1u, abort_flag))) return false;
       if (lane == 0) {
-        volatile int* e = ring + 8 * s;
+        volatile int* e = ring + Cfg::RING_INTS * s;
         e[0] = t.kind;
         e[1] = t.member;
         e[2] = t.row0;
@@ -310,28 +459,48 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE>::THREADS, 1)
         e[5] = t.k_len;
         e[6] = t.n_valid;
         e[7] = t.m_valid;
+        e[8] = t.part;
+        e[9] = t.add;
         mbar_arrive(&tr_full[s]);
       }
       ++pub;
       return true;
     };
     RaggedTile t;
+    t.part = t.add = 0;
     bool ok = true;
     if constexpr (MODE == RAGGED_WGRAD) {
-      const int per = pr.m_tiles * pr.n_tiles;
+      const int tiles = pr.m_tiles * pr.n_tiles, per = tiles * pr.splits;
       const long long total = (long long)pr.P * per;
-      for (long long i = blockIdx.x; ok && i < total; i += gridDim.x) {
+      for (long long i = worker; ok && i < total; i += workers) {
         t.member = (int)(i / per);
         const int r = (int)(i - (long long)t.member * per);
-        t.nt = r / pr.m_tiles;
-        t.row0 = (r - t.nt * pr.m_tiles) * Cfg::BM;
-        int end;
-        ragged_group(pr, t.member, t.rows, end);
-        t.k_len = end - t.rows;
+        t.part = r / tiles;
+        const int tile = r - t.part * tiles;
+        t.nt = tile / pr.m_tiles;
+        t.row0 = (tile - t.nt * pr.m_tiles) * Cfg::TILE_M;
+        int first, end;
+        ragged_group(pr, t.member, first, end);
+        const int share = ((end - first + pr.splits - 1) / pr.splits + 63) & ~63;
+        first = (int)min((long long)end, (long long)first + (long long)t.part * share);
+        end = min(end, first + share);
         t.m_valid = pr.in_f ? min(__ldg(pr.in_f + t.member), pr.in) : pr.in;
         t.n_valid = pr.out_f ? min(__ldg(pr.out_f + t.member), pr.out) : pr.out;
-        t.kind = (t.k_len > 0 && t.row0 < t.m_valid && t.nt * BN < t.n_valid) ? RT_MMA : RT_ZERO;
-        ok = publish(t);
+        if (end > first && t.row0 < t.m_valid && t.nt * BN < t.n_valid) {
+          t.kind = RT_MMA;
+          // pieces of about the same length: a short one would not hide the other's read and write of dw
+          const int pieces = (end - first + RAGGED_SEGMENT - 1) / RAGGED_SEGMENT;
+          const int piece = ((end - first + pieces - 1) / pieces + 63) & ~63;
+          for (int k = first; ok && k < end; k += piece) {
+            t.rows = k;
+            t.k_len = min(piece, end - k);
+            t.add = k > first;
+            ok = publish(t);
+          }
+        } else {
+          t.kind = RT_ZERO;
+          ok = publish(t);
+        }
       }
     } else {
       int g0 = 0;          // first group of the 32 that the lanes hold
@@ -340,7 +509,7 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE>::THREADS, 1)
       auto load_groups = [&]() {
         first = end = 0;
         if (g0 + lane < pr.P + 2) ragged_group(pr, g0 + lane, first, end);
-        tiles = (end - first + Cfg::BM - 1) / Cfg::BM * pr.n_tiles;
+        tiles = (end - first + Cfg::TILE_M - 1) / Cfg::TILE_M * pr.n_tiles;
         inc = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -349,7 +518,7 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE>::THREADS, 1)
         }
       };
       load_groups();
-      for (long long i = blockIdx.x; ok; i += gridDim.x) {
+      for (long long i = worker; ok; i += workers) {
         int sum = __shfl_sync(0xFFFFFFFFu, inc, 31);
         while (i >= before + sum && g0 + 32 < pr.P + 2) {
           before += sum;
@@ -362,11 +531,11 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE>::THREADS, 1)
         const int who = __ffs(__ballot_sync(0xFFFFFFFFu, local < inc)) - 1;
         const int r = local - __shfl_sync(0xFFFFFFFFu, inc - tiles, who);
         const int f = __shfl_sync(0xFFFFFFFFu, first, who), e = __shfl_sync(0xFFFFFFFFu, end, who);
-        const int mt = (e - f + Cfg::BM - 1) / Cfg::BM;
+        const int mt = (e - f + Cfg::TILE_M - 1) / Cfg::TILE_M;
         t.member = g0 + who;
         t.nt = r / mt;
-        t.row0 = f + (r - t.nt * mt) * Cfg::BM;
-        t.rows = min(Cfg::BM, e - t.row0);
+        t.row0 = f + (r - t.nt * mt) * Cfg::TILE_M;
+        t.rows = min(Cfg::TILE_M, e - t.row0);
         t.m_valid = t.rows;
         t.kind = RT_ZERO;
         t.k_len = t.n_valid = 0;
@@ -401,8 +570,8 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE>::THREADS, 1)
       const int cbase = t.nt * BN + half * WCOLS;
       if constexpr (MODE == RAGGED_WGRAD) {
         // lane = input feature, register = output feature: 32 consecutive floats of a row of dw per store
-        const int col = t.row0 + q * 32 + lane;
-        float* base = static_cast<float*>(pr.c) + (long long)t.member * pr.out * pr.in + col;
+        const int col = t.row0 + rank * Cfg::BM + q * 32 + lane;
+        float* base = static_cast<float*>(pr.c) + ((long long)t.part * pr.P + t.member) * pr.out * pr.in + col;
         const int nch = min(NCH, max(0, (pr.out - cbase + 31) / 32));
         const bool store = col < pr.in, valid = col < t.m_valid;
         if (t.kind == RT_MMA) {
@@ -414,11 +583,26 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE>::THREADS, 1)
             uint32_t v[32];
             tmem_ld_32x32b_x32(t_row + (uint32_t)(32 * c), v);
             tmem_wait_ld();
+            if (t.add) {
+              // on top of the sums over earlier rows, which this thread wrote; all loads before the stores
+              float had[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const int o = cbase + 32 * c + j;
-              if (store && o < pr.out)
-                base[(long long)o * pr.in] = (valid && o < t.n_valid) ? __uint_as_float(v[j]) : 0.f;
+              for (int j = 0; j < 32; ++j) {
+                const int o = cbase + 32 * c + j;
+                had[j] = (valid && o < t.n_valid) ? base[(long long)o * pr.in] : 0.f;
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const int o = cbase + 32 * c + j;
+                if (valid && o < t.n_valid) base[(long long)o * pr.in] = had[j] + __uint_as_float(v[j]);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const int o = cbase + 32 * c + j;
+                if (store && o < pr.out)
+                  base[(long long)o * pr.in] = (valid && o < t.n_valid) ? __uint_as_float(v[j]) : 0.f;
+              }
             }
           }
         } else if (store) {
@@ -429,8 +613,8 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE>::THREADS, 1)
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(pr.c);
         const int ld = MODE == RAGGED_FWD ? pr.out : pr.in;
         const int nch = min(NCH, max(0, (ld - cbase + 31) / 32));
-        const int rows = t.rows - q * 32;  // of this warp, may be below 1 or above 32
-        const long long row0 = (long long)t.row0 + q * 32;
+        const int rows = t.rows - rank * Cfg::BM - q * 32;  // of this warp, may be below 1 or above 32
+        const long long row0 = (long long)t.row0 + rank * Cfg::BM + q * 32;
         if (t.kind == RT_MMA) {
           const bool biased = MODE == RAGGED_FWD && pr.bias != nullptr;
           if constexpr (MODE == RAGGED_FWD) {
@@ -481,7 +665,12 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE>::THREADS, 1)
       if (t.kind == RT_MMA) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&tempty[acc]);
+        if (lane == 0) {
+          if constexpr (PAIR)
+            mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));  // the leader's MMA warp waits on it
+          else
+            mbar_arrive(&tempty[acc]);
+        }
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1u;
       }
@@ -490,8 +679,24 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE>::THREADS, 1)
 
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // neither CTA leaves while the other may still signal it
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  if (warp == 1) {
+    if constexpr (PAIR)
+      tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
+    else
+      tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+// dw = the sum of its parts, in their order.
+__global__ void __launch_bounds__(256) ragged_parts_kernel(const float* parts, float* dw, long long n, int count) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float s = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < count; ++k) s += __ldcs(parts + k * n + i);
+  dw[i] = s;
 }
 
 // ---------------------------------------------------------------------------

@@ -257,39 +257,99 @@ RaggedProblem ragged_problem(const tp_ragged_linear_args* a) {
   return p;
 }
 
-template <int BN, int MODE>
-int launch_ragged(RaggedProblem p, const CUtensorMap& ma, const CUtensorMap& mb, long long tiles, cudaStream_t st) {
-  using Cfg = RaggedCfg<BN, MODE>;
-  int rc = allow_smem<ragged_gemm_kernel<BN, MODE>>(Cfg::SMEM_BYTES);
+template <int BN, int MODE, bool PAIR>
+int launch_ragged(const RaggedProblem& p, const CUtensorMap& ma, const CUtensorMap& mb, long long tiles, cudaStream_t st) {
+  using Cfg = RaggedCfg<BN, MODE, PAIR>;
+  constexpr auto kern = ragged_gemm_kernel<BN, MODE, PAIR>;
+  int rc = allow_smem<kern>(Cfg::SMEM_BYTES);
   if (rc) return rc;
-  const int grid = (int)std::min<long long>(std::max<long long>(tiles, 1), device_info().sms);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.blockDim = dim3(Cfg::THREADS);
+  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+  cfg.stream = st;
+  int workers = device_info().sms;
+  if constexpr (PAIR) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    static std::atomic<int> pairs[64] = {};
+    int dev = 0;
+    TP_CUDA_TRY(cudaGetDevice(&dev));
+    int n = pairs[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+      cfg.gridDim = dim3(2 * (workers / 2));
+      TP_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+      if (n <= 0) return fail(TP_EUNSUPPORTED, "no CTA pair of this kernel fits on the device");
+      pairs[dev].store(n, std::memory_order_relaxed);
+    }
+    workers = n;
+  }
+  const int grid = (int)std::min<long long>(std::max<long long>(tiles, 1), workers);
+  cfg.gridDim = dim3(PAIR ? 2 * grid : grid);
   TP_PROF(MODE == RAGGED_FWD ? TP_PROF_FWD : MODE == RAGGED_DGRAD ? TP_PROF_DGRAD : TP_PROF_WGRAD, st);
-  ragged_gemm_kernel<BN, MODE><<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(ma, mb, p);
-  TP_CUDA_TRY(cudaGetLastError());
+  TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, ma, mb, p));
   return TP_OK;
+}
+
+// How a product is cut into tiles, from its sizes alone.
+struct RaggedPlan {
+  bool pair;
+  int bn, tile_m, splits;
+};
+
+RaggedPlan ragged_plan(int mode, int P, int64_t R, int in, int out) {
+  RaggedPlan plan{false, 256, 128, 1};
+  const int cols = mode == RAGGED_DGRAD ? in : out;
+  const long long used = std::min<long long>(P, R);
+  const int sms = 148;
+  // Pairs where their 256-row tiles are mostly full and there is at least one for each pair of SMs: members of 1024
+  // rows on average (wgrad: input widths), since a member's last tile is half empty on average.
+  const long long rows = mode == RAGGED_WGRAD ? in : R / P;
+  const long long pair_tiles = (mode == RAGGED_WGRAD ? (long long)P * ((in + 255) / 256) : R / 256) * ((cols + 255) / 256);
+  if (rows >= 1024 && pair_tiles >= sms / 2) {
+    plan.pair = true;
+    plan.tile_m = 256;
+    return plan;
+  }
+  // tiles along the rows: every member that has rows ends in a partial one
+  const long long m_tiles = mode == RAGGED_WGRAD ? (long long)P * ((in + 127) / 128) : std::max(used, R / 128 + used / 2);
+  // the widest tile that still gives every SM one
+  while (plan.bn > 64 && m_tiles * ((cols + plan.bn - 1) / plan.bn) < sms) plan.bn /= 2;
+  if (mode == RAGGED_WGRAD) {
+    // parts of 512 rows at least, as many as the SMs take at once, 256 MB of results at most
+    const long long tiles = m_tiles * ((cols + plan.bn - 1) / plan.bn);
+    const long long most = std::max(1ll, (256ll << 20) / std::max(1ll, 4ll * P * in * out));
+    plan.splits = (int)std::max(1ll, std::min({sms / tiles, (long long)R / P / 512, most, 64ll}));
+  }
+  return plan;
 }
 
 // bf16 operands: A and B with their row strides.
 template <int MODE>
-int ragged_bf16(RaggedProblem p, const void* a_ptr, long long a_ld, const void* b_ptr, long long b_ld, cudaStream_t st) {
+int ragged_bf16(RaggedProblem p, const void* a_ptr, long long a_ld, const void* b_ptr, long long b_ld, float* parts,
+                cudaStream_t st) {
   const int cols = MODE == RAGGED_DGRAD ? p.in : p.out;  // columns of the result
-  // tiles along the rows: every member that has rows ends in a partial one
-  const long long m_tiles = MODE == RAGGED_WGRAD ? (long long)p.P * ((p.in + 127) / 128)
-                                                 : std::max<long long>(std::min(p.P, p.R), p.R / 128 + std::min(p.P, p.R) / 2);
-  // the widest tile that still gives every SM one
-  int bn = 256;
-  while (bn > 64 && m_tiles * ((cols + bn - 1) / bn) < device_info().sms) bn /= 2;
+  const RaggedPlan plan = ragged_plan(MODE, p.P, p.R, p.in, p.out);
+  const int bn = plan.bn, tm = plan.tile_m;
   p.n_tiles = (cols + bn - 1) / bn;
-  p.m_tiles = (p.in + 127) / 128;
+  p.m_tiles = (p.in + tm - 1) / tm;
+  p.splits = plan.splits;
   p.c_vec = aligned16(p.c) && cols % 8 == 0;
-  const long long most = MODE == RAGGED_WGRAD ? m_tiles * p.n_tiles : ((long long)p.R / 128 + p.P + 2) * p.n_tiles;
+  void* result = p.c;
+  if (MODE == RAGGED_WGRAD && plan.splits > 1) p.c = parts;
+  const long long most = MODE == RAGGED_WGRAD ? (long long)p.P * p.m_tiles * p.n_tiles * p.splits
+                                              : ((long long)p.R / tm + p.P + 2) * p.n_tiles;
   if (most > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many tiles");
   const auto T = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap ma, mb;
   int rc;
   if (MODE == RAGGED_FWD) {
     rc = make_map_ld(&ma, T, 2, a_ptr, p.in, p.R, 1, a_ld, 64, 128);
-    if (!rc) rc = make_map_ld(&mb, T, 2, b_ptr, p.in, p.out, p.P, b_ld, 64, bn);
+    if (!rc) rc = make_map_ld(&mb, T, 2, b_ptr, p.in, p.out, p.P, b_ld, 64, plan.pair ? bn / 2 : bn);
   } else if (MODE == RAGGED_DGRAD) {
     rc = make_map_ld(&ma, T, 2, a_ptr, p.out, p.R, 1, a_ld, 64, 128);
     if (!rc) rc = make_map_ld(&mb, T, 2, b_ptr, p.in, p.out, p.P, b_ld, 64, 64);
@@ -298,11 +358,21 @@ int ragged_bf16(RaggedProblem p, const void* a_ptr, long long a_ld, const void* 
     if (!rc) rc = make_map_ld(&mb, T, 2, b_ptr, p.out, p.R, 1, b_ld, 64, 64);
   }
   if (rc) return rc;
-  switch (bn) {
-    case 256: return launch_ragged<256, MODE>(p, ma, mb, most, st);
-    case 128: return launch_ragged<128, MODE>(p, ma, mb, most, st);
-    default: return launch_ragged<64, MODE>(p, ma, mb, most, st);
+  if (plan.pair)
+    rc = launch_ragged<256, MODE, true>(p, ma, mb, most, st);
+  else if (bn == 256)
+    rc = launch_ragged<256, MODE, false>(p, ma, mb, most, st);
+  else if (bn == 128)
+    rc = launch_ragged<128, MODE, false>(p, ma, mb, most, st);
+  else
+    rc = launch_ragged<64, MODE, false>(p, ma, mb, most, st);
+  if (rc) return rc;
+  if (MODE == RAGGED_WGRAD && plan.splits > 1) {
+    const long long n = (long long)p.P * p.out * p.in;
+    ragged_parts_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(parts, static_cast<float*>(result), n, plan.splits);
+    TP_CUDA_TRY(cudaGetLastError());
   }
+  return TP_OK;
 }
 
 template <int MODE>
@@ -332,6 +402,22 @@ long long ragged_g_stride(const tp_ragged_linear_args* a) {
   return 0;
 }
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// The backward's workspace: g, the shares' sums of g, the parts of dw.
+struct RaggedSpace {
+  size_t shares, parts, parts_bytes;
+};
+RaggedSpace ragged_space(const tp_ragged_linear_args* a) {
+  RaggedSpace s{};
+  s.shares = round256((size_t)a->rows * (size_t)ragged_g_stride(a) * dtype_size(a->dtype));
+  s.parts = s.shares;
+  if (a->dbias && ragged_shares(a) > 1) s.parts += round256((size_t)ragged_shares(a) * a->P * a->max_out * sizeof(float));
+  if (a->dw && a->dtype == TP_DTYPE_BF16) {
+    const int splits = ragged_plan(RAGGED_WGRAD, a->P, a->rows, a->max_in, a->max_out).splits;
+    if (splits > 1) s.parts_bytes = (size_t)splits * a->P * a->max_out * a->max_in * sizeof(float);
+  }
+  return s;
+}
 
 // ------------------------------------------------------------------ 4-bit rows
 
@@ -493,9 +579,8 @@ int tp_combine_rows_backward(const tp_rows_args* a, void* stream) {
 
 size_t tp_ragged_linear_workspace_size(const tp_ragged_linear_args* a) {
   if (!a || a->P <= 0 || a->max_out <= 0 || a->rows <= 0) return 0;
-  size_t n = round256((size_t)a->rows * (size_t)ragged_g_stride(a) * dtype_size(a->dtype));
-  if (a->dbias && ragged_shares(a) > 1) n += (size_t)ragged_shares(a) * a->P * a->max_out * sizeof(float);
-  return n;
+  const RaggedSpace s = ragged_space(a);
+  return s.parts + s.parts_bytes;
 }
 
 int tp_ragged_linear_forward(const tp_ragged_linear_args* a, void* stream) {
@@ -507,7 +592,7 @@ int tp_ragged_linear_forward(const tp_ragged_linear_args* a, void* stream) {
   p.bias = a->bias;
   p.relu = a->relu;
   p.c = a->y;
-  if (a->dtype == TP_DTYPE_BF16) return ragged_bf16<RAGGED_FWD>(p, a->x, a->x_stride, a->w, a->w_stride, st);
+  if (a->dtype == TP_DTYPE_BF16) return ragged_bf16<RAGGED_FWD>(p, a->x, a->x_stride, a->w, a->w_stride, nullptr, st);
   return ragged_f32<RAGGED_FWD>(p, a->x, a->x_stride, a->w, a->w_stride, st);
 }
 
@@ -522,6 +607,8 @@ int tp_ragged_linear_backward(const tp_ragged_linear_args* a, void* stream) {
     return fail(TP_EINVAL, "ragged linear workspace of %zu bytes is smaller than the %zu needed, or not aligned",
                 a->workspace_bytes, need);
   const bool bf16 = a->dtype == TP_DTYPE_BF16;
+  const RaggedSpace space = ragged_space(a);
+  float* parts = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + space.parts);
   const long long g_ld = ragged_g_stride(a);
   const void* g = g_ld ? a->workspace : a->dy;
   const long long ld = g_ld ? g_ld : a->dy_stride;
@@ -539,8 +626,7 @@ int tp_ragged_linear_backward(const tp_ragged_linear_args* a, void* stream) {
     k.g = g_ld ? a->workspace : nullptr;
     k.g_ld = g_ld;
     k.db = a->dbias;
-    k.partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) +
-                                         round256((size_t)a->rows * (size_t)g_ld * dtype_size(a->dtype)));
+    k.partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + space.shares);
     TP_PROF(TP_PROF_ACT_BACKWARD, st);
     const dim3 grid((a->max_out + 63) / 64, a->P, k.S);
     if (bf16)
@@ -554,13 +640,13 @@ int tp_ragged_linear_backward(const tp_ragged_linear_args* a, void* stream) {
   RaggedProblem p = ragged_problem(a);
   if (a->dx) {
     p.c = a->dx;
-    rc = bf16 ? ragged_bf16<RAGGED_DGRAD>(p, g, ld, a->w, a->w_stride, st)
+    rc = bf16 ? ragged_bf16<RAGGED_DGRAD>(p, g, ld, a->w, a->w_stride, nullptr, st)
               : ragged_f32<RAGGED_DGRAD>(p, g, ld, a->w, a->w_stride, st);
     if (rc) return rc;
   }
   if (a->dw) {
     p.c = a->dw;
-    rc = bf16 ? ragged_bf16<RAGGED_WGRAD>(p, a->x, a->x_stride, g, ld, st)
+    rc = bf16 ? ragged_bf16<RAGGED_WGRAD>(p, a->x, a->x_stride, g, ld, parts, st)
               : ragged_f32<RAGGED_WGRAD>(p, a->x, a->x_stride, g, ld, st);
     if (rc) return rc;
   }
