@@ -823,7 +823,7 @@ __global__ void __launch_bounds__(256) ragged_simt_kernel(const RaggedSimt s) {
 
 // ---------------------------------------------------------------------------
 // g = dy [y > 0] with rows at g_ld (a multiple of 8 columns: an operand of the products), and the members' sums of
-// g over their rows.  A block takes 64 columns of a member's share of rows; the shares' sums are added up in order
+// g over their rows.  A block takes 64 or 256 columns of a member's share of rows; the shares' sums are added up in order
 // by a second launch.  Memory: dy and y are read once, g is written once.
 // ---------------------------------------------------------------------------
 struct RaggedAct {
@@ -839,11 +839,37 @@ struct RaggedAct {
   float* partial;  // (S, P, N) where S > 1
 };
 
-template <typename T>
+// Eight columns of a row as they lie in memory, zeros from column n on.
+template <typename T, bool VEC>
+struct Act8 {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p, int c0, int n) {
+    if (VEC) {  // (rows on 16-byte boundaries, n a multiple of 8)
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p + c0) + i);
+    } else {
+      T v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c0 + j < n ? p[c0 + j] : (T)0.f;
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(v)[i];
+    }
+  }
+  __device__ __forceinline__ float get(int j) const {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(u);
+    if (sizeof(T) == 4) return __uint_as_float(w[j]);
+    return __uint_as_float((j & 1) ? (w[j >> 1] & 0xFFFF0000u) : (w[j >> 1] << 16));
+  }
+};
+
+// VEC: dy and y have rows on 16-byte boundaries and N is a multiple of 8.  C threads side by side take 8 C columns.
+template <typename T, bool VEC, int C, bool RELU>
 __global__ void __launch_bounds__(256) ragged_act_kernel(const RaggedAct a) {
-  __shared__ float red[32][65];
-  const int m = blockIdx.y, cg = threadIdx.x & 7, rl = threadIdx.x >> 3;
-  const int c0 = blockIdx.x * 64 + cg * 8;
+  constexpr int U = (RELU ? 4 : 8) * 2 / (int)sizeof(T);  // rows of a thread on their way
+  constexpr int ROWS = 256 / C;                           // rows side by side
+  __shared__ float red[ROWS][8 * C + 1];
+  const int m = blockIdx.y, cg = threadIdx.x % C, rl = threadIdx.x / C;
+  const int c0 = blockIdx.x * 8 * C + cg * 8;
   RaggedProblem p{};
   p.P = a.P;
   p.R = a.R;
@@ -851,24 +877,44 @@ __global__ void __launch_bounds__(256) ragged_act_kernel(const RaggedAct a) {
   int first, end;
   ragged_group(p, m, first, end);
   const int per = (end - first + a.S - 1) / a.S;
-  const int r0 = first + min(end - first, (int)blockIdx.z * per), r1 = min(end, r0 + per);
+  const int r0 = (int)min((long long)end, first + (long long)blockIdx.z * per), r1 = min(end, r0 + per);
   const int out_m = a.out_f ? min(a.out_f[m], a.N) : a.N;
   const T* dy = static_cast<const T*>(a.dy);
   const T* y = static_cast<const T*>(a.y);
   T* g = static_cast<T*>(a.g);
   float sum[8] = {};
-  for (int r = r0 + rl; r < r1; r += 32) {
+  if (c0 < a.N || (g != nullptr && c0 < a.g_ld)) {
+    for (int r = r0 + rl; r < r1; r += ROWS * U) {
+      Act8<T, VEC> d[U], s[RELU ? U : 1];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = c0 + j;
-      if (c < a.N) {
-        T v = dy[(long long)r * a.dy_ld + c];
-        if (y != nullptr && !((float)y[(long long)r * a.N + c] > 0.f)) v = (T)0.f;
-        if (c >= out_m) v = (T)0.f;
-        if (g != nullptr) g[(long long)r * a.g_ld + c] = v;
-        sum[j] += (float)v;
-      } else if (g != nullptr && c < a.g_ld) {
-        g[(long long)r * a.g_ld + c] = (T)0.f;
+      for (int u = 0; u < U; ++u)
+        if (r + ROWS * u < r1) {
+          d[u].load(dy + (long long)(r + ROWS * u) * a.dy_ld, c0, a.N);
+          if constexpr (RELU) s[u].load(y + (long long)(r + ROWS * u) * a.N, c0, a.N);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (r + ROWS * u < r1) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            v[j] = d[u].get(j);
+            if constexpr (RELU) v[j] = s[u].get(j) > 0.f ? v[j] : 0.f;
+            if (c0 + j >= out_m) v[j] = 0.f;
+            sum[j] += v[j];
+          }
+          if (g != nullptr) {
+            T* to = g + (long long)(r + ROWS * u) * a.g_ld + c0;
+            if (sizeof(T) == 2) {  // (rows of g are multiples of 8)
+              *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                         pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (c0 + j < a.g_ld) to[j] = (T)v[j];
+            }
+          }
+        }
       }
     }
   }
@@ -876,12 +922,12 @@ __global__ void __launch_bounds__(256) ragged_act_kernel(const RaggedAct a) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) red[rl][cg * 8 + j] = sum[j];
   __syncthreads();
-  if (threadIdx.x < 64) {
-    const int c = blockIdx.x * 64 + threadIdx.x;
+  if (threadIdx.x < 8 * C) {
+    const int c = blockIdx.x * 8 * C + threadIdx.x;
     if (c < a.N) {
       float s = 0.f;
 #pragma unroll
-      for (int r = 0; r < 32; ++r) s += red[r][threadIdx.x];
+      for (int r = 0; r < ROWS; ++r) s += red[r][threadIdx.x];
       (a.S > 1 ? a.partial + (long long)blockIdx.z * a.P * a.N : a.db)[(long long)m * a.N + c] = s;
     }
   }

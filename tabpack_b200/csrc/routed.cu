@@ -34,14 +34,17 @@ int allow_smem(size_t bytes) {
 
 // ------------------------------------------------------------------ routing
 
-// Rows of a block: few rows go to one block, many to at most two blocks an SM.
-int route_rows_per_block(int64_t rows, int32_t k) {
-  if (rows * k <= 1024) return (int)std::max<int64_t>(rows, 1);
-  return (int)std::max<int64_t>(64, (rows + 147) / 148);
-}
-int route_blocks(int64_t rows, int32_t k) {
-  const int per = route_rows_per_block(rows, k);
-  return (int)((rows + per - 1) / per);
+// Gate blocks: one where there are few rows, else up to four an SM (two run at a time; a warp's rows are a chain of
+// reductions).  A place block takes the rows of `gates` of them.
+struct RoutePlan {
+  int rows, blocks, gates;
+};
+RoutePlan route_plan(int64_t rows, int32_t k) {
+  RoutePlan p{};
+  p.rows = rows * k <= 1024 ? (int)std::max<int64_t>(rows, 1) : (int)std::max<int64_t>(16, (rows + 4 * 148 - 1) / (4 * 148));
+  p.blocks = (int)((rows + p.rows - 1) / p.rows);
+  p.gates = std::max(1, p.blocks / 148);
+  return p;
 }
 
 int check_route(const tp_route_args* a) {
@@ -72,7 +75,10 @@ RouteArgs route_args(const tp_route_args* a) {
   k.position = a->position;
   k.offsets = a->offsets;
   k.importance = a->importance;
-  k.rows_per_block = route_rows_per_block(a->rows, a->top_k);
+  const RoutePlan plan = route_plan(a->rows, a->top_k);
+  k.rows_per_block = plan.rows;
+  k.blocks = plan.blocks;
+  k.gates = plan.gates;
   k.g_weight = a->g_weight;
   k.g_importance = a->g_importance;
   k.dlogits = a->dlogits;
@@ -81,7 +87,7 @@ RouteArgs route_args(const tp_route_args* a) {
 
 template <typename T, int V>
 int launch_route(const RouteArgs& k, cudaStream_t st) {
-  const int blocks = (k.rows + k.rows_per_block - 1) / k.rows_per_block;
+  const int blocks = k.blocks;
   const size_t smem = route_shared_bytes(k.E);
   if (blocks == 1) {
     int rc = allow_smem<route_small_kernel<T, V>>(smem);
@@ -92,14 +98,15 @@ int launch_route(const RouteArgs& k, cudaStream_t st) {
     if (!rc) rc = allow_smem<route_place_kernel>(smem);
     if (rc) return rc;
     route_gate_kernel<T, V><<<blocks, 32 * ROUTE_WARPS, smem, st>>>(k);
-    route_place_kernel<<<blocks, 32 * ROUTE_WARPS, smem, st>>>(k);
+    route_scan_kernel<<<k.E + 1, 256, 0, st>>>(k);
+    route_place_kernel<<<(blocks + k.gates - 1) / k.gates, 32 * ROUTE_WARPS, smem, st>>>(k);
   }
   return TP_OK;
 }
 
 template <typename T, int V>
 int launch_route_backward(const RouteArgs& k, cudaStream_t st) {
-  route_backward_kernel<T, V><<<(k.rows + 7) / 8, 256, 0, st>>>(k);
+  route_backward_kernel<T, V><<<std::min((k.rows + 7) / 8, 8 * device_info().sms), 256, 0, st>>>(k);
   return TP_OK;
 }
 
@@ -388,9 +395,11 @@ int ragged_f32(RaggedProblem p, const void* a_ptr, long long a_ld, const void* b
   return TP_OK;
 }
 
+// Columns of a block of the activation gradient: long pieces of each row where that leaves blocks enough.
+int ragged_strip(const tp_ragged_linear_args* a) { return a->rows * a->max_out >= (4ll << 20) && a->max_out >= 256 ? 256 : 64; }
 // Shares of a member's rows in the bias gradient: about eight blocks an SM, 64 rows each at least.
 int ragged_shares(const tp_ragged_linear_args* a) {
-  const long long strips = (a->max_out + 63) / 64;
+  const long long strips = (a->max_out + ragged_strip(a) - 1) / ragged_strip(a);
   const long long want = 8ll * 148 / std::max(1ll, strips * a->P), most = a->rows / ((long long)a->P * 64);
   return (int)std::max(1ll, std::min({want, most, 64ll}));
 }
@@ -401,6 +410,21 @@ long long ragged_g_stride(const tp_ragged_linear_args* a) {
   if (a->dtype == TP_DTYPE_BF16 && (a->dy_stride % 8 || !aligned16(a->dy))) return (a->max_out + 7ll) / 8 * 8;
   return 0;
 }
+template <typename T, bool VEC, int C>
+void launch_act_relu(const RaggedAct& k, dim3 grid, cudaStream_t st) {
+  if (k.y)
+    ragged_act_kernel<T, VEC, C, true><<<grid, 256, 0, st>>>(k);
+  else
+    ragged_act_kernel<T, VEC, C, false><<<grid, 256, 0, st>>>(k);
+}
+template <typename T>
+void launch_act(const RaggedAct& k, bool vec, bool wide, dim3 grid, cudaStream_t st) {
+  if (vec)
+    wide ? launch_act_relu<T, true, 32>(k, grid, st) : launch_act_relu<T, true, 8>(k, grid, st);
+  else
+    wide ? launch_act_relu<T, false, 32>(k, grid, st) : launch_act_relu<T, false, 8>(k, grid, st);
+}
+
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // The backward's workspace: g, the shares' sums of g, the parts of dw.
@@ -512,7 +536,7 @@ extern "C" {
 
 size_t tp_route_workspace_size(int64_t rows, int32_t E, int32_t top_k) {
   if (rows <= 0 || E <= 0 || top_k <= 0) return 0;
-  return (size_t)route_blocks(rows, top_k) * (2 * (size_t)E + 1) * 4;
+  return ((size_t)route_plan(rows, top_k).blocks * (2 * (size_t)E + 1) + E + 1) * 4;
 }
 
 int tp_route_forward(const tp_route_args* a, void* stream) {
@@ -526,7 +550,8 @@ int tp_route_forward(const tp_route_args* a, void* stream) {
     return fail(TP_EINVAL, "routing workspace of %zu bytes is smaller than the %zu needed", a->workspace_bytes, need);
   RouteArgs k = route_args(a);
   k.counts = static_cast<int32_t*>(a->workspace);
-  k.partial = reinterpret_cast<float*>(k.counts + (size_t)route_blocks(a->rows, a->top_k) * (a->E + 1));
+  k.partial = reinterpret_cast<float*>(k.counts + (size_t)k.blocks * (a->E + 1));
+  k.totals = k.counts + (size_t)k.blocks * (2 * (size_t)a->E + 1);
   rc = a->dtype == TP_DTYPE_BF16 ? dispatch_route<__nv_bfloat16>(k, false, st) : dispatch_route<float>(k, false, st);
   if (rc) return rc;
   TP_CUDA_TRY(cudaGetLastError());
@@ -628,11 +653,14 @@ int tp_ragged_linear_backward(const tp_ragged_linear_args* a, void* stream) {
     k.db = a->dbias;
     k.partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + space.shares);
     TP_PROF(TP_PROF_ACT_BACKWARD, st);
-    const dim3 grid((a->max_out + 63) / 64, a->P, k.S);
+    const bool wide = ragged_strip(a) == 256;
+    const dim3 grid((a->max_out + ragged_strip(a) - 1) / ragged_strip(a), a->P, k.S);
+    const size_t size = dtype_size(a->dtype);
+    const bool vec = a->max_out % 8 == 0 && aligned16(a->dy) && aligned16(k.y) && a->dy_stride * size % 16 == 0;
     if (bf16)
-      ragged_act_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(k);
+      launch_act<__nv_bfloat16>(k, vec, wide, grid, st);
     else
-      ragged_act_kernel<float><<<grid, 256, 0, st>>>(k);
+      launch_act<float>(k, vec, wide, grid, st);
     if (a->dbias && k.S > 1)
       ragged_bias_kernel<<<(unsigned)(((long long)a->P * a->max_out + 255) / 256), 256, 0, st>>>(k);
     TP_CUDA_TRY(cudaGetLastError());

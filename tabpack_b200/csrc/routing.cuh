@@ -26,115 +26,138 @@ struct RouteArgs {
   int32_t* position;      // (rows, k)
   int32_t* offsets;       // (E + 1)
   float* importance;      // (E)
-  int32_t* counts;        // workspace (blocks, E + 1)
-  float* partial;         // workspace (blocks, E): sums of p over a block's rows
-  int rows_per_block;
+  int32_t* counts;        // workspace (E + 1, blocks): pairs of a gate block with each member
+  float* partial;         // workspace (E, blocks): sums of p over a block's rows
+  int32_t* totals;        // workspace (E + 1)
+  int rows_per_block;     // of a gate block
+  int blocks, gates;      // gate blocks, and how many of them a place block takes
   const float* g_weight;      // backward, (rows, k) or null
   const float* g_importance;  // (E) or null
   void* dlogits;              // (rows, E)
 };
-
-// fp32 as an unsigned number of the same order; every NaN above +inf.
-__device__ __forceinline__ uint32_t order_key(float x) {
-  const uint32_t u = __float_as_uint(x);
-  if (x != x) return 0xFFFFFFFFu;
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
-__device__ __forceinline__ float key_value(uint32_t k) {
-  if (k == 0xFFFFFFFFu) return __uint_as_float(0x7FC00000u);
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
-}
-constexpr uint32_t KEY_NEG_INF = 0x007FFFFFu;  // the key of -inf; smaller ones are of no score
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   return v;
 }
+// The warp's largest value (no NaN among them).
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
 
-// A row's scores as keys, lane l holding members l, l + 32, ...; 0 past the last member.
+// A row's scores, lane l holding members l, l + 32, ...; -inf past the last member.
 template <typename T, int V>
-__device__ __forceinline__ void route_load(const T* z, int E, int lane, uint32_t (&key)[V]) {
+__device__ __forceinline__ void route_load(const T* z, int E, int lane, float (&v)[V]) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = lane + 32 * v;
-    key[v] = e < E ? order_key((float)z[e]) : 0u;
-  }
+  for (int i = 0; i < V; ++i) v[i] = lane + 32 * i < E ? (float)z[lane + 32 * i] : -INFINITY;
 }
 
-// Shared memory of both phases: counts[ROUTE_WARPS][E + 1], then base[E + 1], then sums[ROUTE_WARPS][E].
-__host__ __device__ inline size_t route_shared_bytes(int E) {
-  return sizeof(int) * ((size_t)(ROUTE_WARPS + 1) * (E + 1) + (size_t)ROUTE_WARPS * E);
+constexpr float LOG2E = 1.4426950408889634f;
+// exp(z - m) with c = -m log2(e): the rounding of c is one factor of all of a row's terms.
+__device__ __forceinline__ float exp_of(float z, float c) {
+  float r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(fmaf(z, LOG2E, c)));
+  return r;
 }
 
-// Weights and members of the block's rows, their counts per member, and the sums of p.
+// Shared memory of the gate: hist[E + 1], sums[ROUTE_WARPS][E]; of the places: counts[ROUTE_WARPS][E + 1], base[E + 1].
+__host__ __device__ inline size_t route_shared_bytes(int E) { return sizeof(int) * ((size_t)(ROUTE_WARPS + 1) * (E + 1)); }
+
+// Weights and members of the block's rows, their counts per member, and the sums of p.  Instructions bound it, some
+// 300 a row for 257 members and 6 slots: each lane finds its two best at once, so that a slot costs two reductions and
+// a search through the lane's scores only where one lane has three of a row's best.
 template <typename T, int V>
 __device__ __forceinline__ void route_gate(const RouteArgs& a, int block, int* smem) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int E = a.E, k = a.k;
-  int* hist = smem + ROUTE_WARPS * (E + 1);
+  int* hist = smem;
   float* sums = reinterpret_cast<float*>(hist + E + 1);
   for (int e = threadIdx.x; e <= E; e += blockDim.x) hist[e] = 0;
   __syncthreads();
   const int r0 = block * a.rows_per_block, r1 = min(a.rows, r0 + a.rows_per_block);
-  float imp[V];
+  const T* logits = static_cast<const T*>(a.logits);
+  float imp[V], next[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) imp[v] = 0.f;
+  if (r0 + warp < r1) route_load<T, V>(logits + (long long)(r0 + warp) * a.ld, E, lane, next);
   for (int r = r0 + warp; r < r1; r += ROUTE_WARPS) {
-    uint32_t key[V];
-    route_load<T, V>(static_cast<const T*>(a.logits) + (long long)r * a.ld, E, lane, key);
-    // this lane's best and its member: the lowest of equal ones
-    uint32_t best = 0;
-    int which = 0;
+    float z[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (key[v] > best) {
-        best = key[v];
-        which = lane + 32 * v;
+    for (int v = 0; v < V; ++v) z[v] = next[v];
+    if (r + ROUTE_WARPS < r1) route_load<T, V>(logits + (long long)(r + ROUTE_WARPS) * a.ld, E, lane, next);
+    // this lane's two best, b1 and b2, and which they are (equal ones: the lower first; a NaN is never greater)
+    float b1, b2;
+    int w1, w2;
+    auto two_best = [&]() {
+      b1 = b2 = -INFINITY;
+      w1 = w2 = 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const bool first = z[v] > b1, second = z[v] > b2;
+        b2 = first ? b1 : second ? z[v] : b2;
+        w2 = first ? w1 : second ? v : w2;
+        b1 = first ? z[v] : b1;
+        w1 = first ? v : w1;
       }
-    const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
-    const bool some = top > KEY_NEG_INF;
-    const float zmax = some ? key_value(top) : 0.f;
+    };
+    two_best();
+    float top = warp_max(b1);
+    float c = top > -INFINITY ? -top * LOG2E : 0.f;
     float e[V], total = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      e[v] = key[v] > KEY_NEG_INF ? expf(key_value(key[v]) - zmax) : 0.f;
+      e[v] = exp_of(z[v], c);  // 0 for -inf
       total += e[v];
     }
     total = warp_sum(total);
-    const float inv = some ? 1.f / total : 0.f;
+    if (total != total) {
+      // a NaN or +inf: all weights are NaN, and a NaN ranks as +inf
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (z[v] != z[v]) z[v] = INFINITY;
+      two_best();
+      top = warp_max(b1);
+    }
+    const float inv = top > -INFINITY ? 1.f / total : 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) imp[v] = fmaf(e[v], inv, imp[v]);
     // the k best: lane j keeps slot j
-    uint32_t my_key = 0;
-    int my_expert = -1;
+    float mine = 0.f, best = b1;
+    int my_expert = -1, which = lane + 32 * w1;
+    bool spare = true;  // b2 is the next one
     for (int j = 0; j < k; ++j) {
-      const uint32_t b = j == 0 ? top : __reduce_max_sync(0xFFFFFFFFu, best);
-      if (b <= KEY_NEG_INF) break;
+      const float b = j == 0 ? top : warp_max(best);
+      if (b == -INFINITY) break;
       const int who = (int)__reduce_min_sync(0xFFFFFFFFu, best == b ? (unsigned)which : 0xFFFFFFFFu);
       if (lane == j) {
-        my_key = b;
+        mine = b;
         my_expert = who;
       }
-      if (which == who && best == b) {  // this lane's next best
-        best = 0;
+      if (which == who && best == b) {
+        if (spare) {
+          best = b2;
+          which = lane + 32 * w2;
+          spare = false;
+        } else {
+          // the best one behind (b, who)
+          best = -INFINITY;
+          int w = 0;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          if (lane + 32 * v == who) key[v] = 0;
-          if (key[v] > best) {
-            best = key[v];
-            which = lane + 32 * v;
-          }
+          for (int v = 0; v < V; ++v)
+            if ((z[v] < b || (z[v] == b && lane + 32 * v > who)) && z[v] > best) {
+              best = z[v];
+              w = v;
+            }
+          which = lane + 32 * w;
         }
       }
     }
-    float w = my_expert >= 0 ? expf(key_value(my_key) - zmax) : 0.f;
-    if (a.renorm) {
-      const float s = warp_sum(w);
-      w = my_expert >= 0 ? w / s : 0.f;
-    } else {
-      w = my_expert >= 0 ? w / total : 0.f;
-    }
+    float w = my_expert >= 0 ? exp_of(mine, c) : 0.f;
+    const float of = a.renorm ? warp_sum(w) : total;
+    if (my_expert >= 0) w = total == total ? w / of : total;
     if (lane < k) {
       a.weight[(long long)r * k + lane] = w;
       a.expert[(long long)r * k + lane] = my_expert;
@@ -146,37 +169,69 @@ __device__ __forceinline__ void route_gate(const RouteArgs& a, int block, int* s
     if (lane + 32 * v < E) sums[warp * E + lane + 32 * v] = imp[v];
   __syncthreads();
   for (int e = threadIdx.x; e <= E; e += blockDim.x) {
-    a.counts[(long long)block * (E + 1) + e] = hist[e];
+    a.counts[(long long)e * a.blocks + block] = hist[e];
     if (e < E) {
       float s = 0.f;
       for (int w = 0; w < ROUTE_WARPS; ++w) s += sums[w * E + e];
-      a.partial[(long long)block * E + e] = s;
+      a.partial[(long long)e * a.blocks + block] = s;
     }
   }
 }
 
-// Places of the block's pairs, and the block's share of the offsets and sums.
-__device__ __forceinline__ void route_place(const RouteArgs& a, int block, int blocks, int* smem) {
+// Per member, by one block: how many pairs earlier gate blocks have (in place of each one's count), how many there are,
+// and the sum of p.
+__global__ void __launch_bounds__(256) route_scan_kernel(const RouteArgs a) {
+  __shared__ int counts[8];
+  __shared__ float sums[8];
+  const int e = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int32_t* c = a.counts + (long long)e * a.blocks;
+  const int per = (a.blocks + 255) / 256, b0 = threadIdx.x * per, b1 = min(a.blocks, b0 + per);
+  int n = 0;
+  float s = 0.f;
+  for (int b = b0; b < b1; ++b) {
+    n += c[b];
+    if (e < a.E) s += a.partial[(long long)e * a.blocks + b];
+  }
+  int inc = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+    if (lane >= o) inc += t;
+  }
+  s = warp_sum(s);
+  if (lane == 31) {
+    counts[warp] = inc;
+    sums[warp] = s;
+  }
+  __syncthreads();
+  int run = inc - n;
+  for (int w = 0; w < warp; ++w) run += counts[w];
+  for (int b = b0; b < b1; ++b) {
+    const int t = c[b];
+    c[b] = run;
+    run += t;
+  }
+  if (threadIdx.x == 255) {
+    a.totals[e] = run;
+    float all = 0.f;
+    for (int w = 0; w < 8; ++w) all += sums[w];
+    if (e < a.E) a.importance[e] = all;
+  }
+}
+
+// Places of the pairs of a.gates gate blocks from the first one, `gate`, on.
+__device__ __forceinline__ void route_place(const RouteArgs& a, int gate, int* smem) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int E = a.E;
-  int* cnt = smem;                             // [warp][E + 1]
-  int* base = smem + ROUTE_WARPS * (E + 1);    // [E + 1]
-  __shared__ int carry[33];
-  // counts of earlier blocks and of all of them, per member; then where the member's rows begin
-  if (threadIdx.x < 33) carry[threadIdx.x] = 0;
-  __syncthreads();
+  int* cnt = smem;                           // [warp][E + 1]
+  int* base = smem + ROUTE_WARPS * (E + 1);  // [E + 1]
+  __shared__ int carry[ROUTE_WARPS + 1];
+  // where the members' rows begin: sums of the totals
+  if (threadIdx.x == 0) carry[ROUTE_WARPS] = 0;
   for (int e0 = 0; e0 <= E; e0 += blockDim.x) {
     const int e = e0 + threadIdx.x;
-    int before = 0, all = 0;
-    if (e <= E) {
-#pragma unroll 8
-      for (int b = 0; b < blocks; ++b) {
-        const int c = a.counts[(long long)b * (E + 1) + e];
-        before += b < block ? c : 0;
-        all += c;
-      }
-    }
-    int inc = all;  // inclusive sums over the block's threads
+    const int all = e <= E ? a.totals[e] : 0;
+    int inc = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int t = __shfl_up_sync(0xFFFFFFFFu, inc, o);
@@ -184,21 +239,20 @@ __device__ __forceinline__ void route_place(const RouteArgs& a, int block, int b
     }
     if (lane == 31) carry[warp] = inc;
     __syncthreads();
-    int first = carry[32];
+    int first = carry[ROUTE_WARPS] + inc - all;
     for (int w = 0; w < warp; ++w) first += carry[w];
-    first += inc - all;
     __syncthreads();
-    if (threadIdx.x == blockDim.x - 1) carry[32] = first + all;
+    if (threadIdx.x == blockDim.x - 1) carry[ROUTE_WARPS] = first + all;
     if (e <= E) {
-      base[e] = first + before;
-      if (block == 0) a.offsets[e] = first;
+      base[e] = first + a.counts[(long long)e * a.blocks + gate];
+      if (gate == 0) a.offsets[e] = first;
     }
-    __syncthreads();
   }
   // each warp's pairs are consecutive; its counts per member come before its places
   for (int i = threadIdx.x; i < ROUTE_WARPS * (E + 1); i += blockDim.x) cnt[i] = 0;
   __syncthreads();
-  const int r0 = block * a.rows_per_block, r1 = min(a.rows, r0 + a.rows_per_block);
+  const int r0 = (int)min((long long)a.rows, (long long)gate * a.rows_per_block);
+  const int r1 = (int)min((long long)a.rows, (long long)r0 + (long long)a.gates * a.rows_per_block);
   const int pairs = max(0, r1 - r0) * a.k, first_pair = r0 * a.k;
   const int per = ((pairs + ROUTE_WARPS - 1) / ROUTE_WARPS + 31) & ~31;
   const int p0 = min(pairs, warp * per), p1 = min(pairs, p0 + per);
@@ -231,96 +285,99 @@ __device__ __forceinline__ void route_place(const RouteArgs& a, int block, int b
       __syncthreads();
     }
   }
-  // the sums of p: members block, block + blocks, ..., a warp each
-  for (int e = block + blocks * warp; e < E; e += blocks * ROUTE_WARPS) {
-    float s = 0.f;
-    for (int b = lane; b < blocks; b += 32) s += a.partial[(long long)b * E + e];
-    s = warp_sum(s);
-    if (lane == 0) a.importance[e] = s;
-  }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(32 * ROUTE_WARPS) route_gate_kernel(const RouteArgs a) {
+__global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 16 ? 2 : 1) route_gate_kernel(const RouteArgs a) {
   extern __shared__ int route_smem[];
   route_gate<T, V>(a, blockIdx.x, route_smem);
 }
 
 __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_place_kernel(const RouteArgs a) {
   extern __shared__ int route_smem[];
-  route_place(a, blockIdx.x, gridDim.x, route_smem);
+  route_place(a, blockIdx.x * a.gates, route_smem);
 }
 
-// Few rows: both phases in one block.
+// Few rows: all of it in one block.
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_small_kernel(const RouteArgs a) {
   extern __shared__ int route_smem[];
   route_gate<T, V>(a, 0, route_smem);
   __syncthreads();
-  route_place(a, 0, 1, route_smem);
+  for (int e = threadIdx.x; e <= a.E; e += blockDim.x) {  // one block's counts and sums
+    a.totals[e] = a.counts[e];
+    a.counts[e] = 0;
+    if (e < a.E) a.importance[e] = a.partial[e];
+  }
+  __syncthreads();
+  route_place(a, 0, route_smem);
 }
 
-// dz of a row by one warp: p is formed again from the scores (reading it would cost more than the sums).
+// dz of a row by one warp: p is formed again from the scores (reading it would cost more than the sums).  Lane j then
+// writes the chosen member of slot j over what the row's formula without the slots' gradients gave.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs a) {
   const int lane = threadIdx.x & 31;
-  const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (r >= a.rows) return;
-  const int E = a.E, k = a.k;
-  const T* z = static_cast<const T*>(a.logits) + (long long)r * a.ld;
-  float p[V], best = -INFINITY;
+  const int E = a.E, k = a.k, stride = gridDim.x * 8;
+  const T* logits = static_cast<const T*>(a.logits);
+  T* dlogits = static_cast<T*>(a.dlogits);
+  float h[V], next[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = lane + 32 * v;
-    p[v] = e < E ? (float)z[e] : -INFINITY;
-    best = max_nan(best, p[v]);
-  }
+  for (int v = 0; v < V; ++v) h[v] = (a.g_importance != nullptr && lane + 32 * v < E) ? a.g_importance[lane + 32 * v] : 0.f;
+  int r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r < a.rows) route_load<T, V>(logits + (long long)r * a.ld, E, lane, next);
+  for (; r < a.rows; r += stride) {
+    float p[V], best = -INFINITY;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) best = max_nan(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
-  const bool some = best != -INFINITY;
-  float total = 0.f, ph = 0.f;
-  float h[V];
+    for (int v = 0; v < V; ++v) {
+      p[v] = next[v];
+      best = max_nan(best, p[v]);
+    }
+    if (r + stride < a.rows) route_load<T, V>(logits + (long long)(r + stride) * a.ld, E, lane, next);
+    // slot j on lane j
+    float w = 0.f, g = 0.f, z_mine = 0.f, h_mine = 0.f;
+    int who = -1;
+    if (lane < k && a.g_weight != nullptr) {
+      who = a.expert[(long long)r * k + lane];
+      if ((unsigned)who < (unsigned)E) {
+        w = a.weight[(long long)r * k + lane];
+        g = a.g_weight[(long long)r * k + lane];
+        z_mine = (float)logits[(long long)r * a.ld + who];
+        if (a.g_importance != nullptr) h_mine = a.g_importance[who];
+      } else {
+        who = -1;
+      }
+    }
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = lane + 32 * v;
-    p[v] = p[v] == -INFINITY ? 0.f : expf(p[v] - best);
-    total += p[v];
-    h[v] = (a.g_importance != nullptr && e < E) ? a.g_importance[e] : 0.f;
-  }
-  total = warp_sum(total);
-  const float inv = some ? 1.f / total : 0.f;
-  // slot j on lane j
-  float w = 0.f, g = 0.f;
-  int who = -1;
-  if (lane < k && a.g_weight != nullptr) {
-    who = a.expert[(long long)r * k + lane];
-    w = a.weight[(long long)r * k + lane];
-    g = who >= 0 ? a.g_weight[(long long)r * k + lane] : 0.f;
-    if (who < 0) w = 0.f;
-  }
-  const float wg = warp_sum(w * g);
+    for (int o = 16; o; o >>= 1) best = max_nan(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
+    const bool some = best != -INFINITY;
+    const float c = some ? -best * LOG2E : 0.f;
+    float total = 0.f, ph = 0.f;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    p[v] *= inv;
-    ph = fmaf(p[v], h[v], ph);
-  }
-  ph = warp_sum(ph);
-  const float through = ph + (a.renorm ? 0.f : wg);
-  const float own = a.renorm ? w * (g - wg) : w * g;
-  T* out = static_cast<T*>(a.dlogits) + (long long)r * E;
-  float d[V];
+    for (int v = 0; v < V; ++v) {
+      p[v] = exp_of(p[v], c);
+      total += p[v];
+      ph = fmaf(p[v], h[v], ph);
+    }
+    float wg = w * g;
 #pragma unroll
-  for (int v = 0; v < V; ++v) d[v] = p[v] * (h[v] - through);
-  for (int j = 0; j < k; ++j) {
-    const int e = __shfl_sync(0xFFFFFFFFu, who, j);
-    const float t = __shfl_sync(0xFFFFFFFFu, own, j);
+    for (int o = 16; o; o >>= 1) {
+      total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+      ph += __shfl_xor_sync(0xFFFFFFFFu, ph, o);
+      wg += __shfl_xor_sync(0xFFFFFFFFu, wg, o);
+    }
+    const float inv = some ? 1.f / total : 0.f;
+    const float through = fmaf(ph, inv, a.renorm ? 0.f : wg);
+    T* out = dlogits + (long long)r * E;
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      if (lane + 32 * v == e) d[v] += t;
+      if (lane + 32 * v < E) out[lane + 32 * v] = (T)(p[v] * inv * (h[v] - through));
+    __syncwarp();
+    if (who >= 0) {
+      const float p_mine = exp_of(z_mine, c) * inv;
+      out[who] = (T)fmaf(w, a.renorm ? g - wg : g, p_mine * (h_mine - through));
+    }
   }
-#pragma unroll
-  for (int v = 0; v < V; ++v)
-    if (lane + 32 * v < E) out[lane + 32 * v] = (T)d[v];
 }
 
 // ---------------------------------------------------------------------------
