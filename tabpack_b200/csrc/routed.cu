@@ -2,6 +2,7 @@
 // include/tabpack_b200.h): host-side validation, tensor maps and kernel dispatch.
 #include <algorithm>
 
+#include "few_rows.cuh"
 #include "fp4.cuh"
 #include "host.cuh"
 #include "ragged_gemm.cuh"
@@ -181,8 +182,14 @@ int launch_rows(RowsArgs k, int what, cudaStream_t st) {
     if (blocks > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many elements for one row move");
     if (what == ROWS_DISPATCH)
       rows_dispatch_kernel<T, BYTES><<<(unsigned)blocks, 256, 0, st>>>(k);
+    else if (k.k == 1)
+      rows_combine_kernel<T, BYTES, 1><<<(unsigned)blocks, 256, 0, st>>>(k);
+    else if (k.k == 2)
+      rows_combine_kernel<T, BYTES, 2><<<(unsigned)blocks, 256, 0, st>>>(k);
+    else if (k.k == 3)
+      rows_combine_kernel<T, BYTES, 3><<<(unsigned)blocks, 256, 0, st>>>(k);
     else
-      rows_combine_kernel<T, BYTES><<<(unsigned)blocks, 256, 0, st>>>(k);
+      rows_combine_kernel<T, BYTES, 4><<<(unsigned)blocks, 256, 0, st>>>(k);
   } else if (k.vecs <= 16) {
     rows_combine_backward_kernel<T, BYTES, 8><<<(k.T + 31) / 32, 256, 0, st>>>(k);
   } else if (k.vecs <= 128) {
@@ -527,6 +534,43 @@ int launch_fp4(Fp4Problem p, const CUtensorMap& ma, const CUtensorMap& mb, long 
   return TP_OK;
 }
 
+// ------------------------------------------------------------------ a few rows a group
+
+// Groups of up to 32 rows on average: the kernel for few rows reads each weight once (its CTAs look through the groups
+// one by one, so there are not too many).
+bool few_rows(int32_t P, int64_t rows) { return P <= 1024 && rows <= 32 * std::min<int64_t>(P, rows); }
+
+template <int KIND>
+int launch_few(const FewArgs& f, const CUtensorMap& ma, const CUtensorMap& mb, cudaStream_t st) {
+  using Cfg = FewCfg<KIND>;
+  constexpr auto kern = few_rows_kernel<KIND>;
+  int rc = allow_smem<kern>(Cfg::SMEM_BYTES);
+  if (rc) return rc;
+  const long long m_tiles = (f.N + 127) / 128, rows = f.groups.rows, used = std::min<long long>(f.groups.P, rows);
+  // pieces of the rows: at most, and as many as are likely to hold rows
+  constexpr int BN = Cfg::BN;
+  const long long most = f.groups.offsets ? rows / BN + used + 2 : (long long)f.groups.P * ((f.groups.B + BN - 1) / BN);
+  const long long likely = f.groups.offsets ? std::max(used, rows / BN) : most;
+  // the K loop over a cluster while the SMs (two CTAs each) are not full and each part has four blocks
+  int split = 1;
+  while (split < 8 && 2 * split * m_tiles * likely <= 2ll * device_info().sms && f.K >= 2 * split * 4 * Cfg::BK) split *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3((unsigned)(m_tiles * split), (unsigned)most);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  TP_PROF(TP_PROF_FWD, st);
+  TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, ma, mb, f, split));
+  return TP_OK;
+}
+
 }  // namespace
 }  // namespace tp
 
@@ -617,6 +661,22 @@ int tp_ragged_linear_forward(const tp_ragged_linear_args* a, void* stream) {
   p.bias = a->bias;
   p.relu = a->relu;
   p.c = a->y;
+  if (a->dtype == TP_DTYPE_BF16 && few_rows(a->P, a->rows)) {
+    FewArgs f{};
+    f.groups = fp4_groups(a->P, a->rows, a->offsets);
+    f.K = a->max_in;
+    f.N = a->max_out;
+    f.in_f = a->in_features;
+    f.out_f = a->out_features;
+    f.bias = a->bias;
+    f.relu = a->relu;
+    f.y = a->y;
+    const auto T = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    CUtensorMap ma, mb;
+    rc = make_map_ld(&ma, T, 2, a->w, a->max_in, a->max_out, a->P, a->w_stride, 64, 128);
+    if (!rc) rc = make_map_ld(&mb, T, 2, a->x, a->max_in, a->rows, 1, a->x_stride, 64, FewCfg<FEW_BF16>::BN);
+    return rc ? rc : launch_few<FEW_BF16>(f, ma, mb, st);
+  }
   if (a->dtype == TP_DTYPE_BF16) return ragged_bf16<RAGGED_FWD>(p, a->x, a->x_stride, a->w, a->w_stride, nullptr, st);
   return ragged_f32<RAGGED_FWD>(p, a->x, a->x_stride, a->w, a->w_stride, st);
 }
@@ -759,6 +819,31 @@ int tp_fp4_linear_forward(const tp_fp4_linear_args* a, void* stream) {
   p.y_f32 = a->dtype == TP_DTYPE_F32;
   p.y_vec = aligned16(a->y) && (long long)a->N * dtype_size(a->dtype) % 16 == 0;
   const long long rows = p.groups.rows;
+  const int pitch = tp_fp4_pitch(a->K);
+  const auto T = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  CUtensorMap ma, mb;
+  if (p.groups.offsets ? few_rows(a->P, rows) : p.groups.B <= 32 && a->P <= 65535) {
+    FewArgs f{};
+    f.groups = p.groups;
+    f.x_shared = a->x_shared;
+    f.K = a->K;
+    f.N = a->N;
+    f.in_f = a->in_features;
+    f.out_f = a->out_features;
+    f.bias = a->bias;
+    f.relu = a->relu;
+    f.y = a->y;
+    f.y_f32 = p.y_f32;
+    f.x_scales = a->x_scales;
+    f.x_row = a->x_row_scale;
+    f.w_scales = a->w_scales;
+    f.w_row = a->w_row_scale;
+    f.atoms = p.atoms;
+    rc = make_map_ld(&ma, T, 1, a->w_codes, pitch, a->N, a->P, pitch, 128, 128);
+    if (!rc) rc = make_map_ld(&mb, T, 1, a->x_codes, pitch, a->rows, 1, pitch, 128, FewCfg<FEW_NV>::BN);
+    if (rc) return rc;
+    return a->format == TP_FP4_NV ? launch_few<FEW_NV>(f, ma, mb, st) : launch_few<FEW_MX>(f, ma, mb, st);
+  }
   const long long m_tiles = p.groups.offsets ? std::max<long long>(std::min<long long>(a->P, rows), rows / 128 + std::min<long long>(a->P, rows) / 2)
                                              : (long long)a->P * ((p.groups.B + 127) / 128);
   int bn = 256;
@@ -766,9 +851,6 @@ int tp_fp4_linear_forward(const tp_fp4_linear_args* a, void* stream) {
   p.n_tiles = (a->N + bn - 1) / bn;
   const long long most = (p.groups.offsets ? rows / 128 + a->P + 2 : m_tiles) * p.n_tiles;
   if (most > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many tiles");
-  const int pitch = tp_fp4_pitch(a->K);
-  const auto T = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  CUtensorMap ma, mb;
   rc = make_map_ld(&ma, T, 1, a->x_codes, pitch, a->rows, 1, pitch, 128, 128);
   if (!rc) rc = make_map_ld(&mb, T, 1, a->w_codes, pitch, a->N, a->P, pitch, 128, bn);
   if (rc) return rc;

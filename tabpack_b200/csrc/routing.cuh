@@ -464,7 +464,8 @@ __global__ void __launch_bounds__(256) rows_dispatch_kernel(const RowsArgs a) {
   }
 }
 
-template <typename T, int BYTES>
+// U rows on their way at a time (k of them where there are up to four).
+template <typename T, int BYTES, int U>
 __global__ void __launch_bounds__(256) rows_combine_kernel(const RowsArgs a) {
   using V = RowVec<T, BYTES>;
   int t, c;
@@ -473,13 +474,25 @@ __global__ void __launch_bounds__(256) rows_combine_kernel(const RowsArgs a) {
   float s[V::N];
 #pragma unroll
   for (int i = 0; i < V::N; ++i) s[i] = 0.f;
-  for (int j = 0; j < a.k; ++j) {
-    const int p = __ldg(a.position + (long long)t * a.k + j);
-    if ((unsigned)p >= (unsigned)used) continue;
-    const float w = a.weight ? __ldg(a.weight + (long long)t * a.k + j) : 1.f;
-    const V y = row_load<T, BYTES>(a.x, (long long)p * a.x_ld + c * V::N);
+  for (int j0 = 0; j0 < a.k; j0 += U) {
+    int p[U];
+    float w[U];
+    V y[U];
 #pragma unroll
-    for (int i = 0; i < V::N; ++i) s[i] = fmaf(w, (float)y.v[i], s[i]);
+    for (int u = 0; u < U; ++u) {
+      const bool in = U < 4 || j0 + u < a.k;
+      p[u] = in ? __ldg(a.position + (long long)t * a.k + j0 + u) : -1;
+      w[u] = in && a.weight ? __ldg(a.weight + (long long)t * a.k + j0 + u) : 1.f;
+    }
+    // (a row that takes no part is replaced by row 0, so that the loads need not wait for one another's conditions)
+#pragma unroll
+    for (int u = 0; u < U; ++u) y[u] = row_load<T, BYTES>(a.x, ((unsigned)p[u] < (unsigned)used ? (long long)p[u] : 0ll) * a.x_ld + c * V::N);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool there = (unsigned)p[u] < (unsigned)used;
+#pragma unroll
+      for (int i = 0; i < V::N; ++i) s[i] = there ? fmaf(w[u], (float)y[u].v[i], s[i]) : s[i];
+    }
   }
   V out;
 #pragma unroll
