@@ -730,7 +730,7 @@ typedef struct tp_ragged_linear_args {
   void* dx;                 /* (rows, max_in) contiguous, or NULL */
   float* dw;                /* (P, max_out, max_in) contiguous, or NULL */
   float* dbias;             /* (P, max_out), or NULL */
-  void* workspace;          /* backward: tp_ragged_linear_workspace_size */
+  void* workspace;          /* tp_ragged_linear_workspace_size of the call's arguments (dy set: backward) */
   size_t workspace_bytes;
 } tp_ragged_linear_args;
 size_t tp_ragged_linear_workspace_size(const tp_ragged_linear_args* a);

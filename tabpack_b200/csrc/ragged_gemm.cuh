@@ -20,6 +20,10 @@
 // WGRAD sums at most RAGGED_SEGMENT rows in one accumulator and adds the pieces up in dw with the rounding of fp32:
 // the tensor core's own sums do not round to nearest, and over 23054 rows came out 2.6e-5 off (5e-6 with the cut).
 // Few tiles over many rows are split over CTAs, into parts that a second launch adds up in order.
+//
+// fp32 operands come as three bf16 parts each (ragged_split_kernel), and the K loop goes through the six products of
+// parts whose terms exceed 2^-24 of the result, the smallest first (sums of up to 2048 elements per accumulator here,
+// added up in fp32): a sixth of the bf16 rate, where the CUDA cores give a twenty-fifth.
 #pragma once
 
 #include <type_traits>
@@ -30,7 +34,7 @@ namespace tp {
 
 enum : int { RAGGED_FWD = 0, RAGGED_DGRAD = 1, RAGGED_WGRAD = 2 };
 enum : int { RT_MMA = 0, RT_ZERO = 1, RT_END = 2 };
-constexpr int RAGGED_SEGMENT = 4096;
+constexpr int RAGGED_SEGMENT = 4096, RAGGED_SEGMENT_F32 = 2048;
 
 struct RaggedProblem {
   int P, R;                // members, rows of the matrix
@@ -45,6 +49,7 @@ struct RaggedProblem {
   int m_tiles;             // wgrad: tiles of a member along `in`
   int n_tiles;             // tiles along the columns of the result (forward: out, dgrad: in, wgrad: out)
   int splits;              // wgrad: parts of a member's rows; c holds a (P, out, in) result for each
+  int a_part, b_part;      // fp32: columns between the parts of A and B
 };
 
 // Rows of group g: members 0 .. P - 1, then the rows before the first and behind the last member's.
@@ -60,15 +65,17 @@ __device__ __forceinline__ void ragged_group(const RaggedProblem& p, int g, int&
   }
 }
 
-// forward, dgrad: `rows` rows from row0 on; wgrad: input features from row0 on, `rows` is the first row of the sum,
-// `part` its part, `add` whether it goes on top of what dw holds.
+// forward, dgrad: `rows` rows from row0 on, sums from element `part` on; wgrad: input features from row0 on, `rows` is the
+// first row of the sum, `part` its part.  add, bit 0: on top of what the result holds; bit 1: more is to come.
 struct RaggedTile {
   int kind, member, row0, rows, nt, k_len, n_valid, m_valid, part, add;
 };
 
-template <int BN_, int MODE, bool PAIR_>
+template <int BN_, int MODE, bool PAIR_, bool F32 = false>
 struct RaggedCfg {
   static constexpr bool PAIR = PAIR_;
+  static constexpr int PASSES = F32 ? 6 : 1;
+  static constexpr int SEGMENT = F32 ? RAGGED_SEGMENT_F32 : RAGGED_SEGMENT;
   static_assert(!PAIR || BN_ == 256, "pairs take tiles of 256 columns");
   static constexpr int BM = 128, BN = BN_, BK = 64;
   static constexpr int TILE_M = PAIR ? 256 : 128;
@@ -142,17 +149,50 @@ __device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
       : "memory");
 }
 
+// A warp's staged 32 x 16 fp32 values into the result, on top of what it holds (`add`) and with ReLU at last.
+__device__ __forceinline__ void ragged_flush_f32(float* c, int ld, int vec, long long row0, int rows, int col0,
+                                                 const uint8_t* stage, int row_bytes, int lane, bool add, bool relu) {
+  if (vec) {
+    const int q = lane & 3;
+    if (col0 + 4 * q >= ld) return;
+    float* to = c + row0 * ld + col0 + 4 * q;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = (lane >> 2) + 8 * k;
+      if (r < rows) {
+        float4 v = *reinterpret_cast<const float4*>(stage + r * row_bytes + q * 16);
+        float4* at = reinterpret_cast<float4*>(to + (long long)r * ld);
+        if (add) {
+          const float4 had = *at;
+          v = make_float4(v.x + had.x, v.y + had.y, v.z + had.z, v.w + had.w);
+        }
+        if (relu) v = make_float4(max_nan(v.x, 0.f), max_nan(v.y, 0.f), max_nan(v.z, 0.f), max_nan(v.w, 0.f));
+        *at = v;
+      }
+    }
+  } else {
+    const int q = lane & 15;
+    if (col0 + q >= ld) return;
+    float* to = c + row0 * ld + col0 + q;
+    for (int r = lane >> 4; r < min(rows, 32); r += 2) {
+      float v = *reinterpret_cast<const float*>(stage + r * row_bytes + 4 * q);
+      if (add) v += to[(long long)r * ld];
+      to[(long long)r * ld] = relu ? max_nan(v, 0.f) : v;
+    }
+  }
+}
+
 // Columns that a pair multiplies in a tile: the rest of the member's, rounded up to 32 (16 a CTA).
 __device__ __forceinline__ int ragged_n(bool pair, int bn, const RaggedTile& t) {
   const int left = t.n_valid - t.nt * bn;
   return min(bn, pair ? (left + 31) & ~31 : (left + 15) & ~15);
 }
 
-template <int BN, int MODE, bool PAIR>
-__global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR>::THREADS, 1)
+template <int BN, int MODE, bool PAIR, bool F32>
+__global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR, F32>::THREADS, 1)
     ragged_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const RaggedProblem pr) {
-  using Cfg = RaggedCfg<BN, MODE, PAIR>;
+  using Cfg = RaggedCfg<BN, MODE, PAIR, F32>;
   constexpr int STAGES = Cfg::STAGES, TRING = Cfg::TRING;
   extern __shared__ uint8_t dyn_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
@@ -203,7 +243,12 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR>::THREADS, 1)
   };
   // a K loop over the whole width ends where the copies fill with zeros by themselves
   const int k_full = MODE == RAGGED_FWD ? pr.in : MODE == RAGGED_DGRAD ? pr.out : -1;
-  auto is_cut = [&](const RaggedTile& t) { return (t.k_len & 15) != 0 && t.k_len != k_full; };
+  auto is_cut = [&](const RaggedTile& t) {
+    return (t.k_len & 15) != 0 && (MODE == RAGGED_WGRAD || t.part + t.k_len != k_full);
+  };
+  // fp32: which parts of A and B a pass multiplies, two bits each: lh, hl, mm, mh, hm, hh
+  auto a_of = [&](int pass) { return F32 ? (0x052 >> (2 * pass)) & 3 : 0; };
+  auto b_of = [&](int pass) { return F32 ? (0x118 >> (2 * pass)) & 3 : 0; };
   // zeros from element `left` of a stage's K on, up to the next step of 16; by a whole warp
   auto zero_tail = [&](int stage, int left) {
     uint8_t* a = smA + stage * Cfg::A_BYTES;
@@ -303,16 +348,19 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR>::THREADS, 1)
         // the copies' coordinates: along K and along the other side
         const int b_col = t.nt * BN + (PAIR ? rank * (ragged_n(true, BN, t) / 2) : 0);
         const int other = is_a ? t.row0 + rank * Cfg::BM : b_col;
-        const int k_first = WG ? t.rows : 0, z = (is_a || WG) ? 0 : t.member;
+        const int k_first = WG ? t.rows : t.part, z = (is_a || WG) ? 0 : t.member;
         const int common = !PAIR ? 0 : is_cut(t) ? kblocks - 1 : kblocks;  // stages on the common barrier
-        int kb = 0;
-        for (; ok && kb < common; ++kb) {
-          const int at = k_first + kb * Cfg::BK;
-          ok = produce(std::bool_constant<!PAIR>(), mn ? other : at, mn ? at : other, z);
-        }
-        for (; ok && kb < kblocks; ++kb) {
-          const int at = k_first + kb * Cfg::BK;
-          ok = produce(std::bool_constant<true>(), mn ? other : at, mn ? at : other, z);
+        for (int pass = 0; ok && pass < Cfg::PASSES; ++pass) {
+          const int shift = is_a ? a_of(pass) * pr.a_part : b_of(pass) * pr.b_part;  // (0 for bf16)
+          int kb = 0;
+          for (; ok && kb < common; ++kb) {
+            const int at = k_first + kb * Cfg::BK;
+            ok = produce(std::bool_constant<!PAIR>(), (mn ? other : at) + shift, mn ? at : other, z);
+          }
+          for (; ok && kb < kblocks; ++kb) {
+            const int at = k_first + kb * Cfg::BK;
+            ok = produce(std::bool_constant<true>(), (mn ? other : at) + shift, mn ? at : other, z);
+          }
         }
       }
     }
@@ -359,51 +407,53 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR>::THREADS, 1)
       };
       // one thread goes through the blocks; the whole warp comes together for one that needs zeros
       const int plain = cut ? kblocks - 1 : kblocks;
-      if (lane == 0) {
-        int st = stage;
-        uint32_t ph = phase;
-        for (int kb = 0; kb < plain; ++kb) {
-          if (!mbar_wait(&full[st], ph, abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          if (kb < kblocks - 1)
-            multiply(st, Cfg::BK / 16, kb == 0);
-          else
-            multiply(st, (last + 15) >> 4, kb == 0);
-          if (++st == STAGES) {
-            st = 0;
-            ph ^= 1u;
+      for (int pass = 0; ok && pass < Cfg::PASSES; ++pass) {
+        if (lane == 0) {
+          int st = stage;
+          uint32_t ph = phase;
+          for (int kb = 0; kb < plain; ++kb) {
+            if (!mbar_wait(&full[st], ph, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            if (kb < kblocks - 1)
+              multiply(st, Cfg::BK / 16, pass == 0 && kb == 0);
+            else
+              multiply(st, (last + 15) >> 4, pass == 0 && kb == 0);
+            if (++st == STAGES) {
+              st = 0;
+              ph ^= 1u;
+            }
           }
         }
-      }
-      phase ^= (uint32_t)((stage + plain) / STAGES) & 1u;
-      stage = (stage + plain) % STAGES;
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (ok && cut) {
-        if constexpr (PAIR) {
-          const uint32_t ph = (cut_phase >> stage) & 1u;
-          ok = mbar_wait(&cut_full[stage], ph, abort_flag);
-          if (__all_sync(0xFFFFFFFFu, ok)) {
-            zero_tail(stage, last);
-            ok = mbar_wait<true>(&cut_peer[stage], ph, abort_flag);
-          }
-          if (lane == 0) mbar_arrive(&full[stage]);  // the stage's phase goes on without the common barrier
-          cut_phase ^= 1u << stage;
-        } else {
-          ok = mbar_wait(&full[stage], phase, abort_flag);
-          if (__all_sync(0xFFFFFFFFu, ok)) zero_tail(stage, last);
-        }
+        phase ^= (uint32_t)((stage + plain) / STAGES) & 1u;
+        stage = (stage + plain) % STAGES;
         ok = __all_sync(0xFFFFFFFFu, ok);
-        if (ok) {
-          tc_fence_after();
-          if (lane == 0) multiply(stage, (last + 15) >> 4, kblocks == 1);
-          __syncwarp();
-        }
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
+        if (ok && cut) {
+          if constexpr (PAIR) {
+            const uint32_t ph = (cut_phase >> stage) & 1u;
+            ok = mbar_wait(&cut_full[stage], ph, abort_flag);
+            if (__all_sync(0xFFFFFFFFu, ok)) {
+              zero_tail(stage, last);
+              ok = mbar_wait<true>(&cut_peer[stage], ph, abort_flag);
+            }
+            if (lane == 0) mbar_arrive(&full[stage]);  // the stage's phase goes on without the common barrier
+            cut_phase ^= 1u << stage;
+          } else {
+            ok = mbar_wait(&full[stage], phase, abort_flag);
+            if (__all_sync(0xFFFFFFFFu, ok)) zero_tail(stage, last);
+          }
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (ok) {
+            tc_fence_after();
+            if (lane == 0) multiply(stage, (last + 15) >> 4, pass == 0 && kblocks == 1);
+            __syncwarp();
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
         }
       }
       if (!ok) break;
@@ -434,14 +484,18 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR>::THREADS, 1)
       if (t.kind == RT_END) break;
       if (t.kind != RT_MMA) continue;
       const int kblocks = (t.k_len + Cfg::BK - 1) / Cfg::BK;
-      const int last = (stage + kblocks - 1) % STAGES;
-      stage = (stage + kblocks) % STAGES;
-      if (!is_cut(t)) continue;
-      const bool ok = mbar_wait(&cut_full[last], (cut_phase >> last) & 1u, abort_flag);
-      cut_phase ^= 1u << last;
-      if (!__all_sync(0xFFFFFFFFu, ok)) break;
-      zero_tail(last, t.k_len - (kblocks - 1) * Cfg::BK);
-      if (lane == 0) mbar_arrive_release_cluster(mapa_shared(smem_u32(&cut_peer[last]), 0));
+      bool ok = true;
+      for (int pass = 0; ok && pass < Cfg::PASSES; ++pass) {
+        const int last = (stage + kblocks - 1) % STAGES;
+        stage = (stage + kblocks) % STAGES;
+        if (!is_cut(t)) continue;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&cut_full[last], (cut_phase >> last) & 1u, abort_flag));
+        cut_phase ^= 1u << last;
+        if (!ok) break;
+        zero_tail(last, t.k_len - (kblocks - 1) * Cfg::BK);
+        if (lane == 0) mbar_arrive_release_cluster(mapa_shared(smem_u32(&cut_peer[last]), 0));
+      }
+      if (!ok) break;
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ scheduler (a pair's CTAs find the same tiles)
@@ -489,12 +543,12 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR>::THREADS, 1)
         if (end > first && t.row0 < t.m_valid && t.nt * BN < t.n_valid) {
           t.kind = RT_MMA;
           // pieces of about the same length: a short one would not hide the other's read and write of dw
-          const int pieces = (end - first + RAGGED_SEGMENT - 1) / RAGGED_SEGMENT;
+          const int pieces = (end - first + Cfg::SEGMENT - 1) / Cfg::SEGMENT;
           const int piece = ((end - first + pieces - 1) / pieces + 63) & ~63;
           for (int k = first; ok && k < end; k += piece) {
             t.rows = k;
             t.k_len = min(piece, end - k);
-            t.add = k > first;
+            t.add = k > first ? 1 : 0;
             ok = publish(t);
           }
         } else {
@@ -546,7 +600,20 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR>::THREADS, 1)
           t.n_valid = MODE == RAGGED_FWD ? out_m : in_m;
           if (t.nt * BN < t.n_valid && t.k_len > 0) t.kind = RT_MMA;
         }
-        ok = publish(t);
+        if (F32 && t.kind == RT_MMA) {
+          // pieces of the K loop, added up in the result
+          const int whole = t.k_len, pieces = (whole + Cfg::SEGMENT - 1) / Cfg::SEGMENT;
+          const int piece = ((whole + pieces - 1) / pieces + 63) & ~63;
+          for (int k = 0; ok && k < whole; k += piece) {
+            t.part = k;
+            t.k_len = min(piece, whole - k);
+            t.add = (k > 0 ? 1 : 0) | (k + piece < whole ? 2 : 0);
+            ok = publish(t);
+          }
+          t.part = t.add = 0;
+        } else {
+          ok = publish(t);
+        }
       }
     }
     if (ok) {
@@ -583,7 +650,7 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR>::THREADS, 1)
             uint32_t v[32];
             tmem_ld_32x32b_x32(t_row + (uint32_t)(32 * c), v);
             tmem_wait_ld();
-            if (t.add) {
+            if (t.add & 1) {
               // on top of the sums over earlier rows, which this thread wrote; all loads before the stores
               float had[32];
 #pragma unroll
@@ -633,6 +700,26 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR>::THREADS, 1)
               tmem_ld_32x32b_x32(t_row + (uint32_t)(32 * c), v);
               tmem_wait_ld();
               const int nv = t.n_valid - (cbase + 32 * c);
+              if constexpr (F32) {
+#pragma unroll
+                for (int h = 0; h < 32; h += 16) {
+#pragma unroll
+                  for (int j = 0; j < 16; j += 4) {
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                      x[e] = __uint_as_float(v[h + j + e]);
+                      if (MODE == RAGGED_FWD && !(t.add & 1)) x[e] += sbias[32 * c + h + j + e];
+                      if (h + j + e >= nv) x[e] = 0.f;
+                    }
+                    *reinterpret_cast<float4*>(stage_row + j * 4) = make_float4(x[0], x[1], x[2], x[3]);
+                  }
+                  __syncwarp();
+                  ragged_flush_f32(static_cast<float*>(pr.c), ld, pr.c_vec, row0, rows, cbase + 32 * c + h, stage_warp,
+                                   Cfg::ROW_BYTES, lane, t.add & 1, MODE == RAGGED_FWD && pr.relu && !(t.add & 2));
+                  __syncwarp();
+                }
+              } else {
 #pragma unroll
               for (int j = 0; j < 32; j += 8) {
                 float x[8];
@@ -651,6 +738,7 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR>::THREADS, 1)
               __syncwarp();
               ragged_flush(out, ld, pr.c_vec, row0, rows, cbase + 32 * c, stage_warp, Cfg::ROW_BYTES, lane);
               __syncwarp();
+              }
             }
           }
         } else if (rows > 0) {
@@ -658,8 +746,15 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR>::THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage_row + 16 * j) = make_uint4(0, 0, 0, 0);
           __syncwarp();
-          for (int c = 0; c < nch; ++c)
-            ragged_flush(out, ld, pr.c_vec, row0, rows, cbase + 32 * c, stage_warp, Cfg::ROW_BYTES, lane);
+          for (int c = 0; c < nch; ++c) {
+            if constexpr (F32) {
+              for (int h = 0; h < 32; h += 16)
+                ragged_flush_f32(static_cast<float*>(pr.c), ld, pr.c_vec, row0, rows, cbase + 32 * c + h, stage_warp,
+                                 Cfg::ROW_BYTES, lane, false, false);
+            } else {
+              ragged_flush(out, ld, pr.c_vec, row0, rows, cbase + 32 * c, stage_warp, Cfg::ROW_BYTES, lane);
+            }
+          }
         }
       }
       if (t.kind == RT_MMA) {
@@ -700,123 +795,46 @@ __global__ void __launch_bounds__(256) ragged_parts_kernel(const float* parts, f
 }
 
 // ---------------------------------------------------------------------------
-// The same products on the CUDA cores in fp32: 64 x 64 tiles, 4 x 4 results a thread.
+// fp32 operands as three bf16 parts, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m): 24 bits in
+// all, each difference exact.  A row's parts lie side by side, `cols` columns (a multiple of 64) each, zeros at the end.
+// Of a number that is not finite h is the whole.
 // ---------------------------------------------------------------------------
-struct RaggedSimt {
-  RaggedProblem p;
-  const float* a;  // forward: x, dgrad: g, wgrad: x
-  long long a_ld;
-  const float* b;  // forward, dgrad: w (rows at w_ld, members at out * w_ld), wgrad: g
-  long long b_ld;
+struct SplitArgs {
+  const float* x[3];  // up to three matrices in a launch
+  long long ld[3], rows[3];
+  int width[3], cols[3], vec[3];  // vec: rows on 16-byte boundaries
+  FastDiv div[3];                 // by the pieces of 8 columns of a row
+  __nv_bfloat16* out[3];
 };
 
-template <int MODE>
-__global__ void __launch_bounds__(256) ragged_simt_kernel(const RaggedSimt s) {
-  constexpr int TB = 64, TK = 16;
-  __shared__ float As[TK][TB + 4];
-  __shared__ float Bs[TK][TB + 4];
-  const RaggedProblem& p = s.p;
-  const int tid = threadIdx.x, lane = tid & 31;
-  // this block's tile: along M the rows of the member (or its input features), along N the result's columns
-  int member = 0, m0 = 0, m_end = 0, first = 0, k_len = 0, n_valid = 0, m_valid = 0;
-  const int nt = blockIdx.x % p.n_tiles;
-  const int i = blockIdx.x / p.n_tiles;
-  if (MODE == RAGGED_WGRAD) {
-    member = i / p.m_tiles;
-    m0 = (i - member * p.m_tiles) * TB;
-    m_end = p.in;
-    int end;
-    ragged_group(p, member, first, end);
-    k_len = end - first;
-    m_valid = p.in_f ? min(p.in_f[member], p.in) : p.in;
-    n_valid = p.out_f ? min(p.out_f[member], p.out) : p.out;
-  } else {
-    int before = 0, g0 = 0;
-    for (;; g0 += 32) {
-      if (g0 >= p.P + 2) return;
-      int f = 0, e = 0;
-      if (g0 + lane < p.P + 2) ragged_group(p, g0 + lane, f, e);
-      const int tiles = (e - f + TB - 1) / TB;
-      int inc = tiles;
+__global__ void __launch_bounds__(256) ragged_split_kernel(const SplitArgs a) {
+  const int k = blockIdx.y;
+  const int pieces = a.cols[k] / 8;
+  const long long total = a.rows[k] * pieces;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long r = i < 0x7FFFFFFFLL ? (long long)fastdiv((uint32_t)i, a.div[k]) : i / pieces;
+    const int c = 8 * (int)(i - r * pieces);
+    const float* x = a.x[k] + r * a.ld[k] + c;
+    float v[8];
+    if (a.vec[k] && c + 8 <= a.width[k]) {
+      const float4 lo = __ldg(reinterpret_cast<const float4*>(x)), hi = __ldg(reinterpret_cast<const float4*>(x) + 1);
+      v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+    } else {
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      const int sum = __shfl_sync(0xFFFFFFFFu, inc, 31);
-      if (i < before + sum) {
-        const int who = __ffs(__ballot_sync(0xFFFFFFFFu, i - before < inc)) - 1;
-        member = g0 + who;
-        m0 = __shfl_sync(0xFFFFFFFFu, f, who) + (i - before - __shfl_sync(0xFFFFFFFFu, inc - tiles, who)) * TB;
-        m_end = __shfl_sync(0xFFFFFFFFu, e, who);
-        break;
-      }
-      before += sum;
+      for (int e = 0; e < 8; ++e) v[e] = c + e < a.width[k] ? __ldg(x + e) : 0.f;
     }
-    if (member < p.P) {
-      const int in_m = p.in_f ? min(p.in_f[member], p.in) : p.in;
-      const int out_m = p.out_f ? min(p.out_f[member], p.out) : p.out;
-      k_len = MODE == RAGGED_FWD ? in_m : out_m;
-      n_valid = MODE == RAGGED_FWD ? out_m : in_m;
-    }
-    m_valid = m_end;
-  }
-  const int n0 = nt * TB;
-  const int n_end = MODE == RAGGED_DGRAD ? p.in : p.out;
-  const int tx = tid & 15, ty = tid >> 4;
-  float acc[4][4] = {};
-  if (n0 < n_valid && m0 < m_valid) {
-    const float* w = s.b + (MODE == RAGGED_WGRAD ? 0 : (long long)member * p.out * s.b_ld);
-    for (int k0 = 0; k0 < k_len; k0 += TK) {
-      for (int j = tid; j < TB * TK; j += 256) {
-        const int m = MODE == RAGGED_WGRAD ? j % TB : j / TK, k = MODE == RAGGED_WGRAD ? j / TB : j % TK;
-        float v = 0.f;
-        if (k0 + k < k_len && m0 + m < m_valid)
-          v = MODE == RAGGED_WGRAD ? s.a[(long long)(first + k0 + k) * s.a_ld + m0 + m]
-                                   : s.a[(long long)(m0 + m) * s.a_ld + k0 + k];
-        As[k][m] = v;
+    __nv_bfloat16* out = a.out[k] + 3 * r * a.cols[k] + c;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const __nv_bfloat16 h = __float2bfloat16_rn(v[e]);
+        const float f = __bfloat162float(h);
+        w[e >> 1] = (e & 1) ? w[e >> 1] | (uint32_t)__bfloat16_as_ushort(h) << 16 : (uint32_t)__bfloat16_as_ushort(h);
+        v[e] = fabsf(f) < INFINITY ? v[e] - f : 0.f;
       }
-      for (int j = tid; j < TB * TK; j += 256) {
-        const int n = MODE == RAGGED_FWD ? j / TK : j % TB, k = MODE == RAGGED_FWD ? j % TK : j / TB;
-        float v = 0.f;
-        if (k0 + k < k_len && n0 + n < n_valid)
-          v = MODE == RAGGED_FWD     ? w[(long long)(n0 + n) * s.b_ld + k0 + k]
-              : MODE == RAGGED_DGRAD ? w[(long long)(k0 + k) * s.b_ld + n0 + n]
-                                     : w[(long long)(first + k0 + k) * s.b_ld + n0 + n];
-        Bs[k][n] = v;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < TK; ++k) {
-        const float4 a = *reinterpret_cast<const float4*>(&As[k][ty * 4]);
-        const float4 b = *reinterpret_cast<const float4*>(&Bs[k][tx * 4]);
-        const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-          for (int y = 0; y < 4; ++y) acc[x][y] = fmaf(av[x], bv[y], acc[x][y]);
-      }
-      __syncthreads();
-    }
-  }
-#pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    const int m = m0 + ty * 4 + x;
-    if (m >= m_end) continue;
-#pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const int n = n0 + tx * 4 + y;
-      if (n >= n_end) continue;
-      float v = acc[x][y];
-      if (MODE == RAGGED_FWD) {
-        if (p.bias != nullptr && n < n_valid) v += p.bias[(long long)member * p.out + n];
-        if (p.relu) v = max_nan(v, 0.f);
-      }
-      if (n >= n_valid || m >= m_valid) v = 0.f;
-      if (MODE == RAGGED_WGRAD)
-        static_cast<float*>(p.c)[((long long)member * p.out + n) * p.in + m] = v;
-      else
-        static_cast<float*>(p.c)[(long long)m * (MODE == RAGGED_FWD ? p.out : p.in) + n] = v;
+      *reinterpret_cast<uint4*>(out + p * a.cols[k]) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }

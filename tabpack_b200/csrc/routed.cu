@@ -271,10 +271,10 @@ RaggedProblem ragged_problem(const tp_ragged_linear_args* a) {
   return p;
 }
 
-template <int BN, int MODE, bool PAIR>
+template <int BN, int MODE, bool PAIR, bool F32>
 int launch_ragged(const RaggedProblem& p, const CUtensorMap& ma, const CUtensorMap& mb, long long tiles, cudaStream_t st) {
-  using Cfg = RaggedCfg<BN, MODE, PAIR>;
-  constexpr auto kern = ragged_gemm_kernel<BN, MODE, PAIR>;
+  using Cfg = RaggedCfg<BN, MODE, PAIR, F32>;
+  constexpr auto kern = ragged_gemm_kernel<BN, MODE, PAIR, F32>;
   int rc = allow_smem<kern>(Cfg::SMEM_BYTES);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -342,44 +342,46 @@ RaggedPlan ragged_plan(int mode, int P, int64_t R, int in, int out) {
   return plan;
 }
 
-// bf16 operands: A and B with their row strides.
-template <int MODE>
-int ragged_bf16(RaggedProblem p, const void* a_ptr, long long a_ld, const void* b_ptr, long long b_ld, float* parts,
-                cudaStream_t st) {
+// One of the products: A and B with their row strides; fp32 operands as their parts, at a_part and b_part columns.
+template <int MODE, bool F32>
+int ragged_product(RaggedProblem p, const void* a_ptr, long long a_ld, const void* b_ptr, long long b_ld, float* parts,
+                   cudaStream_t st) {
   const int cols = MODE == RAGGED_DGRAD ? p.in : p.out;  // columns of the result
   const RaggedPlan plan = ragged_plan(MODE, p.P, p.R, p.in, p.out);
   const int bn = plan.bn, tm = plan.tile_m;
   p.n_tiles = (cols + bn - 1) / bn;
   p.m_tiles = (p.in + tm - 1) / tm;
   p.splits = plan.splits;
-  p.c_vec = aligned16(p.c) && cols % 8 == 0;
+  p.c_vec = aligned16(p.c) && cols % (F32 ? 4 : 8) == 0;
   void* result = p.c;
   if (MODE == RAGGED_WGRAD && plan.splits > 1) p.c = parts;
   const long long most = MODE == RAGGED_WGRAD ? (long long)p.P * p.m_tiles * p.n_tiles * p.splits
                                               : ((long long)p.R / tm + p.P + 2) * p.n_tiles;
   if (most > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many tiles");
   const auto T = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  // fp32: all three parts of a row are the map's columns
+  const uint64_t in = F32 ? (uint64_t)(MODE == RAGGED_WGRAD ? a_ld : b_ld) : p.in, out = F32 ? (uint64_t)(MODE == RAGGED_DGRAD ? a_ld : b_ld) : p.out;
   CUtensorMap ma, mb;
   int rc;
   if (MODE == RAGGED_FWD) {
-    rc = make_map_ld(&ma, T, 2, a_ptr, p.in, p.R, 1, a_ld, 64, 128);
-    if (!rc) rc = make_map_ld(&mb, T, 2, b_ptr, p.in, p.out, p.P, b_ld, 64, plan.pair ? bn / 2 : bn);
+    rc = make_map_ld(&ma, T, 2, a_ptr, F32 ? (uint64_t)a_ld : p.in, p.R, 1, a_ld, 64, 128);
+    if (!rc) rc = make_map_ld(&mb, T, 2, b_ptr, in, p.out, p.P, b_ld, 64, plan.pair ? bn / 2 : bn);
   } else if (MODE == RAGGED_DGRAD) {
-    rc = make_map_ld(&ma, T, 2, a_ptr, p.out, p.R, 1, a_ld, 64, 128);
-    if (!rc) rc = make_map_ld(&mb, T, 2, b_ptr, p.in, p.out, p.P, b_ld, 64, 64);
+    rc = make_map_ld(&ma, T, 2, a_ptr, out, p.R, 1, a_ld, 64, 128);
+    if (!rc) rc = make_map_ld(&mb, T, 2, b_ptr, in, p.out, p.P, b_ld, 64, 64);
   } else {
-    rc = make_map_ld(&ma, T, 2, a_ptr, p.in, p.R, 1, a_ld, 64, 64);
-    if (!rc) rc = make_map_ld(&mb, T, 2, b_ptr, p.out, p.R, 1, b_ld, 64, 64);
+    rc = make_map_ld(&ma, T, 2, a_ptr, in, p.R, 1, a_ld, 64, 64);
+    if (!rc) rc = make_map_ld(&mb, T, 2, b_ptr, out, p.R, 1, b_ld, 64, 64);
   }
   if (rc) return rc;
   if (plan.pair)
-    rc = launch_ragged<256, MODE, true>(p, ma, mb, most, st);
+    rc = launch_ragged<256, MODE, true, F32>(p, ma, mb, most, st);
   else if (bn == 256)
-    rc = launch_ragged<256, MODE, false>(p, ma, mb, most, st);
+    rc = launch_ragged<256, MODE, false, F32>(p, ma, mb, most, st);
   else if (bn == 128)
-    rc = launch_ragged<128, MODE, false>(p, ma, mb, most, st);
+    rc = launch_ragged<128, MODE, false, F32>(p, ma, mb, most, st);
   else
-    rc = launch_ragged<64, MODE, false>(p, ma, mb, most, st);
+    rc = launch_ragged<64, MODE, false, F32>(p, ma, mb, most, st);
   if (rc) return rc;
   if (MODE == RAGGED_WGRAD && plan.splits > 1) {
     const long long n = (long long)p.P * p.out * p.in;
@@ -389,18 +391,34 @@ int ragged_bf16(RaggedProblem p, const void* a_ptr, long long a_ld, const void* 
   return TP_OK;
 }
 
-template <int MODE>
-int ragged_f32(RaggedProblem p, const void* a_ptr, long long a_ld, const void* b_ptr, long long b_ld, cudaStream_t st) {
-  RaggedSimt s{p, static_cast<const float*>(a_ptr), a_ld, static_cast<const float*>(b_ptr), b_ld};
-  s.p.n_tiles = ((MODE == RAGGED_DGRAD ? p.in : p.out) + 63) / 64;
-  s.p.m_tiles = (p.in + 63) / 64;
-  const long long grid = (MODE == RAGGED_WGRAD ? (long long)p.P * s.p.m_tiles : (long long)p.R / 64 + p.P + 2) * s.p.n_tiles;
-  if (grid > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many tiles");
-  TP_PROF(TP_PROF_GEMM_F32, st);
-  ragged_simt_kernel<MODE><<<(unsigned)grid, 256, 0, st>>>(s);
-  TP_CUDA_TRY(cudaGetLastError());
-  return TP_OK;
-}
+int split_cols(int width) { return (width + 63) / 64 * 64; }
+// Bytes of a matrix's three parts.
+size_t split_bytes(long long rows, int width) { return (size_t)rows * split_cols(width) * 6; }
+
+// The parts of up to three fp32 matrices.
+struct Splits {
+  SplitArgs k{};
+  int count = 0;
+  long long blocks = 1;
+  __nv_bfloat16* add(const void* x, long long ld, long long rows, int width, void* out) {
+    const int i = count++, cols = split_cols(width);
+    k.x[i] = static_cast<const float*>(x);
+    k.ld[i] = ld;
+    k.rows[i] = rows;
+    k.width[i] = width;
+    k.cols[i] = cols;
+    k.vec[i] = aligned16(x) && ld % 4 == 0;
+    k.div[i] = make_fastdiv((uint32_t)(cols / 8));
+    k.out[i] = static_cast<__nv_bfloat16*>(out);
+    blocks = std::max(blocks, (rows * (cols / 8) + 255) / 256);
+    return k.out[i];
+  }
+  int launch(cudaStream_t st) const {
+    ragged_split_kernel<<<dim3((unsigned)std::min<long long>(blocks, 16 * 148), count), 256, 0, st>>>(k);
+    TP_CUDA_TRY(cudaGetLastError());
+    return TP_OK;
+  }
+};
 
 // Columns of a block of the activation gradient: long pieces of each row where that leaves blocks enough.
 int ragged_strip(const tp_ragged_linear_args* a) { return a->rows * a->max_out >= (4ll << 20) && a->max_out >= 256 ? 256 : 64; }
@@ -434,19 +452,27 @@ void launch_act(const RaggedAct& k, bool vec, bool wide, dim3 grid, cudaStream_t
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// The backward's workspace: g, the shares' sums of g, the parts of dw.
+// The workspace.  Forward: the parts of fp32 x and w.  Backward: g, the shares' sums of g, the partial results of dw,
+// the parts of fp32 g, x and w.
 struct RaggedSpace {
-  size_t shares, parts, parts_bytes;
+  size_t shares, parts, g3, x3, w3, bytes;
 };
 RaggedSpace ragged_space(const tp_ragged_linear_args* a) {
   RaggedSpace s{};
-  s.shares = round256((size_t)a->rows * (size_t)ragged_g_stride(a) * dtype_size(a->dtype));
-  s.parts = s.shares;
-  if (a->dbias && ragged_shares(a) > 1) s.parts += round256((size_t)ragged_shares(a) * a->P * a->max_out * sizeof(float));
-  if (a->dw && a->dtype == TP_DTYPE_BF16) {
-    const int splits = ragged_plan(RAGGED_WGRAD, a->P, a->rows, a->max_in, a->max_out).splits;
-    if (splits > 1) s.parts_bytes = (size_t)splits * a->P * a->max_out * a->max_in * sizeof(float);
+  const bool f32 = a->dtype == TP_DTYPE_F32;
+  if (a->dy) {
+    s.shares = round256((size_t)a->rows * (size_t)ragged_g_stride(a) * dtype_size(a->dtype));
+    s.parts = s.shares;
+    if (a->dbias && ragged_shares(a) > 1) s.parts += round256((size_t)ragged_shares(a) * a->P * a->max_out * sizeof(float));
+    s.g3 = s.parts;
+    if (a->dw) {
+      const int splits = ragged_plan(RAGGED_WGRAD, a->P, a->rows, a->max_in, a->max_out).splits;
+      if (splits > 1) s.g3 += round256((size_t)splits * a->P * a->max_out * a->max_in * sizeof(float));
+    }
   }
+  s.x3 = s.g3 + (f32 && (a->dx || a->dw) ? round256(split_bytes(a->rows, a->max_out)) : 0);
+  s.w3 = s.x3 + (f32 && (!a->dy || a->dw) ? round256(split_bytes(a->rows, a->max_in)) : 0);
+  s.bytes = s.w3 + (f32 && (!a->dy || a->dx) ? split_bytes((long long)a->P * a->max_out, a->max_in) : 0);
   return s;
 }
 
@@ -646,10 +672,16 @@ int tp_combine_rows_backward(const tp_rows_args* a, void* stream) {
   return dispatch_rows(&b, ROWS_BACKWARD, stream);
 }
 
+static int check_ragged_workspace(const tp_ragged_linear_args* a, size_t need) {
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace)))
+    return fail(TP_EINVAL, "ragged linear workspace of %zu bytes is smaller than the %zu needed, or not aligned",
+                a->workspace_bytes, need);
+  return TP_OK;
+}
+
 size_t tp_ragged_linear_workspace_size(const tp_ragged_linear_args* a) {
   if (!a || a->P <= 0 || a->max_out <= 0 || a->rows <= 0) return 0;
-  const RaggedSpace s = ragged_space(a);
-  return s.parts + s.parts_bytes;
+  return ragged_space(a).bytes;
 }
 
 int tp_ragged_linear_forward(const tp_ragged_linear_args* a, void* stream) {
@@ -677,8 +709,24 @@ int tp_ragged_linear_forward(const tp_ragged_linear_args* a, void* stream) {
     if (!rc) rc = make_map_ld(&mb, T, 2, a->x, a->max_in, a->rows, 1, a->x_stride, 64, FewCfg<FEW_BF16>::BN);
     return rc ? rc : launch_few<FEW_BF16>(f, ma, mb, st);
   }
-  if (a->dtype == TP_DTYPE_BF16) return ragged_bf16<RAGGED_FWD>(p, a->x, a->x_stride, a->w, a->w_stride, nullptr, st);
-  return ragged_f32<RAGGED_FWD>(p, a->x, a->x_stride, a->w, a->w_stride, st);
+  if (a->dtype == TP_DTYPE_BF16)
+    return ragged_product<RAGGED_FWD, false>(p, a->x, a->x_stride, a->w, a->w_stride, nullptr, st);
+  tp_ragged_linear_args fwd = *a;
+  fwd.dy = nullptr;
+  fwd.dx = nullptr;
+  fwd.dw = nullptr;
+  const RaggedSpace space = ragged_space(&fwd);
+  rc = check_ragged_workspace(a, space.bytes);
+  if (rc) return rc;
+  char* ws = static_cast<char*>(a->workspace);
+  Splits k;
+  const void* x = k.add(a->x, a->x_stride, a->rows, a->max_in, ws + space.x3);
+  const void* w = k.add(a->w, a->w_stride, (long long)a->P * a->max_out, a->max_in, ws + space.w3);
+  rc = k.launch(st);
+  if (rc) return rc;
+  const int cols = split_cols(a->max_in);
+  p.a_part = p.b_part = cols;
+  return ragged_product<RAGGED_FWD, true>(p, x, 3 * cols, w, 3 * cols, nullptr, st);
 }
 
 int tp_ragged_linear_backward(const tp_ragged_linear_args* a, void* stream) {
@@ -687,12 +735,10 @@ int tp_ragged_linear_backward(const tp_ragged_linear_args* a, void* stream) {
   if (rc) return rc;
   if (!a->dy || (a->relu && !a->y)) return fail(TP_EINVAL, "null ragged linear gradient or output");
   if (a->dy_stride < a->max_out) return fail(TP_EINVAL, "rows of dy overlap");
-  const size_t need = tp_ragged_linear_workspace_size(a);
-  if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace)))
-    return fail(TP_EINVAL, "ragged linear workspace of %zu bytes is smaller than the %zu needed, or not aligned",
-                a->workspace_bytes, need);
-  const bool bf16 = a->dtype == TP_DTYPE_BF16;
   const RaggedSpace space = ragged_space(a);
+  rc = check_ragged_workspace(a, space.bytes);
+  if (rc) return rc;
+  const bool bf16 = a->dtype == TP_DTYPE_BF16;
   float* parts = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + space.parts);
   const long long g_ld = ragged_g_stride(a);
   const void* g = g_ld ? a->workspace : a->dy;
@@ -726,19 +772,37 @@ int tp_ragged_linear_backward(const tp_ragged_linear_args* a, void* stream) {
     TP_CUDA_TRY(cudaGetLastError());
   }
   RaggedProblem p = ragged_problem(a);
+  if (bf16) {
+    if (a->dx) {
+      p.c = a->dx;
+      rc = ragged_product<RAGGED_DGRAD, false>(p, g, ld, a->w, a->w_stride, nullptr, st);
+      if (rc) return rc;
+    }
+    if (!a->dw) return TP_OK;
+    p.c = a->dw;
+    return ragged_product<RAGGED_WGRAD, false>(p, a->x, a->x_stride, g, ld, parts, st);
+  }
+  if (!a->dx && !a->dw) return TP_OK;
+  char* ws = static_cast<char*>(a->workspace);
+  const int gc = split_cols(a->max_out), xc = split_cols(a->max_in);
+  Splits k;
+  const void* g3 = k.add(g, ld, a->rows, a->max_out, ws + space.g3);
+  const void* x3 = a->dw ? k.add(a->x, a->x_stride, a->rows, a->max_in, ws + space.x3) : nullptr;
+  const void* w3 = a->dx ? k.add(a->w, a->w_stride, (long long)a->P * a->max_out, a->max_in, ws + space.w3) : nullptr;
+  rc = k.launch(st);
+  if (rc) return rc;
   if (a->dx) {
     p.c = a->dx;
-    rc = bf16 ? ragged_bf16<RAGGED_DGRAD>(p, g, ld, a->w, a->w_stride, nullptr, st)
-              : ragged_f32<RAGGED_DGRAD>(p, g, ld, a->w, a->w_stride, st);
+    p.a_part = gc;
+    p.b_part = xc;
+    rc = ragged_product<RAGGED_DGRAD, true>(p, g3, 3 * gc, w3, 3 * xc, nullptr, st);
     if (rc) return rc;
   }
-  if (a->dw) {
-    p.c = a->dw;
-    rc = bf16 ? ragged_bf16<RAGGED_WGRAD>(p, a->x, a->x_stride, g, ld, parts, st)
-              : ragged_f32<RAGGED_WGRAD>(p, a->x, a->x_stride, g, ld, st);
-    if (rc) return rc;
-  }
-  return TP_OK;
+  if (!a->dw) return TP_OK;
+  p.c = a->dw;
+  p.a_part = xc;
+  p.b_part = gc;
+  return ragged_product<RAGGED_WGRAD, true>(p, x3, 3 * xc, g3, 3 * gc, parts, st);
 }
 
 int32_t tp_fp4_pitch(int32_t K) { return (K + 31) / 32 * 16; }

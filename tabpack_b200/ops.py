@@ -1323,6 +1323,10 @@ def ragged_linear_forward(x: Tensor, weight: Tensor, bias: Tensor | None, offset
         w, ws = _ragged_weight(weight, device)
         a = _lib.RaggedLinearArgs(P, K, N, code, R, offsets.data_ptr(), _ptr(inf), _ptr(outf), int(relu), x.data_ptr(),
                                   xs, w.data_ptr(), ws, _ptr(bias), y.data_ptr())
+        if code == TP_DTYPE_F32:
+            a.workspace_bytes = need = load().tp_ragged_linear_workspace_size(ctypes.byref(a))
+            scratch = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=x.device)
+            a.workspace = scratch.data_ptr()
         _call('tp_ragged_linear_forward', a, device)
     return y
 
