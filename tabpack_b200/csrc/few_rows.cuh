@@ -32,6 +32,14 @@ struct FewArgs {
   int atoms;
 };
 
+// Contiguous bytes (a multiple of 16, on 16-byte boundaries) into shared memory.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 template <int KIND>
 struct FewCfg {
   static constexpr bool FP4 = KIND != FEW_BF16;
@@ -174,11 +182,11 @@ __global__ void __launch_bounds__(128, 2)
         const uint32_t a_base = smem_u32(smA + s * Cfg::A_BYTES), b_base = smem_u32(smB + s * Cfg::B_BYTES);
         if constexpr (Cfg::FP4) {
           constexpr int FORMAT = KIND == FEW_NV ? FP4_NV : FP4_MX;
-          const uint32_t sa = smem_u32(smSA + s * Cfg::S_BYTES), sb = smem_u32(smSB + s * Cfg::S_BYTES);
+          const uint64_t sa = scale_desc(smem_u32(smSA + s * Cfg::S_BYTES)), sb = scale_desc(smem_u32(smSB + s * Cfg::S_BYTES));
 #pragma unroll
           for (int j = 0; j < Cfg::ATOMS; ++j) {
-            tmem_copy_scales(tmem_base + Cfg::SA_COL + 4 * j, sa + 512 * j);
-            tmem_copy_scales(tmem_base + Cfg::SB_COL + 4 * j, sb + 512 * j);
+            tmem_copy_scales(tmem_base + Cfg::SA_COL + 4 * j, sa + 32 * j);
+            tmem_copy_scales(tmem_base + Cfg::SB_COL + 4 * j, sb + 32 * j);
           }
           // 64 rows are two of a scale tile's four columns
           const uint32_t shift = (uint32_t)(local / 64 & 1) * 2u;

@@ -338,12 +338,9 @@ struct Fp4Problem {
   int K, N;
   const int32_t* in_f;   // (P) or null
   const int32_t* out_f;  // (P) or null
-  const uint8_t* x_scales;
   const float* x_row;
-  const uint8_t* w_scales;  // (P, ceil(N / 128), atoms, 512)
-  const float* w_row;       // (P, N)
-  int atoms;                // of 512 bytes per 128 rows of x or w
-  const float* bias;        // (P, N) or null
+  const float* w_row;  // (P, N)
+  const float* bias;   // (P, N) or null
   int relu;
   void* y;  // (rows of y, N)
   int y_f32, y_vec;
@@ -379,20 +376,13 @@ struct Fp4Cfg {
   static_assert(SMEM_BYTES <= 227 * 1024, "fits an SM");
 };
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
+// Descriptor of 128 rows' scales in shared memory: 32 x 16 bytes, 8-row groups 128 bytes apart, no swizzle.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
 }
-
-// 128 rows' scales (32 x 16 bytes) into four columns of tensor memory, the same in each quarter of the lanes.
-__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t saddr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-  d |= (uint64_t)(128 >> 4) << 32;  // 8-row groups 128 bytes apart, no swizzle
-  d |= (uint64_t)1 << 46;
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+// They go into four columns of tensor memory, the same in each quarter of the lanes.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 template <int FORMAT>
@@ -424,7 +414,8 @@ __device__ __forceinline__ uint32_t idesc_fp4(int n, uint32_t id) {
 
 template <int BN, int FORMAT>
 __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
-    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Fp4Problem pr) {
+    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB, const Fp4Problem pr) {
   using Cfg = Fp4Cfg<BN, FORMAT>;
   extern __shared__ uint8_t dyn_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
@@ -486,12 +477,14 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
     mbar_init(done_bar, 1);
     for (int i = 0; i < TRING; ++i) {
       mbar_init(&tr_full[i], 1);
-      mbar_init(&tr_empty[i], 2 + Cfg::EPI_WARPS);
+      mbar_init(&tr_empty[i], 3 + Cfg::EPI_WARPS);  // producers, MMA warp, epilogue warps
     }
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
+    prefetch_tmap(&tmSA);
+    prefetch_tmap(&tmSB);
   }
   if (warp == 1) tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
   tc_fence_before();
@@ -499,9 +492,16 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------ producer
+  if (warp == 0 || warp == 3) {
+    // ------------------------------------------------------------------ producers: x by warp 0, w by warp 3, each with
+    // its scales (a copy takes one thread about 190 cycles, a stage's products 512)
     if (lane == 0) {
+      const bool is_a = warp == 0;
+      const CUtensorMap* map = is_a ? &tmA : &tmB;
+      const CUtensorMap* scale_map = is_a ? &tmSA : &tmSB;
+      uint8_t* const to = is_a ? smA : smB;
+      uint8_t* const scale_to = is_a ? smSA : smSB;
+      const int bytes = is_a ? Cfg::A_BYTES : Cfg::B_BYTES, scale_bytes = is_a ? Cfg::SA_BYTES : Cfg::SB_BYTES;
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -510,22 +510,17 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
         if (t.kind == FT_END) break;
         if (t.kind != FT_MMA) continue;
         const int kblocks = k_blocks(t.member);
-        const uint8_t* sa = pr.x_scales + (long long)t.x_tile * pr.atoms * 512;
-        const int sb_tile = t.nt * BN / 128;
-        const uint8_t* sb = pr.w_scales + ((long long)t.member * n_sb_tiles + sb_tile) * pr.atoms * 512;
-        const int sb_n = min(Cfg::SB_TILES, n_sb_tiles - sb_tile);
+        const int row = is_a ? t.x_row : t.nt * BN, plane = is_a ? 0 : t.member;
+        const int tile = is_a ? t.x_tile : t.member * n_sb_tiles + t.nt * BN / 128;
         for (int kb = 0; kb < kblocks; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&full[stage], Cfg::A_BYTES + Cfg::B_BYTES + Cfg::SA_BYTES + sb_n * Cfg::ATOMS * 512);
-          tma_load_3d(smA + stage * Cfg::A_BYTES, &tmA, &full[stage], kb * 128, t.x_row, 0);
-          tma_load_3d(smB + stage * Cfg::B_BYTES, &tmB, &full[stage], kb * 128, t.nt * BN, t.member);
-          bulk_load(smSA + stage * Cfg::SA_BYTES, sa + kb * Cfg::ATOMS * 512, Cfg::ATOMS * 512, &full[stage]);
-          for (int c = 0; c < sb_n; ++c)
-            bulk_load(smSB + stage * Cfg::SB_BYTES + c * Cfg::ATOMS * 512,
-                      sb + ((long long)c * pr.atoms + kb * Cfg::ATOMS) * 512, Cfg::ATOMS * 512, &full[stage]);
+          // (the bytes of both are announced by the first; the others' may arrive before)
+          if (is_a) mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
+          tma_load_3d(to + stage * bytes, map, &full[stage], kb * 128, row, plane);
+          tma_load_3d(scale_to + stage * scale_bytes, scale_map, &full[stage], 0, kb * 2 * Cfg::ATOMS, tile);
           if (++stage == Cfg::STAGES) {
             stage = 0;
             phase ^= 1u;
@@ -539,40 +534,43 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
+      // descriptors of the first stage; the address field counts 16 bytes
+      const uint64_t adesc0 = smem_desc_sw128(smem_u32(smA), 16, 1024), bdesc0 = smem_desc_sw128(smem_u32(smB), 16, 1024);
+      const uint64_t sadesc0 = scale_desc(smem_u32(smSA)), sbdesc0 = scale_desc(smem_u32(smSB));
+      const uint32_t sa_tmem = tmem_base + Cfg::SA_COL, sb_tmem = tmem_base + Cfg::SB_COL;
       for (int k = 0; ok; ++k) {
         const Fp4Tile t = ring_read(k, false);
         if (t.kind == FT_END) break;
         if (t.kind != FT_MMA) continue;
         const int n_mma = min(BN, (t.n_valid - t.nt * BN + 15) & ~15);
+        const uint32_t idesc[2] = {idesc_fp4<FORMAT>(n_mma, 0), idesc_fp4<FORMAT>(n_mma, FORMAT == FP4_NV ? 0 : 2)};
         const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
         // tiles of 64 columns take one half of a scale tile of 128
-        const uint32_t sb_shift = BN == 64 ? (uint32_t)(t.nt & 1) * 2u : 0u;
+        const uint32_t sb_at = sb_tmem + (BN == 64 ? (uint32_t)(t.nt & 1) * 2u : 0u);
+        const int kblocks = k_blocks(t.member);
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, abort_flag)) break;
         tc_fence_after();
-        const int kblocks = k_blocks(t.member);
         for (int kb = 0; kb < kblocks; ++kb) {
           if (!mbar_wait(&full[stage], phase, abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smSA + stage * Cfg::SA_BYTES), sb = smem_u32(smSB + stage * Cfg::SB_BYTES);
-#pragma unroll
-          for (int i = 0; i < Cfg::ATOMS; ++i) tmem_copy_scales(tmem_base + Cfg::SA_COL + 4 * i, sa + 512 * i);
+          const uint64_t ad = adesc0 + (uint64_t)(stage * (Cfg::A_BYTES / 16)), bd = bdesc0 + (uint64_t)(stage * (Cfg::B_BYTES / 16));
+          const uint64_t sad = sadesc0 + (uint64_t)(stage * (Cfg::SA_BYTES / 16)), sbd = sbdesc0 + (uint64_t)(stage * (Cfg::SB_BYTES / 16));
           // a product's columns of w take consecutive columns of scales: tile c of step i at (i * tiles + c) * 4
 #pragma unroll
-          for (int i = 0; i < Cfg::ATOMS; ++i)
+          for (int i = 0; i < Cfg::ATOMS; ++i) {
+            tmem_copy_scales(sa_tmem + 4 * i, sad + 32 * i);
 #pragma unroll
             for (int c = 0; c < Cfg::SB_TILES; ++c)
-              tmem_copy_scales(tmem_base + Cfg::SB_COL + 4 * (i * Cfg::SB_TILES + c), sb + 512 * (c * Cfg::ATOMS + i));
-          const uint32_t a_base = smem_u32(smA + stage * Cfg::A_BYTES), b_base = smem_u32(smB + stage * Cfg::B_BYTES);
+              tmem_copy_scales(sb_tmem + 4 * (i * Cfg::SB_TILES + c), sbd + 32 * (c * Cfg::ATOMS + i));
+          }
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
             const int i = FORMAT == FP4_NV ? s : s >> 1;
-            const uint32_t id = FORMAT == FP4_NV ? 0u : (uint32_t)(s & 1) * 2u;
-            umma_fp4<FORMAT>(d_tmem, smem_desc_sw128(a_base + s * 32, 16, 1024), smem_desc_sw128(b_base + s * 32, 16, 1024),
-                             idesc_fp4<FORMAT>(n_mma, id), tmem_base + Cfg::SA_COL + 4 * i,
-                             tmem_base + Cfg::SB_COL + 4 * i * Cfg::SB_TILES + sb_shift, (kb | s) != 0 ? 1u : 0u);
+            umma_fp4<FORMAT>(d_tmem, ad + 2 * s, bd + 2 * s, idesc[s & 1], sa_tmem + 4 * i, sb_at + 4 * i * Cfg::SB_TILES,
+                             (kb | s) != 0 ? 1u : 0u);
           }
           umma_commit(&empty[stage]);
           if (++stage == Cfg::STAGES) {

@@ -240,7 +240,30 @@ int make_map_ld(CUtensorMap* map, CUtensorMapDataType type, int size, const void
   return TP_OK;
 }
 
+// Scale tiles (atoms of 512 bytes, row tile by row tile) as rows of 256 bytes, in boxes of `rows` rows of `tiles` tiles.
+int make_scale_map(CUtensorMap* map, const void* ptr, int atoms, long long row_tiles, int rows, int tiles) {
+  auto enc = encode_fn();
+  if (!enc) return fail(TP_EUNSUPPORTED, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {64, (cuuint64_t)atoms * 2, (cuuint64_t)row_tiles};
+  cuuint64_t strides[2] = {256, (cuuint64_t)atoms * 512};
+  cuuint32_t box[3] = {64, (cuuint32_t)rows, (cuuint32_t)tiles};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, const_cast<void*>(ptr), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(TP_EINVAL, "cuTensorMapEncodeTiled failed (%d) for scales", (int)r);
+  return TP_OK;
+}
+
 constexpr int32_t MAX_WIDTH = 1 << 24;
+
+// Columns of a tile: narrower ones while they still fit the SMs at once.  (Two rounds of narrow tiles take as long as
+// one of wide ones, which read less.)
+int tile_columns(long long row_tiles, int cols) {
+  int bn = 256;
+  while (bn > 64 && row_tiles * ((cols + bn / 2 - 1) / (bn / 2)) <= device_info().sms) bn /= 2;
+  return bn;
+}
 
 int check_ragged(const tp_ragged_linear_args* a) {
   if (!a) return fail(TP_EINVAL, "null ragged linear arguments");
@@ -331,8 +354,7 @@ RaggedPlan ragged_plan(int mode, int P, int64_t R, int in, int out) {
   }
   // tiles along the rows: every member that has rows ends in a partial one
   const long long m_tiles = mode == RAGGED_WGRAD ? (long long)P * ((in + 127) / 128) : std::max(used, R / 128 + used / 2);
-  // the widest tile that still gives every SM one
-  while (plan.bn > 64 && m_tiles * ((cols + plan.bn - 1) / plan.bn) < sms) plan.bn /= 2;
+  plan.bn = tile_columns(m_tiles, cols);
   if (mode == RAGGED_WGRAD) {
     // parts of 512 rows at least, as many as the SMs take at once, 256 MB of results at most
     const long long tiles = m_tiles * ((cols + plan.bn - 1) / plan.bn);
@@ -549,13 +571,13 @@ int launch_values(const Fp4ValuesArgs& k, bool vec, cudaStream_t st) {
 }
 
 template <int BN, int FORMAT>
-int launch_fp4(Fp4Problem p, const CUtensorMap& ma, const CUtensorMap& mb, long long tiles, cudaStream_t st) {
+int launch_fp4(const Fp4Problem& p, const CUtensorMap (&m)[4], long long tiles, cudaStream_t st) {
   using Cfg = Fp4Cfg<BN, FORMAT>;
   int rc = allow_smem<fp4_gemm_kernel<BN, FORMAT>>(Cfg::SMEM_BYTES);
   if (rc) return rc;
   const int grid = (int)std::min<long long>(std::max<long long>(tiles, 1), device_info().sms);
   TP_PROF(TP_PROF_FWD, st);
-  fp4_gemm_kernel<BN, FORMAT><<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(ma, mb, p);
+  fp4_gemm_kernel<BN, FORMAT><<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(m[0], m[1], m[2], m[3], p);
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;
 }
@@ -872,11 +894,9 @@ int tp_fp4_linear_forward(const tp_fp4_linear_args* a, void* stream) {
   p.N = a->N;
   p.in_f = a->in_features;
   p.out_f = a->out_features;
-  p.x_scales = a->x_scales;
   p.x_row = a->x_row_scale;
-  p.w_scales = a->w_scales;
   p.w_row = a->w_row_scale;
-  p.atoms = tp_fp4_scale_tiles(a->K, a->format);
+  const int atoms = tp_fp4_scale_tiles(a->K, a->format);
   p.bias = a->bias;
   p.relu = a->relu;
   p.y = a->y;
@@ -902,7 +922,7 @@ int tp_fp4_linear_forward(const tp_fp4_linear_args* a, void* stream) {
     f.x_row = a->x_row_scale;
     f.w_scales = a->w_scales;
     f.w_row = a->w_row_scale;
-    f.atoms = p.atoms;
+    f.atoms = atoms;
     rc = make_map_ld(&ma, T, 1, a->w_codes, pitch, a->N, a->P, pitch, 128, 128);
     if (!rc) rc = make_map_ld(&mb, T, 1, a->x_codes, pitch, a->rows, 1, pitch, 128, FewCfg<FEW_NV>::BN);
     if (rc) return rc;
@@ -910,19 +930,24 @@ int tp_fp4_linear_forward(const tp_fp4_linear_args* a, void* stream) {
   }
   const long long m_tiles = p.groups.offsets ? std::max<long long>(std::min<long long>(a->P, rows), rows / 128 + std::min<long long>(a->P, rows) / 2)
                                              : (long long)a->P * ((p.groups.B + 127) / 128);
-  int bn = 256;
-  while (bn > 64 && m_tiles * ((a->N + bn - 1) / bn) < device_info().sms) bn /= 2;
+  const int bn = tile_columns(m_tiles, a->N);
   p.n_tiles = (a->N + bn - 1) / bn;
   const long long most = (p.groups.offsets ? rows / 128 + a->P + 2 : m_tiles) * p.n_tiles;
   if (most > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many tiles");
-  rc = make_map_ld(&ma, T, 1, a->x_codes, pitch, a->rows, 1, pitch, 128, 128);
-  if (!rc) rc = make_map_ld(&mb, T, 1, a->w_codes, pitch, a->N, a->P, pitch, 128, bn);
+  CUtensorMap m[4];
+  rc = make_map_ld(&m[0], T, 1, a->x_codes, pitch, a->rows, 1, pitch, 128, 128);
+  if (!rc) rc = make_map_ld(&m[1], T, 1, a->w_codes, pitch, a->N, a->P, pitch, 128, bn);
+  // a stage's scales: two or four tiles of 512 bytes as rows of 256, of one or two tiles of 128 rows
+  const long long x_tiles = a->x_shared ? (a->rows + 127) / 128 : fp4_row_tiles(p.groups);
+  const int step = a->format == TP_FP4_NV ? 8 : 4;
+  if (!rc) rc = make_scale_map(&m[2], a->x_scales, atoms, x_tiles, step, 1);
+  if (!rc) rc = make_scale_map(&m[3], a->w_scales, atoms, (long long)a->P * ((a->N + 127) / 128), step, bn == 256 ? 2 : 1);
   if (rc) return rc;
   const bool nv = a->format == TP_FP4_NV;
   switch (bn) {
-    case 256: return nv ? launch_fp4<256, FP4_NV>(p, ma, mb, most, st) : launch_fp4<256, FP4_MX>(p, ma, mb, most, st);
-    case 128: return nv ? launch_fp4<128, FP4_NV>(p, ma, mb, most, st) : launch_fp4<128, FP4_MX>(p, ma, mb, most, st);
-    default: return nv ? launch_fp4<64, FP4_NV>(p, ma, mb, most, st) : launch_fp4<64, FP4_MX>(p, ma, mb, most, st);
+    case 256: return nv ? launch_fp4<256, FP4_NV>(p, m, most, st) : launch_fp4<256, FP4_MX>(p, m, most, st);
+    case 128: return nv ? launch_fp4<128, FP4_NV>(p, m, most, st) : launch_fp4<128, FP4_MX>(p, m, most, st);
+    default: return nv ? launch_fp4<64, FP4_NV>(p, m, most, st) : launch_fp4<64, FP4_MX>(p, m, most, st);
   }
 }
 

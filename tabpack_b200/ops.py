@@ -722,10 +722,15 @@ def binary_roc_auc(scores: Tensor, labels: Tensor, workspace: Tensor | None = No
     return out
 
 
+_functions: dict = {}
+
+
 def _call(name: str, args, device: int) -> None:
     """`name(args)` on the current stream of device number `device`, whichever device is current.
     (The raw stream handle: building a `torch.cuda.Stream` takes as long as the launch.)"""
-    fn = getattr(load(), name)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(load(), name)
     if device == torch._C._cuda_getDevice():
         check(fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device)), name)
     else:
