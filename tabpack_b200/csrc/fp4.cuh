@@ -352,15 +352,19 @@ struct Fp4Tile {
   int kind, member, x_row, y_row, rows, nt, x_tile, n_valid;
 };
 
-template <int BN_, int FORMAT>
+template <int BN_, int FORMAT, bool PAIR_ = false>
 struct Fp4Cfg {
+  static constexpr bool PAIR = PAIR_;
+  static_assert(!PAIR || BN_ == 256, "pairs take tiles of 256 columns");
   static constexpr int BM = 128, BN = BN_, BK = 256;
+  static constexpr int TILE_M = PAIR ? 256 : 128;
+  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;  // rows of w that a CTA stages (of their scales, all of the tile's)
   static constexpr int ATOMS = FORMAT == FP4_NV ? 4 : 2;  // scale tiles of 128 rows a stage
-  static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128;
+  static constexpr int A_BYTES = BM * 128, B_BYTES = B_ROWS * 128;
   static constexpr int SB_TILES = BN > 128 ? BN / 128 : 1;
   static constexpr int SA_BYTES = ATOMS * 512, SB_BYTES = SB_TILES * ATOMS * 512;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;
-  static constexpr int STAGES = BN == 256 ? 3 : BN == 128 ? 5 : 6;
+  static constexpr int STAGES = PAIR ? 4 : BN == 256 ? 3 : BN == 128 ? 5 : 6;
   static constexpr int ACCS = BN == 256 ? 1 : 2;
   static constexpr int SA_COL = ACCS * BN, SB_COL = SA_COL + 16;  // tensor memory columns of the scales
   static constexpr int TMEM_COLS = BN == 64 ? 256 : 512;
@@ -381,42 +385,49 @@ __device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
 }
 // They go into four columns of tensor memory, the same in each quarter of the lanes.
+// PAIR: in both CTAs, each from its own shared memory.
+template <bool PAIR = false>
 __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  if constexpr (PAIR)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
-template <int FORMAT>
+#define TP_UMMA_FP4(group, kind)                                                                                      \
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n tcgen05.mma.cta_group::" group ".kind::" kind                \
+               " [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d_tmem),                                                 \
+               "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)                                \
+               : "memory")
+// A pair's products: 128 rows of A and half of B's from each CTA, A's scales of its own rows and B's of all columns in
+// each CTA's tensor memory.
+template <int FORMAT, bool PAIR = false>
 __device__ __forceinline__ void umma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa,
                                          uint32_t sb, uint32_t accumulate) {
-  if constexpr (FORMAT == FP4_NV)
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(
-            d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-        : "memory");
+  if constexpr (PAIR && FORMAT == FP4_NV)
+    TP_UMMA_FP4("2", "mxf4nvf4.block_scale.scale_vec::4X");
+  else if constexpr (PAIR)
+    TP_UMMA_FP4("2", "mxf4.block_scale.scale_vec::2X");
+  else if constexpr (FORMAT == FP4_NV)
+    TP_UMMA_FP4("1", "mxf4nvf4.block_scale.scale_vec::4X");
   else
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(
-            d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-        : "memory");
+    TP_UMMA_FP4("1", "mxf4.block_scale.scale_vec::2X");
 }
+#undef TP_UMMA_FP4
 
-// Instruction descriptor: A and B e2m1, M = 128; scales e4m3 (nvfp4) or powers of two (mxfp4), `id` the half of a
-// scale word that this product takes (mxfp4: 0 or 2).
+// Instruction descriptor: A and B e2m1; scales e4m3 (nvfp4) or powers of two (mxfp4), `id` the half of a scale word
+// that this product takes (mxfp4: 0 or 2).
 template <int FORMAT>
-__device__ __forceinline__ uint32_t idesc_fp4(int n, uint32_t id) {
+__device__ __forceinline__ uint32_t idesc_fp4(int n, uint32_t id, int m = 128) {
   return (id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((FORMAT == FP4_MX ? 1u : 0u) << 23) |
-         (1u << 27) | (id << 29);
+         ((uint32_t)(m >> 7) << 27) | (id << 29);
 }
 
-template <int BN, int FORMAT>
-__global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
+template <int BN, int FORMAT, bool PAIR>
+__global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB, const Fp4Problem pr) {
-  using Cfg = Fp4Cfg<BN, FORMAT>;
+  using Cfg = Fp4Cfg<BN, FORMAT, PAIR>;
   extern __shared__ uint8_t dyn_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
   uint8_t* smA = smem;
@@ -437,6 +448,8 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
   volatile int* ring = reinterpret_cast<volatile int*>(ctrl + 256);
   static_assert(8 * (2 * Cfg::STAGES + 5 + 2 * TRING) + 8 <= 256 && 256 + 32 * TRING <= Cfg::CTRL_BYTES, "control block");
   const int warp = warp_id(), lane = lane_id();
+  const int rank = PAIR ? (int)cluster_ctarank() : 0;
+  const int worker = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, workers = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
   const int n_sb_tiles = (pr.N + 127) / 128;  // scale tiles of a member's rows of w
 
   // (`whole`: all lanes of the warp read, and lane 0 frees the slot once they have)
@@ -460,6 +473,11 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
     if (!whole || lane == 0) mbar_arrive(&tr_empty[s]);
     return t;
   };
+  // columns that a tile multiplies (16 a CTA at least)
+  auto columns = [&](const Fp4Tile& t) {
+    const int left = t.n_valid - t.nt * BN;
+    return min(BN, PAIR ? (left + 31) & ~31 : (left + 15) & ~15);
+  };
   auto k_blocks = [&](int member) {
     const int k = pr.in_f ? min(__ldg(pr.in_f + member), pr.K) : pr.K;
     return (k + Cfg::BK - 1) / Cfg::BK;
@@ -472,12 +490,12 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], Cfg::EPI_WARPS);
+      mbar_init(&tempty[i], PAIR ? 2 * Cfg::EPI_WARPS : Cfg::EPI_WARPS);  // the leader's counts both CTAs
     }
     mbar_init(done_bar, 1);
     for (int i = 0; i < TRING; ++i) {
       mbar_init(&tr_full[i], 1);
-      mbar_init(&tr_empty[i], 3 + Cfg::EPI_WARPS);  // producers, MMA warp, epilogue warps
+      mbar_init(&tr_empty[i], (rank == 0 ? 3 : 2) + Cfg::EPI_WARPS);  // producers, MMA warp, epilogue warps
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -486,9 +504,15 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
     prefetch_tmap(&tmSA);
     prefetch_tmap(&tmSB);
   }
-  if (warp == 1) tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+  if (warp == 1) {
+    if constexpr (PAIR)
+      tmem_alloc_pair(tmem_slot, Cfg::TMEM_COLS);
+    else
+      tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+  }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the peer's barriers are initialised before any remote arrive
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
@@ -501,6 +525,7 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
       const CUtensorMap* scale_map = is_a ? &tmSA : &tmSB;
       uint8_t* const to = is_a ? smA : smB;
       uint8_t* const scale_to = is_a ? smSA : smSB;
+      const uint32_t leader0 = PAIR ? mapa_shared(smem_u32(full), 0) : 0;
       const int bytes = is_a ? Cfg::A_BYTES : Cfg::B_BYTES, scale_bytes = is_a ? Cfg::SA_BYTES : Cfg::SB_BYTES;
       int stage = 0;
       uint32_t phase = 0;
@@ -510,17 +535,24 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
         if (t.kind == FT_END) break;
         if (t.kind != FT_MMA) continue;
         const int kblocks = k_blocks(t.member);
-        const int row = is_a ? t.x_row : t.nt * BN, plane = is_a ? 0 : t.member;
-        const int tile = is_a ? t.x_tile : t.member * n_sb_tiles + t.nt * BN / 128;
+        const int row = is_a ? t.x_row + rank * Cfg::BM : t.nt * BN + (PAIR ? rank * (columns(t) / 2) : 0);
+        const int plane = is_a ? 0 : t.member;
+        const int tile = is_a ? t.x_tile + rank : t.member * n_sb_tiles + t.nt * BN / 128;
         for (int kb = 0; kb < kblocks; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag)) {
             ok = false;
             break;
           }
           // (the bytes of both are announced by the first; the others' may arrive before)
-          if (is_a) mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
-          tma_load_3d(to + stage * bytes, map, &full[stage], kb * 128, row, plane);
-          tma_load_3d(scale_to + stage * scale_bytes, scale_map, &full[stage], 0, kb * 2 * Cfg::ATOMS, tile);
+          if constexpr (PAIR) {  // both CTAs' bytes complete on the leader's barrier
+            if (is_a && rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * Cfg::STAGE_BYTES);
+            tma_load_3d_pair(to + stage * bytes, map, leader0 + 8u * stage, kb * 128, row, plane);
+            tma_load_3d_pair(scale_to + stage * scale_bytes, scale_map, leader0 + 8u * stage, 0, kb * 2 * Cfg::ATOMS, tile);
+          } else {
+            if (is_a) mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
+            tma_load_3d(to + stage * bytes, map, &full[stage], kb * 128, row, plane);
+            tma_load_3d(scale_to + stage * scale_bytes, scale_map, &full[stage], 0, kb * 2 * Cfg::ATOMS, tile);
+          }
           if (++stage == Cfg::STAGES) {
             stage = 0;
             phase ^= 1u;
@@ -529,8 +561,8 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA
-    if (lane == 0) {
+    // ------------------------------------------------------------------ MMA (a pair's leader fills both CTAs' TMEM)
+    if (lane == 0 && rank == 0) {
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
@@ -542,8 +574,9 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
         const Fp4Tile t = ring_read(k, false);
         if (t.kind == FT_END) break;
         if (t.kind != FT_MMA) continue;
-        const int n_mma = min(BN, (t.n_valid - t.nt * BN + 15) & ~15);
-        const uint32_t idesc[2] = {idesc_fp4<FORMAT>(n_mma, 0), idesc_fp4<FORMAT>(n_mma, FORMAT == FP4_NV ? 0 : 2)};
+        const int n_mma = columns(t);
+        const uint32_t idesc[2] = {idesc_fp4<FORMAT>(n_mma, 0, Cfg::TILE_M),
+                                   idesc_fp4<FORMAT>(n_mma, FORMAT == FP4_NV ? 0 : 2, Cfg::TILE_M)};
         const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
         // tiles of 64 columns take one half of a scale tile of 128
         const uint32_t sb_at = sb_tmem + (BN == 64 ? (uint32_t)(t.nt & 1) * 2u : 0u);
@@ -561,31 +594,40 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
           // a product's columns of w take consecutive columns of scales: tile c of step i at (i * tiles + c) * 4
 #pragma unroll
           for (int i = 0; i < Cfg::ATOMS; ++i) {
-            tmem_copy_scales(sa_tmem + 4 * i, sad + 32 * i);
+            tmem_copy_scales<PAIR>(sa_tmem + 4 * i, sad + 32 * i);
 #pragma unroll
             for (int c = 0; c < Cfg::SB_TILES; ++c)
-              tmem_copy_scales(sb_tmem + 4 * (i * Cfg::SB_TILES + c), sbd + 32 * (c * Cfg::ATOMS + i));
+              tmem_copy_scales<PAIR>(sb_tmem + 4 * (i * Cfg::SB_TILES + c), sbd + 32 * (c * Cfg::ATOMS + i));
           }
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
             const int i = FORMAT == FP4_NV ? s : s >> 1;
-            umma_fp4<FORMAT>(d_tmem, ad + 2 * s, bd + 2 * s, idesc[s & 1], sa_tmem + 4 * i, sb_at + 4 * i * Cfg::SB_TILES,
+            umma_fp4<FORMAT, PAIR>(d_tmem, ad + 2 * s, bd + 2 * s, idesc[s & 1], sa_tmem + 4 * i, sb_at + 4 * i * Cfg::SB_TILES,
                              (kb | s) != 0 ? 1u : 0u);
           }
-          umma_commit(&empty[stage]);
+          if constexpr (PAIR)
+            umma_commit_both(&empty[stage]);
+          else
+            umma_commit(&empty[stage]);
           if (++stage == Cfg::STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
         if (!ok) break;
-        umma_commit(&tfull[acc]);
+        if constexpr (PAIR)
+          umma_commit_both(&tfull[acc]);
+        else
+          umma_commit(&tfull[acc]);
         if (++acc == Cfg::ACCS) {
           acc = 0;
           acc_phase ^= 1u;
         }
       }
-      umma_commit(done_bar);
+      if constexpr (PAIR)
+        umma_commit_pair(smem_u32(done_bar));
+      else
+        umma_commit(done_bar);
       volatile int no_abort = 0;
       mbar_wait(done_bar, 0, &no_abort);
     }
@@ -633,7 +675,7 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
     auto load_groups = [&]() {
       first = end = 0;
       if (g0 + lane < n_groups) group(g0 + lane, first, end);
-      tiles = (end - first + Cfg::BM - 1) / Cfg::BM * pr.n_tiles;
+      tiles = (end - first + Cfg::TILE_M - 1) / Cfg::TILE_M * pr.n_tiles;
       inc = tiles;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -642,7 +684,7 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
       }
     };
     load_groups();
-    for (long long i = blockIdx.x; ok; i += gridDim.x) {
+    for (long long i = worker; ok; i += workers) {
       int sum = __shfl_sync(0xFFFFFFFFu, inc, 31);
       while (i >= before + sum && g0 + 32 < n_groups) {
         before += sum;
@@ -655,17 +697,17 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
       const int who = __ffs(__ballot_sync(0xFFFFFFFFu, local < inc)) - 1;
       const int r = local - __shfl_sync(0xFFFFFFFFu, inc - tiles, who);
       const int f = __shfl_sync(0xFFFFFFFFu, first, who), e = __shfl_sync(0xFFFFFFFFu, end, who);
-      const int mts = (e - f + Cfg::BM - 1) / Cfg::BM;
+      const int mts = (e - f + Cfg::TILE_M - 1) / Cfg::TILE_M;
       t.member = g0 + who;
       t.nt = r / mts;
       const int mt = r - t.nt * mts;
-      t.y_row = f + mt * Cfg::BM;
-      t.x_row = pr.x_shared ? mt * Cfg::BM : t.y_row;
-      t.rows = min(Cfg::BM, e - t.y_row);
+      t.y_row = f + mt * Cfg::TILE_M;
+      t.x_row = pr.x_shared ? mt * Cfg::TILE_M : t.y_row;
+      t.rows = min(Cfg::TILE_M, e - t.y_row);
       t.kind = FT_ZERO;
       t.n_valid = t.x_tile = 0;
       if (t.member < g.P) {
-        t.x_tile = (int)(pr.x_shared ? 0 : fp4_first_tile(g, t.member)) + mt;
+        t.x_tile = (int)(pr.x_shared ? 0 : fp4_first_tile(g, t.member)) + mt * (Cfg::TILE_M / 128);
         t.n_valid = pr.out_f ? min(__ldg(pr.out_f + t.member), pr.N) : pr.N;
         if (t.nt * BN < t.n_valid && k_blocks(t.member) > 0) t.kind = FT_MMA;
       }
@@ -692,8 +734,8 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
       if (t.kind == FT_END) break;
       const int cbase = t.nt * BN + half * WCOLS;
       const int nch = min(NCH, max(0, (pr.N - cbase + 31) / 32));
-      const int rows = t.rows - q * 32;
-      const long long row0 = (long long)t.y_row + q * 32;
+      const int rows = t.rows - rank * Cfg::BM - q * 32;
+      const long long row0 = (long long)t.y_row + rank * Cfg::BM + q * 32;
       const bool mma = t.kind == FT_MMA;
       float rs = 0.f;
       if (mma) {
@@ -703,7 +745,7 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
           sbias[j] = (in && pr.bias) ? __ldg(pr.bias + (long long)t.member * pr.N + cbase + j) : 0.f;
           sscale[j] = in ? __ldg(pr.w_row + (long long)t.member * pr.N + cbase + j) : 0.f;
         }
-        if (lane < rows) rs = __ldg(pr.x_row + (long long)t.x_row + q * 32 + lane);
+        if (lane < rows) rs = __ldg(pr.x_row + (long long)t.x_row + rank * Cfg::BM + q * 32 + lane);
         __syncwarp();
         if (!mbar_wait(&tfull[acc], acc_phase, abort_flag)) break;
         tc_fence_after();
@@ -766,7 +808,12 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
       if (mma) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&tempty[acc]);
+        if (lane == 0) {
+          if constexpr (PAIR)
+            mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));  // the leader's MMA thread waits on it
+          else
+            mbar_arrive(&tempty[acc]);
+        }
         if (++acc == Cfg::ACCS) {
           acc = 0;
           acc_phase ^= 1u;
@@ -777,8 +824,14 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT>::THREADS, 1)
 
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // neither CTA leaves while the other may still signal it
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  if (warp == 1) {
+    if constexpr (PAIR)
+      tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
+    else
+      tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
 }
 
 }  // namespace tp

@@ -141,14 +141,6 @@ __device__ __forceinline__ void ragged_flush(__nv_bfloat16* c, int ld, int vec, 
   }
 }
 
-// Arrive on the mbarrier at this offset in both CTAs of the pair once this thread's MMAs so far have completed.
-__device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
-      "h"((uint16_t)3)
-      : "memory");
-}
-
 // A warp's staged 32 x 16 fp32 values into the result, on top of what it holds (`add`) and with ReLU at last.
 __device__ __forceinline__ void ragged_flush_f32(float* c, int ld, int vec, long long row0, int rows, int col0,
                                                  const uint8_t* stage, int row_bytes, int lane, bool add, bool relu) {

@@ -294,39 +294,48 @@ RaggedProblem ragged_problem(const tp_ragged_linear_args* a) {
   return p;
 }
 
-template <int BN, int MODE, bool PAIR, bool F32>
-int launch_ragged(const RaggedProblem& p, const CUtensorMap& ma, const CUtensorMap& mb, long long tiles, cudaStream_t st) {
-  using Cfg = RaggedCfg<BN, MODE, PAIR, F32>;
-  constexpr auto kern = ragged_gemm_kernel<BN, MODE, PAIR, F32>;
-  int rc = allow_smem<kern>(Cfg::SMEM_BYTES);
+// Launch of a kernel whose CTAs (or CTA pairs) go through tiles: as many as run at once.
+template <auto* KERNEL, bool PAIR>
+int persistent_launch(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, int threads, size_t smem, long long tiles,
+                      cudaStream_t st) {
+  int rc = allow_smem<KERNEL>(smem);
   if (rc) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.blockDim = dim3(Cfg::THREADS);
-  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
-  cfg.stream = st;
+  cfg->blockDim = dim3(threads);
+  cfg->dynamicSmemBytes = smem;
+  cfg->stream = st;
   int workers = device_info().sms;
   if constexpr (PAIR) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg->attrs = attr;
+    cfg->numAttrs = 1;
     static std::atomic<int> pairs[64] = {};
     int dev = 0;
     TP_CUDA_TRY(cudaGetDevice(&dev));
     int n = pairs[dev].load(std::memory_order_relaxed);
     if (n == 0) {
-      cfg.gridDim = dim3(2 * (workers / 2));
-      TP_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+      cfg->gridDim = dim3(2 * (workers / 2));
+      TP_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, KERNEL, cfg));
       if (n <= 0) return fail(TP_EUNSUPPORTED, "no CTA pair of this kernel fits on the device");
       pairs[dev].store(n, std::memory_order_relaxed);
     }
     workers = n;
   }
   const int grid = (int)std::min<long long>(std::max<long long>(tiles, 1), workers);
-  cfg.gridDim = dim3(PAIR ? 2 * grid : grid);
+  cfg->gridDim = dim3(PAIR ? 2 * grid : grid);
+  return TP_OK;
+}
+
+template <int BN, int MODE, bool PAIR, bool F32>
+int launch_ragged(const RaggedProblem& p, const CUtensorMap& ma, const CUtensorMap& mb, long long tiles, cudaStream_t st) {
+  using Cfg = RaggedCfg<BN, MODE, PAIR, F32>;
+  constexpr auto kern = ragged_gemm_kernel<BN, MODE, PAIR, F32>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  int rc = persistent_launch<kern, PAIR>(&cfg, attr, Cfg::THREADS, Cfg::SMEM_BYTES, tiles, st);
+  if (rc) return rc;
   TP_PROF(MODE == RAGGED_FWD ? TP_PROF_FWD : MODE == RAGGED_DGRAD ? TP_PROF_DGRAD : TP_PROF_WGRAD, st);
   TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, ma, mb, p));
   return TP_OK;
@@ -570,16 +579,25 @@ int launch_values(const Fp4ValuesArgs& k, bool vec, cudaStream_t st) {
   return TP_OK;
 }
 
-template <int BN, int FORMAT>
+template <int BN, int FORMAT, bool PAIR>
 int launch_fp4(const Fp4Problem& p, const CUtensorMap (&m)[4], long long tiles, cudaStream_t st) {
-  using Cfg = Fp4Cfg<BN, FORMAT>;
-  int rc = allow_smem<fp4_gemm_kernel<BN, FORMAT>>(Cfg::SMEM_BYTES);
+  using Cfg = Fp4Cfg<BN, FORMAT, PAIR>;
+  constexpr auto kern = fp4_gemm_kernel<BN, FORMAT, PAIR>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  int rc = persistent_launch<kern, PAIR>(&cfg, attr, Cfg::THREADS, Cfg::SMEM_BYTES, tiles, st);
   if (rc) return rc;
-  const int grid = (int)std::min<long long>(std::max<long long>(tiles, 1), device_info().sms);
   TP_PROF(TP_PROF_FWD, st);
-  fp4_gemm_kernel<BN, FORMAT><<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(m[0], m[1], m[2], m[3], p);
-  TP_CUDA_TRY(cudaGetLastError());
+  TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, m[0], m[1], m[2], m[3], p));
   return TP_OK;
+}
+
+template <int FORMAT>
+int dispatch_fp4(const Fp4Problem& p, const CUtensorMap (&m)[4], bool pair, int bn, long long tiles, cudaStream_t st) {
+  if (pair) return launch_fp4<256, FORMAT, true>(p, m, tiles, st);
+  if (bn == 256) return launch_fp4<256, FORMAT, false>(p, m, tiles, st);
+  if (bn == 128) return launch_fp4<128, FORMAT, false>(p, m, tiles, st);
+  return launch_fp4<64, FORMAT, false>(p, m, tiles, st);
 }
 
 // ------------------------------------------------------------------ a few rows a group
@@ -930,25 +948,22 @@ int tp_fp4_linear_forward(const tp_fp4_linear_args* a, void* stream) {
   }
   const long long m_tiles = p.groups.offsets ? std::max<long long>(std::min<long long>(a->P, rows), rows / 128 + std::min<long long>(a->P, rows) / 2)
                                              : (long long)a->P * ((p.groups.B + 127) / 128);
-  const int bn = tile_columns(m_tiles, a->N);
+  // pairs where their 256-row tiles are mostly full and every pair of SMs has one
+  const bool pair = rows / a->P >= 1024 && rows / 256 * ((a->N + 255) / 256) >= device_info().sms / 2;
+  const int bn = pair ? 256 : tile_columns(m_tiles, a->N);
   p.n_tiles = (a->N + bn - 1) / bn;
   const long long most = (p.groups.offsets ? rows / 128 + a->P + 2 : m_tiles) * p.n_tiles;
   if (most > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many tiles");
   CUtensorMap m[4];
   rc = make_map_ld(&m[0], T, 1, a->x_codes, pitch, a->rows, 1, pitch, 128, 128);
-  if (!rc) rc = make_map_ld(&m[1], T, 1, a->w_codes, pitch, a->N, a->P, pitch, 128, bn);
+  if (!rc) rc = make_map_ld(&m[1], T, 1, a->w_codes, pitch, a->N, a->P, pitch, 128, pair ? 128 : bn);
   // a stage's scales: two or four tiles of 512 bytes as rows of 256, of one or two tiles of 128 rows
   const long long x_tiles = a->x_shared ? (a->rows + 127) / 128 : fp4_row_tiles(p.groups);
   const int step = a->format == TP_FP4_NV ? 8 : 4;
   if (!rc) rc = make_scale_map(&m[2], a->x_scales, atoms, x_tiles, step, 1);
   if (!rc) rc = make_scale_map(&m[3], a->w_scales, atoms, (long long)a->P * ((a->N + 127) / 128), step, bn == 256 ? 2 : 1);
   if (rc) return rc;
-  const bool nv = a->format == TP_FP4_NV;
-  switch (bn) {
-    case 256: return nv ? launch_fp4<256, FP4_NV>(p, m, most, st) : launch_fp4<256, FP4_MX>(p, m, most, st);
-    case 128: return nv ? launch_fp4<128, FP4_NV>(p, m, most, st) : launch_fp4<128, FP4_MX>(p, m, most, st);
-    default: return nv ? launch_fp4<64, FP4_NV>(p, m, most, st) : launch_fp4<64, FP4_MX>(p, m, most, st);
-  }
+  return a->format == TP_FP4_NV ? dispatch_fp4<FP4_NV>(p, m, pair, bn, most, st) : dispatch_fp4<FP4_MX>(p, m, pair, bn, most, st);
 }
 
 }  // extern "C"
