@@ -769,15 +769,15 @@ int32_t tp_fp4_scale_tiles(int32_t K, int32_t format);
 int tp_fp4_quantize(const tp_fp4_args* a, void* stream);
 int tp_fp4_values(const tp_fp4_args* a, void* stream);
 
-/* y = relu(q(x) q(w_m)^T + b_m) over rows of x in 4 bits (x.codes, x.scales, x.row_scale as written by tp_fp4_quantize
- * for the same groups) and weights in 4 bits (P groups of N rows, without offsets), sums in fp32.  Groups as in
- * tp_fp4_args; x_shared: every member reads the same `rows` rows (P results of them; offsets NULL).  Rows of no member
- * are zero. */
+/* y = relu(q(x) q(w_m)^T + b_m) over rows of x in 4 bits and weights in 4 bits (P groups of N rows, without offsets), sums
+ * in fp32.  The rows come as codes and scales (as tp_fp4_quantize writes them for the same groups), or as numbers in x
+ * (of type dtype), which the call quantises into its workspace.  Groups as in tp_fp4_args; x_shared: every member reads
+ * the same `rows` rows (P results of them; offsets NULL; in_features do not cut them).  Rows of no member are zero. */
 typedef struct tp_fp4_linear_args {
   int32_t P;
   int32_t K, N;
   int32_t format;
-  int32_t dtype;            /* TP_DTYPE_F32 or TP_DTYPE_BF16: y */
+  int32_t dtype;            /* TP_DTYPE_F32 or TP_DTYPE_BF16: y, x */
   int32_t x_shared;
   int64_t rows;             /* rows of x */
   const int32_t* offsets;
@@ -792,7 +792,12 @@ typedef struct tp_fp4_linear_args {
   const float* bias;        /* (P, N), or NULL */
   int32_t relu;
   void* y;                  /* (rows, N); (P, rows, N) with x_shared */
+  const void* x;            /* (rows, K), or NULL (x_codes, x_scales and x_row_scale are given) */
+  int64_t x_stride;
+  void* workspace;          /* with x: tp_fp4_linear_workspace_size, on a 16-byte boundary */
+  size_t workspace_bytes;
 } tp_fp4_linear_args;
+size_t tp_fp4_linear_workspace_size(const tp_fp4_linear_args* a);
 int tp_fp4_linear_forward(const tp_fp4_linear_args* a, void* stream);
 
 #ifdef __cplusplus

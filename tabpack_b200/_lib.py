@@ -249,7 +249,8 @@ class Fp4LinearArgs(ctypes.Structure):
         ('offsets', ctypes.c_void_p), ('in_features', ctypes.c_void_p), ('out_features', ctypes.c_void_p),
         ('x_codes', ctypes.c_void_p), ('x_scales', ctypes.c_void_p), ('x_row_scale', ctypes.c_void_p),
         ('w_codes', ctypes.c_void_p), ('w_scales', ctypes.c_void_p), ('w_row_scale', ctypes.c_void_p),
-        ('bias', ctypes.c_void_p), ('relu', ctypes.c_int32), ('y', ctypes.c_void_p),
+        ('bias', ctypes.c_void_p), ('relu', ctypes.c_int32), ('y', ctypes.c_void_p), ('x', ctypes.c_void_p),
+        ('x_stride', ctypes.c_int64), ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_size_t),
     ]
 
 
@@ -322,6 +323,7 @@ SIGNATURES = {
     'tp_fp4_scale_tiles': (ctypes.c_int32, [ctypes.c_int32, ctypes.c_int32]),
     'tp_fp4_quantize': (ctypes.c_int, [ctypes.POINTER(Fp4Args), ctypes.c_void_p]),
     'tp_fp4_values': (ctypes.c_int, [ctypes.POINTER(Fp4Args), ctypes.c_void_p]),
+    'tp_fp4_linear_workspace_size': (ctypes.c_size_t, [ctypes.POINTER(Fp4LinearArgs)]),
     'tp_fp4_linear_forward': (ctypes.c_int, [ctypes.POINTER(Fp4LinearArgs), ctypes.c_void_p]),
     'tp_device_error': (ctypes.c_int, []),
     'tp_last_error_string': (ctypes.c_char_p, []),

@@ -541,6 +541,19 @@ Fp4Groups fp4_groups(int32_t P, int64_t rows, const int32_t* offsets) {
   return g;
 }
 
+// The workspace of a 4-bit linear layer that quantises its rows: codes, scales, row scales.
+struct Fp4Space {
+  size_t scales, row_scale, bytes;
+};
+Fp4Space fp4_space(const tp_fp4_linear_args* a) {
+  Fp4Space s{};
+  s.scales = round256((size_t)a->rows * tp_fp4_pitch(a->K));
+  const Fp4Groups g = fp4_groups(a->x_shared ? 1 : a->P, a->rows, a->offsets);
+  s.row_scale = s.scales + (size_t)fp4_row_tiles(g) * tp_fp4_scale_tiles(a->K, a->format) * 512;
+  s.bytes = s.row_scale + (size_t)a->rows * sizeof(float);
+  return s;
+}
+
 Fp4Rows fp4_rows(const tp_fp4_args* a) {
   Fp4Rows r{};
   r.codes = a->codes;
@@ -645,7 +658,7 @@ using namespace tp;
 extern "C" {
 
 size_t tp_route_workspace_size(int64_t rows, int32_t E, int32_t top_k) {
-  if (rows <= 0 || E <= 0 || top_k <= 0) return 0;
+  if (rows <= 0 || E <= 0 || top_k <= 0 || route_plan(rows, top_k).blocks == 1) return 0;
   return ((size_t)route_plan(rows, top_k).blocks * (2 * (size_t)E + 1) + E + 1) * 4;
 }
 
@@ -656,12 +669,12 @@ int tp_route_forward(const tp_route_args* a, void* stream) {
   if (rc) return rc;
   if (!a->position || !a->offsets || !a->importance) return fail(TP_EINVAL, "null routing output");
   const size_t need = tp_route_workspace_size(a->rows, a->E, a->top_k);
-  if (!a->workspace || a->workspace_bytes < need)
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need))
     return fail(TP_EINVAL, "routing workspace of %zu bytes is smaller than the %zu needed", a->workspace_bytes, need);
   RouteArgs k = route_args(a);
-  k.counts = static_cast<int32_t*>(a->workspace);
-  k.partial = reinterpret_cast<float*>(k.counts + (size_t)k.blocks * (a->E + 1));
-  k.totals = k.counts + (size_t)k.blocks * (2 * (size_t)a->E + 1);
+  k.counts = static_cast<int32_t*>(a->workspace);  // (unused with one block)
+  if (need > 0) k.partial = reinterpret_cast<float*>(k.counts + (size_t)k.blocks * (a->E + 1));
+  if (need > 0) k.totals = k.counts + (size_t)k.blocks * (2 * (size_t)a->E + 1);
   rc = a->dtype == TP_DTYPE_BF16 ? dispatch_route<__nv_bfloat16>(k, false, st) : dispatch_route<float>(k, false, st);
   if (rc) return rc;
   TP_CUDA_TRY(cudaGetLastError());
@@ -890,6 +903,11 @@ int tp_fp4_values(const tp_fp4_args* a, void* stream) {
   return TP_OK;
 }
 
+size_t tp_fp4_linear_workspace_size(const tp_fp4_linear_args* a) {
+  if (!a || !a->x || a->P <= 0 || a->K <= 0 || a->rows <= 0) return 0;
+  return fp4_space(a).bytes;
+}
+
 int tp_fp4_linear_forward(const tp_fp4_linear_args* a, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!a) return fail(TP_EINVAL, "null 4-bit linear arguments");
@@ -899,12 +917,41 @@ int tp_fp4_linear_forward(const tp_fp4_linear_args* a, void* stream) {
   if (a->x_shared && a->offsets) return fail(TP_EINVAL, "shared rows have no offsets");
   if (a->x_shared && a->rows * a->P >= (1ll << 31) - 256) return fail(TP_EINVAL, "too many rows of y");
   if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad 4-bit linear dtype");
+  tp_fp4_linear_args q = *a;
+  if (a->x) {
+    const Fp4Space space = fp4_space(a);
+    if (!a->workspace || a->workspace_bytes < space.bytes || !aligned16(a->workspace))
+      return fail(TP_EINVAL, "4-bit linear workspace of %zu bytes is smaller than the %zu needed, or not aligned",
+                  a->workspace_bytes, space.bytes);
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    q.x_codes = ws;
+    q.x_scales = ws + space.scales;
+    q.x_row_scale = reinterpret_cast<const float*>(ws + space.row_scale);
+    a = &q;
+  }
   if (!a->x_codes || !a->x_scales || !a->x_row_scale || !a->w_codes || !a->w_scales || !a->w_row_scale || !a->y)
     return fail(TP_EINVAL, "null 4-bit linear operand or output");
   if (!aligned_to(16, {a->x_codes, a->x_scales, a->w_codes, a->w_scales}) ||
       !aligned_to(4, {a->x_row_scale, a->w_row_scale, a->bias, a->in_features, a->out_features}) ||
       !aligned_to(dtype_size(a->dtype), {a->y}))
     return fail(TP_EALIGN, "codes and scales need 16-byte boundaries");
+  if (a->x) {
+    tp_fp4_args x{};
+    x.P = a->x_shared ? 1 : a->P;
+    x.K = a->K;
+    x.format = a->format;
+    x.dtype = a->dtype;
+    x.rows = a->rows;
+    x.offsets = a->offsets;
+    x.n_features = a->in_features;
+    x.x = a->x;
+    x.x_stride = a->x_stride;
+    x.codes = const_cast<uint8_t*>(a->x_codes);
+    x.scales = const_cast<uint8_t*>(a->x_scales);
+    x.row_scale = const_cast<float*>(a->x_row_scale);
+    rc = tp_fp4_quantize(&x, stream);
+    if (rc) return rc;
+  }
   Fp4Problem p{};
   p.groups = fp4_groups(a->P, a->x_shared ? a->rows * a->P : a->rows, a->offsets);
   p.x_shared = a->x_shared;

@@ -63,7 +63,7 @@ __device__ __forceinline__ float exp_of(float z, float c) {
   return r;
 }
 
-// Shared memory of the gate: hist[E + 1], sums[ROUTE_WARPS][E]; of the places: counts[ROUTE_WARPS][E + 1], base[E + 1].
+// Shared memory of the gate: hist[E + 1], sums[ROUTE_WARPS][E]; of the places: base[E + 1], counts[ROUTE_WARPS][E + 1].
 __host__ __device__ inline size_t route_shared_bytes(int E) { return sizeof(int) * ((size_t)(ROUTE_WARPS + 1) * (E + 1)); }
 
 // Weights and members of the block's rows, their counts per member, and the sums of p.  Instructions bound it, some
@@ -168,12 +168,16 @@ __device__ __forceinline__ void route_gate(const RouteArgs& a, int block, int* s
   for (int v = 0; v < V; ++v)
     if (lane + 32 * v < E) sums[warp * E + lane + 32 * v] = imp[v];
   __syncthreads();
+  // (a single block's sums are the result; its counts stay in shared memory)
   for (int e = threadIdx.x; e <= E; e += blockDim.x) {
-    a.counts[(long long)e * a.blocks + block] = hist[e];
+    if (a.blocks > 1) a.counts[(long long)e * a.blocks + block] = hist[e];
     if (e < E) {
       float s = 0.f;
       for (int w = 0; w < ROUTE_WARPS; ++w) s += sums[w * E + e];
-      a.partial[(long long)e * a.blocks + block] = s;
+      if (a.blocks > 1)
+        a.partial[(long long)e * a.blocks + block] = s;
+      else
+        a.importance[e] = s;
     }
   }
 }
@@ -219,18 +223,20 @@ __global__ void __launch_bounds__(256) route_scan_kernel(const RouteArgs a) {
   }
 }
 
-// Places of the pairs of a.gates gate blocks from the first one, `gate`, on.
+// Places of the pairs of a.gates gate blocks from the first one, `gate`, on.  ONE: there is one block, whose counts the
+// gate left where `base` will be.
+template <bool ONE>
 __device__ __forceinline__ void route_place(const RouteArgs& a, int gate, int* smem) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int E = a.E;
-  int* cnt = smem;                           // [warp][E + 1]
-  int* base = smem + ROUTE_WARPS * (E + 1);  // [E + 1]
+  int* base = smem;         // [E + 1]
+  int* cnt = smem + E + 1;  // [warp][E + 1]
   __shared__ int carry[ROUTE_WARPS + 1];
   // where the members' rows begin: sums of the totals
   if (threadIdx.x == 0) carry[ROUTE_WARPS] = 0;
   for (int e0 = 0; e0 <= E; e0 += blockDim.x) {
     const int e = e0 + threadIdx.x;
-    const int all = e <= E ? a.totals[e] : 0;
+    const int all = e <= E ? (ONE ? base[e] : a.totals[e]) : 0;
     int inc = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -244,7 +250,7 @@ __device__ __forceinline__ void route_place(const RouteArgs& a, int gate, int* s
     __syncthreads();
     if (threadIdx.x == blockDim.x - 1) carry[ROUTE_WARPS] = first + all;
     if (e <= E) {
-      base[e] = first + a.counts[(long long)e * a.blocks + gate];
+      base[e] = first + (ONE ? 0 : a.counts[(long long)e * a.blocks + gate]);
       if (gate == 0) a.offsets[e] = first;
     }
   }
@@ -295,7 +301,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 16 ? 2 : 1) route_gate_
 
 __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_place_kernel(const RouteArgs a) {
   extern __shared__ int route_smem[];
-  route_place(a, blockIdx.x * a.gates, route_smem);
+  route_place<false>(a, blockIdx.x * a.gates, route_smem);
 }
 
 // Few rows: all of it in one block.
@@ -304,13 +310,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_small_kernel(const Rou
   extern __shared__ int route_smem[];
   route_gate<T, V>(a, 0, route_smem);
   __syncthreads();
-  for (int e = threadIdx.x; e <= a.E; e += blockDim.x) {  // one block's counts and sums
-    a.totals[e] = a.counts[e];
-    a.counts[e] = 0;
-    if (e < a.E) a.importance[e] = a.partial[e];
-  }
-  __syncthreads();
-  route_place(a, 0, route_smem);
+  route_place<true>(a, 0, route_smem);
 }
 
 // dz of a row by one warp: p is formed again from the scores (reading it would cost more than the sums).  Lane j then

@@ -725,12 +725,18 @@ def binary_roc_auc(scores: Tensor, labels: Tensor, workspace: Tensor | None = No
 _functions: dict = {}
 
 
-def _call(name: str, args, device: int) -> None:
-    """`name(args)` on the current stream of device number `device`, whichever device is current.
-    (The raw stream handle: building a `torch.cuda.Stream` takes as long as the launch.)"""
+def _function(name: str):
+    """The library's function of that name."""
     fn = _functions.get(name)
     if fn is None:
         fn = _functions[name] = getattr(load(), name)
+    return fn
+
+
+def _call(name: str, args, device: int) -> None:
+    """`name(args)` on the current stream of device number `device`, whichever device is current.
+    (The raw stream handle: building a `torch.cuda.Stream` takes as long as the launch.)"""
+    fn = _functions.get(name) or _function(name)
     if device == torch._C._cuda_getDevice():
         check(fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device)), name)
     else:
@@ -761,6 +767,18 @@ def _operand(name: str, t: Tensor | None, shape: tuple, dtype: torch.dtype, devi
 def _empty2(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> Tensor:
     """A contiguous (rows, cols) tensor (the strided form is the cheapest of torch's factories)."""
     return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
+def _empty(shape: tuple, dtype: torch.dtype, device: torch.device) -> Tensor:
+    strides, n = [], 1
+    for d in reversed(shape):
+        strides.append(n)
+        n *= d
+    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=device)
+
+
+def _empty3(a: int, b: int, c: int, dtype: torch.dtype, device: torch.device) -> Tensor:
+    return torch.empty_strided((a, b, c), (b * c, c, 1), dtype=dtype, device=device)
 
 
 def _empty_as(t: Tensor, dtype: torch.dtype) -> Tensor:
@@ -1155,15 +1173,15 @@ def route_forward(logits: Tensor, top_k: int, *, renormalize: bool = True
         raise ValueError(f'top_k must be between 1 and {min(E, _lib.TP_ROUTE_MAX_K)}, got {top_k}')
     logits, stride = _rows2('logits', logits, (T, E), logits.dtype, device)
     dev, i32, f32 = logits.device, torch.int32, torch.float32
-    weight, expert, position = (_empty2(T, top_k, d, dev) for d in (f32, i32, i32))
+    weight, expert, position = _empty2(T, top_k, f32, dev), _empty2(T, top_k, i32, dev), _empty2(T, top_k, i32, dev)
     if not T:
         return weight, expert, position, torch.zeros(E + 1, dtype=i32, device=dev), torch.zeros(E, device=dev)
     offsets = torch.empty_strided((E + 1,), (1,), dtype=i32, device=dev)
     importance = torch.empty_strided((E,), (1,), dtype=f32, device=dev)
-    need = load().tp_route_workspace_size(T, E, top_k)
-    ws = torch.empty_strided((need // 4,), (1,), dtype=i32, device=dev)
+    need = _function('tp_route_workspace_size')(T, E, top_k)
+    ws = torch.empty_strided((need // 4,), (1,), dtype=i32, device=dev) if need else None
     a = _lib.RouteArgs(T, E, top_k, code, int(renormalize), logits.data_ptr(), stride, weight.data_ptr(),
-                       expert.data_ptr(), position.data_ptr(), offsets.data_ptr(), importance.data_ptr(), ws.data_ptr(),
+                       expert.data_ptr(), position.data_ptr(), offsets.data_ptr(), importance.data_ptr(), _ptr(ws),
                        need)
     _call('tp_route_forward', a, device)
     return weight, expert, position, offsets, importance
@@ -1329,7 +1347,7 @@ def ragged_linear_forward(x: Tensor, weight: Tensor, bias: Tensor | None, offset
         a = _lib.RaggedLinearArgs(P, K, N, code, R, offsets.data_ptr(), _ptr(inf), _ptr(outf), int(relu), x.data_ptr(),
                                   xs, w.data_ptr(), ws, _ptr(bias), y.data_ptr())
         if code == TP_DTYPE_F32:
-            a.workspace_bytes = need = load().tp_ragged_linear_workspace_size(ctypes.byref(a))
+            a.workspace_bytes = need = _function('tp_ragged_linear_workspace_size')(ctypes.byref(a))
             scratch = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=x.device)
             a.workspace = scratch.data_ptr()
         _call('tp_ragged_linear_forward', a, device)
@@ -1363,7 +1381,7 @@ def ragged_linear_backward(dy: Tensor, x: Tensor, weight: Tensor, y: Tensor | No
     a = _lib.RaggedLinearArgs(P, K, N, code, R, offsets.data_ptr(), _ptr(inf), _ptr(outf), int(relu), x.data_ptr(), xs,
                               w.data_ptr(), ws, None, _ptr(y) if relu else None, dy.data_ptr(), ds, _ptr(dx), _ptr(dw),
                               _ptr(db))
-    need = load().tp_ragged_linear_workspace_size(ctypes.byref(a))
+    need = _function('tp_ragged_linear_workspace_size')(ctypes.byref(a))
     if need:
         scratch = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=dev)
         a.workspace, a.workspace_bytes = scratch.data_ptr(), need
@@ -1425,9 +1443,9 @@ def fp4_quantize(x: Tensor, format: str = 'nvfp4', *, offsets: Tensor | None = N
     n_features = _members('n_features', n_features, P, device)
     x, stride = _rows2('x', x if x.ndim == 2 else x.reshape(rows, K), (rows, K), x.dtype, device)
     u8, dev = torch.uint8, x.device
-    codes = torch.empty((*lead, _fp4_pitch(K)), dtype=u8, device=dev)
-    scales = torch.empty((*tiles, _fp4_scale_tiles(K, code), 512), dtype=u8, device=dev)
-    row_scale = torch.empty(lead, dtype=torch.float32, device=dev)
+    codes = _empty((*lead, _fp4_pitch(K)), u8, dev)
+    scales = _empty((*tiles, _fp4_scale_tiles(K, code), 512), u8, dev)
+    row_scale = _empty(lead, torch.float32, dev)
     if rows:
         a = _lib.Fp4Args(P, K, code, dtype, rows, _ptr(offsets), _ptr(n_features), x.data_ptr(), stride,
                          codes.data_ptr(), scales.data_ptr(), row_scale.data_ptr())
@@ -1453,7 +1471,7 @@ def fp4_values(q: Fp4Rows) -> Tensor:
     if len(lead) not in (1, 2) or q.columns < 1:
         raise ValueError('the rows must be (rows, columns) or (pack_size, rows, columns)')
     q = _fp4_checked('q', q, device, (*lead[:-1], (lead[-1] + 127) // 128))
-    out = torch.empty((*lead, q.columns), dtype=torch.bfloat16, device=q.codes.device)
+    out = _empty((*lead, q.columns), torch.bfloat16, q.codes.device)
     if out.numel():
         a = _lib.Fp4Args(lead[0] if len(lead) == 2 else 1, q.columns, _fp4_format(q.format), 0, q.row_scale.numel(), None,
                          None, None, 0, q.codes.data_ptr(), q.scales.data_ptr(), q.row_scale.data_ptr(), out.data_ptr())
@@ -1496,14 +1514,19 @@ def fp4_linear_forward(x: Tensor, weight: Fp4Rows, bias: Tensor | None = None, o
     if shared and inf is not None and P > 1:
         # members of different widths see different rows, and have scales of their own
         x, shared = x.expand(P, *x.shape), False
-    y = torch.empty((P, x.shape[0], N) if shared else (*x.shape[:-1], N), dtype=x.dtype, device=x.device)
-    if not x.numel():
+    lead = x.shape
+    rows = lead[0] if len(lead) == 2 else lead[0] * lead[1]
+    y = (_empty2(rows, N, x.dtype, x.device) if offsets is not None
+         else _empty3(P, lead[-2], N, x.dtype, x.device))
+    if not rows:
         return y
-    q = fp4_quantize(x, weight.format, offsets=offsets, n_features=inf)
-    a = _lib.Fp4LinearArgs(P, K, N, _fp4_format(weight.format), dtype, int(shared), q.row_scale.numel(), _ptr(offsets),
-                           _ptr(inf), _ptr(outf), q.codes.data_ptr(), q.scales.data_ptr(), q.row_scale.data_ptr(),
-                           weight.codes.data_ptr(), weight.scales.data_ptr(), weight.row_scale.data_ptr(), _ptr(bias),
-                           int(relu), y.data_ptr())
+    x, stride = _rows2('x', x if len(lead) == 2 else x.reshape(rows, K), (rows, K), x.dtype, device)
+    a = _lib.Fp4LinearArgs(P, K, N, _lib.TP_FP4[weight.format], dtype, int(shared), rows, _ptr(offsets), _ptr(inf),
+                           _ptr(outf), None, None, None, weight.codes.data_ptr(), weight.scales.data_ptr(),
+                           weight.row_scale.data_ptr(), _ptr(bias), int(relu), y.data_ptr(), x.data_ptr(), stride)
+    a.workspace_bytes = need = _function('tp_fp4_linear_workspace_size')(ctypes.byref(a))
+    scratch = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=x.device)
+    a.workspace = scratch.data_ptr()
     _call('tp_fp4_linear_forward', a, device)
     return y
 
