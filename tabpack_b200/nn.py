@@ -764,13 +764,69 @@ class LinearPack(ModulePack):
             raise ValueError('The number of input features must be equal to the maximum supported number of features')
         return _linear_call(self, x, pack_idx, relu=False, dropout=None, stream=None, n_blocks=None, block_index=0)
 
+    def forward_rows(self, x: Tensor, offsets: Tensor, *, relu: bool = False) -> Tensor:
+        """The layer (+ReLU) over a batch of its own for each member (no counterpart in the reference): x (rows,
+        max_in_features) holds the members' rows one after the other, member m's are x[offsets[m] : offsets[m + 1]].
+        `offsets` (pack_size + 1,) whole numbers on the device, as `Routing.offsets`; rows of no member are zero in
+        the result (rows, max_out_features)."""
+        if x.ndim != 2 or x.shape[-1] != self.max_in_features:
+            raise ValueError('The input must be (rows, maximum supported number of features)')
+        if not x.is_cuda:
+            raise RuntimeError('tabpack_b200 packs run on CUDA devices only')
+        dtype = _compute_dtype(x)
+        cols = _round8(x.shape[-1]) if dtype == torch.bfloat16 else x.shape[-1]
+        # the copy of the weights that `forward` uses, where it pads no rows
+        cache = self._cache
+        if dtype == torch.bfloat16 and self.max_out_features % 8 != 0:
+            cache = self.__dict__.setdefault('_rows_cache', _WeightCache())
+        inf = None if getattr(self, 'full_width_input', False) else _widths_cached(self, 'in', self.in_features)
+        outf = _widths_cached(self, 'out', self.out_features)
+        w = cache.get(self.weight, dtype, cols, widths=(outf, inf, None, 0))
+        x = x.to(dtype)
+        if cols != x.shape[-1]:
+            x = nn.functional.pad(x, (0, cols - x.shape[-1]))
+        with torch.autocast(x.device.type, enabled=False):
+            return _RaggedLinearFn.apply(x, self.weight, self.bias, w, offsets, inf, outf, relu)
+
+
+class _RaggedLinearFn(torch.autograd.Function):
+    """`ops.ragged_linear_forward` / `ops.ragged_linear_backward` on the compute copy of the weight."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, w_compute, offsets, in_features, out_features, relu):
+        y = ops.ragged_linear_forward(x, w_compute, None if bias is None else bias.float(), offsets,
+                                      in_features=in_features, out_features=out_features, relu=relu)
+        ctx.relu, ctx.w_shape, ctx.w_dtype = relu, weight.shape, weight.dtype
+        ctx.b_dtype = None if bias is None else bias.dtype
+        ctx.save_for_backward(x, w_compute, y if relu else None, offsets, in_features, out_features)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, y, offsets, in_features, out_features = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = ops.ragged_linear_backward(dy.to(x.dtype), x, w, y, offsets, in_features=in_features,
+                                                out_features=out_features, relu=ctx.relu, need_dx=need[0],
+                                                need_dw=need[1], need_db=need[2])
+        if dw is not None:
+            dw = dw[..., : ctx.w_shape[-1]].to(ctx.w_dtype)
+        return dx, dw, None if db is None else db.to(ctx.b_dtype), None, None, None, None, None
+
 
 def _linear_call(linear: LinearPack, x: Tensor, pack_idx, *, relu, dropout, stream, n_blocks, block_index,
                  offset_stride: int = 1, offset_add: int = 0, dx_cols: int = 0, row_index: Tensor | None = None,
                  narrow: tuple[int | None, int | None] | None = None):
     """`narrow` = (out, in): with a member selection, the selected weights are cut to their
     first `out` rows / `in` columns (None: all), so the selected members' layer runs with
-    those maximum widths (they must cover every selected member's widths)."""
+    those maximum widths (they must cover every selected member's widths).  A layer in 4 bits
+    runs with its own maximum widths."""
+    if isinstance(linear, Fp4LinearPack):
+        if dropout is not None or row_index is not None:
+            raise RuntimeError('Layers in 4 bits are for prediction: they take neither dropout nor a gathered input')
+        return linear._apply_rows(x, pack_idx, relu=relu, n_blocks=n_blocks, block_index=block_index)
+    if narrow is not None and narrow[1] is not None and x.shape[-1] > narrow[1]:
+        x = x[..., : narrow[1]]  # a layer in 4 bits before this one is as wide as the pack
     w, b = linear.weight, linear.bias
     if row_index is not None and pack_idx is not None:
         raise ValueError('a gathered input runs on the whole pack')
@@ -1021,6 +1077,252 @@ def label_log_probs(logits: Tensor, labels: Tensor, *, top_k: int = 0, ignore_in
     differentiable; rows whose label is `ignore_index` have log probability 0 and no gradient from
     it.  Classes masked with -inf take no part."""
     return LabelLogProbs(*_LabelLogProbsFn.apply(logits, labels, top_k, ignore_index))
+
+
+# >>> routing rows to members
+
+
+class Routing(NamedTuple):
+    """What `route` returns: which members a row goes to and where its copies lie (`tp_route_forward`).  `weight` and
+    `importance` are differentiable."""
+
+    weight: Tensor  # (rows, top_k) fp32
+    expert: Tensor  # (rows, top_k) int32, -1 where a row has no further member
+    position: Tensor  # (rows, top_k) int32: places sorted by member, those of no member last
+    offsets: Tensor  # (pack_size + 1,) int32: where the members' rows begin
+    importance: Tensor  # (pack_size,) fp32: each member's sum of probabilities
+
+    def balance_loss(self) -> Tensor:
+        """pack_size * sum_m (share of the pairs that go to m) * (mean probability of m): 1 where both are even, more
+        where the same few members have most of both.  Its gradient goes through the probabilities."""
+        count = torch.diff(self.offsets).float()
+        share = count / count.sum().clamp(min=1.0)
+        return len(count) * (share * self.importance).sum() / max(1, self.weight.shape[0])
+
+
+class _RouteFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_k, renormalize):
+        ctx.set_materialize_grads(False)
+        weight, expert, position, offsets, importance = ops.route_forward(logits, top_k, renormalize=renormalize)
+        ctx.save_for_backward(logits, weight, expert)
+        ctx.renormalize = renormalize
+        ctx.mark_non_differentiable(expert, position, offsets)
+        return weight, expert, position, offsets, importance
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_weight, g_expert, g_position, g_offsets, g_importance):
+        if g_weight is None and g_importance is None:
+            return None, None, None
+        logits, weight, expert = ctx.saved_tensors
+        return ops.route_backward(g_weight, g_importance, logits, weight, expert, renormalize=ctx.renormalize), None, None
+
+
+def route(logits: Tensor, top_k: int, *, renormalize: bool = True) -> Routing:
+    """Routing of rows to the `top_k` members with the highest scores, `logits` (rows, pack_size) bf16 or fp32
+    (no counterpart in the reference).  Weights are the softmax over the chosen members, or over all with
+    `renormalize=False`.  Scores of -inf leave a member out; a row may end up with fewer members, or none."""
+    return Routing(*_RouteFn.apply(logits, top_k, renormalize))
+
+
+class _DispatchFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, position, offsets):
+        ctx.save_for_backward(position, offsets)
+        return ops.dispatch_rows(x, position, offsets)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dxs):
+        return ops.combine_rows(dxs, None, *ctx.saved_tensors), None, None
+
+
+def dispatch_rows(x: Tensor, routing: Routing) -> Tensor:
+    """The rows of x (rows, features) in the order of `routing`, (rows top_k, features): the members' batches one after
+    the other, then zero rows for the pairs without a member.  Their gradients add up in fp32."""
+    return _DispatchFn.apply(x, routing.position, routing.offsets)
+
+
+class _CombineFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weight, position, offsets):
+        ctx.save_for_backward(y, weight, position, offsets)
+        return ops.combine_rows(y, weight, position, offsets)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        y, weight, position, offsets = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dy, dw = ops.combine_rows_backward(dout, y, weight, position, offsets, need_dy=need[0], need_dweight=need[1])
+        return dy, dw, None, None
+
+
+def combine_rows(y: Tensor, routing: Routing) -> Tensor:
+    """Each row's weighted sum of its members' results, from y (rows top_k, features) in the order of
+    `dispatch_rows`: (rows, features) of y's type, summed in fp32."""
+    return _CombineFn.apply(y, routing.weight, routing.position, routing.offsets)
+
+
+class RoutedMLPPack(ModulePack):
+    """A mixture of a pack's members (no counterpart in the reference): a linear router gives each row to `top_k`
+    members, each an MLP with one hidden layer of its own width, and adds up their outputs by the router's weights.
+    Every member multiplies only the rows that it gets.
+
+    Input (batch, d_in), the same for all members; output (batch, d_out) of the compute type (bf16 under autocast),
+    and the `Routing`, whose `balance_loss` keeps members from falling idle.  The router runs in fp32."""
+
+    def __init__(self, d_in: int, d_block: int | list[int], d_out: int, *, top_k: int, renormalize: bool = True,
+                 max_d_block: int | None = None, pack_size: int, device=None) -> None:
+        if not 1 <= top_k <= pack_size:
+            raise ValueError('The number of members per row must be positive and must not exceed the pack size')
+        super().__init__()
+        self.router = ParameterPack(torch.empty(pack_size, d_in, device=device))
+        self.hidden = LinearPack(d_in, d_block, max_out_features=max_d_block, pack_size=pack_size, device=device)
+        self.output = LinearPack(d_block, d_out, max_in_features=max_d_block, pack_size=pack_size, device=device)
+        self.top_k = top_k
+        self.renormalize = renormalize
+        self.reset_parameters()
+
+    @property
+    def pack_size(self) -> int:
+        return self.router.shape[PACK_DIM]
+
+    def reset_parameters(self, *, pack_idx: Tensor | None = None) -> None:
+        if pack_idx is not None:
+            check_pack_idx(pack_idx, self.pack_size)
+        n, d_in = self.pack_size if pack_idx is None else len(pack_idx), self.router.shape[1]
+        init = (2.0 * torch.rand(n, d_in, device=self.router.device) - 1.0) * d_in ** -0.5
+        with torch.no_grad():
+            self.router[slice(None) if pack_idx is None else pack_idx] = init.to(self.router.dtype)
+        for layer in (self.hidden, self.output):
+            if isinstance(layer, LinearPack):
+                layer.reset_parameters(pack_idx=pack_idx)
+
+    def replace(self, *, pack_idx: Tensor, d_block: list[int] | None = None) -> None:
+        self.hidden.replace(pack_idx=pack_idx, out_features=d_block)
+        self.output.replace(pack_idx=pack_idx, in_features=d_block)
+        self.reset_parameters(pack_idx=pack_idx)
+
+    def forward(self, x: Tensor) -> tuple[Tensor, Routing]:
+        if x.ndim != 2 or x.shape[1] != self.router.shape[1]:
+            raise ValueError('The input must be (batch, number of input features)')
+        if not x.is_cuda:
+            raise RuntimeError('tabpack_b200 packs run on CUDA devices only')
+        with torch.autocast(x.device.type, enabled=False):
+            logits = nn.functional.linear(x.float(), self.router.float())
+        routing = route(logits, self.top_k, renormalize=self.renormalize)
+        rows = dispatch_rows(x.to(_compute_dtype(x)), routing)
+        h = self.hidden.forward_rows(rows, routing.offsets, relu=True)
+        return combine_rows(self.output.forward_rows(h, routing.offsets), routing), routing
+
+
+# >>> layers in 4 bits
+
+
+class Fp4LinearPack(ModulePack):
+    """A `LinearPack` for prediction with weights in 4-bit floating point (no counterpart in the reference): `format`
+    'nvfp4' (blocks of 16 input features share an e4m3 scale, each output a power of two) or 'mxfp4' (blocks of 32, a
+    power of two), 0.56 and 0.53 bytes a weight.  Inputs are quantised in the same format, sums are in fp32; the
+    output has the compute type (bf16 under autocast, else the input's).  It has no parameters and no backward."""
+
+    def __init__(self, codes: Tensor, scales: Tensor, row_scale: Tensor, bias: Tensor | None,
+                 in_features: Tensor | None, out_features: Tensor | None, *, max_in_features: int, format: str,
+                 full_width_input: bool = False) -> None:
+        super().__init__()
+        for name, t in (('codes', codes), ('scales', scales), ('row_scale', row_scale), ('bias', bias),
+                        ('in_features', in_features), ('out_features', out_features)):
+            self.register_buffer(name, None if t is None else _mark_buffer(t))
+        self._max_in_features = max_in_features
+        self.format = format
+        self.full_width_input = full_width_input
+
+    @classmethod
+    def from_linear(cls, linear: LinearPack, format: str = 'nvfp4') -> Fp4LinearPack:
+        """The layer's weights as they are now, rounded to 4 bits."""
+        if not linear.weight.is_cuda:
+            raise RuntimeError('tabpack_b200 packs run on CUDA devices only')
+        full = bool(getattr(linear, 'full_width_input', False))
+        inf = None if full else _widths(linear.in_features)
+        outf = _widths(linear.out_features)
+        q = ops.fp4_quantize(linear.weight.detach().float(), format, n_features=inf)
+        # (clones: the layer's buffers change with `replace`)
+        bias = None if linear.bias is None else linear.bias.detach().float().clone()
+        return cls(q.codes, q.scales, q.row_scale, bias, None if inf is None else inf.clone(),
+                   None if outf is None else outf.clone(), max_in_features=linear.max_in_features, format=format,
+                   full_width_input=full)
+
+    @property
+    def max_in_features(self) -> int:
+        return self._max_in_features
+
+    @property
+    def max_out_features(self) -> int:
+        return self.row_scale.shape[1]
+
+    @property
+    def pack_size(self) -> int:
+        return self.row_scale.shape[PACK_DIM]
+
+    def dequantize(self) -> Tensor:
+        """The weights' values (pack_size, max_out_features, max_in_features), bf16 (which holds them exactly)."""
+        return ops.fp4_values(ops.Fp4Rows(self.codes, self.scales, self.row_scale, self._max_in_features, self.format))
+
+    def _call(self, x: Tensor, pack_idx: Tensor | None, offsets: Tensor | None, relu: bool) -> Tensor:
+        if not x.is_cuda:
+            raise RuntimeError('tabpack_b200 packs run on CUDA devices only')
+        if torch.is_grad_enabled() and (x.requires_grad or self.training):
+            raise RuntimeError('Layers in 4 bits have no backward: call them in evaluation mode or under torch.no_grad()')
+        K = self._max_in_features
+        x = x.detach().to(_compute_dtype(x))
+        if x.shape[-1] > K:  # (the columns of a first layer's input padded to a multiple of eight)
+            x = x[..., :K]
+        elif x.shape[-1] < K:
+            x = nn.functional.pad(x, (0, K - x.shape[-1]))
+        t = (self.codes, self.scales, self.row_scale, self.bias, self.in_features, self.out_features)
+        if pack_idx is not None:
+            check_pack_idx(pack_idx, self.pack_size)
+            t = tuple(_select(v, pack_idx) for v in t)
+        codes, scales, row_scale, bias, inf, outf = t
+        weight = ops.Fp4Rows(codes, scales, row_scale, K, self.format)
+        return ops.fp4_linear_forward(x, weight, bias, offsets, in_features=inf, out_features=outf, relu=relu)
+
+    def _apply_rows(self, x: Tensor, pack_idx: Tensor | None, *, relu: bool, n_blocks: Tensor | None = None,
+                    block_index: int = 0) -> Tensor:
+        P = self.pack_size if pack_idx is None else len(pack_idx)
+        if x.ndim == 3 and (x.shape[0] == 1 or x.stride(0) == 0) and P != 1:
+            x = x[0]  # rows that the members share are quantised once
+        y = self._call(x, pack_idx, None, relu)
+        if n_blocks is not None:  # members without this block pass their input through
+            y = torch.where((n_blocks > block_index).view(-1, 1, 1), y, x.to(y.dtype)[..., : y.shape[-1]])
+        return y
+
+    def forward(self, x: Tensor, pack_idx: Tensor | None = None) -> Tensor:
+        if x.ndim != 3:
+            raise ValueError('The input must have three dimensions')
+        if x.shape[-1] != self.max_in_features:
+            raise ValueError('The number of input features must be equal to the maximum supported number of features')
+        return self._apply_rows(x, pack_idx, relu=False)
+
+    def forward_rows(self, x: Tensor, offsets: Tensor, *, relu: bool = False) -> Tensor:
+        """`LinearPack.forward_rows` in 4 bits."""
+        if x.ndim != 2 or x.shape[-1] != self.max_in_features:
+            raise ValueError('The input must be (rows, maximum supported number of features)')
+        return self._call(x, None, offsets, relu)
+
+
+def fp4_(module: nn.Module, format: str = 'nvfp4', *, keep=()) -> nn.Module:
+    """Replaces every `LinearPack` inside `module` (a `TabPack`, a `RoutedMLPPack`, ...) but those in `keep` by its
+    `Fp4LinearPack`, in place, and puts the module into evaluation mode: a model for prediction.  Returns `module`."""
+    kept = {id(m) for m in keep}
+    if isinstance(module, LinearPack):
+        raise TypeError('Use Fp4LinearPack.from_linear for a single layer')
+    for owner in list(module.modules()):
+        for name, child in list(owner.named_children()):
+            if isinstance(child, LinearPack) and id(child) not in kept:
+                setattr(owner, name, Fp4LinearPack.from_linear(child, format))
+    return module.eval()
 
 
 class MLPBackbonePack(ModulePack):
@@ -1513,6 +1815,8 @@ class TabPack(ModulePack):
         features, the whole pack, inputs whose gradient is not requested, and no backward
         (unless `gather_one_hot_in_training`)."""
         if pack_idx is not None or self.cat_module is None or x_cat is None or not x_cat.is_cuda:
+            return None
+        if isinstance(self.backbone.blocks[0].linear, Fp4LinearPack):  # (its columns share scales: it multiplies them)
             return None
         if (torch.is_grad_enabled() and not self.gather_one_hot_in_training
                 and any(p.requires_grad for p in self.parameters())):

@@ -25,6 +25,7 @@ change) where the reference removes it from the pack.
 
 from __future__ import annotations
 
+import copy
 import dataclasses
 import math
 from typing import Callable
@@ -37,7 +38,7 @@ from torch import Tensor
 from tabpack_b200 import ops
 from tabpack_b200.ensemble import compute_unsanitized_ensemble_predictions, greedy_ensemble
 from tabpack_b200.metrics import PackScore
-from tabpack_b200.nn import CosineEmbeddingsPack, LinearPack, TabPack, label_log_probs
+from tabpack_b200.nn import CosineEmbeddingsPack, LinearPack, TabPack, fp4_, label_log_probs
 from tabpack_b200.optim import AdamWPack, MuonAdamWPack, split_weight_decay
 from tabpack_b200.shard import allreduce_sum_, assign_replacements, gather_members, member_ranges
 
@@ -397,12 +398,15 @@ class PackTrainer:
         return chunks
 
     @torch.no_grad()
-    def predict_local(self, data: dict, *, eval_batch_size: int = 32768, member_chunk: int | None = None) -> Tensor:
-        """Transformed predictions of this rank's members on a shared dataset.  `member_chunk`
+    def predict_local(self, data: dict, *, eval_batch_size: int = 32768, member_chunk: int | None = None,
+                      model: TabPack | None = None) -> Tensor:
+        """Transformed predictions of this rank's members on a shared dataset, by `model` in place of
+        the trainer's own (a copy of it in another form).  `member_chunk`
         runs the members in groups of that size (bounds the activations of wide packs on large
         batches: each group is a `pack_idx` selection of the pack, of members of similar width
         that run with their own maximum width)."""
-        self.model.eval()
+        model = self.model if model is None else model
+        model.eval()
         n = len(data['y']) if 'y' in data else len(next(iter(data.values())))
         P = self.hi - self.lo
         chunks = None if member_chunk is None or member_chunk >= P else self._width_chunks(member_chunk)
@@ -412,13 +416,13 @@ class PackTrainer:
             xc = data['x_cat'][i: i + eval_batch_size] if 'x_cat' in data else None
             if chunks is None:
                 with torch.autocast('cuda', dtype=torch.bfloat16, enabled=self.autocast):
-                    out = self.model(xn, xc)
+                    out = model(xn, xc)
                 parts.append(transform(self.loss, out.float()))
                 continue
             full = None
             for idx, mw in chunks:
                 with torch.autocast('cuda', dtype=torch.bfloat16, enabled=self.autocast):
-                    out = self.model(xn, xc, idx, max_width=mw)
+                    out = model(xn, xc, idx, max_width=mw)
                 out = transform(self.loss, out.float())
                 if full is None:
                     full = out.new_empty((P, *out.shape[1:]))
@@ -602,13 +606,29 @@ class PackTrainer:
         return EpochResult(epoch, train_loss, metric, idx, w, ens_score)
 
 
+def _fp4_copy(model: TabPack, format: str) -> TabPack:
+    """A copy of the model with its layers in 4 bits; their fp32 weights are shared while it is made, not copied."""
+    memo = {}
+    for m in model.modules():
+        if isinstance(m, LinearPack):  # (its caches and reusable buffers are its own)
+            memo.update({id(p): p for p in m.parameters()})
+            memo.update({id(m._cache): m._cache, id(m._dw_slot): {}, id(m._y_slot): {}})
+    return fp4_(copy.deepcopy(model, memo), format)
+
+
 class PackPredictor(torch.nn.Module):
     """Inference over a (sharded) pack: every member's transformed prediction and ensemble
-    heads averaging the selected global members (`_training.py:1909-2018`)."""
+    heads averaging the selected global members (`_training.py:1909-2018`).
 
-    def __init__(self, trainer: PackTrainer, ensembles: dict[str, Tensor]) -> None:
+    `weight_format` ('nvfp4' or 'mxfp4'): predicts with a copy of the model, as it is now, whose
+    layers are in 4 bits (`nn.fp4_`); the trainer's own model stays as it is."""
+
+    def __init__(self, trainer: PackTrainer, ensembles: dict[str, Tensor], *, weight_format: str | None = None) -> None:
         super().__init__()
         self.trainer = trainer
+        self.model = None
+        if weight_format is not None:
+            self.model = _fp4_copy(trainer.model, weight_format)
         self.ensembles = {k: v.to(trainer.device, torch.int64) for k, v in ensembles.items()}
 
     @torch.no_grad()
@@ -620,7 +640,8 @@ class PackPredictor(torch.nn.Module):
             data['x_num'] = x_num
         if x_cat is not None:
             data['x_cat'] = x_cat
-        local = t.predict_local(data, eval_batch_size=eval_batch_size, member_chunk=member_chunk)  # (P_local, B[, C])
+        local = t.predict_local(data, eval_batch_size=eval_batch_size, member_chunk=member_chunk,
+                                model=self.model)  # (P_local, B[, C])
         flat = local.reshape(local.shape[0], -1).contiguous()
         heads = {}
         for name, gidx in self.ensembles.items():
