@@ -17,13 +17,14 @@
 // two thirds of the operand bytes per product.  A stage that needs zeros then completes on a barrier of its own CTA;
 // the peer reports its zeros to the leader, which issues the products.
 //
-// WGRAD sums at most RAGGED_SEGMENT rows in one accumulator and adds the pieces up in dw with the rounding of fp32:
-// the tensor core's own sums do not round to nearest, and over 23054 rows came out 2.6e-5 off (5e-6 with the cut).
+// Results in fp32 are summed over at most RAGGED_SEGMENT elements of K in one accumulator, the pieces in the epilogue's
+// registers with the rounding of fp32: the tensor core's own sums do not round to nearest, and over 23054 rows came out 2.6e-5 off
+// (5e-7 with the cut).
 // Few tiles over many rows are split over CTAs, into parts that a second launch adds up in order.
 //
 // fp32 operands come as three bf16 parts each (ragged_split_kernel), and the K loop goes through the six products of
-// parts whose terms exceed 2^-24 of the result, the smallest first (sums of up to 2048 elements per accumulator here,
-// added up in fp32): a sixth of the bf16 rate, where the CUDA cores give a twenty-fifth.
+// parts whose terms exceed 2^-24 of the result, the smallest first: a sixth of the bf16 rate, where the CUDA cores give a
+// twenty-fifth.
 #pragma once
 
 #include <type_traits>
@@ -34,7 +35,7 @@ namespace tp {
 
 enum : int { RAGGED_FWD = 0, RAGGED_DGRAD = 1, RAGGED_WGRAD = 2 };
 enum : int { RT_MMA = 0, RT_ZERO = 1, RT_END = 2 };
-constexpr int RAGGED_SEGMENT = 4096, RAGGED_SEGMENT_F32 = 2048;
+constexpr int RAGGED_SEGMENT = 1024, RAGGED_SEGMENT_F32 = 512;
 
 struct RaggedProblem {
   int P, R;                // members, rows of the matrix
@@ -66,7 +67,7 @@ __device__ __forceinline__ void ragged_group(const RaggedProblem& p, int g, int&
 }
 
 // forward, dgrad: `rows` rows from row0 on, sums from element `part` on; wgrad: input features from row0 on, `rows` is the
-// first row of the sum, `part` its part.  add, bit 0: on top of what the result holds; bit 1: more is to come.
+// first row of the sum, `part` its part.  add, bit 0: on top of the piece before; bit 1: more is to come.
 struct RaggedTile {
   int kind, member, row0, rows, nt, k_len, n_valid, m_valid, part, add;
 };
@@ -83,17 +84,19 @@ struct RaggedCfg {
   static constexpr bool A_MN = MODE == RAGGED_WGRAD;
   static constexpr bool B_MN = MODE != RAGGED_FWD;
   static constexpr int A_BYTES = BM * BK * 2, B_BYTES = B_ROWS * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = PAIR ? 6 : BN == 256 ? 4 : BN == 128 ? 6 : 7;
+  // fp32 results are summed up over the pieces of the K loop in the epilogue's registers, 64 columns a thread at most
+  static constexpr bool SUMS = F32 || MODE == RAGGED_WGRAD;
+  static constexpr int STAGES = PAIR ? (F32 && MODE != RAGGED_WGRAD ? 5 : 6) : BN == 256 ? (F32 && MODE != RAGGED_WGRAD ? 3 : 4) : BN == 128 ? 6 : 7;
   static constexpr int TMEM_COLS = 2 * BN;
-  static constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
+  static constexpr int EPI_WARP0 = 4, EPI_WARPS = SUMS && BN == 256 ? 16 : 8;
   static constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
   static constexpr int TRING = 4;
   static constexpr int RING_INTS = 10;
   static constexpr int CTRL_BYTES = 640;
   static constexpr int ROW_BYTES = 80;  // a warp's staged row of 32 bf16, padded against bank conflicts
-  static constexpr int WCOLS = BN / 2;  // columns of an epilogue warp
-  static constexpr int SMEM_BYTES =
-      1024 + STAGES * STAGE_BYTES + CTRL_BYTES + EPI_WARPS * (32 * ROW_BYTES + WCOLS * 4);
+  static constexpr int WCOLS = BN / (EPI_WARPS / 4);  // columns of an epilogue warp
+  static constexpr int EPI_BYTES = MODE == RAGGED_WGRAD ? 0 : 32 * ROW_BYTES + WCOLS * 4;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + CTRL_BYTES + EPI_WARPS * EPI_BYTES;
   static_assert(SMEM_BYTES <= 227 * 1024, "fits an SM");
 };
 
@@ -148,9 +151,9 @@ __device__ __forceinline__ void ragged_flush(__nv_bfloat16* c, int ld, int vec, 
   }
 }
 
-// A warp's staged 32 x 16 fp32 values into the result, on top of what it holds (`add`) and with ReLU at last.
+// A warp's staged 32 x 16 fp32 values into the result.
 __device__ __forceinline__ void ragged_flush_f32(float* c, int ld, int vec, long long row0, int rows, int col0,
-                                                 const uint8_t* stage, int row_bytes, int lane, bool add, bool relu) {
+                                                 const uint8_t* stage, int row_bytes, int lane) {
   if (vec) {
     const int q = lane & 3;
     if (col0 + 4 * q >= ld) return;
@@ -158,26 +161,14 @@ __device__ __forceinline__ void ragged_flush_f32(float* c, int ld, int vec, long
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int r = (lane >> 2) + 8 * k;
-      if (r < rows) {
-        float4 v = *reinterpret_cast<const float4*>(stage + r * row_bytes + q * 16);
-        float4* at = reinterpret_cast<float4*>(to + (long long)r * ld);
-        if (add) {
-          const float4 had = *at;
-          v = make_float4(v.x + had.x, v.y + had.y, v.z + had.z, v.w + had.w);
-        }
-        if (relu) v = make_float4(max_nan(v.x, 0.f), max_nan(v.y, 0.f), max_nan(v.z, 0.f), max_nan(v.w, 0.f));
-        *at = v;
-      }
+      if (r < rows) *reinterpret_cast<float4*>(to + (long long)r * ld) = *reinterpret_cast<const float4*>(stage + r * row_bytes + q * 16);
     }
   } else {
     const int q = lane & 15;
     if (col0 + q >= ld) return;
     float* to = c + row0 * ld + col0 + q;
-    for (int r = lane >> 4; r < min(rows, 32); r += 2) {
-      float v = *reinterpret_cast<const float*>(stage + r * row_bytes + 4 * q);
-      if (add) v += to[(long long)r * ld];
-      to[(long long)r * ld] = relu ? max_nan(v, 0.f) : v;
-    }
+    for (int r = lane >> 4; r < min(rows, 32); r += 2)
+      to[(long long)r * ld] = *reinterpret_cast<const float*>(stage + r * row_bytes + 4 * q);
   }
 }
 
@@ -541,13 +532,13 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR, F32>::THREADS, 1)
         t.n_valid = pr.out_f ? min(__ldg(pr.out_f + t.member), pr.out) : pr.out;
         if (end > first && t.row0 < t.m_valid && t.nt * BN < t.n_valid) {
           t.kind = RT_MMA;
-          // pieces of about the same length: a short one would not hide the other's read and write of dw
+          // pieces of about the same length
           const int pieces = (end - first + Cfg::SEGMENT - 1) / Cfg::SEGMENT;
           const int piece = ((end - first + pieces - 1) / pieces + 63) & ~63;
           for (int k = first; ok && k < end; k += piece) {
             t.rows = k;
             t.k_len = min(piece, end - k);
-            t.add = k > first ? 1 : 0;
+            t.add = (k > first ? 1 : 0) | (k + piece < end ? 2 : 0);
             ok = publish(t);
           }
         } else {
@@ -622,58 +613,102 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR, F32>::THREADS, 1)
   } else if (warp >= Cfg::EPI_WARP0) {
     // ------------------------------------------------------------------ epilogue
     const int ew = warp - Cfg::EPI_WARP0;
-    const int q = warp & 3, half = ew >> 2;
+    const int q = warp & 3, slice = ew >> 2;  // lanes and columns of the accumulator
     constexpr int WCOLS = Cfg::WCOLS;
     constexpr int NCH = (WCOLS + 31) / 32;
-    uint8_t* stage_warp = ctrl + Cfg::CTRL_BYTES + ew * (32 * Cfg::ROW_BYTES + WCOLS * 4);
+    uint8_t* stage_warp = ctrl + Cfg::CTRL_BYTES + ew * Cfg::EPI_BYTES;
     float* sbias = reinterpret_cast<float*>(stage_warp + 32 * Cfg::ROW_BYTES);
     uint8_t* stage_row = stage_warp + lane * Cfg::ROW_BYTES;
     int acc = 0;
     uint32_t acc_phase = 0;
+    float sum[Cfg::SUMS ? WCOLS : 1];
+    auto release = [&]() {  // the accumulator has been read
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR)
+          mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));  // the leader's MMA warp waits on it
+        else
+          mbar_arrive(&tempty[acc]);
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    };
     for (int k = 0;; ++k) {
       const RaggedTile t = ring_read(k, true);
       if (t.kind == RT_END) break;
-      const int cbase = t.nt * BN + half * WCOLS;
-      if constexpr (MODE == RAGGED_WGRAD) {
-        // lane = input feature, register = output feature: 32 consecutive floats of a row of dw per store
-        const int col = t.row0 + rank * Cfg::BM + q * 32 + lane;
-        float* base = static_cast<float*>(pr.c) + ((long long)t.part * pr.P + t.member) * pr.out * pr.in + col;
-        const int nch = min(NCH, max(0, (pr.out - cbase + 31) / 32));
-        const bool store = col < pr.in, valid = col < t.m_valid;
-        if (t.kind == RT_MMA) {
-          if (!mbar_wait(&tfull[acc], acc_phase, abort_flag)) break;
-          tc_fence_after();
-          const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * WCOLS);
-#pragma unroll 1
-          for (int c = 0; c < nch; ++c) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(t_row + (uint32_t)(32 * c), v);
+      const int cbase = t.nt * BN + slice * WCOLS;
+      const bool mma = t.kind == RT_MMA;
+      const bool biased = MODE == RAGGED_FWD && mma;
+      if (biased && !(t.add & 1)) {
+        __syncwarp();
+        for (int j = lane; j < WCOLS; j += 32)
+          sbias[j] = (pr.bias != nullptr && cbase + j < t.n_valid) ? __ldg(pr.bias + (long long)t.member * pr.out + cbase + j) : 0.f;
+        __syncwarp();
+      }
+      if (mma) {
+        if (!mbar_wait(&tfull[acc], acc_phase, abort_flag)) break;
+        tc_fence_after();
+      }
+      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + slice * WCOLS);
+      if constexpr (Cfg::SUMS) {
+        if (!(t.add & 1)) {
+#pragma unroll
+          for (int c = 0; c < WCOLS; ++c) sum[c] = 0.f;
+        }
+        if (mma) {
+#pragma unroll
+          for (int c = 0; c < WCOLS; c += 8) {
+            uint32_t v[8];
+            tmem_ld_32x32b_x8(t_row + (uint32_t)c, v);
             tmem_wait_ld();
-            if (t.add & 1) {
-              // on top of the sums over earlier rows, which this thread wrote; all loads before the stores
-              float had[32];
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const int o = cbase + 32 * c + j;
-                had[j] = (valid && o < t.n_valid) ? base[(long long)o * pr.in] : 0.f;
-              }
+            for (int j = 0; j < 8; ++j) sum[c + j] += __uint_as_float(v[j]);
+          }
+          release();
+          if (t.add & 2) continue;
+        }
+        if constexpr (MODE == RAGGED_WGRAD) {
+          // lane = input feature, register = output feature: 32 consecutive floats of a row of dw per store
+          const int col = t.row0 + rank * Cfg::BM + q * 32 + lane;
+          if (col < pr.in) {
+            float* to = static_cast<float*>(pr.c) + (((long long)t.part * pr.P + t.member) * pr.out + cbase) * pr.in + col;
+            const int n_out = pr.out - cbase, n_valid = col < t.m_valid ? t.n_valid - cbase : 0;
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const int o = cbase + 32 * c + j;
-                if (valid && o < t.n_valid) base[(long long)o * pr.in] = had[j] + __uint_as_float(v[j]);
-              }
-            } else {
+            for (int j = 0; j < WCOLS; ++j) {
+              if (j < n_out) *to = j < n_valid ? sum[j] : 0.f;
+              to += pr.in;
+            }
+          }
+        } else {
+          const int ld = MODE == RAGGED_FWD ? pr.out : pr.in;
+          const int rows = t.rows - rank * Cfg::BM - q * 32;  // of this warp, may be below 1 or above 32
+          const long long row0 = (long long)t.row0 + rank * Cfg::BM + q * 32;
+          if (rows > 0) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const int o = cbase + 32 * c + j;
-                if (store && o < pr.out)
-                  base[(long long)o * pr.in] = (valid && o < t.n_valid) ? __uint_as_float(v[j]) : 0.f;
+            for (int c = 0; c < WCOLS; c += 16) {
+              const int col0 = cbase + c;
+              if (col0 < ld) {
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                  float x[4];
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    x[e] = sum[c + j + e];
+                    if (biased) {
+                      x[e] += sbias[c + j + e];
+                      if (pr.relu) x[e] = max_nan(x[e], 0.f);
+                    }
+                    if (col0 + j + e >= t.n_valid) x[e] = 0.f;
+                  }
+                  *reinterpret_cast<float4*>(stage_row + j * 4) = make_float4(x[0], x[1], x[2], x[3]);
+                }
+                __syncwarp();
+                ragged_flush_f32(static_cast<float*>(pr.c), ld, pr.c_vec, row0, rows, col0, stage_warp, Cfg::ROW_BYTES, lane);
+                __syncwarp();
               }
             }
           }
-        } else if (store) {
-          const int o1 = min(cbase + WCOLS, pr.out);
-          for (int o = cbase; o < o1; ++o) base[(long long)o * pr.in] = 0.f;
         }
       } else {
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(pr.c);
@@ -681,92 +716,41 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR, F32>::THREADS, 1)
         const int nch = min(NCH, max(0, (ld - cbase + 31) / 32));
         const int rows = t.rows - rank * Cfg::BM - q * 32;  // of this warp, may be below 1 or above 32
         const long long row0 = (long long)t.row0 + rank * Cfg::BM + q * 32;
-        if (t.kind == RT_MMA) {
-          const bool biased = MODE == RAGGED_FWD && pr.bias != nullptr;
-          if constexpr (MODE == RAGGED_FWD) {
-            __syncwarp();
-            for (int j = lane; j < WCOLS; j += 32)
-              sbias[j] = (biased && cbase + j < t.n_valid) ? __ldg(pr.bias + (long long)t.member * pr.out + cbase + j) : 0.f;
-            __syncwarp();
-          }
-          if (!mbar_wait(&tfull[acc], acc_phase, abort_flag)) break;
-          tc_fence_after();
-          const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * WCOLS);
-          if (rows > 0) {
+        if (rows > 0 && mma) {
 #pragma unroll 1
-            for (int c = 0; c < nch; ++c) {
-              uint32_t v[32];
-              tmem_ld_32x32b_x32(t_row + (uint32_t)(32 * c), v);
-              tmem_wait_ld();
-              const int nv = t.n_valid - (cbase + 32 * c);
-              if constexpr (F32) {
+          for (int c = 0; c < nch; ++c) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(t_row + (uint32_t)(32 * c), v);
+            tmem_wait_ld();
+            const int nv = t.n_valid - (cbase + 32 * c);
 #pragma unroll
-                for (int h = 0; h < 32; h += 16) {
+            for (int j = 0; j < 32; j += 8) {
+              float x[8];
 #pragma unroll
-                  for (int j = 0; j < 16; j += 4) {
-                    float x[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                      x[e] = __uint_as_float(v[h + j + e]);
-                      if (MODE == RAGGED_FWD && !(t.add & 1)) x[e] += sbias[32 * c + h + j + e];
-                      if (h + j + e >= nv) x[e] = 0.f;
-                    }
-                    *reinterpret_cast<float4*>(stage_row + j * 4) = make_float4(x[0], x[1], x[2], x[3]);
-                  }
-                  __syncwarp();
-                  ragged_flush_f32(static_cast<float*>(pr.c), ld, pr.c_vec, row0, rows, cbase + 32 * c + h, stage_warp,
-                                   Cfg::ROW_BYTES, lane, t.add & 1, MODE == RAGGED_FWD && pr.relu && !(t.add & 2));
-                  __syncwarp();
+              for (int e = 0; e < 8; ++e) {
+                x[e] = __uint_as_float(v[j + e]);
+                if constexpr (MODE == RAGGED_FWD) {
+                  x[e] += sbias[32 * c + j + e];
+                  if (pr.relu) x[e] = max_nan(x[e], 0.f);
                 }
-              } else {
-#pragma unroll
-              for (int j = 0; j < 32; j += 8) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  x[e] = __uint_as_float(v[j + e]);
-                  if constexpr (MODE == RAGGED_FWD) {
-                    x[e] += sbias[32 * c + j + e];
-                    if (pr.relu) x[e] = max_nan(x[e], 0.f);
-                  }
-                  if (j + e >= nv) x[e] = 0.f;
-                }
-                *reinterpret_cast<uint4*>(stage_row + j * 2) =
-                    make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+                if (j + e >= nv) x[e] = 0.f;
               }
-              __syncwarp();
-              ragged_flush(out, ld, pr.c_vec, row0, rows, cbase + 32 * c, stage_warp, Cfg::ROW_BYTES, lane);
-              __syncwarp();
-              }
+              *reinterpret_cast<uint4*>(stage_row + j * 2) =
+                  make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
             }
+            __syncwarp();
+            ragged_flush(out, ld, pr.c_vec, row0, rows, cbase + 32 * c, stage_warp, Cfg::ROW_BYTES, lane);
+            __syncwarp();
           }
         } else if (rows > 0) {
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage_row + 16 * j) = make_uint4(0, 0, 0, 0);
           __syncwarp();
-          for (int c = 0; c < nch; ++c) {
-            if constexpr (F32) {
-              for (int h = 0; h < 32; h += 16)
-                ragged_flush_f32(static_cast<float*>(pr.c), ld, pr.c_vec, row0, rows, cbase + 32 * c + h, stage_warp,
-                                 Cfg::ROW_BYTES, lane, false, false);
-            } else {
-              ragged_flush(out, ld, pr.c_vec, row0, rows, cbase + 32 * c, stage_warp, Cfg::ROW_BYTES, lane);
-            }
-          }
+          for (int c = 0; c < nch; ++c)
+            ragged_flush(out, ld, pr.c_vec, row0, rows, cbase + 32 * c, stage_warp, Cfg::ROW_BYTES, lane);
         }
-      }
-      if (t.kind == RT_MMA) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR)
-            mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));  // the leader's MMA warp waits on it
-          else
-            mbar_arrive(&tempty[acc]);
-        }
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1u;
+        if (mma) release();
       }
     }
   }
