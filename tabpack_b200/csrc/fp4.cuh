@@ -366,13 +366,15 @@ struct Fp4Cfg {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;
   static constexpr int STAGES = PAIR ? 4 : BN == 256 ? 3 : BN == 128 ? 5 : 6;
   static constexpr int ACCS = BN == 256 ? 1 : 2;
-  static constexpr int SA_COL = ACCS * BN, SB_COL = SA_COL + 16;  // tensor memory columns of the scales
+  // tensor memory columns: accumulators, then buffers of a stage's scales (of x, of w)
+  static constexpr int SA_COLS = 4 * ATOMS, SB_COLS = 4 * ATOMS * SB_TILES, S_COL = ACCS * BN, S_COLS = SA_COLS + SB_COLS;
   static constexpr int TMEM_COLS = BN == 64 ? 256 : 512;
-  static_assert(SB_COL + SB_TILES * ATOMS * 4 <= TMEM_COLS, "tensor memory");
-  static constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
-  static constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
+  static constexpr int SBUFS = 4;
+  static_assert(S_COL + SBUFS * S_COLS <= TMEM_COLS, "tensor memory");
+  static constexpr int EPI_WARP0 = 4, EPI_WARPS = 8, SCALE_WARP0 = EPI_WARP0 + EPI_WARPS, SCALE_WARPS = 2;
+  static constexpr int THREADS = 32 * (SCALE_WARP0 + SCALE_WARPS);
   static constexpr int TRING = 4;
-  static constexpr int CTRL_BYTES = 512;
+  static constexpr int CTRL_BYTES = 512;  // barriers (384 bytes), tiles
   static constexpr int ROW_BYTES = 144;  // a warp's staged row of 32 values, padded
   static constexpr int WCOLS = BN / 2;
   static constexpr int SMEM_BYTES =
@@ -443,10 +445,13 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
   constexpr int TRING = Cfg::TRING;
   uint64_t* tr_full = done_bar + 1;
   uint64_t* tr_empty = tr_full + TRING;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tr_empty + TRING);
+  uint64_t* s_ready = tr_empty + TRING;          // a buffer of scales is in tensor memory
+  uint64_t* s_free = s_ready + Cfg::SBUFS;       // the products that read it have completed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_free + Cfg::SBUFS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* ring = reinterpret_cast<volatile int*>(ctrl + 256);
-  static_assert(8 * (2 * Cfg::STAGES + 5 + 2 * TRING) + 8 <= 256 && 256 + 32 * TRING <= Cfg::CTRL_BYTES, "control block");
+  volatile int* ring = reinterpret_cast<volatile int*>(ctrl + 384);
+  static_assert(8 * (2 * Cfg::STAGES + 5 + 2 * TRING + 2 * Cfg::SBUFS) + 8 <= 384 && 384 + 32 * TRING <= Cfg::CTRL_BYTES,
+                "control block");
   const int warp = warp_id(), lane = lane_id();
   const int rank = PAIR ? (int)cluster_ctarank() : 0;
   const int worker = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, workers = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
@@ -488,6 +493,10 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
+    for (int i = 0; i < Cfg::SBUFS; ++i) {
+      mbar_init(&s_ready[i], Cfg::SCALE_WARPS);
+      mbar_init(&s_free[i], 1);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
       mbar_init(&tempty[i], PAIR ? 2 * Cfg::EPI_WARPS : Cfg::EPI_WARPS);  // the leader's counts both CTAs
@@ -495,7 +504,7 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
     mbar_init(done_bar, 1);
     for (int i = 0; i < TRING; ++i) {
       mbar_init(&tr_full[i], 1);
-      mbar_init(&tr_empty[i], (rank == 0 ? 3 : 2) + Cfg::EPI_WARPS);  // producers, MMA warp, epilogue warps
+      mbar_init(&tr_empty[i], (rank == 0 ? 3 + Cfg::SCALE_WARPS : 2) + Cfg::EPI_WARPS);  // producers, MMA, scales, epilogue
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -564,12 +573,11 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
     // ------------------------------------------------------------------ MMA (a pair's leader fills both CTAs' TMEM)
     if (lane == 0 && rank == 0) {
       int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
+      uint32_t acc_phase = 0;
       bool ok = true;
       // descriptors of the first stage; the address field counts 16 bytes
       const uint64_t adesc0 = smem_desc_sw128(smem_u32(smA), 16, 1024), bdesc0 = smem_desc_sw128(smem_u32(smB), 16, 1024);
-      const uint64_t sadesc0 = scale_desc(smem_u32(smSA)), sbdesc0 = scale_desc(smem_u32(smSB));
-      const uint32_t sa_tmem = tmem_base + Cfg::SA_COL, sb_tmem = tmem_base + Cfg::SB_COL;
+      uint32_t buf = 0, buf_phase = 0;
       for (int k = 0; ok; ++k) {
         const Fp4Tile t = ring_read(k, false);
         if (t.kind == FT_END) break;
@@ -579,40 +587,35 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
                                    idesc_fp4<FORMAT>(n_mma, FORMAT == FP4_NV ? 0 : 2, Cfg::TILE_M)};
         const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
         // tiles of 64 columns take one half of a scale tile of 128
-        const uint32_t sb_at = sb_tmem + (BN == 64 ? (uint32_t)(t.nt & 1) * 2u : 0u);
+        const uint32_t sb_shift = BN == 64 ? (uint32_t)(t.nt & 1) * 2u : 0u;
         const int kblocks = k_blocks(t.member);
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, abort_flag)) break;
         tc_fence_after();
         for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait(&full[stage], phase, abort_flag)) {
+          if (!mbar_wait(&s_ready[buf], buf_phase, abort_flag)) {  // (the stage has landed before)
             ok = false;
             break;
           }
           tc_fence_after();
           const uint64_t ad = adesc0 + (uint64_t)(stage * (Cfg::A_BYTES / 16)), bd = bdesc0 + (uint64_t)(stage * (Cfg::B_BYTES / 16));
-          const uint64_t sad = sadesc0 + (uint64_t)(stage * (Cfg::SA_BYTES / 16)), sbd = sbdesc0 + (uint64_t)(stage * (Cfg::SB_BYTES / 16));
-          // a product's columns of w take consecutive columns of scales: tile c of step i at (i * tiles + c) * 4
-#pragma unroll
-          for (int i = 0; i < Cfg::ATOMS; ++i) {
-            tmem_copy_scales<PAIR>(sa_tmem + 4 * i, sad + 32 * i);
-#pragma unroll
-            for (int c = 0; c < Cfg::SB_TILES; ++c)
-              tmem_copy_scales<PAIR>(sb_tmem + 4 * (i * Cfg::SB_TILES + c), sbd + 32 * (c * Cfg::ATOMS + i));
-          }
+          const uint32_t sa_at = tmem_base + Cfg::S_COL + buf * Cfg::S_COLS, sb_at = sa_at + Cfg::SA_COLS + sb_shift;
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
             const int i = FORMAT == FP4_NV ? s : s >> 1;
-            umma_fp4<FORMAT, PAIR>(d_tmem, ad + 2 * s, bd + 2 * s, idesc[s & 1], sa_tmem + 4 * i, sb_at + 4 * i * Cfg::SB_TILES,
-                             (kb | s) != 0 ? 1u : 0u);
+            umma_fp4<FORMAT, PAIR>(d_tmem, ad + 2 * s, bd + 2 * s, idesc[s & 1], sa_at + 4 * i, sb_at + 4 * i * Cfg::SB_TILES,
+                                   (kb | s) != 0 ? 1u : 0u);
           }
+          if constexpr (PAIR)
+            umma_commit_pair(smem_u32(&s_free[buf]));
+          else
+            umma_commit(&s_free[buf]);
+          buf = (buf + 1) % Cfg::SBUFS;
+          if (buf == 0) buf_phase ^= 1u;
           if constexpr (PAIR)
             umma_commit_both(&empty[stage]);
           else
             umma_commit(&empty[stage]);
-          if (++stage == Cfg::STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          if (++stage == Cfg::STAGES) stage = 0;
         }
         if (!ok) break;
         if constexpr (PAIR)
@@ -630,6 +633,50 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
         umma_commit(done_bar);
       volatile int no_abort = 0;
       mbar_wait(done_bar, 0, &no_abort);
+    }
+  } else if (warp >= Cfg::SCALE_WARP0) {
+    // ------------------------------------------------------------------ scales to tensor memory, half of a stage a warp
+    // (a thread takes some 36 cycles to issue each of these instructions: with the copies on the thread of the products
+    // a stage took 1400 cycles instead of the products' 512, the copies one stage ahead 1300, on one thread of their own 1090)
+    if (lane == 0 && rank == 0) {
+      const uint64_t sadesc0 = scale_desc(smem_u32(smSA)), sbdesc0 = scale_desc(smem_u32(smSB));
+      int stage = 0;
+      uint32_t phase = 0, buf = 0, buf_phase = 0;
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        const Fp4Tile t = ring_read(k, false);
+        if (t.kind == FT_END) break;
+        if (t.kind != FT_MMA) continue;
+        const int kblocks = k_blocks(t.member);
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait(&full[stage], phase, abort_flag) || !mbar_wait(&s_free[buf], buf_phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t sad = sadesc0 + (uint64_t)(stage * (Cfg::SA_BYTES / 16)), sbd = sbdesc0 + (uint64_t)(stage * (Cfg::SB_BYTES / 16));
+          const uint32_t sa_tmem = tmem_base + Cfg::S_COL + buf * Cfg::S_COLS, sb_tmem = sa_tmem + Cfg::SA_COLS;
+          // a product's columns of w take consecutive columns of scales: tile c of step i at (i * tiles + c) * 4
+#pragma unroll
+          for (int h = 0; h < Cfg::ATOMS / 2; ++h) {
+            const int i = h + (warp - Cfg::SCALE_WARP0) * (Cfg::ATOMS / 2);
+            tmem_copy_scales<PAIR>(sa_tmem + 4 * i, sad + 32 * i);
+#pragma unroll
+            for (int c = 0; c < Cfg::SB_TILES; ++c)
+              tmem_copy_scales<PAIR>(sb_tmem + 4 * (i * Cfg::SB_TILES + c), sbd + 32 * (c * Cfg::ATOMS + i));
+          }
+          if constexpr (PAIR)
+            umma_commit_pair(smem_u32(&s_ready[buf]));
+          else
+            umma_commit(&s_ready[buf]);
+          buf = (buf + 1) % Cfg::SBUFS;
+          if (buf == 0) buf_phase ^= 1u;
+          if (++stage == Cfg::STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ scheduler
@@ -751,6 +798,70 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
         tc_fence_after();
       }
       const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * WCOLS);
+      auto release = [&]() {  // the accumulator has been read
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR)
+            mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));  // the leader's MMA thread waits on it
+          else
+            mbar_arrive(&tempty[acc]);
+        }
+        if (++acc == Cfg::ACCS) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      };
+      if (mma && !pr.y_f32 && pr.y_vec) {
+        // bf16: the whole slice goes to registers, rounded, before the accumulator is given back (there is one)
+        uint32_t y[WCOLS / 2];
+#pragma unroll
+        for (int c = 0; c < WCOLS; c += 16) {
+          uint32_t v[16];
+          tmem_ld_32x32b_x16(t_row + (uint32_t)c, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            const float4 sc = *reinterpret_cast<const float4*>(sscale + c + j), bi = *reinterpret_cast<const float4*>(sbias + c + j);
+            float x0 = fmaf(__uint_as_float(v[j]) * rs, sc.x, bi.x), x1 = fmaf(__uint_as_float(v[j + 1]) * rs, sc.y, bi.y);
+            float x2 = fmaf(__uint_as_float(v[j + 2]) * rs, sc.z, bi.z), x3 = fmaf(__uint_as_float(v[j + 3]) * rs, sc.w, bi.w);
+            if (pr.relu) x0 = max_nan(x0, 0.f), x1 = max_nan(x1, 0.f), x2 = max_nan(x2, 0.f), x3 = max_nan(x3, 0.f);
+            y[(c + j) / 2] = pack_bf16x2(x0, x1);
+            y[(c + j) / 2 + 1] = pack_bf16x2(x2, x3);
+          }
+        }
+        release();
+        if (rows > 0) {
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(pr.y);
+          const int nv = t.n_valid - cbase;  // (columns behind the member's: zeros, whatever was multiplied there)
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) {
+            if (c < nch) {
+              __syncwarp();
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int col = 32 * c + 2 * (j + e);
+                  w[e] = col + 1 < nv ? y[16 * c + j + e] : col < nv ? y[16 * c + j + e] & 0xFFFFu : 0u;
+                }
+                *reinterpret_cast<uint4*>(stage_row + 4 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+              __syncwarp();
+              const int p = lane & 3, col0 = cbase + 32 * c + 8 * p;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int r = (lane >> 2) + 8 * i;
+                if (r < rows && col0 < pr.N)
+                  *reinterpret_cast<uint4*>(out + (row0 + r) * pr.N + col0) =
+                      *reinterpret_cast<const uint4*>(stage_warp + r * Cfg::ROW_BYTES + 16 * p);
+              }
+            }
+          }
+        }
+        continue;
+      }
       if (rows > 0) {
 #pragma unroll 1
         for (int c = 0; c < nch; ++c) {
@@ -805,20 +916,7 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
           }
         }
       }
-      if (mma) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR)
-            mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));  // the leader's MMA thread waits on it
-          else
-            mbar_arrive(&tempty[acc]);
-        }
-        if (++acc == Cfg::ACCS) {
-          acc = 0;
-          acc_phase ^= 1u;
-        }
-      }
+      if (mma) release();
     }
   }
 
