@@ -109,68 +109,66 @@ __device__ __forceinline__ uint32_t fp4_pack8(const float (&q)[8]) {
   return r;
 }
 
-// One block's codes and scale byte from its values; `row` is the row's 2^r (nvfp4).
-template <int FORMAT, int N>
-__device__ __forceinline__ uint8_t fp4_block(const float (&x)[N], float row, uint32_t (&codes)[N / 8]) {
-  float big = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) big = fmaxf(big, fabsf(x[i]));
-  float s;
-  uint8_t byte;
+__device__ __forceinline__ float e4m3_value(uint32_t byte) {  // (of a byte without a sign)
+  const uint32_t e = byte >> 3, f = byte & 7u;
+  return e ? __uint_as_float(((e + 120u) << 23) | (f << 20)) : (float)f * 0.001953125f;
+}
+
+// e4m3(big / (6 row)): the quotient correctly rounded first (Markstein: one correction by the exact remainder).
+__device__ __forceinline__ uint8_t nvfp4_scale_byte(float big, float row_inverse) {
+  const float t = big * row_inverse, sixth = 0.16666667f;
+  const float q = t * sixth;
+  return (uint8_t)__nv_cvt_float_to_fp8(fmaf(fmaf(-q, 6.f, t), sixth, q), __NV_SATFINITE, __NV_E4M3);
+}
+
+// A block's scale byte from its largest magnitude, its scale s and that one's reciprocal; `row` is the row's 2^r (nvfp4),
+// row_inverse its reciprocal.
+template <int FORMAT>
+__device__ __forceinline__ uint8_t fp4_scale(float big, float row, float row_inverse, float& s, float& inv) {
   if constexpr (FORMAT == FP4_NV) {
-    byte = (uint8_t)__nv_cvt_float_to_fp8(__fdiv_rn(big, 6.f * row), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t e = byte >> 3, f = byte & 7u;
-    s = (e ? __uint_as_float(((e + 120u) << 23) | (f << 20)) : (float)f * 0.001953125f) * row;
+    const uint8_t byte = nvfp4_scale_byte(big, row_inverse);
+    const float small = e4m3_value(byte);
+    s = small * row;
+    inv = small > 0.f ? __frcp_rn(small) * row_inverse : 0.f;
+    return byte;
   } else {
     const int e = max((int)(__float_as_uint(big) >> 23) - 129, -100);
-    byte = (uint8_t)(e + 127);
     s = pow2f(e);
+    inv = pow2f(-e);
+    return (uint8_t)(e + 127);
   }
-  const float inv = s > 0.f ? 1.f / s : 0.f;
-  const f32x2 inv2 = pair(inv, inv), neg2 = pair(-s, -s);
+}
+
+// Two values over s: the correctly rounded quotients, by the reciprocal and one correction (exact for a power of two).
+template <int FORMAT>
+__device__ __forceinline__ void fp4_quotients(float& x, float& y, float s, float inv) {
+  const f32x2 v = pair(x, y), i = pair(inv, inv);
+  f32x2 t = mul2(v, i);
+  if constexpr (FORMAT == FP4_NV) t = fma2(fma2(pair(-s, -s), t, v), i, t);
+  const float2 h = halves(t);
+  x = h.x;
+  y = h.y;
+}
+
+// One block's codes and scale byte from its values.
+template <int FORMAT, int N>
+__device__ __forceinline__ uint8_t fp4_block(const float (&x)[N], float row, float row_inverse, uint32_t (&codes)[N / 8]) {
+  float big = 0.f, s, inv;
+#pragma unroll
+  for (int i = 0; i < N; ++i) big = fmaxf(big, fabsf(x[i]));
+  const uint8_t byte = fp4_scale<FORMAT>(big, row, row_inverse, s, inv);
 #pragma unroll
   for (int j = 0; j < N / 8; ++j) {
     float q[8];
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-      const f32x2 v = pair(x[8 * j + i], x[8 * j + i + 1]);
-      f32x2 t = mul2(v, inv2);
-      // the correctly rounded quotient (Markstein: one correction by the exact remainder)
-      if constexpr (FORMAT == FP4_NV) t = fma2(fma2(neg2, t, v), inv2, t);
-      const float2 h = halves(t);
-      q[i] = h.x;
-      q[i + 1] = h.y;
+      q[i] = x[8 * j + i];
+      q[i + 1] = x[8 * j + i + 1];
+      fp4_quotients<FORMAT>(q[i], q[i + 1], s, inv);
     }
     codes[j] = fp4_pack8(q);
   }
   return byte;
-}
-
-// N values from column c on, zeros from column n on.  VEC: the row is on a 16-byte boundary, and so is c.
-template <typename T, int N, bool VEC>
-__device__ __forceinline__ void fp4_load(const T* x, int c, int n, float (&v)[N]) {
-  if (VEC && c + N <= n) {
-    constexpr int L = N * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T);
-    uint4 u[L];
-#pragma unroll
-    for (int i = 0; i < L; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(x + c) + i);
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(T) == 2) {
-          v[E * i + 2 * j] = __uint_as_float(w[j] << 16);
-          v[E * i + 2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-        } else {
-          v[E * i + j] = __uint_as_float(w[j]);
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = c + i < n ? (float)x[c + i] : 0.f;
-  }
 }
 
 // The largest magnitude of a row among the columns of this thread's part (of G), NaN if one is.
@@ -209,9 +207,9 @@ __device__ __forceinline__ float fp4_row_max(const T* x, int n, int at) {
   return big;
 }
 
-// G threads a row.  G = 32: a block takes 8 rows of a tile, i, i + 32, i + 64, i + 96 for two consecutive i, whose
+// Rows off 16-byte boundaries, element by element.  G threads a row.  G = 32: a block takes 8 rows of a tile, i, i + 32, i + 64, i + 96 for two consecutive i, whose
 // scale bytes make up whole 32-byte sectors of the tile.  G = 256: one row (few rows: latency counts).
-template <typename T, int FORMAT, int G, bool VEC>
+template <typename T, int FORMAT, int G>
 __global__ void __launch_bounds__(256) fp4_quantize_kernel(const Fp4QuantArgs a) {
   constexpr int N = FORMAT == FP4_NV ? 16 : 32;
   constexpr int PER = 128 * G / 256;  // blocks of the grid a tile
@@ -239,18 +237,21 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const Fp4QuantArgs a)
     }
   };
   if constexpr (FORMAT == FP4_NV) {
-    if (live) big = fp4_row_max<T, G, VEC>(x, n, at);
+    if (live) big = fp4_row_max<T, G, false>(x, n, at);
     row_max();
     scale = nvfp4_row_scale(big);
   }
   const int blocks = a.out.atoms * 4;  // with those of the padding, which are zero
   uint8_t* to = a.out.scales + (long long)tile * a.out.atoms * 512;
+  // (of a power of two from 2^-100 to 2^117)
+  const float scale_inverse = __uint_as_float((254u << 23) - __float_as_uint(scale));
   const bool zero = !live || (FORMAT == FP4_NV && !(big < INFINITY));
   for (int b = at; b < blocks; b += G) {
     float v[N];
-    fp4_load<T, N, VEC>(x, b * N, zero ? 0 : n, v);
+    #pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = !zero && b * N + i < n ? (float)x[b * N + i] : 0.f;
     uint32_t codes[N / 8];
-    const uint8_t byte = fp4_block<FORMAT, N>(v, scale, codes);
+    const uint8_t byte = fp4_block<FORMAT, N>(v, scale, scale_inverse, codes);
     if constexpr (FORMAT == FP4_MX) {
 #pragma unroll
       for (int i = 0; i < N; ++i) big = max_nan(big, fabsf(v[i]));
@@ -266,6 +267,269 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const Fp4QuantArgs a)
   }
   if constexpr (FORMAT == FP4_MX) row_max();
   if (live && at == 0) a.out.row_scale[row] = big < INFINITY ? scale : __uint_as_float(0x7FC00000u);
+}
+
+// Rows on 16-byte boundaries go by vectors of 16 bytes, consecutive threads of a row's G consecutive ones; the 2 to 8 lanes
+// of a block of columns find its scale together.  The scales' values and reciprocals come from a table by their byte.
+struct Fp4Row {
+  long long row;
+  int n;              // columns that count
+  bool live;
+  uint8_t* scales;    // of this row in its tile
+};
+// Row r of a tile; false where the tile has none.
+__device__ __forceinline__ bool fp4_row(const Fp4QuantArgs& a, long long tile, int r, Fp4Row& q) {
+  int m, rows;
+  long long row0;
+  if (!fp4_tile(a.groups, tile, m, row0, rows)) return false;
+  q.live = r < rows;
+  q.row = row0 + r;
+  q.n = q.live ? (a.n_features ? min(__ldg(a.n_features + m), a.K) : a.K) : 0;
+  q.scales = a.out.scales + tile * a.out.atoms * 512 + (r & 31) * 16 + (r >> 5) * 4;
+  return true;
+}
+
+// The largest magnitude of a vector, NaN if it holds one.
+template <typename T>
+__device__ __forceinline__ float fp4_largest(const uint4& q) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  if constexpr (sizeof(T) == 2) {
+    // magnitudes of bf16 are in the order of their bits, NaN above infinity
+    uint32_t k = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+    for (int j = 1; j < 4; ++j) k = __vmaxu2(k, w[j] & 0x7FFF7FFFu);
+    return max_nan(__uint_as_float(k << 16), __uint_as_float(k & 0xFFFF0000u));
+  } else {
+    return max_nan(max_nan(fabsf(__uint_as_float(w[0])), fabsf(__uint_as_float(w[1]))),
+                   max_nan(fabsf(__uint_as_float(w[2])), fabsf(__uint_as_float(w[3]))));
+  }
+}
+
+// A vector's codes and, by the first lane of a block of columns, its scale byte.  `most`: the vector's largest magnitude;
+// zero: a row that is not finite.
+template <typename T, int FORMAT>
+__device__ __forceinline__ void fp4_vector(const Fp4QuantArgs& a, const Fp4Row& row, const float2* table, int v, const uint4& u,
+                                           float most, float scale, float scale_inverse, bool zero) {
+  constexpr int N = FORMAT == FP4_NV ? 16 : 32, E = 16 / (int)sizeof(T), L = N / E;
+  const int b = v / L;
+#pragma unroll
+  for (int o = 1; o < L; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+  float s, inv;
+  uint8_t byte;
+  if constexpr (FORMAT == FP4_NV) {
+    byte = zero ? (uint8_t)0 : nvfp4_scale_byte(most, scale_inverse);
+    const float2 e = table[byte];
+    s = e.x * scale;
+    inv = e.y * scale_inverse;
+  } else {
+    byte = fp4_scale<FP4_MX>(most, 1.f, 1.f, s, inv);
+  }
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  float q[8] = {};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 2) {
+      q[2 * j] = __uint_as_float(w[j] << 16);
+      q[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+    } else {
+      q[j] = __uint_as_float(w[j]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < E; i += 2) fp4_quotients<FORMAT>(q[i], q[i + 1], s, inv);
+  const uint32_t c = zero ? 0u : fp4_pack8(q);
+  if (b < a.out.atoms * 4) {  // (the padding's blocks too: zero)
+    if (v % L == 0) row.scales[(b >> 2) * 512 + (b & 3)] = row.live && b * N < a.K ? byte : (uint8_t)0;
+    if (row.live && v * (E / 2) < a.out.pitch) {
+      uint8_t* codes = a.out.codes + row.row * a.out.pitch;
+      if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint32_t*>(codes + v * 4) = c;
+      else
+        *reinterpret_cast<uint16_t*>(codes + v * 2) = (uint16_t)c;
+    }
+  }
+}
+
+__device__ __forceinline__ void fp4_table(float2* table) {  // value and reciprocal of an e4m3 byte (0 of 0)
+  for (int i = threadIdx.x; i < 128; i += blockDim.x) {
+    const float v = e4m3_value(i);
+    table[i] = make_float2(v, v > 0.f ? __frcp_rn(v) : 0.f);
+  }
+}
+
+// Element c on of a row, zeros from column n on.
+template <typename T>
+__device__ __forceinline__ uint4 fp4_load(const T* x, int c, int n) {
+  constexpr int E = 16 / (int)sizeof(T);
+  if (c + E <= n) return __ldg(reinterpret_cast<const uint4*>(x + c));
+  T e[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) e[i] = c + i < n ? x[c + i] : (T)0.f;
+  return *reinterpret_cast<const uint4*>(e);
+}
+
+// G threads a row, H vectors at a time; a block of the grid takes four rows (i, i + 32, i + 64, i + 96 of a tile), or one with
+// G = 256.  nvfp4 reads a row twice (for its largest magnitude first), mxfp4 once
+// (16384 rows of 8192 fp32: 113 us, 5.4 TB/s; 140 with a thread's own block by strided vectors, 171 by way of shared memory).
+template <typename T, int FORMAT, int G, int H>
+__global__ void __launch_bounds__(G == 256 ? 256 : 4 * G) fp4_quantize_rows_kernel(const Fp4QuantArgs a) {
+  constexpr int N = FORMAT == FP4_NV ? 16 : 32, E = 16 / (int)sizeof(T), L = N / E;
+  constexpr int ROWS = G == 256 ? 1 : 4, PER = 128 / ROWS;
+  __shared__ float2 table[128];
+  __shared__ float warp_max[ROWS * G / 32];
+  const int tile = blockIdx.x / PER, part = blockIdx.x % PER;
+  const int at = threadIdx.x % G, lane = threadIdx.x & 31;
+  Fp4Row q;
+  if (!fp4_row(a, tile, ROWS == 1 ? part : part + 32 * (int)(threadIdx.x / G), q)) return;
+  if (FORMAT == FP4_NV) fp4_table(table);
+  const T* x = static_cast<const T*>(a.x) + q.row * a.ld;
+  float big = 0.f;
+  auto row_max = [&]() {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) big = max_nan(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+    if constexpr (G > 32) {
+      if (lane == 0) warp_max[threadIdx.x >> 5] = big;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < G / 32; ++w) big = max_nan(big, warp_max[threadIdx.x / G * (G / 32) + w]);
+    }
+  };
+  float scale = 1.f;
+  if constexpr (FORMAT == FP4_NV) {
+    if (q.live) big = fp4_row_max<T, G, true>(x, q.n, at);
+    row_max();
+    if constexpr (G == 32) __syncthreads();  // (the table)
+    scale = nvfp4_row_scale(big);
+  }
+  const bool zero = FORMAT == FP4_NV && !(big < INFINITY);
+  const float scale_inverse = __uint_as_float((254u << 23) - __float_as_uint(scale));  // (of a power of two)
+  const int vecs = a.out.atoms * 4 * L;
+  for (int v0 = 0; v0 < vecs; v0 += G * H) {
+    uint4 u[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) u[h] = fp4_load<T>(x, (v0 + h * G + at) * E, q.n);
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      if (v0 + h * G >= vecs) break;  // (the same for all of the block's threads)
+      const float most = fp4_largest<T>(u[h]);
+      if constexpr (FORMAT == FP4_MX) big = max_nan(big, most);
+      fp4_vector<T, FORMAT>(a, q, table, v0 + h * G + at, u[h], most, scale, scale_inverse, zero);
+    }
+  }
+  if constexpr (FORMAT == FP4_MX) row_max();
+  if (q.live && at == 0) a.out.row_scale[q.row] = big < INFINITY ? scale : __uint_as_float(0x7FC00000u);
+}
+
+// nvfp4 of rows that G threads hold at once (G H vectors), read once: a block goes through groups of four rows, the next one's
+// vectors on their way to shared memory meanwhile, since a row's scale needs its largest magnitude before the first code.  A
+// warp's vectors come in as they lie in memory and are dealt out again so that a lane has whole blocks of columns.
+// (16384 rows of 8192 bf16: 98 us in two passes, of which the second misses L2 by half; 88 us with a vector a lane, the block's
+// scale found by two of them with shuffles, 150 instructions a vector; 80 us like this, 4.3 TB/s.  The instructions still bound it.)
+template <typename T, int G, int H>
+__global__ void __launch_bounds__(4 * G, 256 / G) fp4_quantize_stream_kernel(const Fp4QuantArgs a, const long long groups) {
+  constexpr int N = 16, E = 16 / (int)sizeof(T), L = N / E;  // columns of a block, of a vector; vectors of a block
+  static_assert(H % L == 0, "whole blocks");
+  extern __shared__ uint4 slots[];  // [2][H][threads]
+  __shared__ float2 table[128];
+  __shared__ float warp_max[2][G / 8];
+  const int at = threadIdx.x % G, lane = threadIdx.x & 31, sub = threadIdx.x / G;
+  const int blocks = a.out.atoms * 4;  // with those of the padding, which are zero
+  fp4_table(table);
+  __syncthreads();
+  auto slot = [&](int stage, int h) -> uint4* { return slots + (stage * H + h) * (4 * G) + threadIdx.x; };
+  auto fetch = [&](long long group, int stage, Fp4Row& q) -> bool {
+    bool ok = false;
+    if (group < groups) {
+      ok = fp4_row(a, group / 32, (int)(group % 32) + 32 * sub, q);
+      if (ok) {
+        const T* x = static_cast<const T*>(a.x) + q.row * a.ld;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const int c = (h * G + at) * E;
+          if (c + E <= q.n)
+            cp_async16(smem_u32(slot(stage, h)), x + c);
+          else
+            *slot(stage, h) = fp4_load<T>(x, c, q.n);
+        }
+      }
+    }
+    cp_async_commit();
+    return ok;
+  };
+  Fp4Row now, then;
+  now.row = then.row = 0;
+  now.live = then.live = false;
+  int stage = 0;
+  bool here = fetch(blockIdx.x, 0, now);
+  for (long long group = blockIdx.x; group < groups; group += gridDim.x, stage ^= 1) {
+    const bool there = fetch(group + gridDim.x, stage ^ 1, then);
+    cp_async_wait<1>();
+    __syncwarp();
+    if (here) {  // (of all threads of the row or none)
+      // of the L vectors h = p L.. of all lanes: this lane's block is number lane % (32 / L) of vector p L + lane / (32 / L)
+      uint4 u[H];
+      float most[H / L], big = 0.f;
+#pragma unroll
+      for (int p = 0; p < H / L; ++p) {
+        const uint4* from = slot(stage, p * L + lane / (32 / L)) - lane + L * (lane % (32 / L));
+        most[p] = 0.f;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+          u[p * L + i] = from[i];
+          most[p] = max_nan(most[p], fp4_largest<T>(u[p * L + i]));
+        }
+        big = max_nan(big, most[p]);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) big = max_nan(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+      if constexpr (G > 32) {
+        if (lane == 0) warp_max[stage][threadIdx.x >> 5] = big;
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + sub), "n"(G) : "memory");  // the row's threads
+#pragma unroll
+        for (int w = 0; w < G / 32; ++w) big = max_nan(big, warp_max[stage][sub * (G / 32) + w]);
+      }
+      const float scale = nvfp4_row_scale(big);
+      const float scale_inverse = __uint_as_float((254u << 23) - __float_as_uint(scale));  // (of a power of two)
+      const bool zero = !(big < INFINITY);
+      if (now.live && at == 0) a.out.row_scale[now.row] = zero ? __uint_as_float(0x7FC00000u) : scale;
+#pragma unroll
+      for (int p = 0; p < H / L; ++p) {
+        const int v = (p * L + lane / (32 / L)) * G + (at - lane) + L * (lane % (32 / L)), b = v / L;
+        if (b >= blocks) continue;
+        const uint8_t byte = zero ? (uint8_t)0 : nvfp4_scale_byte(most[p], scale_inverse);
+        const float2 e = table[byte];
+        const float s = e.x * scale, inv = e.y * scale_inverse;
+        now.scales[(b >> 2) * 512 + (b & 3)] = now.live && b * N < a.K ? byte : (uint8_t)0;
+        if (now.live && b * (N / 2) < a.out.pitch) {
+          uint32_t c[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float q[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (sizeof(T) == 2) {
+                const uint4& w4 = u[p * L + j];
+                const uint32_t w = i == 0 ? w4.x : i == 1 ? w4.y : i == 2 ? w4.z : w4.w;
+                q[2 * i] = __uint_as_float(w << 16);
+                q[2 * i + 1] = __uint_as_float(w & 0xFFFF0000u);
+              } else {
+                const uint4& w4 = u[p * L + 2 * j + i / 2];
+                q[2 * i] = __uint_as_float(i & 1 ? w4.z : w4.x);
+                q[2 * i + 1] = __uint_as_float(i & 1 ? w4.w : w4.y);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) fp4_quotients<FP4_NV>(q[i], q[i + 1], s, inv);
+            c[j] = zero ? 0u : fp4_pack8(q);
+          }
+          *reinterpret_cast<uint2*>(a.out.codes + now.row * a.out.pitch + b * (N / 2)) = make_uint2(c[0], c[1]);
+        }
+      }
+    }
+    __syncwarp();  // (the slots are filled again by the next turn's copies)
+    now = then;
+    here = there;
+  }
 }
 
 struct Fp4ValuesArgs {

@@ -568,15 +568,40 @@ Fp4Rows fp4_rows(const tp_fp4_args* a) {
 // row's pieces one after the other.
 constexpr long long FP4_FEW_TILES = 8;
 
+// nvfp4 of rows of at most 4 G vectors: groups of four rows through shared memory, 1024 threads an SM.
+template <typename T, int G>
+int launch_stream(const Fp4QuantArgs& k, long long tiles, cudaStream_t st) {
+  constexpr auto kern = fp4_quantize_stream_kernel<T, G, 4>;
+  constexpr size_t smem = (size_t)2 * 4 * 4 * G * 16;
+  int rc = allow_smem<kern>(smem);
+  if (rc) return rc;
+  const long long groups = tiles * 32, most = (long long)device_info().sms * (256 / G);
+  kern<<<(unsigned)std::min(groups, most), 4 * G, smem, st>>>(k, groups);
+  return TP_OK;
+}
+
 template <typename T, int FORMAT>
 int launch_quantize(const Fp4QuantArgs& k, bool vec, cudaStream_t st) {
   const long long tiles = fp4_row_tiles(k.groups);
   const bool few = tiles <= FP4_FEW_TILES;
   const long long blocks = tiles * (few ? 128 : 16);
-  if (blocks > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many rows");
-  auto kern = few ? (vec ? fp4_quantize_kernel<T, FORMAT, 256, true> : fp4_quantize_kernel<T, FORMAT, 256, false>)
-                  : (vec ? fp4_quantize_kernel<T, FORMAT, 32, true> : fp4_quantize_kernel<T, FORMAT, 32, false>);
-  kern<<<(unsigned)blocks, 256, 0, st>>>(k);
+  if (tiles * 128 > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many rows");
+  if (!vec) {
+    (few ? fp4_quantize_kernel<T, FORMAT, 256> : fp4_quantize_kernel<T, FORMAT, 32>)<<<(unsigned)blocks, 256, 0, st>>>(k);
+    return TP_OK;
+  }
+  constexpr int E = 16 / (int)sizeof(T);
+  if (few) {
+    fp4_quantize_rows_kernel<T, FORMAT, 256, 4><<<(unsigned)(tiles * 128), 256, 0, st>>>(k);
+    return TP_OK;
+  }
+  if constexpr (FORMAT == FP4_NV) {
+    if (k.K <= 32 * 4 * E) return launch_stream<T, 32>(k, tiles, st);
+    if (k.K <= 64 * 4 * E) return launch_stream<T, 64>(k, tiles, st);
+    if (k.K <= 128 * 4 * E) return launch_stream<T, 128>(k, tiles, st);
+    if (k.K <= 256 * 4 * E) return launch_stream<T, 256>(k, tiles, st);
+  }
+  fp4_quantize_rows_kernel<T, FORMAT, 32, 4><<<(unsigned)(tiles * 32), 128, 0, st>>>(k);
   return TP_OK;
 }
 
