@@ -173,30 +173,39 @@ int rows_vector(const tp_rows_args* a) {
 
 enum { ROWS_DISPATCH, ROWS_COMBINE, ROWS_BACKWARD };
 
+template <typename T, int BYTES, int U>
+void launch_rows_backward(const RowsArgs& k, cudaStream_t st) {
+  if (k.vecs <= 16)
+    rows_combine_backward_kernel<T, BYTES, 8, U><<<(k.T + 31) / 32, 256, 0, st>>>(k);
+  else if (k.vecs <= 128)
+    rows_combine_backward_kernel<T, BYTES, 32, U><<<(k.T + 7) / 8, 256, 0, st>>>(k);
+  else
+    rows_combine_backward_kernel<T, BYTES, 256, U><<<k.T, 256, 0, st>>>(k);
+}
+
 template <typename T, int BYTES>
 int launch_rows(RowsArgs k, int what, cudaStream_t st) {
   k.vecs = k.W / (BYTES / (int)sizeof(T));
   k.div_vecs = make_fastdiv((uint32_t)k.vecs);
-  if (what != ROWS_BACKWARD) {
-    const long long blocks = ((long long)k.T * k.vecs + 255) / 256;
-    if (blocks > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many elements for one row move");
-    if (what == ROWS_DISPATCH)
-      rows_dispatch_kernel<T, BYTES><<<(unsigned)blocks, 256, 0, st>>>(k);
-    else if (k.k == 1)
-      rows_combine_kernel<T, BYTES, 1><<<(unsigned)blocks, 256, 0, st>>>(k);
-    else if (k.k == 2)
-      rows_combine_kernel<T, BYTES, 2><<<(unsigned)blocks, 256, 0, st>>>(k);
-    else if (k.k == 3)
-      rows_combine_kernel<T, BYTES, 3><<<(unsigned)blocks, 256, 0, st>>>(k);
-    else
-      rows_combine_kernel<T, BYTES, 4><<<(unsigned)blocks, 256, 0, st>>>(k);
-  } else if (k.vecs <= 16) {
-    rows_combine_backward_kernel<T, BYTES, 8><<<(k.T + 31) / 32, 256, 0, st>>>(k);
-  } else if (k.vecs <= 128) {
-    rows_combine_backward_kernel<T, BYTES, 32><<<(k.T + 7) / 8, 256, 0, st>>>(k);
-  } else {
-    rows_combine_backward_kernel<T, BYTES, 256><<<k.T, 256, 0, st>>>(k);
-  }
+  k.span = std::min(k.T, (0x7FFFFFFF - 1024) / k.vecs);
+  if (k.span < 1) return fail(TP_EINVAL, "rows too long for a row move");
+  // (four vectors a thread once the blocks, eight an SM, come in four rounds all the same)
+  const long long vecs = (long long)k.span * k.vecs;
+  k.turns = what == ROWS_COMBINE && vecs >= 4ll * 8 * 256 * device_info().sms ? 4 : 1;
+  const dim3 blocks((unsigned)((vecs + 256 * k.turns - 1) / (256 * k.turns)), (unsigned)(((long long)k.T + k.span - 1) / k.span));
+  if (blocks.y > 65535) return fail(TP_EINVAL, "too many elements for one row move");
+  if (what == ROWS_DISPATCH)
+    rows_dispatch_kernel<T, BYTES><<<blocks, 256, 0, st>>>(k);
+  else if (what == ROWS_COMBINE)
+    (k.k == 1   ? rows_combine_kernel<T, BYTES, 1>
+     : k.k == 2 ? rows_combine_kernel<T, BYTES, 2>
+     : k.k == 3 ? rows_combine_kernel<T, BYTES, 3>
+                : rows_combine_kernel<T, BYTES, 4>)<<<blocks, 256, 0, st>>>(k);
+  else
+    (k.k == 1   ? launch_rows_backward<T, BYTES, 1>
+     : k.k == 2 ? launch_rows_backward<T, BYTES, 2>
+     : k.k == 3 ? launch_rows_backward<T, BYTES, 3>
+                : launch_rows_backward<T, BYTES, 4>)(k, st);
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;
 }

@@ -399,6 +399,8 @@ struct RowsArgs {
   void* dy;                 // (T k, W), or null
   float* dw;                // (T, k), or null
   int vecs;                 // vectors of a row
+  int span;                 // rows of a grid row
+  int turns;                // vectors of a thread (combine)
   FastDiv div_vecs;
 };
 
@@ -434,25 +436,19 @@ __device__ __forceinline__ void row_store(void* p, long long elem, const RowVec<
     *reinterpret_cast<uint16_t*>(s) = *reinterpret_cast<const uint16_t*>(r.v);
 }
 
-// (row, vector) of each thread: 256 consecutive vectors of the whole table per block.
-__device__ __forceinline__ bool rows_place(const RowsArgs& a, int& t, int& c) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (long long)a.T * a.vecs) return false;
-  if (i < 0x7FFFFFFFLL) {
-    t = (int)fastdiv((uint32_t)i, a.div_vecs);
-    c = (int)((uint32_t)i - (uint32_t)t * (uint32_t)a.vecs);
-  } else {
-    t = (int)(i / a.vecs);
-    c = (int)(i - (long long)t * a.vecs);
-  }
-  return true;
+// (row, vector) of this thread: number i of a.span rows, which have fewer than 2^31 vectors.
+__device__ __forceinline__ bool rows_place(const RowsArgs& a, uint32_t i, int& t, int& c) {
+  const uint32_t r = fastdiv(i, a.div_vecs);
+  t = (int)(blockIdx.y * (uint32_t)a.span + r);
+  c = (int)(i - r * (uint32_t)a.vecs);
+  return r < (uint32_t)a.span && t < a.T;
 }
 
 template <typename T, int BYTES>
 __global__ void __launch_bounds__(256) rows_dispatch_kernel(const RowsArgs a) {
   using V = RowVec<T, BYTES>;
   int t, c;
-  if (!rows_place(a, t, c)) return;
+  if (!rows_place(a, blockIdx.x * 256 + threadIdx.x, t, c)) return;
   const int used = max(0, min(__ldg(a.offsets + a.E), a.T * a.k));
   const V x = row_load<T, BYTES>(a.x, (long long)t * a.x_ld + c * V::N);
   V zero;
@@ -464,44 +460,52 @@ __global__ void __launch_bounds__(256) rows_dispatch_kernel(const RowsArgs a) {
   }
 }
 
-// U rows on their way at a time (k of them where there are up to four).
+// U rows of a vector on their way at a time (k of them where there are up to four); a.turns vectors a thread, 256 apart.
+// (32768 rows of two of 4096 bf16 each: 152 us while a 64-bit index was taken apart on a branch, 134 without it, 119 with
+// four vectors a thread one after the other, 6.8 TB/s; four at once take more registers and 131 us.)
 template <typename T, int BYTES, int U>
 __global__ void __launch_bounds__(256) rows_combine_kernel(const RowsArgs a) {
   using V = RowVec<T, BYTES>;
-  int t, c;
-  if (!rows_place(a, t, c)) return;
   const int used = max(0, min(__ldg(a.offsets + a.E), a.T * a.k));
-  float s[V::N];
+#pragma unroll 1
+  for (int h = 0; h < a.turns; ++h) {
+    int t, c;
+    if (!rows_place(a, (blockIdx.x * a.turns + h) * 256 + threadIdx.x, t, c)) return;
+    float s[V::N];
 #pragma unroll
-  for (int i = 0; i < V::N; ++i) s[i] = 0.f;
-  for (int j0 = 0; j0 < a.k; j0 += U) {
-    int p[U];
-    float w[U];
-    V y[U];
+    for (int i = 0; i < V::N; ++i) s[i] = 0.f;
+    for (int j0 = 0; j0 < (U < 4 ? 1 : a.k); j0 += U) {
+      int p[U];
+      float w[U];
+      V y[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = U < 4 || j0 + u < a.k;
-      p[u] = in ? __ldg(a.position + (long long)t * a.k + j0 + u) : -1;
-      w[u] = in && a.weight ? __ldg(a.weight + (long long)t * a.k + j0 + u) : 1.f;
+      for (int u = 0; u < U; ++u) {
+        const bool in = U < 4 || j0 + u < a.k;
+        p[u] = in ? __ldg(a.position + (long long)t * a.k + j0 + u) : -1;
+        w[u] = in && a.weight ? __ldg(a.weight + (long long)t * a.k + j0 + u) : 1.f;
+      }
+      // (a row that takes no part is replaced by row 0, so that the loads need not wait for one another's conditions)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        y[u] = row_load<T, BYTES>(a.x, ((unsigned)p[u] < (unsigned)used ? (long long)p[u] : 0ll) * a.x_ld + c * V::N);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool there = (unsigned)p[u] < (unsigned)used;
+#pragma unroll
+        for (int i = 0; i < V::N; ++i) s[i] = there ? fmaf(w[u], (float)y[u].v[i], s[i]) : s[i];
+      }
     }
-    // (a row that takes no part is replaced by row 0, so that the loads need not wait for one another's conditions)
+    V out;
 #pragma unroll
-    for (int u = 0; u < U; ++u) y[u] = row_load<T, BYTES>(a.x, ((unsigned)p[u] < (unsigned)used ? (long long)p[u] : 0ll) * a.x_ld + c * V::N);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool there = (unsigned)p[u] < (unsigned)used;
-#pragma unroll
-      for (int i = 0; i < V::N; ++i) s[i] = there ? fmaf(w[u], (float)y[u].v[i], s[i]) : s[i];
-    }
+    for (int i = 0; i < V::N; ++i) out.v[i] = (T)s[i];
+    row_store<T, BYTES>(a.out, (long long)t * a.W + c * V::N, out);
   }
-  V out;
-#pragma unroll
-  for (int i = 0; i < V::N; ++i) out.v[i] = (T)s[i];
-  row_store<T, BYTES>(a.out, (long long)t * a.W + c * V::N, out);
 }
 
-// G threads a row: dy's rows and the dot products <dout[t], y[position[t, j]]>.
-template <typename T, int BYTES, int G>
+// G threads a row: dy's rows and the dot products <dout[t], y[position[t, j]]>, of U slots at a time (all of them where there
+// are up to three), so that dout is loaded once for them.  (32768 rows of two of 4096 bf16: 234 -> 227 us, 5.9 TB/s; 1003 rows of
+// three of 771 fp32: 7.4 -> 6.6, and 9.5 with two slots at a time, one of them row 0 in vain.)
+template <typename T, int BYTES, int G, int U>
 __global__ void __launch_bounds__(256) rows_combine_backward_kernel(const RowsArgs a) {
   using V = RowVec<T, BYTES>;
   constexpr int WARPS = G > 32 ? G / 32 : 1;
@@ -510,37 +514,53 @@ __global__ void __launch_bounds__(256) rows_combine_backward_kernel(const RowsAr
   const int t = blockIdx.x * (256 / G) + group;
   const bool live = t < a.T;
   const int used = max(0, min(__ldg(a.offsets + a.E), a.T * a.k));
-  if (G > 32 || live) {
-    for (int j = 0; j < a.k; ++j) {
-      float dot = 0.f;
-      int p = -1;
-      if (live) {
-        p = __ldg(a.position + (long long)t * a.k + j);
-        const bool there = (unsigned)p < (unsigned)used, inside = (unsigned)p < (unsigned)(a.T * a.k);
-        const float w = there ? (a.weight ? __ldg(a.weight + (long long)t * a.k + j) : 1.f) : 0.f;
-        for (int c = lane; c < a.vecs; c += G) {
-          const V d = row_load<T, BYTES>(a.dout, (long long)t * a.dout_ld + c * V::N);
-          if (there && a.dw) {
-            const V y = row_load<T, BYTES>(a.x, (long long)p * a.x_ld + c * V::N);
+  if (G > 32 || live) {  // (with G > 32 there is a row for every block)
+    for (int j0 = 0; j0 < (U < 4 ? 1 : a.k); j0 += U) {
+      float dot[U], w[U];
+      int p[U];
 #pragma unroll
-            for (int i = 0; i < V::N; ++i) dot = fmaf((float)d.v[i], (float)y.v[i], dot);
-          }
-          if (a.dy && inside) {
+      for (int u = 0; u < U; ++u) {
+        const bool in = U < 4 || j0 + u < a.k;
+        dot[u] = 0.f;
+        p[u] = in ? __ldg(a.position + (long long)t * a.k + j0 + u) : -1;
+        w[u] = in && a.weight ? __ldg(a.weight + (long long)t * a.k + j0 + u) : 1.f;
+      }
+      for (int c = lane; c < a.vecs; c += G) {
+        const V d = row_load<T, BYTES>(a.dout, (long long)t * a.dout_ld + c * V::N);
+        V y[U];
+        if (a.dw) {
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            y[u] = row_load<T, BYTES>(a.x, ((unsigned)p[u] < (unsigned)used ? (long long)p[u] : 0ll) * a.x_ld + c * V::N);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < V::N; ++i) dot[u] = fmaf((float)d.v[i], (float)y[u].v[i], dot[u]);
+        }
+        if (a.dy) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if ((unsigned)p[u] >= (unsigned)(a.T * a.k)) continue;
             V o;
 #pragma unroll
-            for (int i = 0; i < V::N; ++i) o.v[i] = there ? (T)(w * (float)d.v[i]) : (T)0.f;
-            row_store<T, BYTES>(a.dy, (long long)p * a.W + c * V::N, o);
+            for (int i = 0; i < V::N; ++i) o.v[i] = p[u] < used ? (T)(w[u] * (float)d.v[i]) : (T)0.f;
+            row_store<T, BYTES>(a.dy, (long long)p[u] * a.W + c * V::N, o);
           }
         }
       }
       if (a.dw) {
         const unsigned mask = G >= 32 ? 0xFFFFFFFFu : (((1u << (G & 31)) - 1u) << ((threadIdx.x & 31) / G * G));
 #pragma unroll
-        for (int o = (G > 32 ? 32 : G) / 2; o; o >>= 1) dot += __shfl_xor_sync(mask, dot, o);
-        if (G <= 32) {
-          if (lane == 0) a.dw[(long long)t * a.k + j] = dot;
-        } else if ((lane & 31) == 0) {
-          red[group][j][lane >> 5] = dot;
+        for (int u = 0; u < U; ++u) {
+          if (U == 4 && j0 + u >= a.k) break;
+          if ((unsigned)p[u] >= (unsigned)used) dot[u] = 0.f;  // (row 0 was in its place)
+#pragma unroll
+          for (int o = (G > 32 ? 32 : G) / 2; o; o >>= 1) dot[u] += __shfl_xor_sync(mask, dot[u], o);
+          if (G <= 32) {
+            if (lane == 0) a.dw[(long long)t * a.k + j0 + u] = dot[u];
+          } else if ((lane & 31) == 0) {
+            red[group][j0 + u][lane >> 5] = dot[u];
+          }
         }
       }
     }
