@@ -543,6 +543,7 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR, F32>::THREADS, 1)
           }
         } else {
           t.kind = RT_ZERO;
+          t.k_len = t.add = 0;
           ok = publish(t);
         }
       }

@@ -106,6 +106,13 @@ def test_long_batches():
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('widths', [False, True])
+def test_members_without_rows_between_long_ones(widths, dtype):
+    # more tiles than CTAs, so that one CTA goes from a sum in pieces to a tile that is zero
+    check(data([1100, 0] * 20, 520, 520, dtype, widths=widths), False, dtype)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
 def test_one_member_without_rows_and_one_row(dtype):
     check(data([0], 24, 16, dtype, head=2, tail=0), False, dtype)
     d = data([3, 4], 24, 16, dtype, head=0, tail=0)
