@@ -550,42 +550,59 @@ __device__ __forceinline__ uint2 fp4_decode4(uint32_t codes, float s) {
   return make_uint2(pack_bf16x2(x.x * s, x.y * s), pack_bf16x2(y.x * s, y.y * s));
 }
 
-// A thread takes eight columns (four bytes of codes), consecutive threads consecutive ones.
+// A thread takes eight columns (four bytes of codes), consecutive threads consecutive ones.  Rows off 16-byte boundaries are
+// written by way of shared memory, in pairs of a warp's 256 consecutive columns (16384 x 8191: 389 -> 92 us).
 template <int FORMAT, int G, bool VEC>
 __global__ void __launch_bounds__(256) fp4_values_kernel(const Fp4ValuesArgs a) {
   constexpr int N = FORMAT == FP4_NV ? 16 : 32;
   constexpr int PER = 128 * G / 256;
+  __shared__ uint4 staged[VEC ? 1 : 8][32];
   const int tile = blockIdx.x / PER, part = blockIdx.x % PER;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int at = G == 32 ? lane : (int)threadIdx.x;
   const int r = G == 32 ? 2 * part + (warp & 1) + 32 * (warp >> 1) : part;
   int m, rows;
   long long row0;
-  if (!fp4_tile(a.groups, tile, m, row0, rows) || r >= rows) return;
+  if (!fp4_tile(a.groups, tile, m, row0, rows) || r >= rows) return;  // (of a warp all threads)
   const long long row = row0 + r;
   const float rs = __ldg(a.in.row_scale + row);
   const uint8_t* from = a.in.scales + (long long)tile * a.in.atoms * 512 + (r & 31) * 16 + (r >> 5) * 4;
   const uint32_t* codes = reinterpret_cast<const uint32_t*>(a.in.codes + row * a.in.pitch);
   __nv_bfloat16* out = a.out + row * a.K;
 #pragma unroll 4
-  for (int i = at; 8 * i < a.K; i += G) {
-    const int b = 8 * i / N;
-    const uint32_t byte = __ldg(from + (b >> 2) * 512 + (b & 3)), c = __ldg(codes + i);
-    float s;
-    if (FORMAT == FP4_NV) {
-      const uint32_t e = byte >> 3, f = byte & 7u;
-      s = (e ? __uint_as_float(((e + 120u) << 23) | (f << 20)) : (float)f * 0.001953125f) * rs;
-    } else {
-      s = pow2f((int)byte - 127) * rs;
+  for (int i0 = at - lane; 8 * i0 < a.K; i0 += G) {
+    const int i = i0 + lane;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (8 * i < a.K) {
+      const int b = 8 * i / N;
+      const uint32_t byte = __ldg(from + (b >> 2) * 512 + (b & 3)), c = __ldg(codes + i);
+      float s;
+      if (FORMAT == FP4_NV) {
+        const uint32_t e = byte >> 3, f = byte & 7u;
+        s = (e ? __uint_as_float(((e + 120u) << 23) | (f << 20)) : (float)f * 0.001953125f) * rs;
+      } else {
+        s = pow2f((int)byte - 127) * rs;
+      }
+      const uint2 lo = fp4_decode4(c, s), hi = fp4_decode4(c >> 16, s);
+      v = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      if (VEC) *reinterpret_cast<uint4*>(out + 8 * i) = v;  // (K is a multiple of 8)
     }
-    const uint2 lo = fp4_decode4(c, s), hi = fp4_decode4(c >> 16, s);
-    if (VEC && 8 * i + 8 <= a.K) {
-      *reinterpret_cast<uint4*>(out + 8 * i) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-    } else {
-      const uint32_t w[4] = {lo.x, lo.y, hi.x, hi.y};
+    if constexpr (!VEC) {
+      staged[warp][lane] = v;
+      __syncwarp();
+      const uint16_t* s = reinterpret_cast<const uint16_t*>(staged[warp]);
+      uint16_t* to = reinterpret_cast<uint16_t*>(out + 8 * i0);
+      const int count = min(256, a.K - 8 * i0), odd = (int)(reinterpret_cast<uintptr_t>(to) >> 1) & 1;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (8 * i + j < a.K) reinterpret_cast<uint16_t*>(out)[8 * i + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+      for (int k = 0; k < 4; ++k) {
+        const int j = odd + 2 * (lane + 32 * k);
+        if (j + 1 < count)
+          *reinterpret_cast<uint32_t*>(to + j) = (uint32_t)s[j] | (uint32_t)s[j + 1] << 16;
+        else if (j < count)
+          to[j] = s[j];
+      }
+      if (odd && lane == 0) to[0] = s[0];
+      __syncwarp();
     }
   }
 }

@@ -939,6 +939,7 @@ __global__ void __launch_bounds__(256) ragged_bias_kernel(const RaggedAct a) {
   const long long n = (long long)a.P * a.N, i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   float s = 0.f;
+#pragma unroll 8
   for (int k = 0; k < a.S; ++k) s += a.partial[k * n + i];
   a.db[i] = s;
 }

@@ -266,8 +266,9 @@ int make_scale_map(CUtensorMap* map, const void* ptr, int atoms, long long row_t
 
 constexpr int32_t MAX_WIDTH = 1 << 24;
 
-// Columns of a tile: narrower ones while they still fit the SMs at once.  (Two rounds of narrow tiles take as long as
-// one of wide ones, which read less.)
+// Columns of a tile: narrower ones while they still fit the SMs at once.  Two rounds of narrow tiles take longer than one of
+// wide ones, which read less (bf16, tiles of 64 / 128 / 256 columns: 7 x 367 rows, 200 -> 531, 10.0 / 9.4 / 12.1 us;
+// 4 x 512 rows, 2048 -> 1024, 28 / 18.6 / 21; 2048 -> 4096 85 / 55 / 40).
 int tile_columns(long long row_tiles, int cols) {
   int bn = 256;
   while (bn > 64 && row_tiles * ((cols + bn / 2 - 1) / (bn / 2)) <= device_info().sms) bn /= 2;
@@ -362,7 +363,9 @@ RaggedPlan ragged_plan(int mode, int P, int64_t R, int in, int out) {
   const long long used = std::min<long long>(P, R);
   const int sms = 148;
   // Pairs where their 256-row tiles are mostly full and there is at least one for each pair of SMs: members of 1024
-  // rows on average (wgrad: input widths), since a member's last tile is half empty on average.
+  // rows on average (wgrad: input widths), since a member's last tile is half empty on average.  (8 members of 4096 x 4096:
+  // 1024 rows each 191 us against 198, backward 428 against 467; 512 full ones 114 against 124; but 64 members of 1100 rows,
+  // 1024 x 1024, 142 against 136.)
   const long long rows = mode == RAGGED_WGRAD ? in : R / P;
   const long long pair_tiles = (mode == RAGGED_WGRAD ? (long long)P * ((in + 255) / 256) : R / 256) * ((cols + 255) / 256);
   if (rows >= 1024 && pair_tiles >= sms / 2) {
@@ -460,9 +463,11 @@ struct Splits {
   }
 };
 
-// Columns of a block of the activation gradient: long pieces of each row where that leaves blocks enough.
-int ragged_strip(const tp_ragged_linear_args* a) { return a->rows * a->max_out >= (4ll << 20) && a->max_out >= 256 ? 256 : 64; }
-// Shares of a member's rows in the bias gradient: about eight blocks an SM, 64 rows each at least.
+// Columns of a block of the activation gradient: long pieces of each row where that leaves blocks enough (256 / 64 columns:
+// 4080 rows of 512 4.9 / 5.4 us, 8192 of 512 5.6 / 8.5; 2569 of 531 10.7 / 6.3, 9001 of 190 14 / 6.7).
+int ragged_strip(const tp_ragged_linear_args* a) { return a->rows * a->max_out >= (2ll << 20) && a->max_out >= 256 ? 256 : 64; }
+// Shares of a member's rows in the bias gradient: about eight blocks an SM, 64 rows each at least (32768 rows of 4096: 9 shares
+// 55 us with their sum, 4 65, one 91; 9001 rows of 190 to one member: 64 shares 11.4, 32 12, 16 17).
 int ragged_shares(const tp_ragged_linear_args* a) {
   const long long strips = (a->max_out + ragged_strip(a) - 1) / ragged_strip(a);
   const long long want = 8ll * 148 / std::max(1ll, strips * a->P), most = a->rows / ((long long)a->P * 64);
@@ -573,9 +578,13 @@ Fp4Rows fp4_rows(const tp_fp4_args* a) {
   return r;
 }
 
-// Rows of up to this many tiles go to a block each: a warp a row leaves most of the GPU idle there, and takes a
-// row's pieces one after the other.
-constexpr long long FP4_FEW_TILES = 8;
+// Few long rows go to a block each instead of a warp each, which takes a row's pieces one after the other and leaves most
+// of the GPU idle: up to this many columns for each tile of 128 rows.
+// mxfp4, a block / a warp a row: 1024 rows of 8192 bf16 8.6 / 12.9 us, 4096 of them 24.5 / 20.8; 128 rows of 2048 2.8 / 4.3,
+// 1024 of them 6.1 / 5.2.  nvfp4 against the rows through shared memory: 128 rows of 8192 4.3 / 5.3, 512 of them 6.8 / 6.3.
+// Rows off 16-byte boundaries, nvfp4: 1024 rows of 8191 16.8 / 23.1, 4096 of them 49 / 65.
+// Values: 4096 rows of 8192 16.9 / 22.7, 1024 of 2048 3.9 / 6.1, 4096 of 1024 7.6 / 5.2.
+constexpr long long FP4_COLUMNS_MX = 512, FP4_COLUMNS_NV = 4096, FP4_COLUMNS_VALUES = 256;
 
 // nvfp4 of rows of at most 4 G vectors: groups of four rows through shared memory, 1024 threads an SM.
 template <typename T, int G>
@@ -592,14 +601,15 @@ int launch_stream(const Fp4QuantArgs& k, long long tiles, cudaStream_t st) {
 template <typename T, int FORMAT>
 int launch_quantize(const Fp4QuantArgs& k, bool vec, cudaStream_t st) {
   const long long tiles = fp4_row_tiles(k.groups);
-  const bool few = tiles <= FP4_FEW_TILES;
+  constexpr int E = 16 / (int)sizeof(T);
+  const bool stream = FORMAT == FP4_NV && vec && k.K <= 256 * 4 * E;
+  const bool few = tiles * (stream ? FP4_COLUMNS_NV : FP4_COLUMNS_MX) <= k.K;
   const long long blocks = tiles * (few ? 128 : 16);
   if (tiles * 128 > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many rows");
   if (!vec) {
     (few ? fp4_quantize_kernel<T, FORMAT, 256> : fp4_quantize_kernel<T, FORMAT, 32>)<<<(unsigned)blocks, 256, 0, st>>>(k);
     return TP_OK;
   }
-  constexpr int E = 16 / (int)sizeof(T);
   if (few) {
     fp4_quantize_rows_kernel<T, FORMAT, 256, 4><<<(unsigned)(tiles * 128), 256, 0, st>>>(k);
     return TP_OK;
@@ -608,7 +618,7 @@ int launch_quantize(const Fp4QuantArgs& k, bool vec, cudaStream_t st) {
     if (k.K <= 32 * 4 * E) return launch_stream<T, 32>(k, tiles, st);
     if (k.K <= 64 * 4 * E) return launch_stream<T, 64>(k, tiles, st);
     if (k.K <= 128 * 4 * E) return launch_stream<T, 128>(k, tiles, st);
-    if (k.K <= 256 * 4 * E) return launch_stream<T, 256>(k, tiles, st);
+    if (stream) return launch_stream<T, 256>(k, tiles, st);
   }
   fp4_quantize_rows_kernel<T, FORMAT, 32, 4><<<(unsigned)(tiles * 32), 128, 0, st>>>(k);
   return TP_OK;
@@ -617,7 +627,7 @@ int launch_quantize(const Fp4QuantArgs& k, bool vec, cudaStream_t st) {
 template <int FORMAT>
 int launch_values(const Fp4ValuesArgs& k, bool vec, cudaStream_t st) {
   const long long tiles = fp4_row_tiles(k.groups);
-  const bool few = tiles <= FP4_FEW_TILES;
+  const bool few = tiles * FP4_COLUMNS_VALUES <= k.K;
   const long long blocks = tiles * (few ? 128 : 16);
   if (blocks > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many rows");
   auto kern = few ? (vec ? fp4_values_kernel<FORMAT, 256, true> : fp4_values_kernel<FORMAT, 256, false>)
@@ -649,9 +659,15 @@ int dispatch_fp4(const Fp4Problem& p, const CUtensorMap (&m)[4], bool pair, int 
 
 // ------------------------------------------------------------------ a few rows a group
 
-// Groups of up to 32 rows on average: the kernel for few rows reads each weight once (its CTAs look through the groups
-// one by one, so there are not too many).
-bool few_rows(int32_t P, int64_t rows) { return P <= 1024 && rows <= 32 * std::min<int64_t>(P, rows); }
+// The kernel for few rows a member: up to 16, or 32 where the K loop is long, and up to 512 tiles of 128 outputs (each a CTA of
+// its own, which finds its rows by looking through the groups).  It / the kernel for many rows, in bf16: one row through
+// 8192 x 8192 37 / 61 us, 32 of them 42 / 49, 64 of them 44 / 49; 8 members of one row, 4096 x 4096, 60 / 63; 32 of one row,
+// 1024 x 1024, 20 / 22; but 32 rows through 512 x 512 11 / 7.6, 64 members of one row, 1024 x 4096, 106 / 101, of 32 rows
+// 122 / 104.  In 4 bits: 15 / 22.5, 17.9 / 18.6, 21 / 18.8; 23 / 26; 10.8 / 13.7; 8.6 / 5.9, 57 / 48.
+bool few_rows(int32_t P, int64_t rows, int32_t K, int32_t N) {
+  const int64_t used = std::min<int64_t>(P, rows);
+  return P <= 1024 && rows <= (K >= 4096 ? 32 : 16) * used && used * ((N + 127) / 128) <= 512;
+}
 
 template <int KIND>
 int launch_few(const FewArgs& f, const CUtensorMap& ma, const CUtensorMap& mb, cudaStream_t st) {
@@ -780,7 +796,7 @@ int tp_ragged_linear_forward(const tp_ragged_linear_args* a, void* stream) {
   p.bias = a->bias;
   p.relu = a->relu;
   p.c = a->y;
-  if (a->dtype == TP_DTYPE_BF16 && few_rows(a->P, a->rows)) {
+  if (a->dtype == TP_DTYPE_BF16 && few_rows(a->P, a->rows, a->max_in, a->max_out)) {
     FewArgs f{};
     f.groups = fp4_groups(a->P, a->rows, a->offsets);
     f.K = a->max_in;
@@ -1005,7 +1021,7 @@ int tp_fp4_linear_forward(const tp_fp4_linear_args* a, void* stream) {
   const int pitch = tp_fp4_pitch(a->K);
   const auto T = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   CUtensorMap ma, mb;
-  if (p.groups.offsets ? few_rows(a->P, rows) : p.groups.B <= 32 && a->P <= 65535) {
+  if (few_rows(a->P, rows, a->K, a->N)) {
     FewArgs f{};
     f.groups = p.groups;
     f.x_shared = a->x_shared;
@@ -1029,8 +1045,9 @@ int tp_fp4_linear_forward(const tp_fp4_linear_args* a, void* stream) {
   }
   const long long m_tiles = p.groups.offsets ? std::max<long long>(std::min<long long>(a->P, rows), rows / 128 + std::min<long long>(a->P, rows) / 2)
                                              : (long long)a->P * ((p.groups.B + 127) / 128);
-  // pairs where their 256-row tiles are mostly full and every pair of SMs has one
-  const bool pair = rows / a->P >= 1024 && rows / 256 * ((a->N + 255) / 256) >= device_info().sms / 2;
+  // Pairs where their 256-row tiles are mostly full (half a tile of a ragged member is not) and every pair of SMs has one:
+  // 4 x 512 rows, 8192 x 8192, 84 us against 102; 16 x 700, 2048 x 2048, 47 against 50; 16 x 256 of them 24.5 against 24.9.
+  const bool pair = rows / a->P >= 512 && rows / 256 * ((a->N + 255) / 256) >= device_info().sms / 2;
   const int bn = pair ? 256 : tile_columns(m_tiles, a->N);
   p.n_tiles = (a->N + bn - 1) / bn;
   const long long most = (p.groups.offsets ? rows / 128 + a->P + 2 : m_tiles) * p.n_tiles;
