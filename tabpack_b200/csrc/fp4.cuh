@@ -121,22 +121,12 @@ __device__ __forceinline__ uint8_t nvfp4_scale_byte(float big, float row_inverse
   return (uint8_t)__nv_cvt_float_to_fp8(fmaf(fmaf(-q, 6.f, t), sixth, q), __NV_SATFINITE, __NV_E4M3);
 }
 
-// A block's scale byte from its largest magnitude, its scale s and that one's reciprocal; `row` is the row's 2^r (nvfp4),
-// row_inverse its reciprocal.
-template <int FORMAT>
-__device__ __forceinline__ uint8_t fp4_scale(float big, float row, float row_inverse, float& s, float& inv) {
-  if constexpr (FORMAT == FP4_NV) {
-    const uint8_t byte = nvfp4_scale_byte(big, row_inverse);
-    const float small = e4m3_value(byte);
-    s = small * row;
-    inv = small > 0.f ? __frcp_rn(small) * row_inverse : 0.f;
-    return byte;
-  } else {
-    const int e = max((int)(__float_as_uint(big) >> 23) - 129, -100);
-    s = pow2f(e);
-    inv = pow2f(-e);
-    return (uint8_t)(e + 127);
-  }
+// mxfp4: a block's scale byte from its largest magnitude, its scale s and that one's reciprocal.
+__device__ __forceinline__ uint8_t mxfp4_scale(float big, float& s, float& inv) {
+  const int e = max((int)(__float_as_uint(big) >> 23) - 129, -100);
+  s = pow2f(e);
+  inv = pow2f(-e);
+  return (uint8_t)(e + 127);
 }
 
 // Two values over s: the correctly rounded quotients, by the reciprocal and one correction (exact for a power of two).
@@ -150,126 +140,7 @@ __device__ __forceinline__ void fp4_quotients(float& x, float& y, float s, float
   y = h.y;
 }
 
-// One block's codes and scale byte from its values.
-template <int FORMAT, int N>
-__device__ __forceinline__ uint8_t fp4_block(const float (&x)[N], float row, float row_inverse, uint32_t (&codes)[N / 8]) {
-  float big = 0.f, s, inv;
-#pragma unroll
-  for (int i = 0; i < N; ++i) big = fmaxf(big, fabsf(x[i]));
-  const uint8_t byte = fp4_scale<FORMAT>(big, row, row_inverse, s, inv);
-#pragma unroll
-  for (int j = 0; j < N / 8; ++j) {
-    float q[8];
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      q[i] = x[8 * j + i];
-      q[i + 1] = x[8 * j + i + 1];
-      fp4_quotients<FORMAT>(q[i], q[i + 1], s, inv);
-    }
-    codes[j] = fp4_pack8(q);
-  }
-  return byte;
-}
-
-// The largest magnitude of a row among the columns of this thread's part (of G), NaN if one is.
-template <typename T, int G, bool VEC>
-__device__ __forceinline__ float fp4_row_max(const T* x, int n, int at) {
-  float big = 0.f;
-  int c0 = 0;
-  if constexpr (VEC) {
-    constexpr int E = 16 / (int)sizeof(T), U = 4;
-    const int vecs = n / E;
-    auto take = [&](const uint4& u) {
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-      if constexpr (sizeof(T) == 2) {
-        // magnitudes of bf16 are in the order of their bits, NaN above infinity
-        uint32_t m = w[0] & 0x7FFF7FFFu;
-#pragma unroll
-        for (int j = 1; j < 4; ++j) m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
-        big = max_nan(big, max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u)));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) big = max_nan(big, fabsf(__uint_as_float(w[j])));
-      }
-    };
-    int i = at;
-    for (; i + (U - 1) * G < vecs; i += U * G) {
-      uint4 u[U];
-#pragma unroll
-      for (int j = 0; j < U; ++j) u[j] = __ldg(reinterpret_cast<const uint4*>(x) + i + j * G);
-#pragma unroll
-      for (int j = 0; j < U; ++j) take(u[j]);
-    }
-    for (; i < vecs; i += G) take(__ldg(reinterpret_cast<const uint4*>(x) + i));
-    c0 = vecs * E;
-  }
-  for (int c = c0 + at; c < n; c += G) big = max_nan(big, fabsf((float)x[c]));
-  return big;
-}
-
-// Rows off 16-byte boundaries, element by element.  G threads a row.  G = 32: a block takes 8 rows of a tile, i, i + 32, i + 64, i + 96 for two consecutive i, whose
-// scale bytes make up whole 32-byte sectors of the tile.  G = 256: one row (few rows: latency counts).
-template <typename T, int FORMAT, int G>
-__global__ void __launch_bounds__(256) fp4_quantize_kernel(const Fp4QuantArgs a) {
-  constexpr int N = FORMAT == FP4_NV ? 16 : 32;
-  constexpr int PER = 128 * G / 256;  // blocks of the grid a tile
-  const int tile = blockIdx.x / PER, part = blockIdx.x % PER;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int at = G == 32 ? lane : (int)threadIdx.x;
-  const int r = G == 32 ? 2 * part + (warp & 1) + 32 * (warp >> 1) : part;  // row of the tile
-  int m, rows;
-  long long row0;
-  if (!fp4_tile(a.groups, tile, m, row0, rows)) return;
-  const bool live = r < rows;
-  const long long row = row0 + r;
-  const int n = a.n_features ? min(__ldg(a.n_features + m), a.K) : a.K;
-  const T* x = static_cast<const T*>(a.x) + row * a.ld;
-  __shared__ float warp_max[8];
-  float scale = 1.f, big = 0.f;
-  auto row_max = [&]() {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) big = max_nan(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
-    if constexpr (G > 32) {
-      if (lane == 0) warp_max[warp] = big;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < 8; ++w) big = max_nan(big, warp_max[w]);
-    }
-  };
-  if constexpr (FORMAT == FP4_NV) {
-    if (live) big = fp4_row_max<T, G, false>(x, n, at);
-    row_max();
-    scale = nvfp4_row_scale(big);
-  }
-  const int blocks = a.out.atoms * 4;  // with those of the padding, which are zero
-  uint8_t* to = a.out.scales + (long long)tile * a.out.atoms * 512;
-  // (of a power of two from 2^-100 to 2^117)
-  const float scale_inverse = __uint_as_float((254u << 23) - __float_as_uint(scale));
-  const bool zero = !live || (FORMAT == FP4_NV && !(big < INFINITY));
-  for (int b = at; b < blocks; b += G) {
-    float v[N];
-    #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = !zero && b * N + i < n ? (float)x[b * N + i] : 0.f;
-    uint32_t codes[N / 8];
-    const uint8_t byte = fp4_block<FORMAT, N>(v, scale, scale_inverse, codes);
-    if constexpr (FORMAT == FP4_MX) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) big = max_nan(big, fabsf(v[i]));
-    }
-    to[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = live && b * N < a.K ? byte : (uint8_t)0;
-    if (live && b * (N / 2) < a.out.pitch) {
-      uint8_t* cp = a.out.codes + row * a.out.pitch + b * (N / 2);
-      if constexpr (FORMAT == FP4_NV)
-        *reinterpret_cast<uint2*>(cp) = make_uint2(codes[0], codes[1]);
-      else
-        *reinterpret_cast<uint4*>(cp) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-    }
-  }
-  if constexpr (FORMAT == FP4_MX) row_max();
-  if (live && at == 0) a.out.row_scale[row] = big < INFINITY ? scale : __uint_as_float(0x7FC00000u);
-}
-
-// Rows on 16-byte boundaries go by vectors of 16 bytes, consecutive threads of a row's G consecutive ones; the 2 to 8 lanes
+// Rows go by vectors of 16 bytes, consecutive threads of a row's G consecutive ones; the 2 to 8 lanes
 // of a block of columns find its scale together.  The scales' values and reciprocals come from a table by their byte.
 struct Fp4Row {
   long long row;
@@ -322,7 +193,7 @@ __device__ __forceinline__ void fp4_vector(const Fp4QuantArgs& a, const Fp4Row& 
     s = e.x * scale;
     inv = e.y * scale_inverse;
   } else {
-    byte = fp4_scale<FP4_MX>(most, 1.f, 1.f, s, inv);
+    byte = mxfp4_scale(most, s, inv);
   }
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
   float q[8] = {};
@@ -357,21 +228,72 @@ __device__ __forceinline__ void fp4_table(float2* table) {  // value and recipro
   }
 }
 
-// Element c on of a row, zeros from column n on.
-template <typename T>
+// Columns c on of a row, zeros from column n on.  Rows off 16-byte boundaries (ALIGNED false): the two 16-byte blocks of memory
+// that the vector lies in, neither without an element of the row, moved into place (16384 rows of 8191 bf16: mxfp4 264 us element by
+// element, 115 like this; nvfp4 194, 135).
+template <typename T, bool ALIGNED>
 __device__ __forceinline__ uint4 fp4_load(const T* x, int c, int n) {
   constexpr int E = 16 / (int)sizeof(T);
-  if (c + E <= n) return __ldg(reinterpret_cast<const uint4*>(x + c));
-  T e[E];
+  if constexpr (ALIGNED) {
+    if (c + E <= n) return __ldg(reinterpret_cast<const uint4*>(x + c));
+    T e[E];
 #pragma unroll
-  for (int i = 0; i < E; ++i) e[i] = c + i < n ? x[c + i] : (T)0.f;
-  return *reinterpret_cast<const uint4*>(e);
+    for (int i = 0; i < E; ++i) e[i] = c + i < n ? x[c + i] : (T)0.f;
+    return *reinterpret_cast<const uint4*>(e);
+  } else {
+    if (c >= n) return make_uint4(0, 0, 0, 0);
+    const uintptr_t p = reinterpret_cast<uintptr_t>(x + c);
+    const uint32_t off = (uint32_t)p & 15u;
+    const uint4* block = reinterpret_cast<const uint4*>(p - off);
+    const uint4 lo = __ldg(block);
+    uint4 hi = make_uint4(0, 0, 0, 0);
+    if (off && reinterpret_cast<uintptr_t>(block + 1) < reinterpret_cast<uintptr_t>(x + n)) hi = __ldg(block + 1);
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (off & 8u) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (off & 4u) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2u) * 8u);
+    }
+    const int keep = n - c;
+    if (keep < E) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 2)
+          w[i] = 2 * i + 1 < keep ? w[i] : 2 * i < keep ? w[i] & 0xFFFFu : 0u;
+        else
+          w[i] = i < keep ? w[i] : 0u;
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// The largest magnitude of a row among the vectors of this thread (of G), NaN if one is.
+template <typename T, int G, bool ALIGNED>
+__device__ __forceinline__ float fp4_row_max(const T* x, int n, int at) {
+  constexpr int E = 16 / (int)sizeof(T), U = 4;
+  float big = 0.f;
+  for (int v = at; v * E < n; v += U * G) {
+    uint4 u[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) u[j] = fp4_load<T, ALIGNED>(x, (v + j * G) * E, n);
+#pragma unroll
+    for (int j = 0; j < U; ++j) big = max_nan(big, fp4_largest<T>(u[j]));
+  }
+  return big;
 }
 
 // G threads a row, H vectors at a time; a block of the grid takes four rows (i, i + 32, i + 64, i + 96 of a tile), or one with
 // G = 256.  nvfp4 reads a row twice (for its largest magnitude first), mxfp4 once
 // (16384 rows of 8192 fp32: 113 us, 5.4 TB/s; 140 with a thread's own block by strided vectors, 171 by way of shared memory).
-template <typename T, int FORMAT, int G, int H>
+template <typename T, int FORMAT, int G, int H, bool ALIGNED>
 __global__ void __launch_bounds__(G == 256 ? 256 : 4 * G) fp4_quantize_rows_kernel(const Fp4QuantArgs a) {
   constexpr int N = FORMAT == FP4_NV ? 16 : 32, E = 16 / (int)sizeof(T), L = N / E;
   constexpr int ROWS = G == 256 ? 1 : 4, PER = 128 / ROWS;
@@ -396,7 +318,7 @@ __global__ void __launch_bounds__(G == 256 ? 256 : 4 * G) fp4_quantize_rows_kern
   };
   float scale = 1.f;
   if constexpr (FORMAT == FP4_NV) {
-    if (q.live) big = fp4_row_max<T, G, true>(x, q.n, at);
+    if (q.live) big = fp4_row_max<T, G, ALIGNED>(x, q.n, at);
     row_max();
     if constexpr (G == 32) __syncthreads();  // (the table)
     scale = nvfp4_row_scale(big);
@@ -407,7 +329,7 @@ __global__ void __launch_bounds__(G == 256 ? 256 : 4 * G) fp4_quantize_rows_kern
   for (int v0 = 0; v0 < vecs; v0 += G * H) {
     uint4 u[H];
 #pragma unroll
-    for (int h = 0; h < H; ++h) u[h] = fp4_load<T>(x, (v0 + h * G + at) * E, q.n);
+    for (int h = 0; h < H; ++h) u[h] = fp4_load<T, ALIGNED>(x, (v0 + h * G + at) * E, q.n);
 #pragma unroll
     for (int h = 0; h < H; ++h) {
       if (v0 + h * G >= vecs) break;  // (the same for all of the block's threads)
@@ -425,7 +347,7 @@ __global__ void __launch_bounds__(G == 256 ? 256 : 4 * G) fp4_quantize_rows_kern
 // warp's vectors come in as they lie in memory and are dealt out again so that a lane has whole blocks of columns.
 // (16384 rows of 8192 bf16: 98 us in two passes, of which the second misses L2 by half; 88 us with a vector a lane, the block's
 // scale found by two of them with shuffles, 150 instructions a vector; 80 us like this, 4.3 TB/s.  The instructions still bound it.)
-template <typename T, int G, int H>
+template <typename T, int G, int H, bool ALIGNED>
 __global__ void __launch_bounds__(4 * G, 256 / G) fp4_quantize_stream_kernel(const Fp4QuantArgs a, const long long groups) {
   constexpr int N = 16, E = 16 / (int)sizeof(T), L = N / E;  // columns of a block, of a vector; vectors of a block
   static_assert(H % L == 0, "whole blocks");
@@ -446,10 +368,10 @@ __global__ void __launch_bounds__(4 * G, 256 / G) fp4_quantize_stream_kernel(con
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           const int c = (h * G + at) * E;
-          if (c + E <= q.n)
+          if (ALIGNED && c + E <= q.n)
             cp_async16(smem_u32(slot(stage, h)), x + c);
           else
-            *slot(stage, h) = fp4_load<T>(x, c, q.n);
+            *slot(stage, h) = fp4_load<T, ALIGNED>(x, c, q.n);
         }
       }
     }

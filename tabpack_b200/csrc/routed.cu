@@ -582,14 +582,13 @@ Fp4Rows fp4_rows(const tp_fp4_args* a) {
 // of the GPU idle: up to this many columns for each tile of 128 rows.
 // mxfp4, a block / a warp a row: 1024 rows of 8192 bf16 8.6 / 12.9 us, 4096 of them 24.5 / 20.8; 128 rows of 2048 2.8 / 4.3,
 // 1024 of them 6.1 / 5.2.  nvfp4 against the rows through shared memory: 128 rows of 8192 4.3 / 5.3, 512 of them 6.8 / 6.3.
-// Rows off 16-byte boundaries, nvfp4: 1024 rows of 8191 16.8 / 23.1, 4096 of them 49 / 65.
 // Values: 4096 rows of 8192 16.9 / 22.7, 1024 of 2048 3.9 / 6.1, 4096 of 1024 7.6 / 5.2.
 constexpr long long FP4_COLUMNS_MX = 512, FP4_COLUMNS_NV = 4096, FP4_COLUMNS_VALUES = 256;
 
 // nvfp4 of rows of at most 4 G vectors: groups of four rows through shared memory, 1024 threads an SM.
-template <typename T, int G>
+template <typename T, int G, bool ALIGNED>
 int launch_stream(const Fp4QuantArgs& k, long long tiles, cudaStream_t st) {
-  constexpr auto kern = fp4_quantize_stream_kernel<T, G, 4>;
+  constexpr auto kern = fp4_quantize_stream_kernel<T, G, 4, ALIGNED>;
   constexpr size_t smem = (size_t)2 * 4 * 4 * G * 16;
   int rc = allow_smem<kern>(smem);
   if (rc) return rc;
@@ -598,30 +597,30 @@ int launch_stream(const Fp4QuantArgs& k, long long tiles, cudaStream_t st) {
   return TP_OK;
 }
 
-template <typename T, int FORMAT>
-int launch_quantize(const Fp4QuantArgs& k, bool vec, cudaStream_t st) {
+template <typename T, int FORMAT, bool ALIGNED>
+int launch_quantize(const Fp4QuantArgs& k, cudaStream_t st) {
   const long long tiles = fp4_row_tiles(k.groups);
   constexpr int E = 16 / (int)sizeof(T);
-  const bool stream = FORMAT == FP4_NV && vec && k.K <= 256 * 4 * E;
+  const bool stream = FORMAT == FP4_NV && k.K <= 256 * 4 * E;
   const bool few = tiles * (stream ? FP4_COLUMNS_NV : FP4_COLUMNS_MX) <= k.K;
-  const long long blocks = tiles * (few ? 128 : 16);
   if (tiles * 128 > 0x7FFFFFFFLL) return fail(TP_EINVAL, "too many rows");
-  if (!vec) {
-    (few ? fp4_quantize_kernel<T, FORMAT, 256> : fp4_quantize_kernel<T, FORMAT, 32>)<<<(unsigned)blocks, 256, 0, st>>>(k);
-    return TP_OK;
-  }
   if (few) {
-    fp4_quantize_rows_kernel<T, FORMAT, 256, 4><<<(unsigned)(tiles * 128), 256, 0, st>>>(k);
+    fp4_quantize_rows_kernel<T, FORMAT, 256, 4, ALIGNED><<<(unsigned)(tiles * 128), 256, 0, st>>>(k);
     return TP_OK;
   }
   if constexpr (FORMAT == FP4_NV) {
-    if (k.K <= 32 * 4 * E) return launch_stream<T, 32>(k, tiles, st);
-    if (k.K <= 64 * 4 * E) return launch_stream<T, 64>(k, tiles, st);
-    if (k.K <= 128 * 4 * E) return launch_stream<T, 128>(k, tiles, st);
-    if (stream) return launch_stream<T, 256>(k, tiles, st);
+    if (k.K <= 32 * 4 * E) return launch_stream<T, 32, ALIGNED>(k, tiles, st);
+    if (k.K <= 64 * 4 * E) return launch_stream<T, 64, ALIGNED>(k, tiles, st);
+    if (k.K <= 128 * 4 * E) return launch_stream<T, 128, ALIGNED>(k, tiles, st);
+    if (stream) return launch_stream<T, 256, ALIGNED>(k, tiles, st);
   }
-  fp4_quantize_rows_kernel<T, FORMAT, 32, 4><<<(unsigned)(tiles * 32), 128, 0, st>>>(k);
+  fp4_quantize_rows_kernel<T, FORMAT, 32, 4, ALIGNED><<<(unsigned)(tiles * 32), 128, 0, st>>>(k);
   return TP_OK;
+}
+template <typename T>
+int dispatch_quantize(const Fp4QuantArgs& k, bool nv, bool aligned, cudaStream_t st) {
+  if (nv) return aligned ? launch_quantize<T, FP4_NV, true>(k, st) : launch_quantize<T, FP4_NV, false>(k, st);
+  return aligned ? launch_quantize<T, FP4_MX, true>(k, st) : launch_quantize<T, FP4_MX, false>(k, st);
 }
 
 template <int FORMAT>
@@ -928,8 +927,7 @@ int tp_fp4_quantize(const tp_fp4_args* a, void* stream) {
   k.out = fp4_rows(a);
   const size_t size = dtype_size(a->dtype);
   const bool vec = aligned16(a->x) && a->x_stride * size % 16 == 0, nv = a->format == TP_FP4_NV;
-  rc = a->dtype == TP_DTYPE_BF16 ? (nv ? launch_quantize<__nv_bfloat16, FP4_NV>(k, vec, st) : launch_quantize<__nv_bfloat16, FP4_MX>(k, vec, st))
-                                 : (nv ? launch_quantize<float, FP4_NV>(k, vec, st) : launch_quantize<float, FP4_MX>(k, vec, st));
+  rc = a->dtype == TP_DTYPE_BF16 ? dispatch_quantize<__nv_bfloat16>(k, nv, vec, st) : dispatch_quantize<float>(k, nv, vec, st);
   if (rc) return rc;
   TP_CUDA_TRY(cudaGetLastError());
   return TP_OK;
