@@ -19,7 +19,7 @@
 //
 // Results in fp32 are summed over at most RAGGED_SEGMENT elements of K in one accumulator, the pieces in the epilogue's
 // registers with the rounding of fp32: the tensor core's own sums do not round to nearest, and over 23054 rows came out 2.6e-5 off
-// (5e-7 with the cut).
+// (5e-7 with the cut, which costs 5 % of the time: 8 x 4096 x 4096 over 4096 rows each 863 us, 816 with pieces of 8192).
 // Few tiles over many rows are split over CTAs, into parts that a second launch adds up in order.
 //
 // fp32 operands come as three bf16 parts each (ragged_split_kernel), and the K loop goes through the six products of
@@ -178,10 +178,10 @@ __device__ __forceinline__ int ragged_n(bool pair, int bn, const RaggedTile& t) 
   return min(bn, pair ? (left + 31) & ~31 : (left + 15) & ~15);
 }
 
+// One of the products by this CTA (pair), number `worker` of `workers`.
 template <int BN, int MODE, bool PAIR, bool F32>
-__global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR, F32>::THREADS, 1)
-    ragged_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                       const RaggedProblem pr) {
+__device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtensorMap& tmB, const RaggedProblem& pr,
+                                            const int worker, const int workers) {
   using Cfg = RaggedCfg<BN, MODE, PAIR, F32>;
   constexpr int STAGES = Cfg::STAGES, TRING = Cfg::TRING;
   extern __shared__ uint8_t dyn_smem[];
@@ -206,7 +206,6 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR, F32>::THREADS, 1)
 
   const int warp = warp_id(), lane = lane_id();
   const int rank = PAIR ? (int)cluster_ctarank() : 0;
-  const int worker = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, workers = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
 
   // (`whole`: all lanes of the warp read, and lane 0 frees the slot once they have)
   auto ring_read = [&](int k, bool whole) -> RaggedTile {
@@ -766,6 +765,27 @@ __global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR, F32>::THREADS, 1)
     else
       tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
   }
+}
+
+template <int BN, int MODE, bool PAIR, bool F32>
+__global__ void __launch_bounds__(RaggedCfg<BN, MODE, PAIR, F32>::THREADS, 1)
+    ragged_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                       const __grid_constant__ RaggedProblem pr) {
+  constexpr int shift = PAIR ? 1 : 0;
+  ragged_gemm<BN, MODE, PAIR, F32>(tmA, tmB, pr, (int)(blockIdx.x >> shift), (int)(gridDim.x >> shift));
+}
+
+// Both gradients in one launch, dx by the first n CTAs: where all tiles fit the SMs at once, neither waits for the other.
+template <int BN, bool F32>
+__global__ void __launch_bounds__(RaggedCfg<BN, RAGGED_WGRAD, false, F32>::THREADS, 1)
+    ragged_gradients_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                            const __grid_constant__ RaggedProblem pr, const __grid_constant__ CUtensorMap tmA2,
+                            const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ RaggedProblem pr2, const int n) {
+  static_assert(RaggedCfg<BN, RAGGED_WGRAD, false, F32>::THREADS == RaggedCfg<BN, RAGGED_DGRAD, false, F32>::THREADS, "one block size");
+  if ((int)blockIdx.x < n)
+    ragged_gemm<BN, RAGGED_DGRAD, false, F32>(tmA, tmB, pr, (int)blockIdx.x, n);
+  else
+    ragged_gemm<BN, RAGGED_WGRAD, false, F32>(tmA2, tmB2, pr2, (int)blockIdx.x - n, (int)gridDim.x - n);
 }
 
 // dw = the sum of its parts, in their order.
