@@ -491,26 +491,26 @@ __global__ void __launch_bounds__(256) fp4_values_kernel(const Fp4ValuesArgs a) 
   const uint8_t* from = a.in.scales + (long long)tile * a.in.atoms * 512 + (r & 31) * 16 + (r >> 5) * 4;
   const uint32_t* codes = reinterpret_cast<const uint32_t*>(a.in.codes + row * a.in.pitch);
   __nv_bfloat16* out = a.out + row * a.K;
-#pragma unroll 4
-  for (int i0 = at - lane; 8 * i0 < a.K; i0 += G) {
-    const int i = i0 + lane;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (8 * i < a.K) {
-      const int b = 8 * i / N;
-      const uint32_t byte = __ldg(from + (b >> 2) * 512 + (b & 3)), c = __ldg(codes + i);
-      float s;
-      if (FORMAT == FP4_NV) {
-        const uint32_t e = byte >> 3, f = byte & 7u;
-        s = (e ? __uint_as_float(((e + 120u) << 23) | (f << 20)) : (float)f * 0.001953125f) * rs;
-      } else {
-        s = pow2f((int)byte - 127) * rs;
-      }
-      const uint2 lo = fp4_decode4(c, s), hi = fp4_decode4(c >> 16, s);
-      v = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      if (VEC) *reinterpret_cast<uint4*>(out + 8 * i) = v;  // (K is a multiple of 8)
+  auto decode = [&](int i) -> uint4 {
+    const int b = 8 * i / N;
+    const uint32_t byte = __ldg(from + (b >> 2) * 512 + (b & 3)), c = __ldg(codes + i);
+    float s;
+    if (FORMAT == FP4_NV) {
+      const uint32_t e = byte >> 3, f = byte & 7u;
+      s = (e ? __uint_as_float(((e + 120u) << 23) | (f << 20)) : (float)f * 0.001953125f) * rs;
+    } else {
+      s = pow2f((int)byte - 127) * rs;
     }
-    if constexpr (!VEC) {
-      staged[warp][lane] = v;
+    const uint2 lo = fp4_decode4(c, s), hi = fp4_decode4(c >> 16, s);
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+  };
+  if constexpr (VEC) {  // (K is a multiple of 8)
+#pragma unroll 4
+    for (int i = at; 8 * i < a.K; i += G) *reinterpret_cast<uint4*>(out + 8 * i) = decode(i);
+  } else {
+#pragma unroll 2
+    for (int i0 = at - lane; 8 * i0 < a.K; i0 += G) {
+      staged[warp][lane] = 8 * (i0 + lane) < a.K ? decode(i0 + lane) : make_uint4(0, 0, 0, 0);
       __syncwarp();
       const uint16_t* s = reinterpret_cast<const uint16_t*>(staged[warp]);
       uint16_t* to = reinterpret_cast<uint16_t*>(out + 8 * i0);

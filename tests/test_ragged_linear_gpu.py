@@ -106,6 +106,23 @@ def test_long_batches():
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('sizes,K,N', [([4100], 64, 40), ([2600, 1500], 130, 70), ([300, 0, 80], 128, 128)])
+def test_gradients_of_few_tiles(sizes, K, N, dtype):
+    # both gradients in one launch, the rows in parts; each by itself is as near to the exact one
+    d = data(sizes, K, N, dtype, seed=4)
+    check(d, True, dtype)
+    kw = dict(relu=True, need_db=False)
+    dx, none, _ = ops.ragged_linear_backward(d['dy'], d['x'], d['w'], d['saved'], d['offsets'], need_dw=False, **kw)
+    assert none is None
+    none, dw, _ = ops.ragged_linear_backward(d['dy'], d['x'], d['w'], d['saved'], d['offsets'], need_dx=False, **kw)
+    assert none is None
+    (x, w, _), (x_mag, w_mag, _) = routed.ragged_linear(d['x'], d['w'], None, d['edges'], relu=True, dy=d['dy'], y=d['saved'])
+    eps = torch.finfo(dtype).eps / 2 * 1.01
+    assert ((dx.double() - x).abs() <= x.abs() * eps + x_mag * sums(N, dtype)).all()
+    assert ((dw.double() - w).abs() <= w.abs() * U24 + w_mag * sums(max(sizes), dtype)).all()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('widths', [False, True])
 def test_members_without_rows_between_long_ones(widths, dtype):
     # more tiles than CTAs, so that one CTA goes from a sum in pieces to a tile that is zero
