@@ -22,9 +22,12 @@
 // (5e-7 with the cut, which costs 5 % of the time: 8 x 4096 x 4096 over 4096 rows each 863 us, 816 with pieces of 8192).
 // Few tiles over many rows are split over CTAs, into parts that a second launch adds up in order.
 //
-// fp32 operands come as three bf16 parts each (ragged_split_kernel), and the K loop goes through the six products of
-// parts whose terms exceed 2^-24 of the result, the smallest first: a sixth of the bf16 rate, where the CUDA cores give a
-// twenty-fifth.
+// fp32 operands come as three bf16 parts each (ragged_split_kernel), and the six products of parts whose terms exceed 2^-24
+// of the result are summed: a sixth of the bf16 rate, where the CUDA cores give a twenty-fifth.  Single CTAs hold all parts of a
+// block in a stage and sum the large product in an accumulator of its own, so that the others round at their own size;
+// tiles of 256 columns on pairs, for which there is no tensor memory left, go through the K loop once for each product, the
+// smallest first (both gradients of 12 members, 4099 rows, 100 -> 512: 32 us by six loops, 22 by one; forward of 8 members of
+// 512 rows, 512 -> 512, 29 by six loops, 17 by one; 8 x 2048 rows, 1024 -> 1024, 185 by one and 171 on pairs).
 #pragma once
 
 #include <type_traits>
@@ -75,7 +78,11 @@ struct RaggedTile {
 template <int BN_, int MODE, bool PAIR_, bool F32 = false>
 struct RaggedCfg {
   static constexpr bool PAIR = PAIR_;
-  static constexpr int PASSES = F32 ? 6 : 1;
+  // fp32 on single CTAs: a stage holds all three parts of its operands, whose six products go to two accumulators, that of
+  // the first parts and that of the others
+  static constexpr bool ALL = F32 && !PAIR;
+  static_assert(!ALL || BN_ == 128, "two accumulators of two buffers");
+  static constexpr int PARTS = ALL ? 3 : 1, PASSES = F32 && !ALL ? 6 : 1, PRODUCTS = ALL ? 6 : 1;
   static constexpr int SEGMENT = F32 ? RAGGED_SEGMENT_F32 : RAGGED_SEGMENT;
   static_assert(!PAIR || BN_ == 256, "pairs take tiles of 256 columns");
   static constexpr int BM = 128, BN = BN_, BK = 64;
@@ -83,11 +90,11 @@ struct RaggedCfg {
   static constexpr int B_ROWS = PAIR ? BN / 2 : BN;  // columns of B that a CTA stages
   static constexpr bool A_MN = MODE == RAGGED_WGRAD;
   static constexpr bool B_MN = MODE != RAGGED_FWD;
-  static constexpr int A_BYTES = BM * BK * 2, B_BYTES = B_ROWS * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int A_BYTES = BM * BK * 2, B_BYTES = B_ROWS * BK * 2, STAGE_BYTES = PARTS * (A_BYTES + B_BYTES);
   // fp32 results are summed up over the pieces of the K loop in the epilogue's registers, 64 columns a thread at most
   static constexpr bool SUMS = F32 || MODE == RAGGED_WGRAD;
-  static constexpr int STAGES = PAIR ? (F32 && MODE != RAGGED_WGRAD ? 5 : 6) : BN == 256 ? (F32 && MODE != RAGGED_WGRAD ? 3 : 4) : BN == 128 ? 6 : 7;
-  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int STAGES = ALL ? 2 : PAIR ? (F32 && MODE != RAGGED_WGRAD ? 5 : 6) : BN == 256 ? 4 : BN == 128 ? 6 : 7;
+  static constexpr int ACC_COLS = ALL ? 2 * BN : BN, TMEM_COLS = 2 * ACC_COLS;
   static constexpr int EPI_WARP0 = 4, EPI_WARPS = SUMS && BN == 256 ? 16 : 8;
   static constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
   static constexpr int TRING = 4;
@@ -187,7 +194,7 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
   extern __shared__ uint8_t dyn_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
   uint8_t* smA = smem;
-  uint8_t* smB = smem + STAGES * Cfg::A_BYTES;
+  uint8_t* smB = smem + STAGES * Cfg::PARTS * Cfg::A_BYTES;
   uint8_t* ctrl = smem + STAGES * Cfg::STAGE_BYTES;
   uint64_t* full = reinterpret_cast<uint64_t*>(ctrl);
   uint64_t* empty = full + STAGES;
@@ -240,17 +247,20 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
   auto b_of = [&](int pass) { return F32 ? (0x118 >> (2 * pass)) & 3 : 0; };
   // zeros from element `left` of a stage's K on, up to the next step of 16; by a whole warp
   auto zero_tail = [&](int stage, int left) {
-    uint8_t* a = smA + stage * Cfg::A_BYTES;
-    uint8_t* b = smB + stage * Cfg::B_BYTES;
     const int end = (left + 15) & ~15;
-    if constexpr (Cfg::A_MN)
-      zero_mn_major<Cfg::BM / 64>(a, left, end, lane);
-    else
-      zero_k_major(a, Cfg::BM, left, end, lane);
-    if constexpr (Cfg::B_MN)
-      zero_mn_major<Cfg::B_ROWS / 64>(b, left, end, lane);
-    else
-      zero_k_major(b, Cfg::B_ROWS, left, end, lane);
+#pragma unroll
+    for (int part = 0; part < Cfg::PARTS; ++part) {
+      uint8_t* a = smA + (stage * Cfg::PARTS + part) * Cfg::A_BYTES;
+      uint8_t* b = smB + (stage * Cfg::PARTS + part) * Cfg::B_BYTES;
+      if constexpr (Cfg::A_MN)
+        zero_mn_major<Cfg::BM / 64>(a, left, end, lane);
+      else
+        zero_k_major(a, Cfg::BM, left, end, lane);
+      if constexpr (Cfg::B_MN)
+        zero_mn_major<Cfg::B_ROWS / 64>(b, left, end, lane);
+      else
+        zero_k_major(b, Cfg::B_ROWS, left, end, lane);
+    }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
   };
@@ -316,12 +326,16 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
           else if (rank == 0)
             mbar_arrive_expect_tx(bar, 2 * Cfg::STAGE_BYTES);
         }
-        uint8_t* dst = ring0 + stage * bytes;
-        for (int c = 0; c < boxes; ++c) {
-          if constexpr (OWN)
-            tma_load_3d(dst + c * 8192, map, bar, x + (mn ? c * 64 : 0), y, z);
-          else
-            tma_load_3d_pair(dst + c * 8192, map, leader0 + 8u * stage, x + (mn ? c * 64 : 0), y, z);
+#pragma unroll
+        for (int part = 0; part < Cfg::PARTS; ++part) {
+          uint8_t* dst = ring0 + (stage * Cfg::PARTS + part) * bytes;
+          const int at = x + part * (is_a ? pr.a_part : pr.b_part);
+          for (int c = 0; c < boxes; ++c) {
+            if constexpr (OWN)
+              tma_load_3d(dst + c * 8192, map, bar, at + (mn ? c * 64 : 0), y, z);
+            else
+              tma_load_3d_pair(dst + c * 8192, map, leader0 + 8u * stage, at + (mn ? c * 64 : 0), y, z);
+          }
         }
         if (++stage == STAGES) {
           stage = 0;
@@ -340,7 +354,7 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
         const int k_first = WG ? t.rows : t.part, z = (is_a || WG) ? 0 : t.member;
         const int common = !PAIR ? 0 : is_cut(t) ? kblocks - 1 : kblocks;  // stages on the common barrier
         for (int pass = 0; ok && pass < Cfg::PASSES; ++pass) {
-          const int shift = is_a ? a_of(pass) * pr.a_part : b_of(pass) * pr.b_part;  // (0 for bf16)
+          const int shift = Cfg::PASSES == 1 ? 0 : is_a ? a_of(pass) * pr.a_part : b_of(pass) * pr.b_part;
           int kb = 0;
           for (; ok && kb < common; ++kb) {
             const int at = k_first + kb * Cfg::BK;
@@ -366,7 +380,7 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
       if (t.kind == RT_END) break;
       if (t.kind != RT_MMA) continue;
       const uint32_t idesc = idesc_bf16_f32(ragged_n(PAIR, BN, t), Cfg::A_MN, Cfg::B_MN, Cfg::TILE_M);
-      const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+      const uint32_t d_tmem = tmem_base + (uint32_t)(acc * Cfg::ACC_COLS);
       if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, abort_flag)) break;
       tc_fence_after();
       const int kblocks = (t.k_len + Cfg::BK - 1) / Cfg::BK;
@@ -374,18 +388,23 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
       const bool cut = is_cut(t);
       // a stage's products and its release, by one thread
       auto multiply = [&](int stage, int steps, bool first) {
-        const uint64_t adesc = adesc0 + (uint64_t)(stage * (Cfg::A_BYTES / 16));
-        const uint64_t bdesc = bdesc0 + (uint64_t)(stage * (Cfg::B_BYTES / 16));
 #pragma unroll
-        for (int s = 0; s < Cfg::BK / 16; ++s) {
-          // 16 elements further along K: 32 bytes of a K-major row, 16 rows of an MN-major block (in units of 16 bytes)
-          const uint64_t ad = adesc + (uint64_t)(s * (Cfg::A_MN ? 128 : 2)), bd = bdesc + (uint64_t)(s * (Cfg::B_MN ? 128 : 2));
-          const uint32_t on = (first && s == 0) ? 0u : 1u;
-          if (s < steps) {
-            if constexpr (PAIR)
-              umma_f16_pair(d_tmem, ad, bd, idesc, on);
-            else
-              umma_f16(d_tmem, ad, bd, idesc, on);
+        for (int product = 0; product < Cfg::PRODUCTS; ++product) {
+          const int a_part = Cfg::ALL ? a_of(product) : 0, b_part = Cfg::ALL ? b_of(product) : 0;
+          const uint64_t adesc = adesc0 + (uint64_t)((stage * Cfg::PARTS + a_part) * (Cfg::A_BYTES / 16));
+          const uint64_t bdesc = bdesc0 + (uint64_t)((stage * Cfg::PARTS + b_part) * (Cfg::B_BYTES / 16));
+          const uint32_t d = Cfg::ALL && product < 5 ? d_tmem + BN : d_tmem;
+#pragma unroll
+          for (int s = 0; s < Cfg::BK / 16; ++s) {
+            // 16 elements further along K: 32 bytes of a K-major row, 16 rows of an MN-major block (in units of 16 bytes)
+            const uint64_t ad = adesc + (uint64_t)(s * (Cfg::A_MN ? 128 : 2)), bd = bdesc + (uint64_t)(s * (Cfg::B_MN ? 128 : 2));
+            const uint32_t on = (first && s == 0 && (product == 0 || product == 5)) ? 0u : 1u;
+            if (s < steps) {
+              if constexpr (PAIR)
+                umma_f16_pair(d, ad, bd, idesc, on);
+              else
+                umma_f16(d, ad, bd, idesc, on);
+            }
           }
         }
         if constexpr (PAIR) {  // frees the stage in both CTAs
@@ -650,7 +669,7 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
         if (!mbar_wait(&tfull[acc], acc_phase, abort_flag)) break;
         tc_fence_after();
       }
-      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + slice * WCOLS);
+      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * Cfg::ACC_COLS + slice * WCOLS);
       if constexpr (Cfg::SUMS) {
         if (!(t.add & 1)) {
 #pragma unroll
@@ -661,9 +680,17 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
           for (int c = 0; c < WCOLS; c += 8) {
             uint32_t v[8];
             tmem_ld_32x32b_x8(t_row + (uint32_t)c, v);
-            tmem_wait_ld();
+            if constexpr (Cfg::ALL) {
+              uint32_t u[8];
+              tmem_ld_32x32b_x8(t_row + (uint32_t)(BN + c), u);
+              tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum[c + j] += __uint_as_float(v[j]);
+              for (int j = 0; j < 8; ++j) sum[c + j] += __uint_as_float(v[j]) + __uint_as_float(u[j]);
+            } else {
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 8; ++j) sum[c + j] += __uint_as_float(v[j]);
+            }
           }
           release();
           if (t.add & 2) continue;

@@ -352,12 +352,14 @@ int launch_ragged(const RaggedProblem& p, const CUtensorMap& ma, const CUtensorM
 }
 
 // How a product is cut into tiles, from its sizes alone.
+// (fp32: 128 columns, or pairs; with all of a block's parts in a stage 64 or 256 columns were never faster: 8 x 512 rows,
+// 512 -> 512, 24 / 17 / 29 us, 12 x 340 rows, 100 -> 512, 11.5 / 10.4 / 14.8.)
 struct RaggedPlan {
   bool pair;
   int bn, tile_m, splits;
 };
 
-RaggedPlan ragged_plan(int mode, int P, int64_t R, int in, int out) {
+RaggedPlan ragged_plan(int mode, bool f32, int P, int64_t R, int in, int out) {
   RaggedPlan plan{false, 256, 128, 1};
   const int cols = mode == RAGGED_DGRAD ? in : out;
   const long long used = std::min<long long>(P, R);
@@ -375,7 +377,7 @@ RaggedPlan ragged_plan(int mode, int P, int64_t R, int in, int out) {
   }
   // tiles along the rows: every member that has rows ends in a partial one
   const long long m_tiles = mode == RAGGED_WGRAD ? (long long)P * ((in + 127) / 128) : std::max(used, R / 128 + used / 2);
-  plan.bn = tile_columns(m_tiles, cols);
+  plan.bn = f32 ? 128 : tile_columns(m_tiles, cols);
   if (mode == RAGGED_WGRAD) {
     // parts of 512 rows at least, as many as the SMs take at once, 256 MB of results at most
     const long long tiles = m_tiles * ((cols + plan.bn - 1) / plan.bn);
@@ -443,16 +445,15 @@ template <int MODE, bool F32>
 int ragged_product(const RaggedProblem& p, const void* a_ptr, long long a_ld, const void* b_ptr, long long b_ld, float* parts,
                    cudaStream_t st) {
   RaggedCall c;
-  int rc = ragged_call<MODE, F32>(c, p, ragged_plan(MODE, p.P, p.R, p.in, p.out), a_ptr, a_ld, b_ptr, b_ld, parts);
+  int rc = ragged_call<MODE, F32>(c, p, ragged_plan(MODE, F32, p.P, p.R, p.in, p.out), a_ptr, a_ld, b_ptr, b_ld, parts);
   if (rc) return rc;
   if (c.plan.pair)
     rc = launch_ragged<256, MODE, true, F32>(c.p, c.ma, c.mb, c.most, st);
-  else if (c.plan.bn == 256)
-    rc = launch_ragged<256, MODE, false, F32>(c.p, c.ma, c.mb, c.most, st);
-  else if (c.plan.bn == 128)
+  else if (F32 || c.plan.bn == 128)
     rc = launch_ragged<128, MODE, false, F32>(c.p, c.ma, c.mb, c.most, st);
-  else
-    rc = launch_ragged<64, MODE, false, F32>(c.p, c.ma, c.mb, c.most, st);
+  else if constexpr (!F32)
+    rc = c.plan.bn == 256 ? launch_ragged<256, MODE, false, false>(c.p, c.ma, c.mb, c.most, st)
+                          : launch_ragged<64, MODE, false, false>(c.p, c.ma, c.mb, c.most, st);
   return rc || MODE != RAGGED_WGRAD ? rc : ragged_add_parts(c, st);
 }
 
@@ -471,22 +472,24 @@ int launch_gradients(const RaggedCall& x, const RaggedCall& w, cudaStream_t st) 
 
 // Both gradients, g (rows, out) and x (rows, in) with their row strides: in one launch where the tiles of both, of 64 or else
 // 128 columns, fit the SMs at once (7 members, 2571 rows, 200 -> 531 bf16: 19 us one after the other, 12.2 together; 12 members, 4099 rows,
-// 100 -> 512 fp32: 53, 32).
+// 100 -> 512 fp32: 43, 22).
 template <bool F32>
 int ragged_gradients(const RaggedProblem& px, const void* g, long long g_ld, const void* w, long long w_ld, const RaggedProblem& pw,
                      const void* x, long long x_ld, float* parts, cudaStream_t st) {
-  for (int bn = 64; bn <= 128; bn *= 2) {
+  for (int bn = F32 ? 128 : 64; bn <= 128; bn *= 2) {
     RaggedPlan plan_x{false, bn, 128, 1}, plan_w = plan_x;
     const long long tiles_x = ragged_tiles(RAGGED_DGRAD, plan_x, px.P, px.R, px.in, px.out);
     const long long tiles_w = ragged_tiles(RAGGED_WGRAD, plan_w, px.P, px.R, px.in, px.out), sms = device_info().sms;
     if (tiles_x + tiles_w > sms) continue;
     // (the workspace holds the parts that the product alone would be split into)
-    plan_w.splits = (int)std::min<long long>(ragged_plan(RAGGED_WGRAD, px.P, px.R, px.in, px.out).splits, (sms - tiles_x) / tiles_w);
+    plan_w.splits = (int)std::min<long long>(ragged_plan(RAGGED_WGRAD, F32, px.P, px.R, px.in, px.out).splits, (sms - tiles_x) / tiles_w);
     RaggedCall cx, cw;
     int rc = ragged_call<RAGGED_DGRAD, F32>(cx, px, plan_x, g, g_ld, w, w_ld, nullptr);
     if (!rc) rc = ragged_call<RAGGED_WGRAD, F32>(cw, pw, plan_w, x, x_ld, g, g_ld, parts);
     if (rc) return rc;
-    return bn == 64 ? launch_gradients<64, F32>(cx, cw, st) : launch_gradients<128, F32>(cx, cw, st);
+    if constexpr (!F32)
+      if (bn == 64) return launch_gradients<64, false>(cx, cw, st);
+    return launch_gradients<128, F32>(cx, cw, st);
   }
   const int rc = ragged_product<RAGGED_DGRAD, F32>(px, g, g_ld, w, w_ld, nullptr, st);
   return rc ? rc : ragged_product<RAGGED_WGRAD, F32>(pw, x, x_ld, g, g_ld, parts, st);
@@ -569,7 +572,7 @@ RaggedSpace ragged_space(const tp_ragged_linear_args* a) {
     if (a->dbias && ragged_shares(a) > 1) s.parts += round256((size_t)ragged_shares(a) * a->P * a->max_out * sizeof(float));
     s.g3 = s.parts;
     if (a->dw) {
-      const int splits = ragged_plan(RAGGED_WGRAD, a->P, a->rows, a->max_in, a->max_out).splits;
+      const int splits = ragged_plan(RAGGED_WGRAD, a->dtype == TP_DTYPE_F32, a->P, a->rows, a->max_in, a->max_out).splits;
       if (splits > 1) s.g3 += round256((size_t)splits * a->P * a->max_out * a->max_in * sizeof(float));
     }
   }
