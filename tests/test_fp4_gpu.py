@@ -396,3 +396,12 @@ def test_refusals():
         ops.fp4_linear_forward(x, q._replace(format='mxfp4'))
     with pytest.raises(RuntimeError):
         ops.fp4_linear_forward(x.cpu(), q)
+
+
+@pytest.mark.parametrize('K', [32768, 32767])
+def test_more_elements_than_31_bits(K):
+    x = torch.randn(66000, 32768, device='cuda', dtype=torch.bfloat16)[:, :K]
+    for format in ('nvfp4', 'mxfp4'):
+        values = ops.fp4_values(ops.fp4_quantize(x, format))
+        alone = ops.fp4_values(ops.fp4_quantize(x[-130:].contiguous(), format))
+        assert torch.equal(values[-130:], alone)

@@ -310,3 +310,21 @@ def test_refusals():
     with pytest.raises(TypeError):
         ops.combine_rows_backward(torch.zeros(10, 4, device='cuda').bfloat16(), torch.zeros(20, 4, device='cuda'), weight,
                                   position, offsets)
+
+
+def test_more_elements_than_31_bits():
+    T, k, W = 34000, 2, 32768  # 2.2e9 elements in y
+    x = torch.randn(T, W, device='cuda', dtype=torch.bfloat16)
+    weight, _, position, offsets, _ = ops.route_forward(torch.randn(T, 8, device='cuda'), k)
+    y = ops.dispatch_rows(x, position, offsets)
+    some = torch.tensor([0, T // 2, T - 1, int(position.argmax()) // k], device='cuda')
+    for j in range(k):
+        assert torch.equal(y[position[some, j].long()], x[some])
+    out = ops.combine_rows(y, weight, position, offsets)
+    want = x[some].double() * weight[some].double().sum(1, keepdim=True)
+    # a product and a sum in fp32, then one rounding to bf16
+    assert ((out[some].double() - want).abs() <= want.abs() * (2.0 ** -8 + 4 * 2.0 ** -24)).all()
+    del out
+    dy, _ = ops.combine_rows_backward(x, y, weight, position, offsets, need_dweight=False)
+    want = weight[some, 1:].double() * x[some].double()
+    assert ((dy[position[some, 1].long()].double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -24)).all()
