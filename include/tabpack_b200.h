@@ -657,7 +657,7 @@ const char* tp_version(void);
 #define TP_ROUTE_MAX_EXPERTS 1024
 #define TP_ROUTE_MAX_K 32
 typedef struct tp_route_args {
-  int64_t rows;             /* rows * top_k < 2^31 */
+  int64_t rows;             /* rows * top_k <= 2^31 - 2^20 */
   int32_t E, top_k;
   int32_t dtype;            /* TP_DTYPE_F32 or TP_DTYPE_BF16: logits, dlogits */
   int32_t renormalize;

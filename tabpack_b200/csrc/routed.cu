@@ -48,11 +48,13 @@ RoutePlan route_plan(int64_t rows, int32_t k) {
   return p;
 }
 
+constexpr long long ROUTE_MAX_PAIRS = (1ll << 31) - (1ll << 20);  // (the kernels look some rows ahead)
+
 int check_route(const tp_route_args* a) {
   if (!a) return fail(TP_EINVAL, "null routing arguments");
   if (a->rows <= 0 || a->E <= 0 || a->E > ROUTE_MAX_EXPERTS || a->top_k <= 0 ||
-      a->top_k > std::min(ROUTE_MAX_K, a->E) || a->rows * a->top_k >= (1ll << 31))
-    return fail(TP_EINVAL, "routing needs rows > 0, 1 to %d members, top_k up to %d and the members, rows top_k < 2^31 "
+      a->top_k > std::min(ROUTE_MAX_K, a->E) || a->rows * a->top_k > ROUTE_MAX_PAIRS)
+    return fail(TP_EINVAL, "routing needs rows > 0, 1 to %d members, top_k up to %d and the members, rows top_k <= 2^31 - 2^20 "
                 "(got %lld, %d, %d)", ROUTE_MAX_EXPERTS, ROUTE_MAX_K, (long long)a->rows, a->E, a->top_k);
   if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad logits dtype");
   if (!a->logits || !a->weight || !a->expert) return fail(TP_EINVAL, "null logits, weights or members");
@@ -86,39 +88,55 @@ RouteArgs route_args(const tp_route_args* a) {
   return k;
 }
 
-template <typename T, int V>
+template <typename T, int G, int F, int V>
 int launch_route(const RouteArgs& k, cudaStream_t st) {
   const int blocks = k.blocks;
   const size_t smem = route_shared_bytes(k.E);
   if (blocks == 1) {
-    int rc = allow_smem<route_small_kernel<T, V>>(smem);
+    int rc = allow_smem<route_small_kernel<T, G, F, V>>(smem);
     if (rc) return rc;
-    route_small_kernel<T, V><<<1, 32 * ROUTE_WARPS, smem, st>>>(k);
+    route_small_kernel<T, G, F, V><<<1, 32 * ROUTE_WARPS, smem, st>>>(k);
   } else {
-    int rc = allow_smem<route_gate_kernel<T, V>>(smem);
+    int rc = allow_smem<route_gate_kernel<T, G, F, V>>(smem);
     if (!rc) rc = allow_smem<route_place_kernel>(smem);
     if (rc) return rc;
-    route_gate_kernel<T, V><<<blocks, 32 * ROUTE_WARPS, smem, st>>>(k);
+    route_gate_kernel<T, G, F, V><<<blocks, 32 * ROUTE_WARPS, smem, st>>>(k);
     route_scan_kernel<<<k.E + 1, 256, 0, st>>>(k);
     route_place_kernel<<<(blocks + k.gates - 1) / k.gates, 32 * ROUTE_WARPS, smem, st>>>(k);
   }
   return TP_OK;
 }
 
-template <typename T, int V>
+template <typename T, int G, int F, int V>
 int launch_route_backward(const RouteArgs& k, cudaStream_t st) {
-  route_backward_kernel<T, V><<<std::min((k.rows + 7) / 8, 8 * device_info().sms), 256, 0, st>>>(k);
+  constexpr int ROWS = 256 / G;
+  route_backward_kernel<T, G, F, V><<<std::min((k.rows + ROWS - 1) / ROWS, 8 * device_info().sms), 256, 0, st>>>(k);
   return TP_OK;
 }
 
-// Registers a lane needs for a row of E scores.
+// Lanes a row and registers a lane for its scores: few lanes where a row's scores fit eight registers of them (and the slots
+// their lanes), since a row's reductions and ends then share their instructions with other rows'.  Gate and backward of 65536
+// rows: 24 members, 2 slots, 7.4 and 5.2 us with 4 lanes, 17.6 and 15.9 with 32; 64 members, 4 slots, 15.9 and 8.7 with 8
+// lanes, 23.6 and 17.0 with 32.  The backward holds less else and takes 16 lanes up to 18 registers: 32768 rows of 160 8.7
+// against 11.5; the gate does not: 20.3 against 19, and 65521 rows of 257 69 against 39.
 template <typename T>
 int dispatch_route(const RouteArgs& k, bool backward, cudaStream_t st) {
-#define TP_ROUTE_V(v) \
-  if (k.E <= 32 * v) return backward ? launch_route_backward<T, v>(k, st) : launch_route<T, v>(k, st);
-  TP_ROUTE_V(1) TP_ROUTE_V(2) TP_ROUTE_V(3) TP_ROUTE_V(4) TP_ROUTE_V(5) TP_ROUTE_V(6) TP_ROUTE_V(7) TP_ROUTE_V(8) TP_ROUTE_V(9)
-  TP_ROUTE_V(10) TP_ROUTE_V(12) TP_ROUTE_V(14) TP_ROUTE_V(16) TP_ROUTE_V(18) TP_ROUTE_V(20) TP_ROUTE_V(24) TP_ROUTE_V(28) TP_ROUTE_V(32)
-#undef TP_ROUTE_V
+  const int E = k.E, slots = k.k;
+#define TP_ROUTE(g, f, v) \
+  if (E <= g * v && slots <= g) return backward ? launch_route_backward<T, g, f, v>(k, st) : launch_route<T, g, f, v>(k, st);
+#define TP_ROUTE_G(g) TP_ROUTE(g, 0, 2) TP_ROUTE(g, 2, 4) TP_ROUTE(g, 4, 6) TP_ROUTE(g, 6, 8)
+#define TP_ROUTE_BACK(f, v) \
+  if (backward && E <= 16 * v && slots <= 16) return launch_route_backward<T, 16, f, v>(k, st);
+  TP_ROUTE_G(4)
+  TP_ROUTE_G(8)
+  TP_ROUTE_G(16)
+  TP_ROUTE_BACK(8, 10) TP_ROUTE_BACK(10, 12) TP_ROUTE_BACK(12, 14) TP_ROUTE_BACK(14, 16) TP_ROUTE_BACK(16, 18)
+  TP_ROUTE(32, 0, 4)
+  TP_ROUTE(32, 4, 5) TP_ROUTE(32, 5, 6) TP_ROUTE(32, 6, 7) TP_ROUTE(32, 7, 8) TP_ROUTE(32, 8, 9) TP_ROUTE(32, 9, 10)
+  TP_ROUTE(32, 10, 12) TP_ROUTE(32, 12, 14) TP_ROUTE(32, 14, 16) TP_ROUTE(32, 16, 20) TP_ROUTE(32, 20, 24) TP_ROUTE(32, 24, 32)
+#undef TP_ROUTE_BACK
+#undef TP_ROUTE_G
+#undef TP_ROUTE
   return fail(TP_EINVAL, "too many members");
 }
 

@@ -36,27 +36,41 @@ struct RouteArgs {
   void* dlogits;              // (rows, E)
 };
 
-__device__ __forceinline__ float warp_sum(float v) {
+// Sums and largest values over G neighbouring lanes, for every lane of them.
+template <int G>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  for (int o = G / 2; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   return v;
 }
-// The warp's largest value (no NaN among them).
-__device__ __forceinline__ float warp_max(float v) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
+template <int G>
+__device__ __forceinline__ float lanes_max(float v) {  // (no NaN among them)
+  if constexpr (G == 32) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+  } else {
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return v;
+  }
+}
+template <int G>
+__device__ __forceinline__ int lanes_min(unsigned v) {
+  if constexpr (G == 32) {
+    return (int)__reduce_min_sync(0xFFFFFFFFu, v);
+  } else {
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) v = min(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return (int)v;
+  }
 }
 
-// A lane's scores of a row that are sure to be there, where V of them are enough: more than those of the next smaller V.
-// (V goes by one up to ten and in steps of an eighth to a fifth beyond.)
-__host__ __device__ constexpr int route_full(int V) { return V <= 10 ? V - 1 : V <= 20 ? V - 2 : V - 4; }
-
-// A row's scores, lane l holding members l, l + 32, ...; -inf past the last member.
-template <typename T, int V>
-__device__ __forceinline__ void route_load(const T* z, int E, int lane, float (&v)[V]) {
+// A row's scores, lane l of its G holding members l, l + G, ...; -inf past the last member.  The first F are there for sure.
+template <typename T, int G, int F, int V>
+__device__ __forceinline__ void route_load(const T* z, int E, int l, float (&v)[V]) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = i < route_full(V) || lane + 32 * i < E ? (float)z[lane + 32 * i] : -INFINITY;
+  for (int i = 0; i < V; ++i) v[i] = i < F || l + G * i < E ? (float)z[l + G * i] : -INFINITY;
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -70,12 +84,13 @@ __device__ __forceinline__ float exp_of(float z, float c) {
 // Shared memory of the gate: hist[E + 1], sums[ROUTE_WARPS][E]; of the places: base[E + 1], counts[ROUTE_WARPS][E + 1].
 __host__ __device__ inline size_t route_shared_bytes(int E) { return sizeof(int) * ((size_t)(ROUTE_WARPS + 1) * (E + 1)); }
 
-// Weights and members of the block's rows, their counts per member, and the sums of p.  Instructions bound it, some
-// 300 a row for 257 members and 6 slots: each lane finds its two best at once, so that a slot costs two reductions and
-// a search through the lane's scores only where one lane has three of a row's best.
-template <typename T, int V>
+// Weights and members of the block's rows, their counts per member, and the sums of p; G lanes a row.  Instructions bound
+// it (some 500 a row for 257 members and 6 slots with a warp a row, 40 us for 65521 of them): each lane finds its two best at once, so that a slot costs two
+// reductions and a search through the lane's scores only where one lane has three of a row's best.
+template <typename T, int G, int F, int V>
 __device__ __forceinline__ void route_gate(const RouteArgs& a, int block, int* smem) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int RPW = 32 / G;  // rows of a warp at a time
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % G;
   const int E = a.E, k = a.k;
   int* hist = smem;
   float* sums = reinterpret_cast<float*>(hist + E + 1);
@@ -85,13 +100,18 @@ __device__ __forceinline__ void route_gate(const RouteArgs& a, int block, int* s
   const T* logits = static_cast<const T*>(a.logits);
   float imp[V], next[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) imp[v] = 0.f;
-  if (r0 + warp < r1) route_load<T, V>(logits + (long long)(r0 + warp) * a.ld, E, lane, next);
-  for (int r = r0 + warp; r < r1; r += ROUTE_WARPS) {
+  for (int v = 0; v < V; ++v) {
+    imp[v] = 0.f;
+    next[v] = -INFINITY;
+  }
+  int r = r0 + warp * RPW + lane / G;
+  if (r < r1) route_load<T, G, F, V>(logits + (long long)r * a.ld, E, l, next);
+  for (int first = r0 + warp * RPW; first < r1; first += ROUTE_WARPS * RPW, r += ROUTE_WARPS * RPW) {
+    const bool live = r < r1;  // (rows past the last one hold what the lanes had before; nothing of them is kept)
     float z[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) z[v] = next[v];
-    if (r + ROUTE_WARPS < r1) route_load<T, V>(logits + (long long)(r + ROUTE_WARPS) * a.ld, E, lane, next);
+    if (r + ROUTE_WARPS * RPW < r1) route_load<T, G, F, V>(logits + (long long)(r + ROUTE_WARPS * RPW) * a.ld, E, l, next);
     // this lane's two best, b1 and b2, and which they are (equal ones: the lower first; a NaN is never greater)
     float b1, b2;
     int w1, w2;
@@ -108,7 +128,7 @@ __device__ __forceinline__ void route_gate(const RouteArgs& a, int block, int* s
       }
     };
     two_best();
-    float top = warp_max(b1);
+    float top = lanes_max<G>(b1);
     float c = top > -INFINITY ? -top * LOG2E : 0.f;
     float e[V], total = 0.f;
 #pragma unroll
@@ -116,34 +136,37 @@ __device__ __forceinline__ void route_gate(const RouteArgs& a, int block, int* s
       e[v] = exp_of(z[v], c);  // 0 for -inf
       total += e[v];
     }
-    total = warp_sum(total);
-    if (total != total) {
+    total = lanes_sum<G>(total);
+    if (__any_sync(0xFFFFFFFFu, total != total)) {
       // a NaN or +inf: all weights are NaN, and a NaN ranks as +inf
 #pragma unroll
       for (int v = 0; v < V; ++v)
         if (z[v] != z[v]) z[v] = INFINITY;
       two_best();
-      top = warp_max(b1);
+      top = lanes_max<G>(b1);
     }
-    const float inv = top > -INFINITY ? 1.f / total : 0.f;
+    const float inv = !live || !(top > -INFINITY) ? 0.f : 1.f / total;
+    if (live) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) imp[v] = fmaf(e[v], inv, imp[v]);
+      for (int v = 0; v < V; ++v) imp[v] = fmaf(e[v], inv, imp[v]);
+    }
     // the k best: lane j keeps slot j
     float mine = 0.f, best = b1;
-    int my_expert = -1, which = lane + 32 * w1;
+    int my_expert = -1, which = l + G * w1;
     bool spare = true;  // b2 is the next one
     for (int j = 0; j < k; ++j) {
-      const float b = j == 0 ? top : warp_max(best);
-      if (b == -INFINITY) break;
-      const int who = (int)__reduce_min_sync(0xFFFFFFFFu, best == b ? (unsigned)which : 0xFFFFFFFFu);
-      if (lane == j) {
+      const float b = j == 0 ? top : lanes_max<G>(best);
+      if (G == 32 && b == -INFINITY) break;
+      const int who = lanes_min<G>(best == b ? (unsigned)which : 0xFFFFFFFFu);
+      if (b == -INFINITY) continue;  // (of a row that shares the warp with others)
+      if (l == j) {
         mine = b;
         my_expert = who;
       }
       if (which == who && best == b) {
         if (spare) {
           best = b2;
-          which = lane + 32 * w2;
+          which = l + G * w2;
           spare = false;
         } else {
           // the best one behind (b, who)
@@ -151,26 +174,30 @@ __device__ __forceinline__ void route_gate(const RouteArgs& a, int block, int* s
           int w = 0;
 #pragma unroll
           for (int v = 0; v < V; ++v)
-            if ((z[v] < b || (z[v] == b && lane + 32 * v > who)) && z[v] > best) {
+            if ((z[v] < b || (z[v] == b && l + G * v > who)) && z[v] > best) {
               best = z[v];
               w = v;
             }
-          which = lane + 32 * w;
+          which = l + G * w;
         }
       }
     }
+    __syncwarp();
     float w = my_expert >= 0 ? exp_of(mine, c) : 0.f;
-    const float of = a.renorm ? warp_sum(w) : total;
+    const float of = a.renorm ? lanes_sum<G>(w) : total;
     if (my_expert >= 0) w = total == total ? w / of : total;
-    if (lane < k) {
-      a.weight[(long long)r * k + lane] = w;
-      a.expert[(long long)r * k + lane] = my_expert;
+    if (live && l < k) {
+      a.weight[(long long)r * k + l] = w;
+      a.expert[(long long)r * k + l] = my_expert;
       atomicAdd(&hist[my_expert < 0 ? E : my_expert], 1);  // whole numbers: any order gives the same count
     }
   }
 #pragma unroll
-  for (int v = 0; v < V; ++v)
-    if (lane + 32 * v < E) sums[warp * E + lane + 32 * v] = imp[v];
+  for (int v = 0; v < V; ++v) {
+#pragma unroll
+    for (int o = G; o < 32; o <<= 1) imp[v] += __shfl_xor_sync(0xFFFFFFFFu, imp[v], o);
+    if (lane < G && l + G * v < E) sums[warp * E + l + G * v] = imp[v];
+  }
   __syncthreads();
   // (a single block's sums are the result; its counts stay in shared memory)
   for (int e = threadIdx.x; e <= E; e += blockDim.x) {
@@ -206,7 +233,7 @@ __global__ void __launch_bounds__(256) route_scan_kernel(const RouteArgs a) {
     const int t = __shfl_up_sync(0xFFFFFFFFu, inc, o);
     if (lane >= o) inc += t;
   }
-  s = warp_sum(s);
+  s = lanes_sum<32>(s);
   if (lane == 31) {
     counts[warp] = inc;
     sums[warp] = s;
@@ -297,10 +324,10 @@ __device__ __forceinline__ void route_place(const RouteArgs& a, int gate, int* s
   }
 }
 
-template <typename T, int V>
+template <typename T, int G, int F, int V>
 __global__ void __launch_bounds__(32 * ROUTE_WARPS, V <= 16 ? 2 : 1) route_gate_kernel(const RouteArgs a) {
   extern __shared__ int route_smem[];
-  route_gate<T, V>(a, blockIdx.x, route_smem);
+  route_gate<T, G, F, V>(a, blockIdx.x, route_smem);
 }
 
 __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_place_kernel(const RouteArgs a) {
@@ -309,43 +336,47 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_place_kernel(const Rou
 }
 
 // Few rows: all of it in one block.
-template <typename T, int V>
+template <typename T, int G, int F, int V>
 __global__ void __launch_bounds__(32 * ROUTE_WARPS) route_small_kernel(const RouteArgs a) {
   extern __shared__ int route_smem[];
-  route_gate<T, V>(a, 0, route_smem);
+  route_gate<T, G, F, V>(a, 0, route_smem);
   __syncthreads();
   route_place<true>(a, 0, route_smem);
 }
 
-// dz of a row by one warp: p is formed again from the scores (reading it would cost more than the sums).  Lane j then
+// dz of a row by G lanes: p is formed again from the scores (reading it would cost more than the sums).  Lane j then
 // writes the chosen member of slot j over what the row's formula without the slots' gradients gave.
-template <typename T, int V>
+template <typename T, int G, int F, int V>
 __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int E = a.E, k = a.k, stride = gridDim.x * 8;
+  const int l = threadIdx.x % G;
+  const int E = a.E, k = a.k, stride = gridDim.x * (256 / G);
   const T* logits = static_cast<const T*>(a.logits);
   T* dlogits = static_cast<T*>(a.dlogits);
   float h[V], next[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = (a.g_importance != nullptr && lane + 32 * v < E) ? a.g_importance[lane + 32 * v] : 0.f;
-  int r = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (r < a.rows) route_load<T, V>(logits + (long long)r * a.ld, E, lane, next);
-  for (; r < a.rows; r += stride) {
+  for (int v = 0; v < V; ++v) {
+    h[v] = (a.g_importance != nullptr && l + G * v < E) ? a.g_importance[l + G * v] : 0.f;
+    next[v] = -INFINITY;
+  }
+  int r = blockIdx.x * (256 / G) + (int)threadIdx.x / G;
+  if (r < a.rows) route_load<T, G, F, V>(logits + (long long)r * a.ld, E, l, next);
+  for (int first = blockIdx.x * (256 / G) + (int)(threadIdx.x & ~31u) / G; first < a.rows; first += stride, r += stride) {
+    const bool live = r < a.rows;
     float p[V], best = -INFINITY;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       p[v] = next[v];
       best = max_nan(best, p[v]);
     }
-    if (r + stride < a.rows) route_load<T, V>(logits + (long long)(r + stride) * a.ld, E, lane, next);
+    if (r + stride < a.rows) route_load<T, G, F, V>(logits + (long long)(r + stride) * a.ld, E, l, next);
     // slot j on lane j
     float w = 0.f, g = 0.f, z_mine = 0.f, h_mine = 0.f;
     int who = -1;
-    if (lane < k && a.g_weight != nullptr) {
-      who = a.expert[(long long)r * k + lane];
+    if (live && l < k && a.g_weight != nullptr) {
+      who = a.expert[(long long)r * k + l];
       if ((unsigned)who < (unsigned)E) {
-        w = a.weight[(long long)r * k + lane];
-        g = a.g_weight[(long long)r * k + lane];
+        w = a.weight[(long long)r * k + l];
+        g = a.g_weight[(long long)r * k + l];
         z_mine = (float)logits[(long long)r * a.ld + who];
         if (a.g_importance != nullptr) h_mine = a.g_importance[who];
       } else {
@@ -353,7 +384,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs a) 
       }
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) best = max_nan(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
+    for (int o = G / 2; o; o >>= 1) best = max_nan(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
     const bool some = best != -INFINITY;
     const float c = some ? -best * LOG2E : 0.f;
     float total = 0.f, ph = 0.f;
@@ -365,7 +396,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs a) 
     }
     float wg = w * g;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
+    for (int o = G / 2; o; o >>= 1) {
       total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
       ph += __shfl_xor_sync(0xFFFFFFFFu, ph, o);
       wg += __shfl_xor_sync(0xFFFFFFFFu, wg, o);
@@ -373,9 +404,11 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs a) 
     const float inv = some ? 1.f / total : 0.f;
     const float through = fmaf(ph, inv, a.renorm ? 0.f : wg);
     T* out = dlogits + (long long)r * E;
+    if (live) {
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v < route_full(V) || lane + 32 * v < E) out[lane + 32 * v] = (T)(p[v] * inv * (h[v] - through));
+      for (int v = 0; v < V; ++v)
+        if (v < F || l + G * v < E) out[l + G * v] = (T)(p[v] * inv * (h[v] - through));
+    }
     __syncwarp();
     if (who >= 0) {
       const float p_mine = exp_of(z_mine, c) * inv;

@@ -54,6 +54,24 @@ def test_route(T, E, k, renormalize, dtype):
     check_route(scores(T, E, dtype, T + E), k, renormalize)
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('E,k', [(2, 2), (8, 4), (24, 2), (32, 4), (33, 4), (24, 5), (64, 8), (65, 8), (100, 9), (128, 16), (129, 16), (100, 17)])
+def test_rows_that_share_a_warp(E, k, dtype):
+    # 4, 8, 16 and 32 lanes a row; rows with nothing, with NaN and with ties beside ordinary ones
+    z = scores(3001, E, dtype, E * k, masked=0.3)
+    z[::7] = -math.inf
+    z[3::11] = torch.round(z[3::11])
+    check_route(z, k, True)
+    z[5::64, 0] = math.nan
+    weight, expert, position, offsets, _ = ops.route_forward(z, k)
+    rows = torch.isnan(z.float()).any(1)
+    assert torch.isnan(weight[rows][expert[rows] >= 0]).all() and not torch.isnan(weight[~rows]).any()
+    clean = z.clone()
+    clean[rows] = -math.inf
+    other = ops.route_forward(clean, k)
+    assert torch.equal(weight[~rows], other[0][~rows]) and torch.equal(expert[~rows], other[1][~rows])
+
+
 @pytest.mark.parametrize('T', [5, 3000])
 @pytest.mark.parametrize('renormalize', [True, False])
 def test_route_masked(T, renormalize):
