@@ -24,12 +24,15 @@ namespace {
 template <auto* KERNEL>
 int allow_smem(size_t bytes) {
   static std::atomic<size_t> have[64] = {};
+  static std::mutex mu;  // (another thread's smaller size must not come after a larger one)
   int dev = 0;
   TP_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return fail(TP_EUNSUPPORTED, "device index %d out of range", dev);
+  if (have[dev].load(std::memory_order_acquire) >= bytes) return TP_OK;
+  std::lock_guard<std::mutex> lock(mu);
   if (have[dev].load(std::memory_order_relaxed) >= bytes) return TP_OK;
   TP_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  have[dev].store(bytes, std::memory_order_relaxed);
+  have[dev].store(bytes, std::memory_order_release);
   return TP_OK;
 }
 
@@ -53,7 +56,7 @@ constexpr long long ROUTE_MAX_PAIRS = (1ll << 31) - (1ll << 20);  // (the kernel
 int check_route(const tp_route_args* a) {
   if (!a) return fail(TP_EINVAL, "null routing arguments");
   if (a->rows <= 0 || a->E <= 0 || a->E > ROUTE_MAX_EXPERTS || a->top_k <= 0 ||
-      a->top_k > std::min(ROUTE_MAX_K, a->E) || a->rows * a->top_k > ROUTE_MAX_PAIRS)
+      a->top_k > std::min(ROUTE_MAX_K, a->E) || a->rows > ROUTE_MAX_PAIRS || a->rows * a->top_k > ROUTE_MAX_PAIRS)
     return fail(TP_EINVAL, "routing needs rows > 0, 1 to %d members, top_k up to %d and the members, rows top_k <= 2^31 - 2^20 "
                 "(got %lld, %d, %d)", ROUTE_MAX_EXPERTS, ROUTE_MAX_K, (long long)a->rows, a->E, a->top_k);
   if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad logits dtype");
@@ -144,7 +147,8 @@ int dispatch_route(const RouteArgs& k, bool backward, cudaStream_t st) {
 
 int check_rows(const tp_rows_args* a) {
   if (!a) return fail(TP_EINVAL, "null row move arguments");
-  if (a->rows <= 0 || a->k <= 0 || a->k > ROUTE_MAX_K || a->W <= 0 || a->E <= 0 || a->rows * a->k >= (1ll << 31))
+  if (a->rows <= 0 || a->k <= 0 || a->k > ROUTE_MAX_K || a->W <= 0 || a->E <= 0 || a->rows >= (1ll << 31) ||
+      a->rows * a->k >= (1ll << 31))
     return fail(TP_EINVAL, "row moves need rows, W, E > 0, 1 <= k <= %d, rows k < 2^31 (got %lld, %d, %d, %d)", ROUTE_MAX_K,
                 (long long)a->rows, a->W, a->E, a->k);
   if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad row dtype");

@@ -54,7 +54,7 @@ def test_route_arguments(bad, want):
     assert code('tp_route_backward', route(**bad)) == want
 
 
-@pytest.mark.parametrize('rows,top_k', [((1 << 31) - (1 << 20) + 1, 1), ((1 << 30) - (1 << 19) + 1, 2)])
+@pytest.mark.parametrize('rows,top_k', [((1 << 31) - (1 << 20) + 1, 1), ((1 << 30) - (1 << 19) + 1, 2), (1 << 62, 4)])
 def test_route_refuses_more_pairs_than_it_counts(rows, top_k):
     assert code('tp_route_forward', route(rows=rows, top_k=top_k)) == -1
     assert code('tp_route_backward', route(rows=rows, top_k=top_k)) == -1
