@@ -704,6 +704,10 @@ int tp_dispatch_rows(const tp_rows_args* a, void* stream);
 int tp_combine_rows(const tp_rows_args* a, void* stream);
 int tp_combine_rows_backward(const tp_rows_args* a, void* stream);
 
+/* Rows of `cols` bf16 numbers, any stride, as rows at a multiple of 8 elements on a 16-byte boundary, zeros behind column cols:
+ * what tp_ragged_linear_* take. */
+int tp_align_rows(const void* x, int64_t x_stride, int64_t rows, int32_t cols, void* out, int64_t out_stride, void* stream);
+
 /* Linear layer of a pack over ragged groups of rows: member m's rows are offsets[m] .. offsets[m + 1] - 1 of x,
  *   y = relu(x w_m^T + b_m),  g = dy [y > 0],  dx = g w_m,  dw_m = g^T x,  db_m = sum g.
  * offsets (device, P + 1) do not decrease and stay within 0 .. rows (what does not is cut).  Rows of no member are zero

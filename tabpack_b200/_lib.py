@@ -316,6 +316,8 @@ SIGNATURES = {
     'tp_dispatch_rows': (ctypes.c_int, [ctypes.POINTER(RowsArgs), ctypes.c_void_p]),
     'tp_combine_rows': (ctypes.c_int, [ctypes.POINTER(RowsArgs), ctypes.c_void_p]),
     'tp_combine_rows_backward': (ctypes.c_int, [ctypes.POINTER(RowsArgs), ctypes.c_void_p]),
+    'tp_align_rows': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p,
+                                     ctypes.c_int64, ctypes.c_void_p]),
     'tp_ragged_linear_workspace_size': (ctypes.c_size_t, [ctypes.POINTER(RaggedLinearArgs)]),
     'tp_ragged_linear_forward': (ctypes.c_int, [ctypes.POINTER(RaggedLinearArgs), ctypes.c_void_p]),
     'tp_ragged_linear_backward': (ctypes.c_int, [ctypes.POINTER(RaggedLinearArgs), ctypes.c_void_p]),

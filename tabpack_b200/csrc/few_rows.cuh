@@ -1,10 +1,10 @@
 // Linear layers over groups of a few rows: the weights are the bound, each read once from memory.
 //
-// Here the weights' rows are the 128 lanes of the accumulator and 32 rows of x (64 in 4 bits, where a product's
-// scales begin at an even column of a tile's four) its columns: Y^T = W X^T.  A stage is then mostly weights, where 128-row tiles of x would be nearly empty, and the tiles are small enough that
-// every SM gets some; where there are few all the same, the K loop is split over a cluster of up to eight CTAs, which add their
-// parts up in order through distributed shared memory.  Two CTAs share an SM, so that one's start and end lie under the
-// other's copies.
+// Here the weights' rows are the 128 lanes of the accumulator and 32 rows of x (64 in 4 bits, where a product's scales begin at
+// an even column of a tile's four) its columns: Y^T = W X^T.  A stage is then mostly weights, where 128-row tiles of x would be
+// nearly empty, and the tiles are small enough that every SM gets some; where there are few all the same, the K loop is split
+// over a cluster of up to eight CTAs, which add their parts up in order through distributed shared memory.  Two CTAs share an
+// SM, so that one's start and end lie under the other's copies.
 #pragma once
 
 #include "fp4.cuh"

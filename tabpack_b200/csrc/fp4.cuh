@@ -275,6 +275,16 @@ __device__ __forceinline__ uint4 fp4_load(const T* x, int c, int n) {
   }
 }
 
+// Rows onto 16-byte boundaries, a vector a thread; `vecs` of a row of the result.
+__global__ void __launch_bounds__(256) align_rows_kernel(const __nv_bfloat16* x, long long ld, int rows, int cols, uint4* out, int vecs,
+                                                        const FastDiv div, int span) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x, r = fastdiv(i, div);
+  const long long row = (long long)blockIdx.y * span + r;
+  if (r >= (uint32_t)span || row >= rows) return;
+  const int v = (int)(i - r * (uint32_t)vecs);
+  out[row * vecs + v] = fp4_load<__nv_bfloat16, false>(x + row * ld, 8 * v, cols);
+}
+
 // The largest magnitude of a row among the vectors of this thread (of G), NaN if one is.
 template <typename T, int G, bool ALIGNED>
 __device__ __forceinline__ float fp4_row_max(const T* x, int n, int at) {

@@ -1285,14 +1285,22 @@ def combine_rows_backward(dout: Tensor, y: Tensor, weight: Tensor | None, positi
     return dy, dw
 
 
+def _align_rows(t: Tensor, stride: int, rows: int, cols: int, device: int) -> tuple[Tensor, int]:
+    """`rows` bf16 rows of t, `stride` elements apart, as rows on 16-byte boundaries; see `tp_align_rows`."""
+    wide = _round(cols, 8)
+    out = _empty2(rows, wide, t.dtype, t.device)
+    if rows:
+        with torch.cuda.device(device if device != torch._C._cuda_getDevice() else -1):
+            check(_function('tp_align_rows')(t.data_ptr(), stride, rows, cols, out.data_ptr(), wide,
+                                             torch._C._cuda_getCurrentRawStream(device)), 'tp_align_rows')
+    return out, wide
+
+
 def _vector_rows(name: str, t: Tensor, shape: tuple, device: int) -> tuple[Tensor, int]:
     """A matrix as an operand of the ragged products: bf16 rows on 16-byte boundaries (copied to such where not)."""
     t, stride = _rows2(name, t, shape, t.dtype, device)
     if t.dtype is torch.bfloat16 and (stride % 8 or t.data_ptr() % 16):
-        cols = _round(shape[1], 8)
-        wide = _empty2(shape[0], cols, t.dtype, t.device)
-        wide[:, : shape[1]] = t
-        return wide, cols
+        return _align_rows(t, stride, shape[0], shape[1], device)
     return t, stride
 
 
@@ -1304,10 +1312,10 @@ def _ragged_weight(weight: Tensor, device: int) -> tuple[Tensor, int]:
     if s[2] == 1 and s[1] >= K and s[0] == N * s[1] and (weight.dtype is torch.float32 or (
             s[1] % 8 == 0 and weight.data_ptr() % 16 == 0)):
         return weight, s[1]
-    cols = K if weight.dtype is torch.float32 else _round(K, 8)
-    wide = weight.new_empty((P, N, cols))
-    wide[..., :K] = weight
-    return wide, cols
+    if weight.dtype is torch.float32:
+        return weight.contiguous(), K
+    wide, cols = _align_rows(weight.contiguous(), K, P * N, K, device)
+    return wide.view(P, N, cols), cols
 
 
 def _ragged_operands(x, weight, offsets, in_features, out_features):

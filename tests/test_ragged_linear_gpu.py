@@ -151,6 +151,16 @@ def test_offsets_out_of_range_are_cut():
                                                         torch.tensor([3, 3, 10], device='cuda'))[3:])
 
 
+@pytest.mark.parametrize('rows,cols,stride,first', [(1, 1, 9, 8), (7, 5, 5, 0), (1000, 1003, 1003, 0), (33, 515, 600, 1), (3, 4095, 4099, 3)])
+def test_rows_are_moved_onto_boundaries(rows, cols, stride, first):
+    flat = torch.randn(first + rows * stride + 8, device='cuda').bfloat16()
+    x = flat[first: first + rows * stride].view(rows, stride)[:, :cols]
+    x[0, 0] = math.nan
+    out, wide = ops._align_rows(x, stride, rows, cols, 0)
+    assert wide % 8 == 0 and wide - cols < 8
+    assert torch.equal(out[:, :cols].view(torch.int16), x.contiguous().view(torch.int16)) and not out[:, cols:].any()
+
+
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('first', [0, 1, 4, 8])
 def test_strided_operands(first, dtype):

@@ -117,6 +117,14 @@ def test_fp4_linear_arguments(bad, want):
     assert _lib.load().tp_fp4_linear_forward(None, None) == -1
 
 
+@pytest.mark.parametrize('bad,want', [
+    (dict(x=None), -1), (dict(out=None), -1), (dict(rows=0), -1), (dict(rows=1 << 31), -1), (dict(cols=0), -1), (dict(stride=4), -1),
+    (dict(wide=4), -1), (dict(wide=12), -1), (dict(x=FAKE + 1), -2), (dict(out=FAKE + 8), -2)])
+def test_align_rows_arguments(bad, want):
+    a = {**dict(x=FAKE, stride=5, rows=3, cols=5, out=FAKE, wide=8), **bad}
+    assert _lib.load().tp_align_rows(a['x'], a['stride'], a['rows'], a['cols'], a['out'], a['wide'], None) == want
+
+
 def test_sizes_of_the_stored_form():
     lib = _lib.load()
     for K in (1, 16, 31, 32, 33, 255, 256, 257, 8192):
