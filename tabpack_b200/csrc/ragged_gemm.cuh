@@ -958,9 +958,8 @@ __global__ void __launch_bounds__(256) ragged_act_kernel(const RaggedAct a) {
               *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
                                                          pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
             } else {
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (c0 + j < a.g_ld) to[j] = (T)v[j];
+              reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
+              reinterpret_cast<float4*>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
             }
           }
         }

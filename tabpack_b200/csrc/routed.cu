@@ -555,7 +555,7 @@ int ragged_shares(const tp_ragged_linear_args* a) {
 // Columns between rows of the copy of g; 0: dy is taken as it is.
 long long ragged_g_stride(const tp_ragged_linear_args* a) {
   if (a->dx == nullptr && a->dw == nullptr) return 0;
-  if (a->relu) return a->dtype == TP_DTYPE_BF16 ? (a->max_out + 7ll) / 8 * 8 : a->max_out;
+  if (a->relu) return (a->max_out + 7ll) / 8 * 8;
   if (a->dtype == TP_DTYPE_BF16 && (a->dy_stride % 8 || !aligned16(a->dy))) return (a->max_out + 7ll) / 8 * 8;
   return 0;
 }
