@@ -1290,9 +1290,12 @@ def _align_rows(t: Tensor, stride: int, rows: int, cols: int, device: int) -> tu
     wide = _round(cols, 8)
     out = _empty2(rows, wide, t.dtype, t.device)
     if rows:
-        with torch.cuda.device(device if device != torch._C._cuda_getDevice() else -1):
-            check(_function('tp_align_rows')(t.data_ptr(), stride, rows, cols, out.data_ptr(), wide,
-                                             torch._C._cuda_getCurrentRawStream(device)), 'tp_align_rows')
+        args = t.data_ptr(), stride, rows, cols, out.data_ptr(), wide, torch._C._cuda_getCurrentRawStream(device)
+        if device == torch._C._cuda_getDevice():
+            check(_function('tp_align_rows')(*args), 'tp_align_rows')
+        else:
+            with torch.cuda.device(device):
+                check(_function('tp_align_rows')(*args), 'tp_align_rows')
     return out, wide
 
 
