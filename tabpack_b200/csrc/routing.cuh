@@ -74,10 +74,11 @@ __device__ __forceinline__ void route_load(const T* z, int E, int l, float (&v)[
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
-// exp(z - m) with c = -m log2(e): the rounding of c is one factor of all of a row's terms.
-__device__ __forceinline__ float exp_of(float z, float c) {
+// exp(z - m), m the row's largest score: the difference first, so that it is 0 for the largest whatever its size, and at most
+// -inf for the others (the type's lowest number beside ordinary ones: a term of 0).
+__device__ __forceinline__ float exp_of(float z, float m) {
   float r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(fmaf(z, LOG2E, c)));
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"((z - m) * LOG2E));
   return r;
 }
 
@@ -129,11 +130,11 @@ __device__ __forceinline__ void route_gate(const RouteArgs& a, int block, int* s
     };
     two_best();
     float top = lanes_max<G>(b1);
-    float c = top > -INFINITY ? -top * LOG2E : 0.f;
+    const float m = top > -INFINITY ? top : 0.f;
     float e[V], total = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      e[v] = exp_of(z[v], c);  // 0 for -inf
+      e[v] = exp_of(z[v], m);  // 0 for -inf
       total += e[v];
     }
     total = lanes_sum<G>(total);
@@ -183,7 +184,7 @@ __device__ __forceinline__ void route_gate(const RouteArgs& a, int block, int* s
       }
     }
     __syncwarp();
-    float w = my_expert >= 0 ? exp_of(mine, c) : 0.f;
+    float w = my_expert >= 0 ? exp_of(mine, m) : 0.f;
     const float of = a.renorm ? lanes_sum<G>(w) : total;
     if (my_expert >= 0) w = total == total ? w / of : total;
     if (live && l < k) {
@@ -386,11 +387,11 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs a) 
 #pragma unroll
     for (int o = G / 2; o; o >>= 1) best = max_nan(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
     const bool some = best != -INFINITY;
-    const float c = some ? -best * LOG2E : 0.f;
+    const float m = some ? best : 0.f;
     float total = 0.f, ph = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      p[v] = exp_of(p[v], c);
+      p[v] = exp_of(p[v], m);
       total += p[v];
       ph = fmaf(p[v], h[v], ph);
     }
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs a) 
     }
     __syncwarp();
     if (who >= 0) {
-      const float p_mine = exp_of(z_mine, c) * inv;
+      const float p_mine = exp_of(z_mine, m) * inv;
       out[who] = (T)fmaf(w, a.renorm ? g - wg : g, p_mine * (h_mine - through));
     }
   }
