@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(4 * G, 256 / G) fp4_quantize_stream_kernel(con
     const bool there = fetch(group + gridDim.x, stage ^ 1, then);
     cp_async_wait<1>();
     __syncwarp();
-    if (here) {  // (of all threads of the row or none)
+    if (here) {  // (of all threads of the block or none)
       // of the L vectors h = p L.. of all lanes: this lane's block is number lane % (32 / L) of vector p L + lane / (32 / L)
       uint4 u[H];
       float most[H / L], big = 0.f;
@@ -457,6 +457,9 @@ __global__ void __launch_bounds__(4 * G, 256 / G) fp4_quantize_stream_kernel(con
           *reinterpret_cast<uint2*>(a.out.codes + now.row * a.out.pitch + b * (N / 2)) = make_uint2(c[0], c[1]);
         }
       }
+    } else if constexpr (G > 32) {
+      // (a turn without rows too: the maxima of the turn before have been read before the turn after it writes over them)
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + sub), "n"(G) : "memory");
     }
     __syncwarp();  // (the slots are filled again by the next turn's copies)
     now = then;
