@@ -24,10 +24,12 @@
 //
 // fp32 operands come as three bf16 parts each (ragged_split_kernel), and the six products of parts whose terms exceed 2^-24
 // of the result are summed: a sixth of the bf16 rate, where the CUDA cores give a twenty-fifth.  Single CTAs hold all parts of a
-// block in a stage and sum the large product in an accumulator of its own, so that the others round at their own size;
-// tiles of 256 columns on pairs, for which there is no tensor memory left, go through the K loop once for each product, the
-// smallest first (both gradients of 12 members, 4099 rows, 100 -> 512: 32 us by six loops, 22 by one; forward of 8 members of
-// 512 rows, 512 -> 512, 29 by six loops, 17 by one; 8 x 2048 rows, 1024 -> 1024, 185 by one and 171 on pairs).
+// block in a stage; tiles of 256 columns on pairs, which leave no tensor memory for two accumulators a tile, go through the K loop
+// once for each product.  Either way the product of the first parts has an accumulator of its own, on pairs the one before the
+// others': so the others round at their own size, and are left out where it is not finite.  An infinite number is its first
+// part, the other parts are 0, so its large product is infinite or NaN as the definition has it, while the small ones would
+// add inf * 0 or an infinity of the other sign (both gradients of 12 members, 4099 rows, 100 -> 512: 32 us by six loops, 22 by one; forward of 8 members of
+// 512 rows, 512 -> 512, 29 by six loops, 17 by one; 8 x 2048 rows, 1024 -> 1024, 185 by one and 177 on pairs, of which 6 are the second accumulator).
 #pragma once
 
 #include <type_traits>
@@ -83,6 +85,7 @@ struct RaggedCfg {
   static constexpr bool ALL = F32 && !PAIR;
   static_assert(!ALL || BN_ == 128, "two accumulators of two buffers");
   static constexpr int PARTS = ALL ? 3 : 1, PASSES = F32 && !ALL ? 6 : 1, PRODUCTS = ALL ? 6 : 1;
+  static constexpr bool TWICE = F32 && !ALL;  // a tile fills two accumulators one after the other
   static constexpr int SEGMENT = F32 ? RAGGED_SEGMENT_F32 : RAGGED_SEGMENT;
   static_assert(!PAIR || BN_ == 256, "pairs take tiles of 256 columns");
   static constexpr int BM = 128, BN = BN_, BK = 64;
@@ -242,9 +245,9 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
   auto is_cut = [&](const RaggedTile& t) {
     return (t.k_len & 15) != 0 && (MODE == RAGGED_WGRAD || t.part + t.k_len != k_full);
   };
-  // fp32: which parts of A and B a pass multiplies, two bits each: lh, hl, mm, mh, hm, hh
-  auto a_of = [&](int pass) { return F32 ? (0x052 >> (2 * pass)) & 3 : 0; };
-  auto b_of = [&](int pass) { return F32 ? (0x118 >> (2 * pass)) & 3 : 0; };
+  // fp32: which parts of A and B a pass multiplies, two bits each: hh, then lh, hl, mm, mh, hm
+  auto a_of = [&](int pass) { return F32 ? (0x148 >> (2 * pass)) & 3 : 0; };
+  auto b_of = [&](int pass) { return F32 ? (0x460 >> (2 * pass)) & 3 : 0; };
   // zeros from element `left` of a stage's K on, up to the next step of 16; by a whole warp
   auto zero_tail = [&](int stage, int left) {
     const int end = (left + 15) & ~15;
@@ -380,9 +383,21 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
       if (t.kind == RT_END) break;
       if (t.kind != RT_MMA) continue;
       const uint32_t idesc = idesc_bf16_f32(ragged_n(PAIR, BN, t), Cfg::A_MN, Cfg::B_MN, Cfg::TILE_M);
-      const uint32_t d_tmem = tmem_base + (uint32_t)(acc * Cfg::ACC_COLS);
+      uint32_t d_tmem = tmem_base + (uint32_t)(acc * Cfg::ACC_COLS);
       if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, abort_flag)) break;
       tc_fence_after();
+      // an accumulator is complete once this thread's products so far are
+      auto hand_over = [&]() {
+        if (lane == 0) {
+          if constexpr (PAIR) {
+            umma_commit_both(&tfull[acc]);
+          } else {
+            umma_commit(&tfull[acc]);
+          }
+        }
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+      };
       const int kblocks = (t.k_len + Cfg::BK - 1) / Cfg::BK;
       const int last = t.k_len - (kblocks - 1) * Cfg::BK;  // elements of the last block
       const bool cut = is_cut(t);
@@ -393,12 +408,12 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
           const int a_part = Cfg::ALL ? a_of(product) : 0, b_part = Cfg::ALL ? b_of(product) : 0;
           const uint64_t adesc = adesc0 + (uint64_t)((stage * Cfg::PARTS + a_part) * (Cfg::A_BYTES / 16));
           const uint64_t bdesc = bdesc0 + (uint64_t)((stage * Cfg::PARTS + b_part) * (Cfg::B_BYTES / 16));
-          const uint32_t d = Cfg::ALL && product < 5 ? d_tmem + BN : d_tmem;
+          const uint32_t d = Cfg::ALL && product > 0 ? d_tmem + BN : d_tmem;
 #pragma unroll
           for (int s = 0; s < Cfg::BK / 16; ++s) {
             // 16 elements further along K: 32 bytes of a K-major row, 16 rows of an MN-major block (in units of 16 bytes)
             const uint64_t ad = adesc + (uint64_t)(s * (Cfg::A_MN ? 128 : 2)), bd = bdesc + (uint64_t)(s * (Cfg::B_MN ? 128 : 2));
-            const uint32_t on = (first && s == 0 && (product == 0 || product == 5)) ? 0u : 1u;
+            const uint32_t on = (first && s == 0 && product < 2) ? 0u : 1u;
             if (s < steps) {
               if constexpr (PAIR)
                 umma_f16_pair(d, ad, bd, idesc, on);
@@ -416,6 +431,14 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
       // one thread goes through the blocks; the whole warp comes together for one that needs zeros
       const int plain = cut ? kblocks - 1 : kblocks;
       for (int pass = 0; ok && pass < Cfg::PASSES; ++pass) {
+        const bool opens = pass == 0 || (Cfg::TWICE && pass == 1);  // the first products of an accumulator
+        if (Cfg::TWICE && pass == 1) {
+          hand_over();
+          d_tmem = tmem_base + (uint32_t)(acc * Cfg::ACC_COLS);
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(&tempty[acc], acc_phase ^ 1u, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+        }
         if (lane == 0) {
           int st = stage;
           uint32_t ph = phase;
@@ -426,9 +449,9 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
             }
             tc_fence_after();
             if (kb < kblocks - 1)
-              multiply(st, Cfg::BK / 16, pass == 0 && kb == 0);
+              multiply(st, Cfg::BK / 16, opens && kb == 0);
             else
-              multiply(st, (last + 15) >> 4, pass == 0 && kb == 0);
+              multiply(st, (last + 15) >> 4, opens && kb == 0);
             if (++st == STAGES) {
               st = 0;
               ph ^= 1u;
@@ -455,7 +478,7 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
           ok = __all_sync(0xFFFFFFFFu, ok);
           if (ok) {
             tc_fence_after();
-            if (lane == 0) multiply(stage, (last + 15) >> 4, pass == 0 && kblocks == 1);
+            if (lane == 0) multiply(stage, (last + 15) >> 4, opens && kblocks == 1);
             __syncwarp();
           }
           if (++stage == STAGES) {
@@ -465,15 +488,7 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
         }
       }
       if (!ok) break;
-      if (lane == 0) {
-        if constexpr (PAIR) {
-          umma_commit_both(&tfull[acc]);
-        } else {
-          umma_commit(&tfull[acc]);
-        }
-      }
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
+      hand_over();
     }
     if (lane == 0) {  // every MMA of this CTA has completed once it flips
       if constexpr (PAIR)
@@ -685,7 +700,10 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
               tmem_ld_32x32b_x8(t_row + (uint32_t)(BN + c), u);
               tmem_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 8; ++j) sum[c + j] += __uint_as_float(v[j]) + __uint_as_float(u[j]);
+              for (int j = 0; j < 8; ++j) {
+                const float large = __uint_as_float(v[j]);
+                sum[c + j] += fabsf(large) < INFINITY ? large + __uint_as_float(u[j]) : large;
+              }
             } else {
               tmem_wait_ld();
 #pragma unroll
@@ -693,6 +711,21 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
             }
           }
           release();
+          if constexpr (Cfg::TWICE) {
+            if (!mbar_wait(&tfull[acc], acc_phase, abort_flag)) break;
+            tc_fence_after();
+            const uint32_t t_small = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * Cfg::ACC_COLS + slice * WCOLS);
+#pragma unroll
+            for (int c = 0; c < WCOLS; c += 8) {
+              uint32_t v[8];
+              tmem_ld_32x32b_x8(t_small + (uint32_t)c, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (fabsf(sum[c + j]) < INFINITY) sum[c + j] += __uint_as_float(v[j]);
+            }
+            release();
+          }
           if (t.add & 2) continue;
         }
         if constexpr (MODE == RAGGED_WGRAD) {
@@ -828,8 +861,10 @@ __global__ void __launch_bounds__(256) ragged_parts_kernel(const float* parts, f
 // ---------------------------------------------------------------------------
 // fp32 operands as three bf16 parts, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m): 24 bits in
 // all, each difference exact.  A row's parts lie side by side, `cols` columns (a multiple of 64) each, zeros at the end.
-// Of a number that is not finite h is the whole.
+// Of a number that is not finite h is the whole; of one that would round to infinity h is bf16's largest, and m has the rest.
 // ---------------------------------------------------------------------------
+constexpr float BF16_MAX = 3.3895313892515355e38f;
+
 struct SplitArgs {
   const float* x[3];  // up to three matrices in a launch
   long long ld[3], rows[3];
@@ -855,16 +890,29 @@ __global__ void __launch_bounds__(256) ragged_split_kernel(const SplitArgs a) {
       for (int e = 0; e < 8; ++e) v[e] = c + e < a.width[k] ? __ldg(x + e) : 0.f;
     }
     __nv_bfloat16* out = a.out[k] + 3 * r * a.cols[k] + c;
+    bool odd = false;  // a first part is infinite or NaN: of eight numbers hardly ever one
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
       uint32_t w[4];
+      float h[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const __nv_bfloat16 h = __float2bfloat16_rn(v[e]);
-        const float f = __bfloat162float(h);
-        w[e >> 1] = (e & 1) ? w[e >> 1] | (uint32_t)__bfloat16_as_ushort(h) << 16 : (uint32_t)__bfloat16_as_ushort(h);
-        v[e] = fabsf(f) < INFINITY ? v[e] - f : 0.f;
+        h[e] = __bfloat162float(__float2bfloat16_rn(v[e]));
+        if (p == 0) odd |= !(fabsf(h[e]) < INFINITY);
       }
+      if (p == 0 && odd) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool finite = fabsf(v[e]) < INFINITY;
+          if (finite) h[e] = fminf(fmaxf(h[e], -BF16_MAX), BF16_MAX);
+          v[e] = finite ? v[e] - h[e] : 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] -= h[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(h[2 * e], h[2 * e + 1]);
       *reinterpret_cast<uint4*>(out + p * a.cols[k]) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
