@@ -1295,7 +1295,9 @@ class Fp4LinearPack(ModulePack):
             x = x[0]  # rows that the members share are quantised once
         y = self._call(x, pack_idx, None, relu)
         if n_blocks is not None:  # members without this block pass their input through
-            y = torch.where((n_blocks > block_index).view(-1, 1, 1), y, x.to(y.dtype)[..., : y.shape[-1]])
+            # (a layer that is not in 4 bits before this one is as wide as the selected members)
+            x = x[..., : y.shape[-1]] if x.shape[-1] >= y.shape[-1] else nn.functional.pad(x, (0, y.shape[-1] - x.shape[-1]))
+            y = torch.where((n_blocks > block_index).view(-1, 1, 1), y, x.to(y.dtype))
         return y
 
     def forward(self, x: Tensor, pack_idx: Tensor | None = None) -> Tensor:
