@@ -261,9 +261,9 @@ __global__ void __launch_bounds__(128, 2)
   auto store = [&](int j, float x) {
     if constexpr (Cfg::FP4)
       if (real) x *= __ldg(pr.x_row + (pr.x_shared ? local : row0) + j);
-    x = fmaf(x, ws, bias);
+    x = all_blocks > 0 ? fmaf(x, ws, bias) : bias;  // (without input features: the bias alone)
     if (pr.relu) x = max_nan(x, 0.f);
-    if (o >= n_valid || all_blocks == 0) x = 0.f;
+    if (o >= n_valid) x = 0.f;
     if (o < pr.N) {
       const long long at = (long long)(row0 + j) * pr.N + o;
       if (pr.y_f32)

@@ -1001,8 +1001,9 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
       const int rows = t.rows - rank * Cfg::BM - q * 32;
       const long long row0 = (long long)t.y_row + rank * Cfg::BM + q * 32;
       const bool mma = t.kind == FT_MMA;
+      const bool biased = mma || t.nt * BN < t.n_valid;  // (without input features: the bias alone)
       float rs = 0.f;
-      if (mma) {
+      if (biased) {
         __syncwarp();
         for (int j = lane; j < WCOLS; j += 32) {
           const bool in = cbase + j < t.n_valid;
@@ -1011,6 +1012,8 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
         }
         if (lane < rows) rs = __ldg(pr.x_row + (long long)t.x_row + rank * Cfg::BM + q * 32 + lane);
         __syncwarp();
+      }
+      if (mma) {
         if (!mbar_wait(&tfull[acc], acc_phase, abort_flag)) break;
         tc_fence_after();
       }
@@ -1107,8 +1110,8 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
                 for (int e = 0; e < 8; ++e) {
                   const int o = 32 * c + j + e;
                   x[e] = 0.f;
-                  if (mma) {
-                    x[e] = fmaf(__uint_as_float(v[j + e]) * rs, sscale[o], sbias[o]);
+                  if (biased) {
+                    x[e] = mma ? fmaf(__uint_as_float(v[j + e]) * rs, sscale[o], sbias[o]) : sbias[o];
                     if (pr.relu) x[e] = max_nan(x[e], 0.f);
                     if (j + e >= nv) x[e] = 0.f;
                   }

@@ -673,7 +673,7 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
       if (t.kind == RT_END) break;
       const int cbase = t.nt * BN + slice * WCOLS;
       const bool mma = t.kind == RT_MMA;
-      const bool biased = MODE == RAGGED_FWD && mma;
+      const bool biased = MODE == RAGGED_FWD && (mma || t.nt * BN < t.n_valid);  // (without input features: the bias alone)
       if (biased && !(t.add & 1)) {
         __syncwarp();
         for (int j = lane; j < WCOLS; j += 32)
@@ -776,12 +776,14 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
         const int nch = min(NCH, max(0, (ld - cbase + 31) / 32));
         const int rows = t.rows - rank * Cfg::BM - q * 32;  // of this warp, may be below 1 or above 32
         const long long row0 = (long long)t.row0 + rank * Cfg::BM + q * 32;
-        if (rows > 0 && mma) {
+        if (rows > 0 && (mma || biased)) {
 #pragma unroll 1
           for (int c = 0; c < nch; ++c) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(t_row + (uint32_t)(32 * c), v);
-            tmem_wait_ld();
+            uint32_t v[32] = {};
+            if (mma) {
+              tmem_ld_32x32b_x32(t_row + (uint32_t)(32 * c), v);
+              tmem_wait_ld();
+            }
             const int nv = t.n_valid - (cbase + 32 * c);
 #pragma unroll
             for (int j = 0; j < 32; j += 8) {
