@@ -686,7 +686,7 @@ int tp_route_backward(const tp_route_args* a, void* stream);
  *                     <dout[t], x[position[t, j]]>; either may be NULL.
  * Places outside 0 .. rows k - 1 are passed over. */
 typedef struct tp_rows_args {
-  int64_t rows;             /* rows * k < 2^31 */
+  int64_t rows;             /* rows * k <= 2^31 - 2^20, as in tp_route_args */
   int32_t k, W, E;
   int32_t dtype;            /* TP_DTYPE_F32 or TP_DTYPE_BF16: x, out, dout, dy */
   const int32_t* position;

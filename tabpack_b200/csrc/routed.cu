@@ -51,7 +51,7 @@ RoutePlan route_plan(int64_t rows, int32_t k) {
   return p;
 }
 
-constexpr long long ROUTE_MAX_PAIRS = (1ll << 31) - (1ll << 20);  // (the kernels look some rows ahead)
+constexpr long long ROUTE_MAX_PAIRS = (1ll << 31) - (1ll << 20);  // (the kernels look some rows ahead, in 32 bits)
 
 int check_route(const tp_route_args* a) {
   if (!a) return fail(TP_EINVAL, "null routing arguments");
@@ -147,9 +147,9 @@ int dispatch_route(const RouteArgs& k, bool backward, cudaStream_t st) {
 
 int check_rows(const tp_rows_args* a) {
   if (!a) return fail(TP_EINVAL, "null row move arguments");
-  if (a->rows <= 0 || a->k <= 0 || a->k > ROUTE_MAX_K || a->W <= 0 || a->E <= 0 || a->rows >= (1ll << 31) ||
-      a->rows * a->k >= (1ll << 31))
-    return fail(TP_EINVAL, "row moves need rows, W, E > 0, 1 <= k <= %d, rows k < 2^31 (got %lld, %d, %d, %d)", ROUTE_MAX_K,
+  if (a->rows <= 0 || a->k <= 0 || a->k > ROUTE_MAX_K || a->W <= 0 || a->E <= 0 || a->rows > ROUTE_MAX_PAIRS ||
+      a->rows * a->k > ROUTE_MAX_PAIRS)
+    return fail(TP_EINVAL, "row moves need rows, W, E > 0, 1 <= k <= %d, rows k <= 2^31 - 2^20 (got %lld, %d, %d, %d)", ROUTE_MAX_K,
                 (long long)a->rows, a->W, a->E, a->k);
   if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad row dtype");
   if (!a->position || !a->offsets) return fail(TP_EINVAL, "null plan");
