@@ -718,7 +718,7 @@ typedef struct tp_ragged_linear_args {
   int32_t P;
   int32_t max_in, max_out;
   int32_t dtype;            /* TP_DTYPE_F32 or TP_DTYPE_BF16: x, w, y, dy, dx */
-  int64_t rows;             /* < 2^31 */
+  int64_t rows;             /* <= 2^31 - 2^20 */
   const int32_t* offsets;
   const int32_t* in_features;  /* (P), or NULL (= max_in) */
   const int32_t* out_features; /* (P), or NULL (= max_out) */
@@ -758,7 +758,7 @@ typedef struct tp_fp4_args {
   int32_t K;
   int32_t format;           /* TP_FP4_* */
   int32_t dtype;            /* TP_DTYPE_F32 or TP_DTYPE_BF16: x */
-  int64_t rows;             /* < 2^31 */
+  int64_t rows;             /* < 2^31 - 256 */
   const int32_t* offsets;   /* (P + 1), or NULL */
   const int32_t* n_features; /* (P): columns of a group's rows that count, or NULL (= K) */
   const void* x;            /* (rows, K), quantise */

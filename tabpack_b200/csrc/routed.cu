@@ -296,8 +296,8 @@ int tile_columns(long long row_tiles, int cols) {
 int check_ragged(const tp_ragged_linear_args* a) {
   if (!a) return fail(TP_EINVAL, "null ragged linear arguments");
   if (a->P <= 0 || a->P > 65535 || a->max_in <= 0 || a->max_out <= 0 || a->max_in > MAX_WIDTH || a->max_out > MAX_WIDTH ||
-      a->rows <= 0 || a->rows >= (1ll << 31) - 256)
-    return fail(TP_EINVAL, "a ragged linear layer needs 1 <= P <= 65535, widths > 0, 0 < rows < 2^31 - 256 (got %d, %d, %d, %lld)",
+      a->rows <= 0 || a->rows > ROUTE_MAX_PAIRS)
+    return fail(TP_EINVAL, "a ragged linear layer needs 1 <= P <= 65535, widths > 0, 0 < rows <= 2^31 - 2^20 (got %d, %d, %d, %lld)",
                 a->P, a->max_in, a->max_out, (long long)a->rows);
   if (a->dtype != TP_DTYPE_F32 && a->dtype != TP_DTYPE_BF16) return fail(TP_EINVAL, "bad ragged linear dtype");
   if (!a->offsets || !a->x || !a->w) return fail(TP_EINVAL, "null offsets, x or w");
