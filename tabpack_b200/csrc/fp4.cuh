@@ -94,7 +94,6 @@ struct Fp4QuantArgs {
   long long ld;
   const int32_t* n_features;  // (P) or null: columns of a group's rows that count
   Fp4Rows out;
-  int tiles;
 };
 
 // Eight values as four bytes of codes, the first in the lowest half byte.

@@ -1431,7 +1431,8 @@ def fp4_quantize(x: Tensor, format: str = 'nvfp4', *, offsets: Tensor | None = N
     """x (R, K) or (P, R, K), bf16 or fp32, in 4-bit floating point with a scale per block of columns;
     see `tp_fp4_quantize`.  `n_features` (P,): only the first columns of a member's rows count (the others
     are zero).  `offsets` (P + 1,): x is (R, K), member m's rows are x[offsets[m] : offsets[m + 1]] (those
-    of no member stay unwritten), and the scales are laid out for `fp4_linear_forward` over these groups."""
+    of no member stay unwritten), and the scales lie as `tp_fp4_linear_forward` takes rows in 4 bits over these groups
+    (`fp4_linear_forward` quantises its rows itself, `fp4_values` takes rows without offsets)."""
     code = _fp4_format(format)
     if x.ndim not in (2, 3) or (offsets is not None and x.ndim != 2):
         raise ValueError('x must be (rows, columns) or (pack_size, rows, columns)')
