@@ -1007,9 +1007,9 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
         for (int j = lane; j < WCOLS; j += 32) {
           const bool in = cbase + j < t.n_valid;
           sbias[j] = (in && pr.bias) ? __ldg(pr.bias + (long long)t.member * pr.N + cbase + j) : 0.f;
-          sscale[j] = in ? __ldg(pr.w_row + (long long)t.member * pr.N + cbase + j) : 0.f;
+          sscale[j] = in && mma ? __ldg(pr.w_row + (long long)t.member * pr.N + cbase + j) : 0.f;
         }
-        if (lane < rows) rs = __ldg(pr.x_row + (long long)t.x_row + rank * Cfg::BM + q * 32 + lane);
+        if (mma && lane < rows) rs = __ldg(pr.x_row + (long long)t.x_row + rank * Cfg::BM + q * 32 + lane);
         __syncwarp();
       }
       if (mma) {
@@ -1096,6 +1096,9 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
           if (mma) {
             tmem_ld_32x32b_x32(t_row + (uint32_t)(32 * c), v);
             tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0u;
           }
           const int nv = t.n_valid - (cbase + 32 * c), col0 = cbase + 32 * c;
 #pragma unroll 1
@@ -1110,7 +1113,7 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
                   const int o = 32 * c + j + e;
                   x[e] = 0.f;
                   if (biased) {
-                    x[e] = mma ? fmaf(__uint_as_float(v[j + e]) * rs, sscale[o], sbias[o]) : sbias[o];
+                    x[e] = fmaf(__uint_as_float(v[j + e]) * rs, sscale[o], sbias[o]);
                     if (pr.relu) x[e] = max_nan(x[e], 0.f);
                     if (j + e >= nv) x[e] = 0.f;
                   }

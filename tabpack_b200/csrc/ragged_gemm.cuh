@@ -776,14 +776,12 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
         const int nch = min(NCH, max(0, (ld - cbase + 31) / 32));
         const int rows = t.rows - rank * Cfg::BM - q * 32;  // of this warp, may be below 1 or above 32
         const long long row0 = (long long)t.row0 + rank * Cfg::BM + q * 32;
-        if (rows > 0 && (mma || biased)) {
+        if (rows > 0 && mma) {
 #pragma unroll 1
           for (int c = 0; c < nch; ++c) {
-            uint32_t v[32] = {};
-            if (mma) {
-              tmem_ld_32x32b_x32(t_row + (uint32_t)(32 * c), v);
-              tmem_wait_ld();
-            }
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(t_row + (uint32_t)(32 * c), v);
+            tmem_wait_ld();
             const int nv = t.n_valid - (cbase + 32 * c);
 #pragma unroll
             for (int j = 0; j < 32; j += 8) {
@@ -805,12 +803,24 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
             __syncwarp();
           }
         } else if (rows > 0) {
-          __syncwarp();
+#pragma unroll 1
+          for (int c = 0; c < nch; ++c) {
+            if (c == 0 || biased) {
+              __syncwarp();
+#pragma unroll 1
+              for (int j = 0; j < 32; j += 2) {
+                float x[2] = {0.f, 0.f};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage_row + 16 * j) = make_uint4(0, 0, 0, 0);
-          __syncwarp();
-          for (int c = 0; c < nch; ++c)
+                for (int e = 0; e < 2; ++e) {
+                  if (biased && cbase + 32 * c + j + e < t.n_valid) x[e] = sbias[32 * c + j + e];
+                  if (pr.relu) x[e] = max_nan(x[e], 0.f);
+                }
+                *reinterpret_cast<uint32_t*>(stage_row + j * 2) = pack_bf16x2(x[0], x[1]);
+              }
+              __syncwarp();
+            }
             ragged_flush(out, ld, pr.c_vec, row0, rows, cbase + 32 * c, stage_warp, Cfg::ROW_BYTES, lane);
+          }
         }
         if (mma) release();
       }
