@@ -710,8 +710,9 @@ int tp_align_rows(const void* x, int64_t x_stride, int64_t rows, int32_t cols, v
 
 /* Linear layer of a pack over ragged groups of rows: member m's rows are offsets[m] .. offsets[m + 1] - 1 of x,
  *   y = relu(x w_m^T + b_m),  g = dy [y > 0],  dx = g w_m,  dw_m = g^T x,  db_m = sum g.
- * offsets (device, P + 1) do not decrease and stay within 0 .. rows (what does not is cut).  Rows of no member are zero
- * in y and dx and take no part in dw and db.  A member takes its first in_features columns and out_features outputs;
+ * offsets (device, P + 1) do not decrease (members of negative length have no rows, but what rows that two members share
+ * come out as is not defined); what leaves 0 .. rows is cut.  Rows of no member are zero in y and dx and take no part in
+ * dw and db.  A member takes its first in_features columns and out_features outputs;
  * what lies beyond takes no part, whatever it holds, and is zero in every result.  BF16: x_stride, w_stride and
  * dy_stride (without relu) are multiples of 8 and their pointers on 16-byte boundaries. */
 typedef struct tp_ragged_linear_args {
@@ -749,7 +750,8 @@ int tp_ragged_linear_backward(const tp_ragged_linear_args* a, void* stream);
  * column K.  scales: tiles of 128 rows by 4 blocks, byte 16 (row % 32) + 4 (row / 32) + block % 4 of a tile's 512;
  * tp_fp4_scale_tiles(K, format) tiles a row of tiles (K rounded up to 256 columns), zero bytes where there is no block.
  * P groups of rows begin in a tile of their own: equal groups of `rows / P` rows (offsets NULL) group g in row of tiles
- * g ceil(rows / P / 128); ragged ones (offsets as in tp_ragged_linear_args) in floor(offsets[g] / 128) + g, which takes
+ * g ceil(rows / P / 128); ragged ones (offsets as in tp_ragged_linear_args, but none that decrease: what the rows then
+ * come out as is not defined) in floor(offsets[g] / 128) + g, which takes
  * rows / 128 + P rows of tiles in all.  row_scale: 2^r, or 1 (TP_FP4_MX), or NaN. */
 #define TP_FP4_NV 0
 #define TP_FP4_MX 1

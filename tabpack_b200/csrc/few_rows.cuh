@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(128, 2)
     row0 = member * g.B + local;
     rows = min(BN, g.B - local);
   } else {
-    int before = 0;
+    int before = 0, lowest = (int)g.rows;
     for (int g0 = 0; g0 < n_groups; g0 += 32) {
       const int i = g0 + lane;
       int first = 0, end = 0;
@@ -116,6 +116,9 @@ __global__ void __launch_bounds__(128, 2)
         first = (int)fp4_first_row(g, g.P);
         end = (int)g.rows;
       }
+      // (the rows before the first member's end where any member's begin, should the offsets decrease)
+      lowest = min(lowest, __reduce_min_sync(0xFFFFFFFFu, i < g.P ? first : (int)g.rows));
+      if (i == g.P) end = min(end, lowest);
       const int n = (end - first + BN - 1) / BN;
       int inc = n;
 #pragma unroll

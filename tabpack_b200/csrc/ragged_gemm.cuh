@@ -583,10 +583,13 @@ __device__ __forceinline__ void ragged_gemm(const CUtensorMap& tmA, const CUtens
     } else {
       int g0 = 0;          // first group of the 32 that the lanes hold
       long long before = 0;  // tiles of the groups before them
-      int first = 0, end = 0, tiles = 0, inc = 0;
+      int first = 0, end = 0, tiles = 0, inc = 0, lowest = pr.R;
       auto load_groups = [&]() {
         first = end = 0;
         if (g0 + lane < pr.P + 2) ragged_group(pr, g0 + lane, first, end);
+        // (the rows before the first member's end where any member's begin, should the offsets decrease)
+        lowest = min(lowest, __reduce_min_sync(0xFFFFFFFFu, g0 + lane < pr.P ? first : pr.R));
+        if (g0 + lane == pr.P) end = min(end, lowest);
         tiles = (end - first + Cfg::TILE_M - 1) / Cfg::TILE_M * pr.n_tiles;
         inc = tiles;
 #pragma unroll
