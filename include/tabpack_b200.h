@@ -649,8 +649,8 @@ const char* tp_version(void);
  * top_k (<= 32, <= E) best finite z in descending order (ties: lowest member; NaN first) as `expert` (-1 where a row
  * has fewer), their `weight` p / (sum of the chosen p) with renormalize, else p (0 for -1).  The (row, slot) pairs are
  * sorted by member, stably: `position` is a pair's place, `offsets` (E + 1) where the members' rows begin; pairs
- * without a member come behind offsets[E].  importance[e] = sum over rows of p_e.  Scores of -inf take no part; a row
- * of nothing else has no members; a NaN or +inf makes its row's weights (and the importance) NaN.
+ * without a member come behind offsets[E].  importance[e] = sum over rows of p_e.  Finite scores may have any size
+ * (the type's lowest number is one of them).  Scores of -inf take no part; a row of nothing else has no members; a NaN or +inf makes its row's weights (and the importance) NaN.
  * The backward forms dlogits (rows, E), contiguous, from the gradients of weight and importance (either may be NULL):
  *   dz_e = [e chosen] w_e (g_e - s) + p_e (h_e - sum_c p_c h_c)          s = sum_chosen w g, with renormalize,
  *   dz_e = [e chosen] w_e g_e + p_e (h_e - sum_c p_c h_c - s)            without. */
