@@ -262,9 +262,12 @@ __global__ void __launch_bounds__(128, 2)
     }
   };
   auto store = [&](int j, float x) {
-    if constexpr (Cfg::FP4)
-      if (real) x *= __ldg(pr.x_row + (pr.x_shared ? local : row0) + j);
-    x = all_blocks > 0 ? fmaf(x, ws, bias) : bias;  // (without input features: the bias alone)
+    if (all_blocks == 0)
+      x = bias;  // (without input features)
+    else if constexpr (Cfg::FP4)
+      x = fp4_result(x, __ldg(pr.x_row + (pr.x_shared ? local : row0) + j), ws, bias);
+    else
+      x += bias;
     if (pr.relu) x = max_nan(x, 0.f);
     if (o >= n_valid) x = 0.f;
     if (o < pr.N) {

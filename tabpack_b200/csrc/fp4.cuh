@@ -562,6 +562,17 @@ struct Fp4Problem {
   int n_tiles;
 };
 
+// sum * x's row scale * w's row scale + bias, the scales being powers of two of at most 2^117.  A sum (below 2^47: 2^24 products of
+// at most 2688^2) times 2^80 is within fp32; what a larger scale has beyond goes to the other one, so that nothing in between
+// overflows where the result does not.  (Cut at 2^127: then the result is infinite all the same, and a sum of 0 is no NaN.)
+constexpr float FP4_SCALE_STEP = 1208925819614629174706176.f;
+__device__ __forceinline__ float fp4_result(float sum, float x_scale, float w_scale, float bias) {
+  const bool large = x_scale > FP4_SCALE_STEP;
+  const float first = large ? FP4_SCALE_STEP : x_scale, rest = large ? x_scale * (1.f / FP4_SCALE_STEP) : 1.f;
+  const float second = rest * w_scale, most = 1.70141183e38f;
+  return fmaf(sum * first, second > most ? most : second, bias);  // (a NaN stays one)
+}
+
 enum : int { FT_MMA = 0, FT_ZERO = 1, FT_END = 2 };
 struct Fp4Tile {
   int kind, member, x_row, y_row, rows, nt, x_tile, n_valid;
@@ -1031,7 +1042,7 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
           acc_phase ^= 1u;
         }
       };
-      if (mma && !pr.y_f32 && pr.y_vec) {
+      if (mma && !pr.y_f32 && pr.y_vec && !__any_sync(0xFFFFFFFFu, rs > FP4_SCALE_STEP)) {
         // bf16: the whole slice goes to registers, rounded, before the accumulator is given back (there is one)
         uint32_t y[WCOLS / 2], v[2][16];
         tmem_ld_32x32b_x16(t_row, v[0]);
@@ -1113,7 +1124,7 @@ __global__ void __launch_bounds__(Fp4Cfg<BN, FORMAT, PAIR>::THREADS, 1)
                   const int o = 32 * c + j + e;
                   x[e] = 0.f;
                   if (biased) {
-                    x[e] = fmaf(__uint_as_float(v[j + e]) * rs, sscale[o], sbias[o]);
+                    x[e] = fp4_result(__uint_as_float(v[j + e]), rs, sscale[o], sbias[o]);
                     if (pr.relu) x[e] = max_nan(x[e], 0.f);
                     if (j + e >= nv) x[e] = 0.f;
                   }
