@@ -713,7 +713,8 @@ int tp_align_rows(const void* x, int64_t x_stride, int64_t rows, int32_t cols, v
  * offsets (device, P + 1) do not decrease (members of negative length have no rows, but what rows that two members share
  * come out as is not defined); what leaves 0 .. rows is cut.  Rows of no member are zero in y and dx and take no part in
  * dw and db.  A member takes its first in_features columns and out_features outputs;
- * what lies beyond takes no part, whatever it holds, and is zero in every result.  BF16: x_stride, w_stride and
+ * what lies beyond takes no part, whatever it holds, and is zero in every result.  F32: numbers are taken as three bf16 parts,
+ * 24 bits in all; those below 2^-102 in magnitude (2e-31) keep fewer.  BF16: x_stride, w_stride and
  * dy_stride (without relu) are multiples of 8 and their pointers on 16-byte boundaries. */
 typedef struct tp_ragged_linear_args {
   int32_t P;

@@ -875,7 +875,7 @@ __global__ void __launch_bounds__(256) ragged_parts_kernel(const float* parts, f
 
 // ---------------------------------------------------------------------------
 // fp32 operands as three bf16 parts, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m): 24 bits in
-// all, each difference exact.  A row's parts lie side by side, `cols` columns (a multiple of 64) each, zeros at the end.
+// all, each difference exact (of numbers below 2^-102 l falls below bf16's smallest normal number).  A row's parts lie side by side, `cols` columns (a multiple of 64) each, zeros at the end.
 // Of a number that is not finite h is the whole; of one that would round to infinity h is bf16's largest, and m has the rest.
 // ---------------------------------------------------------------------------
 constexpr float BF16_MAX = 3.3895313892515355e38f;
