@@ -28,8 +28,9 @@
 // once for each product.  Either way the product of the first parts has an accumulator of its own, on pairs the one before the
 // others': so the others round at their own size, and are left out where it is not finite.  An infinite number is its first
 // part, the other parts are 0, so its large product is infinite or NaN as the definition has it, while the small ones would
-// add inf * 0 or an infinity of the other sign (both gradients of 12 members, 4099 rows, 100 -> 512: 32 us by six loops, 22 by one; forward of 8 members of
-// 512 rows, 512 -> 512, 29 by six loops, 17 by one; 8 x 2048 rows, 1024 -> 1024, 185 by one and 177 on pairs, of which 6 are the second accumulator).
+// add inf * 0 or an infinity of the other sign.  (Both gradients of 12 members, 4099 rows, 100 -> 512: 32 us by six loops, 22 by
+// one; forward of 8 members of 512 rows, 512 -> 512, 29 by six loops, 17 by one; 8 x 2048 rows, 1024 -> 1024, 185 by one and 177
+// on pairs, of which 6 are the second accumulator.)
 #pragma once
 
 #include <type_traits>
@@ -875,7 +876,8 @@ __global__ void __launch_bounds__(256) ragged_parts_kernel(const float* parts, f
 
 // ---------------------------------------------------------------------------
 // fp32 operands as three bf16 parts, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m): 24 bits in
-// all, each difference exact (of numbers below 2^-102 l falls below bf16's smallest normal number).  A row's parts lie side by side, `cols` columns (a multiple of 64) each, zeros at the end.
+// all, each difference exact (of numbers below 2^-102 l falls below bf16's smallest normal number).  A row's parts lie side by
+// side, `cols` columns (a multiple of 64) each, zeros at the end.
 // Of a number that is not finite h is the whole; of one that would round to infinity h is bf16's largest, and m has the rest.
 // ---------------------------------------------------------------------------
 constexpr float BF16_MAX = 3.3895313892515355e38f;
